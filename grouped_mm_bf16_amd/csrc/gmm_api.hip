@@ -7,6 +7,7 @@
 #include <cstring>
 #include <vector>
 
+#include "gmm_elem.h"
 #include "gmm_launch.h"
 
 namespace {
@@ -237,6 +238,8 @@ int run(Problem& pr, hipStream_t stream) {
 bool dims_ok(int64_t a, int64_t b, int64_t c) { return fits_i32(a) && fits_i32(b) && fits_i32(c); }
 
 }  // namespace
+
+int gmm_num_cus() { return device_cus(); }
 
 extern "C" {
 

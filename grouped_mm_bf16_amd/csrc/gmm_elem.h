@@ -1,0 +1,40 @@
+// Elements of the operators around the grouped product: 16-bit and fp32 values as they lie in memory, read and rounded 8 (16-bit)
+// or 4 (fp32) to a 16-byte access, or one by one where nothing is aligned.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace gmm {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+struct Bf16 { uint16_t bits; };
+struct F16 { uint16_t bits; };
+
+__device__ __forceinline__ float widen(Bf16 x) { return __uint_as_float(uint32_t(x.bits) << 16); }
+__device__ __forceinline__ float widen(F16 x) { return float(__builtin_bit_cast(_Float16, x.bits)); }
+__device__ __forceinline__ float widen(float x) { return x; }
+
+// Round to nearest even (v_cvt_pk_bf16_f32, v_cvt_f16_f32).
+template <typename T> __device__ __forceinline__ T rounded(float f);
+template <> __device__ __forceinline__ Bf16 rounded<Bf16>(float f) { return Bf16{__builtin_bit_cast(uint16_t, static_cast<__bf16>(f))}; }
+template <> __device__ __forceinline__ F16 rounded<F16>(float f) { return F16{__builtin_bit_cast(uint16_t, static_cast<_Float16>(f))}; }
+template <> __device__ __forceinline__ float rounded<float>(float f) { return f; }
+
+// N adjacent elements as they lie in memory: N = 1, or a 16-byte aligned vector.
+template <typename T, int N> struct alignas(N > 1 ? 16 : sizeof(T)) Pack {
+  T v[N];
+  __device__ __forceinline__ float get(int i) const { return widen(v[i]); }
+  __device__ __forceinline__ void set(int i, float f) { v[i] = rounded<T>(f); }
+};
+
+template <typename T> constexpr int kVector = 16 / int(sizeof(T));
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace gmm
+
+// Compute units of the current device (a multiple of 8), 0 if there is none (gmm_api.hip).
+int gmm_num_cus();

@@ -112,6 +112,14 @@ def call_with_workspace(launcher, args: tuple, device: torch.device, stream: int
     return launcher(*args, own.data_ptr(), own.numel(), stream)
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _guard(t: torch.Tensor):
+    """Makes the device of `t` the current one, at no cost where it is."""
+    return torch.cuda.device(t.device) if t.device.index != current_device() else _HERE
+
+
 def _launch_now(variant: int, a: torch.Tensor, b: torch.Tensor, offs: Optional[torch.Tensor],
                 out: torch.Tensor) -> None:
     lib = _lib.load()

@@ -237,6 +237,25 @@ int gmm_moe_combine(const void* y, const int32_t* token_rows, const float* slot_
                     int64_t tokens, int64_t top_k, int64_t hidden, int64_t y_rows,
                     int64_t y_stride, int64_t out_stride, int32_t dtype, void* stream);
 
+/* ---- Layer norm over the last dimension.  No counterpart in the reference.
+ *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps), var the mean square of x - mean,
+ * x [rows, width], y [rows, width], row strides in elements (at least width where there is more than one row), width <= 16384.
+ * dtype: of x and y; weight_dtype: of weight and bias (either may be NULL: ones, zeros), dtype or GMM_DT_F32.  mean, rstd
+ * float[rows]: what the backward pass needs, both or neither NULL.  Everything is summed in fp32 and rounded once. */
+int gmm_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                   int64_t rows, int64_t width, int64_t x_stride, int64_t y_stride, float eps,
+                   int32_t dtype, int32_t weight_dtype, void* stream);
+
+/* Its gradients, for dy [rows, width] and the mean and rstd of the forward pass:
+ *   dx [rows, width] (dtype), dweight and dbias [width] (weight_dtype); any of the three may be NULL.
+ * `workspace`: device memory of at least gmm_layer_norm_workspace_bytes(rows, width) bytes (-1: sizes out of range) where
+ * dweight or dbias is wanted; it need not be initialised.  No atomics: the sums are the same every time. */
+int64_t gmm_layer_norm_workspace_bytes(int64_t rows, int64_t width);
+int gmm_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                            void* dx, void* dweight, void* dbias, int64_t rows, int64_t width,
+                            int64_t dy_stride, int64_t x_stride, int64_t dx_stride,
+                            int32_t dtype, int32_t weight_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Test and tuning hooks (the reference exposes its tile knobs through environment
  * variables read in the launcher, kernels.py:590-634; tests force tiles through
  * them, tests/test_grouped_mm.py:388-394).  gmm_set_path forces a kernel family
