@@ -43,6 +43,8 @@ SIGNATURES = {
     "gmm_moe_route_noalloc": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _i64, _i32] + [_vp] * 5 + [_vp]),
     "gmm_moe_activation": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp]),
     "gmm_moe_combine": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp]),
+    "gmm_moe_few_workspace_bytes": (_i64, [_i64] * 5),
+    "gmm_moe_few": (ctypes.c_int, [_vp] * 5 + [_i64] * 14 + [_i32] * 4 + [_vp, _i64, _vp]),
     "gmm_layer_norm": (ctypes.c_int, [_vp] * 6 + [_i64] * 4 + [ctypes.c_float, _i32, _i32, _vp]),
     "gmm_layer_norm_workspace_bytes": (_i64, [_i64, _i64]),
     "gmm_layer_norm_backward": (ctypes.c_int, [_vp] * 8 + [_i64] * 5 + [_i32, _i32, _vp, _i64, _vp]),

@@ -14,13 +14,12 @@ dispatches to it while a model around it is being traced or compiled.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple
 
 import torch
 
 from . import _lib, kernels
-from .kernels import _dtype_code, _require_gpu, grouped_mm_2d3d
+from .kernels import _dtype_code, _guard, _require_gpu, grouped_mm_2d3d
 
 ACTIVATIONS = {"silu": 0, "swiglu": 1}
 
@@ -32,13 +31,6 @@ class Routing(NamedTuple):
     slot_weight: torch.Tensor   # float32 [S] combine weight of each slot
     row_token: torch.Tensor     # int32 [S]  token whose activations row r of the sorted matrix holds
     token_rows: torch.Tensor    # int32 [S]  row of each slot (inverse permutation)
-
-
-_HERE = contextlib.nullcontext()
-
-
-def _guard(t: torch.Tensor):
-    return torch.cuda.device(t.device) if t.device.index != kernels.current_device() else _HERE
 
 
 def _route_now(router_logits: torch.Tensor, top_k: int, renormalize: bool) -> torch.Tensor:
@@ -392,3 +384,75 @@ def moe_forward(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor
     del act
     return moe_combine(y, routing, T, top_k)
 
+
+# ------------------------------------------------------------------ the whole layer for a few tokens
+FEW_TOKENS = 64   # four products of 16 rows with everything that is read of a matrix
+
+
+def _few_now(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, top_k: int, kind: int,
+             renormalize: bool) -> torch.Tensor:
+    T, H = x.shape
+    E, inner = w_down.shape[:2]
+    out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+    lib = _lib.load()
+    with _guard(x):
+        nbytes = lib.gmm_moe_few_workspace_bytes(T, E, top_k, H, inner)
+        if nbytes < 0:
+            raise RuntimeError("moe_forward_few: sizes out of range")
+        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        rc = lib.gmm_moe_few(x.data_ptr(), router_logits.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), out.data_ptr(), T, E, top_k,
+                             H, inner, x.stride(0), router_logits.stride(0), *w_up.stride(), *w_down.stride(), H, kind, renormalize,
+                             _dtype_code(x.dtype), _dtype_code(router_logits.dtype), ws.data_ptr(), nbytes,
+                             kernels.current_stream(x.device))
+    _lib.check(rc, "moe_forward_few")
+    return out
+
+
+_few_op = torch.library.custom_op("grouped_mm_bf16_amd::few", mutates_args=())(_few_now)
+
+
+@_few_op.register_fake
+def _few_fake(x, router_logits, w_up, w_down, top_k, kind, renormalize):
+    return x.new_empty(x.shape)
+
+
+def moe_forward_few(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, top_k: int,
+                    activation: str = "swiglu", renormalize: bool = True, interleaved: bool = False) -> torch.Tensor:
+    """:func:`moe_forward` for up to ``FEW_TOKENS`` tokens, a decoding step: the chosen experts' matrices are streamed past the
+    tokens' rows in kernels made for that, without tiles for rows that are not there.
+
+    Arguments as there; bf16 or fp16, any sizes and weight strides.  Activations and the experts' results stay in 32 bits: the result is
+    rounded once (``moe_forward`` rounds three times, so the two differ by roundings).
+    """
+    if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
+        raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")
+    if w_up.dim() != 3 or w_down.dim() != 3 or w_up.size(0) != router_logits.size(1) or w_down.size(0) != w_up.size(0):
+        raise RuntimeError("w_up [E, H, I or 2I] and w_down [E, I, H] must agree with router_logits on E")
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"unknown activation {activation!r}; have {sorted(ACTIVATIONS)}")
+    if interleaved and activation != "swiglu":
+        raise RuntimeError("interleaved weights go with the swiglu activation")
+    if activation == "swiglu" and w_up.size(2) % (128 if interleaved else 2):
+        raise RuntimeError("swiglu needs an even number of columns, interleaved weights whole blocks of 128")
+    inner = w_up.size(2) // 2 if ACTIVATIONS[activation] else w_up.size(2)
+    if w_up.size(1) != x.size(1) or w_down.size(1) != inner or w_down.size(2) != x.size(1):
+        raise RuntimeError("weight shapes do not chain: x [T, H], w_up [E, H, I or 2I], w_down [E, I, H]")
+    if x.size(0) > FEW_TOKENS:
+        raise RuntimeError(f"moe_forward_few takes up to {FEW_TOKENS} tokens, got {x.size(0)}: use moe_forward")
+    if x.dtype not in (torch.bfloat16, torch.float16) or w_up.dtype != x.dtype or w_down.dtype != x.dtype:
+        raise RuntimeError(f"x, w_up and w_down have to be of one type, bfloat16 or float16, got {x.dtype}, {w_up.dtype}, {w_down.dtype}")
+    _dtype_code(router_logits.dtype)
+    _require_gpu(x, router_logits, w_up, w_down)
+    if not x.device == router_logits.device == w_up.device == w_down.device:
+        raise RuntimeError("x, router_logits, w_up and w_down must be on the same device")
+    E = router_logits.size(1)
+    if not 1 <= top_k <= min(E, 32):
+        raise RuntimeError(f"top_k must be in [1, min(experts, 32)], got {top_k} for {E} experts")
+    if E > 1023:
+        raise RuntimeError("Can't process more than 1024 groups")
+    if x.numel() and x.stride(1) != 1 and x.size(1) > 1 or x.size(0) > 1 and not x.size(1) <= x.stride(0) <= 1 << 23:
+        x = x.contiguous()
+    if router_logits.numel() and (router_logits.stride(1) != 1 and E > 1 or router_logits.stride(0) < E):
+        router_logits = router_logits.contiguous()
+    impl = _few_op if torch.compiler.is_compiling() else _few_now
+    return impl(x, router_logits, w_up, w_down, top_k, 2 if interleaved else ACTIVATIONS[activation], bool(renormalize))

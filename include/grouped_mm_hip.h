@@ -237,6 +237,25 @@ int gmm_moe_combine(const void* y, const int32_t* token_rows, const float* slot_
                     int64_t tokens, int64_t top_k, int64_t hidden, int64_t y_rows,
                     int64_t y_stride, int64_t out_stride, int32_t dtype, void* stream);
 
+/* The whole layer for a few tokens (up to 64): routing as gmm_moe_route, then
+ *   out[t, :] = sum_{j < top_k} slot_weight[t, j] * act(x[t, :] @ w_up[e_tj]) @ w_down[e_tj].
+ * x [tokens, hidden], logits [tokens, experts], w_up [experts, hidden, inner] or, for the two SwiGLU kinds, [.., 2 * inner] (gate
+ * columns, then partners, or 64 and 64 in turn as gmm_2d3d_swiglu has them: inner a multiple of 64), w_down [experts, inner, hidden];
+ * strides in elements, any for the weights (16-byte aligned ones contiguous along either dimension are read fastest), rows of x,
+ * logits and out contiguous; one expert's matrix below 2 GiB.  dtype bf16 or fp16, logits_dtype any gmm_dtype.  Unlike the calls
+ * it stands for it keeps the activations and the experts' results in 32 bits and rounds once.  `workspace`: device memory of
+ * gmm_moe_few_workspace_bytes(...) bytes (-1: sizes out of range), 16-byte aligned, its contents of no matter.  No host
+ * synchronisation, no allocation, no atomics. */
+enum gmm_activation { GMM_ACT_SILU = 0, GMM_ACT_SWIGLU = 1, GMM_ACT_SWIGLU_INTERLEAVED = 2 };
+int64_t gmm_moe_few_workspace_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner);
+int gmm_moe_few(const void* x, const void* logits, const void* w_up, const void* w_down, void* out,
+                int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner,
+                int64_t x_stride, int64_t logits_stride,
+                int64_t up_stride_g, int64_t up_stride_k, int64_t up_stride_n,
+                int64_t down_stride_g, int64_t down_stride_k, int64_t down_stride_n, int64_t out_stride,
+                int32_t kind, int32_t renormalize, int32_t dtype, int32_t logits_dtype,
+                void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- Layer norm over the last dimension.  No counterpart in the reference.
  *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps), var the mean square of x - mean,
  * x [rows, width], y [rows, width], row strides in elements (at least width where there is more than one row), width <= 16384.

@@ -70,3 +70,46 @@ def layer_norm_bounds(dy, x, weight, bias, eps, dtype, param_dtype):
     return [bounds[0], UNIT[dtype] * (rstd * (g + c1 + z * c2)) + TINY[dtype] + dx_err,
             UNIT[param_dtype] * (dy * z).sum(0) + TINY[param_dtype] + col_err * (dy * z).sum(0) + (dy * z_err).sum(0),
             UNIT[param_dtype] * dy.sum(0) + TINY[param_dtype] + col_err * dy.sum(0)]
+
+
+# ------------------------------------------------------------------ expert layer
+def moe_layer(x, logits, w_up, w_down, top_k, kind, renormalize=True):
+    """out, and its bound for a kernel that holds everything in between in 32 bits or as two 16-bit values and rounds once.
+    kind: "silu", "swiglu", "interleaved"."""
+    x, z, dtype = f64(x), f64(logits), x.dtype
+    order = torch.argsort(z, dim=1, descending=True, stable=True)[:, :top_k]
+    top = z.gather(1, order)
+    best = z.max(1, keepdim=True).values
+    if renormalize:
+        weight = torch.softmax(top, 1)
+    else:
+        weight = torch.exp(top - best) / torch.exp(z - best).sum(1, keepdim=True)
+    odd = torch.isinf(best)[:, 0]        # all weight, in equal shares, on what equals the maximum
+    if odd.any():
+        at = (top == best).double()
+        among = at.sum(1, keepdim=True) if renormalize else (z == best).double().sum(1, keepdim=True)
+        weight[odd] = (at / among)[odd]
+    two16 = {torch.bfloat16: 2.0 ** -15, torch.float16: 2.0 ** -21}[dtype]
+    H, I = x.size(1), w_down.size(1)
+    out, bound = torch.zeros_like(x), torch.zeros_like(x)
+    for e in order.unique().tolist():
+        token, choice = (order == e).nonzero(as_tuple=True)
+        U, D = f64(w_up[e]), f64(w_down[e])
+        h, h_abs = x[token] @ U, x[token].abs() @ U.abs()
+        h_err = (H / 16 + 40) * EPS32 * h_abs
+        if kind == "silu":
+            act = h * torch.sigmoid(h)
+            err = 1.1 * h_err + 32 * EPS32 * act.abs()
+        else:
+            c = torch.arange(I)
+            gate = c if kind == "swiglu" else c // 64 * 128 + c % 64
+            up = gate + (I if kind == "swiglu" else 64)
+            s = h[:, gate] * torch.sigmoid(h[:, gate])
+            act = s * h[:, up]
+            err = 1.1 * h_err[:, gate] * h[:, up].abs() + s.abs() * h_err[:, up] + 1.1 * h_err[:, gate] * h_err[:, up] + 32 * EPS32 * act.abs()
+        err = err + two16 * act.abs() + TINY[dtype]
+        w = weight[token, choice][:, None]
+        y_err = err @ D.abs() + (I / 16 + 60 + 2.0 ** 6) * EPS32 * (act.abs() @ D.abs())
+        out.index_add_(0, token, (act @ D) * w)
+        bound.index_add_(0, token, y_err * w + (act @ D).abs() * w * 2.0 ** -17)
+    return out, bound + UNIT[dtype] * out.abs() + TINY[dtype]
