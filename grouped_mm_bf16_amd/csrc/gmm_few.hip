@@ -58,14 +58,6 @@ __device__ __forceinline__ bool find_expert(const FewArgs& a, int which, int& ex
   return false;
 }
 
-// Range of k of a wave: whole steps, dealt evenly.
-template <int KS>
-__device__ __forceinline__ void wave_range(int begin, int end, int wave, int& from, int& to) {
-  const int steps = (end - begin + KS - 1) / KS, each = (steps + kWaves - 1) / kWaves;
-  from = begin + wave * each * KS;
-  to = min(end, from + each * KS);
-}
-
 // act[r] = act(x[token of row r] @ w_up[e]).  GLU: a strip is 8 * FR gate columns (lanes j < 8) and their partners (lane j + 8).
 template <typename T, int LAY, int MF, bool GLU>
 __global__ void __launch_bounds__(kThreads) few_up_kernel(const FewArgs a) {
@@ -93,12 +85,9 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(const FewArgs a) {
   for (int m = 0; m < MF; ++m)
     s.a_at[m] = 16 * m + j < rows ? uint32_t(a.row_token[row0 + 16 * m + j]) * uint32_t(a.x_ld) * 2 : kNowhere;
   f32x4 acc[MF][FR];
-#pragma unroll
-  for (int m = 0; m < MF; ++m)
-#pragma unroll
-    for (int i = 0; i < FR; ++i) acc[m][i] = f32x4{0, 0, 0, 0};
+  clear(acc);
   int from, to;
-  wave_range<S::KS>(0, a.H, wave, from, to);
+  wave_range<S::KS, kWaves>(0, a.H, wave, from, to);
   s.run(from, to, g, acc);
 
   T* const high = static_cast<T*>(a.act);
@@ -149,12 +138,9 @@ __global__ void __launch_bounds__(kThreads) few_down_kernel(const FewArgs a) {
 #pragma unroll
   for (int m = 0; m < MF; ++m) s.a_at[m] = 16 * m + j < rows ? uint32_t(row0 + 16 * m + j) * a.act_ld * 2 : kNowhere;
   f32x4 acc[MF][FR];
-#pragma unroll
-  for (int m = 0; m < MF; ++m)
-#pragma unroll
-    for (int i = 0; i < FR; ++i) acc[m][i] = f32x4{0, 0, 0, 0};
+  clear(acc);
   int from, to;
-  wave_range<S::KS>(part * a.k_part, min(a.inner, (part + 1) * a.k_part), wave, from, to);
+  wave_range<S::KS, kWaves>(part * a.k_part, min(a.inner, (part + 1) * a.k_part), wave, from, to);
   s.run(from, to, g, acc);
 
   float* const y = a.y + int64_t(part) * a.slots * a.H;
@@ -199,8 +185,6 @@ struct FewPlan {
   int parts, k_part;
 };
 
-int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
 // Parts along k of the second product: enough workgroups for every compute unit to have several, none shorter than two steps of all
 // waves.
 bool plan_few(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, FewPlan& p) {
@@ -222,16 +206,6 @@ bool plan_few(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, FewPlan& p)
   p.parts = p.k_part ? int((I + p.k_part - 1) / p.k_part) : 1;
   p.bytes = p.y_at + p.parts * p.slots * H * 4;
   return p.bytes < (int64_t(1) << 31);
-}
-
-bool multiple8(int64_t v) { return (v & 7) == 0; }
-
-// Layout of a stack of matrices [G, K, N] whose rows of A come 16 bytes at a time or (`whole` false) not.
-int layout_of(const void* w, int64_t sg, int64_t sk, int64_t sn, int64_t K, bool n_whole, bool whole) {
-  if (!whole || !aligned16(w) || !multiple8(sg) || !multiple8(K)) return GMM_W_ANY;
-  if (sn == 1 && multiple8(sk) && n_whole) return GMM_W_ROWS;
-  if (sk == 1 && multiple8(sn)) return GMM_W_COLS;
-  return GMM_W_ANY;
 }
 
 template <typename F>
@@ -271,14 +245,6 @@ int launch_few(FewArgs a, const FewPlan& p, int64_t I, const void* w_up, const i
   });
   hipLaunchKernelGGL((few_combine_kernel<T>), dim3(unsigned((a.H + kThreads - 1) / kThreads), unsigned(a.tokens)), dim3(kThreads), 0, stream, d);
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
-}
-
-// Bytes from the first to behind the last element of a matrix; 0: strides that do not fit or 2 GiB and more.
-uint32_t matrix_bytes(int64_t K, int64_t N, int64_t sk, int64_t sn) {
-  constexpr int64_t most = (int64_t(1) << 30) - 64;
-  if (sk < 0 || sn < 0 || (sk > 0 && K - 1 > most / sk) || (sn > 0 && N - 1 > most / sn)) return 0;
-  const int64_t n = (K - 1) * sk + (N - 1) * sn + 1;
-  return n > most ? 0 : uint32_t(n * 2);
 }
 
 }  // namespace

@@ -1,0 +1,772 @@
+// A projection that all rows share beside low-rank adapters of which each row has its own (declared in include/grouped_mm_hip.h):
+//   y[t] = x[t] @ W + scale[i] * (x[t] @ A[i]) @ B[i],  i = adapter[t]; a number outside [0, L): no adapter
+// and the adapters' gradients.
+//   A few rows (gmm_lora_linear): W and the adapters are read once, past the rows (gmm_skinny.h), in one launch; a second one adds the
+//     parts up.  Reading W bounds it.
+//   Many rows (gmm_lora_add): W's product is a grouped product of one group; what the adapters add is two thin products, bound by
+//     reading x and by reading and writing y.
+//   Gradients (gmm_lora_grad): dA[i] = scale[i] * sum of x[t]^T u[t], dB[i] = scale[i] * sum of low[t]^T dy[t] over the rows t that have
+//     adapter i: thin products along the rows, bound by reading x and dy.
+// The rank-sized values x @ A and dy @ B^T stay in fp32; where they are operands of a 16-bit product they are two values each.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/grouped_mm_hip.h"
+#include "gmm_launch.h"
+#include "gmm_skinny.h"
+
+namespace {
+
+using namespace gmm;
+
+constexpr int kFewRows = 64;
+constexpr int kMaxRank = 256;
+constexpr int kMaxAdapters = 1022;     // one more bin of the sort holds the rows without an adapter
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+
+struct Matrices {          // a stack [L, K, N] of 16-bit matrices, or one
+  const void* at;
+  int64_t sg;              // elements from one to the next
+  uint32_t sk, sn;         // elements
+  uint32_t bytes;          // of one
+};
+
+struct LoraArgs {
+  const void* x;
+  Matrices w, a, b;
+  const int32_t* adapter;
+  const float* scale;      // null: 1
+  void* out;
+  float* low;              // [low_parts][rows][R]: parts of x @ A
+  float* low_out;          // [rows][R]: their sums, null: not wanted
+  float* base;             // [base_parts][rows][N]: parts of x @ W
+  int64_t x_ld, out_ld;
+  int32_t rows, K, N, R, L;
+  int32_t strip_rows, low_parts, low_k, low_tiles;   // rows of a strip; parts of K and their length; strips of columns of A
+  int32_t base_parts, base_k, base_tiles, low_groups;
+};
+
+__device__ __forceinline__ bool has_adapter(int id, int L) { return id >= 0 && id < L; }
+
+template <typename T, typename S>
+__device__ __forceinline__ void set_matrix(S& s, const Matrices& m, int which, int column, int columns) {
+  s.w_buf = buffer(static_cast<const T*>(m.at) + which * m.sg, m.bytes);
+  s.columns = max(0, min(S::FR, columns - column));
+  s.w_at = uint32_t(column) * m.sn * 2;
+  s.w_step_k = m.sk * 2;
+  s.w_step_n = m.sn * 2;
+}
+
+// low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows; one adapter of theirs after the other.
+template <typename T, int LAY>
+__device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnySums<kWaves, Skinny<T, LAY, 1, 1, 2>::FR>& sums) {
+  using S = Skinny<T, LAY, 1, 1, 2>;
+  constexpr int FR = S::FR, OUT = S::COLUMNS;
+  const int part = item % a.low_parts, tile = item / a.low_parts % a.low_tiles, row0 = item / a.low_parts / a.low_tiles * a.strip_rows;
+  const int rows = min(a.strip_rows, a.rows - row0);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int id = j < rows ? a.adapter[row0 + j] : -1;
+  uint32_t todo = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
+  S s;
+  s.a_buf = buffer(static_cast<const T*>(a.x) + row0 * a.x_ld, uint32_t(((rows - 1) * a.x_ld + a.K) * 2));
+  s.a_plane = 0;
+  s.rows16 = 1;
+  int from, to;
+  wave_range<S::KS, kWaves>(part * a.low_k, min(a.K, (part + 1) * a.low_k), wave, from, to);
+  float* const low = a.low + (int64_t(part) * a.rows + row0) * a.R;
+  while (todo) {
+    const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
+    const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
+    todo &= ~mine;
+    set_matrix<T>(s, a.a, which, tile * OUT + FR * j, a.R);
+    s.a_at[0] = mine >> j & 1 ? uint32_t(j) * uint32_t(a.x_ld) * 2 : kNowhere;
+    f32x4 acc[1][FR];
+    clear(acc);
+    s.run(from, to, g, acc);
+    sums.put(wave, lane, acc[0]);
+    __syncthreads();
+    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+      const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
+      if (col >= a.R || !(mine >> 4 * og & 15)) continue;
+      const f32x4 h = sums.get(oc % FR, oc / FR, og);
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (mine >> (4 * og + v) & 1) low[(4 * og + v) * a.R + col] = h[v];
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int LAY>
+__global__ void __launch_bounds__(kThreads) lora_low_kernel(const LoraArgs a) {
+  __shared__ SkinnySums<kWaves, Skinny<T, LAY, 1, 1, 2>::FR> sums;
+  low_product<T, LAY>(a, blockIdx.x, sums);
+}
+
+// A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
+template <typename T, int LAY_W, int LAY_A, int MF>
+__global__ void __launch_bounds__(kThreads) lora_few_kernel(const LoraArgs a) {
+  using S = Skinny<T, LAY_W, MF, 1, 2>;
+  constexpr int FR = S::FR, OUT = S::COLUMNS;
+  __shared__ union Shared {
+    SkinnySums<kWaves, Skinny<T, LAY_A, 1, 1, 2>::FR> low;
+    SkinnySums<kWaves, FR> base;
+    __device__ Shared() {}
+  } shared;
+  if (int(blockIdx.x) < a.low_groups) return low_product<T, LAY_A>(a, blockIdx.x, shared.low);
+  const int item = blockIdx.x - a.low_groups, part = item % a.base_parts, tile = item / a.base_parts;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  S s;
+  set_matrix<T>(s, a.w, 0, tile * OUT + FR * j, a.N);
+  s.a_buf = buffer(a.x, uint32_t(((a.rows - 1) * a.x_ld + a.K) * 2));
+  s.a_plane = 0;
+  s.rows16 = (a.rows + 15) >> 4;
+#pragma unroll
+  for (int m = 0; m < MF; ++m) s.a_at[m] = 16 * m + j < a.rows ? uint32_t(16 * m + j) * uint32_t(a.x_ld) * 2 : kNowhere;
+  f32x4 acc[MF][FR];
+  clear(acc);
+  int from, to;
+  wave_range<S::KS, kWaves>(part * a.base_k, min(a.K, (part + 1) * a.base_k), wave, from, to);
+  s.run(from, to, g, acc);
+  float* const base = a.base + int64_t(part) * a.rows * a.N;
+#pragma unroll
+  for (int m = 0; m < MF; ++m) {
+    if (m >= s.rows16) break;
+    if (m) __syncthreads();
+    shared.base.put(wave, lane, acc[m]);
+    __syncthreads();
+    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+      const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
+      if (col >= a.N) continue;
+      const f32x4 h = shared.base.get(oc % FR, oc / FR, og);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int r = 16 * m + 4 * og + v;
+        if (r < a.rows) base[int64_t(r) * a.N + col] = h[v];
+      }
+    }
+  }
+}
+
+// Sums of the parts of x @ A of one row, times its adapter's scale.
+__device__ __forceinline__ float low_sum(const LoraArgs& a, int row, int r) {
+  float s = 0;
+  for (int p = 0; p < a.low_parts; ++p) s += a.low[(int64_t(p) * a.rows + row) * a.R + r];
+  return s;
+}
+
+// A few rows: y[t] = sum of the parts of x @ W + scale * low @ B.  A wave for 64 lanes' columns of one row: eight columns to a lane where B
+// is contiguous along them, else one.
+template <typename T, int LAY>
+__global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
+  constexpr int W = LAY == GMM_W_ROWS ? 8 : 1;
+  __shared__ float low[kMaxRank];
+  const int t = blockIdx.y, lane = threadIdx.x, c = (blockIdx.x * 64 + lane) * W;
+  const int id = a.adapter[t];
+  const bool has = has_adapter(id, a.L);
+  const float scale = has && a.scale ? a.scale[id] : 1.0f;
+  if (has)
+    for (int r = lane; r < a.R; r += 64) {
+      const float s = low_sum(a, t, r);
+      if (a.low_out && blockIdx.x == 0) a.low_out[int64_t(t) * a.R + r] = s;
+      low[r] = s * scale;
+    }
+  __syncthreads();
+  if (c >= a.N) return;
+  float y[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) y[i] = 0;
+  for (int p = 0; p < a.base_parts; ++p) {
+    const float* base = a.base + (int64_t(p) * a.rows + t) * a.N + c;
+    if constexpr (W == 8) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(base), hi = *reinterpret_cast<const f32x4*>(base + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
+    } else {
+      y[0] += base[0];
+    }
+  }
+  if (has) {
+    const T* b = static_cast<const T*>(a.b.at) + id * a.b.sg + int64_t(c) * a.b.sn;
+    float add[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) add[i] = 0;
+    if constexpr (LAY == GMM_W_ROWS) {
+#pragma unroll 8
+      for (int r = 0; r < a.R; ++r) {
+        const Pack<T, 8> v = *reinterpret_cast<const Pack<T, 8>*>(b + int64_t(r) * a.b.sk);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add[i] += low[r] * v.get(i);
+      }
+    } else if constexpr (LAY == GMM_W_COLS) {
+#pragma unroll 4
+      for (int r = 0; r < a.R; r += 8) {
+        const Pack<T, 8> v = *reinterpret_cast<const Pack<T, 8>*>(b + r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add[0] += low[r + i] * v.get(i);
+      }
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < a.R; ++r) add[0] += low[r] * widen(b[int64_t(r) * a.b.sk]);
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) y[i] += add[i];
+  }
+  T* out = static_cast<T*>(a.out) + t * a.out_ld + c;
+  if constexpr (W == 8) {
+    Pack<T, 8> o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.set(i, y[i]);
+    *reinterpret_cast<Pack<T, 8>*>(out) = o;
+  } else {
+    out[0] = rounded<T>(y[0]);
+  }
+}
+
+// Many rows: y[t] += scale * low @ B.  A workgroup takes 64 rows, a wave 16 of them, and `kAddStrips` strips of columns.  low, as two
+// 16-bit values each, lies in LDS; y is read and written where it is, 16 or 8 bytes to a lane.
+constexpr int kAddRows = 64, kAddStrips = 4;
+
+template <typename T, int LAY>
+__global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraArgs a, int wide_y, int pitch) {
+  using S = Skinny<T, LAY, 1, 2, 1>;
+  constexpr int FR = S::FR, OUT = S::COLUMNS, KS = S::KS;
+  extern __shared__ __align__(16) char shared[];     // [2][kAddRows][pitch]
+  T* const planes = reinterpret_cast<T*>(shared);
+  const int row0 = blockIdx.x * kAddRows;
+  for (int u = threadIdx.x; u < kAddRows * pitch; u += kThreads) {
+    const int r = u % pitch, row = row0 + u / pitch;
+    const int id = row < a.rows ? a.adapter[row] : -1;
+    float v = 0;
+    if (r < a.R && has_adapter(id, a.L)) {
+      v = low_sum(a, row, r);
+      if (a.low_out && blockIdx.y == 0) a.low_out[int64_t(row) * a.R + r] = v;
+      if (a.scale) v *= a.scale[id];
+    }
+    split(v, planes[u], planes[kAddRows * pitch + u]);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int first = row0 + 16 * wave;
+  const int id = first + j < a.rows ? a.adapter[first + j] : -1;
+  const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
+  if (!with) return;
+  S s;
+  s.rows16 = 1;
+  const T* const mine_high = planes + (16 * wave + j) * pitch;
+  const int end = (a.R + KS - 1) / KS * KS;
+  for (int strip = 0; strip < kAddStrips; ++strip) {
+    const int tile = blockIdx.y * kAddStrips + strip, c = tile * OUT + FR * j;
+    if (tile * OUT >= a.N) break;
+    const int columns = max(0, min(FR, a.N - c));
+    T* const y = static_cast<T*>(a.out) + int64_t(first + 4 * g) * a.out_ld + c;
+    T old[4][FR];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (!(with >> (4 * g + v) & 1)) continue;
+      if (wide_y) {
+        if (columns) __builtin_memcpy(old[v], __builtin_assume_aligned(y + v * a.out_ld, 2 * FR), 2 * FR);
+      } else {
+#pragma unroll
+        for (int i = 0; i < FR; ++i) if (i < columns) old[v][i] = y[v * a.out_ld + i];
+      }
+    }
+    for (uint32_t todo = with; todo;) {
+      const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
+      const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
+      todo &= ~mine;
+      set_matrix<T>(s, a.b, which, c, a.N);
+      f32x4 acc[1][FR];
+      clear(acc);
+      for (int k = 0; k < end; k += KS) {
+        typename S::Step step;
+        s.load_w(step, k, a.R, g);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int h = 0; h < KS / 32; ++h)
+            step.a[0][p][h] = *reinterpret_cast<const u32x4*>(mine_high + p * kAddRows * pitch + k + S::KG * g + 8 * h);
+        s.multiply(step, acc);
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        if (!(mine >> (4 * g + v) & 1)) continue;
+        T now[FR];
+#pragma unroll
+        for (int i = 0; i < FR; ++i) now[i] = rounded<T>(widen(old[v][i]) + acc[0][i][v]);
+        if (wide_y) {
+          if (columns) __builtin_memcpy(__builtin_assume_aligned(y + v * a.out_ld, 2 * FR), now, 2 * FR);
+        } else {
+#pragma unroll
+          for (int i = 0; i < FR; ++i) if (i < columns) y[v * a.out_ld + i] = now[i];
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradients
+// Rows are sorted by adapter; adapter i's begin at place(i) of the sorted operands: a multiple of 8, so that 8 rows' values can be read
+// 16 bytes at a time, and past all that earlier adapters have.
+__device__ __forceinline__ int place(const int32_t* offs, int i) { return ((i ? offs[i - 1] : 0) + 7) / 8 * 8 + 8 * i; }
+
+struct GradArgs {
+  const void* p;            // [rows][C]: x or dy
+  const void* q;            // [2][R][places]: low or u by place, times scale: high and low halves
+  const int32_t* row_at;    // [places] the row at a place
+  const int32_t* offs;      // [L + 1] ends of the adapters' rows
+  void* out;                // [L][R][C] with the strides below
+  float* partial;           // [slots][R][C]: of adapters whose rows are more than one chunk
+  int64_t p_ld, out_sg, out_sr, out_sc;
+  int32_t places, C, R, L, chunk, tiles;
+};
+
+// The `which`-th chunk of all adapters' rows: its adapter, first place, number of rows; slot: of its partial sums, -1: it is the only one.
+__device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& adapter, int& first, int& rows, int& slot) {
+  const int lane = threadIdx.x & 63;
+  int slots = 0;
+  for (int base = 0; base < a.L; base += 64) {
+    const int i = base + lane;
+    const int from = i < a.L && i ? a.offs[i - 1] : 0, n = i < a.L ? a.offs[i] - from : 0;
+    const int chunks = (n + a.chunk - 1) / a.chunk, own = chunks > 1 ? chunks : 0;
+    int sum = chunks, slot_sum = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int s = __shfl_up(sum, o), t = __shfl_up(slot_sum, o);
+      if (lane >= o) { sum += s; slot_sum += t; }
+    }
+    const uint64_t it = __ballot(which < sum);
+    if (it) {
+      const int at = __ffsll(static_cast<unsigned long long>(it)) - 1;
+      const int c = which - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(chunks, at));
+      adapter = base + at;
+      first = place(a.offs, adapter) + c * a.chunk;
+      rows = min(a.chunk, __builtin_amdgcn_readlane(n, at) - c * a.chunk);
+      slot = __builtin_amdgcn_readlane(own, at) ? slots + __builtin_amdgcn_readlane(slot_sum, at) - __builtin_amdgcn_readlane(own, at) + c : -1;
+      return true;
+    }
+    which -= __builtin_amdgcn_readlane(sum, 63);
+    slots += __builtin_amdgcn_readlane(slot_sum, 63);
+  }
+  return false;
+}
+
+constexpr int kMaxChunk = 4096;
+
+// out[i] += q^T p over a chunk of adapter i's rows: R rows, a strip of 128 columns of p, the contraction along p's rows.
+template <typename T, int LAY, int MF>
+__global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs a) {
+  using S = Skinny<T, LAY, MF, 2, 2>;
+  constexpr int FR = S::FR, OUT = S::COLUMNS;
+  static_assert(LAY != GMM_W_COLS, "rows of p are read along the columns");
+  __shared__ SkinnySums<kWaves, FR> sums;
+  __shared__ int32_t row_at[kMaxChunk];
+  int adapter, first, rows, slot;
+  if (!find_chunk(a, blockIdx.x / a.tiles, adapter, first, rows, slot)) return;
+  const int tile = blockIdx.x % a.tiles, r0 = blockIdx.y * 16 * MF;
+  for (int u = threadIdx.x; u < rows; u += kThreads) row_at[u] = a.row_at[first + u];
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c));
+  S s;
+  s.rows16 = min(MF, (a.R - r0 + 15) >> 4);
+  s.a_plane = uint32_t(a.R) * a.places * 2;
+  s.a_buf = buffer(a.q, 2 * s.a_plane);
+#pragma unroll
+  for (int m = 0; m < MF; ++m) s.a_at[m] = r0 + 16 * m + j < a.R ? (uint32_t(r0 + 16 * m + j) * a.places + first) * 2 : kNowhere;
+  const T* const p = static_cast<const T*>(a.p) + c;
+  // Steps as Skinny::load has them, from rows that are anywhere: 64-bit addresses, and zeros for the rows behind the end.
+  const auto load = [&](typename S::Step& step, int k, int end) {
+    const int kl = k + 8 * g;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      step.w[r] = u32x4{0, 0, 0, 0};
+      if (kl + r >= end || !columns) continue;
+      const T* at = p + int64_t(row_at[kl + r]) * a.p_ld;
+      if constexpr (LAY == GMM_W_ROWS) {
+        step.w[r] = *reinterpret_cast<const u32x4*>(at);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < columns) step.w[r][i / 2] |= uint32_t(at[i].bits) << 16 * (i & 1);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      if (m >= s.rows16) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        step.a[m][h][0] = __builtin_amdgcn_raw_buffer_load_b128(s.a_buf, int(s.a_at[m] != kNowhere && kl < end ? s.a_at[m] + h * s.a_plane + kl * 2 : kNowhere), 0, 0);
+      }
+    }
+  };
+  f32x4 acc[MF][FR];
+  clear(acc);
+  int from, to;
+  wave_range<32, kWaves>(0, rows, wave, from, to);
+  typename S::Step step[2];
+  load(step[0], from, to);
+  load(step[1], from + 32, to);
+  for (int k = from; k < to; k += 64)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s.multiply(step[u], acc);
+      load(step[u], k + 64 + 32 * u, to);
+    }
+#pragma unroll
+  for (int m = 0; m < MF; ++m) {
+    if (m >= s.rows16) break;
+    if (m) __syncthreads();
+    sums.put(wave, lane, acc[m]);
+    __syncthreads();
+    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+      const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
+      if (col >= a.C) continue;
+      const f32x4 h = sums.get(oc % FR, oc / FR, og);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int r = r0 + 16 * m + 4 * og + v;
+        if (r >= a.R) break;
+        if (slot >= 0) a.partial[(int64_t(slot) * a.R + r) * a.C + col] = h[v];
+        else static_cast<T*>(a.out)[adapter * a.out_sg + r * a.out_sr + col * a.out_sc] = rounded<T>(h[v]);
+      }
+    }
+  }
+}
+
+// Gradients of adapters whose rows were more than one chunk (the sum of the chunks, in order) or none (zeros).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) lora_grad_sum_kernel(const GradArgs a) {
+  const int adapter = blockIdx.y, lane = threadIdx.x & 63;
+  const int from = adapter ? a.offs[adapter - 1] : 0, n = a.offs[adapter] - from, chunks = (n + a.chunk - 1) / a.chunk;
+  if (chunks == 1) return;
+  int slot = 0;      // chunks of earlier adapters that have several
+  if (chunks) {
+    for (int i = lane; i < adapter; i += 64) {
+      const int m = (a.offs[i] - (i ? a.offs[i - 1] : 0) + a.chunk - 1) / a.chunk;
+      slot += m > 1 ? m : 0;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) slot += __shfl_xor(slot, o);
+  }
+  const int64_t each = int64_t(a.R) * a.C;
+  for (int64_t u = int64_t(blockIdx.x) * kThreads + threadIdx.x; u < each; u += int64_t(gridDim.x) * kThreads) {
+    const int64_t r = u / a.C, c = u - r * a.C;
+    float s = 0;
+    for (int k = 0; k < chunks; ++k) s += a.partial[(slot + k) * each + u];
+    static_cast<T*>(a.out)[adapter * a.out_sg + r * a.out_sr + c * a.out_sc] = rounded<T>(s);
+  }
+}
+
+// The bins of the sort: the rows without an adapter come last.
+__global__ void __launch_bounds__(kThreads) lora_bins_kernel(const int32_t* __restrict__ adapter, int rows, int L, int32_t* __restrict__ bins) {
+  const int t = blockIdx.x * kThreads + threadIdx.x;
+  if (t < rows) bins[t] = has_adapter(adapter[t], L) ? adapter[t] : L;
+}
+
+// Sorted operands: q1 and q2 [rows][R] fp32 (either may be null) as [2][R][places] 16-bit halves, times scale; rows by place.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) lora_sorted_kernel(const float* __restrict__ q1, const float* __restrict__ q2,
+                                                               const float* __restrict__ scale, const int32_t* __restrict__ bins,
+                                                               const int32_t* __restrict__ row_token, const int32_t* __restrict__ offs,
+                                                               int rows, int R, int L, int places, T* __restrict__ s1, T* __restrict__ s2,
+                                                               int32_t* __restrict__ row_at) {
+  const int at = blockIdx.x * kThreads + threadIdx.x, r = blockIdx.y;
+  if (at >= rows) return;
+  const int row = row_token[at], id = bins[row];
+  if (id >= L) return;
+  const int to = place(offs, id) + at - (id ? offs[id - 1] : 0);
+  const float by = scale ? scale[id] : 1.0f;
+  if (r == 0) row_at[to] = row;
+  const int64_t plane = int64_t(R) * places, slot = int64_t(r) * places + to;
+  if (q1) split(q1[int64_t(row) * R + r] * by, s1[slot], s1[plane + slot]);
+  if (q2) split(q2[int64_t(row) * R + r] * by, s2[slot], s2[plane + slot]);
+  // the adapter's last row: the places behind it, up to a multiple of 8, are read with it
+  if (at == offs[id] - 1)
+    for (int64_t t = slot + 1; t % 8; ++t) {
+      if (q1) s1[t] = s1[plane + t] = T{};
+      if (q2) s2[t] = s2[plane + t] = T{};
+    }
+}
+
+// ---------------------------------------------------------------- host side
+int clamp(int64_t v, int64_t lo, int64_t hi) { return int(v > hi ? (hi < lo ? lo : hi) : v < lo ? lo : v); }
+
+// `want` parts of k elements, each a multiple of 64 and at least 256 long.
+void cut(int64_t k, int64_t want, int32_t& parts, int32_t& each) {
+  parts = clamp(want, 1, k / 256);
+  each = int32_t(round_up((k + parts - 1) / parts, 64));
+  parts = each ? int32_t((k + each - 1) / each) : 1;
+}
+
+// Rows up to which x @ A is computed one row at a time, so that rows of different adapters are not in one another's way.
+constexpr int64_t kSingleRows = 256;
+
+struct LowPlan { int32_t strip_rows, parts, each; };
+
+LowPlan plan_low(int64_t rows, int64_t K) {
+  LowPlan p;
+  p.strip_rows = rows <= kSingleRows ? 1 : 16;
+  const int64_t strips = (rows + p.strip_rows - 1) / p.strip_rows;
+  cut(K, strips ? 1024 / strips : 1, p.parts, p.each);
+  return p;
+}
+
+struct BasePlan { int32_t parts, each; };
+
+BasePlan plan_base(int64_t rows, int64_t K, int64_t N) {
+  BasePlan p;
+  const int64_t strips = (N + 127) / 128;
+  int64_t want = strips ? 768 / strips : 1;
+  const int64_t most = K / 8 / (rows > 0 ? rows : 1);      // the parts' sums are written and read: half of W's bytes at most
+  if (want > most) want = most;
+  cut(K, want, p.parts, p.each);
+  return p;
+}
+
+template <typename F>
+void by_layout(int lay, F&& f) {
+  if (lay == GMM_W_ROWS) f(std::integral_constant<int, GMM_W_ROWS>{});
+  else if (lay == GMM_W_COLS) f(std::integral_constant<int, GMM_W_COLS>{});
+  else f(std::integral_constant<int, GMM_W_ANY>{});
+}
+
+int strip_columns(int lay) { return lay == GMM_W_COLS ? 64 : 128; }
+
+int layout_of(const Matrices& m, int64_t K, int64_t N, bool whole) { return gmm::layout_of(m.at, m.sg, m.sk, m.sn, K, multiple8(N), whole); }
+
+bool set(Matrices& m, const void* at, int64_t sg, int64_t sk, int64_t sn, int64_t K, int64_t N) {
+  if (sg < 0 || sk < 0 || sn < 0) return false;
+  m.at = at; m.sg = sg;
+  m.bytes = K && N ? matrix_bytes(K, N, sk, sn) : 2;
+  m.sk = K > 1 ? uint32_t(sk) : sk == 1 ? 1 : uint32_t(round_up(N, 8));      // of no matter: such that it does not decide the layout
+  m.sn = N > 1 ? uint32_t(sn) : sn == 1 ? 1 : uint32_t(round_up(K, 8));
+  return m.bytes != 0;
+}
+
+int check_sizes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int32_t dtype) {
+  constexpr int64_t most = (int64_t(1) << 30);
+  if (rows < 0 || K < 0 || N < 0 || R < 1 || L < 0 || rows >= most || K >= most || N >= most || R > kMaxRank || L > kMaxAdapters) return GMM_ERR_BAD_ARGUMENT;
+  return dtype == GMM_DT_BF16 || dtype == GMM_DT_F16 ? GMM_OK : GMM_ERR_UNSUPPORTED;
+}
+
+bool x_fits(int64_t x_ld, int64_t rows, int64_t K) {
+  return rows <= 1 || (x_ld >= K && x_ld <= ((int64_t(1) << 30) - 64 - K) / (rows < kFewRows ? rows : kFewRows));
+}
+
+void set_low(LoraArgs& a, int lay) {
+  const LowPlan lp = plan_low(a.rows, a.K);
+  a.strip_rows = lp.strip_rows; a.low_parts = lp.parts; a.low_k = lp.each;
+  a.low_tiles = (a.R + strip_columns(lay) - 1) / strip_columns(lay);
+  a.low_groups = (a.rows + a.strip_rows - 1) / a.strip_rows * a.low_tiles * a.low_parts;
+}
+
+template <typename T>
+int launch_few(LoraArgs a, int lay_w, int lay_a, int lay_b, hipStream_t stream) {
+  set_low(a, lay_a);
+  const BasePlan bp = plan_base(a.rows, a.K, a.N);
+  a.base_parts = bp.parts; a.base_k = bp.each;
+  a.base_tiles = (a.N + strip_columns(lay_w) - 1) / strip_columns(lay_w);
+  if (a.L == 0) a.low_groups = 0;
+  const dim3 grid(unsigned(a.low_groups + a.base_tiles * a.base_parts)), block(kThreads);
+  by_layout(lay_w, [&](auto w) {
+    by_layout(lay_a, [&](auto l) {
+      constexpr int W = decltype(w)::value, A = decltype(l)::value;
+      if (a.rows <= 16) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 1>), grid, block, 0, stream, a);
+      else if (a.rows <= 32) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 2>), grid, block, 0, stream, a);
+      else hipLaunchKernelGGL((lora_few_kernel<T, W, A, 4>), grid, block, 0, stream, a);
+    });
+  });
+  by_layout(lay_b, [&](auto l) {
+    constexpr int B = decltype(l)::value, W = B == GMM_W_ROWS ? 8 : 1;
+    hipLaunchKernelGGL((lora_finish_kernel<T, B>), dim3(unsigned((a.N + 64 * W - 1) / (64 * W)), unsigned(a.rows)), dim3(64), 0, stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_low(LoraArgs& a, int lay_a, hipStream_t stream) {
+  set_low(a, lay_a);
+  by_layout(lay_a, [&](auto l) {
+    hipLaunchKernelGGL((lora_low_kernel<T, decltype(l)::value>), dim3(unsigned(a.low_groups)), dim3(kThreads), 0, stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_add(LoraArgs a, int lay_a, int lay_b, hipStream_t stream) {
+  const int rc = launch_low<T>(a, lay_a, stream);
+  if (rc != GMM_OK) return rc;
+  const int wide = aligned16(a.out) && multiple8(a.out_ld) && multiple8(a.N);
+  by_layout(lay_b, [&](auto l) {
+    constexpr int B = decltype(l)::value;
+    const int pitch = int(round_up(a.R, B == GMM_W_COLS ? 64 : 32)) + 8;      // 16 bytes more: rows begin in other banks
+    const int columns = kAddStrips * strip_columns(B);
+    const dim3 grid(unsigned((a.rows + kAddRows - 1) / kAddRows), unsigned(a.N ? (a.N + columns - 1) / columns : 1));
+    hipLaunchKernelGGL((lora_add_kernel<T, B>), grid, dim3(kThreads), 2 * kAddRows * pitch * 2, stream, a, wide, pitch);
+  });
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+// Where the operands of gmm_lora_grad lie in its workspace.
+struct GradPlan {
+  int64_t table, places, bins_at, offs_at, token_at, rows_at, table_at, row_at, q_at[2], partial_at, bytes;
+  int32_t chunk;
+};
+
+bool plan_grad(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, GradPlan& p) {
+  p.table = gmm_moe_route_workspace_bytes(rows, L + 1, 1);
+  if (p.table < 0) return false;
+  // chunks: as long as gives every compute unit some strips of 128 columns, and the partial sums some 16 chunks of all rows at most
+  const int64_t widest = K > N ? K : N;
+  p.chunk = clamp(round_up(rows / 32, 128), 512, kMaxChunk);
+  p.places = round_up(rows, 8) + 8 * (L + 1);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) { const int64_t here = at; at = round_up(at + bytes, 256); return here; };
+  p.bins_at = take(rows * 4);
+  p.offs_at = take((L + 1) * 4);
+  p.token_at = take(rows * 4);
+  p.rows_at = take(rows * 4);
+  p.table_at = take(p.table);
+  p.row_at = take(p.places * 4);
+  for (int i = 0; i < 2; ++i) p.q_at[i] = take(2 * R * p.places * 2);
+  p.partial_at = take(2 * (rows / p.chunk) * R * widest * 4);      // adapters of several chunks: fewer than two per chunk of all rows
+  p.bytes = at;
+  return 2 * R * p.places * 2 < (int64_t(1) << 31);
+}
+
+template <typename T>
+int launch_grad(GradArgs g, int64_t rows, hipStream_t stream) {
+  if (g.C == 0) return GMM_OK;
+  const bool whole = aligned16(g.p) && multiple8(g.p_ld) && multiple8(g.C);
+  g.tiles = (g.C + 127) / 128;
+  const int64_t chunks = rows / g.chunk + (rows < g.L ? rows : g.L);
+  const auto launch = [&](auto lay, auto mf) {
+    constexpr int LAY = decltype(lay)::value, MF = decltype(mf)::value;
+    if (chunks)
+      hipLaunchKernelGGL((lora_grad_kernel<T, LAY, MF>), dim3(unsigned(chunks * g.tiles), unsigned((g.R + 16 * MF - 1) / (16 * MF))),
+                         dim3(kThreads), 0, stream, g);
+  };
+  const auto rank = [&](auto lay) {
+    if (g.R <= 16) launch(lay, std::integral_constant<int, 1>{});
+    else if (g.R <= 32) launch(lay, std::integral_constant<int, 2>{});
+    else launch(lay, std::integral_constant<int, 4>{});
+  };
+  if (whole) rank(std::integral_constant<int, GMM_W_ROWS>{});
+  else rank(std::integral_constant<int, GMM_W_ANY>{});
+  const int64_t blocks = (int64_t(g.R) * g.C + 4 * kThreads - 1) / (4 * kThreads);
+  hipLaunchKernelGGL((lora_grad_sum_kernel<T>), dim3(unsigned(blocks < 1024 ? blocks : 1024), unsigned(g.L)), dim3(kThreads), 0, stream, g);
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R) {
+  if (check_sizes(rows, K, N, R, 0, GMM_DT_BF16) != GMM_OK) return -1;
+  int64_t bytes = round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256);
+  if (rows <= kFewRows) bytes += int64_t(plan_base(rows, K, N).parts) * rows * N * 4;
+  return bytes;
+}
+
+int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* adapter, const float* scale, void* out,
+                    float* low, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride, int64_t w_stride_k,
+                    int64_t w_stride_n, int64_t a_stride_l, int64_t a_stride_k, int64_t a_stride_r, int64_t b_stride_l, int64_t b_stride_r,
+                    int64_t b_stride_n, int64_t out_stride, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int bad = check_sizes(rows, K, N, R, L, dtype);
+  if (bad) return bad;
+  if (rows > kFewRows) return GMM_ERR_UNSUPPORTED;
+  if (rows == 0 || N == 0) return GMM_OK;
+  LoraArgs g{};
+  if (!out || !adapter || (K && (!x || !w)) || (L && (!b || (K && !a))) || !x_fits(x_stride, rows, K) || (rows > 1 && out_stride < N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!set(g.w, w, 0, w_stride_k, w_stride_n, K, N)) return w_stride_k < 0 || w_stride_n < 0 ? GMM_ERR_BAD_ARGUMENT : GMM_ERR_UNSUPPORTED;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < gmm_lora_workspace_bytes(rows, K, N, R)) return GMM_ERR_WORKSPACE;
+  g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low;
+  g.low = static_cast<float*>(workspace);
+  g.base = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256));
+  g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
+  g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
+  const bool whole = aligned16(x) && multiple8(g.x_ld);
+  const int lay_w = layout_of(g.w, K, N, whole), lay_a = layout_of(g.a, K, R, whole);
+  const int lay_b = layout_of(g.b, R, N, true);
+  const bool wide = aligned16(out) && multiple8(g.out_ld);       // eight columns of the result at a time
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == GMM_DT_BF16) return launch_few<Bf16>(g, lay_w, lay_a, lay_b == GMM_W_ROWS && !wide ? GMM_W_ANY : lay_b, s);
+  return launch_few<F16>(g, lay_w, lay_a, lay_b == GMM_W_ROWS && !wide ? GMM_W_ANY : lay_b, s);
+}
+
+int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, void* out, float* low,
+                 int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride, int64_t a_stride_l, int64_t a_stride_k,
+                 int64_t a_stride_r, int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride, int32_t dtype,
+                 void* workspace, int64_t workspace_bytes, void* stream) {
+  const int bad = check_sizes(rows, K, N, R, L, dtype);
+  if (bad) return bad;
+  if (!out) N = 0;
+  if (rows == 0 || L == 0 || (N == 0 && !low)) return GMM_OK;
+  LoraArgs g{};
+  if (!adapter || (out && !b) || (K && (!x || !a)) || !x_fits(x_stride, rows, K) || (rows > 1 && out_stride < N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < int64_t(plan_low(rows, K).parts) * rows * R * 4) return GMM_ERR_WORKSPACE;
+  g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low; g.low = static_cast<float*>(workspace);
+  g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
+  g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
+  const int lay_a = layout_of(g.a, K, R, aligned16(x) && multiple8(g.x_ld)), lay_b = layout_of(g.b, R, N, true);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == GMM_DT_BF16 ? launch_add<Bf16>(g, lay_a, lay_b, s) : launch_add<F16>(g, lay_a, lay_b, s);
+}
+
+int64_t gmm_lora_grad_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L) {
+  GradPlan p;
+  return check_sizes(rows, K, N, R, L, GMM_DT_BF16) == GMM_OK && plan_grad(rows, K, N, R, L, p) ? p.bytes : -1;
+}
+
+int gmm_lora_grad(const void* x, const void* dy, const float* low, const float* u, const int32_t* adapter, const float* scale, void* da,
+                  void* db, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride, int64_t dy_stride,
+                  int64_t da_stride_l, int64_t da_stride_k, int64_t da_stride_r, int64_t db_stride_l, int64_t db_stride_r,
+                  int64_t db_stride_n, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int bad = check_sizes(rows, K, N, R, L, dtype);
+  if (bad) return bad;
+  if (L == 0 || (!da && !db)) return GMM_OK;
+  GradPlan p;
+  if (!plan_grad(rows, K, N, R, L, p)) return GMM_ERR_BAD_ARGUMENT;
+  if (rows && (!adapter || (da && (!u || (K && !x))) || (db && (!low || (N && !dy))))) return GMM_ERR_BAD_ARGUMENT;
+  if (rows > 1 && ((da && x_stride < K) || (db && dy_stride < N))) return GMM_ERR_BAD_ARGUMENT;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < p.bytes) return GMM_ERR_WORKSPACE;
+  char* const ws = static_cast<char*>(workspace);
+  const auto ints = [&](int64_t at) { return reinterpret_cast<int32_t*>(ws + at); };
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const unsigned blocks = unsigned((rows + kThreads - 1) / kThreads);
+  if (rows) hipLaunchKernelGGL(lora_bins_kernel, dim3(blocks), dim3(kThreads), 0, s, adapter, int(rows), int(L), ints(p.bins_at));
+  const int rc = gmm_sort_slots(ints(p.bins_at), rows, L + 1, ints(p.offs_at), ints(p.token_at), ints(p.rows_at), ws + p.table_at, s);
+  if (rc != GMM_OK) return rc;
+  GradArgs g{};
+  g.row_at = ints(p.row_at); g.offs = ints(p.offs_at); g.partial = reinterpret_cast<float*>(ws + p.partial_at);
+  g.places = int(p.places); g.R = int(R); g.L = int(L); g.chunk = p.chunk;
+  const auto both = [&](auto zero) {
+    using T = decltype(zero);
+    T* const qa = reinterpret_cast<T*>(ws + p.q_at[0]);
+    T* const qb = reinterpret_cast<T*>(ws + p.q_at[1]);
+    if (rows)
+      hipLaunchKernelGGL((lora_sorted_kernel<T>), dim3(blocks, unsigned(R)), dim3(kThreads), 0, s, da ? u : nullptr, db ? low : nullptr, scale,
+                         ints(p.bins_at), ints(p.token_at), ints(p.offs_at), int(rows), int(R), int(L), int(p.places), qa, qb, ints(p.row_at));
+    if (da) {
+      g.p = x; g.q = qa; g.out = da; g.p_ld = x_stride; g.C = int(K);
+      g.out_sg = da_stride_l; g.out_sr = da_stride_r; g.out_sc = da_stride_k;
+      const int rc = launch_grad<T>(g, rows, s);
+      if (rc != GMM_OK) return rc;
+    }
+    if (db) {
+      g.p = dy; g.q = qb; g.out = db; g.p_ld = dy_stride; g.C = int(N);
+      g.out_sg = db_stride_l; g.out_sr = db_stride_r; g.out_sc = db_stride_n;
+      return launch_grad<T>(g, rows, s);
+    }
+    return hipGetLastError() == hipSuccess ? int(GMM_OK) : int(GMM_ERR_LAUNCH);
+  };
+  return dtype == GMM_DT_BF16 ? both(Bf16{}) : both(F16{});
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "../../include/grouped_mm_hip.h"
+#include "gmm_launch.h"
 
 namespace {
 
@@ -490,6 +491,22 @@ bool plan_sort(int64_t tokens, int64_t top_k, SortPlan& pl) {
   return true;
 }
 
+// Stable sort of the slots by expert: offs, row_token, token_rows.
+int sort_planned(const int32_t* slot_expert, const SortPlan& pl, int64_t E, int64_t top_k, int32_t* offs, int32_t* row_token,
+                 int32_t* token_rows, int32_t* table, hipStream_t stream) {
+  if (pl.slots > 0 && pl.slots <= kPlaceSlots) {
+    hipLaunchKernelGGL(moe_place_kernel, dim3((pl.slots + kPlaceBlock - 1) / kPlaceBlock), dim3(kPlaceBlock), 0, stream, slot_expert,
+                       pl.slots, int(E), int(top_k), offs, row_token, token_rows);
+    return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+  }
+  if (pl.slots > 0) hipLaunchKernelGGL(moe_hist_kernel, dim3(pl.nb), dim3(256), 0, stream, slot_expert, pl.slots, pl.spb, int(E), table);
+  hipLaunchKernelGGL(moe_scan_kernel, dim3(1), dim3(1024), 0, stream, table, pl.nb, int(E), offs);
+  if (pl.slots > 0)
+    hipLaunchKernelGGL(moe_scatter_kernel, dim3(pl.nb), dim3(64), 0, stream, slot_expert, pl.slots, pl.spb, int(E), int(top_k),
+                       table, offs, row_token, token_rows);
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
 int route_checked(const void* logits, int64_t ld, int dtype, int64_t tokens, int64_t E, int64_t top_k, int renorm,
                   int32_t* offs, int32_t* slot_expert, float* slot_weight, int32_t* row_token, int32_t* token_rows,
                   int32_t* table, size_t table_bytes, hipStream_t stream) {
@@ -526,17 +543,9 @@ int route_checked(const void* logits, int64_t ld, int dtype, int64_t tokens, int
     if (dtype == GMM_DT_BF16) topk(static_cast<const Bf16*>(logits));
     else if (dtype == GMM_DT_F16) topk(static_cast<const F16*>(logits));
     else topk(static_cast<const float*>(logits));
-    if (!one && pl.slots <= kPlaceSlots)
-      hipLaunchKernelGGL(moe_place_kernel, dim3((pl.slots + kPlaceBlock - 1) / kPlaceBlock), dim3(kPlaceBlock), 0, stream, slot_expert,
-                         pl.slots, int(E), int(top_k), offs, row_token, token_rows);
-    if (one || pl.slots <= kPlaceSlots) return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
-    hipLaunchKernelGGL(moe_hist_kernel, dim3(pl.nb), dim3(256), 0, stream, slot_expert, pl.slots, pl.spb, int(E), table);
+    if (one) return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
   }
-  hipLaunchKernelGGL(moe_scan_kernel, dim3(1), dim3(1024), 0, stream, table, pl.nb, int(E), offs);
-  if (tokens > 0)
-    hipLaunchKernelGGL(moe_scatter_kernel, dim3(pl.nb), dim3(64), 0, stream, slot_expert, pl.slots, pl.spb, int(E), int(top_k),
-                       table, offs, row_token, token_rows);
-  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+  return sort_planned(slot_expert, pl, E, top_k, offs, row_token, token_rows, table, stream);
 }
 
 // Address of the current device's copy of `scratch`, looked up on the first call on that device.
@@ -554,6 +563,13 @@ int32_t* device_scratch() {
 }
 
 }  // namespace
+
+int gmm_sort_slots(const int32_t* slot_expert, int64_t slots, int64_t E, int32_t* offs, int32_t* row_token, int32_t* token_rows,
+                   void* table, hipStream_t stream) {
+  SortPlan pl;
+  if (slots < 0 || E < 1 || E > kMaxExperts || !plan_sort(slots, 1, pl)) return GMM_ERR_BAD_ARGUMENT;
+  return sort_planned(slot_expert, pl, E, 1, offs, row_token, token_rows, static_cast<int32_t*>(table), stream);
+}
 
 extern "C" {
 

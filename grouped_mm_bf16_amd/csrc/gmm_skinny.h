@@ -70,6 +70,11 @@ struct Skinny {
 
   // Loads k .. k + KS - 1, of which those before `end` exist.
   __device__ __forceinline__ void load(Step& s, int k, int end, int g) const {
+    load_w(s, k, end, g);
+    load_a(s, k, end, g);
+  }
+
+  __device__ __forceinline__ void load_w(Step& s, int k, int end, int g) const {
     const int kl = k + KG * g;
     if constexpr (LAY == GMM_W_ROWS) {
       const uint32_t at = w_at + uint32_t(kl) * w_step_k;
@@ -96,6 +101,10 @@ struct Skinny {
           s.w[r][q] = lo | hi << 16;
         }
     }
+  }
+
+  __device__ __forceinline__ void load_a(Step& s, int k, int end, int g) const {
+    const int kl = k + KG * g;
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
       if (m >= rows16) break;
@@ -161,6 +170,22 @@ struct Skinny {
   }
 };
 
+// Range of k of one of WAVES waves: whole steps of KS, dealt evenly.
+template <int KS, int WAVES>
+__device__ __forceinline__ void wave_range(int begin, int end, int wave, int& from, int& to) {
+  const int steps = (end - begin + KS - 1) / KS, each = (steps + WAVES - 1) / WAVES;
+  from = begin + wave * each * KS;
+  to = min(end, from + each * KS);
+}
+
+template <int MF, int FR>
+__device__ __forceinline__ void clear(f32x4 (&acc)[MF][FR]) {
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int i = 0; i < FR; ++i) acc[m][i] = f32x4{0, 0, 0, 0};
+}
+
 // Sums over the waves of a workgroup, one sixteen of rows at a time: sums[wave][product i][lane].
 template <int WAVES, int FR>
 struct SkinnySums {
@@ -179,5 +204,25 @@ struct SkinnySums {
     return s;
   }
 };
+
+// ---------------------------------------------------------------- host side
+inline bool multiple8(int64_t v) { return (v & 7) == 0; }
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Layout of a stack of matrices [G, K, N].  n_whole: columns come in whole eights; whole: 16 bytes of A can be read at a time.
+inline int layout_of(const void* w, int64_t sg, int64_t sk, int64_t sn, int64_t K, bool n_whole, bool whole) {
+  if (!whole || !aligned16(w) || !multiple8(sg) || !multiple8(K)) return GMM_W_ANY;
+  if (sn == 1 && multiple8(sk) && n_whole) return GMM_W_ROWS;
+  if (sk == 1 && multiple8(sn)) return GMM_W_COLS;
+  return GMM_W_ANY;
+}
+
+// Bytes from the first to behind the last element of a matrix of 16-bit elements; 0: strides that do not fit or 2 GiB and more.
+inline uint32_t matrix_bytes(int64_t K, int64_t N, int64_t sk, int64_t sn) {
+  constexpr int64_t most = (int64_t(1) << 30) - 64;
+  if (sk < 0 || sn < 0 || (sk > 0 && K - 1 > most / sk) || (sn > 0 && N - 1 > most / sn)) return 0;
+  const int64_t n = (K - 1) * sk + (N - 1) * sn + 1;
+  return n > most ? 0 : uint32_t(n * 2);
+}
 
 }  // namespace gmm

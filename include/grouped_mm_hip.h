@@ -256,6 +256,38 @@ int gmm_moe_few(const void* x, const void* logits, const void* w_up, const void*
                 int32_t kind, int32_t renormalize, int32_t dtype, int32_t logits_dtype,
                 void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- A projection that all rows share beside low-rank adapters of which each row has its own.  No counterpart in the reference.
+ *   out[t] = x[t] @ w + scale[i] * (x[t] @ a[i]) @ b[i],  i = adapter[t];  i outside [0, L): x[t] @ w alone.
+ * x [rows, K], w [K, N], a [L, K, R], b [L, R, N], out [rows, N] in bf16 or fp16 (dtype), adapter int32[rows], scale float[L] (NULL: ones);
+ * strides in elements, any for w, a and b (16-byte aligned and contiguous along one dimension: fastest), rows of x and out contiguous.
+ * R <= 256, L <= 1022, one matrix below 2 GiB.  `low`: float [rows, R], gets x[t] @ a[i] of the rows that have an adapter (NULL: not wanted;
+ * gmm_lora_grad needs it).  x @ a stays in fp32.  `workspace`: device memory of gmm_lora_workspace_bytes(...) bytes (-1: sizes out of
+ * range), 16-byte aligned, contents of no matter.
+ *   gmm_lora_linear   all of it, for up to 64 rows (GMM_ERR_UNSUPPORTED: more, or w of 2 GiB and more); rounded once.
+ *   gmm_lora_add      for any number: out += scale * (x @ a) @ b, to the product x @ w in `out`.  out NULL: `low` alone. */
+int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R);
+int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* adapter, const float* scale,
+                    void* out, float* low, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride,
+                    int64_t w_stride_k, int64_t w_stride_n, int64_t a_stride_l, int64_t a_stride_k, int64_t a_stride_r,
+                    int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride, int32_t dtype,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, void* out, float* low,
+                 int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride,
+                 int64_t a_stride_l, int64_t a_stride_k, int64_t a_stride_r,
+                 int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride, int32_t dtype,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The adapters' gradients, for dy [rows, N], low (above) and u float [rows, R], u[t] = dy[t] @ b[i]^T (what gmm_lora_add gives as `low`
+ * for dy and b, a with their last two strides swapped; dx is its `out`, added to dy @ w^T):
+ *   da[i] = scale[i] * sum over the rows t of adapter i of x[t]^T u[t]  [L, K, R],   db[i] = scale[i] * sum of low[t]^T dy[t]  [L, R, N],
+ * zeros for an adapter without rows; either may be NULL (and then x and u, or dy and low).  No atomics: the same every time. */
+int64_t gmm_lora_grad_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L);
+int gmm_lora_grad(const void* x, const void* dy, const float* low, const float* u, const int32_t* adapter, const float* scale,
+                  void* da, void* db, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L,
+                  int64_t x_stride, int64_t dy_stride, int64_t da_stride_l, int64_t da_stride_k, int64_t da_stride_r,
+                  int64_t db_stride_l, int64_t db_stride_r, int64_t db_stride_n, int32_t dtype,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- Layer norm over the last dimension.  No counterpart in the reference.
  *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps), var the mean square of x - mean,
  * x [rows, width], y [rows, width], row strides in elements (at least width where there is more than one row), width <= 16384.

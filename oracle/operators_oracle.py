@@ -113,3 +113,51 @@ def moe_layer(x, logits, w_up, w_down, top_k, kind, renormalize=True):
         out.index_add_(0, token, (act @ D) * w)
         bound.index_add_(0, token, y_err * w + (act @ D).abs() * w * 2.0 ** -17)
     return out, bound + UNIT[dtype] * out.abs() + TINY[dtype]
+
+
+# ------------------------------------------------------------------ projection with low-rank adapters
+def lora_linear(x, weight, lora_a, lora_b, adapter, scale=None):
+    """out and its bound: one rounding of the result, for more than 64 rows one of weight's product before it; fp32 sums; the rank-sized
+    product as two 16-bit values."""
+    dtype, many = x.dtype, x.size(0) > 64
+    x, weight, a, b = f64(x), f64(weight), f64(lora_a), f64(lora_b)
+    two16 = {torch.bfloat16: 2.0 ** -15, torch.float16: 2.0 ** -21}[dtype]
+    K, R = x.size(1), a.size(2)
+    base = x @ weight
+    err = (K / 16 + 80) * EPS32 * (x.abs() @ weight.abs()) + (UNIT[dtype] * base.abs() if many else 0)
+    out = base.clone()
+    for i in adapter.cpu().unique().tolist():
+        if not 0 <= i < a.size(0):
+            continue
+        at = (adapter.cpu() == i).nonzero()[:, 0]
+        s = 1.0 if scale is None else float(scale[i])
+        low = x[at] @ a[i]
+        low_err = (K / 16 + 80) * EPS32 * (x[at].abs() @ a[i].abs()) + (two16 + 4 * EPS32) * low.abs() + TINY[dtype] / max(abs(s), 1e-30)
+        out[at] += s * (low @ b[i])
+        err[at] += abs(s) * (low_err @ b[i].abs() + (R + 8) * EPS32 * (low.abs() @ b[i].abs()))
+    return out, err * (1 + UNIT[dtype]) + UNIT[dtype] * out.abs() + TINY[dtype]
+
+
+def lora_backward(dy, x, weight, lora_a, lora_b, adapter, scale=None):
+    """(dx, its bound), (dweight, ..), (da, ..), (db, ..)."""
+    dtype = x.dtype
+    dx = lora_linear(dy, weight.mT, lora_b.mT, lora_a.mT, adapter, scale)
+    dy, x, a, b = f64(dy), f64(x), f64(lora_a), f64(lora_b)
+    two16 = {torch.bfloat16: 2.0 ** -15, torch.float16: 2.0 ** -21}[dtype]
+    T, K, N = x.size(0), x.size(1), dy.size(1)
+    dw = x.T @ dy
+    dw_err = (T + 80) * EPS32 * (x.abs().T @ dy.abs())
+    da, db, da_err, db_err = (torch.zeros_like(t) for t in (a, b, a, b))
+    for i in adapter.cpu().unique().tolist():
+        if not 0 <= i < a.size(0):
+            continue
+        at = (adapter.cpu() == i).nonzero()[:, 0]
+        s = 1.0 if scale is None else float(scale[i])
+        low, u = x[at] @ a[i], dy[at] @ b[i].T
+        low_err = abs(s) * (K / 16 + 80) * EPS32 * (x[at].abs() @ a[i].abs()) + (two16 + 4 * EPS32) * abs(s) * low.abs() + TINY[dtype]
+        u_err = abs(s) * (N / 16 + 80) * EPS32 * (dy[at].abs() @ b[i].abs().T) + (two16 + 4 * EPS32) * abs(s) * u.abs() + TINY[dtype]
+        rows = (len(at) / 16 + 80) * EPS32
+        da[i], db[i] = s * (x[at].T @ u), s * (low.T @ dy[at])
+        da_err[i] = x[at].abs().T @ u_err + rows * abs(s) * (x[at].abs().T @ u.abs())
+        db_err[i] = low_err.T @ dy[at].abs() + rows * abs(s) * (low.abs().T @ dy[at].abs())
+    return dx, *((v, e + UNIT[dtype] * v.abs() + TINY[dtype]) for v, e in ((dw, dw_err), (da, da_err), (db, db_err)))
