@@ -23,11 +23,35 @@ template <> __device__ __forceinline__ Bf16 rounded<Bf16>(float f) { return Bf16
 template <> __device__ __forceinline__ F16 rounded<F16>(float f) { return F16{__builtin_bit_cast(uint16_t, static_cast<_Float16>(f))}; }
 template <> __device__ __forceinline__ float rounded<float>(float f) { return f; }
 
-// N adjacent elements as they lie in memory: N = 1, or a 16-byte aligned vector.
+// N adjacent elements as they lie in memory: one, or a 16-byte aligned vector, whose 16-bit elements stay two to a register.
 template <typename T, int N> struct alignas(N > 1 ? 16 : sizeof(T)) Pack {
   T v[N];
   __device__ __forceinline__ float get(int i) const { return widen(v[i]); }
-  __device__ __forceinline__ void set(int i, float f) { v[i] = rounded<T>(f); }
+  static __device__ __forceinline__ Pack of(const float (&f)[N]) {
+    Pack p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) p.v[i] = rounded<T>(f[i]);
+    return p;
+  }
+};
+
+template <typename T> struct alignas(16) Half8 {
+  u32x4 w;
+  __device__ __forceinline__ float get(int i) const { return widen(T{uint16_t(w[i / 2] >> 16 * (i & 1))}); }
+  static __device__ __forceinline__ Half8 of(const float (&f)[8]) {
+    Half8 p;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p.w[q] = uint32_t(rounded<T>(f[2 * q]).bits) | uint32_t(rounded<T>(f[2 * q + 1]).bits) << 16;
+    return p;
+  }
+};
+template <> struct Pack<Bf16, 8> : Half8<Bf16> {
+  __device__ Pack() = default;
+  __device__ __forceinline__ Pack(const Half8<Bf16>& h) : Half8<Bf16>(h) {}
+};
+template <> struct Pack<F16, 8> : Half8<F16> {
+  __device__ Pack() = default;
+  __device__ __forceinline__ Pack(const Half8<F16>& h) : Half8<F16>(h) {}
 };
 
 template <typename T> constexpr int kVector = 16 / int(sizeof(T));

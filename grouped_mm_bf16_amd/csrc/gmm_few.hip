@@ -60,8 +60,8 @@ __device__ __forceinline__ bool find_expert(const FewArgs& a, int which, int& ex
 
 // act[r] = act(x[token of row r] @ w_up[e]).  GLU: a strip is 8 * FR gate columns (lanes j < 8) and their partners (lane j + 8).
 template <typename T, int LAY, int MF, bool GLU>
-__global__ void __launch_bounds__(kThreads) few_up_kernel(const FewArgs a) {
-  using S = Skinny<T, LAY, MF, 1, 2>;
+__global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1) few_up_kernel(const FewArgs a) {
+  using S = Strip<T, LAY, MF, 1, 2>;
   constexpr int FR = S::FR, OUT = GLU ? 8 * FR : 16 * FR;
   __shared__ SkinnySums<kWaves, FR> sums;
   int expert, row0, rows;
@@ -80,7 +80,6 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(const FewArgs a) {
   s.w_step_k = a.w_sk * 2;
   s.w_step_n = a.w_sn * 2;
   s.a_plane = 0;
-  s.rows16 = (rows + 15) >> 4;
 #pragma unroll
   for (int m = 0; m < MF; ++m)
     s.a_at[m] = 16 * m + j < rows ? uint32_t(a.row_token[row0 + 16 * m + j]) * uint32_t(a.x_ld) * 2 : kNowhere;
@@ -88,13 +87,13 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(const FewArgs a) {
   clear(acc);
   int from, to;
   wave_range<S::KS, kWaves>(0, a.H, wave, from, to);
-  s.run(from, to, g, acc);
+  s.run(rows, from, to, g, acc);
 
   T* const high = static_cast<T*>(a.act);
   T* const low = high + int64_t(a.slots) * a.act_ld;
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
-    if (m >= s.rows16) break;
+    if (16 * m >= rows) break;
     if (m) __syncthreads();
     sums.put(wave, lane, acc[m]);
     __syncthreads();
@@ -117,8 +116,8 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(const FewArgs a) {
 
 // y[part][r] = act[r] @ w_down[e], over the part's range of k.
 template <typename T, int LAY, int MF>
-__global__ void __launch_bounds__(kThreads) few_down_kernel(const FewArgs a) {
-  using S = Skinny<T, LAY, MF, 2, 2>;
+__global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1) few_down_kernel(const FewArgs a) {
+  using S = Strip<T, LAY, MF, 2, 2>;
   constexpr int FR = S::FR, OUT = 16 * FR;
   __shared__ SkinnySums<kWaves, FR> sums;
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
@@ -134,19 +133,18 @@ __global__ void __launch_bounds__(kThreads) few_down_kernel(const FewArgs a) {
   s.w_at = uint32_t(c) * a.w_sn * 2;
   s.w_step_k = a.w_sk * 2;
   s.w_step_n = a.w_sn * 2;
-  s.rows16 = (rows + 15) >> 4;
 #pragma unroll
   for (int m = 0; m < MF; ++m) s.a_at[m] = 16 * m + j < rows ? uint32_t(row0 + 16 * m + j) * a.act_ld * 2 : kNowhere;
   f32x4 acc[MF][FR];
   clear(acc);
   int from, to;
   wave_range<S::KS, kWaves>(part * a.k_part, min(a.inner, (part + 1) * a.k_part), wave, from, to);
-  s.run(from, to, g, acc);
+  s.run(rows, from, to, g, acc);
 
   float* const y = a.y + int64_t(part) * a.slots * a.H;
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
-    if (m >= s.rows16) break;
+    if (16 * m >= rows) break;
     if (m) __syncthreads();
     sums.put(wave, lane, acc[m]);
     __syncthreads();

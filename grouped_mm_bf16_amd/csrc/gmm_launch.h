@@ -24,7 +24,7 @@ bool gmm_staged_uses_workspace(const GmmParams& p, int in_dtype, int num_cus);
 // Zeros in the rows (jagged rows) or columns (jagged columns) of the output that no group owns.
 int gmm_launch_zero_unowned(const GmmParams& p, int out_dtype, hipStream_t stream);
 
-// Stable sort of slots by expert, slot_expert[s] in [0, E), E <= 1023, as gmm_moe_route has it for one slot a token: offs [E],
+// Stable sort of slots by expert, E <= 1023, as gmm_moe_route has it for one slot a token; numbers outside [0, E) count as E - 1: offs [E],
 // row_token and token_rows [slots]; table: gmm_moe_route_workspace_bytes(slots, E, 1) bytes.  Returns a gmm_status.
 int gmm_sort_slots(const int32_t* slot_expert, int64_t slots, int64_t E, int32_t* offs, int32_t* row_token, int32_t* token_rows,
                    void* table, hipStream_t stream);

@@ -25,6 +25,8 @@ constexpr int kFewRows = 64;
 constexpr int kMaxRank = 256;
 constexpr int kMaxAdapters = 1022;     // one more bin of the sort holds the rows without an adapter
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
+// Waves of a workgroup of a few rows' launch: eight, four where the sums of 64 rows by 128 columns need half of the registers.
+constexpr int few_waves(int MF) { return MF == 4 ? 4 : 8; }
 
 struct Matrices {          // a stack [L, K, N] of 16-bit matrices, or one
   const void* at;
@@ -60,9 +62,11 @@ __device__ __forceinline__ void set_matrix(S& s, const Matrices& m, int which, i
 }
 
 // low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows; one adapter of theirs after the other.
-template <typename T, int LAY>
-__device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnySums<kWaves, Skinny<T, LAY, 1, 1, 2>::FR>& sums) {
-  using S = Skinny<T, LAY, 1, 1, 2>;
+template <typename T, int LAY, int FR, bool AE>
+using LowSkinny = Skinny<T, LAY, FR, LAY == GMM_W_COLS ? 2 : 1, AE, 1, 1, FR <= 2 ? 4 : 2>;
+
+template <typename T, typename S, int WAVES>
+__device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnySums<WAVES, S::FR>& sums) {
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   const int part = item % a.low_parts, tile = item / a.low_parts % a.low_tiles, row0 = item / a.low_parts / a.low_tiles * a.strip_rows;
   const int rows = min(a.strip_rows, a.rows - row0);
@@ -72,9 +76,8 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
   S s;
   s.a_buf = buffer(static_cast<const T*>(a.x) + row0 * a.x_ld, uint32_t(((rows - 1) * a.x_ld + a.K) * 2));
   s.a_plane = 0;
-  s.rows16 = 1;
   int from, to;
-  wave_range<S::KS, kWaves>(part * a.low_k, min(a.K, (part + 1) * a.low_k), wave, from, to);
+  wave_range<S::KS, WAVES>(part * a.low_k, min(a.K, (part + 1) * a.low_k), wave, from, to);
   float* const low = a.low + (int64_t(part) * a.rows + row0) * a.R;
   while (todo) {
     const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
@@ -84,10 +87,10 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
     s.a_at[0] = mine >> j & 1 ? uint32_t(j) * uint32_t(a.x_ld) * 2 : kNowhere;
     f32x4 acc[1][FR];
     clear(acc);
-    s.run(from, to, g, acc);
+    s.run(16, from, to, g, acc);
     sums.put(wave, lane, acc[0]);
     __syncthreads();
-    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+    for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.R || !(mine >> 4 * og & 15)) continue;
       const f32x4 h = sums.get(oc % FR, oc / FR, og);
@@ -99,45 +102,47 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
   }
 }
 
-template <typename T, int LAY>
-__global__ void __launch_bounds__(kThreads) lora_low_kernel(const LoraArgs a) {
-  __shared__ SkinnySums<kWaves, Skinny<T, LAY, 1, 1, 2>::FR> sums;
-  low_product<T, LAY>(a, blockIdx.x, sums);
+template <typename T, int LAY, int FR, bool AE>
+__global__ void __launch_bounds__(kThreads, FR <= 2 ? 3 : 2) lora_low_kernel(const LoraArgs a) {
+  using S = LowSkinny<T, LAY, FR, AE>;
+  __shared__ SkinnySums<kWaves, FR> sums;
+  low_product<T, S, kWaves>(a, blockIdx.x, sums);
 }
 
 // A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
 template <typename T, int LAY_W, int LAY_A, int MF>
-__global__ void __launch_bounds__(kThreads) lora_few_kernel(const LoraArgs a) {
-  using S = Skinny<T, LAY_W, MF, 1, 2>;
+__global__ void __launch_bounds__(64 * few_waves(MF)) lora_few_kernel(const LoraArgs a) {
+  constexpr int WAVES = few_waves(MF);
+  using S = Strip<T, LAY_W, MF, 1, 2>;
+  using SA = LowSkinny<T, LAY_A, 1, LAY_W == GMM_W_ANY>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   __shared__ union Shared {
-    SkinnySums<kWaves, Skinny<T, LAY_A, 1, 1, 2>::FR> low;
-    SkinnySums<kWaves, FR> base;
+    SkinnySums<WAVES, 1> low;
+    SkinnySums<WAVES, FR> base;
     __device__ Shared() {}
   } shared;
-  if (int(blockIdx.x) < a.low_groups) return low_product<T, LAY_A>(a, blockIdx.x, shared.low);
+  if (int(blockIdx.x) < a.low_groups) return low_product<T, SA, WAVES>(a, blockIdx.x, shared.low);
   const int item = blockIdx.x - a.low_groups, part = item % a.base_parts, tile = item / a.base_parts;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   S s;
   set_matrix<T>(s, a.w, 0, tile * OUT + FR * j, a.N);
   s.a_buf = buffer(a.x, uint32_t(((a.rows - 1) * a.x_ld + a.K) * 2));
   s.a_plane = 0;
-  s.rows16 = (a.rows + 15) >> 4;
 #pragma unroll
   for (int m = 0; m < MF; ++m) s.a_at[m] = 16 * m + j < a.rows ? uint32_t(16 * m + j) * uint32_t(a.x_ld) * 2 : kNowhere;
   f32x4 acc[MF][FR];
   clear(acc);
   int from, to;
-  wave_range<S::KS, kWaves>(part * a.base_k, min(a.K, (part + 1) * a.base_k), wave, from, to);
-  s.run(from, to, g, acc);
+  wave_range<S::KS, WAVES>(part * a.base_k, min(a.K, (part + 1) * a.base_k), wave, from, to);
+  s.run(a.rows, from, to, g, acc);
   float* const base = a.base + int64_t(part) * a.rows * a.N;
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
-    if (m >= s.rows16) break;
+    if (16 * m >= a.rows) break;
     if (m) __syncthreads();
     shared.base.put(wave, lane, acc[m]);
     __syncthreads();
-    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+    for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.N) continue;
       const f32x4 h = shared.base.get(oc % FR, oc / FR, og);
@@ -153,6 +158,7 @@ __global__ void __launch_bounds__(kThreads) lora_few_kernel(const LoraArgs a) {
 // Sums of the parts of x @ A of one row, times its adapter's scale.
 __device__ __forceinline__ float low_sum(const LoraArgs& a, int row, int r) {
   float s = 0;
+#pragma unroll 4
   for (int p = 0; p < a.low_parts; ++p) s += a.low[(int64_t(p) * a.rows + row) * a.R + r];
   return s;
 }
@@ -165,6 +171,23 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   __shared__ float low[kMaxRank];
   const int t = blockIdx.y, lane = threadIdx.x, c = (blockIdx.x * 64 + lane) * W;
   const int id = a.adapter[t];
+  float y[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) y[i] = 0;
+  if (c < a.N) {
+    const float* base = a.base + int64_t(t) * a.N + c;
+    const int64_t next = int64_t(a.rows) * a.N;
+#pragma unroll 4
+    for (int p = 0; p < a.base_parts; ++p, base += next) {
+      if constexpr (W == 8) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(base), hi = *reinterpret_cast<const f32x4*>(base + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
+      } else {
+        y[0] += base[0];
+      }
+    }
+  }
   const bool has = has_adapter(id, a.L);
   const float scale = has && a.scale ? a.scale[id] : 1.0f;
   if (has)
@@ -175,19 +198,6 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
     }
   __syncthreads();
   if (c >= a.N) return;
-  float y[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) y[i] = 0;
-  for (int p = 0; p < a.base_parts; ++p) {
-    const float* base = a.base + (int64_t(p) * a.rows + t) * a.N + c;
-    if constexpr (W == 8) {
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(base), hi = *reinterpret_cast<const f32x4*>(base + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
-    } else {
-      y[0] += base[0];
-    }
-  }
   if (has) {
     const T* b = static_cast<const T*>(a.b.at) + id * a.b.sg + int64_t(c) * a.b.sn;
     float add[W];
@@ -216,36 +226,36 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   }
   T* out = static_cast<T*>(a.out) + t * a.out_ld + c;
   if constexpr (W == 8) {
-    Pack<T, 8> o;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o.set(i, y[i]);
-    *reinterpret_cast<Pack<T, 8>*>(out) = o;
+    *reinterpret_cast<Pack<T, 8>*>(out) = Pack<T, 8>::of(y);
   } else {
     out[0] = rounded<T>(y[0]);
   }
 }
 
-// Many rows: y[t] += scale * low @ B.  A workgroup takes 64 rows, a wave 16 of them, and `kAddStrips` strips of columns.  low, as two
-// 16-bit values each, lies in LDS; y is read and written where it is, 16 or 8 bytes to a lane.
+// low of a row and its place in the rank, summed, written out where it is wanted, times scale; zero for a row without an adapter.
+__device__ __forceinline__ float scaled_low(const LoraArgs& a, int row, int r) {
+  const int id = row < a.rows ? a.adapter[row] : -1;
+  if (r >= a.R || !has_adapter(id, a.L)) return 0;
+  const float v = low_sum(a, row, r);
+  if (a.low_out && blockIdx.y == 0) a.low_out[int64_t(row) * a.R + r] = v;
+  return a.scale ? v * a.scale[id] : v;
+}
+
+// Many rows: y[t] += scale * low @ B.  A workgroup takes 64 rows, a wave 16 of them, and kAddStrips strips of 128 columns.  low, as two
+// 16-bit values each, lies in LDS; y is read and written where it is, 16 bytes to a lane where it can be.  16 waves to a compute
+// unit hide its latency.
 constexpr int kAddRows = 64, kAddStrips = 4;
 
 template <typename T, int LAY>
-__global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraArgs a, int wide_y, int pitch) {
-  using S = Skinny<T, LAY, 1, 2, 1>;
+__global__ void __launch_bounds__(kThreads, 3) lora_add_kernel(const LoraArgs a, int wide_y, int pitch) {
+  using S = Skinny<T, LAY, 8, 1, false, 1, 2, 1>;
   constexpr int FR = S::FR, OUT = S::COLUMNS, KS = S::KS;
   extern __shared__ __align__(16) char shared[];     // [2][kAddRows][pitch]
   T* const planes = reinterpret_cast<T*>(shared);
   const int row0 = blockIdx.x * kAddRows;
   for (int u = threadIdx.x; u < kAddRows * pitch; u += kThreads) {
-    const int r = u % pitch, row = row0 + u / pitch;
-    const int id = row < a.rows ? a.adapter[row] : -1;
-    float v = 0;
-    if (r < a.R && has_adapter(id, a.L)) {
-      v = low_sum(a, row, r);
-      if (a.low_out && blockIdx.y == 0) a.low_out[int64_t(row) * a.R + r] = v;
-      if (a.scale) v *= a.scale[id];
-    }
-    split(v, planes[u], planes[kAddRows * pitch + u]);
+    const int r = u % pitch;
+    split(scaled_low(a, row0 + u / pitch, r), planes[u], planes[kAddRows * pitch + u]);
   }
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
@@ -254,25 +264,25 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraArgs a, in
   const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
   if (!with) return;
   S s;
-  s.rows16 = 1;
-  const T* const mine_high = planes + (16 * wave + j) * pitch;
-  const int end = (a.R + KS - 1) / KS * KS;
+  const T* const mine_high = planes + (16 * wave + j) * pitch + 8 * g;
+#pragma unroll 1
   for (int strip = 0; strip < kAddStrips; ++strip) {
     const int tile = blockIdx.y * kAddStrips + strip, c = tile * OUT + FR * j;
     if (tile * OUT >= a.N) break;
     const int columns = max(0, min(FR, a.N - c));
     T* const y = static_cast<T*>(a.out) + int64_t(first + 4 * g) * a.out_ld + c;
-    T old[4][FR];
+    Pack<T, FR> old[4];
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       if (!(with >> (4 * g + v) & 1)) continue;
       if (wide_y) {
-        if (columns) __builtin_memcpy(old[v], __builtin_assume_aligned(y + v * a.out_ld, 2 * FR), 2 * FR);
+        if (columns) old[v] = *reinterpret_cast<const Pack<T, FR>*>(y + v * a.out_ld);
       } else {
 #pragma unroll
-        for (int i = 0; i < FR; ++i) if (i < columns) old[v][i] = y[v * a.out_ld + i];
+        for (int i = 0; i < FR; ++i) if (i < columns) old[v].w[i / 2] = i & 1 ? old[v].w[i / 2] | uint32_t(y[v * a.out_ld + i].bits) << 16 : y[v * a.out_ld + i].bits;
       }
     }
+#pragma unroll 1
     for (uint32_t todo = with; todo;) {
       const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
       const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
@@ -280,30 +290,69 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraArgs a, in
       set_matrix<T>(s, a.b, which, c, a.N);
       f32x4 acc[1][FR];
       clear(acc);
-      for (int k = 0; k < end; k += KS) {
+#pragma unroll 1
+      for (int k = 0; k < a.R; k += KS) {
         typename S::Step step;
         s.load_w(step, k, a.R, g);
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int h = 0; h < KS / 32; ++h)
-            step.a[0][p][h] = *reinterpret_cast<const u32x4*>(mine_high + p * kAddRows * pitch + k + S::KG * g + 8 * h);
-        s.multiply(step, acc);
+        for (int p = 0; p < 2; ++p) step.a[0][p][0] = *reinterpret_cast<const u32x4*>(mine_high + p * kAddRows * pitch + k);
+        s.template multiply<1>(step, acc);
       }
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         if (!(mine >> (4 * g + v) & 1)) continue;
-        T now[FR];
+        float now[FR];
 #pragma unroll
-        for (int i = 0; i < FR; ++i) now[i] = rounded<T>(widen(old[v][i]) + acc[0][i][v]);
+        for (int i = 0; i < FR; ++i) now[i] = old[v].get(i) + acc[0][i][v];
         if (wide_y) {
-          if (columns) __builtin_memcpy(__builtin_assume_aligned(y + v * a.out_ld, 2 * FR), now, 2 * FR);
+          if (columns) *reinterpret_cast<Pack<T, FR>*>(y + v * a.out_ld) = Pack<T, FR>::of(now);
         } else {
 #pragma unroll
-          for (int i = 0; i < FR; ++i) if (i < columns) y[v * a.out_ld + i] = now[i];
+          for (int i = 0; i < FR; ++i) if (i < columns) y[v * a.out_ld + i] = rounded<T>(now[i]);
         }
       }
     }
+  }
+}
+
+// The same where B has no alignment: a thread has one column and 16 rows, and multiplies on the vector units, in fp32.
+constexpr int kAnyRows = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) lora_add_any_kernel(const LoraArgs a) {
+  __shared__ f32x4 low[kAnyRows][kMaxRank / 4 + 1];
+  const int row0 = blockIdx.x * kAnyRows, c = blockIdx.y * kThreads + threadIdx.x, lane = threadIdx.x & 63;
+  const int span = int(a.R + 3) / 4 * 4;
+  for (int u = threadIdx.x; u < kAnyRows * span; u += kThreads)
+    reinterpret_cast<float*>(low[u / span])[u % span] = scaled_low(a, row0 + u / span, u % span);
+  __syncthreads();
+  const int id = lane < kAnyRows && row0 + lane < a.rows ? a.adapter[row0 + lane] : -1;
+  const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L)));
+  if (c >= a.N) return;
+  for (uint32_t todo = with; todo;) {
+    const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
+    uint32_t mine = 0;
+    for (int t = 0; t < kAnyRows; ++t) mine |= __builtin_amdgcn_readlane(id, t) == which ? 1u << t : 0u;
+    todo &= ~mine;
+    const T* b = static_cast<const T*>(a.b.at) + which * a.b.sg + int64_t(c) * a.b.sn;
+    float acc[kAnyRows];
+#pragma unroll
+    for (int t = 0; t < kAnyRows; ++t) acc[t] = 0;
+    for (int r = 0; r < a.R; r += 4) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = r + i < a.R ? widen(b[int64_t(r + i) * a.b.sk]) : 0.0f;
+#pragma unroll
+      for (int t = 0; t < kAnyRows; ++t) {
+        const f32x4 l = low[t][r / 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t] += l[i] * v[i];
+      }
+    }
+    T* const y = static_cast<T*>(a.out) + int64_t(row0) * a.out_ld + c;
+#pragma unroll
+    for (int t = 0; t < kAnyRows; ++t)
+      if (mine >> t & 1) y[t * a.out_ld] = rounded<T>(widen(y[t * a.out_ld]) + acc[t]);
   }
 }
 
@@ -312,16 +361,26 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraArgs a, in
 // 16 bytes at a time, and past all that earlier adapters have.
 __device__ __forceinline__ int place(const int32_t* offs, int i) { return ((i ? offs[i - 1] : 0) + 7) / 8 * 8 + 8 * i; }
 
-struct GradArgs {
+// One of the two gradients: out[i] = q^T p over adapter i's rows.
+struct GradOf {
   const void* p;            // [rows][C]: x or dy
-  const void* q;            // [2][R][places]: low or u by place, times scale: high and low halves
+  const void* q;            // [2][R][places]: u or low by place, times scale: high and low halves
+  void* out;                // [L][R][C] with the strides below
+  float* partial;           // [slots][R * C] as `out` has it: of adapters whose rows are more than one chunk
+  int64_t p_ld, out_sg, out_sr, out_sc;
+  int32_t C, tiles, whole;  // whole: rows of p can be read 16 bytes at a time
+  int32_t r_first;          // out is contiguous along R (of partial: always along one of the two)
+};
+
+struct GradArgs {
+  GradOf of[2];
   const int32_t* row_at;    // [places] the row at a place
   const int32_t* offs;      // [L + 1] ends of the adapters' rows
-  void* out;                // [L][R][C] with the strides below
-  float* partial;           // [slots][R][C]: of adapters whose rows are more than one chunk
-  int64_t p_ld, out_sg, out_sr, out_sc;
-  int32_t places, C, R, L, chunk, tiles;
+  int32_t places, R, L, chunk, groups0;   // groups0: workgroups of of[0]
 };
+
+// An adapter's n rows are dealt evenly to as many chunks as are needed (one for no rows: its gradient is zero).
+__device__ __forceinline__ int chunks_of(int n, int chunk) { return n > chunk ? (n + chunk - 1) / chunk : 1; }
 
 // The `which`-th chunk of all adapters' rows: its adapter, first place, number of rows; slot: of its partial sums, -1: it is the only one.
 __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& adapter, int& first, int& rows, int& slot) {
@@ -330,7 +389,7 @@ __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& ad
   for (int base = 0; base < a.L; base += 64) {
     const int i = base + lane;
     const int from = i < a.L && i ? a.offs[i - 1] : 0, n = i < a.L ? a.offs[i] - from : 0;
-    const int chunks = (n + a.chunk - 1) / a.chunk, own = chunks > 1 ? chunks : 0;
+    const int chunks = i < a.L ? chunks_of(n, a.chunk) : 0, own = chunks > 1 ? chunks : 0;
     int sum = chunks, slot_sum = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -340,11 +399,12 @@ __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& ad
     const uint64_t it = __ballot(which < sum);
     if (it) {
       const int at = __ffsll(static_cast<unsigned long long>(it)) - 1;
-      const int c = which - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(chunks, at));
+      const int count = __builtin_amdgcn_readlane(chunks, at), all = __builtin_amdgcn_readlane(n, at);
+      const int c = which - (__builtin_amdgcn_readlane(sum, at) - count), each = ((all + count - 1) / count + 7) / 8 * 8;
       adapter = base + at;
-      first = place(a.offs, adapter) + c * a.chunk;
-      rows = min(a.chunk, __builtin_amdgcn_readlane(n, at) - c * a.chunk);
-      slot = __builtin_amdgcn_readlane(own, at) ? slots + __builtin_amdgcn_readlane(slot_sum, at) - __builtin_amdgcn_readlane(own, at) + c : -1;
+      first = place(a.offs, adapter) + c * each;
+      rows = max(0, min(each, all - c * each));
+      slot = count > 1 ? slots + __builtin_amdgcn_readlane(slot_sum, at) - count + c : -1;
       return true;
     }
     which -= __builtin_amdgcn_readlane(sum, 63);
@@ -356,51 +416,48 @@ __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& ad
 constexpr int kMaxChunk = 4096;
 
 // out[i] += q^T p over a chunk of adapter i's rows: R rows, a strip of 128 columns of p, the contraction along p's rows.
-template <typename T, int LAY, int MF>
-__global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs a) {
-  using S = Skinny<T, LAY, MF, 2, 2>;
+template <typename T, int MF>
+__global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args) {
+  using S = Skinny<T, GMM_W_ROWS, 8, 1, false, MF, 2, 2>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
-  static_assert(LAY != GMM_W_COLS, "rows of p are read along the columns");
   __shared__ SkinnySums<kWaves, FR> sums;
   __shared__ int32_t row_at[kMaxChunk];
+  const bool second = int(blockIdx.x) >= args.groups0;
+  const GradOf& a = args.of[second];
+  const int item = blockIdx.x - (second ? args.groups0 : 0);
   int adapter, first, rows, slot;
-  if (!find_chunk(a, blockIdx.x / a.tiles, adapter, first, rows, slot)) return;
-  const int tile = blockIdx.x % a.tiles, r0 = blockIdx.y * 16 * MF;
-  for (int u = threadIdx.x; u < rows; u += kThreads) row_at[u] = a.row_at[first + u];
+  if (!find_chunk(args, item / a.tiles, adapter, first, rows, slot)) return;
+  const int tile = item % a.tiles, r0 = blockIdx.y * 16 * MF;
+  for (int u = threadIdx.x; u < rows; u += kThreads) row_at[u] = args.row_at[first + u];
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c));
+  const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c)), R = args.R;
   S s;
-  s.rows16 = min(MF, (a.R - r0 + 15) >> 4);
-  s.a_plane = uint32_t(a.R) * a.places * 2;
+  s.a_plane = uint32_t(R) * args.places * 2;
   s.a_buf = buffer(a.q, 2 * s.a_plane);
 #pragma unroll
-  for (int m = 0; m < MF; ++m) s.a_at[m] = r0 + 16 * m + j < a.R ? (uint32_t(r0 + 16 * m + j) * a.places + first) * 2 : kNowhere;
+  for (int m = 0; m < MF; ++m) s.a_at[m] = r0 + 16 * m + j < R ? (uint32_t(r0 + 16 * m + j) * args.places + first) * 2 : kNowhere;
   const T* const p = static_cast<const T*>(a.p) + c;
   // Steps as Skinny::load has them, from rows that are anywhere: 64-bit addresses, and zeros for the rows behind the end.
   const auto load = [&](typename S::Step& step, int k, int end) {
     const int kl = k + 8 * g;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      step.w[r] = u32x4{0, 0, 0, 0};
-      if (kl + r >= end || !columns) continue;
-      const T* at = p + int64_t(row_at[kl + r]) * a.p_ld;
-      if constexpr (LAY == GMM_W_ROWS) {
-        step.w[r] = *reinterpret_cast<const u32x4*>(at);
-      } else {
+      u32x4 v = {0, 0, 0, 0};
+      if (kl + r < end && columns) {
+        const T* at = p + int64_t(row_at[kl + r]) * a.p_ld;
+        if (a.whole) {
+          v = *reinterpret_cast<const u32x4*>(at);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < columns) step.w[r][i / 2] |= uint32_t(at[i].bits) << 16 * (i & 1);
+          for (int i = 0; i < 8; ++i)
+            if (i < columns) v[i / 2] |= uint32_t(at[i].bits) << 16 * (i & 1);
+        }
       }
-    }
 #pragma unroll
-    for (int m = 0; m < MF; ++m) {
-      if (m >= s.rows16) break;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        step.a[m][h][0] = __builtin_amdgcn_raw_buffer_load_b128(s.a_buf, int(s.a_at[m] != kNowhere && kl < end ? s.a_at[m] + h * s.a_plane + kl * 2 : kNowhere), 0, 0);
-      }
+      for (int i = 0; i < 4; ++i) step.w[4 * r + i] = v[i];
     }
+    s.template load_a<MF>(step, k, end, g);
   };
   f32x4 acc[MF][FR];
   clear(acc);
@@ -412,12 +469,12 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs a) {
   for (int k = from; k < to; k += 64)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      s.multiply(step[u], acc);
+      s.template multiply<MF>(step[u], acc);
       load(step[u], k + 64 + 32 * u, to);
     }
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
-    if (m >= s.rows16) break;
+    if (r0 + 16 * m >= R) break;
     if (m) __syncthreads();
     sums.put(wave, lane, acc[m]);
     __syncthreads();
@@ -425,58 +482,61 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs a) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.C) continue;
       const f32x4 h = sums.get(oc % FR, oc / FR, og);
+      const int r = r0 + 16 * m + 4 * og;
+      if (slot >= 0) {
+        float* const to = a.partial + int64_t(slot) * R * a.C + (a.r_first ? int64_t(col) * R + r : int64_t(r) * a.C + col);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int r = r0 + 16 * m + 4 * og + v;
-        if (r >= a.R) break;
-        if (slot >= 0) a.partial[(int64_t(slot) * a.R + r) * a.C + col] = h[v];
-        else static_cast<T*>(a.out)[adapter * a.out_sg + r * a.out_sr + col * a.out_sc] = rounded<T>(h[v]);
+        for (int v = 0; v < 4; ++v) if (r + v < R) to[a.r_first ? v : int64_t(v) * a.C] = h[v];
+      } else {
+        T* const to = static_cast<T*>(a.out) + adapter * a.out_sg + r * a.out_sr + col * a.out_sc;
+        if (a.r_first == 2 && r < R) {
+          const uint64_t v = uint64_t(rounded<T>(h[0]).bits) | uint64_t(rounded<T>(h[1]).bits) << 16 | uint64_t(rounded<T>(h[2]).bits) << 32 |
+                             uint64_t(rounded<T>(h[3]).bits) << 48;
+          *reinterpret_cast<uint64_t*>(to) = v;
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) if (r + v < R) to[v * a.out_sr] = rounded<T>(h[v]);
+        }
       }
     }
   }
 }
 
-// Gradients of adapters whose rows were more than one chunk (the sum of the chunks, in order) or none (zeros).
+// Gradients of adapters whose rows were more than one chunk: the sum of the chunks, in order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) lora_grad_sum_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(kThreads) lora_grad_sum_kernel(const GradArgs args) {
+  const GradOf& a = args.of[blockIdx.z];
   const int adapter = blockIdx.y, lane = threadIdx.x & 63;
-  const int from = adapter ? a.offs[adapter - 1] : 0, n = a.offs[adapter] - from, chunks = (n + a.chunk - 1) / a.chunk;
+  const int chunks = chunks_of(args.offs[adapter] - (adapter ? args.offs[adapter - 1] : 0), args.chunk);
   if (chunks == 1) return;
   int slot = 0;      // chunks of earlier adapters that have several
-  if (chunks) {
-    for (int i = lane; i < adapter; i += 64) {
-      const int m = (a.offs[i] - (i ? a.offs[i - 1] : 0) + a.chunk - 1) / a.chunk;
-      slot += m > 1 ? m : 0;
-    }
+  for (int i = lane; i < adapter; i += 64) {
+    const int m = chunks_of(args.offs[i] - (i ? args.offs[i - 1] : 0), args.chunk);
+    slot += m > 1 ? m : 0;
+  }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) slot += __shfl_xor(slot, o);
-  }
-  const int64_t each = int64_t(a.R) * a.C;
-  for (int64_t u = int64_t(blockIdx.x) * kThreads + threadIdx.x; u < each; u += int64_t(gridDim.x) * kThreads) {
-    const int64_t r = u / a.C, c = u - r * a.C;
+  for (int o = 32; o > 0; o >>= 1) slot += __shfl_xor(slot, o);
+  const int inner = a.r_first ? args.R : a.C, each = args.R * a.C;
+  const int64_t s_outer = a.r_first ? a.out_sc : a.out_sr, s_inner = a.r_first ? a.out_sr : a.out_sc;
+  for (int u = blockIdx.x * kThreads + threadIdx.x; u < each; u += gridDim.x * kThreads) {
     float s = 0;
-    for (int k = 0; k < chunks; ++k) s += a.partial[(slot + k) * each + u];
-    static_cast<T*>(a.out)[adapter * a.out_sg + r * a.out_sr + c * a.out_sc] = rounded<T>(s);
+#pragma unroll 4
+    for (int k = 0; k < chunks; ++k) s += a.partial[int64_t(slot + k) * each + u];
+    static_cast<T*>(a.out)[adapter * a.out_sg + u / inner * s_outer + u % inner * s_inner] = rounded<T>(s);
   }
-}
-
-// The bins of the sort: the rows without an adapter come last.
-__global__ void __launch_bounds__(kThreads) lora_bins_kernel(const int32_t* __restrict__ adapter, int rows, int L, int32_t* __restrict__ bins) {
-  const int t = blockIdx.x * kThreads + threadIdx.x;
-  if (t < rows) bins[t] = has_adapter(adapter[t], L) ? adapter[t] : L;
 }
 
 // Sorted operands: q1 and q2 [rows][R] fp32 (either may be null) as [2][R][places] 16-bit halves, times scale; rows by place.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) lora_sorted_kernel(const float* __restrict__ q1, const float* __restrict__ q2,
-                                                               const float* __restrict__ scale, const int32_t* __restrict__ bins,
+                                                               const float* __restrict__ scale, const int32_t* __restrict__ adapter,
                                                                const int32_t* __restrict__ row_token, const int32_t* __restrict__ offs,
                                                                int rows, int R, int L, int places, T* __restrict__ s1, T* __restrict__ s2,
                                                                int32_t* __restrict__ row_at) {
   const int at = blockIdx.x * kThreads + threadIdx.x, r = blockIdx.y;
   if (at >= rows) return;
-  const int row = row_token[at], id = bins[row];
-  if (id >= L) return;
+  const int row = row_token[at], id = adapter[row];
+  if (!has_adapter(id, L)) return;
   const int to = place(offs, id) + at - (id ? offs[id - 1] : 0);
   const float by = scale ? scale[id] : 1.0f;
   if (r == 0) row_at[to] = row;
@@ -494,9 +554,9 @@ __global__ void __launch_bounds__(kThreads) lora_sorted_kernel(const float* __re
 // ---------------------------------------------------------------- host side
 int clamp(int64_t v, int64_t lo, int64_t hi) { return int(v > hi ? (hi < lo ? lo : hi) : v < lo ? lo : v); }
 
-// `want` parts of k elements, each a multiple of 64 and at least 256 long.
-void cut(int64_t k, int64_t want, int32_t& parts, int32_t& each) {
-  parts = clamp(want, 1, k / 256);
+// `want` parts of k elements, each a multiple of 64 and at least `least` long.
+void cut(int64_t k, int64_t want, int64_t least, int32_t& parts, int32_t& each) {
+  parts = clamp(want, 1, k / least);
   each = int32_t(round_up((k + parts - 1) / parts, 64));
   parts = each ? int32_t((k + each - 1) / each) : 1;
 }
@@ -510,19 +570,18 @@ LowPlan plan_low(int64_t rows, int64_t K) {
   LowPlan p;
   p.strip_rows = rows <= kSingleRows ? 1 : 16;
   const int64_t strips = (rows + p.strip_rows - 1) / p.strip_rows;
-  cut(K, strips ? 1024 / strips : 1, p.parts, p.each);
+  if (rows <= kFewRows) cut(K, strips ? 128 / strips : 1, 512, p.parts, p.each);
+  else cut(K, 2048 / strips, 256, p.parts, p.each);
   return p;
 }
 
 struct BasePlan { int32_t parts, each; };
 
-BasePlan plan_base(int64_t rows, int64_t K, int64_t N) {
+// A workgroup for each compute unit.
+BasePlan plan_base(int64_t K, int64_t N, int columns) {
   BasePlan p;
-  const int64_t strips = (N + 127) / 128;
-  int64_t want = strips ? 768 / strips : 1;
-  const int64_t most = K / 8 / (rows > 0 ? rows : 1);      // the parts' sums are written and read: half of W's bytes at most
-  if (want > most) want = most;
-  cut(K, want, p.parts, p.each);
+  const int64_t strips = (N + columns - 1) / columns, cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256;
+  cut(K, strips ? (cus + strips / 2) / strips : 1, 512, p.parts, p.each);
   return p;
 }
 
@@ -537,6 +596,13 @@ int strip_columns(int lay) { return lay == GMM_W_COLS ? 64 : 128; }
 
 int layout_of(const Matrices& m, int64_t K, int64_t N, bool whole) { return gmm::layout_of(m.at, m.sg, m.sk, m.sn, K, multiple8(N), whole); }
 
+// B's layout: nothing is asked of the rank where it is contiguous along its columns.
+int layout_of_b(const Matrices& b, int64_t R, int64_t N) {
+  if (!aligned16(b.at) || !multiple8(b.sg)) return GMM_W_ANY;
+  if (b.sn == 1 && multiple8(b.sk) && multiple8(N)) return GMM_W_ROWS;
+  return b.sk == 1 && multiple8(b.sn) && multiple8(R) ? GMM_W_COLS : GMM_W_ANY;
+}
+
 bool set(Matrices& m, const void* at, int64_t sg, int64_t sk, int64_t sn, int64_t K, int64_t N) {
   if (sg < 0 || sk < 0 || sn < 0) return false;
   m.at = at; m.sg = sg;
@@ -547,7 +613,7 @@ bool set(Matrices& m, const void* at, int64_t sg, int64_t sk, int64_t sn, int64_
 }
 
 int check_sizes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int32_t dtype) {
-  constexpr int64_t most = (int64_t(1) << 30);
+  constexpr int64_t most = (int64_t(1) << 30) / kMaxRank * 16;
   if (rows < 0 || K < 0 || N < 0 || R < 1 || L < 0 || rows >= most || K >= most || N >= most || R > kMaxRank || L > kMaxAdapters) return GMM_ERR_BAD_ARGUMENT;
   return dtype == GMM_DT_BF16 || dtype == GMM_DT_F16 ? GMM_OK : GMM_ERR_UNSUPPORTED;
 }
@@ -556,29 +622,35 @@ bool x_fits(int64_t x_ld, int64_t rows, int64_t K) {
   return rows <= 1 || (x_ld >= K && x_ld <= ((int64_t(1) << 30) - 64 - K) / (rows < kFewRows ? rows : kFewRows));
 }
 
-void set_low(LoraArgs& a, int lay) {
+void set_low(LoraArgs& a, int columns) {
   const LowPlan lp = plan_low(a.rows, a.K);
   a.strip_rows = lp.strip_rows; a.low_parts = lp.parts; a.low_k = lp.each;
-  a.low_tiles = (a.R + strip_columns(lay) - 1) / strip_columns(lay);
+  a.low_tiles = (a.R + columns - 1) / columns;
   a.low_groups = (a.rows + a.strip_rows - 1) / a.strip_rows * a.low_tiles * a.low_parts;
 }
 
 template <typename T>
-int launch_few(LoraArgs a, int lay_w, int lay_a, int lay_b, hipStream_t stream) {
-  set_low(a, lay_a);
-  const BasePlan bp = plan_base(a.rows, a.K, a.N);
+int launch_few(LoraArgs a, bool whole, int lay_b, hipStream_t stream) {
+  int lay_w = layout_of(a.w, a.K, a.N, whole), lay_a = layout_of(a.a, a.K, 8, whole);
+  if (lay_w == GMM_W_ANY || lay_a != GMM_W_COLS) lay_a = GMM_W_ANY;
+  set_low(a, 16);
+  const BasePlan bp = plan_base(a.K, a.N, strip_columns(lay_w));
   a.base_parts = bp.parts; a.base_k = bp.each;
   a.base_tiles = (a.N + strip_columns(lay_w) - 1) / strip_columns(lay_w);
   if (a.L == 0) a.low_groups = 0;
-  const dim3 grid(unsigned(a.low_groups + a.base_tiles * a.base_parts)), block(kThreads);
-  by_layout(lay_w, [&](auto w) {
-    by_layout(lay_a, [&](auto l) {
-      constexpr int W = decltype(w)::value, A = decltype(l)::value;
-      if (a.rows <= 16) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 1>), grid, block, 0, stream, a);
-      else if (a.rows <= 32) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 2>), grid, block, 0, stream, a);
-      else hipLaunchKernelGGL((lora_few_kernel<T, W, A, 4>), grid, block, 0, stream, a);
-    });
-  });
+  const dim3 grid(unsigned(a.low_groups + a.base_tiles * a.base_parts));
+  const auto launch = [&](auto w, auto l) {
+    constexpr int W = decltype(w)::value, A = decltype(l)::value;
+    if (a.rows <= 16) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 1>), grid, dim3(64 * few_waves(1)), 0, stream, a);
+    else if (a.rows <= 32) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 2>), grid, dim3(64 * few_waves(2)), 0, stream, a);
+    else hipLaunchKernelGGL((lora_few_kernel<T, W, A, 4>), grid, dim3(64 * few_waves(4)), 0, stream, a);
+  };
+  constexpr std::integral_constant<int, GMM_W_ROWS> rows{};
+  constexpr std::integral_constant<int, GMM_W_COLS> cols{};
+  constexpr std::integral_constant<int, GMM_W_ANY> any{};
+  if (lay_w == GMM_W_ROWS) lay_a == GMM_W_COLS ? launch(rows, cols) : launch(rows, any);
+  else if (lay_w == GMM_W_COLS) lay_a == GMM_W_COLS ? launch(cols, cols) : launch(cols, any);
+  else launch(any, any);
   by_layout(lay_b, [&](auto l) {
     constexpr int B = decltype(l)::value, W = B == GMM_W_ROWS ? 8 : 1;
     hipLaunchKernelGGL((lora_finish_kernel<T, B>), dim3(unsigned((a.N + 64 * W - 1) / (64 * W)), unsigned(a.rows)), dim3(64), 0, stream, a);
@@ -586,78 +658,107 @@ int launch_few(LoraArgs a, int lay_w, int lay_a, int lay_b, hipStream_t stream) 
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
+// Columns of a lane: as few as hold the rank, as many as lie side by side and aligned.
 template <typename T>
-int launch_low(LoraArgs& a, int lay_a, hipStream_t stream) {
-  set_low(a, lay_a);
-  by_layout(lay_a, [&](auto l) {
-    hipLaunchKernelGGL((lora_low_kernel<T, decltype(l)::value>), dim3(unsigned(a.low_groups)), dim3(kThreads), 0, stream, a);
-  });
+int launch_low(LoraArgs& a, bool whole, hipStream_t stream) {
+  const bool cols = layout_of(a.a, a.K, 8, whole) == GMM_W_COLS;
+  int fr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : a.R <= 64 || cols ? 4 : 8;
+  if (!cols) {
+    const int64_t all = a.R | a.a.sk | a.a.sg | int64_t(reinterpret_cast<uintptr_t>(a.a.at) / 2);
+    while (fr > 1 && (a.a.sn != 1 || !whole || !multiple8(a.K) || all % fr)) fr /= 2;
+  }
+  set_low(a, 16 * fr);
+  const dim3 grid(unsigned(a.low_groups)), block(kThreads);
+  const bool edge = !whole || !multiple8(a.K);     // x has no alignment
+  if (cols && fr == 1) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_COLS, 1, false>), grid, block, 0, stream, a);
+  else if (cols && fr == 2) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_COLS, 2, false>), grid, block, 0, stream, a);
+  else if (cols) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_COLS, 4, false>), grid, block, 0, stream, a);
+  else if (fr == 8) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ROWS, 8, false>), grid, block, 0, stream, a);
+  else if (fr == 4) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ROWS, 4, false>), grid, block, 0, stream, a);
+  else if (fr == 2) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ROWS, 2, false>), grid, block, 0, stream, a);
+  else if (edge) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ANY, 1, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ANY, 1, false>), grid, block, 0, stream, a);
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
 template <typename T>
-int launch_add(LoraArgs a, int lay_a, int lay_b, hipStream_t stream) {
-  const int rc = launch_low<T>(a, lay_a, stream);
-  if (rc != GMM_OK) return rc;
+int launch_add(LoraArgs a, bool whole, hipStream_t stream) {
+  const int rc = launch_low<T>(a, whole, stream);
+  if (rc != GMM_OK || (a.N == 0 && !a.low_out)) return rc;
+  const int lay = layout_of_b(a.b, a.R, a.N);
+  if (lay == GMM_W_ANY) {
+    const dim3 grid(unsigned((a.rows + kAnyRows - 1) / kAnyRows), unsigned(a.N ? (a.N + kThreads - 1) / kThreads : 1));
+    hipLaunchKernelGGL((lora_add_any_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+  }
   const int wide = aligned16(a.out) && multiple8(a.out_ld) && multiple8(a.N);
-  by_layout(lay_b, [&](auto l) {
-    constexpr int B = decltype(l)::value;
-    const int pitch = int(round_up(a.R, B == GMM_W_COLS ? 64 : 32)) + 8;      // 16 bytes more: rows begin in other banks
-    const int columns = kAddStrips * strip_columns(B);
-    const dim3 grid(unsigned((a.rows + kAddRows - 1) / kAddRows), unsigned(a.N ? (a.N + columns - 1) / columns : 1));
-    hipLaunchKernelGGL((lora_add_kernel<T, B>), grid, dim3(kThreads), 2 * kAddRows * pitch * 2, stream, a, wide, pitch);
-  });
+  const int pitch = int(round_up(a.R, 32)) + 8;      // 16 bytes more: rows begin in other banks
+  const dim3 grid(unsigned((a.rows + kAddRows - 1) / kAddRows), unsigned(a.N ? (a.N + 128 * kAddStrips - 1) / (128 * kAddStrips) : 1));
+  const int lds = 2 * kAddRows * pitch * 2;
+  if (lay == GMM_W_ROWS) hipLaunchKernelGGL((lora_add_kernel<T, GMM_W_ROWS>), grid, dim3(kThreads), lds, stream, a, wide, pitch);
+  else hipLaunchKernelGGL((lora_add_kernel<T, GMM_W_COLS>), grid, dim3(kThreads), lds, stream, a, wide, pitch);
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
 // Where the operands of gmm_lora_grad lie in its workspace.
 struct GradPlan {
-  int64_t table, places, bins_at, offs_at, token_at, rows_at, table_at, row_at, q_at[2], partial_at, bytes;
+  int64_t places, offs_at, token_at, rows_at, table_at, row_at, q_at[2], partial_at[2], bytes;
   int32_t chunk;
 };
 
 bool plan_grad(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, GradPlan& p) {
-  p.table = gmm_moe_route_workspace_bytes(rows, L + 1, 1);
-  if (p.table < 0) return false;
-  // chunks: as long as gives every compute unit some strips of 128 columns, and the partial sums some 16 chunks of all rows at most
-  const int64_t widest = K > N ? K : N;
-  p.chunk = clamp(round_up(rows / 32, 128), 512, kMaxChunk);
+  const int64_t table = gmm_moe_route_workspace_bytes(rows, L + 1, 1);
+  if (table < 0) return false;
+  // chunks: as long as leaves some workgroups, one for a chunk and 128 columns, to a compute unit; the partial sums of at most 32 chunks
+  // of all rows
+  const int64_t tiles = (K + 127) / 128 + (N + 127) / 128;
+  p.chunk = clamp(round_up(rows * tiles / 1024 > rows / 32 ? rows * tiles / 1024 : rows / 32, 128), 256, kMaxChunk);
   p.places = round_up(rows, 8) + 8 * (L + 1);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) { const int64_t here = at; at = round_up(at + bytes, 256); return here; };
-  p.bins_at = take(rows * 4);
   p.offs_at = take((L + 1) * 4);
   p.token_at = take(rows * 4);
   p.rows_at = take(rows * 4);
-  p.table_at = take(p.table);
+  p.table_at = take(table);
   p.row_at = take(p.places * 4);
   for (int i = 0; i < 2; ++i) p.q_at[i] = take(2 * R * p.places * 2);
-  p.partial_at = take(2 * (rows / p.chunk) * R * widest * 4);      // adapters of several chunks: fewer than two per chunk of all rows
+  for (int i = 0; i < 2; ++i)      // adapters of several chunks have fewer than two for each chunk of all rows
+    p.partial_at[i] = take(2 * (rows / p.chunk) * R * (i ? N : K) * 4);
   p.bytes = at;
-  return 2 * R * p.places * 2 < (int64_t(1) << 31);
+  return 2 * R * p.places * 2 < (int64_t(1) << 31) && R * K < (int64_t(1) << 30) && R * N < (int64_t(1) << 30);
+}
+
+void set_grad(GradOf& g, const void* p, int64_t p_ld, const void* q, void* out, float* partial, int64_t C, int64_t R, int64_t sg, int64_t sr,
+              int64_t sc) {
+  g.p = p; g.q = q; g.out = out; g.partial = partial; g.p_ld = p_ld;
+  g.out_sg = sg; g.out_sr = sr; g.out_sc = sc;
+  g.C = int32_t(C);
+  g.tiles = out ? int32_t((C + 127) / 128) : 0;
+  g.whole = aligned16(p) && multiple8(p_ld) && multiple8(C);
+  const bool four = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && R % 4 == 0 && sg % 4 == 0 && sc % 4 == 0;   // four of R in 8 bytes
+  g.r_first = sr != 1 || R == 1 ? 0 : four ? 2 : 1;
 }
 
 template <typename T>
-int launch_grad(GradArgs g, int64_t rows, hipStream_t stream) {
-  if (g.C == 0) return GMM_OK;
-  const bool whole = aligned16(g.p) && multiple8(g.p_ld) && multiple8(g.C);
-  g.tiles = (g.C + 127) / 128;
-  const int64_t chunks = rows / g.chunk + (rows < g.L ? rows : g.L);
-  const auto launch = [&](auto lay, auto mf) {
-    constexpr int LAY = decltype(lay)::value, MF = decltype(mf)::value;
-    if (chunks)
-      hipLaunchKernelGGL((lora_grad_kernel<T, LAY, MF>), dim3(unsigned(chunks * g.tiles), unsigned((g.R + 16 * MF - 1) / (16 * MF))),
-                         dim3(kThreads), 0, stream, g);
+int launch_grad(GradArgs& g, int64_t rows, hipStream_t stream) {
+  const int64_t chunks = rows / g.chunk + g.L;
+  g.groups0 = int32_t(chunks * g.of[0].tiles);
+  const int64_t groups = g.groups0 + chunks * g.of[1].tiles;
+  if (groups == 0) return GMM_OK;
+  const auto launch = [&](auto mf) {
+    constexpr int MF = decltype(mf)::value;
+    hipLaunchKernelGGL((lora_grad_kernel<T, MF>), dim3(unsigned(groups), unsigned((g.R + 16 * MF - 1) / (16 * MF))), dim3(kThreads), 0, stream, g);
   };
-  const auto rank = [&](auto lay) {
-    if (g.R <= 16) launch(lay, std::integral_constant<int, 1>{});
-    else if (g.R <= 32) launch(lay, std::integral_constant<int, 2>{});
-    else launch(lay, std::integral_constant<int, 4>{});
-  };
-  if (whole) rank(std::integral_constant<int, GMM_W_ROWS>{});
-  else rank(std::integral_constant<int, GMM_W_ANY>{});
-  const int64_t blocks = (int64_t(g.R) * g.C + 4 * kThreads - 1) / (4 * kThreads);
-  hipLaunchKernelGGL((lora_grad_sum_kernel<T>), dim3(unsigned(blocks < 1024 ? blocks : 1024), unsigned(g.L)), dim3(kThreads), 0, stream, g);
+  if (g.R <= 16) launch(std::integral_constant<int, 1>{});
+  else if (g.R <= 32) launch(std::integral_constant<int, 2>{});
+  else launch(std::integral_constant<int, 4>{});
+  if (rows > g.chunk) {      // an adapter may have several chunks
+    if (!g.of[0].tiles) g.of[0] = g.of[1];
+    const int64_t widest = g.of[1].tiles && g.of[1].C > g.of[0].C ? g.of[1].C : g.of[0].C;
+    const int64_t blocks = (int64_t(g.R) * widest + 4 * kThreads - 1) / (4 * kThreads);
+    const bool both = g.of[1].tiles && g.of[0].out != g.of[1].out;
+    hipLaunchKernelGGL((lora_grad_sum_kernel<T>), dim3(unsigned(blocks < 256 ? blocks : 256), unsigned(g.L), both ? 2 : 1), dim3(kThreads), 0, stream, g);
+  }
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
@@ -668,7 +769,7 @@ extern "C" {
 int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R) {
   if (check_sizes(rows, K, N, R, 0, GMM_DT_BF16) != GMM_OK) return -1;
   int64_t bytes = round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256);
-  if (rows <= kFewRows) bytes += int64_t(plan_base(rows, K, N).parts) * rows * N * 4;
+  if (rows <= kFewRows) bytes += int64_t(plan_base(K, N, 128).parts) * rows * N * 4;     // the layout with the more parts
   return bytes;
 }
 
@@ -691,12 +792,10 @@ int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, 
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
   const bool whole = aligned16(x) && multiple8(g.x_ld);
-  const int lay_w = layout_of(g.w, K, N, whole), lay_a = layout_of(g.a, K, R, whole);
-  const int lay_b = layout_of(g.b, R, N, true);
-  const bool wide = aligned16(out) && multiple8(g.out_ld);       // eight columns of the result at a time
+  int lay_b = layout_of_b(g.b, R, N);
+  if (lay_b == GMM_W_ROWS && !(aligned16(out) && multiple8(g.out_ld))) lay_b = GMM_W_ANY;       // eight columns of the result at a time
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == GMM_DT_BF16) return launch_few<Bf16>(g, lay_w, lay_a, lay_b == GMM_W_ROWS && !wide ? GMM_W_ANY : lay_b, s);
-  return launch_few<F16>(g, lay_w, lay_a, lay_b == GMM_W_ROWS && !wide ? GMM_W_ANY : lay_b, s);
+  return dtype == GMM_DT_BF16 ? launch_few<Bf16>(g, whole, lay_b, s) : launch_few<F16>(g, whole, lay_b, s);
 }
 
 int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, void* out, float* low,
@@ -714,9 +813,9 @@ int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* ada
   g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low; g.low = static_cast<float*>(workspace);
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
-  const int lay_a = layout_of(g.a, K, R, aligned16(x) && multiple8(g.x_ld)), lay_b = layout_of(g.b, R, N, true);
+  const bool whole = aligned16(x) && multiple8(g.x_ld);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GMM_DT_BF16 ? launch_add<Bf16>(g, lay_a, lay_b, s) : launch_add<F16>(g, lay_a, lay_b, s);
+  return dtype == GMM_DT_BF16 ? launch_add<Bf16>(g, whole, s) : launch_add<F16>(g, whole, s);
 }
 
 int64_t gmm_lora_grad_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L) {
@@ -739,32 +838,20 @@ int gmm_lora_grad(const void* x, const void* dy, const float* low, const float* 
   char* const ws = static_cast<char*>(workspace);
   const auto ints = [&](int64_t at) { return reinterpret_cast<int32_t*>(ws + at); };
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = unsigned((rows + kThreads - 1) / kThreads);
-  if (rows) hipLaunchKernelGGL(lora_bins_kernel, dim3(blocks), dim3(kThreads), 0, s, adapter, int(rows), int(L), ints(p.bins_at));
-  const int rc = gmm_sort_slots(ints(p.bins_at), rows, L + 1, ints(p.offs_at), ints(p.token_at), ints(p.rows_at), ws + p.table_at, s);
+  const int rc = gmm_sort_slots(adapter, rows, L + 1, ints(p.offs_at), ints(p.token_at), ints(p.rows_at), ws + p.table_at, s);
   if (rc != GMM_OK) return rc;
   GradArgs g{};
-  g.row_at = ints(p.row_at); g.offs = ints(p.offs_at); g.partial = reinterpret_cast<float*>(ws + p.partial_at);
+  g.row_at = ints(p.row_at); g.offs = ints(p.offs_at);
   g.places = int(p.places); g.R = int(R); g.L = int(L); g.chunk = p.chunk;
+  set_grad(g.of[0], x, x_stride, ws + p.q_at[0], da, reinterpret_cast<float*>(ws + p.partial_at[0]), K, R, da_stride_l, da_stride_r, da_stride_k);
+  set_grad(g.of[1], dy, dy_stride, ws + p.q_at[1], db, reinterpret_cast<float*>(ws + p.partial_at[1]), N, R, db_stride_l, db_stride_r, db_stride_n);
   const auto both = [&](auto zero) {
     using T = decltype(zero);
-    T* const qa = reinterpret_cast<T*>(ws + p.q_at[0]);
-    T* const qb = reinterpret_cast<T*>(ws + p.q_at[1]);
     if (rows)
-      hipLaunchKernelGGL((lora_sorted_kernel<T>), dim3(blocks, unsigned(R)), dim3(kThreads), 0, s, da ? u : nullptr, db ? low : nullptr, scale,
-                         ints(p.bins_at), ints(p.token_at), ints(p.offs_at), int(rows), int(R), int(L), int(p.places), qa, qb, ints(p.row_at));
-    if (da) {
-      g.p = x; g.q = qa; g.out = da; g.p_ld = x_stride; g.C = int(K);
-      g.out_sg = da_stride_l; g.out_sr = da_stride_r; g.out_sc = da_stride_k;
-      const int rc = launch_grad<T>(g, rows, s);
-      if (rc != GMM_OK) return rc;
-    }
-    if (db) {
-      g.p = dy; g.q = qb; g.out = db; g.p_ld = dy_stride; g.C = int(N);
-      g.out_sg = db_stride_l; g.out_sr = db_stride_r; g.out_sc = db_stride_n;
-      return launch_grad<T>(g, rows, s);
-    }
-    return hipGetLastError() == hipSuccess ? int(GMM_OK) : int(GMM_ERR_LAUNCH);
+      hipLaunchKernelGGL((lora_sorted_kernel<T>), dim3(unsigned((rows + kThreads - 1) / kThreads), unsigned(R)), dim3(kThreads), 0, s, da ? u : nullptr,
+                         db ? low : nullptr, scale, adapter, ints(p.token_at), ints(p.offs_at), int(rows), int(R), int(L), int(p.places),
+                         reinterpret_cast<T*>(ws + p.q_at[0]), reinterpret_cast<T*>(ws + p.q_at[1]), ints(p.row_at));
+    return launch_grad<T>(g, rows, s);
   };
   return dtype == GMM_DT_BF16 ? both(Bf16{}) : both(F16{});
 }

@@ -170,6 +170,10 @@ __global__ void __launch_bounds__(256) moe_topk_kernel(const T* __restrict__ log
   }
 }
 
+// The bin that a slot is sorted into.  The routing's experts are all below E; of a caller's own numbers (gmm_sort_slots) those outside
+// share the last bin.
+__device__ __forceinline__ int slot_bin(int32_t expert, int E) { return int(min(uint32_t(expert), uint32_t(E - 1))); }
+
 // ---------------------------------------------------------------- routing of many slots 1/3: per-workgroup histograms
 // Workgroup b counts the experts of slots [b * spb, (b + 1) * spb) into row b of the table.
 __global__ void __launch_bounds__(256) moe_hist_kernel(const int32_t* __restrict__ slot_expert, int slots, int spb, int E,
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(256) moe_hist_kernel(const int32_t* __restrict
   for (int e = threadIdx.x; e < E; e += 256) hist[e] = 0;
   __syncthreads();
   const int s0 = blockIdx.x * spb, s1 = min(slots, s0 + spb);
-  for (int s = s0 + threadIdx.x; s < s1; s += 256) atomicAdd(&hist[slot_expert[s]], 1);
+  for (int s = s0 + threadIdx.x; s < s1; s += 256) atomicAdd(&hist[slot_bin(slot_expert[s], E)], 1);
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += 256) table[int64_t(blockIdx.x) * E + e] = hist[e];
 }
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(64) moe_scatter_kernel(const int32_t* __restri
   for (int c4 = s0; c4 < s1; c4 += 256) {
     int ev[4];   // four chunks' loads in flight at once: each is a trip to L2 or further
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ev[i] = c4 + 64 * i + lane < s1 ? slot_expert[c4 + 64 * i + lane] : -1;
+    for (int i = 0; i < 4; ++i) ev[i] = c4 + 64 * i + lane < s1 ? slot_bin(slot_expert[c4 + 64 * i + lane], E) : -1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int s = c4 + 64 * i + lane, e = ev[i];
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(kPlaceBlock) moe_place_kernel(const int32_t* _
   __shared__ int32_t sums[2 * kMaxExperts];
   __shared__ int32_t part[kPlaceWaves];
   const int tid = threadIdx.x, own = blockIdx.x, blocks = gridDim.x;
-  const int expert = own * kPlaceBlock + tid < slots ? slot_expert[own * kPlaceBlock + tid] : -1;
+  const int expert = own * kPlaceBlock + tid < slots ? slot_bin(slot_expert[own * kPlaceBlock + tid], E) : -1;
   const int copy_bits = place_copy_bits(E), copy = tid & ((1 << copy_bits) - 1);
   int32_t* const count = words + kPlaceWaves * E;
   for (int i = tid; i < (kPlaceWaves + (blocks > 1 ? 2 << copy_bits : 0)) * E / 4; i += kPlaceBlock)
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(kPlaceBlock) moe_place_kernel(const int32_t* _
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int s = (b0 + i) * kPlaceBlock + tid;
-        e[i] = b0 + i != own && s < slots ? slot_expert[s] : -1;
+        e[i] = b0 + i != own && s < slots ? slot_bin(slot_expert[s], E) : -1;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)

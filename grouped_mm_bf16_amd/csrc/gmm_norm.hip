@@ -143,10 +143,9 @@ __global__ void __launch_bounds__(kBlock<LANES>) norm_forward_kernel(const NormA
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int c = (p * LANES + lane) * N;
-      Pack<T, N> o;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o.set(i, x[p][i] * rstd * w[p][i] + b[p][i]);
-      if (c < a.width) *reinterpret_cast<Pack<T, N>*>(y + c) = o;
+      for (int i = 0; i < N; ++i) x[p][i] = x[p][i] * rstd * w[p][i] + b[p][i];
+      if (c < a.width) *reinterpret_cast<Pack<T, N>*>(y + c) = Pack<T, N>::of(x[p]);
     }
   }
 }
@@ -217,10 +216,9 @@ __global__ void __launch_bounds__(kBlock<LANES>) norm_backward_kernel(const Norm
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int c = (p * LANES + lane) * N;
-      Pack<T, N> o;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o.set(i, rstd * (dy[p][i] * w[p][i] - c1 - z[p][i] * c2));
-      if (c < a.width) *reinterpret_cast<Pack<T, N>*>(dx + c) = o;
+      for (int i = 0; i < N; ++i) dy[p][i] = rstd * (dy[p][i] * w[p][i] - c1 - z[p][i] * c2);
+      if (c < a.width) *reinterpret_cast<Pack<T, N>*>(dx + c) = Pack<T, N>::of(dy[p]);
     }
   }
   if (!a.partial) return;

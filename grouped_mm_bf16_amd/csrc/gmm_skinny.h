@@ -46,13 +46,21 @@ __device__ __forceinline__ void split(float f, T& high, T& low) {
   low = rounded<T>(__builtin_isfinite(back) ? f - back : 0.0f);
 }
 
-// One strip of columns of one product, by one wave.  MF: sixteens of rows.  NA: planes of A (2: A = high + low).  ST: steps in flight.
-template <typename T, int LAY, int MF, int NA, int ST>
+// One strip of columns of one product, by one wave.
+//   FR: columns of a lane, which is products of 16 columns (GMM_W_ROWS: 2, 4, 8; GMM_W_COLS: any; GMM_W_ANY: 1, 8).
+//   KH: 32s of k in a step (2 for GMM_W_COLS where k is long: whole cache lines).
+//   AE: rows of A are read element by element (no alignment).
+//   MF: sixteens of rows.  NA: planes of A (2: A = high + low).  ST: steps in flight.
+template <typename T, int LAY, int FR_, int KH, bool AE, int MF, int NA, int ST>
 struct Skinny {
-  static constexpr int FR = LAY == GMM_W_COLS ? 4 : 8;        // columns of a lane: products of 16 columns
-  static constexpr int KS = LAY == GMM_W_COLS ? 64 : 32;      // k of a step
-  static constexpr int KG = KS / 4;                           // of them a lane's
+  static constexpr int FR = FR_;
+  static constexpr int KS = 32 * KH;          // k of a step
+  static constexpr int KG = KS / 4;           // of them a lane's
   static constexpr int COLUMNS = 16 * FR;
+  static constexpr int WORDS = LAY == GMM_W_COLS ? 4 * FR * KH : FR == 1 ? 4 : 4 * FR;   // of W in a step, of a lane
+  static_assert(LAY == GMM_W_COLS || KH == 1, "");
+  static_assert(LAY != GMM_W_ANY || FR == 1 || FR == 8, "");
+  static_assert(LAY != GMM_W_ROWS || FR == 2 || FR == 4 || FR == 8, "");
 
   __amdgpu_buffer_rsrc_t w_buf, a_buf;
   uint32_t w_at;          // byte offset of the lane's first column
@@ -60,18 +68,18 @@ struct Skinny {
   int columns;            // the lane's columns that exist (GMM_W_ROWS: all or none)
   uint32_t a_at[MF];      // byte offset of the lane's rows of A, kNowhere: no such row
   uint32_t a_plane;       // bytes from the high to the low plane
-  int rows16;             // sixteens of rows that hold any
 
-  struct Step { u32x4 w[8]; u32x4 a[MF][NA][KS / 32]; };
+  struct Step { uint32_t w[WORDS]; u32x4 a[MF][NA][KH]; };
 
-  __device__ __forceinline__ uint32_t element(__amdgpu_buffer_rsrc_t buf, uint32_t at) const {
+  static __device__ __forceinline__ uint32_t element(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
     return uint32_t(uint16_t(__builtin_amdgcn_raw_buffer_load_b16(buf, int(at), 0, 0)));
   }
 
   // Loads k .. k + KS - 1, of which those before `end` exist.
+  template <int M>
   __device__ __forceinline__ void load(Step& s, int k, int end, int g) const {
     load_w(s, k, end, g);
-    load_a(s, k, end, g);
+    load_a<M>(s, k, end, g);
   }
 
   __device__ __forceinline__ void load_w(Step& s, int k, int end, int g) const {
@@ -79,16 +87,39 @@ struct Skinny {
     if constexpr (LAY == GMM_W_ROWS) {
       const uint32_t at = w_at + uint32_t(kl) * w_step_k;
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        s.w[r] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(columns && kl + r < end ? at + r * w_step_k : kNowhere), 0, kStream);
+      for (int r = 0; r < 8; ++r) {
+        const int from = int(columns && kl + r < end ? at + r * w_step_k : kNowhere);
+        if constexpr (FR == 8) {
+          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(w_buf, from, 0, kStream);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s.w[4 * r + i] = v[i];
+        } else if constexpr (FR == 4) {
+          const auto v = __builtin_amdgcn_raw_buffer_load_b64(w_buf, from, 0, 0);
+          s.w[2 * r] = v[0];
+          s.w[2 * r + 1] = v[1];
+        } else {
+          s.w[r] = __builtin_amdgcn_raw_buffer_load_b32(w_buf, from, 0, 0);
+        }
+      }
     } else if constexpr (LAY == GMM_W_COLS) {
       const uint32_t at = w_at + uint32_t(kl) * 2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          s.w[2 * i + h] = __builtin_amdgcn_raw_buffer_load_b128(
+        for (int h = 0; h < KH; ++h) {
+          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(
               w_buf, int(i < columns && kl + 8 * h < end ? at + i * w_step_n + 16 * h : kNowhere), 0, kStream);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) s.w[4 * (KH * i + h) + q] = v[q];
+        }
+    } else if constexpr (FR == 1) {
+      const uint32_t at = w_at + uint32_t(kl) * w_step_k;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t lo = element(w_buf, columns && kl + 2 * q < end ? at + 2 * q * w_step_k : kNowhere);
+        const uint32_t hi = element(w_buf, columns && kl + 2 * q + 1 < end ? at + (2 * q + 1) * w_step_k : kNowhere);
+        s.w[q] = lo | hi << 16;
+      }
     } else {
 #pragma unroll
       for (int r = 0; r < 8; ++r)
@@ -98,26 +129,28 @@ struct Skinny {
           const bool in = kl + r < end;
           const uint32_t lo = element(w_buf, in && 2 * q < columns ? at : kNowhere);
           const uint32_t hi = element(w_buf, in && 2 * q + 1 < columns ? at + w_step_n : kNowhere);
-          s.w[r][q] = lo | hi << 16;
+          s.w[4 * r + q] = lo | hi << 16;
         }
     }
   }
 
+  // The first M of the sixteens of rows.
+  template <int M>
   __device__ __forceinline__ void load_a(Step& s, int k, int end, int g) const {
     const int kl = k + KG * g;
 #pragma unroll
-    for (int m = 0; m < MF; ++m) {
-      if (m >= rows16) break;
+    for (int m = 0; m < M; ++m) {
 #pragma unroll
       for (int p = 0; p < NA; ++p)
 #pragma unroll
-        for (int h = 0; h < KS / 32; ++h) {
+        for (int h = 0; h < KH; ++h) {
           const uint32_t at = a_at[m] + p * a_plane + uint32_t(kl + 8 * h) * 2;
-          if constexpr (LAY == GMM_W_ANY) {
+          if constexpr (AE) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const uint32_t lo = element(a_buf, a_at[m] != kNowhere && kl + 2 * q < end ? at + 4 * q : kNowhere);
-              const uint32_t hi = element(a_buf, a_at[m] != kNowhere && kl + 2 * q + 1 < end ? at + 4 * q + 2 : kNowhere);
+              const int kq = kl + 8 * h + 2 * q;
+              const uint32_t lo = element(a_buf, a_at[m] != kNowhere && kq < end ? at + 4 * q : kNowhere);
+              const uint32_t hi = element(a_buf, a_at[m] != kNowhere && kq + 1 < end ? at + 4 * q + 2 : kNowhere);
               s.a[m][p][h][q] = lo | hi << 16;
             }
           } else {
@@ -127,48 +160,62 @@ struct Skinny {
     }
   }
 
+  // Second operand of product i, half h of the step.
+  static __device__ __forceinline__ u32x4 operand(const Step& s, int i, int h) {
+    u32x4 b;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if constexpr (LAY == GMM_W_COLS) b[q] = s.w[4 * (KH * i + h) + q];
+      else if constexpr (FR == 1) b[q] = s.w[q];
+      else b[q] = __builtin_amdgcn_perm(s.w[(2 * q + 1) * (FR / 2) + i / 2], s.w[2 * q * (FR / 2) + i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+    }
+    return b;
+  }
+
+  template <int M>
   __device__ __forceinline__ void multiply(const Step& s, f32x4 (&acc)[MF][FR]) const {
-    if constexpr (LAY == GMM_W_COLS) {
 #pragma unroll
-      for (int i = 0; i < FR; ++i)
+    for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int m = 0; m < MF; ++m) {
-          if (m >= rows16) break;
+      for (int h = 0; h < KH; ++h) {
+        const u32x4 b = operand(s, i, h);
 #pragma unroll
-          for (int p = 0; p < NA; ++p)
+        for (int m = 0; m < M; ++m) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) acc[m][i] = mfma(T{}, s.a[m][p][h], s.w[2 * i + h], acc[m][i]);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < FR; ++i) {
-        u32x4 b;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          b[q] = __builtin_amdgcn_perm(s.w[2 * q + 1][i / 2], s.w[2 * q][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int m = 0; m < MF; ++m) {
-          if (m >= rows16) break;
-#pragma unroll
-          for (int p = 0; p < NA; ++p) acc[m][i] = mfma(T{}, s.a[m][p][0], b, acc[m][i]);
+          for (int p = 0; p < NA; ++p) acc[m][i] = mfma(T{}, s.a[m][p][h], b, acc[m][i]);
         }
       }
-    }
   }
 
   // acc += A[:, begin .. end) W[begin .. end).  Steps past the end load nothing: no branch stands between the loads in flight.
-  __device__ __forceinline__ void run(int begin, int end, int g, f32x4 (&acc)[MF][FR]) const {
+  template <int M>
+  __device__ __forceinline__ void steps(int begin, int end, int g, f32x4 (&acc)[MF][FR]) const {
     Step step[ST];
 #pragma unroll
-    for (int u = 0; u < ST; ++u) load(step[u], begin + u * KS, end, g);
+    for (int u = 0; u < ST; ++u) load<M>(step[u], begin + u * KS, end, g);
     for (int k = begin; k < end; k += ST * KS)
 #pragma unroll
       for (int u = 0; u < ST; ++u) {
-        multiply(step[u], acc);
-        load(step[u], k + (ST + u) * KS, end, g);
+        multiply<M>(step[u], acc);
+        load<M>(step[u], k + (ST + u) * KS, end, g);
       }
   }
+
+  // rows: how many there are; sixteens that hold none take no part.
+  __device__ __forceinline__ void run(int rows, int begin, int end, int g, f32x4 (&acc)[MF][FR]) const {
+    if constexpr (MF >= 2) {
+      if (rows <= 16) return steps<1>(begin, end, g, acc);
+    }
+    if constexpr (MF >= 4) {
+      if (rows <= 32) return steps<2>(begin, end, g, acc);
+    }
+    steps<MF>(begin, end, g, acc);
+  }
 };
+
+// A strip of a matrix that is large: all columns of a lane in 16-byte loads, whole cache lines.
+template <typename T, int LAY, int MF, int NA, int ST>
+using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, LAY == GMM_W_COLS ? 2 : 1, LAY == GMM_W_ANY, MF, NA, ST>;
 
 // Range of k of one of WAVES waves: whole steps of KS, dealt evenly.
 template <int KS, int WAVES>
