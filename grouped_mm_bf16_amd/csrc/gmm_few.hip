@@ -58,50 +58,47 @@ __device__ __forceinline__ bool find_expert(const FewArgs& a, int which, int& ex
   return false;
 }
 
-// act[r] = act(x[token of row r] @ w_up[e]).  GLU: a strip is 8 * FR gate columns (lanes j < 8) and their partners (lane j + 8).
+// act[r] = act(x[token of row r] @ w_up[e]).  GLU: a strip is 8 * FR gate columns and their partners.
 template <typename T, int LAY, int MF, bool GLU>
 __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1) few_up_kernel(const FewArgs a) {
-  using S = Strip<T, LAY, MF, 1, 2>;
+  using S = Strip<T, LAY, MF, 1>;
   constexpr int FR = S::FR, OUT = GLU ? 8 * FR : 16 * FR;
-  __shared__ SkinnySums<kWaves, FR> sums;
+  __shared__ SkinnyShared<S, kWaves> shared;
   int expert, row0, rows;
   if (!find_expert(a, blockIdx.x / a.tiles, expert, row0, rows)) return;
   const int tile = blockIdx.x % a.tiles;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   S s;
+  s.lane = lane;
+  s.lds = shared.wave[wave];
   s.w_buf = buffer(static_cast<const T*>(a.w) + expert * a.w_sg, a.w_bytes);
   s.a_buf = buffer(a.x, uint32_t((int64_t(a.tokens - 1) * a.x_ld + a.H) * 2));
-  const int c = tile * OUT + FR * (GLU ? j & 7 : j);     // of the result
-  int at = c;
-  if (GLU && a.kind == GMM_ACT_SWIGLU) at += j < 8 ? 0 : a.inner;
-  if (GLU && a.kind == GMM_ACT_SWIGLU_INTERLEAVED) at = c / 64 * 128 + c % 64 + (j < 8 ? 0 : 64);
-  s.columns = max(0, min(FR, a.inner - c));
-  s.w_at = uint32_t(at) * a.w_sn * 2;
-  s.w_step_k = a.w_sk * 2;
-  s.w_step_n = a.w_sn * 2;
   s.a_plane = 0;
-#pragma unroll
-  for (int m = 0; m < MF; ++m)
-    s.a_at[m] = 16 * m + j < rows ? uint32_t(a.row_token[row0 + 16 * m + j]) * uint32_t(a.x_ld) * 2 : kNowhere;
+  const int c = tile * OUT;     // of the result
+  if constexpr (GLU) {
+    if (a.kind == GMM_ACT_SWIGLU) s.set_columns(c, a.inner - c, a.w_sk, a.w_sn, OUT, a.inner + c);
+    else s.set_columns(c / 64 * 128 + c % 64, a.inner - c, a.w_sk, a.w_sn, OUT, c / 64 * 128 + c % 64 + 64);
+  } else {
+    s.set_columns(c, a.inner - c, a.w_sk, a.w_sn);
+  }
+  s.set_rows([&](int r) { return r < rows ? uint32_t(a.row_token[row0 + r]) * uint32_t(a.x_ld) * 2 : kNowhere; });
   f32x4 acc[MF][FR];
   clear(acc);
-  int from, to;
-  wave_range<S::KS, kWaves>(0, a.H, wave, from, to);
-  s.run(rows, from, to, g, acc);
+  s.template run<kWaves>(rows, 0, a.H, wave, acc);
 
   T* const high = static_cast<T*>(a.act);
   T* const low = high + int64_t(a.slots) * a.act_ld;
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     if (16 * m >= rows) break;
-    if (m) __syncthreads();
-    sums.put(wave, lane, acc[m]);
+    __syncthreads();
+    shared.sums.put(wave, lane, acc[m]);
     __syncthreads();
     for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.inner) continue;
-      const f32x4 h = sums.get(oc % FR, oc / FR, og);
-      const f32x4 partner = GLU ? sums.get(oc % FR, oc / FR + 8, og) : f32x4{1, 1, 1, 1};
+      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
+      const f32x4 partner = GLU ? shared.sums.get(S::product_of(OUT + oc), S::lane_of(OUT + oc), og) : f32x4{1, 1, 1, 1};
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int r = 16 * m + 4 * og + v;
@@ -117,41 +114,36 @@ __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1)
 // y[part][r] = act[r] @ w_down[e], over the part's range of k.
 template <typename T, int LAY, int MF>
 __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1) few_down_kernel(const FewArgs a) {
-  using S = Strip<T, LAY, MF, 2, 2>;
+  using S = Strip<T, LAY, MF, 2>;
   constexpr int FR = S::FR, OUT = 16 * FR;
-  __shared__ SkinnySums<kWaves, FR> sums;
+  __shared__ SkinnyShared<S, kWaves> shared;
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
   int expert, row0, rows;
   if (!find_expert(a, item / a.tiles, expert, row0, rows)) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   S s;
+  s.lane = lane;
+  s.lds = shared.wave[wave];
   s.w_buf = buffer(static_cast<const T*>(a.w) + expert * a.w_sg, a.w_bytes);
   s.a_plane = uint32_t(a.slots) * a.act_ld * 2;
   s.a_buf = buffer(a.act, 2 * s.a_plane);
-  const int c = tile * OUT + FR * j;
-  s.columns = max(0, min(FR, a.H - c));
-  s.w_at = uint32_t(c) * a.w_sn * 2;
-  s.w_step_k = a.w_sk * 2;
-  s.w_step_n = a.w_sn * 2;
-#pragma unroll
-  for (int m = 0; m < MF; ++m) s.a_at[m] = 16 * m + j < rows ? uint32_t(row0 + 16 * m + j) * a.act_ld * 2 : kNowhere;
+  s.set_columns(tile * OUT, a.H - tile * OUT, a.w_sk, a.w_sn);
+  s.set_rows([&](int r) { return r < rows ? uint32_t(row0 + r) * a.act_ld * 2 : kNowhere; });
   f32x4 acc[MF][FR];
   clear(acc);
-  int from, to;
-  wave_range<S::KS, kWaves>(part * a.k_part, min(a.inner, (part + 1) * a.k_part), wave, from, to);
-  s.run(rows, from, to, g, acc);
+  s.template run<kWaves>(rows, part * a.k_part, min(a.inner, (part + 1) * a.k_part), wave, acc);
 
   float* const y = a.y + int64_t(part) * a.slots * a.H;
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     if (16 * m >= rows) break;
-    if (m) __syncthreads();
-    sums.put(wave, lane, acc[m]);
+    __syncthreads();
+    shared.sums.put(wave, lane, acc[m]);
     __syncthreads();
     for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.H) continue;
-      const f32x4 h = sums.get(oc % FR, oc / FR, og);
+      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int r = 16 * m + 4 * og + v;

@@ -43,57 +43,57 @@ struct LoraArgs {
   void* out;
   float* low;              // [low_parts][rows][R]: parts of x @ A
   float* low_out;          // [rows][R]: their sums, null: not wanted
+  void* planes;            // many rows: [2][rows][pitch], null: not wanted
   float* base;             // [base_parts][rows][N]: parts of x @ W
   int64_t x_ld, out_ld;
   int32_t rows, K, N, R, L;
   int32_t strip_rows, low_parts, low_k, low_tiles;   // rows of a strip; parts of K and their length; strips of columns of A
-  int32_t base_parts, base_k, base_tiles, low_groups;
+  int32_t base_parts, base_k, base_tiles, low_groups, pitch, strips;
 };
 
 __device__ __forceinline__ bool has_adapter(int id, int L) { return id >= 0 && id < L; }
 
-template <typename T, typename S>
-__device__ __forceinline__ void set_matrix(S& s, const Matrices& m, int which, int column, int columns) {
-  s.w_buf = buffer(static_cast<const T*>(m.at) + which * m.sg, m.bytes);
-  s.columns = max(0, min(S::FR, columns - column));
-  s.w_at = uint32_t(column) * m.sn * 2;
-  s.w_step_k = m.sk * 2;
-  s.w_step_n = m.sn * 2;
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix(const Matrices& m, int which) {
+  return buffer(static_cast<const T*>(m.at) + which * m.sg, m.bytes);
 }
 
 // low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows; one adapter of theirs after the other.
 template <typename T, int LAY, int FR, bool AE>
-using LowSkinny = Skinny<T, LAY, FR, LAY == GMM_W_COLS ? 2 : 1, AE, 1, 1, FR <= 2 ? 4 : 2>;
+using LowSkinny = Skinny<T, LAY, FR, 1, 1, AE, FR <= 2 ? 4 : 2>;
 
 template <typename T, typename S, int WAVES>
-__device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnySums<WAVES, S::FR>& sums) {
+__device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyShared<S, WAVES>& shared) {
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   const int part = item % a.low_parts, tile = item / a.low_parts % a.low_tiles, row0 = item / a.low_parts / a.low_tiles * a.strip_rows;
   const int rows = min(a.strip_rows, a.rows - row0);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15;
   const int id = j < rows ? a.adapter[row0 + j] : -1;
   uint32_t todo = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
   S s;
+  s.lane = lane;
+  s.lds = shared.wave[wave];
   s.a_buf = buffer(static_cast<const T*>(a.x) + row0 * a.x_ld, uint32_t(((rows - 1) * a.x_ld + a.K) * 2));
   s.a_plane = 0;
-  int from, to;
-  wave_range<S::KS, WAVES>(part * a.low_k, min(a.K, (part + 1) * a.low_k), wave, from, to);
+  s.set_columns(tile * OUT, a.R - tile * OUT, a.a.sk, a.a.sn);
+  const int from = part * a.low_k, to = min(a.K, from + a.low_k);
   float* const low = a.low + (int64_t(part) * a.rows + row0) * a.R;
   while (todo) {
     const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
     const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
     todo &= ~mine;
-    set_matrix<T>(s, a.a, which, tile * OUT + FR * j, a.R);
-    s.a_at[0] = mine >> j & 1 ? uint32_t(j) * uint32_t(a.x_ld) * 2 : kNowhere;
+    s.w_buf = matrix<T>(a.a, which);
+    s.set_rows([&](int r) { return mine >> r & 1 ? uint32_t(r) * uint32_t(a.x_ld) * 2 : kNowhere; });
     f32x4 acc[1][FR];
     clear(acc);
-    s.run(16, from, to, g, acc);
-    sums.put(wave, lane, acc[0]);
+    s.template run<WAVES>(16, from, to, wave, acc);
+    __syncthreads();
+    shared.sums.put(wave, lane, acc[0]);
     __syncthreads();
     for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.R || !(mine >> 4 * og & 15)) continue;
-      const f32x4 h = sums.get(oc % FR, oc / FR, og);
+      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
 #pragma unroll
       for (int v = 0; v < 4; ++v)
         if (mine >> (4 * og + v) & 1) low[(4 * og + v) * a.R + col] = h[v];
@@ -105,47 +105,47 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
 template <typename T, int LAY, int FR, bool AE>
 __global__ void __launch_bounds__(kThreads, FR <= 2 ? 3 : 2) lora_low_kernel(const LoraArgs a) {
   using S = LowSkinny<T, LAY, FR, AE>;
-  __shared__ SkinnySums<kWaves, FR> sums;
-  low_product<T, S, kWaves>(a, blockIdx.x, sums);
+  __shared__ SkinnyShared<S, kWaves> shared;
+  low_product<T, S, kWaves>(a, blockIdx.x, shared);
 }
 
 // A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
 template <typename T, int LAY_W, int LAY_A, int MF>
 __global__ void __launch_bounds__(64 * few_waves(MF)) lora_few_kernel(const LoraArgs a) {
   constexpr int WAVES = few_waves(MF);
-  using S = Strip<T, LAY_W, MF, 1, 2>;
+  using S = Strip<T, LAY_W, MF, 1>;
   using SA = LowSkinny<T, LAY_A, 1, LAY_W == GMM_W_ANY>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   __shared__ union Shared {
-    SkinnySums<WAVES, 1> low;
-    SkinnySums<WAVES, FR> base;
+    SkinnyShared<SA, WAVES> low;
+    SkinnyShared<S, WAVES> base;
     __device__ Shared() {}
   } shared;
   if (int(blockIdx.x) < a.low_groups) return low_product<T, SA, WAVES>(a, blockIdx.x, shared.low);
   const int item = blockIdx.x - a.low_groups, part = item % a.base_parts, tile = item / a.base_parts;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   S s;
-  set_matrix<T>(s, a.w, 0, tile * OUT + FR * j, a.N);
+  s.lane = lane;
+  s.lds = shared.base.wave[wave];
+  s.w_buf = matrix<T>(a.w, 0);
   s.a_buf = buffer(a.x, uint32_t(((a.rows - 1) * a.x_ld + a.K) * 2));
   s.a_plane = 0;
-#pragma unroll
-  for (int m = 0; m < MF; ++m) s.a_at[m] = 16 * m + j < a.rows ? uint32_t(16 * m + j) * uint32_t(a.x_ld) * 2 : kNowhere;
+  s.set_columns(tile * OUT, a.N - tile * OUT, a.w.sk, a.w.sn);
+  s.set_rows([&](int r) { return r < a.rows ? uint32_t(r) * uint32_t(a.x_ld) * 2 : kNowhere; });
   f32x4 acc[MF][FR];
   clear(acc);
-  int from, to;
-  wave_range<S::KS, WAVES>(part * a.base_k, min(a.K, (part + 1) * a.base_k), wave, from, to);
-  s.run(a.rows, from, to, g, acc);
+  s.template run<WAVES>(a.rows, part * a.base_k, min(a.K, (part + 1) * a.base_k), wave, acc);
   float* const base = a.base + int64_t(part) * a.rows * a.N;
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     if (16 * m >= a.rows) break;
-    if (m) __syncthreads();
-    shared.base.put(wave, lane, acc[m]);
+    __syncthreads();
+    shared.base.sums.put(wave, lane, acc[m]);
     __syncthreads();
     for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.N) continue;
-      const f32x4 h = shared.base.get(oc % FR, oc / FR, og);
+      const f32x4 h = shared.base.sums.get(S::product_of(oc), S::lane_of(oc), og);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int r = 16 * m + 4 * og + v;
@@ -232,85 +232,145 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   }
 }
 
-// low of a row and its place in the rank, summed, written out where it is wanted, times scale; zero for a row without an adapter.
-__device__ __forceinline__ float scaled_low(const LoraArgs& a, int row, int r) {
-  const int id = row < a.rows ? a.adapter[row] : -1;
-  if (r >= a.R || !has_adapter(id, a.L)) return 0;
-  const float v = low_sum(a, row, r);
-  if (a.low_out && blockIdx.y == 0) a.low_out[int64_t(row) * a.R + r] = v;
-  return a.scale ? v * a.scale[id] : v;
+// Many rows: the parts of x @ A summed, written out where that is wanted, and times scale as the operand of the second product: two 16-bit
+// values each, [2][rows][pitch], zeros past the rank and in rows without an adapter.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a) {
+  const int64_t u = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int row = int(u / a.pitch), r = int(u % a.pitch);
+  if (row >= a.rows) return;
+  const int id = a.adapter[row];
+  float v = 0;
+  if (r < a.R && has_adapter(id, a.L)) {
+    v = low_sum(a, row, r);
+    if (a.low_out) a.low_out[int64_t(row) * a.R + r] = v;
+    if (a.scale) v *= a.scale[id];
+  }
+  if (a.planes) split(v, static_cast<T*>(a.planes)[u], static_cast<T*>(a.planes)[int64_t(a.rows) * a.pitch + u]);
 }
 
-// Many rows: y[t] += scale * low @ B.  A workgroup takes 64 rows, a wave 16 of them, and kAddStrips strips of 128 columns.  low, as two
-// 16-bit values each, lies in LDS; y is read and written where it is, 16 bytes to a lane where it can be.  16 waves to a compute
-// unit hide its latency.
-constexpr int kAddRows = 64, kAddStrips = 4;
-
-template <typename T, int LAY>
-__global__ void __launch_bounds__(kThreads, 3) lora_add_kernel(const LoraArgs a, int wide_y, int pitch) {
-  using S = Skinny<T, LAY, 8, 1, false, 1, 2, 1>;
-  constexpr int FR = S::FR, OUT = S::COLUMNS, KS = S::KS;
-  extern __shared__ __align__(16) char shared[];     // [2][kAddRows][pitch]
-  T* const planes = reinterpret_cast<T*>(shared);
-  const int row0 = blockIdx.x * kAddRows;
-  for (int u = threadIdx.x; u < kAddRows * pitch; u += kThreads) {
-    const int r = u % pitch;
-    split(scaled_low(a, row0 + u / pitch, r), planes[u], planes[kAddRows * pitch + u]);
-  }
-  __syncthreads();
+// Many rows: y[t] += scale * low @ B.  A wave takes 16 rows and strips of 128 columns, one after the other; y is read and written where
+// it is, 16 bytes to a lane where it can be.  The next strip's y and B are on their way while one is written: of 4 waves and one strip
+// at a time 8192 x 4096 took 65 us, five trips to memory one after the other for each.  NK: steps of 32 of the rank that are held.
+template <typename T, int LAY, int NK, bool WIDE>
+__global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_kernel(const LoraArgs a) {
+  using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, false, 1>;
+  constexpr int FR = S::FR, OUT = S::COLUMNS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int first = row0 + 16 * wave;
+  const int first = (blockIdx.x * kWaves + wave) * 16;
   const int id = first + j < a.rows ? a.adapter[first + j] : -1;
   const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
   if (!with) return;
-  S s;
-  const T* const mine_high = planes + (16 * wave + j) * pitch + 8 * g;
-#pragma unroll 1
-  for (int strip = 0; strip < kAddStrips; ++strip) {
-    const int tile = blockIdx.y * kAddStrips + strip, c = tile * OUT + FR * j;
-    if (tile * OUT >= a.N) break;
-    const int columns = max(0, min(FR, a.N - c));
-    T* const y = static_cast<T*>(a.out) + int64_t(first + 4 * g) * a.out_ld + c;
-    Pack<T, FR> old[4];
+  const T* const high = static_cast<const T*>(a.planes) + int64_t(min(first + j, a.rows - 1)) * a.pitch + 8 * g;
+  const T* const low = high + int64_t(a.rows) * a.pitch;
+  const int tile0 = blockIdx.y * a.strips, tiles = min(a.strips, (a.N + OUT - 1) / OUT - tile0);
+  // y from row `first` on; what is not to be read or written lies nowhere, so that no branch stands around an access
+  const int there = min(16, a.rows - first);
+  const __amdgpu_buffer_rsrc_t y = buffer(static_cast<T*>(a.out) + first * a.out_ld, uint32_t(((there - 1) * a.out_ld + a.N) * 2));
+  const uint32_t y_at = uint32_t(4 * g) * uint32_t(a.out_ld) * 2, y_step = uint32_t(a.out_ld) * 2;
+  const auto load_y = [&](u32x4 (&old)[4], int tile, uint32_t mine) {
+    const int c = (tile0 + tile) * OUT + FR * j;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      if (!(with >> (4 * g + v) & 1)) continue;
-      if (wide_y) {
-        if (columns) old[v] = *reinterpret_cast<const Pack<T, FR>*>(y + v * a.out_ld);
+      const bool in = mine >> (4 * g + v) & 1;
+      const uint32_t at = y_at + v * y_step + uint32_t(c) * 2;
+      if constexpr (WIDE) {
+        old[v] = __builtin_amdgcn_raw_buffer_load_b128(y, int(in && c < a.N ? at : kNowhere), 0, 0);
       } else {
 #pragma unroll
-        for (int i = 0; i < FR; ++i) if (i < columns) old[v].w[i / 2] = i & 1 ? old[v].w[i / 2] | uint32_t(y[v * a.out_ld + i].bits) << 16 : y[v * a.out_ld + i].bits;
-      }
-    }
-#pragma unroll 1
-    for (uint32_t todo = with; todo;) {
-      const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
-      const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
-      todo &= ~mine;
-      set_matrix<T>(s, a.b, which, c, a.N);
-      f32x4 acc[1][FR];
-      clear(acc);
-#pragma unroll 1
-      for (int k = 0; k < a.R; k += KS) {
-        typename S::Step step;
-        s.load_w(step, k, a.R, g);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) step.a[0][p][0] = *reinterpret_cast<const u32x4*>(mine_high + p * kAddRows * pitch + k);
-        s.template multiply<1>(step, acc);
-      }
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        if (!(mine >> (4 * g + v) & 1)) continue;
-        float now[FR];
-#pragma unroll
-        for (int i = 0; i < FR; ++i) now[i] = old[v].get(i) + acc[0][i][v];
-        if (wide_y) {
-          if (columns) *reinterpret_cast<Pack<T, FR>*>(y + v * a.out_ld) = Pack<T, FR>::of(now);
-        } else {
-#pragma unroll
-          for (int i = 0; i < FR; ++i) if (i < columns) y[v * a.out_ld + i] = rounded<T>(now[i]);
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t lo = S::element(y, in && c + 2 * q < a.N ? at + 4 * q : kNowhere);
+          old[v][q] = lo | S::element(y, in && c + 2 * q + 1 < a.N ? at + 4 * q + 2 : kNowhere) << 16;
         }
       }
+    }
+  };
+  const auto store_y = [&](const float (&now)[4][FR], int tile, uint32_t mine) {
+    const int c = (tile0 + tile) * OUT + FR * j;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const bool in = mine >> (4 * g + v) & 1;
+      const uint32_t at = y_at + v * y_step + uint32_t(c) * 2;
+      if constexpr (WIDE) {
+        __builtin_amdgcn_raw_buffer_store_b128(Pack<T, 8>::of(now[v]).w, y, int(in && c < a.N ? at : kNowhere), 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+          __builtin_amdgcn_raw_buffer_store_b16(rounded<T>(now[v][i]).bits, y, int(in && c + i < a.N ? at + 2 * i : kNowhere), 0, 0);
+      }
+    }
+  };
+  S s;
+  s.lane = lane;
+  const auto load_b = [&](u32x4 (&w)[8], int tile, int k) {
+    s.set_columns((tile0 + tile) * OUT, a.N - (tile0 + tile) * OUT, a.b.sk, a.b.sn);
+    if constexpr (LAY == GMM_W_ROWS) {
+      s.load_w(w, k, a.R);
+    } else {      // a rank's values of a column lie side by side: the operands as they are
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(s.w_buf, int(i < s.columns && k + 8 * g < a.R ? s.w_at + i * s.w_step_n + (k + 8 * g) * 2 : kNowhere), 0, 0);
+    }
+  };
+  const auto multiply = [&](const u32x4 (&w)[8], u32x4 h, u32x4 l, f32x4 (&acc)[FR]) {
+#pragma unroll
+    for (int i = 0; i < FR; ++i) {
+      const u32x4 b = LAY == GMM_W_ROWS ? S::turned(w, i) : w[i];
+      acc[i] = mfma(T{}, h, b, acc[i]);
+      acc[i] = mfma(T{}, l, b, acc[i]);
+    }
+  };
+  // rows of different adapters: one adapter after the other
+#pragma unroll 1
+  for (uint32_t todo = with; todo;) {
+    const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
+    const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
+    todo &= ~mine;
+    s.w_buf = matrix<T>(a.b, which);
+    u32x4 h[NK], l[NK], w[NK][8];
+    u32x4 next[4];
+    const auto load_low = [&](int k) {
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int at = k + 32 * n < a.pitch ? k + 32 * n : 0;      // past the rank B's rows read as zeros
+        h[n] = *reinterpret_cast<const u32x4*>(high + at);
+        l[n] = *reinterpret_cast<const u32x4*>(low + at);
+      }
+    };
+    load_low(0);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) load_b(w[n], 0, 32 * n);
+    load_y(next, 0, mine);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (int tile = 0; tile < tiles; ++tile) {
+      f32x4 acc[FR];
+#pragma unroll
+      for (int i = 0; i < FR; ++i) acc[i] = f32x4{0, 0, 0, 0};
+#pragma unroll 1
+      for (int k = 0;;) {
+#pragma unroll
+        for (int n = 0; n < NK; ++n) multiply(w[n], h[n], l[n], acc);
+        k += 32 * NK;
+        if (k >= a.R) break;
+        load_low(k);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) load_b(w[n], tile, k + 32 * n);
+      }
+      if (a.R > 32 * NK) load_low(0);
+      __builtin_amdgcn_sched_barrier(0);
+      const int ahead = tile + 1 < tiles ? tile + 1 : tile;
+#pragma unroll
+      for (int n = 0; n < NK; ++n) load_b(w[n], ahead, 32 * n);
+      __builtin_amdgcn_sched_barrier(0);
+      float now[4][FR];
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int i = 0; i < FR; ++i) now[v][i] = widen(T{uint16_t(next[v][i / 2] >> 16 * (i & 1))}) + acc[i][v];
+      load_y(next, ahead, mine);
+      __builtin_amdgcn_sched_barrier(0);
+      store_y(now, tile, mine);
     }
   }
 }
@@ -323,8 +383,11 @@ __global__ void __launch_bounds__(kThreads) lora_add_any_kernel(const LoraArgs a
   __shared__ f32x4 low[kAnyRows][kMaxRank / 4 + 1];
   const int row0 = blockIdx.x * kAnyRows, c = blockIdx.y * kThreads + threadIdx.x, lane = threadIdx.x & 63;
   const int span = int(a.R + 3) / 4 * 4;
-  for (int u = threadIdx.x; u < kAnyRows * span; u += kThreads)
-    reinterpret_cast<float*>(low[u / span])[u % span] = scaled_low(a, row0 + u / span, u % span);
+  for (int u = threadIdx.x; u < kAnyRows * span; u += kThreads) {
+    const int64_t at = int64_t(min(row0 + u / span, a.rows - 1)) * a.pitch + u % span;
+    const T* const planes = static_cast<const T*>(a.planes);
+    reinterpret_cast<float*>(low[u / span])[u % span] = widen(planes[at]) + widen(planes[int64_t(a.rows) * a.pitch + at]);
+  }
   __syncthreads();
   const int id = lane < kAnyRows && row0 + lane < a.rows ? a.adapter[row0 + lane] : -1;
   const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L)));
@@ -416,11 +479,11 @@ __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& ad
 constexpr int kMaxChunk = 4096;
 
 // out[i] += q^T p over a chunk of adapter i's rows: R rows, a strip of 128 columns of p, the contraction along p's rows.
-template <typename T, int MF>
+template <typename T, int MF, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args) {
-  using S = Skinny<T, GMM_W_ROWS, 8, 1, false, MF, 2, 2>;
+  using S = Skinny<T, GMM_W_ROWS, 8, MF, 2, false, 2>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
-  __shared__ SkinnySums<kWaves, FR> sums;
+  __shared__ SkinnyShared<S, kWaves> shared;
   __shared__ int32_t row_at[kMaxChunk];
   const bool second = int(blockIdx.x) >= args.groups0;
   const GradOf& a = args.of[second];
@@ -433,55 +496,65 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c)), R = args.R;
   S s;
+  s.lane = lane;
+  s.lds = shared.wave[wave];
   s.a_plane = uint32_t(R) * args.places * 2;
   s.a_buf = buffer(a.q, 2 * s.a_plane);
-#pragma unroll
-  for (int m = 0; m < MF; ++m) s.a_at[m] = r0 + 16 * m + j < R ? (uint32_t(r0 + 16 * m + j) * args.places + first) * 2 : kNowhere;
-  const T* const p = static_cast<const T*>(a.p) + c;
-  // Steps as Skinny::load has them, from rows that are anywhere: 64-bit addresses, and zeros for the rows behind the end.
-  const auto load = [&](typename S::Step& step, int k, int end) {
+  s.set_rows([&](int r) { return r0 + r < R ? (uint32_t(r0 + r) * args.places + first) * 2 : kNowhere; });
+  // Steps as Skinny has them, from rows that are anywhere (64-bit addresses).  Past the end the last row is read again and not used.
+  const T* const p = static_cast<const T*>(a.p) + (columns ? c : 0);
+  const auto load = [&](typename S::Step& step, int k) {
     const int kl = k + 8 * g;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
+      const T* at = p + int64_t(row_at[min(kl + r, rows - 1)]) * a.p_ld;
       u32x4 v = {0, 0, 0, 0};
-      if (kl + r < end && columns) {
-        const T* at = p + int64_t(row_at[kl + r]) * a.p_ld;
-        if (a.whole) {
-          v = *reinterpret_cast<const u32x4*>(at);
-        } else {
+      if constexpr (WHOLE) {
+        v = *reinterpret_cast<const u32x4*>(at);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < columns) v[i / 2] |= uint32_t(at[i].bits) << 16 * (i & 1);
-        }
+        for (int i = 0; i < 8; ++i) v[i / 2] |= uint32_t(at[max(0, min(i, columns - 1))].bits) << 16 * (i & 1);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) step.w[4 * r + i] = v[i];
+      step.w[r] = v;
     }
-    s.template load_a<MF>(step, k, end, g);
+    s.template load_a<MF>(step, k, rows);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto multiply = [&](typename S::Step& step, int k, f32x4 (&acc)[MF][FR]) {
+    if (k >= rows) return;
+    if (k + 32 > rows) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) step.w[r][q] = k + 8 * g + r < rows ? step.w[r][q] : 0u;
+    }
+    s.template multiply<MF>(step, acc);
+    __builtin_amdgcn_sched_barrier(0);
   };
   f32x4 acc[MF][FR];
   clear(acc);
-  int from, to;
-  wave_range<32, kWaves>(0, rows, wave, from, to);
-  typename S::Step step[2];
-  load(step[0], from, to);
-  load(step[1], from + 32, to);
-  for (int k = from; k < to; k += 64)
+  if (rows) {
+    constexpr int NEXT = 32 * kWaves;
+    typename S::Step step[2];
+    load(step[0], 32 * wave);
+    load(step[1], 32 * wave + NEXT);
+    for (int k = 32 * wave; k < rows; k += 2 * NEXT)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s.template multiply<MF>(step[u], acc);
-      load(step[u], k + 64 + 32 * u, to);
-    }
+      for (int u = 0; u < 2; ++u) {
+        multiply(step[u], k + u * NEXT, acc);
+        load(step[u], k + (2 + u) * NEXT);
+      }
+  }
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     if (r0 + 16 * m >= R) break;
-    if (m) __syncthreads();
-    sums.put(wave, lane, acc[m]);
+    __syncthreads();
+    shared.sums.put(wave, lane, acc[m]);
     __syncthreads();
     for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.C) continue;
-      const f32x4 h = sums.get(oc % FR, oc / FR, og);
+      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
       const int r = r0 + 16 * m + 4 * og;
       if (slot >= 0) {
         float* const to = a.partial + int64_t(slot) * R * a.C + (a.r_first ? int64_t(col) * R + r : int64_t(r) * a.C + col);
@@ -613,11 +686,12 @@ bool set(Matrices& m, const void* at, int64_t sg, int64_t sk, int64_t sn, int64_
 }
 
 int check_sizes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int32_t dtype) {
-  constexpr int64_t most = (int64_t(1) << 30) / kMaxRank * 16;
-  if (rows < 0 || K < 0 || N < 0 || R < 1 || L < 0 || rows >= most || K >= most || N >= most || R > kMaxRank || L > kMaxAdapters) return GMM_ERR_BAD_ARGUMENT;
+  constexpr int64_t most = int64_t(1) << 22, most_rows = int64_t(1) << 26;
+  if (rows < 0 || K < 0 || N < 0 || R < 1 || L < 0 || rows >= most_rows || K >= most || N >= most || R > kMaxRank || L > kMaxAdapters) return GMM_ERR_BAD_ARGUMENT;
   return dtype == GMM_DT_BF16 || dtype == GMM_DT_F16 ? GMM_OK : GMM_ERR_UNSUPPORTED;
 }
 
+// Rows that are read (or written) a strip of them at a time, from one base.
 bool x_fits(int64_t x_ld, int64_t rows, int64_t K) {
   return rows <= 1 || (x_ld >= K && x_ld <= ((int64_t(1) << 30) - 64 - K) / (rows < kFewRows ? rows : kFewRows));
 }
@@ -631,8 +705,8 @@ void set_low(LoraArgs& a, int columns) {
 
 template <typename T>
 int launch_few(LoraArgs a, bool whole, int lay_b, hipStream_t stream) {
-  int lay_w = layout_of(a.w, a.K, a.N, whole), lay_a = layout_of(a.a, a.K, 8, whole);
-  if (lay_w == GMM_W_ANY || lay_a != GMM_W_COLS) lay_a = GMM_W_ANY;
+  const int lay_w = layout_of(a.w, a.K, a.N, whole);
+  const int lay_a = lay_w == GMM_W_ANY ? GMM_W_ANY : layout_of(a.a, a.K, a.R, whole);
   set_low(a, 16);
   const BasePlan bp = plan_base(a.K, a.N, strip_columns(lay_w));
   a.base_parts = bp.parts; a.base_k = bp.each;
@@ -648,8 +722,14 @@ int launch_few(LoraArgs a, bool whole, int lay_b, hipStream_t stream) {
   constexpr std::integral_constant<int, GMM_W_ROWS> rows{};
   constexpr std::integral_constant<int, GMM_W_COLS> cols{};
   constexpr std::integral_constant<int, GMM_W_ANY> any{};
-  if (lay_w == GMM_W_ROWS) lay_a == GMM_W_COLS ? launch(rows, cols) : launch(rows, any);
-  else if (lay_w == GMM_W_COLS) lay_a == GMM_W_COLS ? launch(cols, cols) : launch(cols, any);
+  constexpr std::integral_constant<int, GMM_W_THIN> thin{};
+  const auto with_a = [&](auto w) {
+    if (lay_a == GMM_W_COLS) launch(w, cols);
+    else if (lay_a == GMM_W_ROWS) launch(w, thin);
+    else launch(w, any);
+  };
+  if (lay_w == GMM_W_ROWS) with_a(rows);
+  else if (lay_w == GMM_W_COLS) with_a(cols);
   else launch(any, any);
   by_layout(lay_b, [&](auto l) {
     constexpr int B = decltype(l)::value, W = B == GMM_W_ROWS ? 8 : 1;
@@ -658,45 +738,70 @@ int launch_few(LoraArgs a, bool whole, int lay_b, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
-// Columns of a lane: as few as hold the rank, as many as lie side by side and aligned.
+// Columns of a strip: as few as hold the rank.
 template <typename T>
 int launch_low(LoraArgs& a, bool whole, hipStream_t stream) {
-  const bool cols = layout_of(a.a, a.K, 8, whole) == GMM_W_COLS;
-  int fr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : a.R <= 64 || cols ? 4 : 8;
-  if (!cols) {
-    const int64_t all = a.R | a.a.sk | a.a.sg | int64_t(reinterpret_cast<uintptr_t>(a.a.at) / 2);
-    while (fr > 1 && (a.a.sn != 1 || !whole || !multiple8(a.K) || all % fr)) fr /= 2;
-  }
+  const int lay = layout_of(a.a, a.K, a.R, whole);
+  int fr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : a.R <= 64 || lay == GMM_W_COLS ? 4 : 8;
+  if (lay == GMM_W_ANY) fr = 1;
   set_low(a, 16 * fr);
   const dim3 grid(unsigned(a.low_groups)), block(kThreads);
   const bool edge = !whole || !multiple8(a.K);     // x has no alignment
-  if (cols && fr == 1) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_COLS, 1, false>), grid, block, 0, stream, a);
-  else if (cols && fr == 2) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_COLS, 2, false>), grid, block, 0, stream, a);
-  else if (cols) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_COLS, 4, false>), grid, block, 0, stream, a);
-  else if (fr == 8) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ROWS, 8, false>), grid, block, 0, stream, a);
-  else if (fr == 4) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ROWS, 4, false>), grid, block, 0, stream, a);
-  else if (fr == 2) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ROWS, 2, false>), grid, block, 0, stream, a);
-  else if (edge) hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ANY, 1, true>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((lora_low_kernel<T, GMM_W_ANY, 1, false>), grid, block, 0, stream, a);
+  const auto launch = [&](auto l, auto n, auto e) {
+    hipLaunchKernelGGL((lora_low_kernel<T, decltype(l)::value, decltype(n)::value, decltype(e)::value>), grid, block, 0, stream, a);
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  if (lay == GMM_W_COLS) {
+    constexpr std::integral_constant<int, GMM_W_COLS> cols{};
+    if (fr == 1) launch(cols, one, std::false_type{});
+    else if (fr == 2) launch(cols, two, std::false_type{});
+    else launch(cols, four, std::false_type{});
+  } else if (lay == GMM_W_ROWS) {
+    constexpr std::integral_constant<int, GMM_W_THIN> thin{};
+    if (fr == 1) launch(thin, one, std::false_type{});
+    else if (fr == 2) launch(thin, two, std::false_type{});
+    else if (fr == 4) launch(thin, four, std::false_type{});
+    else launch(std::integral_constant<int, GMM_W_ROWS>{}, std::integral_constant<int, 8>{}, std::false_type{});
+  } else {
+    constexpr std::integral_constant<int, GMM_W_ANY> any{};
+    if (edge) launch(any, one, std::true_type{});
+    else launch(any, one, std::false_type{});
+  }
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
+
+int64_t pitch_of(int64_t R) { return round_up(R, 32); }
 
 template <typename T>
 int launch_add(LoraArgs a, bool whole, hipStream_t stream) {
   const int rc = launch_low<T>(a, whole, stream);
-  if (rc != GMM_OK || (a.N == 0 && !a.low_out)) return rc;
-  const int lay = layout_of_b(a.b, a.R, a.N);
-  if (lay == GMM_W_ANY) {
-    const dim3 grid(unsigned((a.rows + kAnyRows - 1) / kAnyRows), unsigned(a.N ? (a.N + kThreads - 1) / kThreads : 1));
-    hipLaunchKernelGGL((lora_add_any_kernel<T>), grid, dim3(kThreads), 0, stream, a);
-    return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+  if (rc != GMM_OK) return rc;
+  a.pitch = int(pitch_of(a.R));
+  const unsigned blocks = unsigned((int64_t(a.rows) * a.pitch + kThreads - 1) / kThreads);
+  hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
+  if (a.N) {
+    const int lay = layout_of_b(a.b, a.R, a.N);
+    const int wide = aligned16(a.out) && multiple8(a.out_ld) && multiple8(a.N);
+    const dim3 any((a.rows + kAnyRows - 1) / kAnyRows, (a.N + kThreads - 1) / kThreads);
+    // strips to a wave: as many as leave every place for one a wave
+    const int tiles = (a.N + 127) / 128, row_groups = (a.rows + 16 * kWaves - 1) / (16 * kWaves);
+    a.strips = clamp(int64_t(row_groups) * tiles / (3 * gmm_num_cus()), 1, tiles);
+    const dim3 grid(row_groups, (tiles + a.strips - 1) / a.strips);
+    const auto launch = [&](auto lay, auto nk) {
+      constexpr int B = decltype(lay)::value, NK = decltype(nk)::value;
+      if (wide) hipLaunchKernelGGL((lora_add_kernel<T, B, NK, true>), grid, dim3(kThreads), 0, stream, a);
+      else hipLaunchKernelGGL((lora_add_kernel<T, B, 1, false>), grid, dim3(kThreads), 0, stream, a);
+    };
+    const auto rank = [&](auto lay) {
+      if (a.R <= 32) launch(lay, std::integral_constant<int, 1>{});
+      else launch(lay, std::integral_constant<int, 2>{});
+    };
+    if (lay == GMM_W_ANY) hipLaunchKernelGGL((lora_add_any_kernel<T>), any, dim3(kThreads), 0, stream, a);
+    else if (lay == GMM_W_ROWS) rank(std::integral_constant<int, GMM_W_ROWS>{});
+    else rank(std::integral_constant<int, GMM_W_COLS>{});
   }
-  const int wide = aligned16(a.out) && multiple8(a.out_ld) && multiple8(a.N);
-  const int pitch = int(round_up(a.R, 32)) + 8;      // 16 bytes more: rows begin in other banks
-  const dim3 grid(unsigned((a.rows + kAddRows - 1) / kAddRows), unsigned(a.N ? (a.N + 128 * kAddStrips - 1) / (128 * kAddStrips) : 1));
-  const int lds = 2 * kAddRows * pitch * 2;
-  if (lay == GMM_W_ROWS) hipLaunchKernelGGL((lora_add_kernel<T, GMM_W_ROWS>), grid, dim3(kThreads), lds, stream, a, wide, pitch);
-  else hipLaunchKernelGGL((lora_add_kernel<T, GMM_W_COLS>), grid, dim3(kThreads), lds, stream, a, wide, pitch);
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
@@ -745,9 +850,12 @@ int launch_grad(GradArgs& g, int64_t rows, hipStream_t stream) {
   g.groups0 = int32_t(chunks * g.of[0].tiles);
   const int64_t groups = g.groups0 + chunks * g.of[1].tiles;
   if (groups == 0) return GMM_OK;
+  const bool whole = (!g.of[0].tiles || g.of[0].whole) && (!g.of[1].tiles || g.of[1].whole);
   const auto launch = [&](auto mf) {
     constexpr int MF = decltype(mf)::value;
-    hipLaunchKernelGGL((lora_grad_kernel<T, MF>), dim3(unsigned(groups), unsigned((g.R + 16 * MF - 1) / (16 * MF))), dim3(kThreads), 0, stream, g);
+    const dim3 grid(unsigned(groups), unsigned((g.R + 16 * MF - 1) / (16 * MF)));
+    if (whole) hipLaunchKernelGGL((lora_grad_kernel<T, MF, true>), grid, dim3(kThreads), 0, stream, g);
+    else hipLaunchKernelGGL((lora_grad_kernel<T, MF, false>), grid, dim3(kThreads), 0, stream, g);
   };
   if (g.R <= 16) launch(std::integral_constant<int, 1>{});
   else if (g.R <= 32) launch(std::integral_constant<int, 2>{});
@@ -764,11 +872,14 @@ int launch_grad(GradArgs& g, int64_t rows, hipStream_t stream) {
 
 }  // namespace
 
+// Bytes of the parts of x @ A.
+static int64_t low_bytes(int64_t rows, int64_t K, int64_t R) { return round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256); }
+
 extern "C" {
 
 int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R) {
   if (check_sizes(rows, K, N, R, 0, GMM_DT_BF16) != GMM_OK) return -1;
-  int64_t bytes = round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256);
+  int64_t bytes = low_bytes(rows, K, R) + round_up(2 * rows * pitch_of(R) * 2, 256);
   if (rows <= kFewRows) bytes += int64_t(plan_base(K, N, 128).parts) * rows * N * 4;     // the layout with the more parts
   return bytes;
 }
@@ -782,13 +893,13 @@ int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, 
   if (rows > kFewRows) return GMM_ERR_UNSUPPORTED;
   if (rows == 0 || N == 0) return GMM_OK;
   LoraArgs g{};
-  if (!out || !adapter || (K && (!x || !w)) || (L && (!b || (K && !a))) || !x_fits(x_stride, rows, K) || (rows > 1 && out_stride < N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!out || !adapter || (K && (!x || !w)) || (L && (!b || (K && !a))) || !x_fits(x_stride, rows, K) || !x_fits(out_stride, rows, N)) return GMM_ERR_BAD_ARGUMENT;
   if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
   if (!set(g.w, w, 0, w_stride_k, w_stride_n, K, N)) return w_stride_k < 0 || w_stride_n < 0 ? GMM_ERR_BAD_ARGUMENT : GMM_ERR_UNSUPPORTED;
   if (!workspace || !aligned16(workspace) || workspace_bytes < gmm_lora_workspace_bytes(rows, K, N, R)) return GMM_ERR_WORKSPACE;
   g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low;
   g.low = static_cast<float*>(workspace);
-  g.base = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256));
+  g.base = reinterpret_cast<float*>(static_cast<char*>(workspace) + low_bytes(rows, K, R));
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
   const bool whole = aligned16(x) && multiple8(g.x_ld);
@@ -807,10 +918,11 @@ int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* ada
   if (!out) N = 0;
   if (rows == 0 || L == 0 || (N == 0 && !low)) return GMM_OK;
   LoraArgs g{};
-  if (!adapter || (out && !b) || (K && (!x || !a)) || !x_fits(x_stride, rows, K) || (rows > 1 && out_stride < N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!adapter || (out && !b) || (K && (!x || !a)) || !x_fits(x_stride, rows, K) || !x_fits(out_stride, rows, N)) return GMM_ERR_BAD_ARGUMENT;
   if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
-  if (!workspace || !aligned16(workspace) || workspace_bytes < int64_t(plan_low(rows, K).parts) * rows * R * 4) return GMM_ERR_WORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < low_bytes(rows, K, R) + 2 * rows * pitch_of(R) * 2) return GMM_ERR_WORKSPACE;
   g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low; g.low = static_cast<float*>(workspace);
+  g.planes = N ? static_cast<char*>(workspace) + low_bytes(rows, K, R) : nullptr;
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
   const bool whole = aligned16(x) && multiple8(g.x_ld);

@@ -1,21 +1,24 @@
 // Products of a few rows with a matrix that is read once: D[m, n] = sum over k of A[m, k] * W[k, n], m < 64.
 //
-// Reading W bounds them (2 bytes for 2 * m operations).  So W goes from memory into registers past no LDS: a wave takes a strip of
-// columns and a range of k, and what it loads is the second operand of v_mfma_f32_16x16x32 as it is, or nearly so:
-//   W contiguous along n (GMM_W_ROWS): the operand wants 8 values of k for one column in a lane, memory gives 8 columns for one k.  Lane
-//     (j = lane & 15, g = lane >> 4) loads columns 8 j .. 8 j + 7 of rows k + 8 g .. k + 8 g + 7 (16 bytes each, 256 side by side over the
-//     lanes); byte permutes of pairs of rows, half an instruction an element, make them the operands of eight products, product i having
-//     columns i, 8 + i, 16 + i, ...  Nothing has to be undone: a column of the result is a column of its product.
-//   W contiguous along k (GMM_W_COLS): a lane loads 16 values of k of each of 4 columns, 128 bytes side by side over the four g's.
-//   anything else (GMM_W_ANY): as GMM_W_ROWS, element by element.
-// Rows of A are the first operand: 16 rows to a product, rows that do not exist read as zeros and cost no access.  The waves of a
-// workgroup share the range of k and add their results up in LDS.
+// Reading W bounds them (2 bytes for 2 * m operations).  A wave takes a strip of columns and a range of k, loads both operands 16 bytes
+// to a lane, some steps ahead, into registers, and multiplies with v_mfma_f32_16x16x32, whose operands want 8 values of k for one column
+// (or row) in a lane.  How they get there, by the way W lies in memory:
+//   along n, in strips of 128 columns (GMM_W_ROWS): a lane (j = lane & 15, g = lane >> 4) loads columns 8 j .. 8 j + 7 of rows
+//     k + 8 g .. k + 8 g + 7; byte permutes of pairs of rows, half an instruction an element, make them the operands of eight
+//     products, product i having columns i, 8 + i, 16 + i, ...  Nothing has to be undone: a column of the result is one of its product.
+//   along k (GMM_W_COLS): eight lanes load 64 values of k of a column, and the lanes swap through LDS.  Loaded as the operand wants it, four
+//     neighbouring lanes would ask for four cache lines: such a load takes the unit that looks lines up 64 cycles, not 16, and that
+//     is what bounded these products (67 MB past 64 rows 27 us).
+//   along n, 16 to 64 columns (GMM_W_THIN): rows of k side by side, turned by LDS reads that transpose.
+//   anything else (GMM_W_ANY): as GMM_W_ROWS, or 16 columns, element by element.
+// A goes through LDS as well, for the same reason.  Its rows that do not exist read as zeros and cost no access.  LDS is a wave's own
+// here: its instructions run in order, nobody waits for anybody.  The waves of a workgroup share the range of k and add up in LDS.
 #pragma once
 #include "gmm_elem.h"
 
 namespace gmm {
 
-constexpr int GMM_W_ROWS = 0, GMM_W_COLS = 1, GMM_W_ANY = 2;
+constexpr int GMM_W_ROWS = 0, GMM_W_COLS = 1, GMM_W_ANY = 2, GMM_W_THIN = 3;
 constexpr uint32_t kNowhere = 0x80000000u;   // an offset past every buffer: reads as zeros
 constexpr int kStream = 2;                   // cache policy of loads of what is read once: non-temporal
 
@@ -46,79 +49,121 @@ __device__ __forceinline__ void split(float f, T& high, T& low) {
   low = rounded<T>(__builtin_isfinite(back) ? f - back : 0.0f);
 }
 
+// Order of a wave's LDS accesses for the compiler; the hardware keeps it.
+__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
+
 // One strip of columns of one product, by one wave.
-//   FR: columns of a lane, which is products of 16 columns (GMM_W_ROWS: 2, 4, 8; GMM_W_COLS: any; GMM_W_ANY: 1, 8).
-//   KH: 32s of k in a step (2 for GMM_W_COLS where k is long: whole cache lines).
-//   AE: rows of A are read element by element (no alignment).
-//   MF: sixteens of rows.  NA: planes of A (2: A = high + low).  ST: steps in flight.
-template <typename T, int LAY, int FR_, int KH, bool AE, int MF, int NA, int ST>
+//   FR: products of 16 columns (GMM_W_ROWS: 8; GMM_W_COLS, GMM_W_THIN: 1, 2, 4; GMM_W_ANY: 1, 8).
+//   MF: sixteens of rows.  NA: planes of A (2: A = high + low).  AE: rows of A are read element by element (no alignment).
+//   ST: steps in flight.
+template <typename T, int LAY, int FR_, int MF, int NA, bool AE, int ST>
 struct Skinny {
   static constexpr int FR = FR_;
-  static constexpr int KS = 32 * KH;          // k of a step
-  static constexpr int KG = KS / 4;           // of them a lane's
+  static constexpr int KS = LAY == GMM_W_COLS ? 64 : 32;      // k of a step
+  static constexpr int KH = KS / 32;                          // products' halves of it
   static constexpr int COLUMNS = 16 * FR;
-  static constexpr int WORDS = LAY == GMM_W_COLS ? 4 * FR * KH : FR == 1 ? 4 : 4 * FR;   // of W in a step, of a lane
-  static_assert(LAY == GMM_W_COLS || KH == 1, "");
+  static constexpr int CH = KS / 8;                           // 16-byte chunks of a row (or column) in a step
+  static constexpr int ROWS_AT_ONCE = 64 / CH;                // that a load has
+  static constexpr int WL = LAY == GMM_W_COLS ? 2 * FR : LAY == GMM_W_THIN ? FR : LAY == GMM_W_ROWS || FR == 8 ? 8 : 1;   // loads of W
+  static constexpr int AL = MF * KH;                          // loads of a plane of A
+  static constexpr int W_BYTES = LAY == GMM_W_COLS ? 128 * COLUMNS : LAY == GMM_W_THIN ? 1024 * FR : 0;
+  static constexpr int PLANE_BYTES = AE ? 0 : 32 * MF * KS;
+  static constexpr int LDS_BYTES = W_BYTES + NA * PLANE_BYTES;      // of a wave
+  static_assert(LAY != GMM_W_ROWS || FR == 8, "");
   static_assert(LAY != GMM_W_ANY || FR == 1 || FR == 8, "");
-  static_assert(LAY != GMM_W_ROWS || FR == 2 || FR == 4 || FR == 8, "");
+  static_assert(!AE || LAY == GMM_W_ANY, "");
 
   __amdgpu_buffer_rsrc_t w_buf, a_buf;
-  uint32_t w_at;          // byte offset of the lane's first column
+  char* lds;
+  int lane;
+  uint32_t w_at;          // byte offset of what the lane loads first, k = 0
   uint32_t w_step_k, w_step_n;   // bytes from one k, one column, to the next
-  int columns;            // the lane's columns that exist (GMM_W_ROWS: all or none)
-  uint32_t a_at[MF];      // byte offset of the lane's rows of A, kNowhere: no such row
+  int columns;            // the lane's columns that exist (GMM_W_ROWS, GMM_W_THIN: all or none); GMM_W_COLS: the strip's (of either half)
+  uint32_t w_jump;        // GMM_W_COLS: bytes that the second half of the columns lies further away than it would
+  int w_half;             // and where it begins
+  uint32_t a_at[AL];      // byte offset of the lane's rows of A, kNowhere: no such row
   uint32_t a_plane;       // bytes from the high to the low plane
 
-  struct Step { uint32_t w[WORDS]; u32x4 a[MF][NA][KH]; };
+  struct Step { u32x4 w[WL]; u32x4 a[NA][AL]; };
 
   static __device__ __forceinline__ uint32_t element(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
     return uint32_t(uint16_t(__builtin_amdgcn_raw_buffer_load_b16(buf, int(at), 0, 0)));
   }
 
-  // Loads k .. k + KS - 1, of which those before `end` exist.
-  template <int M>
-  __device__ __forceinline__ void load(Step& s, int k, int end, int g) const {
-    load_w(s, k, end, g);
-    load_a<M>(s, k, end, g);
+  // Column of the strip that product i has in lanes j, 16 + j, ...; and back.
+  static __device__ __forceinline__ int product_of(int column) { return LAY == GMM_W_ROWS || LAY == GMM_W_ANY ? column % FR : column / 16; }
+  static __device__ __forceinline__ int lane_of(int column) { return LAY == GMM_W_ROWS || LAY == GMM_W_ANY ? column / FR : column % 16; }
+
+  // The strip of columns from `first` on, of which `count` (or more than the strip holds) exist; steps in elements.  With `half` > 0 it is
+  // that many columns from `first` on and as many from `other` on, `count` of each.
+  __device__ __forceinline__ void set_columns(int first, int count, uint32_t sk, uint32_t sn, int half = 0, int other = 0) {
+    const int j = lane & 15;
+    w_step_k = sk * 2;
+    w_step_n = sn * 2;
+    if constexpr (LAY == GMM_W_COLS) {
+      columns = count;
+      w_half = half ? half : COLUMNS;
+      w_jump = half ? uint32_t(other - first - half) * w_step_n : 0;
+      w_at = uint32_t(first + (lane >> 3)) * w_step_n + (lane & 7) * 16;
+    } else if constexpr (LAY == GMM_W_THIN) {
+      const int c = lane % (2 * FR) * 8;
+      columns = count - c;
+      w_at = uint32_t(lane / (2 * FR)) * w_step_k + uint32_t(first + c) * 2;
+    } else {
+      const int c = FR * j, in = half ? c % half : c;
+      columns = max(0, min(FR, count - in));
+      w_at = uint32_t((half && c >= half ? other : first) + in) * w_step_n;
+    }
   }
 
-  __device__ __forceinline__ void load_w(Step& s, int k, int end, int g) const {
-    const int kl = k + KG * g;
+  // at(r): byte offset of row r of A, kNowhere if there is none.
+  template <typename F>
+  __device__ __forceinline__ void set_rows(F&& at) {
+#pragma unroll
+    for (int i = 0; i < AL; ++i) {
+      const uint32_t from = at(AE ? 16 * i + (lane & 15) : ROWS_AT_ONCE * i + lane / CH);
+      a_at[i] = from == kNowhere || AE ? from : from + lane % CH * 16;
+    }
+  }
+
+  // Loads k .. k + KS - 1, of which those before `end` exist, and the first M of the sixteens of rows.
+  template <int M>
+  __device__ __forceinline__ void load(Step& s, int k, int end) const {
+    load_w(s.w, k, end);
+    load_a<M>(s, k, end);
+  }
+
+  __device__ __forceinline__ void load_w(u32x4 (&w)[WL], int k, int end) const {
+    const int kl = k + 8 * (lane >> 4);
     if constexpr (LAY == GMM_W_ROWS) {
       const uint32_t at = w_at + uint32_t(kl) * w_step_k;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int from = int(columns && kl + r < end ? at + r * w_step_k : kNowhere);
-        if constexpr (FR == 8) {
-          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(w_buf, from, 0, kStream);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s.w[4 * r + i] = v[i];
-        } else if constexpr (FR == 4) {
-          const auto v = __builtin_amdgcn_raw_buffer_load_b64(w_buf, from, 0, 0);
-          s.w[2 * r] = v[0];
-          s.w[2 * r + 1] = v[1];
-        } else {
-          s.w[r] = __builtin_amdgcn_raw_buffer_load_b32(w_buf, from, 0, 0);
-        }
-      }
+      for (int r = 0; r < 8; ++r)
+        w[r] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(columns && kl + r < end ? at + r * w_step_k : kNowhere), 0, kStream);
     } else if constexpr (LAY == GMM_W_COLS) {
-      const uint32_t at = w_at + uint32_t(kl) * 2;
+      const uint32_t at = w_at + uint32_t(k) * 2;
+      const bool in = k + 8 * (lane & 7) < end;
 #pragma unroll
-      for (int i = 0; i < FR; ++i)
+      for (int i = 0; i < WL; ++i) {
+        const int c = 8 * i + (lane >> 3);
+        const bool second = 8 * i >= w_half;
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(
+            w_buf, int(in && c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere), 0, kStream);
+      }
+    } else if constexpr (LAY == GMM_W_THIN) {
 #pragma unroll
-        for (int h = 0; h < KH; ++h) {
-          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(
-              w_buf, int(i < columns && kl + 8 * h < end ? at + i * w_step_n + 16 * h : kNowhere), 0, kStream);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) s.w[4 * (KH * i + h) + q] = v[q];
-        }
+      for (int i = 0; i < WL; ++i) {
+        const int row = k + 32 / FR * i;
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(
+            w_buf, int(columns > 0 && row + lane / (2 * FR) < end ? w_at + uint32_t(row) * w_step_k : kNowhere), 0, 0);
+      }
     } else if constexpr (FR == 1) {
       const uint32_t at = w_at + uint32_t(kl) * w_step_k;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t lo = element(w_buf, columns && kl + 2 * q < end ? at + 2 * q * w_step_k : kNowhere);
         const uint32_t hi = element(w_buf, columns && kl + 2 * q + 1 < end ? at + (2 * q + 1) * w_step_k : kNowhere);
-        s.w[q] = lo | hi << 16;
+        w[0][q] = lo | hi << 16;
       }
     } else {
 #pragma unroll
@@ -129,101 +174,135 @@ struct Skinny {
           const bool in = kl + r < end;
           const uint32_t lo = element(w_buf, in && 2 * q < columns ? at : kNowhere);
           const uint32_t hi = element(w_buf, in && 2 * q + 1 < columns ? at + w_step_n : kNowhere);
-          s.w[4 * r + q] = lo | hi << 16;
+          w[r][q] = lo | hi << 16;
         }
     }
   }
 
-  // The first M of the sixteens of rows.
   template <int M>
-  __device__ __forceinline__ void load_a(Step& s, int k, int end, int g) const {
-    const int kl = k + KG * g;
+  __device__ __forceinline__ void load_a(Step& s, int k, int end) const {
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
+    for (int i = 0; i < M * KH; ++i)
 #pragma unroll
-      for (int p = 0; p < NA; ++p)
+      for (int p = 0; p < NA; ++p) {
+        if constexpr (AE) {
+          const int kl = k + 8 * (lane >> 4);
+          const uint32_t at = a_at[i] + p * a_plane + uint32_t(kl) * 2;
 #pragma unroll
-        for (int h = 0; h < KH; ++h) {
-          const uint32_t at = a_at[m] + p * a_plane + uint32_t(kl + 8 * h) * 2;
-          if constexpr (AE) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int kq = kl + 8 * h + 2 * q;
-              const uint32_t lo = element(a_buf, a_at[m] != kNowhere && kq < end ? at + 4 * q : kNowhere);
-              const uint32_t hi = element(a_buf, a_at[m] != kNowhere && kq + 1 < end ? at + 4 * q + 2 : kNowhere);
-              s.a[m][p][h][q] = lo | hi << 16;
-            }
-          } else {
-            s.a[m][p][h] = __builtin_amdgcn_raw_buffer_load_b128(a_buf, int(a_at[m] != kNowhere && kl + 8 * h < end ? at : kNowhere), 0, 0);
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t lo = element(a_buf, a_at[i] != kNowhere && kl + 2 * q < end ? at + 4 * q : kNowhere);
+            const uint32_t hi = element(a_buf, a_at[i] != kNowhere && kl + 2 * q + 1 < end ? at + 4 * q + 2 : kNowhere);
+            s.a[p][i][q] = lo | hi << 16;
           }
+        } else {
+          const bool in = a_at[i] != kNowhere && k + 8 * (lane % CH) < end;
+          s.a[p][i] = __builtin_amdgcn_raw_buffer_load_b128(a_buf, int(in ? a_at[i] + p * a_plane + uint32_t(k) * 2 : kNowhere), 0, 0);
         }
-    }
+      }
   }
 
-  // Second operand of product i, half h of the step.
-  static __device__ __forceinline__ u32x4 operand(const Step& s, int i, int h) {
+  // GMM_W_ROWS: the second operand of product i.
+  static __device__ __forceinline__ u32x4 turned(const u32x4 (&w)[WL], int i) {
     u32x4 b;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if constexpr (LAY == GMM_W_COLS) b[q] = s.w[4 * (KH * i + h) + q];
-      else if constexpr (FR == 1) b[q] = s.w[q];
-      else b[q] = __builtin_amdgcn_perm(s.w[(2 * q + 1) * (FR / 2) + i / 2], s.w[2 * q * (FR / 2) + i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-    }
+    for (int q = 0; q < 4; ++q) b[q] = __builtin_amdgcn_perm(w[2 * q + 1][i / 2], w[2 * q][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
     return b;
   }
 
+  // Where chunk c of row (or column) r of a step lies: such that 16 rows' chunks lie in different banks.
+  static __device__ __forceinline__ int chunk_at(int r, int c) { return r * 16 * CH + 16 * (CH == 8 ? c ^ (r >> 1 & 7) : c ^ (r >> 2 & 3)); }
+
   template <int M>
   __device__ __forceinline__ void multiply(const Step& s, f32x4 (&acc)[MF][FR]) const {
+    const int j = lane & 15, g = lane >> 4;
+    lds_order();
+    if constexpr (LAY == GMM_W_COLS)
 #pragma unroll
-    for (int i = 0; i < FR; ++i)
+      for (int i = 0; i < WL; ++i) *reinterpret_cast<u32x4*>(lds + chunk_at(8 * i + (lane >> 3), lane & 7)) = s.w[i];
+    if constexpr (LAY == GMM_W_THIN)
 #pragma unroll
-      for (int h = 0; h < KH; ++h) {
-        const u32x4 b = operand(s, i, h);
+      for (int i = 0; i < WL; ++i) *reinterpret_cast<u32x4*>(lds + 1024 * i + 16 * lane) = s.w[i];
+    if constexpr (!AE)
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
+      for (int i = 0; i < M * KH; ++i)
 #pragma unroll
-          for (int p = 0; p < NA; ++p) acc[m][i] = mfma(T{}, s.a[m][p][h], b, acc[m][i]);
+        for (int p = 0; p < NA; ++p)
+          *reinterpret_cast<u32x4*>(lds + W_BYTES + p * PLANE_BYTES + chunk_at(ROWS_AT_ONCE * i + lane / CH, lane % CH)) = s.a[p][i];
+    lds_order();
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      u32x4 a[M][NA];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int p = 0; p < NA; ++p) {
+          if constexpr (AE) a[m][p] = s.a[p][m];
+          else a[m][p] = *reinterpret_cast<const u32x4*>(lds + W_BYTES + p * PLANE_BYTES + chunk_at(16 * m + j, 4 * h + g));
         }
+#pragma unroll
+      for (int i = 0; i < FR; ++i) {
+        u32x4 b;
+        if constexpr (LAY == GMM_W_COLS) {
+          b = *reinterpret_cast<const u32x4*>(lds + chunk_at(16 * i + j, 4 * h + g));
+        } else if constexpr (LAY == GMM_W_THIN) {
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+          char* const from = lds + (8 * g + j / 4) * 32 * FR + 32 * i + j % 4 * 8;
+          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(from)));
+          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(from + 4 * 32 * FR)));
+          b = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        } else if constexpr (FR == 1) {
+          b = s.w[0];
+        } else {
+          b = turned(s.w, i);
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int p = 0; p < NA; ++p) acc[m][i] = mfma(T{}, a[m][p], b, acc[m][i]);
       }
+    }
   }
 
-  // acc += A[:, begin .. end) W[begin .. end).  Steps past the end load nothing: no branch stands between the loads in flight.
-  template <int M>
-  __device__ __forceinline__ void steps(int begin, int end, int g, f32x4 (&acc)[MF][FR]) const {
+  // acc += A[:, k] W[k] over every WAVES-th step of begin .. end.  Steps past the end load nothing: no branch stands between the loads in
+  // flight, and nothing moves past the barriers: moved loads would be waited for together.
+  template <int M, int WAVES>
+  __device__ __forceinline__ void steps(int begin, int end, f32x4 (&acc)[MF][FR]) const {
+    constexpr int NEXT = WAVES * KS;
     Step step[ST];
 #pragma unroll
-    for (int u = 0; u < ST; ++u) load<M>(step[u], begin + u * KS, end, g);
-    for (int k = begin; k < end; k += ST * KS)
+    for (int u = 0; u < ST; ++u) {
+      load<M>(step[u], begin + u * NEXT, end);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int k = begin; k < end; k += ST * NEXT)
 #pragma unroll
       for (int u = 0; u < ST; ++u) {
         multiply<M>(step[u], acc);
-        load<M>(step[u], k + (ST + u) * KS, end, g);
+        __builtin_amdgcn_sched_barrier(0);
+        load<M>(step[u], k + (ST + u) * NEXT, end);
+        __builtin_amdgcn_sched_barrier(0);
       }
   }
 
-  // rows: how many there are; sixteens that hold none take no part.
-  __device__ __forceinline__ void run(int rows, int begin, int end, int g, f32x4 (&acc)[MF][FR]) const {
+  // The part of wave `wave` of WAVES of the product over begin .. end: the waves' steps lie side by side in memory.  rows: how many there
+  // are; sixteens that hold none take no part.
+  template <int WAVES>
+  __device__ __forceinline__ void run(int rows, int begin, int end, int wave, f32x4 (&acc)[MF][FR]) const {
+    begin += wave * KS;
     if constexpr (MF >= 2) {
-      if (rows <= 16) return steps<1>(begin, end, g, acc);
+      if (rows <= 16) return steps<1, WAVES>(begin, end, acc);
     }
     if constexpr (MF >= 4) {
-      if (rows <= 32) return steps<2>(begin, end, g, acc);
+      if (rows <= 32) return steps<2, WAVES>(begin, end, acc);
     }
-    steps<MF>(begin, end, g, acc);
+    steps<MF, WAVES>(begin, end, acc);
   }
 };
 
-// A strip of a matrix that is large: all columns of a lane in 16-byte loads, whole cache lines.
-template <typename T, int LAY, int MF, int NA, int ST>
-using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, LAY == GMM_W_COLS ? 2 : 1, LAY == GMM_W_ANY, MF, NA, ST>;
-
-// Range of k of one of WAVES waves: whole steps of KS, dealt evenly.
-template <int KS, int WAVES>
-__device__ __forceinline__ void wave_range(int begin, int end, int wave, int& from, int& to) {
-  const int steps = (end - begin + KS - 1) / KS, each = (steps + WAVES - 1) / WAVES;
-  from = begin + wave * each * KS;
-  to = min(end, from + each * KS);
-}
+// A strip of a matrix that is large.
+template <typename T, int LAY, int MF, int NA>
+using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, MF, NA, LAY == GMM_W_ANY, 2>;
 
 template <int MF, int FR>
 __device__ __forceinline__ void clear(f32x4 (&acc)[MF][FR]) {
@@ -243,13 +322,21 @@ struct SkinnySums {
 #pragma unroll
     for (int i = 0; i < FR; ++i) at[wave][i][lane] = acc[i];
   }
-  // Rows 4 g .. 4 g + 3 of column FR * j + i of the strip.
+  // Rows 4 g .. 4 g + 3 of the column that product i has in lane j.
   __device__ __forceinline__ f32x4 get(int i, int j, int g) const {
     f32x4 s = at[0][i][16 * g + j];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) s += at[w][i][16 * g + j];
     return s;
   }
+};
+
+// LDS of a workgroup: the waves' own parts while they multiply, then (behind a barrier) the sums.
+template <typename S, int WAVES>
+union SkinnyShared {
+  char wave[WAVES][S::LDS_BYTES > 0 ? S::LDS_BYTES : 16];
+  SkinnySums<WAVES, S::FR> sums;
+  __device__ SkinnyShared() {}
 };
 
 // ---------------------------------------------------------------- host side
