@@ -60,7 +60,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix(const Matrices& m, int 
 
 // low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows; one adapter of theirs after the other.
 template <typename T, int LAY, int FR, bool AE>
-using LowSkinny = Skinny<T, LAY, FR, 1, 1, AE, FR <= 2 ? 4 : 2>;
+using LowSkinny = Skinny<T, LAY, FR, 1, 1, AE ? GMM_A_ELEMENTS : GMM_A_STAGED, FR <= 2 ? 4 : 2>;
 
 template <typename T, typename S, int WAVES>
 __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyShared<S, WAVES>& shared) {
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a)
 // at a time 8192 x 4096 took 65 us, five trips to memory one after the other for each.  NK: steps of 32 of the rank that are held.
 template <typename T, int LAY, int NK, bool WIDE>
 __global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_kernel(const LoraArgs a) {
-  using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, false, 1>;
+  using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, GMM_A_STAGED, 1>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int first = (blockIdx.x * kWaves + wave) * 16;
@@ -481,7 +481,7 @@ constexpr int kMaxChunk = 4096;
 // out[i] += q^T p over a chunk of adapter i's rows: R rows, a strip of 128 columns of p, the contraction along p's rows.
 template <typename T, int MF, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args) {
-  using S = Skinny<T, GMM_W_ROWS, 8, MF, 2, false, 2>;
+  using S = Skinny<T, GMM_W_ROWS, 8, MF, 2, GMM_A_STAGED, 2>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   __shared__ SkinnyShared<S, kWaves> shared;
   __shared__ int32_t row_at[kMaxChunk];
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
 #pragma unroll
         for (int q = 0; q < 4; ++q) step.w[r][q] = k + 8 * g + r < rows ? step.w[r][q] : 0u;
     }
-    s.template multiply<MF>(step, acc);
+    s.template multiply<MF>(step, k, rows, acc);
     __builtin_amdgcn_sched_barrier(0);
   };
   f32x4 acc[MF][FR];

@@ -14,6 +14,9 @@
 // A goes through LDS as well, for the same reason.  Its rows that do not exist read as zeros and cost no access.  LDS is a wave's own
 // here: its instructions run in order, nobody waits for anybody.  The waves of a workgroup share the range of k and add up in LDS.
 #pragma once
+#ifndef ST_4
+#define ST_4 2
+#endif
 #include "gmm_elem.h"
 
 namespace gmm {
@@ -54,9 +57,12 @@ __device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
 
 // One strip of columns of one product, by one wave.
 //   FR: products of 16 columns (GMM_W_ROWS: 8; GMM_W_COLS, GMM_W_THIN: 1, 2, 4; GMM_W_ANY: 1, 8).
-//   MF: sixteens of rows.  NA: planes of A (2: A = high + low).  AE: rows of A are read element by element (no alignment).
-//   ST: steps in flight.
-template <typename T, int LAY, int FR_, int MF, int NA, bool AE, int ST>
+//   MF: sixteens of rows.  NA: planes of A (2: A = high + low).  AM: how A comes (GMM_A_..).  ST: steps in flight.
+constexpr int GMM_A_STAGED = 0;      // from memory, 16 bytes at a time
+constexpr int GMM_A_ELEMENTS = 1;    // from memory, element by element (no alignment)
+constexpr int GMM_A_RESIDENT = 2;    // lies in LDS
+
+template <typename T, int LAY, int FR_, int MF, int NA, int AM, int ST>
 struct Skinny {
   static constexpr int FR = FR_;
   static constexpr int KS = LAY == GMM_W_COLS ? 64 : 32;      // k of a step
@@ -67,11 +73,10 @@ struct Skinny {
   static constexpr int WL = LAY == GMM_W_COLS ? 2 * FR : LAY == GMM_W_THIN ? FR : LAY == GMM_W_ROWS || FR == 8 ? 8 : 1;   // loads of W
   static constexpr int AL = MF * KH;                          // loads of a plane of A
   static constexpr int W_BYTES = LAY == GMM_W_COLS ? 128 * COLUMNS : LAY == GMM_W_THIN ? 1024 * FR : 0;
-  static constexpr int PLANE_BYTES = AE ? 0 : 32 * MF * KS;
+  static constexpr int PLANE_BYTES = AM == GMM_A_STAGED ? 32 * MF * KS : 0;
   static constexpr int LDS_BYTES = W_BYTES + NA * PLANE_BYTES;      // of a wave
   static_assert(LAY != GMM_W_ROWS || FR == 8, "");
   static_assert(LAY != GMM_W_ANY || FR == 1 || FR == 8, "");
-  static_assert(!AE || LAY == GMM_W_ANY, "");
 
   __amdgpu_buffer_rsrc_t w_buf, a_buf;
   char* lds;
@@ -83,8 +88,10 @@ struct Skinny {
   int w_half;             // and where it begins
   uint32_t a_at[AL];      // byte offset of the lane's rows of A, kNowhere: no such row
   uint32_t a_plane;       // bytes from the high to the low plane
+  const char* resident;   // GMM_A_RESIDENT: row 0 of the high plane, from k = resident_k on,
+  int pitch, resident_k, resident_rows;   // bytes from one row to the next, number of rows
 
-  struct Step { u32x4 w[WL]; u32x4 a[NA][AL]; };
+  struct Step { u32x4 w[WL]; u32x4 a[AM == GMM_A_RESIDENT ? 1 : NA][AL]; };
 
   static __device__ __forceinline__ uint32_t element(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
     return uint32_t(uint16_t(__builtin_amdgcn_raw_buffer_load_b16(buf, int(at), 0, 0)));
@@ -121,8 +128,8 @@ struct Skinny {
   __device__ __forceinline__ void set_rows(F&& at) {
 #pragma unroll
     for (int i = 0; i < AL; ++i) {
-      const uint32_t from = at(AE ? 16 * i + (lane & 15) : ROWS_AT_ONCE * i + lane / CH);
-      a_at[i] = from == kNowhere || AE ? from : from + lane % CH * 16;
+      const uint32_t from = at(AM == GMM_A_ELEMENTS ? 16 * i + (lane & 15) : ROWS_AT_ONCE * i + lane / CH);
+      a_at[i] = from == kNowhere || AM == GMM_A_ELEMENTS ? from : from + lane % CH * 16;
     }
   }
 
@@ -181,11 +188,12 @@ struct Skinny {
 
   template <int M>
   __device__ __forceinline__ void load_a(Step& s, int k, int end) const {
+    if constexpr (AM == GMM_A_RESIDENT) return;
 #pragma unroll
     for (int i = 0; i < M * KH; ++i)
 #pragma unroll
       for (int p = 0; p < NA; ++p) {
-        if constexpr (AE) {
+        if constexpr (AM == GMM_A_ELEMENTS) {
           const int kl = k + 8 * (lane >> 4);
           const uint32_t at = a_at[i] + p * a_plane + uint32_t(kl) * 2;
 #pragma unroll
@@ -213,7 +221,7 @@ struct Skinny {
   static __device__ __forceinline__ int chunk_at(int r, int c) { return r * 16 * CH + 16 * (CH == 8 ? c ^ (r >> 1 & 7) : c ^ (r >> 2 & 3)); }
 
   template <int M>
-  __device__ __forceinline__ void multiply(const Step& s, f32x4 (&acc)[MF][FR]) const {
+  __device__ __forceinline__ void multiply(const Step& s, int k, int end, f32x4 (&acc)[MF][FR]) const {
     const int j = lane & 15, g = lane >> 4;
     lds_order();
     if constexpr (LAY == GMM_W_COLS)
@@ -222,7 +230,7 @@ struct Skinny {
     if constexpr (LAY == GMM_W_THIN)
 #pragma unroll
       for (int i = 0; i < WL; ++i) *reinterpret_cast<u32x4*>(lds + 1024 * i + 16 * lane) = s.w[i];
-    if constexpr (!AE)
+    if constexpr (AM == GMM_A_STAGED)
 #pragma unroll
       for (int i = 0; i < M * KH; ++i)
 #pragma unroll
@@ -236,7 +244,12 @@ struct Skinny {
       for (int m = 0; m < M; ++m)
 #pragma unroll
         for (int p = 0; p < NA; ++p) {
-          if constexpr (AE) a[m][p] = s.a[p][m];
+          if constexpr (AM == GMM_A_ELEMENTS) a[m][p] = s.a[p][KH * m + h];
+          else if constexpr (AM == GMM_A_RESIDENT) {
+            const int at = k + 8 * (4 * h + g);      // zeros behind the end, whose W reads as zeros: what lies there may be no number
+            a[m][p] = *reinterpret_cast<const u32x4*>(resident + p * a_plane + min(16 * m + j, resident_rows - 1) * pitch + (at < end ? at - resident_k : 0) * 2);
+            a[m][p] = at < end ? a[m][p] : u32x4{0, 0, 0, 0};
+          }
           else a[m][p] = *reinterpret_cast<const u32x4*>(lds + W_BYTES + p * PLANE_BYTES + chunk_at(16 * m + j, 4 * h + g));
         }
 #pragma unroll
@@ -267,22 +280,32 @@ struct Skinny {
   // acc += A[:, k] W[k] over every WAVES-th step of begin .. end.  Steps past the end load nothing: no branch stands between the loads in
   // flight, and nothing moves past the barriers: moved loads would be waited for together.
   template <int M, int WAVES>
-  __device__ __forceinline__ void steps(int begin, int end, f32x4 (&acc)[MF][FR]) const {
-    constexpr int NEXT = WAVES * KS;
-    Step step[ST];
+  __device__ __forceinline__ void prime(Step (&step)[ST], int begin, int end) const {
 #pragma unroll
     for (int u = 0; u < ST; ++u) {
-      load<M>(step[u], begin + u * NEXT, end);
+      load<M>(step[u], begin + u * WAVES * KS, end);
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+
+  template <int M, int WAVES>
+  __device__ __forceinline__ void primed(Step (&step)[ST], int begin, int end, f32x4 (&acc)[MF][FR]) const {
+    constexpr int NEXT = WAVES * KS;
     for (int k = begin; k < end; k += ST * NEXT)
 #pragma unroll
       for (int u = 0; u < ST; ++u) {
-        multiply<M>(step[u], acc);
+        multiply<M>(step[u], k + u * NEXT, end, acc);
         __builtin_amdgcn_sched_barrier(0);
         load<M>(step[u], k + (ST + u) * NEXT, end);
         __builtin_amdgcn_sched_barrier(0);
       }
+  }
+
+  template <int M, int WAVES>
+  __device__ __forceinline__ void steps(int begin, int end, f32x4 (&acc)[MF][FR]) const {
+    Step step[ST];
+    prime<M, WAVES>(step, begin, end);
+    primed<M, WAVES>(step, begin, end, acc);
   }
 
   // The part of wave `wave` of WAVES of the product over begin .. end: the waves' steps lie side by side in memory.  rows: how many there
@@ -301,8 +324,8 @@ struct Skinny {
 };
 
 // A strip of a matrix that is large.
-template <typename T, int LAY, int MF, int NA>
-using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, MF, NA, LAY == GMM_W_ANY, 2>;
+template <typename T, int LAY, int MF, int NA, int AM = LAY == GMM_W_ANY ? GMM_A_ELEMENTS : GMM_A_STAGED>
+using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, MF, NA, AM, MF == 4 ? ST_4 : 2>;
 
 template <int MF, int FR>
 __device__ __forceinline__ void clear(f32x4 (&acc)[MF][FR]) {
@@ -322,11 +345,12 @@ struct SkinnySums {
 #pragma unroll
     for (int i = 0; i < FR; ++i) at[wave][i][lane] = acc[i];
   }
-  // Rows 4 g .. 4 g + 3 of the column that product i has in lane j.
+  // Rows 4 g .. 4 g + 3 of the column that product i has in lane j; of one wave alone, or the sum over all.
+  __device__ __forceinline__ f32x4 of(int wave, int i, int j, int g) const { return at[wave][i][16 * g + j]; }
   __device__ __forceinline__ f32x4 get(int i, int j, int g) const {
-    f32x4 s = at[0][i][16 * g + j];
+    f32x4 s = of(0, i, j, g);
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s += at[w][i][16 * g + j];
+    for (int w = 1; w < WAVES; ++w) s += of(w, i, j, g);
     return s;
   }
 };

@@ -9,6 +9,7 @@ grouped product of one group and two kernels for the adapters.  Registered as to
 """
 from __future__ import annotations
 
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -20,32 +21,40 @@ from .kernels import _dtype_code, _guard, _require_gpu
 FEW_TOKENS = 64
 MAX_RANK = 256
 MAX_ADAPTERS = 1022
+_DTYPES = (torch.bfloat16, torch.float16)
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter: torch.Tensor,
            scale: Optional[torch.Tensor]) -> None:
     if x.dim() != 2 or weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
         raise RuntimeError("lora_linear takes x [T, K], weight [K, N], lora_a [L, K, R] and lora_b [L, R, N]")
-    if x.dtype not in (torch.bfloat16, torch.float16) or not x.dtype == weight.dtype == lora_a.dtype == lora_b.dtype:
+    dtype = x.dtype
+    if dtype not in _DTYPES or not dtype == weight.dtype == lora_a.dtype == lora_b.dtype:
         raise RuntimeError("x, weight, lora_a and lora_b have to be of one type, bfloat16 or float16, got "
                            f"{x.dtype}, {weight.dtype}, {lora_a.dtype}, {lora_b.dtype}")
-    L, K, R = lora_a.shape
-    if x.size(1) != weight.size(0) or K != x.size(1) or lora_b.shape != (L, R, weight.size(1)):
+    (T, K), (inner, N), (L, Ka, R) = x.shape, weight.shape, lora_a.shape
+    if K != inner or Ka != K or lora_b.shape != (L, R, N):
         raise RuntimeError("shapes do not chain: x [T, K], weight [K, N], lora_a [L, K, R], lora_b [L, R, N]")
     if not 1 <= R <= MAX_RANK:
         raise RuntimeError(f"the adapters' rank must be in [1, {MAX_RANK}], got {R}")
     if L > MAX_ADAPTERS:
         raise RuntimeError(f"Can't process more than {MAX_ADAPTERS} adapters")
-    if adapter.dtype != torch.int32 or adapter.dim() != 1 or adapter.size(0) != x.size(0) or not adapter.is_contiguous():
+    if adapter.dtype != torch.int32 or adapter.shape != (T,) or not adapter.is_contiguous():
         raise RuntimeError("adapter has to be a contiguous 1D int32 tensor with one number a row of x")
-    if scale is not None and (scale.dtype != torch.float32 or scale.dim() != 1 or scale.size(0) != L or not scale.is_contiguous()):
-        raise RuntimeError("scale has to be a contiguous 1D float32 tensor with one number an adapter")
-    if scale is not None and scale.requires_grad:
-        raise RuntimeError("scale has no gradient: it must not require one")
-    _require_gpu(x, weight, lora_a, lora_b, adapter, scale)
-    if any(t is not None and t.device != x.device for t in (weight, lora_a, lora_b, adapter, scale)):
+    device = x.device
+    if scale is not None:
+        if scale.dtype != torch.float32 or scale.shape != (L,) or not scale.is_contiguous():
+            raise RuntimeError("scale has to be a contiguous 1D float32 tensor with one number an adapter")
+        if scale.requires_grad:
+            raise RuntimeError("scale has no gradient: it must not require one")
+        if scale.device != device:
+            raise RuntimeError("all operands must be on the same device")
+    _require_gpu(x)
+    if weight.device != device or lora_a.device != device or lora_b.device != device or adapter.device != device:
         raise RuntimeError("all operands must be on the same device")
-    is_row_major(weight)
+    row, column = weight.stride()
+    if not (column == 1 and row >= N or row == 1 and column >= K):
+        is_row_major(weight)      # empty and single-element dimensions, or the error
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -59,42 +68,50 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device: int, T: int, K: int, N: int, R: int) -> int:
+    return _lib.load().gmm_lora_workspace_bytes(T, K, N, R)
+
+
 def _forward_now(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter: torch.Tensor,
-                 scale: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The result, and x @ lora_a of the rows that have an adapter, [T, R] float32."""
-    (T, K), N = x.shape, weight.size(1)
+                 scale: Optional[torch.Tensor], save: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The result, and (with `save`) x @ lora_a of the rows that have an adapter, [T, R] float32."""
+    (T, K), N, dev = x.shape, weight.size(1), x.device
     L, _, R = lora_a.shape
-    out = torch.empty(T, N, device=x.device, dtype=x.dtype)
-    low = torch.empty(T, R, device=x.device, dtype=torch.float32)
+    out = torch.empty(T, N, device=dev, dtype=x.dtype)
+    low = torch.empty(T, R, device=dev, dtype=torch.float32) if save else None
     lib = _lib.load()
     with _guard(x):
-        stream = kernels.current_stream(x.device)
-        nbytes = lib.gmm_lora_workspace_bytes(T, K, N, R)
-        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-        code = _dtype_code(x.dtype)
+        stream, code = kernels.current_stream(dev), _dtype_code(x.dtype)
+        nbytes = _workspace_bytes(dev.index, T, K, N, R)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        adapters = lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr(), _ptr(scale), out.data_ptr(), _ptr(low)
+        strides = (*lora_a.stride(), *lora_b.stride(), N, code, ws.data_ptr(), nbytes, stream)
         rc = _lib.ERR_UNSUPPORTED
         if T <= FEW_TOKENS:
-            rc = lib.gmm_lora_linear(x.data_ptr(), weight.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr(), _ptr(scale),
-                                     out.data_ptr(), low.data_ptr(), T, K, N, R, L, x.stride(0), *weight.stride(), *lora_a.stride(),
-                                     *lora_b.stride(), N, code, ws.data_ptr(), nbytes, stream)
+            rc = lib.gmm_lora_linear(x.data_ptr(), weight.data_ptr(), *adapters, T, K, N, R, L, x.stride(0), *weight.stride(), *strides)
         if rc == _lib.ERR_UNSUPPORTED:
             if K == 0:
                 out.zero_()
             elif out.numel():
                 kernels._launch_now(kernels.V_3D3D, x.unsqueeze(0), weight.unsqueeze(0), None, out.unsqueeze(0))
-            rc = lib.gmm_lora_add(x.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr(), _ptr(scale), out.data_ptr(),
-                                  low.data_ptr(), T, K, N, R, L, x.stride(0), *lora_a.stride(), *lora_b.stride(), N, code, ws.data_ptr(),
-                                  nbytes, stream)
+            rc = lib.gmm_lora_add(x.data_ptr(), *adapters, T, K, N, R, L, x.stride(0), *strides)
     _lib.check(rc, "lora_linear")
     return out, low
 
 
-_forward_op = torch.library.custom_op("grouped_mm_bf16_amd::lora", mutates_args=())(_forward_now)
+def _forward_functional(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter: torch.Tensor,
+                        scale: Optional[torch.Tensor], save: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    out, low = _forward_now(x, weight, lora_a, lora_b, adapter, scale, save)
+    return out, low if save else x.new_empty(0, lora_a.size(2), dtype=torch.float32)
+
+
+_forward_op = torch.library.custom_op("grouped_mm_bf16_amd::lora", mutates_args=())(_forward_functional)
 
 
 @_forward_op.register_fake
-def _forward_fake(x, weight, lora_a, lora_b, adapter, scale):
-    return x.new_empty(x.size(0), weight.size(1)), x.new_empty(x.size(0), lora_a.size(2), dtype=torch.float32)
+def _forward_fake(x, weight, lora_a, lora_b, adapter, scale, save):
+    return x.new_empty(x.size(0), weight.size(1)), x.new_empty(x.size(0) if save else 0, lora_a.size(2), dtype=torch.float32)
 
 
 def _grad_now(x: torch.Tensor, dy: torch.Tensor, low: torch.Tensor, u: torch.Tensor, adapter: torch.Tensor, scale: Optional[torch.Tensor],
@@ -110,7 +127,7 @@ def _grad_now(x: torch.Tensor, dy: torch.Tensor, low: torch.Tensor, u: torch.Ten
         stream, code = kernels.current_stream(x.device), _dtype_code(x.dtype)
         if need_a and not u.numel() and T:
             u = torch.empty(T, R, device=x.device, dtype=torch.float32)
-            nbytes = lib.gmm_lora_workspace_bytes(T, N, K, R)
+            nbytes = _workspace_bytes(x.device.index, T, N, K, R)
             ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
             sl, sr, sn = lora_b.stride()
             rc = lib.gmm_lora_add(dy.data_ptr(), lora_b.data_ptr(), None, adapter.data_ptr(), None, None, u.data_ptr(), T, N, 0, R, L,
@@ -144,7 +161,7 @@ class _Lora(torch.autograd.Function):
     def forward(ctx, x, weight, lora_a, lora_b, adapter, scale):
         x = _rows(x)
         impl = _forward_op if torch.compiler.is_compiling() else _forward_now
-        out, low = impl(x, weight, lora_a, lora_b, adapter, scale)
+        out, low = impl(x, weight, lora_a, lora_b, adapter, scale, any(ctx.needs_input_grad[2:4]))
         ctx.save_for_backward(x, weight, lora_a, lora_b, adapter, scale, low)
         return out
 
@@ -155,9 +172,12 @@ class _Lora(torch.autograd.Function):
         dy = _rows(grad)
         compiling = torch.compiler.is_compiling()
         dx = dw = da = db = None
-        u = low.new_empty(0)
+        low = low if low is not None else x.new_empty(0, dtype=torch.float32)
+        u = x.new_empty(0, dtype=torch.float32)
         if need_x:
-            dx, u = (_forward_op if compiling else _forward_now)(dy, weight.t(), lora_b.transpose(1, 2), lora_a.transpose(1, 2), adapter, scale)
+            dx, u_now = (_forward_op if compiling else _forward_now)(dy, weight.t(), lora_b.transpose(1, 2), lora_a.transpose(1, 2), adapter, scale,
+                                                                         need_a)
+            u = u_now if need_a else u
         if need_a or need_b:
             da, db = (_grad_op if compiling else _grad_now)(x, dy, low, u, adapter, scale, lora_a, lora_b, need_a, need_b)
         if need_w:
@@ -179,7 +199,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     The rank-sized products stay in float32; the result is rounded once up to ``FEW_TOKENS`` tokens, above that weight's product as well.
     """
     _check(x, weight, lora_a, lora_b, adapter, scale)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, lora_a, lora_b)):
+    if (x.requires_grad or weight.requires_grad or lora_a.requires_grad or lora_b.requires_grad) and torch.is_grad_enabled():
         return _Lora.apply(x, weight, lora_a, lora_b, adapter, scale)
     impl = _forward_op if torch.compiler.is_compiling() else _forward_now
-    return impl(_rows(x), weight, lora_a, lora_b, adapter, scale)[0]
+    return impl(_rows(x), weight, lora_a, lora_b, adapter, scale, False)[0]

@@ -14,6 +14,7 @@ dispatches to it while a model around it is being traced or compiled.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -389,6 +390,11 @@ def moe_forward(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor
 FEW_TOKENS = 64   # four products of 16 rows with everything that is read of a matrix
 
 
+@functools.lru_cache(maxsize=4096)
+def _few_workspace_bytes(device: int, T: int, E: int, top_k: int, H: int, inner: int) -> int:
+    return _lib.load().gmm_moe_few_workspace_bytes(T, E, top_k, H, inner)
+
+
 def _few_now(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, top_k: int, kind: int,
              renormalize: bool) -> torch.Tensor:
     T, H = x.shape
@@ -396,7 +402,7 @@ def _few_now(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor, w
     out = torch.empty(T, H, device=x.device, dtype=x.dtype)
     lib = _lib.load()
     with _guard(x):
-        nbytes = lib.gmm_moe_few_workspace_bytes(T, E, top_k, H, inner)
+        nbytes = _few_workspace_bytes(x.device.index, T, E, top_k, H, inner)
         if nbytes < 0:
             raise RuntimeError("moe_forward_few: sizes out of range")
         ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
@@ -426,33 +432,36 @@ def moe_forward_few(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Te
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
         raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")
-    if w_up.dim() != 3 or w_down.dim() != 3 or w_up.size(0) != router_logits.size(1) or w_down.size(0) != w_up.size(0):
+    (T, H), E = x.shape, router_logits.size(1)
+    if w_up.dim() != 3 or w_down.dim() != 3 or w_up.size(0) != E or w_down.size(0) != E:
         raise RuntimeError("w_up [E, H, I or 2I] and w_down [E, I, H] must agree with router_logits on E")
     if activation not in ACTIVATIONS:
         raise RuntimeError(f"unknown activation {activation!r}; have {sorted(ACTIVATIONS)}")
-    if interleaved and activation != "swiglu":
+    kind = ACTIVATIONS[activation]
+    if interleaved and not kind:
         raise RuntimeError("interleaved weights go with the swiglu activation")
-    if activation == "swiglu" and w_up.size(2) % (128 if interleaved else 2):
+    (_, up_rows, columns), (_, inner, down_columns) = w_up.shape, w_down.shape
+    if kind and columns % (128 if interleaved else 2):
         raise RuntimeError("swiglu needs an even number of columns, interleaved weights whole blocks of 128")
-    inner = w_up.size(2) // 2 if ACTIVATIONS[activation] else w_up.size(2)
-    if w_up.size(1) != x.size(1) or w_down.size(1) != inner or w_down.size(2) != x.size(1):
+    if up_rows != H or inner * (1 + kind) != columns or down_columns != H:
         raise RuntimeError("weight shapes do not chain: x [T, H], w_up [E, H, I or 2I], w_down [E, I, H]")
-    if x.size(0) > FEW_TOKENS:
-        raise RuntimeError(f"moe_forward_few takes up to {FEW_TOKENS} tokens, got {x.size(0)}: use moe_forward")
-    if x.dtype not in (torch.bfloat16, torch.float16) or w_up.dtype != x.dtype or w_down.dtype != x.dtype:
-        raise RuntimeError(f"x, w_up and w_down have to be of one type, bfloat16 or float16, got {x.dtype}, {w_up.dtype}, {w_down.dtype}")
+    if T > FEW_TOKENS:
+        raise RuntimeError(f"moe_forward_few takes up to {FEW_TOKENS} tokens, got {T}: use moe_forward")
+    dtype = x.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float16 or w_up.dtype != dtype or w_down.dtype != dtype:
+        raise RuntimeError(f"x, w_up and w_down have to be of one type, bfloat16 or float16, got {dtype}, {w_up.dtype}, {w_down.dtype}")
     _dtype_code(router_logits.dtype)
-    _require_gpu(x, router_logits, w_up, w_down)
-    if not x.device == router_logits.device == w_up.device == w_down.device:
+    _require_gpu(x)
+    device = x.device
+    if router_logits.device != device or w_up.device != device or w_down.device != device:
         raise RuntimeError("x, router_logits, w_up and w_down must be on the same device")
-    E = router_logits.size(1)
     if not 1 <= top_k <= min(E, 32):
         raise RuntimeError(f"top_k must be in [1, min(experts, 32)], got {top_k} for {E} experts")
     if E > 1023:
         raise RuntimeError("Can't process more than 1024 groups")
-    if x.numel() and x.stride(1) != 1 and x.size(1) > 1 or x.size(0) > 1 and not x.size(1) <= x.stride(0) <= 1 << 23:
+    if not (x.is_contiguous() or T == 0 or H == 0) and (x.stride(1) != 1 and H > 1 or T > 1 and not H <= x.stride(0) <= 1 << 23):
         x = x.contiguous()
-    if router_logits.numel() and (router_logits.stride(1) != 1 and E > 1 or router_logits.stride(0) < E):
+    if not (router_logits.is_contiguous() or T == 0) and (router_logits.stride(1) != 1 and E > 1 or router_logits.stride(0) < E):
         router_logits = router_logits.contiguous()
     impl = _few_op if torch.compiler.is_compiling() else _few_now
-    return impl(x, router_logits, w_up, w_down, top_k, 2 if interleaved else ACTIVATIONS[activation], bool(renormalize))
+    return impl(x, router_logits, w_up, w_down, top_k, 2 if interleaved else kind, bool(renormalize))

@@ -18,25 +18,27 @@ MAX_WIDTH = 16384
 
 def _check(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> torch.dtype:
     """The rules of :func:`layer_norm`; returns the type of weight and bias."""
-    _require_gpu(x, weight, bias)
-    _dtype_code(x.dtype)
+    _require_gpu(x)
+    dtype = x.dtype
+    _dtype_code(dtype)
     if x.dim() < 1:
         raise RuntimeError("layer_norm takes a tensor of at least one dimension")
     width = x.size(-1)
     if width > MAX_WIDTH:
         raise RuntimeError(f"layer_norm takes rows of up to {MAX_WIDTH} elements, got {width}")
-    dtype = None
-    for name, t in (("weight", weight), ("bias", bias)):
+    param_dtype = None
+    for t in (weight, bias):
         if t is None:
             continue
-        if t.dim() != 1 or t.size(0) != width or not t.is_contiguous():
+        name = "bias" if t is bias else "weight"
+        if t.shape != (width,) or not t.is_contiguous():
             raise RuntimeError(f"layer_norm: {name} has to be a contiguous 1D tensor of {width} elements, got {tuple(t.shape)}")
         if t.device != x.device:
             raise RuntimeError(f"layer_norm: {name} has to be on {x.device}, got {t.device}")
-        if t.dtype not in (x.dtype, torch.float32) or dtype not in (None, t.dtype):
-            raise RuntimeError(f"layer_norm: weight and bias have to be {x.dtype} or both float32, got {t.dtype}")
-        dtype = t.dtype
-    return dtype or x.dtype
+        if t.dtype != dtype and t.dtype != torch.float32 or param_dtype is not None and t.dtype != param_dtype:
+            raise RuntimeError(f"layer_norm: weight and bias have to be {dtype} or both float32, got {t.dtype}")
+        param_dtype = t.dtype
+    return param_dtype or dtype
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -53,12 +55,12 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _forward_now(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
-                 save: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The norm of a matrix's rows, and the rows' mean and rstd [2, rows] (empty unless `save`)."""
+                 save: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The norm of a matrix's rows, and (with `save`) the rows' mean and rstd [2, rows]."""
     code = _dtype_code(weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype)
     rows, width = x.shape
     out = torch.empty(rows, width, device=x.device, dtype=x.dtype)
-    stats = torch.empty(2, rows if save else 0, device=x.device, dtype=torch.float32)
+    stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if save else None
     mean = stats.data_ptr() if save else None
     with _guard(x):
         rc = _lib.load().gmm_layer_norm(x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), mean, mean + 4 * rows if save else None,
@@ -68,12 +70,18 @@ def _forward_now(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional
     return out, stats
 
 
-_forward_op = torch.library.custom_op("grouped_mm_bf16_amd::layer_norm", mutates_args=())(_forward_now)
+def _forward_functional(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
+                        save: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    out, stats = _forward_now(x, weight, bias, eps, save)
+    return out, stats if save else x.new_empty(0, dtype=torch.float32)
+
+
+_forward_op = torch.library.custom_op("grouped_mm_bf16_amd::layer_norm", mutates_args=())(_forward_functional)
 
 
 @_forward_op.register_fake
 def _forward_fake(x, weight, bias, eps, save):
-    return x.new_empty(x.shape), x.new_empty(2, x.size(0) if save else 0, dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty((2, x.size(0)) if save else (0,), dtype=torch.float32)
 
 
 def _backward_now(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor, param_dtype: torch.dtype,
@@ -137,8 +145,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x [..., W], bf16, fp16 or fp32, W up to 16384; weight and bias [W] in x's type or in float32 (None: ones, zeros).  Sums in fp32, one
     rounding.  A matrix whose rows lie apart is read as it is; other tensors are copied unless they are contiguous.
     """
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if (x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, eps)
     _check(x, weight, bias)
     impl = _forward_op if torch.compiler.is_compiling() else _forward_now
-    return impl(_rows(x), weight, bias, float(eps), False)[0].reshape(x.shape)
+    out = impl(_rows(x), weight, bias, float(eps), False)[0]
+    return out if x.dim() == 2 else out.reshape(x.shape)

@@ -305,10 +305,10 @@ def test_on_another_stream_and_in_a_graph(T):
 def test_compiled_ops_agree():
     x, weight, a, b, adapter, scale = make(70, 128, 64, 8, 3)
     ops = torch.ops.grouped_mm_bf16_amd
-    out, low = ops.lora(x, weight, a, b, adapter, scale)
+    out, low = ops.lora(x, weight, a, b, adapter, scale, True)
     assert torch.equal(out, lora.lora_linear(x, weight, a, b, adapter, scale))
     adapter.clamp_(min=0)       # rows without an adapter leave their part of `low` as it was
-    torch.library.opcheck(ops.lora, (x, weight, a, b, adapter, scale), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(ops.lora, (x, weight, a, b, adapter, scale, True), test_utils=("test_schema", "test_faketensor"))
     dy = torch.ones(70, 64, dtype=BF, device=DEV)
     torch.library.opcheck(ops.lora_grad, (x, dy, low, low.new_empty(0), adapter, scale, a, b, True, True),
                           test_utils=("test_schema", "test_faketensor"))
