@@ -22,6 +22,7 @@ namespace {
 using namespace gmm;
 
 constexpr int kFewRows = 64;
+constexpr int kSingleRows = 256;       // up to which rows are taken one at a time: they are likely to be of different adapters
 constexpr int kMaxRank = 256;
 constexpr int kMaxAdapters = 1022;     // one more bin of the sort holds the rows without an adapter
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
@@ -49,6 +50,7 @@ struct LoraArgs {
   int32_t rows, K, N, R, L;
   int32_t strip_rows, low_parts, low_k, low_tiles;   // rows of a strip; parts of K and their length; strips of columns of A
   int32_t base_parts, base_k, base_tiles, low_groups, pitch, strips;
+  int32_t keep;            // x @ A of one part goes where the second product wants it
 };
 
 __device__ __forceinline__ bool has_adapter(int id, int L) { return id >= 0 && id < L; }
@@ -58,47 +60,110 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix(const Matrices& m, int 
   return buffer(static_cast<const T*>(m.at) + which * m.sg, m.bytes);
 }
 
-// low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows; one adapter of theirs after the other.
+// Many rows: low of a row as the operand of the second product, times scale: two 16-bit values each, [2][rows][pitch], zeros past the rank;
+// and as it is where that is wanted.
+template <typename T>
+__device__ __forceinline__ void keep_low(const LoraArgs& a, int row, int r, float v, float scale) {
+  if (a.low_out && r < a.R) a.low_out[int64_t(row) * a.R + r] = v;
+  if (!a.planes) return;
+  T* const at = static_cast<T*>(a.planes) + int64_t(row) * a.pitch + r;
+  split(v * scale, at[0], at[int64_t(a.rows) * a.pitch]);
+}
+
+// low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows.  Of rows with different adapters one adapter comes
+// after the other; their steps are one sequence, so that the next adapter's loads are on their way while the last one's are
+// multiplied (16 adapters a strip, drained each time: 1024 rows of 64 adapters 233 us, as one sequence see the plan below).
 template <typename T, int LAY, int FR, bool AE>
 using LowSkinny = Skinny<T, LAY, FR, 1, 1, AE ? GMM_A_ELEMENTS : GMM_A_STAGED, FR <= 2 ? 4 : 2>;
 
-template <typename T, typename S, int WAVES>
+// The adapters of a strip's rows, one after the other.
+struct Adapters {
+  uint32_t todo, mine;      // rows of adapters to come; of this one
+  int which;
+
+  __device__ __forceinline__ void next(int id) {
+    which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
+    mine = uint32_t(__ballot(id == which)) & 0xffffu;
+    todo &= ~mine;
+  }
+};
+
+template <typename T, typename S, int WAVES, int ST>
 __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyShared<S, WAVES>& shared) {
-  constexpr int FR = S::FR, OUT = S::COLUMNS;
+  constexpr int FR = S::FR, OUT = S::COLUMNS, NEXT = WAVES * S::KS;
   const int part = item % a.low_parts, tile = item / a.low_parts % a.low_tiles, row0 = item / a.low_parts / a.low_tiles * a.strip_rows;
   const int rows = min(a.strip_rows, a.rows - row0);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int id = j < rows ? a.adapter[row0 + j] : -1;
-  uint32_t todo = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
+  const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
+  if (!with) return;
   S s;
   s.lane = lane;
   s.lds = shared.wave[wave];
   s.a_buf = buffer(static_cast<const T*>(a.x) + row0 * a.x_ld, uint32_t(((rows - 1) * a.x_ld + a.K) * 2));
   s.a_plane = 0;
   s.set_columns(tile * OUT, a.R - tile * OUT, a.a.sk, a.a.sn);
-  const int from = part * a.low_k, to = min(a.K, from + a.low_k);
-  float* const low = a.low + (int64_t(part) * a.rows + row0) * a.R;
-  while (todo) {
-    const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
-    const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
-    todo &= ~mine;
-    s.w_buf = matrix<T>(a.a, which);
-    s.set_rows([&](int r) { return mine >> r & 1 ? uint32_t(r) * uint32_t(a.x_ld) * 2 : kNowhere; });
-    f32x4 acc[1][FR];
-    clear(acc);
-    s.template run<WAVES>(16, from, to, wave, acc);
-    __syncthreads();
-    shared.sums.put(wave, lane, acc[0]);
-    __syncthreads();
-    for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
-      const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
-      if (col >= a.R || !(mine >> 4 * og & 15)) continue;
-      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
+  const int to = min(a.K, (part + 1) * a.low_k), begin = part * a.low_k + wave * S::KS;
+  const int steps = max(1, (to - begin + NEXT - 1) / NEXT);      // of an adapter, of this wave
+  Adapters loading{with, 0, 0}, adding{with, 0, 0};
+  int load_step = 0, add_step = 0;
+  const auto open = [&] {
+    loading.next(id);
+    s.w_buf = matrix<T>(a.a, loading.which);
+    s.set_rows([&](int r) { return loading.mine >> r & 1 ? uint32_t(r) * uint32_t(a.x_ld) * 2 : kNowhere; });
+    load_step = 0;
+  };
+  const auto load = [&](typename S::Step& step) {
+    s.template load<1>(step, begin + load_step * NEXT, load_step < steps ? to : 0);
+    if (++load_step >= steps && loading.todo) open();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  typename S::Step step[ST];
+  f32x4 acc[1][FR], low[FR];
+  clear(acc);
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        if (mine >> (4 * og + v) & 1) low[(4 * og + v) * a.R + col] = h[v];
+  for (int i = 0; i < FR; ++i) low[i] = f32x4{0, 0, 0, 0};
+  open();
+#pragma unroll
+  for (int u = 0; u < ST; ++u) load(step[u]);
+  adding.next(id);
+  for (bool more = true; more;) {
+#pragma unroll
+    for (int u = 0; u < ST; ++u) {
+      s.template multiply<1>(step[u], 0, 0, acc);
+      // behind an adapter's last step its rows are taken over: what is no number in it stays with them.  (Steps behind all of them
+      // add zeros to a row that has been taken.)
+      if (++add_step == steps) {
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) low[i][v] = adding.mine >> (4 * g + v) & 1 ? acc[0][i][v] : low[i][v];
+        clear(acc);
+        add_step = 0;
+        if (adding.todo) adding.next(id);
+        else { adding.mine = 0; more = false; }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load(step[u]);
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  shared.sums.put(wave, lane, low);
+  __syncthreads();
+  float* const out = a.low + (int64_t(part) * a.rows + row0) * a.R;
+  for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
+    const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
+    const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int r = 4 * og + v;
+      if (!(with >> r & 1)) continue;
+      if (a.low_parts > 1 || !a.keep) {
+        if (col < a.R) out[r * a.R + col] = h[v];
+      } else if (col < a.pitch) {
+        keep_low<T>(a, row0 + r, col, h[v], a.scale ? a.scale[a.adapter[row0 + r]] : 1.0f);
+      }
+    }
   }
 }
 
@@ -106,7 +171,7 @@ template <typename T, int LAY, int FR, bool AE>
 __global__ void __launch_bounds__(kThreads, FR <= 2 ? 3 : 2) lora_low_kernel(const LoraArgs a) {
   using S = LowSkinny<T, LAY, FR, AE>;
   __shared__ SkinnyShared<S, kWaves> shared;
-  low_product<T, S, kWaves>(a, blockIdx.x, shared);
+  low_product<T, S, kWaves, FR <= 2 ? 4 : 2>(a, blockIdx.x, shared);
 }
 
 // A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
@@ -121,7 +186,7 @@ __global__ void __launch_bounds__(64 * few_waves(MF)) lora_few_kernel(const Lora
     SkinnyShared<S, WAVES> base;
     __device__ Shared() {}
   } shared;
-  if (int(blockIdx.x) < a.low_groups) return low_product<T, SA, WAVES>(a, blockIdx.x, shared.low);
+  if (int(blockIdx.x) < a.low_groups) return low_product<T, SA, WAVES, 4>(a, blockIdx.x, shared.low);
   const int item = blockIdx.x - a.low_groups, part = item % a.base_parts, tile = item / a.base_parts;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   S s;
@@ -163,8 +228,8 @@ __device__ __forceinline__ float low_sum(const LoraArgs& a, int row, int r) {
   return s;
 }
 
-// A few rows: y[t] = sum of the parts of x @ W + scale * low @ B.  A wave for 64 lanes' columns of one row: eight columns to a lane where B
-// is contiguous along them, else one.
+// One row after the other: y[t] = sum of the parts of x @ W (without any: what lies in y) + scale * low @ B.  A wave for 64 lanes' columns
+// of one row: eight columns to a lane where B is contiguous along them, else one.
 template <typename T, int LAY>
 __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   constexpr int W = LAY == GMM_W_ROWS ? 8 : 1;
@@ -174,6 +239,16 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   float y[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) y[i] = 0;
+  T* const out = static_cast<T*>(a.out) + t * a.out_ld + c;
+  if (c < a.N && a.base_parts == 0) {
+    if constexpr (W == 8) {
+      const Pack<T, 8> there = *reinterpret_cast<const Pack<T, 8>*>(out);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = there.get(i);
+    } else {
+      y[0] = widen(out[0]);
+    }
+  }
   if (c < a.N) {
     const float* base = a.base + int64_t(t) * a.N + c;
     const int64_t next = int64_t(a.rows) * a.N;
@@ -224,7 +299,6 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
 #pragma unroll
     for (int i = 0; i < W; ++i) y[i] += add[i];
   }
-  T* out = static_cast<T*>(a.out) + t * a.out_ld + c;
   if constexpr (W == 8) {
     *reinterpret_cast<Pack<T, 8>*>(out) = Pack<T, 8>::of(y);
   } else {
@@ -232,21 +306,14 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   }
 }
 
-// Many rows: the parts of x @ A summed, written out where that is wanted, and times scale as the operand of the second product: two 16-bit
-// values each, [2][rows][pitch], zeros past the rank and in rows without an adapter.
+// The parts of x @ A of many rows summed.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a) {
   const int64_t u = int64_t(blockIdx.x) * kThreads + threadIdx.x;
   const int row = int(u / a.pitch), r = int(u % a.pitch);
   if (row >= a.rows) return;
   const int id = a.adapter[row];
-  float v = 0;
-  if (r < a.R && has_adapter(id, a.L)) {
-    v = low_sum(a, row, r);
-    if (a.low_out) a.low_out[int64_t(row) * a.R + r] = v;
-    if (a.scale) v *= a.scale[id];
-  }
-  if (a.planes) split(v, static_cast<T*>(a.planes)[u], static_cast<T*>(a.planes)[int64_t(a.rows) * a.pitch + u]);
+  if (has_adapter(id, a.L)) keep_low<T>(a, row, r, r < a.R ? low_sum(a, row, r) : 0.0f, a.scale ? a.scale[id] : 1.0f);
 }
 
 // Many rows: y[t] += scale * low @ B.  A wave takes 16 rows and strips of 128 columns, one after the other; y is read and written where
@@ -320,58 +387,68 @@ __global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_ke
       acc[i] = mfma(T{}, l, b, acc[i]);
     }
   };
-  // rows of different adapters: one adapter after the other
-#pragma unroll 1
-  for (uint32_t todo = with; todo;) {
-    const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
-    const uint32_t mine = uint32_t(__ballot(id == which)) & 0xffffu;
-    todo &= ~mine;
-    s.w_buf = matrix<T>(a.b, which);
-    u32x4 h[NK], l[NK], w[NK][8];
-    u32x4 next[4];
-    const auto load_low = [&](int k) {
+  // strips, and in a strip the adapters of the rows, one after the other: one sequence
+  u32x4 h[NK], l[NK], w[NK][8], next[4];
+  const auto load_low = [&](int k) {
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int at = k + 32 * n < a.pitch ? k + 32 * n : 0;      // past the rank B's rows read as zeros
-        h[n] = *reinterpret_cast<const u32x4*>(high + at);
-        l[n] = *reinterpret_cast<const u32x4*>(low + at);
+    for (int n = 0; n < NK; ++n) {
+      const int at = k + 32 * n;      // of a lane's eight values none are there, or all
+      const bool in = at + 8 * g < a.pitch;
+      h[n] = *reinterpret_cast<const u32x4*>(high + (in ? at : -8 * g));
+      l[n] = *reinterpret_cast<const u32x4*>(low + (in ? at : -8 * g));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        h[n][q] = in ? h[n][q] : 0u;
+        l[n][q] = in ? l[n][q] : 0u;
       }
-    };
-    load_low(0);
-#pragma unroll
-    for (int n = 0; n < NK; ++n) load_b(w[n], 0, 32 * n);
-    load_y(next, 0, mine);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll 1
-    for (int tile = 0; tile < tiles; ++tile) {
-      f32x4 acc[FR];
-#pragma unroll
-      for (int i = 0; i < FR; ++i) acc[i] = f32x4{0, 0, 0, 0};
-#pragma unroll 1
-      for (int k = 0;;) {
-#pragma unroll
-        for (int n = 0; n < NK; ++n) multiply(w[n], h[n], l[n], acc);
-        k += 32 * NK;
-        if (k >= a.R) break;
-        load_low(k);
-#pragma unroll
-        for (int n = 0; n < NK; ++n) load_b(w[n], tile, k + 32 * n);
-      }
-      if (a.R > 32 * NK) load_low(0);
-      __builtin_amdgcn_sched_barrier(0);
-      const int ahead = tile + 1 < tiles ? tile + 1 : tile;
-#pragma unroll
-      for (int n = 0; n < NK; ++n) load_b(w[n], ahead, 32 * n);
-      __builtin_amdgcn_sched_barrier(0);
-      float now[4][FR];
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-#pragma unroll
-        for (int i = 0; i < FR; ++i) now[v][i] = widen(T{uint16_t(next[v][i / 2] >> 16 * (i & 1))}) + acc[i][v];
-      load_y(next, ahead, mine);
-      __builtin_amdgcn_sched_barrier(0);
-      store_y(now, tile, mine);
     }
+  };
+  load_low(0);
+  Adapters ahead{with, 0, 0};
+  int tile = 0;
+  ahead.next(id);
+  s.w_buf = matrix<T>(a.b, ahead.which);
+#pragma unroll
+  for (int n = 0; n < NK; ++n) load_b(w[n], 0, 32 * n);
+  load_y(next, 0, ahead.mine);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+  while (tile < tiles) {
+    const uint32_t mine = ahead.mine;
+    const int here = tile;
+    f32x4 acc[FR];
+#pragma unroll
+    for (int i = 0; i < FR; ++i) acc[i] = f32x4{0, 0, 0, 0};
+#pragma unroll 1
+    for (int k = 0;;) {
+#pragma unroll
+      for (int n = 0; n < NK; ++n) multiply(w[n], h[n], l[n], acc);
+      k += 32 * NK;
+      if (k >= a.R) break;
+      load_low(k);
+#pragma unroll
+      for (int n = 0; n < NK; ++n) load_b(w[n], here, k + 32 * n);
+    }
+    if (a.R > 32 * NK) load_low(0);
+    if (!ahead.todo) {
+      ahead.todo = with;
+      ++tile;
+    }
+    ahead.next(id);
+    s.w_buf = matrix<T>(a.b, ahead.which);
+    const int then = min(tile, tiles - 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) load_b(w[n], then, 32 * n);
+    __builtin_amdgcn_sched_barrier(0);
+    float now[4][FR];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int i = 0; i < FR; ++i) now[v][i] = widen(T{uint16_t(next[v][i / 2] >> 16 * (i & 1))}) + acc[i][v];
+    load_y(next, then, tile < tiles ? ahead.mine : 0);
+    __builtin_amdgcn_sched_barrier(0);
+    store_y(now, here, mine);
   }
 }
 
@@ -634,8 +711,6 @@ void cut(int64_t k, int64_t want, int64_t least, int32_t& parts, int32_t& each) 
   parts = each ? int32_t((k + each - 1) / each) : 1;
 }
 
-// Rows up to which x @ A is computed one row at a time, so that rows of different adapters are not in one another's way.
-constexpr int64_t kSingleRows = 256;
 
 struct LowPlan { int32_t strip_rows, parts, each; };
 
@@ -704,7 +779,18 @@ void set_low(LoraArgs& a, int columns) {
 }
 
 template <typename T>
-int launch_few(LoraArgs a, bool whole, int lay_b, hipStream_t stream) {
+int launch_finish(const LoraArgs& a, hipStream_t stream) {
+  int lay = layout_of_b(a.b, a.R, a.N);
+  if (lay == GMM_W_ROWS && !(aligned16(a.out) && multiple8(a.out_ld))) lay = GMM_W_ANY;       // eight columns of the result at a time
+  by_layout(lay, [&](auto l) {
+    constexpr int B = decltype(l)::value, W = B == GMM_W_ROWS ? 8 : 1;
+    hipLaunchKernelGGL((lora_finish_kernel<T, B>), dim3(unsigned(a.N ? (a.N + 64 * W - 1) / (64 * W) : 1), unsigned(a.rows)), dim3(64), 0, stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_few(LoraArgs a, bool whole, hipStream_t stream) {
   const int lay_w = layout_of(a.w, a.K, a.N, whole);
   const int lay_a = lay_w == GMM_W_ANY ? GMM_W_ANY : layout_of(a.a, a.K, a.R, whole);
   set_low(a, 16);
@@ -731,11 +817,7 @@ int launch_few(LoraArgs a, bool whole, int lay_b, hipStream_t stream) {
   if (lay_w == GMM_W_ROWS) with_a(rows);
   else if (lay_w == GMM_W_COLS) with_a(cols);
   else launch(any, any);
-  by_layout(lay_b, [&](auto l) {
-    constexpr int B = decltype(l)::value, W = B == GMM_W_ROWS ? 8 : 1;
-    hipLaunchKernelGGL((lora_finish_kernel<T, B>), dim3(unsigned((a.N + 64 * W - 1) / (64 * W)), unsigned(a.rows)), dim3(64), 0, stream, a);
-  });
-  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+  return launch_finish<T>(a, stream);
 }
 
 // Columns of a strip: as few as hold the rank.
@@ -772,15 +854,17 @@ int launch_low(LoraArgs& a, bool whole, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
-int64_t pitch_of(int64_t R) { return round_up(R, 32); }
+int64_t pitch_of(int64_t R) { return round_up(R, 16); }
 
 template <typename T>
 int launch_add(LoraArgs a, bool whole, hipStream_t stream) {
+  a.pitch = int(pitch_of(a.R));
+  a.keep = a.rows > kSingleRows;
   const int rc = launch_low<T>(a, whole, stream);
   if (rc != GMM_OK) return rc;
-  a.pitch = int(pitch_of(a.R));
+  if (!a.keep) return launch_finish<T>(a, stream);
   const unsigned blocks = unsigned((int64_t(a.rows) * a.pitch + kThreads - 1) / kThreads);
-  hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
+  if (a.low_parts > 1) hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
   if (a.N) {
     const int lay = layout_of_b(a.b, a.R, a.N);
     const int wide = aligned16(a.out) && multiple8(a.out_ld) && multiple8(a.N);
@@ -903,10 +987,8 @@ int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, 
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
   const bool whole = aligned16(x) && multiple8(g.x_ld);
-  int lay_b = layout_of_b(g.b, R, N);
-  if (lay_b == GMM_W_ROWS && !(aligned16(out) && multiple8(g.out_ld))) lay_b = GMM_W_ANY;       // eight columns of the result at a time
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GMM_DT_BF16 ? launch_few<Bf16>(g, whole, lay_b, s) : launch_few<F16>(g, whole, lay_b, s);
+  return dtype == GMM_DT_BF16 ? launch_few<Bf16>(g, whole, s) : launch_few<F16>(g, whole, s);
 }
 
 int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, void* out, float* low,
