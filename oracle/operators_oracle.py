@@ -116,10 +116,10 @@ def moe_layer(x, logits, w_up, w_down, top_k, kind, renormalize=True):
 
 
 # ------------------------------------------------------------------ projection with low-rank adapters
-def lora_linear(x, weight, lora_a, lora_b, adapter, scale=None):
+def lora_linear(x, weight, lora_a, lora_b, adapter, scale=None, dtype=None):
     """out and its bound: one rounding of the result, for more than 64 rows one of weight's product before it; fp32 sums; the rank-sized
     product as two 16-bit values."""
-    dtype, many = x.dtype, x.size(0) > 64
+    dtype, many = dtype or x.dtype, x.size(0) > 64
     x, weight, a, b = f64(x), f64(weight), f64(lora_a), f64(lora_b)
     two16 = {torch.bfloat16: 2.0 ** -15, torch.float16: 2.0 ** -21}[dtype]
     K, R = x.size(1), a.size(2)
@@ -138,10 +138,10 @@ def lora_linear(x, weight, lora_a, lora_b, adapter, scale=None):
     return out, err * (1 + UNIT[dtype]) + UNIT[dtype] * out.abs() + TINY[dtype]
 
 
-def lora_backward(dy, x, weight, lora_a, lora_b, adapter, scale=None):
+def lora_backward(dy, x, weight, lora_a, lora_b, adapter, scale=None, dtype=None):
     """(dx, its bound), (dweight, ..), (da, ..), (db, ..)."""
-    dtype = x.dtype
-    dx = lora_linear(dy, weight.mT, lora_b.mT, lora_a.mT, adapter, scale)
+    dtype = dtype or x.dtype
+    dx = lora_linear(dy, weight.mT, lora_b.mT, lora_a.mT, adapter, scale, dtype)
     dy, x, a, b = f64(dy), f64(x), f64(lora_a), f64(lora_b)
     two16 = {torch.bfloat16: 2.0 ** -15, torch.float16: 2.0 ** -21}[dtype]
     T, K, N = x.size(0), x.size(1), dy.size(1)
