@@ -54,6 +54,14 @@ template <> struct Pack<F16, 8> : Half8<F16> {
   __device__ __forceinline__ Pack(const Half8<F16>& h) : Half8<F16>(h) {}
 };
 
+// What lies at any address: the hardware asks for no alignment.
+template <typename V>
+__device__ __forceinline__ V unaligned(const void* p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+
 template <typename T> constexpr int kVector = 16 / int(sizeof(T));
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

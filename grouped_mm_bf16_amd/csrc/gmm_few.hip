@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1)
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.inner) continue;
       const auto result = [&](int c) {
-        return SIDE ? shared.sums.of(wave, S::product_of(c), S::lane_of(c), og) : shared.sums.get(S::product_of(c), S::lane_of(c), og);
+        const int at = S::position(c, a.inner - col);
+        return SIDE ? shared.sums.of(wave, S::product_of(at), S::lane_of(at), og) : shared.sums.get(S::product_of(at), S::lane_of(at), og);
       };
       const f32x4 h = result(oc), partner = GLU ? result(OUT + oc) : f32x4{1, 1, 1, 1};
 #pragma unroll
@@ -303,14 +304,15 @@ __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1)
     for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.H) continue;
-      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
+      const int at = S::position(oc, a.H - col);
+      const f32x4 h = shared.sums.get(S::product_of(at), S::lane_of(at), og);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int r = 16 * m + 4 * og + v;
         if (r >= rows) break;
-        const int at = int((y_at + uint32_t(r) * a.H + col) * 4);
-        if (a.join) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(h[v]), y, at, 0, kDeviceScope);
-        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(h[v]), y, at, 0, 0);
+        const int to = int((y_at + uint32_t(r) * a.H + col) * 4);
+        if (a.join) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(h[v]), y, to, 0, kDeviceScope);
+        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(h[v]), y, to, 0, 0);
       }
     }
   }
@@ -411,14 +413,13 @@ void by_layout(int lay, int64_t tokens, F&& f) {
 template <typename T>
 int launch_few(FewArgs a, const FewPlan& p, int64_t I, const void* w_up, const int64_t* up, const void* w_down, const int64_t* down,
                uint32_t up_bytes, uint32_t down_bytes, hipStream_t stream, void* table) {
-  const bool x_whole = aligned16(a.x) && multiple8(a.x_ld);
   const bool glu = a.kind != GMM_ACT_SILU;
   const int64_t cus = gmm_num_cus();
   int rc = GMM_OK;
   bool routed = false;
   FewArgs u = a;
   u.w = w_up; u.w_sg = up[0]; u.w_sk = uint32_t(up[1]); u.w_sn = uint32_t(up[2]); u.w_bytes = up_bytes;
-  by_layout(layout_of(w_up, up[0], up[1], up[2], a.H, multiple8(I), x_whole), a.tokens, [&](auto l, auto m) {
+  by_layout(layout_of(up[1], up[2], a.H, I), a.tokens, [&](auto l, auto m) {
     constexpr int LAY = decltype(l)::value, MF = decltype(m)::value, FR = LAY == GMM_W_COLS ? 4 : 8;
     const int out = (glu ? 8 : 16) * FR;
     u.tiles = int((I + out - 1) / out);
@@ -457,7 +458,7 @@ int launch_few(FewArgs a, const FewPlan& p, int64_t I, const void* w_up, const i
   if (rc != GMM_OK) return rc;
   FewArgs d = a;
   d.w = w_down; d.w_sg = down[0]; d.w_sk = uint32_t(down[1]); d.w_sn = uint32_t(down[2]); d.w_bytes = down_bytes;
-  by_layout(layout_of(w_down, down[0], down[1], down[2], I, multiple8(a.H), true), a.tokens, [&](auto l, auto m) {
+  by_layout(layout_of(down[1], down[2], I, a.H), a.tokens, [&](auto l, auto m) {
     constexpr int LAY = decltype(l)::value, MF = decltype(m)::value, FR = LAY == GMM_W_COLS ? 4 : 8;
     d.tiles = (a.H + 16 * FR - 1) / (16 * FR);
     const dim3 grid(unsigned(p.used * d.tiles * p.parts));

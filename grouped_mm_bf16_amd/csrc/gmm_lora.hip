@@ -26,8 +26,9 @@ constexpr int kSingleRows = 256;       // up to which rows are taken one at a ti
 constexpr int kMaxRank = 256;
 constexpr int kMaxAdapters = 1022;     // one more bin of the sort holds the rows without an adapter
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-// Waves of a workgroup of a few rows' launch: eight, four where the sums of 64 rows by 128 columns need half of the registers.
-constexpr int few_waves(int MF) { return MF == 4 ? 4 : 8; }
+// Waves of a workgroup of a few rows' launch: eight, four where the sums of 64 rows by 128 columns, or what is loaded element by element,
+// need half of the registers.
+constexpr int few_waves(int MF, int lay) { return MF == 4 || (MF == 2 && lay == GMM_W_ANY) ? 4 : 8; }
 
 struct Matrices {          // a stack [L, K, N] of 16-bit matrices, or one
   const void* at;
@@ -130,7 +131,7 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
   for (bool more = true; more;) {
 #pragma unroll
     for (int u = 0; u < ST; ++u) {
-      s.template multiply<1>(step[u], 0, 0, acc);
+      s.template multiply<1>(step[u], begin + add_step * NEXT, to, acc);
       // behind an adapter's last step its rows are taken over: what is no number in it stays with them.  (Steps behind all of them
       // add zeros to a row that has been taken.)
       if (++add_step == steps) {
@@ -153,7 +154,8 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
   float* const out = a.low + (int64_t(part) * a.rows + row0) * a.R;
   for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
     const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
-    const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
+    const int at = S::position(oc, max(1, a.R - col));
+    const f32x4 h = shared.sums.get(S::product_of(at), S::lane_of(at), og);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int r = 4 * og + v;
@@ -161,7 +163,7 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
       if (a.low_parts > 1 || !a.keep) {
         if (col < a.R) out[r * a.R + col] = h[v];
       } else if (col < a.pitch) {
-        keep_low<T>(a, row0 + r, col, h[v], a.scale ? a.scale[a.adapter[row0 + r]] : 1.0f);
+        keep_low<T>(a, row0 + r, col, col < a.R ? h[v] : 0.0f, a.scale ? a.scale[a.adapter[row0 + r]] : 1.0f);
       }
     }
   }
@@ -176,8 +178,8 @@ __global__ void __launch_bounds__(kThreads, FR <= 2 ? 3 : 2) lora_low_kernel(con
 
 // A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
 template <typename T, int LAY_W, int LAY_A, int MF>
-__global__ void __launch_bounds__(64 * few_waves(MF)) lora_few_kernel(const LoraArgs a) {
-  constexpr int WAVES = few_waves(MF);
+__global__ void __launch_bounds__(64 * few_waves(MF, LAY_W)) lora_few_kernel(const LoraArgs a) {
+  constexpr int WAVES = few_waves(MF, LAY_W);
   using S = Strip<T, LAY_W, MF, 1>;
   using SA = LowSkinny<T, LAY_A, 1, LAY_W == GMM_W_ANY>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
@@ -210,7 +212,8 @@ __global__ void __launch_bounds__(64 * few_waves(MF)) lora_few_kernel(const Lora
     for (int u = threadIdx.x; u < OUT * 4; u += 64 * WAVES) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.N) continue;
-      const f32x4 h = shared.base.sums.get(S::product_of(oc), S::lane_of(oc), og);
+      const int at = S::position(oc, a.N - col);
+      const f32x4 h = shared.base.sums.get(S::product_of(at), S::lane_of(at), og);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int r = 16 * m + 4 * og + v;
@@ -229,33 +232,34 @@ __device__ __forceinline__ float low_sum(const LoraArgs& a, int row, int r) {
 }
 
 // One row after the other: y[t] = sum of the parts of x @ W (without any: what lies in y) + scale * low @ B.  A wave for 64 lanes' columns
-// of one row: eight columns to a lane where B is contiguous along them, else one.
+// of one row: eight columns to a lane where B is contiguous along them (where fewer are left the last eight, of which the lane writes its
+// own), else one.
 template <typename T, int LAY>
 __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   constexpr int W = LAY == GMM_W_ROWS ? 8 : 1;
   __shared__ float low[kMaxRank];
-  const int t = blockIdx.y, lane = threadIdx.x, c = (blockIdx.x * 64 + lane) * W;
+  const int t = blockIdx.y, lane = threadIdx.x, own = (blockIdx.x * 64 + lane) * W, c = W == 8 ? min(own, max(0, a.N - 8)) : own;
   const int id = a.adapter[t];
   float y[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) y[i] = 0;
   T* const out = static_cast<T*>(a.out) + t * a.out_ld + c;
-  if (c < a.N && a.base_parts == 0) {
+  if (own < a.N && a.base_parts == 0) {
     if constexpr (W == 8) {
-      const Pack<T, 8> there = *reinterpret_cast<const Pack<T, 8>*>(out);
+      const Pack<T, 8> there = unaligned<Pack<T, 8>>(out);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = there.get(i);
     } else {
       y[0] = widen(out[0]);
     }
   }
-  if (c < a.N) {
+  if (own < a.N) {
     const float* base = a.base + int64_t(t) * a.N + c;
     const int64_t next = int64_t(a.rows) * a.N;
 #pragma unroll 4
     for (int p = 0; p < a.base_parts; ++p, base += next) {
       if constexpr (W == 8) {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(base), hi = *reinterpret_cast<const f32x4*>(base + 4);
+        const f32x4 lo = unaligned<f32x4>(base), hi = unaligned<f32x4>(base + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
       } else {
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
       low[r] = s * scale;
     }
   __syncthreads();
-  if (c >= a.N) return;
+  if (own >= a.N) return;
   if (has) {
     const T* b = static_cast<const T*>(a.b.at) + id * a.b.sg + int64_t(c) * a.b.sn;
     float add[W];
@@ -281,17 +285,18 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
     if constexpr (LAY == GMM_W_ROWS) {
 #pragma unroll 8
       for (int r = 0; r < a.R; ++r) {
-        const Pack<T, 8> v = *reinterpret_cast<const Pack<T, 8>*>(b + int64_t(r) * a.b.sk);
+        const Pack<T, 8> v = unaligned<Pack<T, 8>>(b + int64_t(r) * a.b.sk);
 #pragma unroll
         for (int i = 0; i < 8; ++i) add[i] += low[r] * v.get(i);
       }
     } else if constexpr (LAY == GMM_W_COLS) {
 #pragma unroll 4
-      for (int r = 0; r < a.R; r += 8) {
-        const Pack<T, 8> v = *reinterpret_cast<const Pack<T, 8>*>(b + r);
+      for (int r = 0; r + 8 <= a.R; r += 8) {
+        const Pack<T, 8> v = unaligned<Pack<T, 8>>(b + r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) add[0] += low[r + i] * v.get(i);
       }
+      for (int r = a.R / 8 * 8; r < a.R; ++r) add[0] += low[r] * widen(b[r]);
     } else {
 #pragma unroll 4
       for (int r = 0; r < a.R; ++r) add[0] += low[r] * widen(b[int64_t(r) * a.b.sk]);
@@ -300,7 +305,13 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
     for (int i = 0; i < W; ++i) y[i] += add[i];
   }
   if constexpr (W == 8) {
-    *reinterpret_cast<Pack<T, 8>*>(out) = Pack<T, 8>::of(y);
+    const Pack<T, 8> now = Pack<T, 8>::of(y);
+    if (c == own) {
+      __builtin_memcpy(out, &now, 16);
+    } else {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) if (c + i >= own) out[i] = rounded<T>(y[i]);
+    }
   } else {
     out[0] = rounded<T>(y[0]);
   }
@@ -319,8 +330,8 @@ __global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a)
 // Many rows: y[t] += scale * low @ B.  A wave takes 16 rows and strips of 128 columns, one after the other; y is read and written where
 // it is, 16 bytes to a lane where it can be.  The next strip's y and B are on their way while one is written: of 4 waves and one strip
 // at a time 8192 x 4096 took 65 us, five trips to memory one after the other for each.  NK: steps of 32 of the rank that are held.
-template <typename T, int LAY, int NK, bool WIDE>
-__global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_kernel(const LoraArgs a) {
+template <typename T, int LAY, int NK>
+__global__ void __launch_bounds__(kThreads, NK == 1 ? 3 : 2) lora_add_kernel(const LoraArgs a) {
   using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, GMM_A_STAGED, 1>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
@@ -337,33 +348,24 @@ __global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_ke
   const uint32_t y_at = uint32_t(4 * g) * uint32_t(a.out_ld) * 2, y_step = uint32_t(a.out_ld) * 2;
   const auto load_y = [&](u32x4 (&old)[4], int tile, uint32_t mine) {
     const int c = (tile0 + tile) * OUT + FR * j;
+    const uint32_t at = y_at + uint32_t(min(c, a.N - FR)) * 2;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const bool in = mine >> (4 * g + v) & 1;
-      const uint32_t at = y_at + v * y_step + uint32_t(c) * 2;
-      if constexpr (WIDE) {
-        old[v] = __builtin_amdgcn_raw_buffer_load_b128(y, int(in && c < a.N ? at : kNowhere), 0, 0);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t lo = S::element(y, in && c + 2 * q < a.N ? at + 4 * q : kNowhere);
-          old[v][q] = lo | S::element(y, in && c + 2 * q + 1 < a.N ? at + 4 * q + 2 : kNowhere) << 16;
-        }
-      }
-    }
+    for (int v = 0; v < 4; ++v)
+      old[v] = __builtin_amdgcn_raw_buffer_load_b128(y, int(mine >> (4 * g + v) & 1 && c < a.N ? at + v * y_step : kNowhere), 0, 0);
   };
   const auto store_y = [&](const float (&now)[4][FR], int tile, uint32_t mine) {
-    const int c = (tile0 + tile) * OUT + FR * j;
+    const int c = (tile0 + tile) * OUT + FR * j, left = a.N - c;
+    const uint32_t at = y_at + uint32_t(c) * 2;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
+      const u32x4 p = Pack<T, 8>::of(now[v]).w;
       const bool in = mine >> (4 * g + v) & 1;
-      const uint32_t at = y_at + v * y_step + uint32_t(c) * 2;
-      if constexpr (WIDE) {
-        __builtin_amdgcn_raw_buffer_store_b128(Pack<T, 8>::of(now[v]).w, y, int(in && c < a.N ? at : kNowhere), 0, 0);
-      } else {
+      __builtin_amdgcn_raw_buffer_store_b128(p, y, int(in && left >= FR ? at + v * y_step : kNowhere), 0, 0);
+      if (in && left > 0 && left < FR) {      // the lane that has fewer than eight: they are the last ones of what it loaded
+        const uint32_t last = at + v * y_step + 2 * left - 2;
 #pragma unroll
-        for (int i = 0; i < FR; ++i)
-          __builtin_amdgcn_raw_buffer_store_b16(rounded<T>(now[v][i]).bits, y, int(in && c + i < a.N ? at + 2 * i : kNowhere), 0, 0);
+        for (int i = 1; i < FR; ++i)
+          if (i >= FR - left) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(p[i / 2] >> 16 * (i & 1)), y, int(last - 2 * (FR - 1 - i)), 0, 0);
       }
     }
   };
@@ -376,10 +378,15 @@ __global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_ke
     } else {      // a rank's values of a column lie side by side: the operands as they are
 #pragma unroll
       for (int i = 0; i < FR; ++i)
-        w[i] = __builtin_amdgcn_raw_buffer_load_b128(s.w_buf, int(i < s.columns && k + 8 * g < a.R ? s.w_at + i * s.w_step_n + (k + 8 * g) * 2 : kNowhere), 0, 0);
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(
+            s.w_buf, int(s.columns && k + 8 * g < a.R ? s.w_at + i * s.w_step_n + (k + 8 * g) * 2 - S::back(k + 8 * g, a.R) : kNowhere), 0, 0);
     }
   };
-  const auto multiply = [&](const u32x4 (&w)[8], u32x4 h, u32x4 l, f32x4 (&acc)[FR]) {
+  const auto multiply = [&](u32x4 (&w)[8], int k, u32x4 h, u32x4 l, f32x4 (&acc)[FR]) {
+    if (LAY != GMM_W_ROWS && k + 32 > a.R) {
+#pragma unroll
+      for (int i = 0; i < FR; ++i) w[i] = S::tail(w[i], k + 8 * g, a.R);
+    }
 #pragma unroll
     for (int i = 0; i < FR; ++i) {
       const u32x4 b = LAY == GMM_W_ROWS ? S::turned(w, i) : w[i];
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_ke
 #pragma unroll 1
     for (int k = 0;;) {
 #pragma unroll
-      for (int n = 0; n < NK; ++n) multiply(w[n], h[n], l[n], acc);
+      for (int n = 0; n < NK; ++n) multiply(w[n], k + 32 * n, h[n], l[n], acc);
       k += 32 * NK;
       if (k >= a.R) break;
       load_low(k);
@@ -452,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, NK == 1 && WIDE ? 3 : 2) lora_add_ke
   }
 }
 
-// The same where B has no alignment: a thread has one column and 16 rows, and multiplies on the vector units, in fp32.
+// The same where neither step of B is one element, or there are fewer than eight columns: a thread has one column and 16 rows, and multiplies on the vector units, in fp32.
 constexpr int kAnyRows = 16;
 
 template <typename T>
@@ -508,7 +515,7 @@ struct GradOf {
   void* out;                // [L][R][C] with the strides below
   float* partial;           // [slots][R * C] as `out` has it: of adapters whose rows are more than one chunk
   int64_t p_ld, out_sg, out_sr, out_sc;
-  int32_t C, tiles, whole;  // whole: rows of p can be read 16 bytes at a time
+  int32_t C, tiles;
   int32_t r_first;          // out is contiguous along R (of partial: always along one of the two)
 };
 
@@ -556,6 +563,7 @@ __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& ad
 constexpr int kMaxChunk = 4096;
 
 // out[i] += q^T p over a chunk of adapter i's rows: R rows, a strip of 128 columns of p, the contraction along p's rows.
+// WHOLE: there are eight columns.
 template <typename T, int MF, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args) {
   using S = Skinny<T, GMM_W_ROWS, 8, MF, 2, GMM_A_STAGED, 2>;
@@ -571,7 +579,7 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   for (int u = threadIdx.x; u < rows; u += kThreads) row_at[u] = args.row_at[first + u];
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c)), R = args.R;
+  const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c)), R = args.R, end = (rows + 7) / 8 * 8;   // zeros behind the last row
   S s;
   s.lane = lane;
   s.lds = shared.wave[wave];
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   s.a_buf = buffer(a.q, 2 * s.a_plane);
   s.set_rows([&](int r) { return r0 + r < R ? (uint32_t(r0 + r) * args.places + first) * 2 : kNowhere; });
   // Steps as Skinny has them, from rows that are anywhere (64-bit addresses).  Past the end the last row is read again and not used.
-  const T* const p = static_cast<const T*>(a.p) + (columns ? c : 0);
+  const T* const p = static_cast<const T*>(a.p) + (WHOLE ? min(c, a.C - FR) : columns ? c : 0);
   const auto load = [&](typename S::Step& step, int k) {
     const int kl = k + 8 * g;
 #pragma unroll
@@ -587,14 +595,14 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
       const T* at = p + int64_t(row_at[min(kl + r, rows - 1)]) * a.p_ld;
       u32x4 v = {0, 0, 0, 0};
       if constexpr (WHOLE) {
-        v = *reinterpret_cast<const u32x4*>(at);
+        v = unaligned<u32x4>(at);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i / 2] |= uint32_t(at[max(0, min(i, columns - 1))].bits) << 16 * (i & 1);
       }
       step.w[r] = v;
     }
-    s.template load_a<MF>(step, k, rows);
+    s.template load_a<MF>(step, k, end);
     __builtin_amdgcn_sched_barrier(0);
   };
   const auto multiply = [&](typename S::Step& step, int k, f32x4 (&acc)[MF][FR]) {
@@ -605,7 +613,7 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
 #pragma unroll
         for (int q = 0; q < 4; ++q) step.w[r][q] = k + 8 * g + r < rows ? step.w[r][q] : 0u;
     }
-    s.template multiply<MF>(step, k, rows, acc);
+    s.template multiply<MF>(step, k, end, acc);
     __builtin_amdgcn_sched_barrier(0);
   };
   f32x4 acc[MF][FR];
@@ -631,7 +639,8 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
     for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.C) continue;
-      const f32x4 h = shared.sums.get(S::product_of(oc), S::lane_of(oc), og);
+      const int at = WHOLE ? S::position(oc, a.C - col) : oc;
+      const f32x4 h = shared.sums.get(S::product_of(at), S::lane_of(at), og);
       const int r = r0 + 16 * m + 4 * og;
       if (slot >= 0) {
         float* const to = a.partial + int64_t(slot) * R * a.C + (a.r_first ? int64_t(col) * R + r : int64_t(r) * a.C + col);
@@ -742,13 +751,12 @@ void by_layout(int lay, F&& f) {
 
 int strip_columns(int lay) { return lay == GMM_W_COLS ? 64 : 128; }
 
-int layout_of(const Matrices& m, int64_t K, int64_t N, bool whole) { return gmm::layout_of(m.at, m.sg, m.sk, m.sn, K, multiple8(N), whole); }
+int layout_of(const Matrices& m, int64_t K, int64_t N) { return gmm::layout_of(m.sk, m.sn, K, N); }
 
 // B's layout: nothing is asked of the rank where it is contiguous along its columns.
 int layout_of_b(const Matrices& b, int64_t R, int64_t N) {
-  if (!aligned16(b.at) || !multiple8(b.sg)) return GMM_W_ANY;
-  if (b.sn == 1 && multiple8(b.sk) && multiple8(N)) return GMM_W_ROWS;
-  return b.sk == 1 && multiple8(b.sn) && multiple8(R) ? GMM_W_COLS : GMM_W_ANY;
+  if (N < 8) return GMM_W_ANY;
+  return b.sn == 1 ? GMM_W_ROWS : b.sk == 1 && R >= 8 ? GMM_W_COLS : GMM_W_ANY;
 }
 
 bool set(Matrices& m, const void* at, int64_t sg, int64_t sk, int64_t sn, int64_t K, int64_t N) {
@@ -780,9 +788,7 @@ void set_low(LoraArgs& a, int columns) {
 
 template <typename T>
 int launch_finish(const LoraArgs& a, hipStream_t stream) {
-  int lay = layout_of_b(a.b, a.R, a.N);
-  if (lay == GMM_W_ROWS && !(aligned16(a.out) && multiple8(a.out_ld))) lay = GMM_W_ANY;       // eight columns of the result at a time
-  by_layout(lay, [&](auto l) {
+  by_layout(layout_of_b(a.b, a.R, a.N), [&](auto l) {
     constexpr int B = decltype(l)::value, W = B == GMM_W_ROWS ? 8 : 1;
     hipLaunchKernelGGL((lora_finish_kernel<T, B>), dim3(unsigned(a.N ? (a.N + 64 * W - 1) / (64 * W) : 1), unsigned(a.rows)), dim3(64), 0, stream, a);
   });
@@ -790,9 +796,9 @@ int launch_finish(const LoraArgs& a, hipStream_t stream) {
 }
 
 template <typename T>
-int launch_few(LoraArgs a, bool whole, hipStream_t stream) {
-  const int lay_w = layout_of(a.w, a.K, a.N, whole);
-  const int lay_a = lay_w == GMM_W_ANY ? GMM_W_ANY : layout_of(a.a, a.K, a.R, whole);
+int launch_few(LoraArgs a, hipStream_t stream) {
+  const int lay_w = layout_of(a.w, a.K, a.N);
+  const int lay_a = lay_w == GMM_W_ANY ? GMM_W_ANY : layout_of(a.a, a.K, a.R);
   set_low(a, 16);
   const BasePlan bp = plan_base(a.K, a.N, strip_columns(lay_w));
   a.base_parts = bp.parts; a.base_k = bp.each;
@@ -801,9 +807,9 @@ int launch_few(LoraArgs a, bool whole, hipStream_t stream) {
   const dim3 grid(unsigned(a.low_groups + a.base_tiles * a.base_parts));
   const auto launch = [&](auto w, auto l) {
     constexpr int W = decltype(w)::value, A = decltype(l)::value;
-    if (a.rows <= 16) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 1>), grid, dim3(64 * few_waves(1)), 0, stream, a);
-    else if (a.rows <= 32) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 2>), grid, dim3(64 * few_waves(2)), 0, stream, a);
-    else hipLaunchKernelGGL((lora_few_kernel<T, W, A, 4>), grid, dim3(64 * few_waves(4)), 0, stream, a);
+    if (a.rows <= 16) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 1>), grid, dim3(64 * few_waves(1, W)), 0, stream, a);
+    else if (a.rows <= 32) hipLaunchKernelGGL((lora_few_kernel<T, W, A, 2>), grid, dim3(64 * few_waves(2, W)), 0, stream, a);
+    else hipLaunchKernelGGL((lora_few_kernel<T, W, A, 4>), grid, dim3(64 * few_waves(4, W)), 0, stream, a);
   };
   constexpr std::integral_constant<int, GMM_W_ROWS> rows{};
   constexpr std::integral_constant<int, GMM_W_COLS> cols{};
@@ -822,13 +828,13 @@ int launch_few(LoraArgs a, bool whole, hipStream_t stream) {
 
 // Columns of a strip: as few as hold the rank.
 template <typename T>
-int launch_low(LoraArgs& a, bool whole, hipStream_t stream) {
-  const int lay = layout_of(a.a, a.K, a.R, whole);
+int launch_low(LoraArgs& a, hipStream_t stream) {
+  const int lay = layout_of(a.a, a.K, a.R);
   int fr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : a.R <= 64 || lay == GMM_W_COLS ? 4 : 8;
   if (lay == GMM_W_ANY) fr = 1;
   set_low(a, 16 * fr);
   const dim3 grid(unsigned(a.low_groups)), block(kThreads);
-  const bool edge = !whole || !multiple8(a.K);     // x has no alignment
+  const bool edge = a.K < 8;
   const auto launch = [&](auto l, auto n, auto e) {
     hipLaunchKernelGGL((lora_low_kernel<T, decltype(l)::value, decltype(n)::value, decltype(e)::value>), grid, block, 0, stream, a);
   };
@@ -857,17 +863,16 @@ int launch_low(LoraArgs& a, bool whole, hipStream_t stream) {
 int64_t pitch_of(int64_t R) { return round_up(R, 16); }
 
 template <typename T>
-int launch_add(LoraArgs a, bool whole, hipStream_t stream) {
+int launch_add(LoraArgs a, hipStream_t stream) {
   a.pitch = int(pitch_of(a.R));
   a.keep = a.rows > kSingleRows;
-  const int rc = launch_low<T>(a, whole, stream);
+  const int rc = launch_low<T>(a, stream);
   if (rc != GMM_OK) return rc;
   if (!a.keep) return launch_finish<T>(a, stream);
   const unsigned blocks = unsigned((int64_t(a.rows) * a.pitch + kThreads - 1) / kThreads);
   if (a.low_parts > 1) hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
   if (a.N) {
     const int lay = layout_of_b(a.b, a.R, a.N);
-    const int wide = aligned16(a.out) && multiple8(a.out_ld) && multiple8(a.N);
     const dim3 any((a.rows + kAnyRows - 1) / kAnyRows, (a.N + kThreads - 1) / kThreads);
     // strips to a wave: as many as leave every place for one a wave
     const int tiles = (a.N + 127) / 128, row_groups = (a.rows + 16 * kWaves - 1) / (16 * kWaves);
@@ -875,8 +880,7 @@ int launch_add(LoraArgs a, bool whole, hipStream_t stream) {
     const dim3 grid(row_groups, (tiles + a.strips - 1) / a.strips);
     const auto launch = [&](auto lay, auto nk) {
       constexpr int B = decltype(lay)::value, NK = decltype(nk)::value;
-      if (wide) hipLaunchKernelGGL((lora_add_kernel<T, B, NK, true>), grid, dim3(kThreads), 0, stream, a);
-      else hipLaunchKernelGGL((lora_add_kernel<T, B, 1, false>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((lora_add_kernel<T, B, NK>), grid, dim3(kThreads), 0, stream, a);
     };
     const auto rank = [&](auto lay) {
       if (a.R <= 32) launch(lay, std::integral_constant<int, 1>{});
@@ -923,7 +927,6 @@ void set_grad(GradOf& g, const void* p, int64_t p_ld, const void* q, void* out, 
   g.out_sg = sg; g.out_sr = sr; g.out_sc = sc;
   g.C = int32_t(C);
   g.tiles = out ? int32_t((C + 127) / 128) : 0;
-  g.whole = aligned16(p) && multiple8(p_ld) && multiple8(C);
   const bool four = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && R % 4 == 0 && sg % 4 == 0 && sc % 4 == 0;   // four of R in 8 bytes
   g.r_first = sr != 1 || R == 1 ? 0 : four ? 2 : 1;
 }
@@ -934,7 +937,7 @@ int launch_grad(GradArgs& g, int64_t rows, hipStream_t stream) {
   g.groups0 = int32_t(chunks * g.of[0].tiles);
   const int64_t groups = g.groups0 + chunks * g.of[1].tiles;
   if (groups == 0) return GMM_OK;
-  const bool whole = (!g.of[0].tiles || g.of[0].whole) && (!g.of[1].tiles || g.of[1].whole);
+  const bool whole = (!g.of[0].tiles || g.of[0].C >= 8) && (!g.of[1].tiles || g.of[1].C >= 8);
   const auto launch = [&](auto mf) {
     constexpr int MF = decltype(mf)::value;
     const dim3 grid(unsigned(groups), unsigned((g.R + 16 * MF - 1) / (16 * MF)));
@@ -986,9 +989,8 @@ int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, 
   g.base = reinterpret_cast<float*>(static_cast<char*>(workspace) + low_bytes(rows, K, R));
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
-  const bool whole = aligned16(x) && multiple8(g.x_ld);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GMM_DT_BF16 ? launch_few<Bf16>(g, whole, s) : launch_few<F16>(g, whole, s);
+  return dtype == GMM_DT_BF16 ? launch_few<Bf16>(g, s) : launch_few<F16>(g, s);
 }
 
 int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, void* out, float* low,
@@ -1007,9 +1009,8 @@ int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* ada
   g.planes = N ? static_cast<char*>(workspace) + low_bytes(rows, K, R) : nullptr;
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
-  const bool whole = aligned16(x) && multiple8(g.x_ld);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GMM_DT_BF16 ? launch_add<Bf16>(g, whole, s) : launch_add<F16>(g, whole, s);
+  return dtype == GMM_DT_BF16 ? launch_add<Bf16>(g, s) : launch_add<F16>(g, s);
 }
 
 int64_t gmm_lora_grad_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L) {

@@ -10,13 +10,13 @@
 //     neighbouring lanes would ask for four cache lines: such a load takes the unit that looks lines up 64 cycles, not 16, and that
 //     is what bounded these products (67 MB past 64 rows 27 us).
 //   along n, 16 to 64 columns (GMM_W_THIN): rows of k side by side, turned by LDS reads that transpose.
-//   anything else (GMM_W_ANY): as GMM_W_ROWS, or 16 columns, element by element.
+//   anything else (GMM_W_ANY: neither step is one element, or fewer than eight of a kind): as GMM_W_ROWS, or 16 columns, element by element.
+// Nothing is asked of alignment: a load of 16 bytes may begin at any element.  Where fewer than eight are left, along n as along k, the
+// last eight are loaded: so no load leaves the matrix.  Along n, columns then lie elsewhere in the result (`position`); along k, the
+// ones that were there already are shifted out (`tail`), in a range's last step.
 // A goes through LDS as well, for the same reason.  Its rows that do not exist read as zeros and cost no access.  LDS is a wave's own
 // here: its instructions run in order, nobody waits for anybody.  The waves of a workgroup share the range of k and add up in LDS.
 #pragma once
-#ifndef ST_4
-#define ST_4 2
-#endif
 #include "gmm_elem.h"
 
 namespace gmm {
@@ -97,9 +97,26 @@ struct Skinny {
     return uint32_t(uint16_t(__builtin_amdgcn_raw_buffer_load_b16(buf, int(at), 0, 0)));
   }
 
-  // Column of the strip that product i has in lanes j, 16 + j, ...; and back.
-  static __device__ __forceinline__ int product_of(int column) { return LAY == GMM_W_ROWS || LAY == GMM_W_ANY ? column % FR : column / 16; }
-  static __device__ __forceinline__ int lane_of(int column) { return LAY == GMM_W_ROWS || LAY == GMM_W_ANY ? column / FR : column % 16; }
+  // Where a column of the strip is: in the lanes j, 16 + j, ... of product i.  left: how many columns there are from it on.
+  static __device__ __forceinline__ int position(int column, int left) {
+    return LAY == GMM_W_ROWS || LAY == GMM_W_THIN ? column - column % 8 + max(column % 8, 8 - left) : column;
+  }
+  static __device__ __forceinline__ int product_of(int position) { return LAY == GMM_W_ROWS || LAY == GMM_W_ANY ? position % FR : position / 16; }
+  static __device__ __forceinline__ int lane_of(int position) { return LAY == GMM_W_ROWS || LAY == GMM_W_ANY ? position / FR : position % 16; }
+
+  // Eight values of k from `from` on of a row, of which those before `end` exist: where they are loaded, relative to it; and, loaded, the
+  // ones that exist, zeros behind them.
+  static __device__ __forceinline__ uint32_t back(int from, int end) { return uint32_t(max(0, from + 8 - end)) * 2; }
+  static __device__ __forceinline__ u32x4 tail(u32x4 v, int from, int end) {
+    const int over = from + 8 - end;      // nothing was loaded: zeros
+    const bool four = over & 4, two = over & 2, one = over & 1, any = over > 0;
+    if (any) {
+      v = four ? u32x4{v[2], v[3], 0, 0} : v;
+      v = two ? u32x4{v[1], v[2], v[3], 0} : v;
+      v = one ? u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16} : v;
+    }
+    return v;
+  }
 
   // The strip of columns from `first` on, of which `count` (or more than the strip holds) exist; steps in elements.  With `half` > 0 it is
   // that many columns from `first` on and as many from `other` on, `count` of each.
@@ -115,11 +132,11 @@ struct Skinny {
     } else if constexpr (LAY == GMM_W_THIN) {
       const int c = lane % (2 * FR) * 8;
       columns = count - c;
-      w_at = uint32_t(lane / (2 * FR)) * w_step_k + uint32_t(first + c) * 2;
+      w_at = uint32_t(lane / (2 * FR)) * w_step_k + uint32_t(first + c - max(0, 8 - max(1, columns))) * 2;
     } else {
       const int c = FR * j, in = half ? c % half : c;
       columns = max(0, min(FR, count - in));
-      w_at = uint32_t((half && c >= half ? other : first) + in) * w_step_n;
+      w_at = uint32_t((half && c >= half ? other : first) + in - (LAY == GMM_W_ROWS ? 8 - max(1, columns) : 0)) * w_step_n;
     }
   }
 
@@ -148,7 +165,7 @@ struct Skinny {
       for (int r = 0; r < 8; ++r)
         w[r] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(columns && kl + r < end ? at + r * w_step_k : kNowhere), 0, kStream);
     } else if constexpr (LAY == GMM_W_COLS) {
-      const uint32_t at = w_at + uint32_t(k) * 2;
+      const uint32_t at = w_at + uint32_t(k) * 2 - back(k + 8 * (lane & 7), end);
       const bool in = k + 8 * (lane & 7) < end;
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
@@ -204,7 +221,8 @@ struct Skinny {
           }
         } else {
           const bool in = a_at[i] != kNowhere && k + 8 * (lane % CH) < end;
-          s.a[p][i] = __builtin_amdgcn_raw_buffer_load_b128(a_buf, int(in ? a_at[i] + p * a_plane + uint32_t(k) * 2 : kNowhere), 0, 0);
+          const uint32_t at = a_at[i] + p * a_plane + uint32_t(k) * 2 - back(k + 8 * (lane % CH), end);
+          s.a[p][i] = __builtin_amdgcn_raw_buffer_load_b128(a_buf, int(in ? at : kNowhere), 0, 0);
         }
       }
   }
@@ -221,8 +239,18 @@ struct Skinny {
   static __device__ __forceinline__ int chunk_at(int r, int c) { return r * 16 * CH + 16 * (CH == 8 ? c ^ (r >> 1 & 7) : c ^ (r >> 2 & 3)); }
 
   template <int M>
-  __device__ __forceinline__ void multiply(const Step& s, int k, int end, f32x4 (&acc)[MF][FR]) const {
+  __device__ __forceinline__ void multiply(Step& s, int k, int end, f32x4 (&acc)[MF][FR]) const {
     const int j = lane & 15, g = lane >> 4;
+    if (k + KS > end) {
+      if constexpr (LAY == GMM_W_COLS)
+#pragma unroll
+        for (int i = 0; i < WL; ++i) s.w[i] = tail(s.w[i], k + 8 * (lane & 7), end);
+      if constexpr (AM == GMM_A_STAGED)
+#pragma unroll
+        for (int i = 0; i < M * KH; ++i)
+#pragma unroll
+          for (int p = 0; p < NA; ++p) s.a[p][i] = tail(s.a[p][i], k + 8 * (lane % CH), end);
+    }
     lds_order();
     if constexpr (LAY == GMM_W_COLS)
 #pragma unroll
@@ -325,7 +353,7 @@ struct Skinny {
 
 // A strip of a matrix that is large.
 template <typename T, int LAY, int MF, int NA, int AM = LAY == GMM_W_ANY ? GMM_A_ELEMENTS : GMM_A_STAGED>
-using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, MF, NA, AM, MF == 4 ? ST_4 : 2>;
+using Strip = Skinny<T, LAY, LAY == GMM_W_COLS ? 4 : 8, MF, NA, AM, 2>;
 
 template <int MF, int FR>
 __device__ __forceinline__ void clear(f32x4 (&acc)[MF][FR]) {
@@ -364,15 +392,12 @@ union SkinnyShared {
 };
 
 // ---------------------------------------------------------------- host side
-inline bool multiple8(int64_t v) { return (v & 7) == 0; }
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Layout of a stack of matrices [G, K, N].  n_whole: columns come in whole eights; whole: 16 bytes of A can be read at a time.
-inline int layout_of(const void* w, int64_t sg, int64_t sk, int64_t sn, int64_t K, bool n_whole, bool whole) {
-  if (!whole || !aligned16(w) || !multiple8(sg) || !multiple8(K)) return GMM_W_ANY;
-  if (sn == 1 && multiple8(sk) && n_whole) return GMM_W_ROWS;
-  if (sk == 1 && multiple8(sn)) return GMM_W_COLS;
-  return GMM_W_ANY;
+// Layout of matrices [K, N] with the steps sk and sn of which eight columns belong together.
+inline int layout_of(int64_t sk, int64_t sn, int64_t K, int64_t N) {
+  if (K < 8) return GMM_W_ANY;
+  return sn == 1 && N >= 8 ? GMM_W_ROWS : sk == 1 ? GMM_W_COLS : GMM_W_ANY;
 }
 
 // Bytes from the first to behind the last element of a matrix of 16-bit elements; 0: strides that do not fit or 2 GiB and more.

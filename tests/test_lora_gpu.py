@@ -97,6 +97,28 @@ def test_rows_of_x_that_lie_apart(T, pad, offset):
     check(*make(T, 256, 128, 16, 4, pad=pad, offset=offset))
 
 
+def island(t, lay, pad=0):
+    """t at an odd address (2 bytes past a multiple of 4), rows pad elements apart, NaN all around."""
+    src = t.transpose(-2, -1) if lay == "cols" else t
+    rows, columns = src.shape[:-1].numel(), src.size(-1)
+    flat = torch.full((rows * (columns + pad) + 18,), float("nan"), dtype=t.dtype, device=DEV)
+    strides = [columns + pad, 1] if src.dim() == 2 else [src.size(1) * (columns + pad), columns + pad, 1]
+    view = torch.as_strided(flat, src.shape, strides, 9)
+    view.copy_(src)
+    return view.transpose(-2, -1) if lay == "cols" else view
+
+
+@pytest.mark.parametrize("K,N,R", [(8, 8, 8), (9, 11, 9), (65, 130, 31), (254, 261, 33), (1031, 519, 12), (3000, 77, 100)])
+@pytest.mark.parametrize("T", [1, 20, 40, 130, 300])
+@pytest.mark.parametrize("lay", ["rows", "cols"])
+def test_matrices_at_odd_addresses_among_nan(K, N, R, T, lay):
+    x, weight, a, b, adapter, scale = make(T, K, N, R, 3, dtype=HF)
+    x, weight, a, b = island(x, "rows", 3), island(weight, lay), island(a, lay, 5), island(b, lay)
+    check(x, weight, a, b, adapter, scale)
+    if T in (40, 300):
+        check_grads(x, weight, a, b, adapter, scale)
+
+
 @pytest.mark.parametrize("T", [6, 100, 400])
 @pytest.mark.parametrize("pattern", ["one", "none"])
 def test_one_adapter_or_none(T, pattern):

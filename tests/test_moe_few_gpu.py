@@ -133,6 +133,29 @@ def test_rows_of_x_and_logits_that_lie_apart(pad, offset):
     oracle.assert_within(run(x.t().contiguous().t(), z.t().contiguous().t(), up, down, 2, "swiglu"), oracle_out, bound)
 
 
+def island(t, lay, pad=0):
+    """t at an odd address (2 bytes past a multiple of 4), rows pad elements apart, NaN all around."""
+    src = t.transpose(-2, -1) if lay == "cols" else t
+    *front, rows, columns = src.shape
+    count = src.numel() // max(columns, 1) if src.numel() else 0
+    flat = torch.full((count * (columns + pad) + 18,), float("nan"), dtype=t.dtype, device=DEV)
+    strides = [columns + pad, 1]
+    for n in reversed(src.shape[1:-1]):
+        strides.insert(0, strides[0] * n)
+    view = torch.as_strided(flat, src.shape, strides[-src.dim():], 9)
+    view.copy_(src)
+    return view.transpose(-2, -1) if lay == "cols" else view
+
+
+@pytest.mark.parametrize("H,I", [(8, 8), (9, 11), (63, 65), (130, 71), (65, 64), (1031, 519), (500, 2050)])
+@pytest.mark.parametrize("lay", ["rows", "cols"])
+@pytest.mark.parametrize("T", [1, 5, 20, 40])
+def test_matrices_at_odd_addresses_among_nan(H, I, lay, T):
+    for kind in ("silu", "swiglu", "interleaved") if I % 64 == 0 else ("silu", "swiglu"):
+        x, z, up, down = make(T, 5, H, I, kind, dtype=HF)
+        check(island(x, "rows", 3), z, island(up, lay), island(down, lay, 5), 2, kind)
+
+
 def test_experts_that_share_their_weights():
     x, z, up, down = make(9, 5, 128, 64)
     up, down = up[:1].expand(5, -1, -1), down[:1].expand(5, -1, -1)
