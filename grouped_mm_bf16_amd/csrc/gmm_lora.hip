@@ -73,7 +73,8 @@ __device__ __forceinline__ void keep_low(const LoraArgs& a, int row, int r, floa
 
 // low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows.  Of rows with different adapters one adapter comes
 // after the other; their steps are one sequence, so that the next adapter's loads are on their way while the last one's are
-// multiplied (16 adapters a strip, drained each time: 1024 rows of 64 adapters 233 us, as one sequence see the plan below).
+// multiplied (1024
+// rows of 64 adapters, rank 64, with W's product: drained each time 233 us, as one sequence 167).
 template <typename T, int LAY, int FR, bool AE>
 using LowSkinny = Skinny<T, LAY, FR, 1, 1, AE ? GMM_A_ELEMENTS : GMM_A_STAGED, FR <= 2 ? 4 : 2>;
 
@@ -169,11 +170,17 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
   }
 }
 
+// Up to rank 16 (FR 1) eight waves share K, which then needs few parts or none, and no launch for their sums: 615 rows of 1031 -> 519 with
+// gradients 158 -> 151 us, 96 rows of 4096 -> 4096 with column-major W 37 -> 34 (but 8192 rows with gradients 569 -> 572).  Above, four
+// waves and more parts: with the steps of many adapters one after the other, 257 rows of 64 adapters of rank 64 94 us, with 16 waves 108.
+constexpr int low_waves(int FR) { return FR == 1 ? 8 : 4; }
+
 template <typename T, int LAY, int FR, bool AE>
-__global__ void __launch_bounds__(kThreads, FR <= 2 ? 3 : 2) lora_low_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(64 * low_waves(FR), FR == 1 ? 4 : FR == 2 ? 3 : 2) lora_low_kernel(const LoraArgs a) {
+  constexpr int WAVES = low_waves(FR);
   using S = LowSkinny<T, LAY, FR, AE>;
-  __shared__ SkinnyShared<S, kWaves> shared;
-  low_product<T, S, kWaves, FR <= 2 ? 4 : 2>(a, blockIdx.x, shared);
+  __shared__ SkinnyShared<S, WAVES> shared;
+  low_product<T, S, WAVES, FR <= 2 ? 4 : 2>(a, blockIdx.x, shared);
 }
 
 // A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
@@ -723,11 +730,12 @@ void cut(int64_t k, int64_t want, int64_t least, int32_t& parts, int32_t& each) 
 
 struct LowPlan { int32_t strip_rows, parts, each; };
 
-LowPlan plan_low(int64_t rows, int64_t K) {
+LowPlan plan_low(int64_t rows, int64_t K, int64_t R) {
   LowPlan p;
   p.strip_rows = rows <= kSingleRows ? 1 : 16;
   const int64_t strips = (rows + p.strip_rows - 1) / p.strip_rows;
   if (rows <= kFewRows) cut(K, strips ? 128 / strips : 1, 512, p.parts, p.each);
+  else if (R <= 16) cut(K, 256 / strips, 1024, p.parts, p.each);
   else cut(K, 2048 / strips, 256, p.parts, p.each);
   return p;
 }
@@ -780,7 +788,7 @@ bool x_fits(int64_t x_ld, int64_t rows, int64_t K) {
 }
 
 void set_low(LoraArgs& a, int columns) {
-  const LowPlan lp = plan_low(a.rows, a.K);
+  const LowPlan lp = plan_low(a.rows, a.K, a.R);
   a.strip_rows = lp.strip_rows; a.low_parts = lp.parts; a.low_k = lp.each;
   a.low_tiles = (a.R + columns - 1) / columns;
   a.low_groups = (a.rows + a.strip_rows - 1) / a.strip_rows * a.low_tiles * a.low_parts;
@@ -833,10 +841,11 @@ int launch_low(LoraArgs& a, hipStream_t stream) {
   int fr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : a.R <= 64 || lay == GMM_W_COLS ? 4 : 8;
   if (lay == GMM_W_ANY) fr = 1;
   set_low(a, 16 * fr);
-  const dim3 grid(unsigned(a.low_groups)), block(kThreads);
+  const dim3 grid(unsigned(a.low_groups));
   const bool edge = a.K < 8;
   const auto launch = [&](auto l, auto n, auto e) {
-    hipLaunchKernelGGL((lora_low_kernel<T, decltype(l)::value, decltype(n)::value, decltype(e)::value>), grid, block, 0, stream, a);
+    constexpr int LAY = decltype(l)::value, FR = decltype(n)::value;
+    hipLaunchKernelGGL((lora_low_kernel<T, LAY, FR, decltype(e)::value>), grid, dim3(64 * low_waves(FR)), 0, stream, a);
   };
   constexpr std::integral_constant<int, 1> one{};
   constexpr std::integral_constant<int, 2> two{};
@@ -960,7 +969,7 @@ int launch_grad(GradArgs& g, int64_t rows, hipStream_t stream) {
 }  // namespace
 
 // Bytes of the parts of x @ A.
-static int64_t low_bytes(int64_t rows, int64_t K, int64_t R) { return round_up(int64_t(plan_low(rows, K).parts) * rows * R * 4, 256); }
+static int64_t low_bytes(int64_t rows, int64_t K, int64_t R) { return round_up(int64_t(plan_low(rows, K, R).parts) * rows * R * 4, 256); }
 
 extern "C" {
 

@@ -241,7 +241,7 @@ struct Skinny {
   template <int M>
   __device__ __forceinline__ void multiply(Step& s, int k, int end, f32x4 (&acc)[MF][FR]) const {
     const int j = lane & 15, g = lane >> 4;
-    if (k + KS > end) {
+    if ((end & 7) && k + KS > end) {      // asked of every product it cost 2 %
       if constexpr (LAY == GMM_W_COLS)
 #pragma unroll
         for (int i = 0; i < WL; ++i) s.w[i] = tail(s.w[i], k + 8 * (lane & 7), end);

@@ -73,6 +73,11 @@ def _workspace_bytes(device: int, T: int, K: int, N: int, R: int) -> int:
     return _lib.load().gmm_lora_workspace_bytes(T, K, N, R)
 
 
+@functools.lru_cache(maxsize=4096)
+def _grad_workspace_bytes(device: int, T: int, K: int, N: int, R: int, L: int) -> int:
+    return _lib.load().gmm_lora_grad_workspace_bytes(T, K, N, R, L)
+
+
 def _forward_now(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter: torch.Tensor,
                  scale: Optional[torch.Tensor], save: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """The result, and (with `save`) x @ lora_a of the rows that have an adapter, [T, R] float32."""
@@ -119,9 +124,8 @@ def _grad_now(x: torch.Tensor, dy: torch.Tensor, low: torch.Tensor, u: torch.Ten
     """The gradients of lora_a and lora_b, laid out as those are (empty where not needed).  u is computed here if it is empty."""
     (T, K), N = x.shape, dy.size(1)
     L, _, R = lora_a.shape
-    none = x.new_empty(0)
-    da = torch.empty_like(lora_a) if need_a else none
-    db = torch.empty_like(lora_b) if need_b else none
+    da = torch.empty_like(lora_a) if need_a else x.new_empty(0)
+    db = torch.empty_like(lora_b) if need_b else x.new_empty(0)
     lib = _lib.load()
     with _guard(x):
         stream, code = kernels.current_stream(x.device), _dtype_code(x.dtype)
@@ -133,7 +137,7 @@ def _grad_now(x: torch.Tensor, dy: torch.Tensor, low: torch.Tensor, u: torch.Ten
             rc = lib.gmm_lora_add(dy.data_ptr(), lora_b.data_ptr(), None, adapter.data_ptr(), None, None, u.data_ptr(), T, N, 0, R, L,
                                   dy.stride(0), sl, sn, sr, 0, 0, 0, 0, code, ws.data_ptr(), nbytes, stream)
             _lib.check(rc, "lora_linear backward")
-        nbytes = lib.gmm_lora_grad_workspace_bytes(T, K, N, R, L)
+        nbytes = _grad_workspace_bytes(x.device.index, T, K, N, R, L)
         if nbytes < 0:
             raise RuntimeError("lora_linear backward: sizes out of range")
         ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
@@ -172,13 +176,12 @@ class _Lora(torch.autograd.Function):
         dy = _rows(grad)
         compiling = torch.compiler.is_compiling()
         dx = dw = da = db = None
-        low = low if low is not None else x.new_empty(0, dtype=torch.float32)
-        u = x.new_empty(0, dtype=torch.float32)
+        u = None
         if need_x:
-            dx, u_now = (_forward_op if compiling else _forward_now)(dy, weight.t(), lora_b.transpose(1, 2), lora_a.transpose(1, 2), adapter, scale,
-                                                                         need_a)
-            u = u_now if need_a else u
+            dx, u = (_forward_op if compiling else _forward_now)(dy, weight.t(), lora_b.transpose(1, 2), lora_a.transpose(1, 2), adapter, scale, need_a)
         if need_a or need_b:
+            if u is None:
+                u = x.new_empty(0, dtype=torch.float32)
             da, db = (_grad_op if compiling else _grad_now)(x, dy, low, u, adapter, scale, lora_a, lora_b, need_a, need_b)
         if need_w:
             dw = torch.empty(weight.shape, device=x.device, dtype=x.dtype)

@@ -126,7 +126,7 @@ class _LayerNorm(torch.autograd.Function):
         if save:
             ctx.save_for_backward(rows, weight, stats)
             ctx.param_dtype, ctx.shape = param_dtype, x.shape
-        return out.reshape(x.shape)
+        return out if x.dim() == 2 else out.reshape(x.shape)
 
     @staticmethod
     def backward(ctx, grad):
@@ -135,7 +135,9 @@ class _LayerNorm(torch.autograd.Function):
         impl = _backward_op if torch.compiler.is_compiling() else _backward_now
         need = ctx.needs_input_grad
         dx, dw, db = impl(dy, x, weight, stats, ctx.param_dtype, need[0], need[1], need[2])
-        return dx.reshape(ctx.shape) if need[0] else None, dw if need[1] else None, db if need[2] else None, None
+        if need[0]:
+            dx = dx if len(ctx.shape) == 2 else dx.reshape(ctx.shape)
+        return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
