@@ -1,10 +1,12 @@
 // A mixture-of-experts layer for a few tokens (gmm_moe_few in include/grouped_mm_hip.h):
 //   out[t] = sum over the choices j of w_tj * act(x[t] @ w_up[e_tj]) @ w_down[e_tj]
 // Routing as gmm_moe_route, then every chosen expert's matrices are read once, past a few rows (gmm_skinny.h).  Reading them bounds
-// it.  Between the two products the activations stay in 32 bits (two 16-bit values each), the second products in fp32: the result is
+// it: 8 tokens, 2 of 8 experts of 4096 -> 2 x 14336 368 us (7.0 TB/s), 32 tokens, 8 of 128 experts of 2048 -> 2 x 768 157 us (6.7 TB/s).
+// Between the two products the activations stay in 32 bits (two 16-bit values each), the second products in fp32: the result is
 // rounded once.
-// Of very few tokens the time is that of the launches and of the trips to memory behind one another.  Then there are two launches: every
-// workgroup of the first routes for itself, and of the second's, the last that is done with some columns adds them up.
+// Of very few tokens the time is that of the launches and of the trips to memory behind one another (1 token, 8 of 128 experts of
+// 2048 -> 2 x 768 28 us, of which the weights are 11).  Then there are two launches: every workgroup of the first routes for
+// itself, and of the second's, the last that is done with some columns adds them up.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -21,12 +23,14 @@ using namespace gmm;
 constexpr int kMaxTokens = 64;
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
-// Slots (choices of all tokens) and experts up to which a workgroup routes for itself, one wave to a token: 64 slots are a wave's lanes.
-constexpr int kRouteSlots = 64, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
+// Slots (choices of all tokens; at most a wave's lanes) and experts up to which a workgroup routes for itself, one wave to a token.  1 token, 1 of
+// 8 experts of 3674 -> 2 x 151 18 us, with a launch for the routing 20; 64 slots, 4 of 8 experts of 432 -> 2 x 10752 87 and 81.
+constexpr int kRouteSlots = 32, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
 
 // Slots up to which the second product's last workgroup of some columns adds them up: a launch less, but one workgroup reads what otherwise
-// all of them would.
-constexpr int kJoinSlots = 64;
+// all of them would.  3 tokens, 6 of 23 experts of 680 -> 2 x 2648 58 us, with a launch for the sums 63; 16 tokens, 4 of 8 experts of
+// 432 -> 2 x 10752 81 and 60.
+constexpr int kJoinSlots = 32;
 constexpr int kLine = 32;          // words from one counter to the next: 384 arrivals at 16 counters of one cache line took 8 us
 
 struct FewArgs {
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1)
   s.lds = shared.wave[wave];
   s.w_buf = buffer(static_cast<const T*>(a.w) + expert * a.w_sg, a.w_bytes);
   s.set_columns(tile * OUT, a.H - tile * OUT, a.w_sk, a.w_sn);
-  typename S::Step step[2];
+  typename S::Step step[S::STEPS];
   if constexpr (PARTS) {
     s.pitch = (a.k_part + 8) * 2;
     s.a_plane = uint32_t(a.tokens) * s.pitch;
@@ -339,19 +343,40 @@ __global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1)
   }
 }
 
-// out[t] = sum over j of weight * sum over the parts of y, in that order.
+// out[t] = sum over j of weight * sum over the parts of y, in that order.  Where they lie is looked up at once, and eight of them are on their
+// way together: one after the other 6 of 32 tokens took 14 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) few_combine_kernel(const FewArgs a) {
+  __shared__ uint32_t from[32];
+  __shared__ float weight[32];
   const int t = blockIdx.y, c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.H) return;
-  float sum = 0;
-  for (int j = 0; j < a.top_k; ++j) {
-    const int64_t row = a.token_rows[t * a.top_k + j];
-    float v = 0;
-#pragma unroll 8
-    for (int p = 0; p < a.parts; ++p) v += a.y[(int64_t(p) * a.slots + row) * a.H + c];
-    sum += a.slot_weight[t * a.top_k + j] * v;
+  if (int(threadIdx.x) < a.top_k) {
+    from[threadIdx.x] = uint32_t(a.token_rows[t * a.top_k + threadIdx.x]) * a.H;
+    weight[threadIdx.x] = a.slot_weight[t * a.top_k + threadIdx.x];
   }
+  __syncthreads();
+  if (c >= a.H) return;
+  const uint32_t next = uint32_t(a.slots) * a.H;
+  const float* const y = a.y + c;
+  float sum = 0;
+  const auto add = [&](auto parts) {
+    constexpr int P = decltype(parts)::value;
+#pragma unroll 8 / P
+    for (int j = 0; j < a.top_k; ++j) {
+      float v = 0;
+      if constexpr (P == 8) {
+#pragma unroll 8
+        for (int p = 0; p < a.parts; ++p) v += y[from[j] + p * next];
+      } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) v += y[from[j] + p * next];
+      }
+      sum += weight[j] * v;
+    }
+  };
+  if (a.parts == 1) add(std::integral_constant<int, 1>{});
+  else if (a.parts == 2) add(std::integral_constant<int, 2>{});
+  else add(std::integral_constant<int, 8>{});
   static_cast<T*>(a.out)[t * a.out_ld + c] = rounded<T>(sum);
 }
 

@@ -64,7 +64,7 @@ constexpr int GMM_A_RESIDENT = 2;    // lies in LDS
 
 template <typename T, int LAY, int FR_, int MF, int NA, int AM, int ST>
 struct Skinny {
-  static constexpr int FR = FR_;
+  static constexpr int FR = FR_, STEPS = ST;
   static constexpr int KS = LAY == GMM_W_COLS ? 64 : 32;      // k of a step
   static constexpr int KH = KS / 32;                          // products' halves of it
   static constexpr int COLUMNS = 16 * FR;
