@@ -335,12 +335,16 @@ __global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a)
 }
 
 // Many rows: y[t] += scale * low @ B.  A wave takes 16 rows and strips of 128 columns, one after the other; y is read and written where
-// it is, 16 bytes to a lane where it can be.  The next strip's y and B are on their way while one is written: of 4 waves and one strip
+// it is, 16 bytes to a lane.  The next strip's y and B are on their way while one is written: of 4 waves and one strip
 // at a time 8192 x 4096 took 65 us, five trips to memory one after the other for each.  NK: steps of 32 of the rank that are held.
-template <typename T, int LAY, int NK>
-__global__ void __launch_bounds__(kThreads, NK == 1 ? 3 : 2) lora_add_kernel(const LoraArgs a) {
+// ALIGNED: y's rows begin at whole 16 bytes; its accesses are then non-temporal (8192 x 4096, with x @ A 57 -> 52 us).  Elsewhere neighbours
+// share cache lines, and are not (8192 x 4099 72 us, non-temporal 75).
+constexpr int add_groups(int NK) { return NK == 1 ? 3 : 2; }      // that a compute unit holds
+
+template <typename T, int LAY, int NK, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, add_groups(NK)) lora_add_kernel(const LoraArgs a) {
   using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, GMM_A_STAGED, 1>;
-  constexpr int FR = S::FR, OUT = S::COLUMNS;
+  constexpr int FR = S::FR, OUT = S::COLUMNS, POLICY = ALIGNED ? kStream : 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int first = (blockIdx.x * kWaves + wave) * 16;
   const int id = first + j < a.rows ? a.adapter[first + j] : -1;
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, NK == 1 ? 3 : 2) lora_add_kernel(con
     const uint32_t at = y_at + uint32_t(min(c, a.N - FR)) * 2;
 #pragma unroll
     for (int v = 0; v < 4; ++v)
-      old[v] = __builtin_amdgcn_raw_buffer_load_b128(y, int(mine >> (4 * g + v) & 1 && c < a.N ? at + v * y_step : kNowhere), 0, 0);
+      old[v] = __builtin_amdgcn_raw_buffer_load_b128(y, int(mine >> (4 * g + v) & 1 && c < a.N ? at + v * y_step : kNowhere), 0, POLICY);
   };
   const auto store_y = [&](const float (&now)[4][FR], int tile, uint32_t mine) {
     const int c = (tile0 + tile) * OUT + FR * j, left = a.N - c;
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, NK == 1 ? 3 : 2) lora_add_kernel(con
     for (int v = 0; v < 4; ++v) {
       const u32x4 p = Pack<T, 8>::of(now[v]).w;
       const bool in = mine >> (4 * g + v) & 1;
-      __builtin_amdgcn_raw_buffer_store_b128(p, y, int(in && left >= FR ? at + v * y_step : kNowhere), 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(p, y, int(in && left >= FR ? at + v * y_step : kNowhere), 0, POLICY);
       if (in && left > 0 && left < FR) {      // the lane that has fewer than eight: they are the last ones of what it loaded
         const uint32_t last = at + v * y_step + 2 * left - 2;
 #pragma unroll
@@ -883,13 +887,14 @@ int launch_add(LoraArgs a, hipStream_t stream) {
   if (a.N) {
     const int lay = layout_of_b(a.b, a.R, a.N);
     const dim3 any((a.rows + kAnyRows - 1) / kAnyRows, (a.N + kThreads - 1) / kThreads);
-    // strips to a wave: as many as leave every place for one a wave
+    // strips to a wave: as many as leave every place for one a wave (rank 64: for three groups 54 us, for the two that there is room for 50)
     const int tiles = (a.N + 127) / 128, row_groups = (a.rows + 16 * kWaves - 1) / (16 * kWaves);
-    a.strips = clamp(int64_t(row_groups) * tiles / (3 * gmm_num_cus()), 1, tiles);
+    a.strips = clamp(int64_t(row_groups) * tiles / (add_groups(a.R <= 32 ? 1 : 2) * gmm_num_cus()), 1, tiles);
     const dim3 grid(row_groups, (tiles + a.strips - 1) / a.strips);
     const auto launch = [&](auto lay, auto nk) {
       constexpr int B = decltype(lay)::value, NK = decltype(nk)::value;
-      hipLaunchKernelGGL((lora_add_kernel<T, B, NK>), grid, dim3(kThreads), 0, stream, a);
+      if (aligned16(a.out) && a.out_ld % 8 == 0) hipLaunchKernelGGL((lora_add_kernel<T, B, NK, true>), grid, dim3(kThreads), 0, stream, a);
+      else hipLaunchKernelGGL((lora_add_kernel<T, B, NK, false>), grid, dim3(kThreads), 0, stream, a);
     };
     const auto rank = [&](auto lay) {
       if (a.R <= 32) launch(lay, std::integral_constant<int, 1>{});
