@@ -2,11 +2,13 @@
 //   y[t] = x[t] @ W + scale[i] * (x[t] @ A[i]) @ B[i],  i = adapter[t]; a number outside [0, L): no adapter
 // and the adapters' gradients.
 //   A few rows (gmm_lora_linear): W and the adapters are read once, past the rows (gmm_skinny.h), in one launch; a second one adds the
-//     parts up.  Reading W bounds it.
+//     parts up.  Reading W bounds it: 48 rows of 64 adapters of rank 16, 4096 -> 8192, 25 us, of which W takes 9.5 at the fastest reads; of one
+//     row, 4096 -> 4096, 12 us, mostly the two launches and the trips to memory behind one another.
 //   Many rows (gmm_lora_add): W's product is a grouped product of one group; what the adapters add is two thin products, bound by
-//     reading x and by reading and writing y.
+//     reading x and by reading and writing y: 8192 rows of 4096 -> 4096, rank 16, 52 us (201 MB, 3.9 TB/s).
 //   Gradients (gmm_lora_grad): dA[i] = scale[i] * sum of x[t]^T u[t], dB[i] = scale[i] * sum of low[t]^T dy[t] over the rows t that have
-//     adapter i: thin products along the rows, bound by reading x and dy.
+//     adapter i: thin products along the rows, bound by reading x and dy: of those 8192 rows 30 us (134 MB, 4.5 TB/s), and 20 for the sort before
+//     and the sums behind.
 // The rank-sized values x @ A and dy @ B^T stay in fp32; where they are operands of a 16-bit product they are two values each.
 #include <hip/hip_runtime.h>
 

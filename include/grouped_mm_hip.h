@@ -241,11 +241,12 @@ int gmm_moe_combine(const void* y, const int32_t* token_rows, const float* slot_
  *   out[t, :] = sum_{j < top_k} slot_weight[t, j] * act(x[t, :] @ w_up[e_tj]) @ w_down[e_tj].
  * x [tokens, hidden], logits [tokens, experts], w_up [experts, hidden, inner] or, for the two SwiGLU kinds, [.., 2 * inner] (gate
  * columns, then partners, or 64 and 64 in turn as gmm_2d3d_swiglu has them: inner a multiple of 64), w_down [experts, inner, hidden];
- * strides in elements, any for the weights (16-byte aligned ones contiguous along either dimension are read fastest), rows of x,
+ * strides in elements, any for the weights (those contiguous along either dimension are read fastest, at any alignment), rows of x,
  * logits and out contiguous; one expert's matrix below 2 GiB.  dtype bf16 or fp16, logits_dtype any gmm_dtype.  Unlike the calls
  * it stands for it keeps the activations and the experts' results in 32 bits and rounds once.  `workspace`: device memory of
  * gmm_moe_few_workspace_bytes(...) bytes (-1: sizes out of range), 16-byte aligned, its contents of no matter.  No host
- * synchronisation, no allocation, no atomics. */
+ * synchronisation, no allocation.  Two to five launches; up to 32 slots the second product's workgroups count their arrivals with an
+ * atomic, which decides who adds up, not what or in which order: the result does not depend on timing. */
 enum gmm_activation { GMM_ACT_SILU = 0, GMM_ACT_SWIGLU = 1, GMM_ACT_SWIGLU_INTERLEAVED = 2 };
 int64_t gmm_moe_few_workspace_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner);
 int gmm_moe_few(const void* x, const void* logits, const void* w_up, const void* w_down, void* out,
@@ -259,7 +260,7 @@ int gmm_moe_few(const void* x, const void* logits, const void* w_up, const void*
 /* ---- A projection that all rows share beside low-rank adapters of which each row has its own.  No counterpart in the reference.
  *   out[t] = x[t] @ w + scale[i] * (x[t] @ a[i]) @ b[i],  i = adapter[t];  i outside [0, L): x[t] @ w alone.
  * x [rows, K], w [K, N], a [L, K, R], b [L, R, N], out [rows, N] in bf16 or fp16 (dtype), adapter int32[rows], scale float[L] (NULL: ones);
- * strides in elements, any for w, a and b (16-byte aligned and contiguous along one dimension: fastest), rows of x and out contiguous.
+ * strides in elements, any for w, a and b (contiguous along one dimension: fastest, at any alignment), rows of x and out contiguous.
  * R <= 256, L <= 1022, one matrix below 2 GiB.  `low`: float [rows, R], gets x[t] @ a[i] of the rows that have an adapter (NULL: not wanted;
  * gmm_lora_grad needs it).  x @ a stays in fp32.  `workspace`: device memory of gmm_lora_workspace_bytes(...) bytes (-1: sizes out of
  * range), 16-byte aligned, contents of no matter.
