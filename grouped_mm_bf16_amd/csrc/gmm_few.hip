@@ -33,6 +33,10 @@ constexpr int kRouteSlots = 32, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
 constexpr int kJoinSlots = 32;
 constexpr int kLine = 32;          // words from one counter to the next: 384 arrivals at 16 counters of one cache line took 8 us
 
+// Workgroups that a compute unit is to hold: two where their sums leave the registers.  Column-major, 33 tokens and more (strips of half as many
+// columns): 64 tokens through 8 of 128 experts of 2048 -> 2 x 768 214 us, held to two 202; 40 through 4 of 8 of 432 -> 2 x 10752 108 and 88.
+constexpr int few_groups(int lay, int MF) { return lay == GMM_W_COLS || (lay == GMM_W_ROWS && MF <= 2) ? 2 : 1; }
+
 struct FewArgs {
   const void* x;
   const void* w;            // w_up or w_down
@@ -164,7 +168,7 @@ __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x));
 // act[r] = act(x[token of row r] @ w_up[e]), or parts of the product.  GLU: a strip is 8 * FR gate columns and their partners.
 // SIDE: the waves of a workgroup take strips side by side and all of k, and have no sums to share.
 template <typename T, int LAY, int MF, bool GLU, bool ROUTE, bool SIDE>
-__global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1) few_up_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(kThreads, few_groups(LAY, MF)) few_up_kernel(const FewArgs a) {
   using S = Strip<T, LAY, MF, 1>;
   constexpr int FR = S::FR, OUT = GLU ? 8 * FR : 16 * FR;
   __shared__ SkinnyShared<S, kWaves> shared;
@@ -240,7 +244,7 @@ constexpr int kDeviceScope = 16;   // sc1
 // y[part][r] = act[r] @ w_down[e], over the part's range of k; with a.join the result as well.
 // PARTS: the first product lies in parts; a workgroup adds up those that it needs, and keeps their activations in LDS.
 template <typename T, int LAY, int MF, bool PARTS>
-__global__ void __launch_bounds__(kThreads, MF <= 2 && LAY != GMM_W_ANY ? 2 : 1) few_down_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(kThreads, few_groups(LAY, MF)) few_down_kernel(const FewArgs a) {
   using S = Strip<T, LAY, MF, 2, PARTS ? GMM_A_RESIDENT : LAY == GMM_W_ANY ? GMM_A_ELEMENTS : GMM_A_STAGED>;
   constexpr int FR = S::FR, OUT = 16 * FR;
   __shared__ SkinnyShared<S, kWaves> shared;

@@ -2,7 +2,7 @@
 //   y[t] = x[t] @ W + scale[i] * (x[t] @ A[i]) @ B[i],  i = adapter[t]; a number outside [0, L): no adapter
 // and the adapters' gradients.
 //   A few rows (gmm_lora_linear): W and the adapters are read once, past the rows (gmm_skinny.h), in one launch; a second one adds the
-//     parts up.  Reading W bounds it: 48 rows of 64 adapters of rank 16, 4096 -> 8192, 25 us, of which W takes 9.5 at the fastest reads; of one
+//     parts up.  Reading W bounds it: 48 rows of 64 adapters of rank 16, 4096 -> 8192, 23 us, of which W takes 9.5 at the fastest reads; of one
 //     row, 4096 -> 4096, 12 us, mostly the two launches and the trips to memory behind one another.
 //   Many rows (gmm_lora_add): W's product is a grouped product of one group; what the adapters add is two thin products, bound by
 //     reading x and by reading and writing y: 8192 rows of 4096 -> 4096, rank 16, 52 us (201 MB, 3.9 TB/s).
@@ -31,6 +31,10 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves;
 // Waves of a workgroup of a few rows' launch: eight, four where the sums of 64 rows by 128 columns, or what is loaded element by element,
 // need half of the registers.
 constexpr int few_waves(int MF, int lay) { return MF == 4 || (MF == 2 && lay == GMM_W_ANY) ? 4 : 8; }
+
+// ... and how many of four waves a compute unit is to hold: two where half of the registers do (48 rows, 64 adapters, column-major 4096 -> 8192
+// 24.5 -> 23.2 us: all workgroups, those of the adapters and those of W, then run at once).
+constexpr int few_at_once(int MF, int lay) { return MF == 4 && lay == GMM_W_COLS ? 2 : 1; }
 
 struct Matrices {          // a stack [L, K, N] of 16-bit matrices, or one
   const void* at;
@@ -187,7 +191,7 @@ __global__ void __launch_bounds__(64 * low_waves(FR), FR == 1 ? 4 : FR == 2 ? 3 
 
 // A few rows: workgroups for x @ A first, then those for x @ W: base[part][t] over a part of K.
 template <typename T, int LAY_W, int LAY_A, int MF>
-__global__ void __launch_bounds__(64 * few_waves(MF, LAY_W)) lora_few_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(64 * few_waves(MF, LAY_W), few_at_once(MF, LAY_W)) lora_few_kernel(const LoraArgs a) {
   constexpr int WAVES = few_waves(MF, LAY_W);
   using S = Strip<T, LAY_W, MF, 1>;
   using SA = LowSkinny<T, LAY_A, 1, LAY_W == GMM_W_ANY>;
