@@ -94,6 +94,29 @@ __device__ __forceinline__ bool find_expert(const FewArgs& a, int which, int& ex
   return found;
 }
 
+// f(i, in) for all i < n, eight and then four at a time: as many loads are on their way together.  Past the end the last one again, `in` false.
+// (A loop that the compiler unrolls takes what is left over one by one: a trip to memory each.)
+template <typename F>
+__device__ __forceinline__ void in_fours(int n, F&& f) {
+  int i = 0;
+  for (; i + 4 < n; i += 8)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f(min(i + u, n - 1), i + u < n);
+  if (i < n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f(min(i + u, n - 1), i + u < n);
+}
+
+// The parts of the choices of a token, one after the other; behind the last one that one's first part again.
+struct Choice {
+  int j, part;
+  __device__ __forceinline__ void next(const FewArgs& a) {
+    const bool last = ++part == a.parts;
+    part = last ? 0 : part;
+    j = min(j + last, a.top_k - 1);
+  }
+};
+
 // Routing by every workgroup for itself: up to kRouteSlots slots, kRouteExperts experts, a wave to a token.  The first workgroup leaves the
 // results for the kernels behind.  Rows are sorted by expert, stably, as gmm_moe_route has them.
 struct FewRouting {
@@ -280,11 +303,12 @@ __global__ void __launch_bounds__(kThreads, few_groups(LAY, MF)) few_down_kernel
       float gate = 0, partner = 0;
       if (from + c < to) {
         const float* at = a.part + int64_t(row0 + r) * columns + from + c;
-#pragma unroll 8
-        for (int p = 0; p < a.up_parts; ++p, at += int64_t(a.slots) * columns) {
-          gate += at[0];
-          if (a.kind != GMM_ACT_SILU) partner += at[a.inner];
-        }
+        in_fours(a.up_parts, [&](int p, bool in) {
+          const float* const here = at + int64_t(p) * a.slots * columns;
+          const float g = here[0], u = a.kind == GMM_ACT_SILU ? 0.0f : here[a.inner];
+          gate += in ? g : 0.0f;
+          partner += in ? u : 0.0f;
+        });
       }
       T* const keep = reinterpret_cast<T*>(resident + r * s.pitch) + c;
       split(silu(gate) * (a.kind == GMM_ACT_SILU ? 1.0f : partner), keep[0], *reinterpret_cast<T*>(reinterpret_cast<char*>(keep) + s.a_plane));
@@ -337,12 +361,14 @@ __global__ void __launch_bounds__(kThreads, few_groups(LAY, MF)) few_down_kernel
     const int t = u / OUT, col = tile * OUT + u % OUT;
     if (col >= a.H) continue;
     float sum = 0;
-#pragma unroll 8
-    for (int q = 0; q < a.top_k * a.parts; ++q) {
-      const int slot = t * a.top_k + q / a.parts;
-      const uint32_t at = (uint32_t(q % a.parts) * a.slots + slot_row[slot]) * a.H + col;
-      sum += slot_weight[slot] * __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(y, int(at * 4), 0, kDeviceScope));
-    }
+    Choice q{0, 0};
+    in_fours(a.top_k * a.parts, [&](int, bool in) {
+      const int slot = t * a.top_k + q.j;
+      const uint32_t at = (uint32_t(q.part) * a.slots + slot_row[slot]) * a.H + col;
+      const float v = slot_weight[slot] * __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(y, int(at * 4), 0, kDeviceScope));
+      sum += in ? v : 0.0f;
+      q.next(a);
+    });
     static_cast<T*>(a.out)[t * a.out_ld + col] = rounded<T>(sum);
   }
 }
@@ -351,36 +377,22 @@ __global__ void __launch_bounds__(kThreads, few_groups(LAY, MF)) few_down_kernel
 // way together: one after the other 6 of 32 tokens took 14 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) few_combine_kernel(const FewArgs a) {
-  __shared__ uint32_t from[32];
-  __shared__ float weight[32];
-  const int t = blockIdx.y, c = blockIdx.x * kThreads + threadIdx.x;
-  if (int(threadIdx.x) < a.top_k) {
-    from[threadIdx.x] = uint32_t(a.token_rows[t * a.top_k + threadIdx.x]) * a.H;
-    weight[threadIdx.x] = a.slot_weight[t * a.top_k + threadIdx.x];
-  }
-  __syncthreads();
-  if (c >= a.H) return;
+  const int t = blockIdx.y, c = blockIdx.x * kThreads + threadIdx.x, lane = threadIdx.x & 63;
+  // of choice j: in lane j
+  const int mine = t * a.top_k + min(lane, a.top_k - 1);
+  const int from = a.token_rows[mine] * a.H, weight = __builtin_bit_cast(int, a.slot_weight[mine]);
   const uint32_t next = uint32_t(a.slots) * a.H;
-  const float* const y = a.y + c;
-  float sum = 0;
-  const auto add = [&](auto parts) {
-    constexpr int P = decltype(parts)::value;
-#pragma unroll 8 / P
-    for (int j = 0; j < a.top_k; ++j) {
-      float v = 0;
-      if constexpr (P == 8) {
-#pragma unroll 8
-        for (int p = 0; p < a.parts; ++p) v += y[from[j] + p * next];
-      } else {
-#pragma unroll
-        for (int p = 0; p < P; ++p) v += y[from[j] + p * next];
-      }
-      sum += weight[j] * v;
-    }
-  };
-  if (a.parts == 1) add(std::integral_constant<int, 1>{});
-  else if (a.parts == 2) add(std::integral_constant<int, 2>{});
-  else add(std::integral_constant<int, 8>{});
+  const float* const y = a.y + min(c, a.H - 1);      // every lane has its part in the lookup
+  float sum = 0, v = 0;
+  Choice q{0, 0};
+  in_fours(a.top_k * a.parts, [&](int, bool in) {
+    const float one = (y + uint32_t(__builtin_amdgcn_readlane(from, q.j)))[q.part * next];
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(weight, q.j));
+    v = in ? (q.part ? v : 0.0f) + one : v;
+    if (in && q.part == a.parts - 1) sum += w * v;
+    q.next(a);
+  });
+  if (c >= a.H) return;
   static_cast<T*>(a.out)[t * a.out_ld + c] = rounded<T>(sum);
 }
 
