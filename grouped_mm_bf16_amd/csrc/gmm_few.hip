@@ -28,9 +28,9 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kRouteSlots = 32, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
 
 // Slots up to which the second product's last workgroup of some columns adds them up: a launch less, but one workgroup reads what otherwise
-// all of them would.  3 tokens, 6 of 23 experts of 680 -> 2 x 2648 58 us, with a launch for the sums 63; 16 tokens, 4 of 8 experts of
-// 432 -> 2 x 10752 81 and 60.
-constexpr int kJoinSlots = 32;
+// all of them would.  2 tokens, 6 of 34 experts of 280 -> 600 16 us, with a launch for the sums 17 (1 token of small experts 15 and 16); 6
+// tokens, 4 of 8 experts of 432 -> 2 x 10752 60 and 56.
+constexpr int kJoinSlots = 16;
 constexpr int kLine = 32;          // words from one counter to the next: 384 arrivals at 16 counters of one cache line took 8 us
 
 // Workgroups that a compute unit is to hold: two where their sums leave the registers.  Column-major, 33 tokens and more (strips of half as many
@@ -92,19 +92,6 @@ __device__ __forceinline__ bool find_expert(const FewArgs& a, int which, int& ex
     if (found && !a.join) break;      // nobody wants to know the rest
   }
   return found;
-}
-
-// f(i, in) for all i < n, eight and then four at a time: as many loads are on their way together.  Past the end the last one again, `in` false.
-// (A loop that the compiler unrolls takes what is left over one by one: a trip to memory each.)
-template <typename F>
-__device__ __forceinline__ void in_fours(int n, F&& f) {
-  int i = 0;
-  for (; i + 4 < n; i += 8)
-#pragma unroll
-    for (int u = 0; u < 8; ++u) f(min(i + u, n - 1), i + u < n);
-  if (i < n)
-#pragma unroll
-    for (int u = 0; u < 4; ++u) f(min(i + u, n - 1), i + u < n);
 }
 
 // The parts of the choices of a token, one after the other; behind the last one that one's first part again.

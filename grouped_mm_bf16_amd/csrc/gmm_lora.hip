@@ -239,8 +239,10 @@ __global__ void __launch_bounds__(64 * few_waves(MF, LAY_W), few_at_once(MF, LAY
 // Sums of the parts of x @ A of one row, times its adapter's scale.
 __device__ __forceinline__ float low_sum(const LoraArgs& a, int row, int r) {
   float s = 0;
-#pragma unroll 4
-  for (int p = 0; p < a.low_parts; ++p) s += a.low[(int64_t(p) * a.rows + row) * a.R + r];
+  in_fours(a.low_parts, [&](int p, bool in) {
+    const float v = a.low[(int64_t(p) * a.rows + row) * a.R + r];
+    s += in ? v : 0.0f;
+  });
   return s;
 }
 
@@ -269,16 +271,17 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
   if (own < a.N) {
     const float* base = a.base + int64_t(t) * a.N + c;
     const int64_t next = int64_t(a.rows) * a.N;
-#pragma unroll 4
-    for (int p = 0; p < a.base_parts; ++p, base += next) {
+    in_fours(a.base_parts, [&](int p, bool in) {
+      const float* const at = base + p * next;
       if constexpr (W == 8) {
-        const f32x4 lo = unaligned<f32x4>(base), hi = unaligned<f32x4>(base + 4);
+        const f32x4 lo = unaligned<f32x4>(at), hi = unaligned<f32x4>(at + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
+        for (int i = 0; i < 4; ++i) { y[i] += in ? lo[i] : 0.0f; y[4 + i] += in ? hi[i] : 0.0f; }
       } else {
-        y[0] += base[0];
+        const float v = at[0];
+        y[0] += in ? v : 0.0f;
       }
-    }
+    });
   }
   const bool has = has_adapter(id, a.L);
   const float scale = has && a.scale ? a.scale[id] : 1.0f;

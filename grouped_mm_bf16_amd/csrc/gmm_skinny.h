@@ -391,6 +391,19 @@ union SkinnyShared {
   __device__ SkinnyShared() {}
 };
 
+// f(i, in) for all i < n, eight and then four at a time: as many loads are on their way together.  Past the end the last one again, `in` false.
+// (A loop that the compiler unrolls takes what is left over one by one: a trip to memory each.)
+template <typename F>
+__device__ __forceinline__ void in_fours(int n, F&& f) {
+  int i = 0;
+  for (; i + 4 < n; i += 8)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f(min(i + u, n - 1), i + u < n);
+  if (i < n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f(min(i + u, n - 1), i + u < n);
+}
+
 // ---------------------------------------------------------------- host side
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 

@@ -245,7 +245,7 @@ int gmm_moe_combine(const void* y, const int32_t* token_rows, const float* slot_
  * logits and out contiguous; one expert's matrix below 2 GiB.  dtype bf16 or fp16, logits_dtype any gmm_dtype.  Unlike the calls
  * it stands for it keeps the activations and the experts' results in 32 bits and rounds once.  `workspace`: device memory of
  * gmm_moe_few_workspace_bytes(...) bytes (-1: sizes out of range), 16-byte aligned, its contents of no matter.  No host
- * synchronisation, no allocation.  Two to five launches; up to 32 slots the second product's workgroups count their arrivals with an
+ * synchronisation, no allocation.  Two to five launches; up to 16 slots the second product's workgroups count their arrivals with an
  * atomic, which decides who adds up, not what or in which order: the result does not depend on timing. */
 enum gmm_activation { GMM_ACT_SILU = 0, GMM_ACT_SWIGLU = 1, GMM_ACT_SWIGLU_INTERLEAVED = 2 };
 int64_t gmm_moe_few_workspace_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner);
