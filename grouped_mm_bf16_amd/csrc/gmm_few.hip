@@ -1,11 +1,11 @@
 // A mixture-of-experts layer for a few tokens (gmm_moe_few in include/grouped_mm_hip.h):
 //   out[t] = sum over the choices j of w_tj * act(x[t] @ w_up[e_tj]) @ w_down[e_tj]
 // Routing as gmm_moe_route, then every chosen expert's matrices are read once, past a few rows (gmm_skinny.h).  Reading them bounds
-// it: 8 tokens, 2 of 8 experts of 4096 -> 2 x 14336 368 us (7.0 TB/s), 32 tokens, 8 of 128 experts of 2048 -> 2 x 768 157 us (6.7 TB/s).
+// it: 8 tokens, 2 of 8 experts of 4096 -> 2 x 14336 361 to 397 us by card (7.0 to 6.4 TB/s), 32 tokens, 8 of 128 experts of 2048 -> 2 x 768 151 to 160 us (7.0 to 6.6).
 // Between the two products the activations stay in 32 bits (two 16-bit values each), the second products in fp32: the result is
 // rounded once.
 // Of very few tokens the time is that of the launches and of the trips to memory behind one another (1 token, 8 of 128 experts of
-// 2048 -> 2 x 768 28 us, of which the weights are 11).  Then there are two launches: every workgroup of the first routes for
+// 2048 -> 2 x 768 25 us, of which the weights are 11).  Then there are two launches: every workgroup of the first routes for
 // itself, and of the second's, the last that is done with some columns adds them up.
 #include <hip/hip_runtime.h>
 
