@@ -51,8 +51,9 @@ struct Chunk {
   __device__ __forceinline__ bool own(int i) const { return in && (!TAIL || i >= skip); }
 };
 
-// A chunk of a row that is read once.  Non-temporal, which keeps it from driving out what is written (4096 x 16384 fp32 99 -> 81 us), but not
-// where chunks begin anywhere: neighbours then share cache lines (21800 x 329 fp32 11.8 -> 15.3 us).
+// A chunk of a row that is read once.  Non-temporal, which keeps it from driving out what is written (4096 x 16384 fp32 99 -> 81 us; rows that
+// lie at odd addresses too: 8192 x 14336 fp16, 14337 apart, 111 -> 103), but not where a row ends inside a chunk: two lanes then read its
+// last cache line, one after the other (21800 x 329 fp32 11.8, non-temporal 15.3 us).
 template <typename T, int N, bool TAIL>
 __device__ __forceinline__ Pack<T, N> load_row(const T* row, const Chunk<N, TAIL>& c) {
   if constexpr (TAIL || N == 1) {
