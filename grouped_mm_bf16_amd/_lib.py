@@ -48,6 +48,7 @@ SIGNATURES = {
     "gmm_lora_workspace_bytes": (_i64, [_i64] * 4),
     "gmm_lora_linear": (ctypes.c_int, [_vp] * 8 + [_i64] * 15 + [_i32, _vp, _i64, _vp]),
     "gmm_lora_add": (ctypes.c_int, [_vp] * 7 + [_i64] * 13 + [_i32, _vp, _i64, _vp]),
+    "gmm_lora_sum": (ctypes.c_int, [_vp] * 8 + [_i64] * 13 + [_i32, _vp, _i64, _vp]),
     "gmm_lora_grad_workspace_bytes": (_i64, [_i64] * 5),
     "gmm_lora_grad": (ctypes.c_int, [_vp] * 8 + [_i64] * 13 + [_i32, _vp, _i64, _vp]),
     "gmm_layer_norm": (ctypes.c_int, [_vp] * 6 + [_i64] * 4 + [ctypes.c_float, _i32, _i32, _vp]),

@@ -4,8 +4,8 @@
 //   A few rows (gmm_lora_linear): W and the adapters are read once, past the rows (gmm_skinny.h), in one launch; a second one adds the
 //     parts up.  Reading W bounds it: 48 rows of 64 adapters of rank 16, 4096 -> 8192, 23 us, of which W takes 9.5 at the fastest reads; of one
 //     row, 4096 -> 4096, 12 us, mostly the two launches and the trips to memory behind one another.
-//   Many rows (gmm_lora_add): W's product is a grouped product of one group; what the adapters add is two thin products, bound by
-//     reading x and by reading and writing y: 8192 rows of 4096 -> 4096, rank 16, 52 us (201 MB, 3.9 TB/s).
+//   Many rows (gmm_lora_sum): W's product is a grouped product of one group, in fp32; what the adapters add is two thin products, bound by
+//     reading x, by reading that product and by writing y: 8192 rows of 4096 -> 4096, rank 16, 69 us (268 MB, 3.9 TB/s).
 //   Gradients (gmm_lora_grad): dA[i] = scale[i] * sum of x[t]^T u[t], dB[i] = scale[i] * sum of low[t]^T dy[t] over the rows t that have
 //     adapter i: thin products along the rows, bound by reading x and dy: of those 8192 rows 30 us (134 MB, 4.5 TB/s), and 20 for the sort before
 //     and the sums behind.
@@ -52,7 +52,7 @@ struct LoraArgs {
   float* low;              // [low_parts][rows][R]: parts of x @ A
   float* low_out;          // [rows][R]: their sums, null: not wanted
   void* planes;            // many rows: [2][rows][pitch], null: not wanted
-  float* base;             // [base_parts][rows][N]: parts of x @ W
+  float* base;             // [base_parts][rows][N]: parts of x @ W; without any: it lies in `out`
   int64_t x_ld, out_ld;
   int32_t rows, K, N, R, L;
   int32_t strip_rows, low_parts, low_k, low_tiles;   // rows of a strip; parts of K and their length; strips of columns of A
@@ -343,42 +343,65 @@ __global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a)
   if (has_adapter(id, a.L)) keep_low<T>(a, row, r, r < a.R ? low_sum(a, row, r) : 0.0f, a.scale ? a.scale[id] : 1.0f);
 }
 
-// Many rows: y[t] += scale * low @ B.  A wave takes 16 rows and strips of 128 columns, one after the other; y is read and written where
-// it is, 16 bytes to a lane.  The next strip's y and B are on their way while one is written: of 4 waves and one strip
-// at a time 8192 x 4096 took 65 us, five trips to memory one after the other for each.  NK: steps of 32 of the rank that are held.
-// ALIGNED: y's rows begin at whole 16 bytes; its accesses are then non-temporal (8192 x 4096, with x @ A 57 -> 52 us).  Elsewhere neighbours
-// share cache lines, and are not (8192 x 4099 72 us, non-temporal 75).
-constexpr int add_groups(int NK) { return NK == 1 ? 3 : 2; }      // that a compute unit holds
+// Eight values of x @ W on their way: two to a register where they lie in y, fp32 elsewhere.
+template <typename T> struct OnTheWay {
+  u32x4 w;
+  __device__ __forceinline__ float get(int i) const { return widen(T{uint16_t(w[i / 2] >> 16 * (i & 1))}); }
+};
+template <> struct OnTheWay<float> {
+  u32x4 w[2];
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float(w[i / 4][i % 4]); }
+};
 
-template <typename T, int LAY, int NK, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, add_groups(NK)) lora_add_kernel(const LoraArgs a) {
+// Many rows: y[t] = x @ W + scale * low @ B, for x @ W in fp32 (P float: all rows are written, and rounded once) or in y as it is (P = T: the
+// rows that have an adapter).  A wave takes 16 rows and strips of 128 columns, one after the other, 16 bytes to a lane.  The next strip's
+// x @ W and B are on their way while one is written: of 4 waves and one strip at a time 8192 x 4096 took 65 us, five trips to memory one after the other for each.
+// NK: steps of 32 of the rank that are held.
+// ALIGNED: y's rows begin at whole 16 bytes; its accesses are then non-temporal (P = T, 8192 x 4096, with x @ A 57 -> 52 us).  Elsewhere
+// neighbours share cache lines, and are not (8192 x 4099 72 us, non-temporal 75).  Nor is x @ W in fp32, which the product has just
+// written (8192 rows of 4096 -> 4096 with the product 285 -> 282 us).
+// that a compute unit holds; of fp32 rows three would spill (column-major B) or give nothing (282 us both ways)
+constexpr int add_groups(int NK, bool here) { return NK == 1 && here ? 3 : 2; }
+
+template <typename T, typename P, int LAY, int NK, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, add_groups(NK, sizeof(P) == 2)) lora_add_kernel(const LoraArgs a) {
   using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, GMM_A_STAGED, 1>;
   constexpr int FR = S::FR, OUT = S::COLUMNS, POLICY = ALIGNED ? kStream : 0;
+  constexpr bool HERE = sizeof(P) == 2;      // x @ W lies in y
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int first = (blockIdx.x * kWaves + wave) * 16;
   const int id = first + j < a.rows ? a.adapter[first + j] : -1;
   const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L))) & 0xffffu;
-  if (!with) return;
+  const int there = min(16, a.rows - first);
+  if (HERE ? !with : there <= 0) return;
+  const uint32_t none = HERE ? 0 : ~with & ((1u << there) - 1);      // rows that only have to be rounded
   const T* const high = static_cast<const T*>(a.planes) + int64_t(min(first + j, a.rows - 1)) * a.pitch + 8 * g;
   const T* const low = high + int64_t(a.rows) * a.pitch;
   const int tile0 = blockIdx.y * a.strips, tiles = min(a.strips, (a.N + OUT - 1) / OUT - tile0);
   // y from row `first` on; what is not to be read or written lies nowhere, so that no branch stands around an access
-  const int there = min(16, a.rows - first);
   const __amdgpu_buffer_rsrc_t y = buffer(static_cast<T*>(a.out) + first * a.out_ld, uint32_t(((there - 1) * a.out_ld + a.N) * 2));
   const uint32_t y_at = uint32_t(4 * g) * uint32_t(a.out_ld) * 2, y_step = uint32_t(a.out_ld) * 2;
-  const auto load_y = [&](u32x4 (&old)[4], int tile, uint32_t mine) {
+  const __amdgpu_buffer_rsrc_t base = HERE ? y : buffer(a.base + int64_t(first) * a.N, uint32_t(there) * a.N * 4);
+  const auto load_y = [&](OnTheWay<P> (&old)[4], int tile, uint32_t mine) {
     const int c = (tile0 + tile) * OUT + FR * j;
-    const uint32_t at = y_at + uint32_t(min(c, a.N - FR)) * 2;
+    const uint32_t step = HERE ? y_step : uint32_t(a.N) * 4, at = 4 * g * step + uint32_t(min(c, a.N - FR)) * uint32_t(sizeof(P));
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-      old[v] = __builtin_amdgcn_raw_buffer_load_b128(y, int(mine >> (4 * g + v) & 1 && c < a.N ? at + v * y_step : kNowhere), 0, POLICY);
+    for (int v = 0; v < 4; ++v) {
+      const int from = int(mine >> (4 * g + v) & 1 && c < a.N ? at + v * step : kNowhere);
+      if constexpr (HERE) {
+        old[v].w = __builtin_amdgcn_raw_buffer_load_b128(base, from, 0, POLICY);
+      } else {
+        old[v].w[0] = __builtin_amdgcn_raw_buffer_load_b128(base, from, 0, 0);
+        old[v].w[1] = __builtin_amdgcn_raw_buffer_load_b128(base, from, 16, 0);
+      }
+    }
   };
-  const auto store_y = [&](const float (&now)[4][FR], int tile, uint32_t mine) {
+  const auto store_y = [&](const u32x4 (&now)[4], int tile, uint32_t mine) {
     const int c = (tile0 + tile) * OUT + FR * j, left = a.N - c;
     const uint32_t at = y_at + uint32_t(c) * 2;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const u32x4 p = Pack<T, 8>::of(now[v]).w;
+      const u32x4 p = now[v];
       const bool in = mine >> (4 * g + v) & 1;
       __builtin_amdgcn_raw_buffer_store_b128(p, y, int(in && left >= FR ? at + v * y_step : kNowhere), 0, POLICY);
       if (in && left > 0 && left < FR) {      // the lane that has fewer than eight: they are the last ones of what it loaded
@@ -415,7 +438,8 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK)) lora_add_kernel(cons
     }
   };
   // strips, and in a strip the adapters of the rows, one after the other: one sequence
-  u32x4 h[NK], l[NK], w[NK][8], next[4];
+  u32x4 h[NK], l[NK], w[NK][8];
+  OnTheWay<P> next[4];
   const auto load_low = [&](int k) {
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
@@ -433,8 +457,13 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK)) lora_add_kernel(cons
   load_low(0);
   Adapters ahead{with, 0, 0};
   int tile = 0;
-  ahead.next(id);
-  s.w_buf = matrix<T>(a.b, ahead.which);
+  const auto go_on = [&] {      // rows without an adapter come with a strip's first adapter, or alone
+    const bool first_one = ahead.todo == with;
+    if (HERE || with) ahead.next(id);
+    ahead.mine = first_one ? ahead.mine | none : ahead.mine;
+    s.w_buf = HERE || with ? matrix<T>(a.b, ahead.which) : buffer(a.b.at, 0);
+  };
+  go_on();
 #pragma unroll
   for (int n = 0; n < NK; ++n) load_b(w[n], 0, 32 * n);
   load_y(next, 0, ahead.mine);
@@ -461,18 +490,20 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK)) lora_add_kernel(cons
       ahead.todo = with;
       ++tile;
     }
-    ahead.next(id);
-    s.w_buf = matrix<T>(a.b, ahead.which);
+    go_on();
     const int then = min(tile, tiles - 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < NK; ++n) load_b(w[n], then, 32 * n);
     __builtin_amdgcn_sched_barrier(0);
-    float now[4][FR];
+    u32x4 now[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < 4; ++v) {
+      float sum[FR];
 #pragma unroll
-      for (int i = 0; i < FR; ++i) now[v][i] = widen(T{uint16_t(next[v][i / 2] >> 16 * (i & 1))}) + acc[i][v];
+      for (int i = 0; i < FR; ++i) sum[i] = next[v].get(i) + (HERE || with >> (4 * g + v) & 1 ? acc[i][v] : 0.0f);
+      now[v] = Pack<T, 8>::of(sum).w;
+    }
     load_y(next, then, tile < tiles ? ahead.mine : 0);
     __builtin_amdgcn_sched_barrier(0);
     store_y(now, here, mine);
@@ -482,8 +513,9 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK)) lora_add_kernel(cons
 // The same where neither step of B is one element, or there are fewer than eight columns: a thread has one column and 16 rows, and multiplies on the vector units, in fp32.
 constexpr int kAnyRows = 16;
 
-template <typename T>
+template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads) lora_add_any_kernel(const LoraArgs a) {
+  constexpr bool HERE = sizeof(P) == 2;      // as above
   __shared__ f32x4 low[kAnyRows][kMaxRank / 4 + 1];
   const int row0 = blockIdx.x * kAnyRows, c = blockIdx.y * kThreads + threadIdx.x, lane = threadIdx.x & 63;
   const int span = int(a.R + 3) / 4 * 4;
@@ -496,6 +528,11 @@ __global__ void __launch_bounds__(kThreads) lora_add_any_kernel(const LoraArgs a
   const int id = lane < kAnyRows && row0 + lane < a.rows ? a.adapter[row0 + lane] : -1;
   const uint32_t with = uint32_t(__ballot(has_adapter(id, a.L)));
   if (c >= a.N) return;
+  T* const y = static_cast<T*>(a.out) + int64_t(row0) * a.out_ld + c;
+  const float* const base = HERE ? nullptr : a.base + int64_t(row0) * a.N + c;
+  if constexpr (!HERE)
+    for (int t = 0; t < min(kAnyRows, a.rows - row0); ++t)
+      if (!(with >> t & 1)) y[t * a.out_ld] = rounded<T>(base[int64_t(t) * a.N]);
   for (uint32_t todo = with; todo;) {
     const int which = __builtin_amdgcn_readlane(id, __ffs(todo) - 1);
     uint32_t mine = 0;
@@ -516,10 +553,9 @@ __global__ void __launch_bounds__(kThreads) lora_add_any_kernel(const LoraArgs a
         for (int i = 0; i < 4; ++i) acc[t] += l[i] * v[i];
       }
     }
-    T* const y = static_cast<T*>(a.out) + int64_t(row0) * a.out_ld + c;
 #pragma unroll
     for (int t = 0; t < kAnyRows; ++t)
-      if (mine >> t & 1) y[t * a.out_ld] = rounded<T>(widen(y[t * a.out_ld]) + acc[t]);
+      if (mine >> t & 1) y[t * a.out_ld] = rounded<T>((HERE ? widen(y[t * a.out_ld]) : base[int64_t(t) * a.N]) + acc[t]);
   }
 }
 
@@ -884,32 +920,32 @@ int launch_low(LoraArgs& a, hipStream_t stream) {
 
 int64_t pitch_of(int64_t R) { return round_up(R, 16); }
 
-template <typename T>
+template <typename T, typename P>
 int launch_add(LoraArgs a, hipStream_t stream) {
   a.pitch = int(pitch_of(a.R));
   a.keep = a.rows > kSingleRows;
-  const int rc = launch_low<T>(a, stream);
+  const int rc = a.L ? launch_low<T>(a, stream) : GMM_OK;
   if (rc != GMM_OK) return rc;
   if (!a.keep) return launch_finish<T>(a, stream);
   const unsigned blocks = unsigned((int64_t(a.rows) * a.pitch + kThreads - 1) / kThreads);
-  if (a.low_parts > 1) hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
+  if (a.L && a.low_parts > 1) hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
   if (a.N) {
     const int lay = layout_of_b(a.b, a.R, a.N);
     const dim3 any((a.rows + kAnyRows - 1) / kAnyRows, (a.N + kThreads - 1) / kThreads);
     // strips to a wave: as many as leave every place for one a wave (rank 64: for three groups 54 us, for the two that there is room for 50)
     const int tiles = (a.N + 127) / 128, row_groups = (a.rows + 16 * kWaves - 1) / (16 * kWaves);
-    a.strips = clamp(int64_t(row_groups) * tiles / (add_groups(a.R <= 32 ? 1 : 2) * gmm_num_cus()), 1, tiles);
+    a.strips = clamp(int64_t(row_groups) * tiles / (add_groups(a.R <= 32 ? 1 : 2, sizeof(P) == 2) * gmm_num_cus()), 1, tiles);
     const dim3 grid(row_groups, (tiles + a.strips - 1) / a.strips);
     const auto launch = [&](auto lay, auto nk) {
       constexpr int B = decltype(lay)::value, NK = decltype(nk)::value;
-      if (aligned16(a.out) && a.out_ld % 8 == 0) hipLaunchKernelGGL((lora_add_kernel<T, B, NK, true>), grid, dim3(kThreads), 0, stream, a);
-      else hipLaunchKernelGGL((lora_add_kernel<T, B, NK, false>), grid, dim3(kThreads), 0, stream, a);
+      if (aligned16(a.out) && a.out_ld % 8 == 0) hipLaunchKernelGGL((lora_add_kernel<T, P, B, NK, true>), grid, dim3(kThreads), 0, stream, a);
+      else hipLaunchKernelGGL((lora_add_kernel<T, P, B, NK, false>), grid, dim3(kThreads), 0, stream, a);
     };
     const auto rank = [&](auto lay) {
       if (a.R <= 32) launch(lay, std::integral_constant<int, 1>{});
       else launch(lay, std::integral_constant<int, 2>{});
     };
-    if (lay == GMM_W_ANY) hipLaunchKernelGGL((lora_add_any_kernel<T>), any, dim3(kThreads), 0, stream, a);
+    if (lay == GMM_W_ANY) hipLaunchKernelGGL((lora_add_any_kernel<T, P>), any, dim3(kThreads), 0, stream, a);
     else if (lay == GMM_W_ROWS) rank(std::integral_constant<int, GMM_W_ROWS>{});
     else rank(std::integral_constant<int, GMM_W_COLS>{});
   }
@@ -985,6 +1021,29 @@ int launch_grad(GradArgs& g, int64_t rows, hipStream_t stream) {
 // Bytes of the parts of x @ A.
 static int64_t low_bytes(int64_t rows, int64_t K, int64_t R) { return round_up(int64_t(plan_low(rows, K, R).parts) * rows * R * 4, 256); }
 
+// gmm_lora_sum, and with `base` null gmm_lora_add.
+static int lora_add(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, const float* base, void* out,
+                    float* low, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride, int64_t a_stride_l,
+                    int64_t a_stride_k, int64_t a_stride_r, int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride,
+                    int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int bad = check_sizes(rows, K, N, R, L, dtype);
+  if (bad) return bad;
+  if (!out) N = 0;
+  if (rows == 0 || (N == 0 && (!low || L == 0))) return GMM_OK;
+  LoraArgs g{};
+  if (!adapter || (L && ((N && !b) || (K && (!x || !a)))) || !x_fits(x_stride, rows, K) || !x_fits(out_stride, rows, N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < low_bytes(rows, K, R) + 2 * rows * pitch_of(R) * 2) return GMM_ERR_WORKSPACE;
+  g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low; g.low = static_cast<float*>(workspace);
+  g.planes = N ? static_cast<char*>(workspace) + low_bytes(rows, K, R) : nullptr;
+  g.base = const_cast<float*>(base); g.base_parts = base ? 1 : 0;
+  g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
+  g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (base) return dtype == GMM_DT_BF16 ? launch_add<Bf16, float>(g, s) : launch_add<F16, float>(g, s);
+  return dtype == GMM_DT_BF16 ? launch_add<Bf16, Bf16>(g, s) : launch_add<F16, F16>(g, s);
+}
+
 extern "C" {
 
 int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R) {
@@ -1020,20 +1079,20 @@ int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* ada
                  int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride, int64_t a_stride_l, int64_t a_stride_k,
                  int64_t a_stride_r, int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride, int32_t dtype,
                  void* workspace, int64_t workspace_bytes, void* stream) {
+  if (L == 0) return check_sizes(rows, K, N, R, L, dtype);
+  return lora_add(x, a, b, adapter, scale, nullptr, out, low, rows, K, N, R, L, x_stride, a_stride_l, a_stride_k, a_stride_r, b_stride_l,
+                  b_stride_r, b_stride_n, out_stride, dtype, workspace, workspace_bytes, stream);
+}
+
+int gmm_lora_sum(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, const float* base, void* out,
+                 float* low, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride, int64_t a_stride_l,
+                 int64_t a_stride_k, int64_t a_stride_r, int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride,
+                 int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   const int bad = check_sizes(rows, K, N, R, L, dtype);
   if (bad) return bad;
-  if (!out) N = 0;
-  if (rows == 0 || L == 0 || (N == 0 && !low)) return GMM_OK;
-  LoraArgs g{};
-  if (!adapter || (out && !b) || (K && (!x || !a)) || !x_fits(x_stride, rows, K) || !x_fits(out_stride, rows, N)) return GMM_ERR_BAD_ARGUMENT;
-  if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
-  if (!workspace || !aligned16(workspace) || workspace_bytes < low_bytes(rows, K, R) + 2 * rows * pitch_of(R) * 2) return GMM_ERR_WORKSPACE;
-  g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low; g.low = static_cast<float*>(workspace);
-  g.planes = N ? static_cast<char*>(workspace) + low_bytes(rows, K, R) : nullptr;
-  g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
-  g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GMM_DT_BF16 ? launch_add<Bf16>(g, s) : launch_add<F16>(g, s);
+  if (rows && N && (!base || !out)) return GMM_ERR_BAD_ARGUMENT;
+  return lora_add(x, a, b, adapter, scale, base, out, low, rows, K, N, R, L, x_stride, a_stride_l, a_stride_k, a_stride_r, b_stride_l,
+                  b_stride_r, b_stride_n, out_stride, dtype, workspace, workspace_bytes, stream);
 }
 
 int64_t gmm_lora_grad_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L) {

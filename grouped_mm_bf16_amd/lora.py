@@ -4,7 +4,7 @@
 
 Which token has which adapter is device data that the host never sees, tokens come in any order, and a number outside the adapters means
 none.  Up to ``FEW_TOKENS`` tokens (a decoding step) run in two kernels that read W and the adapters once, past the tokens; more run as W's
-grouped product of one group and two kernels for the adapters.  Registered as torch custom ops (``grouped_mm_bf16_amd::lora``,
+grouped product of one group, in float32, and two kernels for the adapters, the last of which rounds the sum.  Registered as torch custom ops (``grouped_mm_bf16_amd::lora``,
 ``lora_grad``), which calls dispatch to while a model around them is being traced or compiled.  The reference has no counterpart.
 """
 from __future__ import annotations
@@ -73,6 +73,14 @@ def _workspace_bytes(device: int, T: int, K: int, N: int, R: int) -> int:
     return _lib.load().gmm_lora_workspace_bytes(T, K, N, R)
 
 
+def _rows_at_once(T: int, N: int) -> int:
+    """Rows whose product with W is held in float32 at a time: 128 MiB of it, which half of the card's last cache holds, at least 2048, parts
+    of even length."""
+    most = max(2048, (1 << 25) // max(N, 1))
+    parts = -(-T // most)
+    return T if parts <= 1 else -(-T // (parts * 256)) * 256
+
+
 @functools.lru_cache(maxsize=4096)
 def _grad_workspace_bytes(device: int, T: int, K: int, N: int, R: int, L: int) -> int:
     return _lib.load().gmm_lora_grad_workspace_bytes(T, K, N, R, L)
@@ -88,19 +96,30 @@ def _forward_now(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lo
     lib = _lib.load()
     with _guard(x):
         stream, code = kernels.current_stream(dev), _dtype_code(x.dtype)
-        nbytes = _workspace_bytes(dev.index, T, K, N, R)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        adapters = lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr(), _ptr(scale), out.data_ptr(), _ptr(low)
-        strides = (*lora_a.stride(), *lora_b.stride(), N, code, ws.data_ptr(), nbytes, stream)
         rc = _lib.ERR_UNSUPPORTED
         if T <= FEW_TOKENS:
-            rc = lib.gmm_lora_linear(x.data_ptr(), weight.data_ptr(), *adapters, T, K, N, R, L, x.stride(0), *weight.stride(), *strides)
+            nbytes = _workspace_bytes(dev.index, T, K, N, R)
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            rc = lib.gmm_lora_linear(x.data_ptr(), weight.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr(), _ptr(scale),
+                                     out.data_ptr(), _ptr(low), T, K, N, R, L, x.stride(0), *weight.stride(), *lora_a.stride(),
+                                     *lora_b.stride(), N, code, ws.data_ptr(), nbytes, stream)
         if rc == _lib.ERR_UNSUPPORTED:
-            if K == 0:
-                out.zero_()
-            elif out.numel():
-                kernels._launch_now(kernels.V_3D3D, x.unsqueeze(0), weight.unsqueeze(0), None, out.unsqueeze(0))
-            rc = lib.gmm_lora_add(x.data_ptr(), *adapters, T, K, N, R, L, x.stride(0), *strides)
+            most = _rows_at_once(T, N)
+            nbytes = max(_workspace_bytes(dev.index, rows, K, N, R) for rows in (most, (T - 1) % most + 1))     # the last part's may be more
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            base = torch.empty(most, N, device=dev, dtype=torch.float32)
+            for first in range(0, T, most):
+                rows = min(most, T - first)
+                part, product, here = (x, base, out) if rows == T else (x[first:first + rows], base[:rows], out[first:first + rows])
+                if K == 0:
+                    product.zero_()
+                elif N:
+                    kernels._launch_now(kernels.V_3D3D, part.unsqueeze(0), weight.unsqueeze(0), None, product.unsqueeze(0))
+                rc = lib.gmm_lora_sum(part.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr() + 4 * first, _ptr(scale),
+                                      product.data_ptr(), here.data_ptr(), low.data_ptr() + 4 * R * first if save else None, rows, K, N, R, L,
+                                      part.stride(0), *lora_a.stride(), *lora_b.stride(), N, code, ws.data_ptr(), nbytes, stream)
+                if rc:
+                    break
     _lib.check(rc, "lora_linear")
     return out, low
 
@@ -199,7 +218,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     x [T, K]; weight [K, N], row- or column-major; lora_a [L, K, R], lora_b [L, R, N], any strides (views of linear layers' weights as they
     are: ``.transpose(-2, -1)``), rank R up to 256, adapters of lower rank padded with zeros; bf16 or fp16.  adapter int32 [T]: a number outside
     [0, L), such as -1, stands for none.  scale float32 [L] (None: ones) has no gradient; x, weight, lora_a and lora_b have.
-    The rank-sized products stay in float32; the result is rounded once up to ``FEW_TOKENS`` tokens, above that weight's product as well.
+    The rank-sized products and weight's product stay in float32; the result is rounded once.
     """
     _check(x, weight, lora_a, lora_b, adapter, scale)
     if (x.requires_grad or weight.requires_grad or lora_a.requires_grad or lora_b.requires_grad) and torch.is_grad_enabled():

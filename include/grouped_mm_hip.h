@@ -265,7 +265,9 @@ int gmm_moe_few(const void* x, const void* logits, const void* w_up, const void*
  * gmm_lora_grad needs it).  x @ a stays in fp32.  `workspace`: device memory of gmm_lora_workspace_bytes(...) bytes (-1: sizes out of
  * range), 16-byte aligned, contents of no matter.
  *   gmm_lora_linear   all of it, for up to 64 rows (GMM_ERR_UNSUPPORTED: more, or w of 2 GiB and more); rounded once.
- *   gmm_lora_add      for any number: out += scale * (x @ a) @ b, to the product x @ w in `out`.  out NULL: `low` alone. */
+ *   gmm_lora_sum      for any number: out = base + scale * (x @ a) @ b, for the product x @ w in `base`, float [rows, N] contiguous; rounded
+ *                     once.
+ *   gmm_lora_add      for any number: out += scale * (x @ a) @ b, to a product x @ w that lies in `out`, rounded.  out NULL: `low` alone. */
 int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R);
 int gmm_lora_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* adapter, const float* scale,
                     void* out, float* low, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride,
@@ -278,8 +280,14 @@ int gmm_lora_add(const void* x, const void* a, const void* b, const int32_t* ada
                  int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride, int32_t dtype,
                  void* workspace, int64_t workspace_bytes, void* stream);
 
+int gmm_lora_sum(const void* x, const void* a, const void* b, const int32_t* adapter, const float* scale, const float* base, void* out,
+                 float* low, int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, int64_t x_stride,
+                 int64_t a_stride_l, int64_t a_stride_k, int64_t a_stride_r,
+                 int64_t b_stride_l, int64_t b_stride_r, int64_t b_stride_n, int64_t out_stride, int32_t dtype,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
 /* The adapters' gradients, for dy [rows, N], low (above) and u float [rows, R], u[t] = dy[t] @ b[i]^T (what gmm_lora_add gives as `low`
- * for dy and b, a with their last two strides swapped; dx is its `out`, added to dy @ w^T):
+ * for dy and b, a with their last two strides swapped; dx is the `out` of gmm_lora_sum, for dy @ w^T):
  *   da[i] = scale[i] * sum over the rows t of adapter i of x[t]^T u[t]  [L, K, R],   db[i] = scale[i] * sum of low[t]^T dy[t]  [L, R, N],
  * zeros for an adapter without rows; either may be NULL (and then x and u, or dy and low).  No atomics: the same every time. */
 int64_t gmm_lora_grad_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L);
