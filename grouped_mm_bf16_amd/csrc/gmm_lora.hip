@@ -9,7 +9,8 @@
 //   Gradients (gmm_lora_grad): dA[i] = scale[i] * sum of x[t]^T u[t], dB[i] = scale[i] * sum of low[t]^T dy[t] over the rows t that have
 //     adapter i: thin products along the rows, bound by reading x and dy: of those 8192 rows 30 us (134 MB, 4.5 TB/s), and 20 for the sort before
 //     and the sums behind.
-// The rank-sized values x @ A and dy @ B^T stay in fp32; where they are operands of a 16-bit product they are two values each.
+// The rank-sized values x @ A and dy @ B^T stay in fp32; where they are operands of a 16-bit product they are two values each, in fp16 behind
+// a power of two that brings them into its range.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -51,7 +52,7 @@ struct LoraArgs {
   void* out;
   float* low;              // [low_parts][rows][R]: parts of x @ A
   float* low_out;          // [rows][R]: their sums, null: not wanted
-  void* planes;            // many rows: [2][rows][pitch], null: not wanted
+  float* sums;             // many rows: [rows][pitch], x @ A times scale, zeros past the rank; null: not wanted
   float* base;             // [base_parts][rows][N]: parts of x @ W; without any: it lies in `out`
   int64_t x_ld, out_ld;
   int32_t rows, K, N, R, L;
@@ -67,14 +68,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix(const Matrices& m, int 
   return buffer(static_cast<const T*>(m.at) + which * m.sg, m.bytes);
 }
 
-// Many rows: low of a row as the operand of the second product, times scale: two 16-bit values each, [2][rows][pitch], zeros past the rank;
-// and as it is where that is wanted.
-template <typename T>
+// Many rows: low of a row for the second product, times scale, zeros past the rank; and as it is where that is wanted.
 __device__ __forceinline__ void keep_low(const LoraArgs& a, int row, int r, float v, float scale) {
   if (a.low_out && r < a.R) a.low_out[int64_t(row) * a.R + r] = v;
-  if (!a.planes) return;
-  T* const at = static_cast<T*>(a.planes) + int64_t(row) * a.pitch + r;
-  split(v * scale, at[0], at[int64_t(a.rows) * a.pitch]);
+  if (a.sums) a.sums[int64_t(row) * a.pitch + r] = v * scale;
 }
 
 // low[part][t] = x[t] @ A[adapter[t]] over a part of K, for a strip of up to 16 rows.  Of rows with different adapters one adapter comes
@@ -170,7 +167,7 @@ __device__ __forceinline__ void low_product(const LoraArgs& a, int item, SkinnyS
       if (a.low_parts > 1 || !a.keep) {
         if (col < a.R) out[r * a.R + col] = h[v];
       } else if (col < a.pitch) {
-        keep_low<T>(a, row0 + r, col, col < a.R ? h[v] : 0.0f, a.scale ? a.scale[a.adapter[row0 + r]] : 1.0f);
+        keep_low(a, row0 + r, col, col < a.R ? h[v] : 0.0f, a.scale ? a.scale[a.adapter[row0 + r]] : 1.0f);
       }
     }
   }
@@ -334,14 +331,29 @@ __global__ void __launch_bounds__(64) lora_finish_kernel(const LoraArgs a) {
 }
 
 // The parts of x @ A of many rows summed.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) lora_planes_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(kThreads) lora_low_sum_kernel(const LoraArgs a) {
   const int64_t u = int64_t(blockIdx.x) * kThreads + threadIdx.x;
   const int row = int(u / a.pitch), r = int(u % a.pitch);
   if (row >= a.rows) return;
   const int id = a.adapter[row];
-  if (has_adapter(id, a.L)) keep_low<T>(a, row, r, r < a.R ? low_sum(a, row, r) : 0.0f, a.scale ? a.scale[id] : 1.0f);
+  if (has_adapter(id, a.L)) keep_low(a, row, r, r < a.R ? low_sum(a, row, r) : 0.0f, a.scale ? a.scale[id] : 1.0f);
 }
+
+// The power of two that brings the largest of some values between 2^14 and 2^15 (as near as fp32 has one).  Two fp16 values then hold each
+// of them to 2^-22 of it, or 2^-39 of the largest; without it, what is smaller than 2^-3 would lose bits (of 1e-6 all but five) and what
+// is past 65504 would be infinite.  Values that are no finite numbers do not count.
+struct Exponent {
+  uint32_t most = 0;      // bits of the largest absolute value
+
+  __device__ __forceinline__ void take(float v) {
+    const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
+    most = max(most, bits < 0x7f800000u ? bits : 0u);
+  }
+  __device__ __forceinline__ void join(int distance) { most = max(most, uint32_t(__shfl_xor(int(most), distance))); }
+  __device__ __forceinline__ uint32_t field() const { return max(most >> 23, 15u); }      // at most 254
+  __device__ __forceinline__ float down() const { return __uint_as_float((268 - field()) << 23); }
+  __device__ __forceinline__ float up() const { return __uint_as_float((field() - 14) << 23); }
+};
 
 // Eight values of x @ W on their way: two to a register where they lie in y, fp32 elsewhere.
 template <typename T> struct OnTheWay {
@@ -368,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK, sizeof(P) == 2)) lora
   using S = Skinny<T, GMM_W_ROWS, 8, 1, 2, GMM_A_STAGED, 1>;
   constexpr int FR = S::FR, OUT = S::COLUMNS, POLICY = ALIGNED ? kStream : 0;
   constexpr bool HERE = sizeof(P) == 2;      // x @ W lies in y
+  constexpr bool FP16 = std::is_same_v<T, F16>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int first = (blockIdx.x * kWaves + wave) * 16;
   const int id = first + j < a.rows ? a.adapter[first + j] : -1;
@@ -375,8 +388,7 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK, sizeof(P) == 2)) lora
   const int there = min(16, a.rows - first);
   if (HERE ? !with : there <= 0) return;
   const uint32_t none = HERE ? 0 : ~with & ((1u << there) - 1);      // rows that only have to be rounded
-  const T* const high = static_cast<const T*>(a.planes) + int64_t(min(first + j, a.rows - 1)) * a.pitch + 8 * g;
-  const T* const low = high + int64_t(a.rows) * a.pitch;
+  const float* const low = a.sums + int64_t(min(first + j, a.rows - 1)) * a.pitch + 8 * g;
   const int tile0 = blockIdx.y * a.strips, tiles = min(a.strips, (a.N + OUT - 1) / OUT - tile0);
   // y from row `first` on; what is not to be read or written lies nowhere, so that no branch stands around an access
   const __amdgpu_buffer_rsrc_t y = buffer(static_cast<T*>(a.out) + first * a.out_ld, uint32_t(((there - 1) * a.out_ld + a.N) * 2));
@@ -440,21 +452,23 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK, sizeof(P) == 2)) lora
   // strips, and in a strip the adapters of the rows, one after the other: one sequence
   u32x4 h[NK], l[NK], w[NK][8];
   OnTheWay<P> next[4];
+  Exponent exponent;
   const auto load_low = [&](int k) {
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
       const int at = k + 32 * n;      // of a lane's eight values none are there, or all
       const bool in = at + 8 * g < a.pitch;
-      h[n] = *reinterpret_cast<const u32x4*>(high + (in ? at : -8 * g));
-      l[n] = *reinterpret_cast<const u32x4*>(low + (in ? at : -8 * g));
+      const Pack<float, 8> v = *reinterpret_cast<const Pack<float, 8>*>(low + (in ? at : -8 * g));
+      T high[8], rest[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) split(in ? (FP16 ? v.get(i) * exponent.down() : v.get(i)) : 0.0f, high[i], rest[i]);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        h[n][q] = in ? h[n][q] : 0u;
-        l[n][q] = in ? l[n][q] : 0u;
+        h[n][q] = uint32_t(high[2 * q].bits) | uint32_t(high[2 * q + 1].bits) << 16;
+        l[n][q] = uint32_t(rest[2 * q].bits) | uint32_t(rest[2 * q + 1].bits) << 16;
       }
     }
   };
-  load_low(0);
   Adapters ahead{with, 0, 0};
   int tile = 0;
   const auto go_on = [&] {      // rows without an adapter come with a strip's first adapter, or alone
@@ -468,6 +482,17 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK, sizeof(P) == 2)) lora
   for (int n = 0; n < NK; ++n) load_b(w[n], 0, 32 * n);
   load_y(next, 0, ahead.mine);
   __builtin_amdgcn_sched_barrier(0);
+  float up[4];      // of the lane's rows of the result
+  if constexpr (FP16) {
+    for (int k = 0; k + 8 * g < a.pitch; k += 32)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) exponent.take(low[k + i]);
+    exponent.join(16);
+    exponent.join(32);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) up[v] = __shfl(exponent.up(), 4 * g + v);
+  }
+  load_low(0);
 #pragma unroll 1
   while (tile < tiles) {
     const uint32_t mine = ahead.mine;
@@ -501,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, add_groups(NK, sizeof(P) == 2)) lora
     for (int v = 0; v < 4; ++v) {
       float sum[FR];
 #pragma unroll
-      for (int i = 0; i < FR; ++i) sum[i] = next[v].get(i) + (HERE || with >> (4 * g + v) & 1 ? acc[i][v] : 0.0f);
+      for (int i = 0; i < FR; ++i) sum[i] = next[v].get(i) + (HERE || with >> (4 * g + v) & 1 ? (FP16 ? acc[i][v] * up[v] : acc[i][v]) : 0.0f);
       now[v] = Pack<T, 8>::of(sum).w;
     }
     load_y(next, then, tile < tiles ? ahead.mine : 0);
@@ -520,9 +545,7 @@ __global__ void __launch_bounds__(kThreads) lora_add_any_kernel(const LoraArgs a
   const int row0 = blockIdx.x * kAnyRows, c = blockIdx.y * kThreads + threadIdx.x, lane = threadIdx.x & 63;
   const int span = int(a.R + 3) / 4 * 4;
   for (int u = threadIdx.x; u < kAnyRows * span; u += kThreads) {
-    const int64_t at = int64_t(min(row0 + u / span, a.rows - 1)) * a.pitch + u % span;
-    const T* const planes = static_cast<const T*>(a.planes);
-    reinterpret_cast<float*>(low[u / span])[u % span] = widen(planes[at]) + widen(planes[int64_t(a.rows) * a.pitch + at]);
+    reinterpret_cast<float*>(low[u / span])[u % span] = a.sums[int64_t(min(row0 + u / span, a.rows - 1)) * a.pitch + u % span];
   }
   __syncthreads();
   const int id = lane < kAnyRows && row0 + lane < a.rows ? a.adapter[row0 + lane] : -1;
@@ -928,7 +951,7 @@ int launch_add(LoraArgs a, hipStream_t stream) {
   if (rc != GMM_OK) return rc;
   if (!a.keep) return launch_finish<T>(a, stream);
   const unsigned blocks = unsigned((int64_t(a.rows) * a.pitch + kThreads - 1) / kThreads);
-  if (a.L && a.low_parts > 1) hipLaunchKernelGGL((lora_planes_kernel<T>), dim3(blocks), dim3(kThreads), 0, stream, a);
+  if (a.L && a.low_parts > 1) hipLaunchKernelGGL(lora_low_sum_kernel, dim3(blocks), dim3(kThreads), 0, stream, a);
   if (a.N) {
     const int lay = layout_of_b(a.b, a.R, a.N);
     const dim3 any((a.rows + kAnyRows - 1) / kAnyRows, (a.N + kThreads - 1) / kThreads);
@@ -1033,9 +1056,9 @@ static int lora_add(const void* x, const void* a, const void* b, const int32_t* 
   LoraArgs g{};
   if (!adapter || (L && ((N && !b) || (K && (!x || !a)))) || !x_fits(x_stride, rows, K) || !x_fits(out_stride, rows, N)) return GMM_ERR_BAD_ARGUMENT;
   if (!set(g.a, a, a_stride_l, a_stride_k, a_stride_r, K, R) || !set(g.b, b, b_stride_l, b_stride_r, b_stride_n, R, N)) return GMM_ERR_BAD_ARGUMENT;
-  if (!workspace || !aligned16(workspace) || workspace_bytes < low_bytes(rows, K, R) + 2 * rows * pitch_of(R) * 2) return GMM_ERR_WORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < low_bytes(rows, K, R) + rows * pitch_of(R) * 4) return GMM_ERR_WORKSPACE;
   g.x = x; g.adapter = adapter; g.scale = scale; g.out = out; g.low_out = low; g.low = static_cast<float*>(workspace);
-  g.planes = N ? static_cast<char*>(workspace) + low_bytes(rows, K, R) : nullptr;
+  g.sums = N ? reinterpret_cast<float*>(static_cast<char*>(workspace) + low_bytes(rows, K, R)) : nullptr;
   g.base = const_cast<float*>(base); g.base_parts = base ? 1 : 0;
   g.x_ld = rows > 1 ? x_stride : round_up(K, 8); g.out_ld = rows > 1 ? out_stride : round_up(N, 8);
   g.rows = int(rows); g.K = int(K); g.N = int(N); g.R = int(R); g.L = int(L);
@@ -1048,7 +1071,7 @@ extern "C" {
 
 int64_t gmm_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t R) {
   if (check_sizes(rows, K, N, R, 0, GMM_DT_BF16) != GMM_OK) return -1;
-  int64_t bytes = low_bytes(rows, K, R) + round_up(2 * rows * pitch_of(R) * 2, 256);
+  int64_t bytes = low_bytes(rows, K, R) + round_up(rows * pitch_of(R) * 4, 256);
   if (rows <= kFewRows) bytes += int64_t(plan_base(K, N, 128).parts) * rows * N * 4;     // the layout with the more parts
   return bytes;
 }
