@@ -590,7 +590,8 @@ __device__ __forceinline__ int place(const int32_t* offs, int i) { return ((i ? 
 // One of the two gradients: out[i] = q^T p over adapter i's rows.
 struct GradOf {
   const void* p;            // [rows][C]: x or dy
-  const void* q;            // [2][R][places]: u or low by place, times scale: high and low halves
+  const void* q;            // [2][R][places]: u or low by place, times scale (fp16: and an Exponent's power of two): high and low halves
+  const uint32_t* peak;     // fp16: [peak_parts][L][R]: what an Exponent takes of the adapter's rows
   void* out;                // [L][R][C] with the strides below
   float* partial;           // [slots][R * C] as `out` has it: of adapters whose rows are more than one chunk
   int64_t p_ld, out_sg, out_sr, out_sc;
@@ -603,7 +604,15 @@ struct GradArgs {
   const int32_t* row_at;    // [places] the row at a place
   const int32_t* offs;      // [L + 1] ends of the adapters' rows
   int32_t places, R, L, chunk, groups0;   // groups0: workgroups of of[0]
+  int32_t peak_parts;
 };
+
+// fp16: the power of two that rank r of adapter i's values are brought down by, all rows alike, as the sum over them needs it.
+__device__ __forceinline__ Exponent exponent_of(const uint32_t* peak, int parts, int L, int R, int i, int r) {
+  Exponent e;
+  in_fours(parts, [&](int p, bool) { e.most = max(e.most, peak[(int64_t(p) * L + i) * R + r]); });
+  return e;
+}
 
 // An adapter's n rows are dealt evenly to as many chunks as are needed (one for no rows: its gradient is zero).
 __device__ __forceinline__ int chunks_of(int n, int chunk) { return n > chunk ? (n + chunk - 1) / chunk : 1; }
@@ -649,6 +658,8 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   __shared__ SkinnyShared<S, kWaves> shared;
   __shared__ int32_t row_at[kMaxChunk];
+  __shared__ __align__(16) float up[16 * MF];
+  constexpr bool FP16 = std::is_same_v<T, F16>;
   const bool second = int(blockIdx.x) >= args.groups0;
   const GradOf& a = args.of[second];
   const int item = blockIdx.x - (second ? args.groups0 : 0);
@@ -656,6 +667,9 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   if (!find_chunk(args, item / a.tiles, adapter, first, rows, slot)) return;
   const int tile = item % a.tiles, r0 = blockIdx.y * 16 * MF;
   for (int u = threadIdx.x; u < rows; u += kThreads) row_at[u] = args.row_at[first + u];
+  if constexpr (FP16)
+    if (int(threadIdx.x) < 16 * MF)
+      up[threadIdx.x] = exponent_of(a.peak, args.peak_parts, args.L, args.R, adapter, min(r0 + int(threadIdx.x), args.R - 1)).up();
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c)), R = args.R, end = (rows + 7) / 8 * 8;   // zeros behind the last row
@@ -719,7 +733,8 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
       const int oc = u % OUT, og = u / OUT, col = tile * OUT + oc;
       if (col >= a.C) continue;
       const int at = WHOLE ? S::position(oc, a.C - col) : oc;
-      const f32x4 h = shared.sums.get(S::product_of(at), S::lane_of(at), og);
+      f32x4 h = shared.sums.get(S::product_of(at), S::lane_of(at), og);
+      if constexpr (FP16) h *= *reinterpret_cast<const f32x4*>(up + 16 * m + 4 * og);
       const int r = r0 + 16 * m + 4 * og;
       if (slot >= 0) {
         float* const to = a.partial + int64_t(slot) * R * a.C + (a.r_first ? int64_t(col) * R + r : int64_t(r) * a.C + col);
@@ -764,23 +779,69 @@ __global__ void __launch_bounds__(kThreads) lora_grad_sum_kernel(const GradArgs 
   }
 }
 
+// The largest absolute values of each adapter's rows of q1 and q2 [rows][R] times scale (either may be null), for exponent_of: part `y` of them,
+// q1 or q2 by `z`.
+__global__ void __launch_bounds__(kThreads) lora_peak_kernel(const float* __restrict__ q1, const float* __restrict__ q2,
+                                                             const float* __restrict__ scale, const int32_t* __restrict__ row_token,
+                                                             const int32_t* __restrict__ offs, int R, int L, uint32_t* __restrict__ peak1,
+                                                             uint32_t* __restrict__ peak2) {
+  __shared__ uint32_t most[kThreads];
+  const float* const q = blockIdx.z ? q2 : q1;
+  const int i = blockIdx.x, part = blockIdx.y, parts = gridDim.y;
+  const int begin = i ? offs[i - 1] : 0, n = q ? offs[i] - begin : 0;
+  const int from = begin + int(int64_t(n) * part / parts), to = begin + int(int64_t(n) * (part + 1) / parts);
+  const int columns = 1 << (32 - __clz(R - 1)), lines = kThreads / columns;      // (of one column: 1 << 0)
+  const int r = threadIdx.x % columns;
+  const float by = scale ? scale[i] : 1.0f;
+  Exponent e;
+  if (r < R)
+    for (int k = from + int(threadIdx.x) / columns; k < to; k += 8 * lines)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) e.take(q[int64_t(row_token[min(k + u * lines, to - 1)]) * R + r] * by);      // past the end the last one again
+  most[threadIdx.x] = e.most;
+  __syncthreads();
+  if (int(threadIdx.x) >= R) return;
+  for (int k = 1; k < lines; ++k) e.most = max(e.most, most[threadIdx.x + k * columns]);
+  (blockIdx.z ? peak2 : peak1)[(int64_t(part) * L + i) * R + r] = e.most;
+}
+
 // Sorted operands: q1 and q2 [rows][R] fp32 (either may be null) as [2][R][places] 16-bit halves, times scale; rows by place.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) lora_sorted_kernel(const float* __restrict__ q1, const float* __restrict__ q2,
                                                                const float* __restrict__ scale, const int32_t* __restrict__ adapter,
                                                                const int32_t* __restrict__ row_token, const int32_t* __restrict__ offs,
                                                                int rows, int R, int L, int places, T* __restrict__ s1, T* __restrict__ s2,
-                                                               int32_t* __restrict__ row_at) {
+                                                               int32_t* __restrict__ row_at, const uint32_t* __restrict__ peak1,
+                                                               const uint32_t* __restrict__ peak2, int peak_parts) {
   const int at = blockIdx.x * kThreads + threadIdx.x, r = blockIdx.y;
-  if (at >= rows) return;
-  const int row = row_token[at], id = adapter[row];
-  if (!has_adapter(id, L)) return;
+  const int row = row_token[min(at, rows - 1)], id = adapter[row];
+  float down[2] = {1.0f, 1.0f};
+  if constexpr (std::is_same_v<T, F16>) {
+    // a wave of one adapter's rows looks the parts up together (gradients of 8192 rows of one adapter of rank 64 115 -> 111 us)
+    const int lead = __builtin_amdgcn_readfirstlane(id), lane = threadIdx.x & 63;
+    const bool together = __all(id == lead);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t* const peak = i ? peak2 : peak1;
+      if (!(i ? q2 : q1) || !has_adapter(id, L)) continue;
+      Exponent e;
+      if (together) {
+        e.most = peak[(int64_t(min(lane, peak_parts - 1)) * L + lead) * R + r];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) e.join(o);
+      } else {
+        e = exponent_of(peak, peak_parts, L, R, id, r);
+      }
+      down[i] = e.down();
+    }
+  }
+  if (at >= rows || !has_adapter(id, L)) return;
   const int to = place(offs, id) + at - (id ? offs[id - 1] : 0);
   const float by = scale ? scale[id] : 1.0f;
   if (r == 0) row_at[to] = row;
   const int64_t plane = int64_t(R) * places, slot = int64_t(r) * places + to;
-  if (q1) split(q1[int64_t(row) * R + r] * by, s1[slot], s1[plane + slot]);
-  if (q2) split(q2[int64_t(row) * R + r] * by, s2[slot], s2[plane + slot]);
+  if (q1) split(q1[int64_t(row) * R + r] * by * down[0], s1[slot], s1[plane + slot]);
+  if (q2) split(q2[int64_t(row) * R + r] * by * down[1], s2[slot], s2[plane + slot]);
   // the adapter's last row: the places behind it, up to a multiple of 8, are read with it
   if (at == offs[id] - 1)
     for (int64_t t = slot + 1; t % 8; ++t) {
@@ -977,8 +1038,8 @@ int launch_add(LoraArgs a, hipStream_t stream) {
 
 // Where the operands of gmm_lora_grad lie in its workspace.
 struct GradPlan {
-  int64_t places, offs_at, token_at, rows_at, table_at, row_at, q_at[2], partial_at[2], bytes;
-  int32_t chunk;
+  int64_t places, offs_at, token_at, rows_at, table_at, row_at, q_at[2], partial_at[2], peak_at[2], bytes;
+  int32_t chunk, peak_parts;
 };
 
 bool plan_grad(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, GradPlan& p) {
@@ -999,6 +1060,9 @@ bool plan_grad(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, GradPla
   for (int i = 0; i < 2; ++i) p.q_at[i] = take(2 * R * p.places * 2);
   for (int i = 0; i < 2; ++i)      // adapters of several chunks have fewer than two for each chunk of all rows
     p.partial_at[i] = take(2 * (rows / p.chunk) * R * (i ? N : K) * 4);
+  // as many as leave a thread two trips to memory or so (8192 rows of one adapter, rank 64, in 8 parts: 28 us), while there are few adapters
+  p.peak_parts = clamp(rows * R / 8192, 1, clamp(1024 / (L + 1), 1, 32));
+  for (int i = 0; i < 2; ++i) p.peak_at[i] = take(int64_t(p.peak_parts) * L * R * 4);
   p.bytes = at;
   return 2 * R * p.places * 2 < (int64_t(1) << 31) && R * K < (int64_t(1) << 30) && R * N < (int64_t(1) << 30);
 }
@@ -1142,15 +1206,22 @@ int gmm_lora_grad(const void* x, const void* dy, const float* low, const float* 
   if (rc != GMM_OK) return rc;
   GradArgs g{};
   g.row_at = ints(p.row_at); g.offs = ints(p.offs_at);
-  g.places = int(p.places); g.R = int(R); g.L = int(L); g.chunk = p.chunk;
+  g.places = int(p.places); g.R = int(R); g.L = int(L); g.chunk = p.chunk; g.peak_parts = p.peak_parts;
+  uint32_t* const peak[2] = {reinterpret_cast<uint32_t*>(ws + p.peak_at[0]), reinterpret_cast<uint32_t*>(ws + p.peak_at[1])};
+  for (int i = 0; i < 2; ++i) g.of[i].peak = peak[i];
+  const float* const q1 = da ? u : nullptr;
+  const float* const q2 = db ? low : nullptr;
+  if (dtype == GMM_DT_F16)
+    hipLaunchKernelGGL(lora_peak_kernel, dim3(unsigned(L), unsigned(p.peak_parts), 2), dim3(kThreads), 0, s, q1, q2, scale, ints(p.token_at), ints(p.offs_at),
+                       int(R), int(L), peak[0], peak[1]);
   set_grad(g.of[0], x, x_stride, ws + p.q_at[0], da, reinterpret_cast<float*>(ws + p.partial_at[0]), K, R, da_stride_l, da_stride_r, da_stride_k);
   set_grad(g.of[1], dy, dy_stride, ws + p.q_at[1], db, reinterpret_cast<float*>(ws + p.partial_at[1]), N, R, db_stride_l, db_stride_r, db_stride_n);
   const auto both = [&](auto zero) {
     using T = decltype(zero);
     if (rows)
-      hipLaunchKernelGGL((lora_sorted_kernel<T>), dim3(unsigned((rows + kThreads - 1) / kThreads), unsigned(R)), dim3(kThreads), 0, s, da ? u : nullptr,
-                         db ? low : nullptr, scale, adapter, ints(p.token_at), ints(p.offs_at), int(rows), int(R), int(L), int(p.places),
-                         reinterpret_cast<T*>(ws + p.q_at[0]), reinterpret_cast<T*>(ws + p.q_at[1]), ints(p.row_at));
+      hipLaunchKernelGGL((lora_sorted_kernel<T>), dim3(unsigned((rows + kThreads - 1) / kThreads), unsigned(R)), dim3(kThreads), 0, s, q1, q2, scale,
+                         adapter, ints(p.token_at), ints(p.offs_at), int(rows), int(R), int(L), int(p.places), reinterpret_cast<T*>(ws + p.q_at[0]),
+                         reinterpret_cast<T*>(ws + p.q_at[1]), ints(p.row_at), peak[0], peak[1], p.peak_parts);
     return launch_grad<T>(g, rows, s);
   };
   return dtype == GMM_DT_BF16 ? both(Bf16{}) : both(F16{});

@@ -82,3 +82,68 @@ def test_infinities_stay_in_their_rows_of_half_precision(T):
     got = lora.lora_linear(x, weight, a, b, adapter, scale)
     keep = torch.arange(T, device=DEV) != 3
     assert torch.equal(got[keep], want[keep]) and not torch.isfinite(got[3]).any()
+
+
+# ------------------------------------------------------------------ gradients of the adapters
+def grad_bounds(dy, x, a, b, adapter, scale):
+    """(da, its bound), (db, its bound): one rounding, sums in float32, and of the values that are held as two 16-bit ones a relative error."""
+    dtype = x.dtype
+    dy, x, a, b = oracle.f64(dy), oracle.f64(x), oracle.f64(a), oracle.f64(b)
+    (T, K), N = x.shape, dy.size(1)
+    da, db, da_err, db_err = (torch.zeros_like(t) for t in (a, b, a, b))
+    for i in adapter.cpu().unique().tolist():
+        if not 0 <= i < a.size(0):
+            continue
+        at, s = (adapter.cpu() == i).nonzero()[:, 0], float(scale[i])
+        sums = (len(at) / 16 + 80) * EPS
+        for p, q, m, size, out, err in ((x[at], dy[at] @ b[i].T, dy[at].abs() @ b[i].abs().T, N, da, da_err),
+                                        (dy[at], x[at] @ a[i], x[at].abs() @ a[i].abs(), K, db, db_err)):
+            q_err = s * ((size / 16 + 80) * EPS * m + (TWO16[dtype] + 4 * EPS) * q.abs() + FLOOR * q.abs().max(0).values)
+            value, bound = s * (p.T @ q), p.abs().T @ q_err + sums * s * (p.abs().T @ q.abs())
+            out[i], err[i] = (value, bound) if out is da else (value.T, bound.T)
+    unit = oracle.UNIT[dtype]
+    return [(v, e * (1 + unit) + unit * v.abs() + oracle.TINY[dtype]) for v, e in ((da, da_err), (db, db_err))]
+
+
+def check_adapter_grads(dy, x, a, b, adapter, scale, least):
+    weight = torch.zeros(x.size(1), dy.size(1), dtype=x.dtype, device=DEV)
+    leaves = [t.detach().requires_grad_() for t in (a, b)]
+    got = torch.autograd.grad(lora.lora_linear(x, weight, *leaves, adapter, scale), leaves, dy)
+    for name, g, (want, bound), low in zip(("da", "db"), got, grad_bounds(dy, x, a, b, adapter, scale), least):
+        assert torch.isfinite(want).all() and low < want.abs().max() < 60000
+        oracle.assert_within(g, want, bound, name)
+
+
+@pytest.mark.parametrize("T", [40, 300, 1500])
+@pytest.mark.parametrize("R,lay", [(16, "rows"), (5, "cols"), (72, "cols"), (256, "rows"), (1, "rows")])
+@pytest.mark.parametrize("size", [1e-5, 1e-6])
+def test_gradients_of_small_gradients(T, R, lay, size):
+    """A first step of tuning: dy as it is without loss scaling, B of 0.02.  dB is of the size of dy, so its adapters get a large A."""
+    x, _, a, b, adapter, scale = make(T, 136, 256, R, 3, lay, "rows", HF)
+    dy = (torch.randn(T, 256, generator=torch.Generator().manual_seed(5)) * size).to(HF).to(DEV)
+    check_adapter_grads(dy, x * 64, a * 64, b * 0.02 * R ** 0.5, adapter, scale, (size, size))
+
+
+@pytest.mark.parametrize("T", [40, 300, 1500])
+def test_gradients_of_rank_sized_values_past_65504(T):
+    x, _, a, b, adapter, scale = make(T, 128, 96, 16, 3, dtype=HF)
+    dy = torch.randn(T, 96, generator=torch.Generator().manual_seed(5)).to(HF).to(DEV)
+    large, small = 30000.0, 2.0 ** -12
+    check_adapter_grads(dy * 4, x * small, a, b * large, adapter, scale, (1, 0))       # u = dy B^T
+    check_adapter_grads(dy * small, x * 4, a * large, b, adapter, scale, (0, 1))       # low = x A
+
+
+def test_gradients_of_requests_of_very_different_size():
+    """Each adapter's rows have a power of two of their own: one's large gradients do not take another's bits."""
+    x, _, a, b, adapter, scale = make(900, 64, 96, 8, 5, dtype=HF, pattern="requests")
+    dy = torch.randn(900, 96, generator=torch.Generator().manual_seed(5))
+    dy = (dy * 10.0 ** (adapter.cpu().float() * 2 - 6)[:, None]).to(HF).to(DEV)
+    check_adapter_grads(dy, x, a, b, adapter, scale, (1, 1))
+
+
+def test_gradients_of_no_rows_in_half_precision():
+    x, weight, a, b, adapter, scale = make(0, 64, 32, 8, 3, dtype=HF)
+    leaves = [t.detach().requires_grad_() for t in (a, b)]
+    torch.full((1 << 20,), float("nan"), device=DEV)      # what a workspace may be given next
+    grads = torch.autograd.grad(lora.lora_linear(x, weight, *leaves, adapter, scale).sum(), leaves)
+    assert all(torch.equal(g, torch.zeros_like(g)) for g in grads)
