@@ -14,7 +14,7 @@ from typing import List, Optional, Tuple
 
 import torch
 
-from . import _lib, kernels
+from . import _lib, derivatives, kernels
 from .api import is_row_major
 from .kernels import _dtype_code, _guard, _require_gpu
 
@@ -208,7 +208,7 @@ class _Lora(torch.autograd.Function):
                 dw.zero_()
             elif dw.numel():
                 kernels.grouped_mm_3d3d(x.t().unsqueeze(0), dy.unsqueeze(0), dw.unsqueeze(0))
-        return dx, dw, da if need_a else None, db if need_b else None, None, None
+        return *derivatives.gradients("lora_linear", dx, dw, da if need_a else None, db if need_b else None), None, None
 
 
 def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter: torch.Tensor,

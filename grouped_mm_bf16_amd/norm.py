@@ -10,7 +10,7 @@ from typing import List, Optional, Tuple
 
 import torch
 
-from . import _lib, kernels
+from . import _lib, derivatives, kernels
 from .kernels import _dtype_code, _guard, _require_gpu
 
 MAX_WIDTH = 16384
@@ -137,7 +137,7 @@ class _LayerNorm(torch.autograd.Function):
         dx, dw, db = impl(dy, x, weight, stats, ctx.param_dtype, need[0], need[1], need[2])
         if need[0]:
             dx = dx if len(ctx.shape) == 2 else dx.reshape(ctx.shape)
-        return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
+        return *derivatives.gradients("layer_norm", dx if need[0] else None, dw if need[1] else None, db if need[2] else None), None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

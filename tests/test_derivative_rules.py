@@ -1,0 +1,102 @@
+"""What torch would differentiate that has no derivative here raises (CPU: the kernels are replaced by the formulas, without a graph)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from grouped_mm_bf16_amd import kernels, lora, norm
+
+
+@pytest.fixture
+def formulas(monkeypatch):
+    """The launches, as opaque to torch as they are."""
+    def norm_forward(x, weight, bias, eps, save):
+        with torch.no_grad():
+            mean = x.mean(1)
+            rstd = 1 / ((x - mean[:, None]).square().mean(1) + eps).sqrt()
+            y = (x - mean[:, None]) * rstd[:, None] * (1 if weight is None else weight) + (0 if bias is None else bias)
+            return y, torch.stack([mean, rstd]) if save else None
+
+    def norm_backward(dy, x, weight, stats, param_dtype, need_x, need_weight, need_bias):
+        with torch.no_grad():
+            z = (x - stats[0][:, None]) * stats[1][:, None]
+            g = dy * (1 if weight is None else weight)
+            dx = stats[1][:, None] * (g - g.mean(1, keepdim=True) - z * (g * z).mean(1, keepdim=True))
+            return [dx, (dy * z).sum(0), dy.sum(0)]
+
+    def per_token(x, a, b, adapter, scale):
+        return torch.stack([float(scale[i]) * (x[t] @ a[i]) @ b[i] for t, i in enumerate(adapter.tolist())])
+
+    def lora_forward(x, weight, a, b, adapter, scale, save):
+        with torch.no_grad():
+            low = torch.stack([x[t] @ a[i] for t, i in enumerate(adapter.tolist())])
+            return x @ weight + per_token(x, a, b, adapter, scale), low if save else None
+
+    def lora_grad(x, dy, low, u, adapter, scale, a, b, need_a, need_b):
+        with torch.no_grad():
+            da, db = torch.zeros_like(a), torch.zeros_like(b)
+            for t, i in enumerate(adapter.tolist()):
+                da[i] += float(scale[i]) * torch.outer(x[t], b[i] @ dy[t])
+                db[i] += float(scale[i]) * torch.outer(low[t], dy[t])
+            return [da, db]
+
+    for module, name, to in ((norm, "_require_gpu", lambda *t: None), (lora, "_require_gpu", lambda *t: None),
+                             (norm, "_forward_now", norm_forward), (norm, "_backward_now", norm_backward),
+                             (lora, "_forward_now", lora_forward), (lora, "_grad_now", lora_grad),
+                             (kernels, "grouped_mm_3d3d", lambda p, q, out: out.copy_(p @ q))):
+        monkeypatch.setattr(module, name, to)
+
+
+def norm_call(seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    leaves = [torch.randn(5, 8, generator=gen), torch.randn(8, generator=gen), torch.randn(8, generator=gen)]
+    return norm.layer_norm, leaves, lambda x, w, b: torch.nn.functional.layer_norm(x, (8,), w, b)
+
+
+def lora_call(seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    leaves = [torch.randn(*s, generator=gen).to(torch.float16) for s in ((5, 6), (6, 7), (3, 6, 2), (3, 2, 7))]
+    adapter, scale = torch.tensor([0, 2, 2, 1, 0], dtype=torch.int32), torch.ones(3)
+    return lambda *t: lora.lora_linear(*t, adapter, scale), leaves, None
+
+
+CALLS = pytest.mark.parametrize("call", [norm_call, lora_call])
+
+
+@CALLS
+def test_first_derivatives(formulas, call):
+    """The same with and without create_graph."""
+    f, leaves, plain = call()
+    leaves = [t.requires_grad_() for t in leaves]
+    y = f(*leaves)
+    dy = torch.ones_like(y)
+    grads = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    for i, (p, q) in enumerate(zip(grads, again)):
+        assert torch.equal(p, q.detach()) and not p.requires_grad
+        if plain:
+            want = torch.autograd.grad(plain(*leaves), leaves, dy)
+            assert torch.allclose(p, want[i], atol=1e-5)
+
+
+@CALLS
+@pytest.mark.parametrize("through", ["sum", "cubes"])
+def test_second_derivatives_raise(formulas, call, through):
+    """A gradient penalty, for an upstream gradient that requires a gradient itself (cubes) and for a constant one."""
+    for which in range(3):
+        f, leaves, _ = call()
+        leaves[which].requires_grad_()
+        leaf = leaves[which]
+        y = f(*leaves)
+        value = y.float().sum() if through == "sum" else (y.float() ** 3).sum()
+        grad, = torch.autograd.grad(value, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (value + grad.float().square().sum()).backward()
+
+
+def test_second_derivatives_raise_for_copied_operands(formulas):
+    """The saved rows are a copy, which has no graph of its own."""
+    x = torch.randn(4, 6, 8).transpose(0, 1).requires_grad_()
+    y = norm.layer_norm(x)
+    grad, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        grad.square().sum().backward()
