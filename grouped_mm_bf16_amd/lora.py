@@ -221,7 +221,8 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     The rank-sized products and weight's product stay in float32; the result is rounded once.
     """
     _check(x, weight, lora_a, lora_b, adapter, scale)
-    if (x.requires_grad or weight.requires_grad or lora_a.requires_grad or lora_b.requires_grad) and torch.is_grad_enabled():
+    if ((x.requires_grad or weight.requires_grad or lora_a.requires_grad or lora_b.requires_grad) and torch.is_grad_enabled()
+            or derivatives.forward_mode()):      # with a tangent it raises: there is no forward-mode derivative
         return _Lora.apply(x, weight, lora_a, lora_b, adapter, scale)
     impl = _forward_op if torch.compiler.is_compiling() else _forward_now
     return impl(_rows(x), weight, lora_a, lora_b, adapter, scale, False)[0]

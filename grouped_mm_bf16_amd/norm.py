@@ -147,7 +147,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x [..., W], bf16, fp16 or fp32, W up to 16384; weight and bias [W] in x's type or in float32 (None: ones, zeros).  Sums in fp32, one
     rounding.  A matrix whose rows lie apart is read as it is; other tensors are copied unless they are contiguous.
     """
-    if (x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
+    if ((x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled()
+            or derivatives.forward_mode()):      # with a tangent it raises: there is no forward-mode derivative
         return _LayerNorm.apply(x, weight, bias, eps)
     _check(x, weight, bias)
     impl = _forward_op if torch.compiler.is_compiling() else _forward_now

@@ -100,3 +100,24 @@ def test_second_derivatives_raise_for_copied_operands(formulas):
     grad, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
         grad.square().sum().backward()
+
+
+@CALLS
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_raises(formulas, call, which):
+    f, leaves, _ = call()
+    plain = f(*leaves)
+    with forward_ad.dual_level():
+        assert torch.equal(f(*leaves), plain)       # no tangent: as ever
+        leaves[which] = forward_ad.make_dual(leaves[which], torch.ones_like(leaves[which]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            f(*leaves)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
+            f(*leaves)
+
+
+@CALLS
+def test_function_transforms_raise(formulas, call):
+    f, leaves, _ = call()
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(f, tuple(leaves), tuple(torch.ones_like(t) for t in leaves))
