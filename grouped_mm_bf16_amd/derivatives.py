@@ -36,8 +36,6 @@ def forward_mode() -> bool:
     return forward_ad._current_level >= 0
 
 
-def wanted(*tensors) -> bool:
-    """Whether torch would record a derivative, backward or forward, of what is done with these tensors."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return forward_mode() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+def tangent(*tensors) -> bool:
+    """Whether one of the tensors has a tangent."""
+    return forward_mode() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)

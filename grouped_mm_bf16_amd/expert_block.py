@@ -33,8 +33,9 @@ class ExpertBlock(NamedTuple):
         """The block's first half, with gradients."""
         return x + lora.lora_linear(norm.layer_norm(x, *self.norm_in), self.projection, self.lora_a, self.lora_b, adapter, self.scale)
 
+    @torch.no_grad()
     def __call__(self, x: torch.Tensor, adapter: torch.Tensor) -> torch.Tensor:
-        """x [T, H], adapter int32 [T] (-1: none) -> [T, H]; inference."""
+        """x [T, H], adapter int32 [T] (-1: none) -> [T, H]; inference: the experts have no gradient, so the result has none."""
         h = self.project(x, adapter)
         n = norm.layer_norm(h, *self.norm_experts)
         logits = grouped_mm(n.unsqueeze(0), self.router.unsqueeze(0)).squeeze(0)

@@ -19,7 +19,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib, kernels
+from . import _lib, derivatives, kernels
 from .kernels import _dtype_code, _guard, _require_gpu, grouped_mm_2d3d
 
 ACTIVATIONS = {"silu": 0, "swiglu": 1}
@@ -428,7 +428,8 @@ def moe_forward_few(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Te
     tokens' rows in kernels made for that, without tiles for rows that are not there.
 
     Arguments as there; bf16 or fp16, any sizes and weight strides.  Activations and the experts' results stay in 32 bits: the result is
-    rounded once (``moe_forward`` rounds three times, so the two differ by roundings).
+    rounded once (``moe_forward`` rounds three times, so the two differ by roundings).  Forward only: it refuses operands that require a
+    gradient unless gradients are off.
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
         raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")
@@ -459,6 +460,9 @@ def moe_forward_few(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Te
         raise RuntimeError(f"top_k must be in [1, min(experts, 32)], got {top_k} for {E} experts")
     if E > 1023:
         raise RuntimeError("Can't process more than 1024 groups")
+    if ((x.requires_grad or router_logits.requires_grad or w_up.requires_grad or w_down.requires_grad) and torch.is_grad_enabled()
+            or derivatives.forward_mode() and derivatives.tangent(x, router_logits, w_up, w_down)):
+        raise RuntimeError("moe_forward_few is forward only: call it under torch.no_grad(), or with detached operands")
     if not (x.is_contiguous() or T == 0 or H == 0) and (x.stride(1) != 1 and H > 1 or T > 1 and not H <= x.stride(0) <= 1 << 23):
         x = x.contiguous()
     if not (router_logits.is_contiguous() or T == 0) and (router_logits.stride(1) != 1 and E > 1 or router_logits.stride(0) < E):

@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from grouped_mm_bf16_amd import kernels, lora, norm
+from grouped_mm_bf16_amd import expert_block, kernels, lora, moe, norm
 
 
 @pytest.fixture
@@ -121,3 +121,56 @@ def test_function_transforms_raise(formulas, call):
     f, leaves, _ = call()
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.func.jvp(f, tuple(leaves), tuple(torch.ones_like(t) for t in leaves))
+
+
+# ------------------------------------------------------------------ forward only
+def layer_args():
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    return [bf(4, 64), torch.zeros(4, 8), bf(8, 64, 64), bf(8, 32, 64)]
+
+
+@pytest.fixture
+def few_launched(monkeypatch):
+    launched = []
+    monkeypatch.setattr(moe, "_require_gpu", lambda *t: None)
+    monkeypatch.setattr(moe, "_few_now", lambda x, *rest: launched.append(1) or torch.zeros_like(x))
+    return launched
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_few_tokens_refuse_a_gradient(few_launched, which):
+    args = layer_args()
+    args[which].requires_grad_()
+    with pytest.raises(RuntimeError, match="forward only"):
+        moe.moe_forward_few(*args, 2)
+    assert not few_launched
+    with torch.no_grad():
+        assert not moe.moe_forward_few(*args, 2).requires_grad
+    assert not moe.moe_forward_few(*(t.detach() for t in args), 2).requires_grad
+    assert len(few_launched) == 2
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_few_tokens_refuse_a_tangent(few_launched, which):
+    args = layer_args()
+    with forward_ad.dual_level():
+        moe.moe_forward_few(*args, 2)
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward only"):
+            moe.moe_forward_few(*args, 2)
+    assert len(few_launched) == 1
+
+
+@pytest.mark.parametrize("tokens", [4, 80])
+def test_the_example_block_is_inference(monkeypatch, tokens):
+    """Its result would otherwise have the gradient of everything but the experts."""
+    monkeypatch.setattr(expert_block.norm, "layer_norm", lambda x, w, b: x * w + b)
+    monkeypatch.setattr(expert_block.lora, "lora_linear", lambda x, w, a, b, adapter, scale: x @ w)
+    monkeypatch.setattr(expert_block, "grouped_mm", lambda a, b: a @ b)
+    for name in ("moe_forward", "moe_forward_few"):
+        monkeypatch.setattr(expert_block.moe, name, lambda n, *rest: n.detach().clone())
+    block = expert_block.random_block(16, 4, 2, 64, 3, 4, dtype=torch.float32, device="cpu")
+    block.lora_a.requires_grad_()
+    x, adapter = torch.randn(tokens, 16, requires_grad=True), torch.zeros(tokens, dtype=torch.int32)
+    assert not block(x, adapter).requires_grad
+    assert block.project(x, adapter).requires_grad
