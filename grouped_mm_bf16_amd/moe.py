@@ -359,6 +359,8 @@ def moe_forward(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor
 
     ``interleaved`` ("swiglu" only): ``w_up`` is in the layout of :func:`interleave_gate_up`; the activation then
     runs inside the up projection's epilogue on the fp32 products (one rounding less, no [S, 2I] intermediate).
+
+    It has no gradient: where an operand requires one the result does too, and a backward pass that reaches it raises.
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
         raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")
@@ -383,7 +385,14 @@ def moe_forward(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Tensor
     y = torch.empty(act.size(0), w_down.size(2), device=x.device, dtype=x.dtype)
     grouped_mm_2d3d(act, w_down, routing.offs, y)   # rows are already sorted by expert
     del act
-    return moe_combine(y, routing, T, top_k)
+    out = moe_combine(y, routing, T, top_k)
+    if torch.compiler.is_compiling():
+        return out
+    if derivatives.tangent(x, router_logits, w_up, w_down):
+        raise RuntimeError("moe_forward has no forward-mode derivative")
+    if (x.requires_grad or router_logits.requires_grad or w_up.requires_grad or w_down.requires_grad) and torch.is_grad_enabled():
+        out, = derivatives.without_derivative("moe_forward has no gradient: call it under torch.no_grad(), or with detached operands", out)
+    return out
 
 
 # ------------------------------------------------------------------ the whole layer for a few tokens

@@ -174,3 +174,32 @@ def test_the_example_block_is_inference(monkeypatch, tokens):
     x, adapter = torch.randn(tokens, 16, requires_grad=True), torch.zeros(tokens, dtype=torch.int32)
     assert not block(x, adapter).requires_grad
     assert block.project(x, adapter).requires_grad
+
+
+@pytest.fixture
+def layer_stages(monkeypatch):
+    """moe_forward's launches."""
+    routing = moe.Routing(*(torch.zeros(8, dtype=torch.int32) for _ in range(5)))
+    monkeypatch.setattr(moe, "moe_route", lambda logits, k, renormalize: routing)
+    monkeypatch.setattr(moe, "_gate_up_now", lambda x, rows, w, offs: torch.zeros(8, 32, dtype=x.dtype))
+    monkeypatch.setattr(moe, "grouped_mm_2d3d", lambda a, b, offs, out: None)
+    monkeypatch.setattr(moe, "moe_combine", lambda y, r, tokens, k: torch.ones(tokens, y.size(1), dtype=y.dtype))
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_the_layer_of_many_launches_raises_in_the_backward_pass(layer_stages, which):
+    """It has always taken operands that require a gradient: it still does, but a gradient through it is an error."""
+    args = layer_args()
+    want = moe.moe_forward(*args, 2)
+    assert not want.requires_grad
+    args[which].requires_grad_()
+    got = moe.moe_forward(*args, 2)
+    assert torch.equal(got.detach(), want)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        (args[0].float() + got.float()).sum().backward()
+    with torch.no_grad():
+        assert not moe.moe_forward(*args, 2).requires_grad
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which].detach(), torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            moe.moe_forward(*args, 2)
