@@ -24,6 +24,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from . import derivatives
 from . import kernels as _k
 
 _FLOAT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -219,7 +220,7 @@ class _GroupedMM(torch.autograd.Function):
                     _k.grouped_mm_2d2d(_t(mat_a), grad_out, offs, grad_b)
                 else:
                     _k.grouped_mm_3d3d(_t(mat_a), grad_out, grad_b)
-        return grad_a, grad_b, None, None, None
+        return *derivatives.gradients("grouped_mm", grad_a, grad_b), None, None, None
 
 
 def grouped_mm(

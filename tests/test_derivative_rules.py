@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from grouped_mm_bf16_amd import expert_block, kernels, lora, moe, norm
+from grouped_mm_bf16_amd import api, expert_block, kernels, lora, moe, norm
 
 
 @pytest.fixture
@@ -203,3 +203,21 @@ def test_the_layer_of_many_launches_raises_in_the_backward_pass(layer_stages, wh
         args[which] = forward_ad.make_dual(args[which].detach(), torch.ones_like(args[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             moe.moe_forward(*args, 2)
+
+
+# ------------------------------------------------------------------ the grouped product
+@pytest.mark.parametrize("through", ["sum", "cubes"])
+def test_the_grouped_product_has_no_second_derivative(monkeypatch, through):
+    monkeypatch.setattr(api, "validate_inputs", lambda a, b, *rest: api.Checked(False, False, a.dtype))
+    monkeypatch.setattr(api._k, "grouped_mm_3d3d", lambda a, b, out: out.copy_((a.detach() @ b.detach())))
+    gen = torch.Generator().manual_seed(0)
+    for which in range(2):
+        ab = [torch.randn(2, 3, 4, generator=gen), torch.randn(2, 4, 5, generator=gen)]
+        ab[which].requires_grad_()
+        y = api.grouped_mm(*ab)
+        value = y.sum() if through == "sum" else (y ** 3).sum()
+        first, = torch.autograd.grad(value, ab[which], retain_graph=True)
+        grad, = torch.autograd.grad(value, ab[which], create_graph=True)
+        assert torch.equal(first, grad.detach())
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (value + grad.square().sum()).backward()
