@@ -2,7 +2,8 @@
 //   z = (x - mean) * rstd,  rstd = 1 / sqrt(var + eps),  y = z * w + b
 //   g = dy * w:  dx = rstd * (g - mean(g) - z * mean(g * z));   dw = sum over the rows of dy * z;   db = sum over the rows of dy
 // Memory bounds both directions: forward reads x and writes y, backward reads x and dy and writes dx.  A row is read once and stays
-// in registers between its sums; mean and variance are two sums over registers (no cancellation as with the sum of squares).  All
+// in registers between its sums; mean and variance are two sums over registers (no cancellation as with the sum of squares), and
+// what the first mean's rounding left is added up and taken back: of a constant row of 1e4 the result was 0.3 off.  All
 // sums are fp32.  8 to 1024 lanes share a row, 16 bytes to an access, so that short rows fill a wave and long ones fit into
 // registers; the next row is on its way while one is summed.
 //   forward   16384 x 4096 bf16 47 us, 8192 x 14336 fp16 89 us, 4096 x 16384 fp32 82 us (5.3 to 6.6 TB/s; a copy of that size 5.0)
@@ -166,29 +167,48 @@ __global__ void __launch_bounds__(kBlock<LANES>) norm_forward_kernel(const NormA
     }
     fetch(row + step);
     row_sum<LANES>(s, 1, slots, turn);
-    const float mean = s[0] * inv;
-    s[0] = 0;
+    float mean = s[0] * inv;
+    asm volatile("" : "+v"(mean));      // rounded: what is subtracted is what `rest` is added to (and not the product, in a fused operation)
+    s[0] = s[1] = 0;
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const Chunk<N, TAIL> c((p * LANES + lane) * N, a.width);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         x[p][i] -= mean;
-        s[0] += c.own(i) ? x[p][i] * x[p][i] : 0.0f;
+        const float d = c.own(i) ? x[p][i] : 0.0f;
+        s[0] += d * d;
+        if constexpr (sizeof(T) == 4) s[1] += d;
       }
     }
-    row_sum<LANES>(s, 1, slots, turn);
-    const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
+    row_sum<LANES>(s, sizeof(T) == 4 ? 2 : 1, slots, turn);
+    // What the mean's rounding left: of 16-bit rows only where it shows, the same for all lanes of a row (always: 8192 x 14336 fp16 89 -> 98 us)
+    float var = s[0] * inv;
+    if (sizeof(T) == 2 && mean * mean > 256.0f * (var + a.eps)) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const Chunk<N, TAIL> c((p * LANES + lane) * N, a.width);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[1] += c.own(i) ? x[p][i] : 0.0f;
+      }
+      s[0] = s[1];
+      row_sum<LANES>(s, 1, slots, turn);
+      s[1] = s[0];
+    }
+    const float rest = s[1] * inv;
+    var -= rest * rest;
+    const float rstd = 1.0f / sqrtf((var < 0 ? 0.0f : var) + a.eps);
     if (row >= a.rows) continue;
     if (lane == 0 && a.mean) {
-      a.mean[row] = mean;
+      a.mean[row] = mean + rest;
       a.rstd[row] = rstd;
     }
     T* y = static_cast<T*>(a.out) + row * a.out_stride;
+    const float shift = -rest * rstd;
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[p][i] = x[p][i] * rstd * w[p][i] + b[p][i];
+      for (int i = 0; i < N; ++i) x[p][i] = (x[p][i] * rstd + shift) * w[p][i] + b[p][i];
       store_row(y, Chunk<N, TAIL>((p * LANES + lane) * N, a.width), x[p]);
     }
   }
