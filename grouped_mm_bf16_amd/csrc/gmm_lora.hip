@@ -648,7 +648,7 @@ __device__ __forceinline__ bool find_chunk(const GradArgs& a, int which, int& ad
   return false;
 }
 
-constexpr int kMaxChunk = 4096;
+constexpr int kPiece = 4096;      // rows of a chunk whose places are in LDS at a time
 
 // out[i] += q^T p over a chunk of adapter i's rows: R rows, a strip of 128 columns of p, the contraction along p's rows.
 // WHOLE: there are eight columns.
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   using S = Skinny<T, GMM_W_ROWS, 8, MF, 2, GMM_A_STAGED, 2>;
   constexpr int FR = S::FR, OUT = S::COLUMNS;
   __shared__ SkinnyShared<S, kWaves> shared;
-  __shared__ int32_t row_at[kMaxChunk];
+  __shared__ int32_t row_at[kPiece];
   __shared__ __align__(16) float up[16 * MF];
   constexpr bool FP16 = std::is_same_v<T, F16>;
   const bool second = int(blockIdx.x) >= args.groups0;
@@ -666,11 +666,9 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   int adapter, first, rows, slot;
   if (!find_chunk(args, item / a.tiles, adapter, first, rows, slot)) return;
   const int tile = item % a.tiles, r0 = blockIdx.y * 16 * MF;
-  for (int u = threadIdx.x; u < rows; u += kThreads) row_at[u] = args.row_at[first + u];
   if constexpr (FP16)
     if (int(threadIdx.x) < 16 * MF)
       up[threadIdx.x] = exponent_of(a.peak, args.peak_parts, args.L, args.R, adapter, min(r0 + int(threadIdx.x), args.R - 1)).up();
-  __syncthreads();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int c = tile * OUT + FR * j, columns = max(0, min(FR, a.C - c)), R = args.R, end = (rows + 7) / 8 * 8;   // zeros behind the last row
   S s;
@@ -679,13 +677,14 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   s.a_plane = uint32_t(R) * args.places * 2;
   s.a_buf = buffer(a.q, 2 * s.a_plane);
   s.set_rows([&](int r) { return r0 + r < R ? (uint32_t(r0 + r) * args.places + first) * 2 : kNowhere; });
-  // Steps as Skinny has them, from rows that are anywhere (64-bit addresses).  Past the end the last row is read again and not used.
+  // Steps as Skinny has them, from rows that are anywhere (64-bit addresses).  Past the end of a piece its last row is read again and not used.
   const T* const p = static_cast<const T*>(a.p) + (WHOLE ? min(c, a.C - FR) : columns ? c : 0);
+  int piece = 0, piece_end = 0;
   const auto load = [&](typename S::Step& step, int k) {
-    const int kl = k + 8 * g;
+    const int kl = k + 8 * g - piece;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      const T* at = p + int64_t(row_at[min(kl + r, rows - 1)]) * a.p_ld;
+      const T* at = p + int64_t(row_at[min(kl + r, piece_end - piece - 1)]) * a.p_ld;
       u32x4 v = {0, 0, 0, 0};
       if constexpr (WHOLE) {
         v = unaligned<u32x4>(at);
@@ -699,7 +698,7 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
     __builtin_amdgcn_sched_barrier(0);
   };
   const auto multiply = [&](typename S::Step& step, int k, f32x4 (&acc)[MF][FR]) {
-    if (k >= rows) return;
+    if (k >= piece_end) return;
     if (k + 32 > rows) {
 #pragma unroll
       for (int r = 0; r < 8; ++r)
@@ -711,12 +710,17 @@ __global__ void __launch_bounds__(kThreads) lora_grad_kernel(const GradArgs args
   };
   f32x4 acc[MF][FR];
   clear(acc);
-  if (rows) {
+  for (; piece < rows; piece = piece_end) {
     constexpr int NEXT = 32 * kWaves;
+    static_assert(kPiece % (2 * NEXT) == 0);
+    piece_end = min(rows, piece + kPiece);
+    __syncthreads();
+    for (int u = threadIdx.x; u < piece_end - piece; u += kThreads) row_at[u] = args.row_at[first + piece + u];
+    __syncthreads();
     typename S::Step step[2];
-    load(step[0], 32 * wave);
-    load(step[1], 32 * wave + NEXT);
-    for (int k = 32 * wave; k < rows; k += 2 * NEXT)
+    load(step[0], piece + 32 * wave);
+    load(step[1], piece + 32 * wave + NEXT);
+    for (int k = piece + 32 * wave; k < piece_end; k += 2 * NEXT)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         multiply(step[u], k + u * NEXT, acc);
@@ -1045,10 +1049,10 @@ struct GradPlan {
 bool plan_grad(int64_t rows, int64_t K, int64_t N, int64_t R, int64_t L, GradPlan& p) {
   const int64_t table = gmm_moe_route_workspace_bytes(rows, L + 1, 1);
   if (table < 0) return false;
-  // chunks: as long as leaves some workgroups, one for a chunk and 128 columns, to a compute unit; the partial sums of at most 32 chunks
-  // of all rows
-  const int64_t tiles = (K + 127) / 128 + (N + 127) / 128;
-  p.chunk = clamp(round_up(rows * tiles / 1024 > rows / 32 ? rows * tiles / 1024 : rows / 32, 128), 256, kMaxChunk);
+  // chunks: as long as leaves some workgroups, one for a chunk and 128 columns, to a compute unit, up to 4096 rows; or a 32nd of all rows, so
+  // that the partial sums stay few (1 million rows of 4096 -> 4096, rank 64: 0.7 GB with the operands, in chunks of 4096 rows 1.6)
+  const int64_t tiles = (K + 127) / 128 + (N + 127) / 128, least = round_up(rows / 32, 128);
+  p.chunk = clamp(round_up(rows * tiles / 1024 > rows / 32 ? rows * tiles / 1024 : rows / 32, 128), 256, least > 4096 ? least : 4096);
   p.places = round_up(rows, 8) + 8 * (L + 1);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) { const int64_t here = at; at = round_up(at + bytes, 256); return here; };

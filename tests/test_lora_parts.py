@@ -1,7 +1,8 @@
 """Rows of the projection with adapters whose product is held in float32 at a time (host arithmetic, no GPU)."""
 import pytest
+import torch
 
-from grouped_mm_bf16_amd import lora
+from grouped_mm_bf16_amd import _lib, lora
 
 
 @pytest.mark.parametrize("N", [64, 4096, 1 << 21])
@@ -10,3 +11,16 @@ def test_the_product_in_float32_stays_small(N):
         most = lora._rows_at_once(T, N)
         assert T <= most or most % 256 == 0 and 2 * ((T - 1) % most + 1) >= most
         assert most <= 2304 or most * N <= 1 << 25
+
+
+def test_the_gradients_workspace_stays_near_its_operands():
+    """Of 1 million rows: 0.54 GB of operands, at most 32 + 32 partial sums of [64, 4096] in float32 for each gradient."""
+    size = _lib.load().gmm_lora_grad_workspace_bytes
+    rows, K, N, R, L = 1 << 20, 4096, 4096, 64, 8
+    operands = 2 * 2 * R * (rows + 8 * (L + 2)) * 2
+    partial = 2 * 64 * R * K * 4
+    places = 5 * 4 * (rows + 8 * (L + 2)) + (1 << 20)
+    peaks = 2 * 32 * L * R * 4
+    assert 0 < size(rows, K, N, R, L) <= operands + partial + places + peaks
+    for rows in (100, 5000, 131072, 1 << 18, 1 << 20):
+        assert size(rows, 512, 512, 16, 4) > 0
