@@ -223,6 +223,10 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     _check(x, weight, lora_a, lora_b, adapter, scale)
     if ((x.requires_grad or weight.requires_grad or lora_a.requires_grad or lora_b.requires_grad) and torch.is_grad_enabled()
             or derivatives.forward_mode()):      # with a tangent it raises: there is no forward-mode derivative
+        if ((lora_a.requires_grad or lora_b.requires_grad)
+                and _grad_workspace_bytes(x.device.index, x.size(0), *weight.shape, lora_a.size(2), lora_a.size(0)) < 0):
+            raise RuntimeError(f"lora_linear: too many rows for gradients of adapters of rank {lora_a.size(2)}, or too large ones: got "
+                               f"{x.size(0)} rows, {weight.size(0)} to {weight.size(1)}")
         return _Lora.apply(x, weight, lora_a, lora_b, adapter, scale)
     impl = _forward_op if torch.compiler.is_compiling() else _forward_now
     return impl(_rows(x), weight, lora_a, lora_b, adapter, scale, False)[0]
