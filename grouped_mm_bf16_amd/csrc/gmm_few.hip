@@ -2,8 +2,8 @@
 //   out[t] = sum over the choices j of w_tj * act(x[t] @ w_up[e_tj]) @ w_down[e_tj]
 // Routing as gmm_moe_route, then every chosen expert's matrices are read once, past a few rows (gmm_skinny.h).  Reading them bounds
 // it: 8 tokens, 2 of 8 experts of 4096 -> 2 x 14336 361 to 397 us by card (7.0 to 6.4 TB/s), 32 tokens, 8 of 128 experts of 2048 -> 2 x 768 151 to 160 us (7.0 to 6.6).
-// Between the two products the activations stay in 32 bits (two 16-bit values each), the second products in fp32: the result is
-// rounded once.
+// Between the two products the activations are two 16-bit values each (bf16: 2^-16 of them is lost, fp16: 2^-22 or, below 2^-3, 2^-25;
+// past 65504 fp16 has infinity, as the layer of many launches), the second products fp32: the result is rounded once.
 // Of very few tokens the time is that of the launches and of the trips to memory behind one another (1 token, 8 of 128 experts of
 // 2048 -> 2 x 768 25 us, of which the weights are 11).  Then there are two launches: every workgroup of the first routes for
 // itself, and of the second's, the last that is done with some columns adds them up.
@@ -31,7 +31,9 @@ constexpr int kRouteSlots = 32, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
 // all of them would.  2 tokens, 6 of 34 experts of 280 -> 600 16 us, with a launch for the sums 17 (1 token of small experts 15 and 16); 6
 // tokens, 4 of 8 experts of 432 -> 2 x 10752 60 and 56.
 constexpr int kJoinSlots = 16;
-constexpr int kLine = 32;          // words from one counter to the next: 384 arrivals at 16 counters of one cache line took 8 us
+// Words from one counter to the next.  2 tokens, 6 of 64 experts of 2048 -> 2 x 1408 38 to 41 us, with the counters side by side 60 (1 token, 8 of
+// 128 of 2 x 768 25 and 26).
+constexpr int kLine = 32;
 
 // Workgroups that a compute unit is to hold: two where their sums leave the registers.  Column-major, 33 tokens and more (strips of half as many
 // columns): 64 tokens through 8 of 128 experts of 2048 -> 2 x 768 214 us, held to two 202; 40 through 4 of 8 of 432 -> 2 x 10752 108 and 88.

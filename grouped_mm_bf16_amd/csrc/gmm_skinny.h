@@ -44,7 +44,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint3
 }
 
 // Value f as the sum of two 16-bit values: an operand that is held in 32 bits takes part in a product of 16-bit operands as two, and
-// its error is then 2^-16 (bf16) or 2^-22 (fp16) of it.  Where the first overflows there is no second (fp16: |f| >= 65520).
+// its error is then 2^-16 of it (bf16), or 2^-22 of it and 2^-25 at least (fp16, whose second value is below its normal range for |f| < 2^-3).
+// Where the first overflows there is no second (fp16: |f| >= 65520).
 template <typename T>
 __device__ __forceinline__ void split(float f, T& high, T& low) {
   high = rounded<T>(f);

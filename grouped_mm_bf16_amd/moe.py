@@ -436,8 +436,9 @@ def moe_forward_few(x: torch.Tensor, router_logits: torch.Tensor, w_up: torch.Te
     """:func:`moe_forward` for up to ``FEW_TOKENS`` tokens, a decoding step: the chosen experts' matrices are streamed past the
     tokens' rows in kernels made for that, without tiles for rows that are not there.
 
-    Arguments as there; bf16 or fp16, any sizes and weight strides.  Activations and the experts' results stay in 32 bits: the result is
-    rounded once (``moe_forward`` rounds three times, so the two differ by roundings).  Forward only: it refuses operands that require a
+    Arguments as there; bf16 or fp16, any sizes and weight strides.  Activations are held as two 16-bit values each (in fp16 with its range:
+    infinite past 65504, 2^-25 off at least), the experts' results in float32: the result is rounded once (``moe_forward`` rounds
+    three times, so the two differ by roundings).  Forward only: it refuses operands that require a
     gradient unless gradients are off.
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):

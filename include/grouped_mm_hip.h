@@ -243,7 +243,8 @@ int gmm_moe_combine(const void* y, const int32_t* token_rows, const float* slot_
  * columns, then partners, or 64 and 64 in turn as gmm_2d3d_swiglu has them: inner a multiple of 64), w_down [experts, inner, hidden];
  * strides in elements, any for the weights (those contiguous along either dimension are read fastest, at any alignment), rows of x,
  * logits and out contiguous; one expert's matrix below 2 GiB.  dtype bf16 or fp16, logits_dtype any gmm_dtype.  Unlike the calls
- * it stands for it keeps the activations and the experts' results in 32 bits and rounds once.  `workspace`: device memory of
+ * it stands for it keeps the activations as two 16-bit values each (in fp16 within its range) and the experts' results in fp32, and rounds
+ * once.  `workspace`: device memory of
  * gmm_moe_few_workspace_bytes(...) bytes (-1: sizes out of range), 16-byte aligned, its contents of no matter.  No host
  * synchronisation, no allocation.  Two to five launches; up to 16 slots the second product's workgroups count their arrivals with an
  * atomic, which decides who adds up, not what or in which order: the result does not depend on timing. */
