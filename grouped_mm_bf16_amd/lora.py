@@ -74,11 +74,9 @@ def _workspace_bytes(device: int, T: int, K: int, N: int, R: int) -> int:
 
 
 def _rows_at_once(T: int, N: int) -> int:
-    """Rows whose product with W is held in float32 at a time: 128 MiB of it, which half of the card's last cache holds, at least 2048, parts
-    of even length."""
-    most = max(2048, (1 << 25) // max(N, 1))
-    parts = -(-T // most)
-    return T if parts <= 1 else -(-T // (parts * 256)) * 256
+    """Rows whose product with W is held in float32 at a time: 512 MiB of it, at least 2048.  Smaller parts cost rounds of tiles that are not full:
+    65536 rows of 4096 -> 4096 2.07 ms in parts of 32768 rows, 2.29 in parts of 8192, 2.1 all at once."""
+    return min(T, max(2048, (1 << 27) // max(N, 1) // 256 * 256))
 
 
 @functools.lru_cache(maxsize=4096)
