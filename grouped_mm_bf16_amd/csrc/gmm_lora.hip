@@ -8,7 +8,7 @@
 //     reading x, by reading that product and by writing y: 8192 rows of 4096 -> 4096, rank 16, 69 us (268 MB, 3.9 TB/s).
 //   Gradients (gmm_lora_grad): dA[i] = scale[i] * sum of x[t]^T u[t], dB[i] = scale[i] * sum of low[t]^T dy[t] over the rows t that have
 //     adapter i: thin products along the rows, bound by reading x and dy: of those 8192 rows 30 us (134 MB, 4.5 TB/s), and 20 for the sort before
-//     and the sums behind.
+//     and the sums behind; in fp16 6 more for the powers of two.
 // The rank-sized values x @ A and dy @ B^T stay in fp32; where they are operands of a 16-bit product they are two values each, in fp16 behind
 // a power of two that brings them into its range.
 #include <hip/hip_runtime.h>

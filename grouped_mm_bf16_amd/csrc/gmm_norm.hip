@@ -6,7 +6,7 @@
 // what the first mean's rounding left is added up and taken back: of a constant row of 1e4 the result was 0.3 off.  All
 // sums are fp32.  8 to 1024 lanes share a row, 16 bytes to an access, so that short rows fill a wave and long ones fit into
 // registers; the next row is on its way while one is summed.
-//   forward   16384 x 4096 bf16 47 us, 8192 x 14336 fp16 89 us, 4096 x 16384 fp32 82 us (5.3 to 6.6 TB/s; a copy of that size 5.0)
+//   forward   16384 x 4096 bf16 47 us, 8192 x 14336 fp16 91 us, 4096 x 16384 fp32 83 us (5.2 to 6.5 TB/s; a copy of that size 5.0)
 //   backward  16384 x 4096 bf16 70 us, 8192 x 14336 fp16 143 us (5.7 and 4.9 TB/s), with the sums over the rows
 // Rows that are no whole number of vectors cost about half as much again for an element: 4320 x 4397 bf16 27 and 40 us.
 #include <hip/hip_runtime.h>
