@@ -89,6 +89,8 @@ def _forward_now(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lo
     """The result, and (with `save`) x @ lora_a of the rows that have an adapter, [T, R] float32."""
     (T, K), N, dev = x.shape, weight.size(1), x.device
     L, _, R = lora_a.shape
+    if save and _grad_workspace_bytes(dev.index, T, K, N, R, L) < 0:
+        raise RuntimeError(f"lora_linear: too many rows for gradients of adapters of rank {R}, or too large ones: got {T} rows, {K} to {N}")
     out = torch.empty(T, N, device=dev, dtype=x.dtype)
     low = torch.empty(T, R, device=dev, dtype=torch.float32) if save else None
     lib = _lib.load()
@@ -221,10 +223,6 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     _check(x, weight, lora_a, lora_b, adapter, scale)
     if ((x.requires_grad or weight.requires_grad or lora_a.requires_grad or lora_b.requires_grad) and torch.is_grad_enabled()
             or derivatives.forward_mode()):      # with a tangent it raises: there is no forward-mode derivative
-        if ((lora_a.requires_grad or lora_b.requires_grad)
-                and _grad_workspace_bytes(x.device.index, x.size(0), *weight.shape, lora_a.size(2), lora_a.size(0)) < 0):
-            raise RuntimeError(f"lora_linear: too many rows for gradients of adapters of rank {lora_a.size(2)}, or too large ones: got "
-                               f"{x.size(0)} rows, {weight.size(0)} to {weight.size(1)}")
         return _Lora.apply(x, weight, lora_a, lora_b, adapter, scale)
     impl = _forward_op if torch.compiler.is_compiling() else _forward_now
     return impl(_rows(x), weight, lora_a, lora_b, adapter, scale, False)[0]
