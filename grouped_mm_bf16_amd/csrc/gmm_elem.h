@@ -64,6 +64,21 @@ __device__ __forceinline__ V unaligned(const void* p) {
 
 template <typename T> constexpr int kVector = 16 / int(sizeof(T));
 
+// Eight (fp32: four) elements to an access, which may begin anywhere.  Where fewer are left in a row (TAIL) the last eight are loaded: `skip`
+// of them are another lane's.
+template <int N, bool TAIL>
+struct Chunk {
+  int at, skip;
+  bool in;
+  __device__ __forceinline__ Chunk(int c, int width) : at(c), skip(0), in(c < width) {
+    if constexpr (TAIL) {
+      at = min(c, width - N);
+      skip = c - at;
+    }
+  }
+  __device__ __forceinline__ bool own(int i) const { return in && (!TAIL || i >= skip); }
+};
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace gmm

@@ -37,21 +37,6 @@ struct NormArgs {
   float eps;
 };
 
-// Eight (fp32: four) elements to an access, which may begin anywhere.  Where fewer are left in a row (TAIL) the last eight are loaded: `skip`
-// of them are another lane's.
-template <int N, bool TAIL>
-struct Chunk {
-  int at, skip;
-  bool in;
-  __device__ __forceinline__ Chunk(int c, int width) : at(c), skip(0), in(c < width) {
-    if constexpr (TAIL) {
-      at = min(c, width - N);
-      skip = c - at;
-    }
-  }
-  __device__ __forceinline__ bool own(int i) const { return in && (!TAIL || i >= skip); }
-};
-
 // A chunk of a row that is read once.  Non-temporal, which keeps it from driving out what is written (4096 x 16384 fp32 99 -> 81 us; rows that
 // lie at odd addresses too: 8192 x 14336 fp16, 14337 apart, 111 -> 103), but not where a row ends inside a chunk: two lanes then read its
 // last cache line, one after the other (21800 x 329 fp32 11.8, non-temporal 15.3 us).

@@ -275,7 +275,7 @@ def _run_sort(s):
         from grouped_mm_bf16_amd import moe_train
         routing = moe_train.route(s["logits"], s["top_k"], s["renormalize"])
         rows = moe_train.sort_rows(s["x"], routing)
-        out = moe_train.combine_rows(s["y"], routing)
+        out = moe_train.combine_rows(s["y"], routing, s["top_k"])
         grads = torch.autograd.grad((rows, out), (s["x"], s["y"], s["logits"]), (s["grad_sorted"], s["grad_out"]))
         return {"row_token": routing.row_token, "offs": routing.offs, "sorted": rows.detach(), "out": out.detach(), "grad_x": grads[0],
                 "grad_y": grads[1], "grad_logits": grads[2]}
