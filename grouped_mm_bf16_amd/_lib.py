@@ -54,6 +54,13 @@ SIGNATURES = {
     "gmm_layer_norm": (ctypes.c_int, [_vp] * 6 + [_i64] * 4 + [ctypes.c_float, _i32, _i32, _vp]),
     "gmm_layer_norm_workspace_bytes": (_i64, [_i64, _i64]),
     "gmm_layer_norm_backward": (ctypes.c_int, [_vp] * 8 + [_i64] * 5 + [_i32, _i32, _vp, _i64, _vp]),
+    "gmm_moe_sort_rows": (ctypes.c_int, [_vp] * 3 + [_i64] * 6 + [_i32, _vp]),
+    "gmm_moe_sum_rows": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp]),
+    "gmm_moe_combine_backward": (ctypes.c_int, [_vp] * 6 + [_i64] * 7 + [_i32, _vp]),
+    "gmm_moe_route_backward": (ctypes.c_int, [_vp] * 5 + [_i64] * 4 + [_i32, _vp]),
+    "gmm_gated": (ctypes.c_int, [_vp] * 2 + [_i64] * 4 + [_i32, _i32, _vp]),
+    "gmm_gated_backward": (ctypes.c_int, [_vp] * 3 + [_i64] * 5 + [_i32, _i32, _vp]),
+    "gmm_dropout": (ctypes.c_int, [_vp] * 5 + [_i64] * 5 + [_i32, _i32, _i32, _vp]),
     "gmm_set_path": (ctypes.c_int, [ctypes.c_int]),
     "gmm_last_path": (ctypes.c_int, []),
     "gmm_last_kernel": (ctypes.c_int, []),

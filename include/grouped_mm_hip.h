@@ -317,6 +317,45 @@ int gmm_layer_norm_backward(const void* dy, const void* x, const void* weight, c
                             int64_t dy_stride, int64_t x_stride, int64_t dx_stride,
                             int32_t dtype, int32_t weight_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- What stands around the grouped products of an expert layer that is trained.  No counterpart in the reference.
+ * Slot t * top_k + j is choice j of token t, token_rows (as gmm_moe_route writes it) its row among those sorted by expert; a slot whose row is
+ * outside [0, rows) takes no part.  bf16, fp16 or fp32 (dtype), any width, any alignment, row strides in elements (at least the width where
+ * there is more than one row), top_k <= 32.  Sums in fp32, in the order of the choices, no atomics.
+ *   gmm_moe_sort_rows         out[row of slot (t, j)] = x[t]: x [tokens, hidden], out [out_rows, hidden]
+ *   gmm_moe_sum_rows          out[t] = sum of slot_weight[t, j] * y[row of slot (t, j)] (slot_weight NULL: ones): y [y_rows, hidden],
+ *                             out [tokens, hidden]; without weights the gradient of gmm_moe_sort_rows
+ *   gmm_moe_combine_backward  of gmm_moe_sum_rows, for dout [tokens, hidden]: dy[row of slot (t, j)] = slot_weight[t, j] * dout[t]  [y_rows,
+ *                             hidden] (rows that no slot has are left as they are), dweight[t, j] = <dout[t], y[row of slot (t, j)]> float;
+ *                             either may be NULL (without dweight y is not read) */
+int gmm_moe_sort_rows(const void* x, const int32_t* token_rows, void* out, int64_t tokens, int64_t top_k, int64_t hidden,
+                      int64_t out_rows, int64_t x_stride, int64_t out_stride, int32_t dtype, void* stream);
+int gmm_moe_sum_rows(const void* y, const int32_t* token_rows, const float* slot_weight, void* out, int64_t tokens, int64_t top_k,
+                     int64_t hidden, int64_t y_rows, int64_t y_stride, int64_t out_stride, int32_t dtype, void* stream);
+int gmm_moe_combine_backward(const void* dout, const void* y, const int32_t* token_rows, const float* slot_weight, void* dy, float* dweight,
+                             int64_t tokens, int64_t top_k, int64_t hidden, int64_t y_rows, int64_t dout_stride, int64_t y_stride,
+                             int64_t dy_stride, int32_t dtype, void* stream);
+
+/* Gradient of gmm_moe_route's weights: dlogits [tokens, experts] (logits_dtype, contiguous) for dweight float[tokens * top_k], of the softmax over
+ * the chosen logits (logits NULL; slot_weight as it was written: zeros for what was not chosen) or over all (logits as they were given). */
+int gmm_moe_route_backward(const float* dweight, const int32_t* slot_expert, const float* slot_weight, const void* logits, void* dlogits,
+                           int64_t tokens, int64_t experts, int64_t top_k, int64_t logits_stride, int32_t logits_dtype, void* stream);
+
+/* Activation between the projections as gmm_moe_activation has it (kind GMM_ACT_SILU or GMM_ACT_SWIGLU), for any type, width and alignment, and its
+ * gradient dh [rows, inner or 2 * inner] for dout [rows, inner]. */
+int gmm_gated(const void* h, void* out, int64_t rows, int64_t inner, int64_t h_stride, int64_t out_stride, int32_t kind, int32_t dtype,
+              void* stream);
+int gmm_gated_backward(const void* dout, const void* h, void* dh, int64_t rows, int64_t inner, int64_t dout_stride, int64_t h_stride,
+                       int64_t dh_stride, int32_t kind, int32_t dtype, void* stream);
+
+/* ---- Dropout.  No counterpart in the reference.
+ *   out = residual + (bits >= limit ? x * 65536 / (65536 - limit) : 0)      (residual NULL: without), in fp32, rounded once
+ * x, residual, out [rows, width] (dtype), row strides in elements.  The 16 bits of element i = row * width + column are number i % 8, the low half
+ * of a word first, of what Philox 4x32-10 makes of the key rng[0] and the counter (i / 8 + site * 2^48, rng[1]).  rng: two int64 on the device; `used`
+ * (NULL: not wanted) gets a copy of them.  The gradient of x is the same call with rng = used and without a residual.  limit in [0, 65536], site in
+ * [0, 65535]. */
+int gmm_dropout(const void* x, const void* residual, void* out, const int64_t* rng, int64_t* used, int64_t rows, int64_t width,
+                int64_t x_stride, int64_t residual_stride, int64_t out_stride, int32_t limit, int32_t site, int32_t dtype, void* stream);
+
 /* Test and tuning hooks (the reference exposes its tile knobs through environment
  * variables read in the launcher, kernels.py:590-634; tests force tiles through
  * them, tests/test_grouped_mm.py:388-394).  gmm_set_path forces a kernel family
