@@ -66,15 +66,16 @@ def _compile(src: str, force: bool) -> str:
 
 
 def generate(force: bool = False) -> str:
-    """Run gen_tile_asm.py -> csrc/gmm_tile_asm.inc (the hand-scheduled tile assembly)."""
+    """Run gen_tile_asm.py -> csrc/gmm_tile_asm.inc (the hand-scheduled tile assembly), csrc/gmm_tile_asm_int8.inc (on 8-bit integers)."""
     gen = os.path.join(CSRC, "gen_tile_asm.py")
-    inc = os.path.join(CSRC, "gmm_tile_asm.inc")
-    if force or _stale(inc, [gen]):
-        res = subprocess.run([sys.executable, gen], capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"gen_tile_asm.py failed:\n{res.stderr}")
-        with open(inc, "w") as f:
-            f.write(res.stdout)
+    for name, args in (("gmm_tile_asm_int8.inc", ["--int8"]), ("gmm_tile_asm.inc", [])):
+        inc = os.path.join(CSRC, name)
+        if force or _stale(inc, [gen]):
+            res = subprocess.run([sys.executable, gen, *args], capture_output=True, text=True)
+            if res.returncode != 0:
+                raise RuntimeError(f"gen_tile_asm.py failed:\n{res.stderr}")
+            with open(inc, "w") as f:
+                f.write(res.stdout)
     return inc
 
 

@@ -2,7 +2,8 @@
 """Generates gmm_tile_asm.inc: the per-tile main loop and epilogue of the MFMA
 grouped GEMM kernels as hand-scheduled gfx950 assembly.
 
-    python gen_tile_asm.py > gmm_tile_asm.inc      (build.py does this)
+    python gen_tile_asm.py > gmm_tile_asm.inc                  (build.py does both)
+    python gen_tile_asm.py --int8 > gmm_tile_asm_int8.inc
 
 Why generated assembly: the loop keeps 256 accumulator registers, two sets of
 MFMA operand fragments and sixteen in-flight direct-to-LDS copies alive at once.
@@ -55,6 +56,12 @@ Registers:
   v[32:63]     B fragments set 0 (eight of 16 columns x 32 k), v[64:95] set 1
   v[96:119]    temporaries, per-buffer fragment addresses of the 3-buffer variants
   inputs are pinned by the C++ wrapper to v[120:191] and s[28:55] (see GmmTileRegs).
+
+8-bit integers (f16 = 2, 3): the same tile on v_mfma_i32_16x16x64_i8, whose fragments are 16 bytes of K to a lane as well.  Every
+offset, step and K tile is one of bytes, so nothing but the instruction differs in the loop; "64 k" above are 128 bytes, 128
+integers.  Both operands are contiguous along K.  The prologue also copies the scales of the tile's rows and columns into LDS, before
+everything else (its first wait covers them); the epilogue turns each sum into fp32 and multiplies it by its column's, then its row's: a
+weight's scale is small, and what overflows in between would have overflowed anyway.
 """
 import sys
 
@@ -104,6 +111,12 @@ S_RA, S_RB, S_RC = 36, 40, 44   # buffer resources
 S_SC = 48                        # scalars s[48:55]
 S_NK, S_ASTEP, S_BSTEP, S_LDS, S_ROWCNT, S_CSTEP, S_NVALID, S_SPARE = range(48, 56)
 S_T = 56                         # temporaries s[56:79]
+# 8-bit integers: byte offsets of the scale that this lane copies, of a row and of a column (+0, +1), their buffer resources, and
+# where they lie in LDS: 256 of rows, 256 of columns, behind the buffers of all tile heights.  Their read addresses come in
+# the unused halves of the fragment addresses.
+V_SCALE = V_IN + 66
+S_RROWS, S_RCOLS = 92, 96
+SCALES = 147456
 
 
 class Emit:
@@ -142,7 +155,10 @@ class Variant:
         self.rounded = act == 3
         self.partial = act == 2      # fp32 partial tile of a tile cut along K: stored through to memory (sc1)
         assert not (self.act and (out_f32 or a_tr)) and not (self.partial and (not out_f32 or b_nt))
-        self.dt = "f16" if f16 else "bf16"   # element type of A, B and of a 16-bit output
+        self.i8 = f16 >= 2               # 8-bit integers; a 16-bit output is bf16 (2) or fp16 (3)
+        assert not self.i8 or not (a_tr or b_tr or self.act)
+        self.dt = "f16" if f16 & 1 else "bf16"   # element type of A, B and of a 16-bit output
+        self.mfma = "v_mfma_i32_16x16x64_i8" if self.i8 else "v_mfma_f32_16x16x32_" + self.dt
         assert tm in (1, 2, 4) and (tm == 4 or not a_tr)
         self.tn = 8                      # 16-column MFMA blocks per wave (the wave grid is 2 x 2)
         self.na = 2 * tm                 # copies of the A tile per wave and K tile
@@ -168,7 +184,7 @@ class Variant:
         self.a_stage = TR_STAGE if a_tr else (64 * tm * 128 if self.stages == 3 else KC_STAGE)
         self.b_stage = TR_STAGE if b_tr else KC_STAGE
         self.b_base = self.stages * self.a_stage   # LDS offset of B buffer 0
-        self.name = "%s%s_%s_%s_m%d%s%s" % ("t" if a_tr else "k", "t" if b_tr else "k", self.dt, "f32" if out_f32 else self.dt, 64 * tm,
+        self.name = "%s%s_%s_%s_m%d%s%s" % ("t" if a_tr else "k", "t" if b_tr else "k", "i8" if self.i8 else self.dt, "f32" if out_f32 else self.dt, 64 * tm,
                                             "_bnt" if b_nt else "", ("", "_swiglu", "_partial", "_swiglu_rounded")[act])
 
     def acc(self, i, j):
@@ -229,7 +245,7 @@ class Variant:
                 b = vr(V_BF[sp] + 4 * j, 4)
                 c = "a[%d:%d]" % (self.acc(i, j), self.acc(i, j) + 3)
                 # operands swapped: the result block is transposed, a lane owns 4 consecutive columns of a row
-                out.append(((("A", st, x), ("B", sp, j)), "v_mfma_f32_16x16x32_%s %s, %s, %s, %s" % (self.dt, c, b, a, c)))
+                out.append(((("A", st, x), ("B", sp, j)), "%s %s, %s, %s, %s" % (self.mfma, c, b, a, c)))
         return out
 
     # -- copy instruction with issue index n (0..15) of a K tile into buffer buf.
@@ -398,6 +414,13 @@ def gen_main(v, e, L):
     e("s_add_u32 %s, %s, %s" % (sr(s_waveA), sr(s_waveA), sr(S_LDS)))
     e("s_mul_i32 %s, %s, %d" % (sr(s_waveB), sr(sT + 19), v.nb * (TR_BLOCK if v.b_tr else 1024)))
     e("s_add_u32 %s, %s, %s" % (sr(s_waveB), sr(s_waveB), sr(S_LDS)))
+    if v.i8 and not v.partial:
+        e("s_lshl_b32 %s, %s, 8" % (sr(s_t1), sr(sT + 19)))
+        e("s_add_u32 %s, %s, %s" % (sr(s_t1), sr(s_t1), sr(S_LDS)))
+        for k, res in enumerate((S_RROWS, S_RCOLS)):
+            e("s_add_u32 m0, %s, %d" % (sr(s_t1), SCALES + 1024 * k))
+            e("s_nop 0")
+            e("buffer_load_dword %s, %s, 0 offen lds" % (vr(V_SCALE + k), sr(res, 4)))
     # tile 0 -> buffer 0 (head offsets)
     for n in range(v.ncopy):
         for ins in m0_gaps(v.dma(n, 0, "head", 0, 0, s_zero, s_zero, V_TMP)):
@@ -616,6 +639,14 @@ def gen_epilogue(v, e, L):
     e.label("L_nopart_setup_%s" % L)
     if v.rounded:
         e("s_mov_b32 %s, 0x3e800000" % sr(S_T))       # 0.25
+    scaled = v.i8 and not v.partial
+    vcols, vrows = t + 48, t + 48 + 4 * v.tn          # scales of the lane's four columns of each block, of its row of each block row
+    if scaled:
+        for j in range(v.tn):
+            e("ds_read_b128 %s, %s offset:%d" % (vr(vcols + 4 * j, 4), vr(V_RB + 2), 64 * j))
+        for i in range(2 * v.tm):
+            e("ds_read_b32 %s, %s offset:%d" % (vr(vrows + i), vr(V_RA + 2), 64 * i))
+        e("s_waitcnt lgkmcnt(0)")
     nstore = 0
     for p0 in range(0, v.tm, ipp):
         k = 0
@@ -693,6 +724,13 @@ def gen_epilogue(v, e, L):
                 a0 = v.acc(i, j)
                 for r in range(4):
                     e("v_accvgpr_read_b32 %s, a%d" % (vr(b + r), a0 + r))
+                if scaled:
+                    for r in range(4):
+                        e("v_cvt_f32_i32 %s, %s" % (vr(b + r), vr(b + r)))
+                    for r in range(4):
+                        e("v_mul_f32 %s, %s, %s" % (vr(b + r), vr(vcols + 4 * j + r), vr(b + r)))
+                    for r in range(4):
+                        e("v_mul_f32 %s, %s, %s" % (vr(b + r), vr(vrows + i), vr(b + r)))
                 if f32:
                     e("ds_write_b128 %s, %s offset:%d" % (vr(V_EPI), vr(b, 4), rowoff + 16 * j * 4))
                 else:
@@ -747,10 +785,28 @@ def clobbers(v):
     return ", ".join('"%s"' % x for x in c)
 
 
-def main():
-    out = []
-    out.append("// Generated by gen_tile_asm.py -- do not edit.")
-    out.append("// Per-tile main loop + epilogue in gfx950 assembly, one function per operand-layout / output variant.")
+def emit(out, v):
+    """The function of one variant."""
+    e = gen_variant(v)
+    out.append("")
+    out.append("template <> __device__ __forceinline__ void gmm_tile_asm<%d, %d, %d, %d, %d, %d, %d>(GmmTileRegs& r) {"
+               % (v.a_tr, v.b_tr, v.out_f32, v.tm, v.f16, v.b_nt, 2 if v.partial else 3 if v.rounded else 1 if v.act else 0))
+    out.append("  asm volatile(")
+    out.append(e.text())
+    out.append("      :")
+    pins = [(V_VOA_HEAD, 8, "voa_head"), (V_VOB_HEAD, 8, "vob_head"), (V_VOA, 8, "voa"), (V_VOB, 8, "vob"),
+            (V_VOA_TAIL, 8, "voa_tail"), (V_VOB_TAIL, 8, "vob_tail"), (V_RA, 4, "ra_addr"), (V_RB, 4, "rb_addr"),
+            (V_EPI, 4, "epi"), (V_EPI2, 2, "epi2"), (V_TOUCH, 2, "touch"), (V_FIX, 4, "fix")]
+    if v.i8:
+        pins.append((V_SCALE, 2, "scale"))
+    out.append("      : " + ", ".join('"{v[%d:%d]}"(r.%s)' % (b0, b0 + n - 1, name) for b0, n, name in pins) + ",")
+    scales = ', "{s[%d:%d]}"(r.rsrc_rows), "{s[%d:%d]}"(r.rsrc_cols)' % (S_RROWS, S_RROWS + 3, S_RCOLS, S_RCOLS + 3) if v.i8 else ""
+    out.append('        "{s[28:35]}"(r.masks), "{s[36:39]}"(r.rsrc_a), "{s[40:43]}"(r.rsrc_b), "{s[44:47]}"(r.rsrc_c), "{s[48:55]}"(r.scal)' + scales)
+    out.append("      : %s);" % clobbers(v))
+    out.append("}")
+
+
+def defines(out):
     out.append("#define GMM_TILE_PITCH %d" % PITCH)
     out.append("#define GMM_TILE_PITCH32 %d" % PITCH32)
     out.append("#define GMM_TILE_TR_BLOCK %d" % TR_BLOCK)
@@ -759,6 +815,26 @@ def main():
     out.append("#define GMM_TILE_STAGING_BYTES %d" % STAGE_BYTES)
     out.append("#define GMM_TILE_STAGES_SHORT %d" % STAGES_SHORT)
     out.append("#define GMM_TILE_PITCH_ACT %d" % PITCH_ACT)
+    out.append("#define GMM_TILE_SCALES %d" % SCALES)
+
+
+def main_int8():
+    """Of the 8-bit products: bf16 (2), fp16 (3) or fp32 out; partial tiles are sums as they are, 32-bit integers."""
+    out = ["// Generated by gen_tile_asm.py -- do not edit.", "// The tile on 8-bit integers."]
+    defines(out)
+    for f16, f32 in ((2, 0), (2, 1), (3, 0)):
+        for tm in (4, 2, 1):
+            for b_nt, act in ((0, 0), (1, 0), (0, 2)):
+                if not (b_nt and tm == 4) and not (act and not f32):
+                    emit(out, Variant(0, 0, f32, tm, f16, b_nt, act))
+    sys.stdout.write("\n".join(out) + "\n")
+
+
+def main():
+    out = []
+    out.append("// Generated by gen_tile_asm.py -- do not edit.")
+    out.append("// Per-tile main loop + epilogue in gfx950 assembly, one function per operand-layout / output variant.")
+    defines(out)
     for f16 in (0, 1):
         for a_tr, b_tr, f32, tm, b_nt, act in [(a, b, f, t, n, c) for a in (0, 1) for b in (0, 1) for f in (0, 1) for t in (4, 2, 1)
                                                for n in (0, 1) for c in (0, 1, 2, 3)]:
@@ -770,22 +846,9 @@ def main():
                 continue      # the gated epilogue: K-contiguous first operand, 16-bit output
             if act == 2 and (not f32 or b_nt):
                 continue      # partial tiles: fp32, ordinary B copies
-            v = Variant(a_tr, b_tr, f32, tm, f16, b_nt, act)
-            e = gen_variant(v)
-            out.append("")
-            out.append("template <> __device__ __forceinline__ void gmm_tile_asm<%d, %d, %d, %d, %d, %d, %d>(GmmTileRegs& r) {" % (a_tr, b_tr, f32, tm, f16, b_nt, act))
-            out.append("  asm volatile(")
-            out.append(e.text())
-            out.append("      :")
-            pins = [(V_VOA_HEAD, 8, "voa_head"), (V_VOB_HEAD, 8, "vob_head"), (V_VOA, 8, "voa"), (V_VOB, 8, "vob"),
-                    (V_VOA_TAIL, 8, "voa_tail"), (V_VOB_TAIL, 8, "vob_tail"), (V_RA, 4, "ra_addr"), (V_RB, 4, "rb_addr"),
-                    (V_EPI, 4, "epi"), (V_EPI2, 2, "epi2"), (V_TOUCH, 2, "touch"), (V_FIX, 4, "fix")]
-            out.append("      : " + ", ".join('"{v[%d:%d]}"(r.%s)' % (b0, b0 + n - 1, name) for b0, n, name in pins) + ",")
-            out.append('        "{s[28:35]}"(r.masks), "{s[36:39]}"(r.rsrc_a), "{s[40:43]}"(r.rsrc_b), "{s[44:47]}"(r.rsrc_c), "{s[48:55]}"(r.scal)')
-            out.append("      : %s);" % clobbers(v))
-            out.append("}")
+            emit(out, Variant(a_tr, b_tr, f32, tm, f16, b_nt, act))
     sys.stdout.write("\n".join(out) + "\n")
 
 
 if __name__ == "__main__":
-    main()
+    main_int8() if sys.argv[1:] == ["--int8"] else main()

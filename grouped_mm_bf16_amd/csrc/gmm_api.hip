@@ -370,6 +370,43 @@ int gmm_3d2d(const void* a, const void* b, void* out, const int32_t* offs, int32
   return run(pr, static_cast<hipStream_t>(stream));
 }
 
+int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, void* out,
+                const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
+                int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!dims_ok(M, N, a_rows) || K < 0 || K >= 131072 || G < 0 || G >= GMM_MAX_GROUPS || (!offs && G != 1)) return GMM_ERR_BAD_ARGUMENT;
+  if (out_dtype < GMM_DT_BF16 || out_dtype > GMM_DT_F32) return GMM_ERR_UNSUPPORTED;
+  if (G == 0 || M == 0 || N == 0) return GMM_OK;
+  if (!out || (!row_index && a_rows != M) || (out_stride < N && M > 1)) return GMM_ERR_BAD_ARGUMENT;
+  if (!a_scale || !b_scale || (K > 0 && (!a || !b)) || !aligned16(a) || !aligned16(b)) return GMM_ERR_BAD_ARGUMENT;
+  // rows of either operand may lie on one another only where there is one
+  if ((a_stride & 15) || (b_stride_g & 15) || (b_stride_n & 15) || a_stride < 0 || b_stride_g < 0 || b_stride_n < 0) return GMM_ERR_BAD_ARGUMENT;
+  if ((a_stride < K && a_rows > 1) || (b_stride_n < K && N > 1)) return GMM_ERR_BAD_ARGUMENT;
+  // byte offsets inside a tile of 256 rows or columns stay below 2^31
+  constexpr int64_t most = int64_t(1) << 22;
+  if (a_stride >= 2 * most || b_stride_n >= 2 * most || out_stride >= (out_dtype == GMM_DT_F32 ? most / 2 : most)) return GMM_ERR_UNSUPPORTED;
+  if (row_index && a_rows > (int64_t(1) << 31) / (a_stride > 0 ? a_stride : 1) - 1) return GMM_ERR_UNSUPPORTED;
+  const int cus = device_cus();
+  if (cus <= 0) return GMM_ERR_LAUNCH;
+  Problem pr{};
+  pr.p = GmmParams{a, b, out, offs, G, offs ? GMM_JAG_M : GMM_JAG_NONE, int32_t(M), int32_t(N), int32_t((K + 1) / 2), 1,
+                   0, a_stride / 2, 1, b_stride_g / 2, 1, b_stride_n / 2, 0, out_stride, 1, 0, 0};
+  pr.p.gather = row_index;
+  pr.p.a_rows = int32_t(a_rows);
+  set_workspace(pr, workspace, workspace_bytes);
+  GmmInt8Params p{};
+  static_cast<GmmParams&>(p) = pr.p;
+  p.a_scale = a_scale;
+  p.b_scale = b_scale;
+  p.k_odd = int32_t(K & 1);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (pr.eager_only) {
+    GmmInt8Params full = p;
+    full.ws_parts = 2 * cus;
+    if (gmm_int8_tile_uses_workspace(full, cus) && capture_id(s)) return GMM_ERR_WORKSPACE;
+  }
+  return gmm_launch_int8_tile(p, out_dtype, cus, s) == 0 ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
 int gmm_zero_unowned(void* out, const int32_t* offs, int32_t G, int32_t by_columns, int64_t M, int64_t N, int64_t o_sm, int64_t o_sn,
                      int32_t dtype, void* stream) {
   if (!dims_ok(M, N, G) || G >= GMM_MAX_GROUPS) return GMM_ERR_BAD_ARGUMENT;

@@ -21,6 +21,11 @@ int gmm_launch_staged(GmmParams p, int in_dtype, int out_dtype, int num_cus, hip
 // Would this launch use a workspace of p.ws_parts slots?
 bool gmm_staged_uses_workspace(const GmmParams& p, int in_dtype, int num_cus);
 
+// Product of 8-bit integers on the assembly tile, fp32, bf16 or fp16 out (gmm_int8_tile.hip): jagged rows or none, p.ws and p.ws_parts set.
+int gmm_launch_int8_tile(GmmInt8Params p, int out_dtype, int num_cus, hipStream_t stream);
+// Would that launch use a workspace of p.ws_parts slots?
+bool gmm_int8_tile_uses_workspace(GmmInt8Params p, int num_cus);
+
 // Zeros in the rows (jagged rows) or columns (jagged columns) of the output that no group owns.
 int gmm_launch_zero_unowned(const GmmParams& p, int out_dtype, hipStream_t stream);
 

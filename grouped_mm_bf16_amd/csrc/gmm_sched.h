@@ -71,6 +71,13 @@ struct GmmParams {
   int32_t k_alone;
 };
 
+// 8-bit integers, both operands contiguous along K: K and the strides of a and b count pairs of them.
+struct GmmInt8Params : GmmParams {
+  const float* a_scale;   // of the rows of `a`
+  const float* b_scale;   // [G][N]
+  int32_t k_odd;          // the last pair along K has one element only
+};
+
 constexpr int GMM_WS_HEADER = 4096;          // 1024 int32: arrival counters, one per tile of the split round, ...
 constexpr int GMM_WS_SLOT = 256 * 256 * 4;   // one fp32 partial tile
 constexpr int GMM_SPLIT_MAX = 8;             // most parts a tile is cut into

@@ -21,11 +21,15 @@ struct GmmTileRegs {
   gmm_v4i fix;                 // LDS addresses of this thread's row in the first / last k chunk (A, A, B, B)
   gmm_v8i masks;               // keep-masks of the first and of the last 16-byte k chunk
   gmm_v4i rsrc_a, rsrc_b, rsrc_c;
+  gmm_v2i scale;               // 8-bit integers: byte offset of the row's scale that this thread copies, of the column's
+  gmm_v4i rsrc_rows, rsrc_cols;
   gmm_v8i scal;                // nk, a_step, b_step, lds_base, row_cnt, c_step, (unused), wave | flags << 8
 };
 
 // TM = MFMA block rows per wave: the tile is 64 * TM rows (256, 128 or 64) by 256 columns.
 // F16 = 1: A, B and a 16-bit output are fp16 instead of bf16 (same layouts, other MFMA and conversion).
+// F16 = 2, 3: A and B are 8-bit integers with a scale for each row of A and each column of B, a 16-bit output is bf16 (2) or fp16 (3).
+// Elements of A and B, leading dimensions and K then count pairs of them.
 // B_NT = 1 (128- and 64-row tiles): B is copied with the non-temporal hint, for a tile that is the only
 // reader of its B panel (it then does not push panels that other tiles share out of the L2).
 // ACT = 2: the tile is a partial sum (a part of a tile cut along K): fp32, stored through to memory at
@@ -37,7 +41,11 @@ struct GmmTileRegs {
 template <int A_TR, int B_TR, int OUT_F32, int TM, int F16, int B_NT, int ACT>
 __device__ __forceinline__ void gmm_tile_asm(GmmTileRegs& r);
 
+#ifdef GMM_TILE_INT8
+#include "gmm_tile_asm_int8.inc"
+#else
 #include "gmm_tile_asm.inc"
+#endif
 
 constexpr int GMM_TILE_M = 256, GMM_TILE_N = 256, GMM_TILE_K = 64;
 constexpr unsigned GMM_OOB = 0x80000000u;
@@ -106,6 +114,12 @@ struct GmmTileDesc {
   int col_lo, col_hi;    // columns [col_lo, col_hi) of the tile are stored (relative to n0; with the SwiGLU
                          // epilogue: output columns relative to n0 / 2)
   int share, sharers;    // L2 prefetch of B: this tile touches share number `share` of `sharers` (0: none)
+  // 8-bit integers: scales from the tile's first row on (with a gather list: of all rows), from its first column on, how many there
+  // are; and whether the last pair of klen has one element only.
+  const float* row_scale;
+  const float* col_scale;
+  int row_scales, col_scales;
+  bool k_odd;
 };
 
 // Column of the matrix, from the tile's first gate column, that is column `c` of a SwiGLU tile: turns of 64 gate columns and
@@ -175,6 +189,7 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
   static_assert(TM == 4 || !A_TR, "short tiles exist for a K-contiguous A only");
   static_assert(!(ACT & 1) || (!A_TR && !OUT_F32), "the SwiGLU epilogue: K-contiguous A, 16-bit output");
   static_assert(ACT != 2 || (OUT_F32 && !B_NT), "partial tiles are fp32");
+  static_assert(F16 < 2 || (!A_TR && !B_TR && !(ACT & 1)), "8-bit integers: both operands contiguous along K");
   constexpr int WROWS = 32 * TM;  // rows of the tile per wave row
   constexpr int B_BASE = GmmTileLayout<A_TR, TM>::b_base;
   const int wm = wave & 1, wn = wave >> 1;
@@ -259,7 +274,7 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
   const int a_step = A_TR ? GMM_TILE_K * t.a.ld * 2 : GMM_TILE_K * 2;
   const int b_step = B_TR ? GMM_TILE_K * t.b.ld * 2 : GMM_TILE_K * 2;
   // partial first / last chunk of the k range (jagged contraction with an operand contiguous along K)
-  const int ktail = t.klen & 7;
+  const int ktail = F16 >= 2 && t.k_odd && (t.klen & 7) == 0 ? 8 : t.klen & 7;
   int flags = 0;
   if (!(A_TR && B_TR)) flags = (t.khead ? 1 : 0) | (ktail ? 2 : 0);
   flags |= partial << 2;
@@ -275,10 +290,28 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const unsigned h0 = (2 * w >= t.khead) ? 0x0000ffffu : 0u, h1 = (2 * w + 1 >= t.khead) ? 0xffff0000u : 0u;
-      const unsigned t0 = (2 * w < ktail) ? 0x0000ffffu : 0u, t1 = (2 * w + 1 < ktail) ? 0xffff0000u : 0u;
+      unsigned t0 = (2 * w < ktail) ? 0x0000ffffu : 0u, t1 = (2 * w + 1 < ktail) ? 0xffff0000u : 0u;
+      if (F16 >= 2 && t.k_odd) {
+        if (2 * w == ktail - 1) t0 = 0x000000ffu;
+        if (2 * w + 1 == ktail - 1) t1 = 0x00ff0000u;
+      }
       r.masks[w] = __builtin_amdgcn_readfirstlane((int)(h0 | h1));
       r.masks[4 + w] = __builtin_amdgcn_readfirstlane((int)(t0 | t1));
     }
+  }
+  if constexpr (F16 >= 2 && ACT != 2) {
+    const int at = wave * 64 + lane;
+    int row = at;
+    if (t.a.gather) row = at < t.a.gather_n ? t.a.gather[at] : -1;
+    r.scale[0] = row >= 0 && row < t.row_scales ? row * 4 : (int)GMM_OOB;
+    r.scale[1] = at * 4;
+    r.rsrc_rows = gmm_make_rsrc(t.row_scale, (long long)t.row_scales * 4);
+    r.rsrc_cols = gmm_make_rsrc(t.col_scale, (long long)t.col_scales * 4);
+    r.ra_addr[2] = lds_base + GMM_TILE_SCALES + (wm * WROWS + (lane & 15)) * 4;
+    r.rb_addr[2] = lds_base + GMM_TILE_SCALES + 1024 + (wn * 128 + 4 * (lane >> 4)) * 4;
+  } else if constexpr (F16 >= 2) {
+    r.scale = gmm_v2i{0, 0};
+    r.rsrc_rows = r.rsrc_cols = gmm_v4i{0, 0, 0, 0};
   }
   const int sc[8] = {nk, a_step, b_step, (int)lds_base, t.row_cnt, c_step, n_valid, wave | (flags << 8)};
 #pragma unroll

@@ -1,0 +1,281 @@
+"""Products on 8-bit integers with a scale for each token (row of the first operand) and each channel (column of the second), for serving: a linear
+layer, the grouped product, and the whole mixture-of-experts layer, whose activations are rounded to 8 bits in front of both products.
+
+    y[t, n] = a.scale[t] * b.scale[n] * sum over k of a.values[t, k] * b.values[k, n]
+
+Weights are rounded once (:func:`quantize_columns`), activations in each call (:func:`quantize_rows`).  Sums are exact, scales are applied in
+float32, the result is rounded once.  No count reaches the host.  Registered as torch custom ops (``grouped_mm_bf16_amd::int8_quantize``,
+``int8_gated``, ``int8_mm``), which calls dispatch to while a model around them is being traced or compiled.  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib, derivatives, kernels, moe, moe_train
+from .kernels import _dtype_code, _guard, _require_gpu
+from .moe import ACTIVATIONS
+
+MAX_K = 131071       # sums of products of -128 .. 127 stay below 2^31
+
+
+class Rows(NamedTuple):
+    """A matrix whose rows have a scale each: row t stands for ``scale[t] * values[t]``."""
+    values: torch.Tensor     # int8 [T, K]
+    scale: torch.Tensor      # float32 [T]
+
+
+class Columns(NamedTuple):
+    """A matrix, or one for each group, whose columns have a scale each: column n stands for ``scale[n] * values[:, n]``."""
+    values: torch.Tensor     # int8 [K, N] or [G, K, N], contiguous along K
+    scale: torch.Tensor      # float32 [N] or [G, N]
+
+
+def _pitch(width: int) -> int:
+    """Bytes from one row (or column) to the next: a multiple of 16."""
+    return max(16, (width + 15) // 16 * 16)
+
+
+def _forward_only(what: str, *tensors: torch.Tensor) -> None:
+    if any(t.requires_grad for t in tensors) and torch.is_grad_enabled() or derivatives.forward_mode() and derivatives.tangent(*tensors):
+        raise RuntimeError(f"{what} is forward only: call it under torch.no_grad(), or with detached operands")
+
+
+# ------------------------------------------------------------------ rounding
+def _quantize_now(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """values [rows, pitch], of which a row's first x.size(1) count, and scales."""
+    rows, width = x.shape
+    values = torch.empty(rows, _pitch(width), device=x.device, dtype=torch.int8)
+    scale = torch.empty(rows, device=x.device, dtype=torch.float32)
+    with _guard(x):
+        rc = _lib.load().gmm_int8_quantize(x.data_ptr(), values.data_ptr(), scale.data_ptr(), rows, width, x.stride(0), values.size(1),
+                                           _dtype_code(x.dtype), kernels.current_stream(x.device))
+    _lib.check(rc, "quantize_rows")
+    return values, scale
+
+
+_quantize_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_quantize", mutates_args=())(_quantize_now)
+
+
+@_quantize_op.register_fake
+def _quantize_fake(x):
+    return x.new_empty(x.size(0), _pitch(x.size(1)), dtype=torch.int8), x.new_empty(x.size(0), dtype=torch.float32)
+
+
+def _quantize(x: torch.Tensor) -> Rows:
+    values, scale = (_quantize_op if torch.compiler.is_compiling() else _quantize_now)(moe_train._rows(x))
+    return Rows(values[:, :x.size(1)], scale)
+
+
+def quantize_rows(x: torch.Tensor) -> Rows:
+    """Each row of x rounded to whole steps of a 127th of its largest magnitude (of 2^-100 at least), ties to even.
+
+    x [T, K], bf16, fp16 or fp32, any row stride.  A row with an infinity or NaN has it as its scale, and products with it are NaN.  The values' rows
+    lie at multiples of 16 bytes, as the products want them.
+    """
+    _dtype_code(x.dtype)
+    if x.dim() != 2:
+        raise RuntimeError(f"quantize_rows takes a 2D tensor, got {x.dim()}D")
+    _require_gpu(x)
+    _forward_only("quantize_rows", x)
+    return _quantize(x)
+
+
+def quantize_columns(w: torch.Tensor) -> Columns:
+    """Each column of a weight matrix [K, N], or of one for each group [G, K, N], as :func:`quantize_rows` has rows: bf16, fp16 or fp32, any
+    strides (a linear layer's weight as it is: ``weight.t()``).  Done once, when the weights are loaded."""
+    _dtype_code(w.dtype)
+    if w.dim() not in (2, 3):
+        raise RuntimeError(f"quantize_columns takes a 2D or 3D tensor, got {w.dim()}D")
+    _require_gpu(w)
+    _forward_only("quantize_columns", w)
+    turned = w.transpose(-2, -1)
+    rows = _quantize(turned.reshape(turned.shape[:-1].numel(), w.size(-2)))
+    return Columns(rows.values.unflatten(0, turned.shape[:-1]).transpose(-2, -1), rows.scale.reshape(turned.shape[:-1]))
+
+
+# ------------------------------------------------------------------ products
+def _aligned(values: torch.Tensor) -> torch.Tensor:
+    """Rows [.., R, K] contiguous along K at multiples of 16 bytes; copied only where they do not lie so."""
+    K = values.size(-1)
+    lies = values.data_ptr() % 16 == 0
+    for d in range(values.dim() - 1):
+        lies = lies and (values.size(d) == 1 or values.stride(d) % 16 == 0 and values.stride(d) >= (K if d == values.dim() - 2 else 0))
+    if lies and (values.stride(-1) == 1 or K == 1):
+        return values
+    own = torch.empty(*values.shape[:-1], _pitch(K), device=values.device, dtype=torch.int8)[..., :K]
+    return own.copy_(values)
+
+
+def _mm_now(a: torch.Tensor, a_scale: torch.Tensor, row_index: Optional[torch.Tensor], b: torch.Tensor, b_scale: torch.Tensor,
+            offs: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    """b [G, N, K]; G = 1 without offs."""
+    G, N, K = b.shape
+    M = a.size(0) if row_index is None else row_index.numel()
+    out = torch.empty(M, N, device=a.device, dtype=out_dtype)
+    if out.numel() == 0:
+        return out
+    if K == 0:
+        return out.zero_()
+    a, b = _aligned(a), _aligned(b)
+    lib = _lib.load()
+    pitch = lambda stride, count, width: stride if count > 1 else _pitch(width)
+    with _guard(a):
+        args = (a.data_ptr(), a_scale.data_ptr(), None if row_index is None else row_index.data_ptr(), b.data_ptr(), b_scale.data_ptr(), out.data_ptr(),
+                None if offs is None else offs.data_ptr(), G, a.size(0), M, N, K, pitch(a.stride(0), a.size(0), K),
+                b.stride(0) if G > 1 else 0, pitch(b.stride(1), N, K), N, _dtype_code(out_dtype))
+        rc = kernels.call_with_workspace(lib.gmm_int8_mm, args, a.device, kernels.current_stream(a.device))
+    _lib.check(rc, "int8 product")
+    return out
+
+
+_mm_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_mm", mutates_args=())(_mm_now)
+
+
+@_mm_op.register_fake
+def _mm_fake(a, a_scale, row_index, b, b_scale, offs, out_dtype):
+    return a.new_empty(a.size(0) if row_index is None else row_index.numel(), b.size(1), dtype=out_dtype)
+
+
+def _mm(a: Rows, row_index: Optional[torch.Tensor], b: Columns, offs: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    values = b.values.transpose(-2, -1)
+    return (_mm_op if torch.compiler.is_compiling() else _mm_now)(a.values, a.scale, row_index, values if values.dim() == 3 else values.unsqueeze(0),
+                                                                  b.scale, offs, out_dtype)
+
+
+def _check_columns(what: str, b: Columns, device: torch.device, dims: int) -> None:
+    if b.values.dtype != torch.int8 or b.values.dim() != dims:
+        raise RuntimeError(f"{what}: the columns' values have to be {dims}D int8, got {b.values.dim()}D {b.values.dtype}")
+    shape = b.values.shape[:-2] + b.values.shape[-1:]
+    if b.scale.dtype != torch.float32 or b.scale.shape != shape or not b.scale.is_contiguous():
+        raise RuntimeError(f"{what}: the columns' scale has to be a contiguous float32 tensor {tuple(shape)}, got {tuple(b.scale.shape)} {b.scale.dtype}")
+    if b.values.numel() and b.values.stride(-2) != 1 and b.values.size(-2) > 1:
+        raise RuntimeError(f"{what}: the columns' values have to be contiguous along K, as quantize_columns lays them out; got strides {tuple(b.values.stride())}")
+    if b.values.size(-2) > MAX_K:
+        raise RuntimeError(f"{what}: K is at most {MAX_K}, got {b.values.size(-2)}")
+    if b.values.device != device or b.scale.device != device:
+        raise RuntimeError(f"{what}: all operands have to be on {device}")
+
+
+def _check_rows(what: str, a: Rows, K: int) -> None:
+    if a.values.dtype != torch.int8 or a.values.dim() != 2:
+        raise RuntimeError(f"{what}: the rows' values have to be 2D int8, got {a.values.dim()}D {a.values.dtype}")
+    if a.scale.dtype != torch.float32 or a.scale.shape != a.values.shape[:1] or not a.scale.is_contiguous():
+        raise RuntimeError(f"{what}: the rows' scale has to be a contiguous float32 tensor ({a.values.size(0)},), got {tuple(a.scale.shape)} {a.scale.dtype}")
+    if a.scale.device != a.values.device:
+        raise RuntimeError(f"{what}: all operands have to be on {a.values.device}")
+    if a.values.size(1) != K:
+        raise RuntimeError(f"{what}: contraction dimensions have to match, got {a.values.size(1)} and {K}")
+
+
+def _check_groups(what: str, b: Columns, offs: torch.Tensor) -> None:
+    if offs.dtype != torch.int32 or offs.dim() != 1 or not offs.is_contiguous():
+        raise RuntimeError("Offsets have to be int32")
+    if offs.numel() != b.values.size(0):
+        raise RuntimeError("matrix batch sizes have to match")
+    if offs.numel() >= 1024:
+        raise RuntimeError("Can't process more than 1024 groups")
+    if offs.device != b.values.device:
+        raise RuntimeError(f"{what}: all operands have to be on {b.values.device}")
+
+
+def int8_mm(a: Rows, b: Columns, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(a.scale[:, None] * a.values) @ (b.values * b.scale)`` [T, N] in out_dtype (bf16, fp16 or fp32): a.values [T, K], b.values [K, N].
+
+    Values may be any of -128 .. 127, K is at most 131071.  Operands whose rows and columns lie at multiples of 16 bytes are taken as they are, others
+    copied first.
+    """
+    _dtype_code(out_dtype)
+    _check_columns("int8_mm", b, a.values.device, 2)
+    _check_rows("int8_mm", a, b.values.size(0))
+    _require_gpu(a.values)
+    return _mm(a, None, b, None, out_dtype)
+
+
+def grouped_int8_mm(a: Rows, b: Columns, offs: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
+                    row_index: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`int8_mm` of jagged rows: rows offs[g - 1] .. offs[g] - 1 of the result are those of a times b's matrix g.
+
+    a.values [M, K], b.values [G, K, N], offs int32 [G].  With row_index (int32 [M]) row m is row row_index[m] of a; a number outside a reads a row of
+    zeros.  Rows past the last offset are left uninitialised, as ``grouped_mm`` leaves them.
+    """
+    _dtype_code(out_dtype)
+    _check_columns("grouped_int8_mm", b, a.values.device, 3)
+    _check_rows("grouped_int8_mm", a, b.values.size(1))
+    _check_groups("grouped_int8_mm", b, offs)
+    if row_index is not None and (row_index.dtype != torch.int32 or row_index.dim() != 1 or not row_index.is_contiguous()):
+        raise RuntimeError("row_index has to be a contiguous 1D int32 tensor")
+    if row_index is not None and row_index.device != a.values.device:
+        raise RuntimeError(f"grouped_int8_mm: all operands have to be on {a.values.device}")
+    _require_gpu(a.values)
+    return _mm(a, row_index, b, offs, out_dtype)
+
+
+def linear_int8(x: torch.Tensor, weight: Columns) -> torch.Tensor:
+    """``int8_mm(quantize_rows(x), weight)`` in x's type: x [T, K], bf16, fp16 or fp32; weight of :func:`quantize_columns`, [K, N].  Forward only."""
+    _dtype_code(x.dtype)
+    if x.dim() != 2:
+        raise RuntimeError(f"linear_int8 takes a 2D tensor, got {x.dim()}D")
+    _check_columns("linear_int8", weight, x.device, 2)
+    if x.size(1) != weight.values.size(0):
+        raise RuntimeError(f"linear_int8: contraction dimensions have to match, got {x.size(1)} and {weight.values.size(0)}")
+    _require_gpu(x)
+    _forward_only("linear_int8", x)
+    return _mm(_quantize(x), None, weight, None, x.dtype)
+
+
+# ------------------------------------------------------------------ the expert layer
+def _gated_now(h: torch.Tensor, kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    rows, inner = h.size(0), h.size(1) // (1 + kind)
+    values = torch.empty(rows, _pitch(inner), device=h.device, dtype=torch.int8)
+    scale = torch.empty(rows, device=h.device, dtype=torch.float32)
+    with _guard(h):
+        rc = _lib.load().gmm_int8_gated(h.data_ptr(), values.data_ptr(), scale.data_ptr(), rows, inner, h.stride(0), values.size(1), kind,
+                                        kernels.current_stream(h.device))
+    _lib.check(rc, "int8 activation")
+    return values, scale
+
+
+_gated_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_gated", mutates_args=())(_gated_now)
+
+
+@_gated_op.register_fake
+def _gated_fake(h, kind):
+    return h.new_empty(h.size(0), _pitch(h.size(1) // (1 + kind)), dtype=torch.int8), h.new_empty(h.size(0))
+
+
+def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_up: Columns, w_down: Columns, top_k: int, activation: str = "swiglu",
+                     renormalize: bool = True) -> torch.Tensor:
+    """:func:`moe.moe_forward` on 8-bit weights, for any number of tokens: x and the activations are rounded as :func:`quantize_rows` does, in front of
+    either product.
+
+    x [T, H], bf16 or fp16; router_logits [T, E]; w_up of :func:`quantize_columns`, [E, H, I] ("silu") or [E, H, 2 I] ("swiglu": gate columns first);
+    w_down [E, I, H].  The activation takes the first product in float32; the experts' rows are rounded to x's type, their weighted sum again.
+    Forward only.
+    """
+    if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
+        raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")
+    if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
+        raise RuntimeError(f"moe_forward_int8: x has to be bfloat16 or float16, got {x.dtype}")
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"unknown activation {activation!r}; have {sorted(ACTIVATIONS)}")
+    kind = ACTIVATIONS[activation]
+    _check_columns("moe_forward_int8", w_up, x.device, 3)
+    _check_columns("moe_forward_int8", w_down, x.device, 3)
+    E = router_logits.size(1)
+    if w_up.values.size(0) != E or w_down.values.size(0) != E:
+        raise RuntimeError("w_up [E, H, I or 2I] and w_down [E, I, H] must agree with router_logits on E")
+    if w_up.values.shape[1:] != (x.size(1), w_down.values.size(1) * (1 + kind)) or w_down.values.size(2) != x.size(1):
+        raise RuntimeError("weight shapes do not chain: x [T, H], w_up [E, H, I or 2I], w_down [E, I, H]")
+    _require_gpu(x, router_logits)
+    if router_logits.device != x.device:
+        raise RuntimeError(f"moe_forward_int8: all operands have to be on {x.device}")
+    _forward_only("moe_forward_int8", x, router_logits)
+    compiling = torch.compiler.is_compiling()
+    routing = moe.moe_route(router_logits, top_k, renormalize)
+    h = _mm(_quantize(x), routing.row_token, w_up, routing.offs, torch.float32)
+    values, scale = (_gated_op if compiling else _gated_now)(h, kind)
+    del h
+    y = _mm(Rows(values[:, :w_down.values.size(1)], scale), None, w_down, routing.offs, x.dtype)
+    return (moe_train._sum_op if compiling else moe_train._sum_now)(y, routing.token_rows, routing.slot_weight, x.size(0), top_k)

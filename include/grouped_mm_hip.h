@@ -317,6 +317,26 @@ int gmm_layer_norm_backward(const void* dy, const void* x, const void* weight, c
                             int64_t dy_stride, int64_t x_stride, int64_t dx_stride,
                             int32_t dtype, int32_t weight_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Products of 8-bit integers with a scale for each row of the first operand and each column of the second.  No counterpart in the reference.
+ *   gmm_int8_quantize  rows of x [rows, width] (dtype, row stride in elements):  scale[r] = max(max |x[r]|, 2^-100) / 127,  values[r] = x[r] / scale[r]
+ *                      rounded to whole numbers (ties to even).  values_stride in bytes, a multiple of 16, values 16-byte aligned; bytes from `width`
+ *                      up to the next multiple of 16 of a row become zeros.  A row with an infinity or NaN has it as its scale, and zeros.
+ *   gmm_int8_gated     the same of silu(h[r, c]) or silu(h[r, c]) * h[r, inner + c] (kind GMM_ACT_SILU, GMM_ACT_SWIGLU), h float [rows, ..]
+ *   gmm_int8_mm        out[m, n] = a_scale[m'] * b_scale[g, n] * sum over k of a[m', k] * b[g, k, n]
+ *                      for rows m of group g (offs as in gmm_2d3d; NULL: one group that has all M rows), m' = m or row_index[m] (row_index NULL: m;
+ *                      outside [0, a_rows): a row of zeros).  a [a_rows, K] row-major, b [G, K, N] contiguous along K: a_stride, b_stride_g and
+ *                      b_stride_n in bytes, multiples of 16, a and b 16-byte aligned; K < 131072 (sums are 32-bit integers, exact);
+ *                      b_scale [G, N] contiguous; out [M, N] row-major, out_dtype any gmm_dtype, out_stride in elements; scaled in fp32, by the
+ *                      column's scale and then by the row's, rounded once.  Bytes behind a row's or a column's end, up to the next multiple of 16, may be read and do not count.  With row_index,
+ *                      a below 2 GiB.  workspace as for gmm_2d3d: results do not depend on it. */
+int gmm_int8_quantize(const void* x, int8_t* values, float* scale, int64_t rows, int64_t width, int64_t x_stride, int64_t values_stride,
+                      int32_t dtype, void* stream);
+int gmm_int8_gated(const float* h, int8_t* values, float* scale, int64_t rows, int64_t inner, int64_t h_stride, int64_t values_stride,
+                   int32_t kind, void* stream);
+int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, void* out,
+                const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
+                int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- What stands around the grouped products of an expert layer that is trained.  No counterpart in the reference.
  * Slot t * top_k + j is choice j of token t, token_rows (as gmm_moe_route writes it) its row among those sorted by expert; a slot whose row is
  * outside [0, rows) takes no part.  bf16, fp16 or fp32 (dtype), any width, any alignment, row strides in elements (at least the width where
