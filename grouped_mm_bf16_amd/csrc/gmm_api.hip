@@ -399,10 +399,16 @@ int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index,
   p.b_scale = b_scale;
   p.k_odd = int32_t(K & 1);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool few = gmm_int8_few_preferred(p, cus);
   if (pr.eager_only) {
     GmmInt8Params full = p;
     full.ws_parts = 2 * cus;
-    if (gmm_int8_tile_uses_workspace(full, cus) && capture_id(s)) return GMM_ERR_WORKSPACE;
+    const bool uses = few ? gmm_int8_few_bytes(p, cus) > 0 : gmm_int8_tile_uses_workspace(full, cus);
+    if (uses && capture_id(s)) return GMM_ERR_WORKSPACE;
+  }
+  if (few) {
+    char* const planes = p.ws ? static_cast<char*>(p.ws) + GMM_WS_HEADER : nullptr;
+    return gmm_launch_int8_few(p, planes, int64_t(p.ws_parts) * GMM_WS_SLOT, out_dtype, cus, s);
   }
   return gmm_launch_int8_tile(p, out_dtype, cus, s) == 0 ? GMM_OK : GMM_ERR_LAUNCH;
 }

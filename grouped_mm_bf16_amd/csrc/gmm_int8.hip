@@ -10,6 +10,7 @@
 
 #include "../../include/grouped_mm_hip.h"
 #include "gmm_elem.h"
+#include "gmm_launch.h"
 
 namespace {
 
@@ -25,13 +26,16 @@ struct QuantArgs {
   float* scale;
   int64_t rows, x_stride, values_stride;
   int32_t width;
+  int32_t parts;          // of the activation's operand, each `plane` elements behind the one before: it is their sum
+  int64_t plane;
 };
 
 // 16 elements from column c on; zeros past the row's end.
 template <typename T>
 struct Plain {
   typedef T Elem;
-  static __device__ __forceinline__ void load(const T* row, int c, int width, float (&v)[kSpan]) {
+  static __device__ __forceinline__ void load(const QuantArgs& a, const T* row, int c, float (&v)[kSpan]) { get(row, c, a.width, v); }
+  static __device__ __forceinline__ void get(const T* row, int c, int width, float (&v)[kSpan]) {
     constexpr int N = kVector<T>;
     if (c + kSpan <= width) {
 #pragma unroll
@@ -51,10 +55,21 @@ struct Plain {
 template <bool SWIGLU>
 struct Gated {
   typedef float Elem;
-  static __device__ __forceinline__ void load(const float* row, int c, int width, float (&v)[kSpan]) {
+  static __device__ __forceinline__ void load(const QuantArgs& a, const float* row, int c, float (&v)[kSpan]) {
     float u[kSpan];
-    Plain<float>::load(row, c, width, v);
-    if constexpr (SWIGLU) Plain<float>::load(row + width, c, width, u);
+    Plain<float>::get(row, c, a.width, v);
+    if constexpr (SWIGLU) Plain<float>::get(row + a.width, c, a.width, u);
+    for (int p = 1; p < a.parts; ++p) {
+      float more[kSpan];
+      Plain<float>::get(row + p * a.plane, c, a.width, more);
+#pragma unroll
+      for (int i = 0; i < kSpan; ++i) v[i] += more[i];
+      if constexpr (SWIGLU) {
+        Plain<float>::get(row + p * a.plane + a.width, c, a.width, more);
+#pragma unroll
+        for (int i = 0; i < kSpan; ++i) u[i] += more[i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kSpan; ++i) {
       v[i] = v[i] / (1.0f + __expf(-v[i]));
@@ -81,7 +96,7 @@ __global__ void __launch_bounds__(kGroup) quantize_kernel(const QuantArgs a) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int c = (p * LANES + lane) * kSpan;
-      if (live && c < a.width) S::load(x, c, a.width, v[p]);
+      if (live && c < a.width) S::load(a, x, c, v[p]);
       else
 #pragma unroll
         for (int i = 0; i < kSpan; ++i) v[p][i] = 0;
@@ -92,7 +107,7 @@ __global__ void __launch_bounds__(kGroup) quantize_kernel(const QuantArgs a) {
       for (int i = 0; i < kSpan; ++i) most = max(most, magnitude(v[p][i]));
   } else {
     for (int c = lane * kSpan; live && c < a.width; c += LANES * kSpan) {
-      S::load(x, c, a.width, v[0]);
+      S::load(a, x, c, v[0]);
 #pragma unroll
       for (int i = 0; i < kSpan; ++i) most = max(most, magnitude(v[0][i]));
     }
@@ -136,7 +151,7 @@ __global__ void __launch_bounds__(kGroup) quantize_kernel(const QuantArgs a) {
     }
   } else {
     for (int c = lane * kSpan; c < a.width; c += LANES * kSpan) {
-      S::load(x, c, a.width, v[0]);
+      S::load(a, x, c, v[0]);
       store(c, v[0]);
     }
   }
@@ -171,6 +186,15 @@ int check(const void* x, int8_t* values, float* scale, int64_t rows, int64_t wid
 
 }  // namespace
 
+int gmm_int8_gated_parts(const float* h, int parts, int64_t plane, int8_t* values, float* scale, int64_t rows, int64_t inner, int64_t h_stride,
+                         int64_t values_stride, int32_t kind, hipStream_t stream) {
+  if (kind < GMM_ACT_SILU || kind > GMM_ACT_SWIGLU) return GMM_ERR_BAD_ARGUMENT;
+  const int bad = check(h, values, scale, rows, inner, (kind == GMM_ACT_SWIGLU ? 2 : 1) * inner, h_stride, values_stride);
+  if (bad || rows == 0) return bad;
+  const QuantArgs a{h, values, scale, rows, h_stride, values_stride, int32_t(inner), parts, plane};
+  return kind == GMM_ACT_SWIGLU ? launch<Gated<true>>(a, stream) : launch<Gated<false>>(a, stream);
+}
+
 extern "C" {
 
 int gmm_int8_quantize(const void* x, int8_t* values, float* scale, int64_t rows, int64_t width, int64_t x_stride, int64_t values_stride,
@@ -178,7 +202,7 @@ int gmm_int8_quantize(const void* x, int8_t* values, float* scale, int64_t rows,
   if (dtype < GMM_DT_BF16 || dtype > GMM_DT_F32) return GMM_ERR_UNSUPPORTED;
   const int bad = check(x, values, scale, rows, width, width, x_stride, values_stride);
   if (bad || rows == 0) return bad;
-  const QuantArgs a{x, values, scale, rows, x_stride, values_stride, int32_t(width)};
+  const QuantArgs a{x, values, scale, rows, x_stride, values_stride, int32_t(width), 1, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GMM_DT_BF16) return launch<Plain<Bf16>>(a, s);
   if (dtype == GMM_DT_F16) return launch<Plain<F16>>(a, s);
@@ -187,12 +211,7 @@ int gmm_int8_quantize(const void* x, int8_t* values, float* scale, int64_t rows,
 
 int gmm_int8_gated(const float* h, int8_t* values, float* scale, int64_t rows, int64_t inner, int64_t h_stride, int64_t values_stride,
                    int32_t kind, void* stream) {
-  if (kind < GMM_ACT_SILU || kind > GMM_ACT_SWIGLU) return GMM_ERR_BAD_ARGUMENT;
-  const int bad = check(h, values, scale, rows, inner, (kind == GMM_ACT_SWIGLU ? 2 : 1) * inner, h_stride, values_stride);
-  if (bad || rows == 0) return bad;
-  const QuantArgs a{h, values, scale, rows, h_stride, values_stride, int32_t(inner)};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  return kind == GMM_ACT_SWIGLU ? launch<Gated<true>>(a, s) : launch<Gated<false>>(a, s);
+  return gmm_int8_gated_parts(h, 1, 0, values, scale, rows, inner, h_stride, values_stride, kind, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

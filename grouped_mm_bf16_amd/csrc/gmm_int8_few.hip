@@ -1,0 +1,417 @@
+// Products of 8-bit integers for a few rows, a linear layer for a few tokens and the expert layer for them (gmm_int8_linear, gmm_int8_moe_few in
+// include/grouped_mm_hip.h).  Reading the weights bounds them: they are streamed past the rows as the 16-bit ones are (gmm_skinny.h), 64 columns
+// to a workgroup, whose waves share k; where that leaves compute units idle, k is cut into parts as well.
+//   one matrix        parts are planes of integer sums, which a second kernel adds up and scales: exact, as in one part
+//   expert layer      route, rows of x to 8 bits, first product, activation to 8 bits, second product, sum over choices and parts.  The planes
+//                     between its launches are scaled fp32 values; SwiGLU is computed by the first product where k is in one part
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/grouped_mm_hip.h"
+#include "gmm_device.h"
+#include "gmm_launch.h"
+#include "gmm_skinny.h"
+
+namespace {
+
+using namespace gmm;
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kColumns = 64;
+constexpr int kMaxTokens = 64;
+
+enum Result : int { kOut, kSums, kScaled, kActivated };
+
+struct FewArgs {
+  const void* a;
+  const void* b;
+  const float* a_scale;
+  const float* b_scale;
+  const int32_t* offs;        // null: one group
+  const int32_t* row_index;   // null: rows as they are
+  void* out;                  // kOut: [M][out_ld] of out_dtype; kSums: int32 [parts][M][N]; kScaled: float [parts][M][N]; kActivated: float [M][N / 2]
+  int64_t a_ld, b_sg, b_ld, out_ld;      // pairs of integers (out_ld: elements)
+  uint32_t a_bytes, b_bytes;
+  int32_t G, M, N, K, a_rows; // K: pairs
+  int32_t used, most;         // groups that can have rows; rows that a group can have, 64 at most
+  int32_t tiles, parts, k_part;
+  int32_t result, out_dtype;
+};
+
+// The `which`-th group that has rows, found by every wave for itself.
+__device__ __forceinline__ bool find_group(const FewArgs& a, int which, int& g, int& row0, int& rows) {
+  constexpr int AT_ONCE = 4;
+  const int lane = threadIdx.x & 63;
+  int used = 0, start = 0;
+  for (int base = 0; base < a.G; base += 64 * AT_ONCE) {
+    int ends[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) ends[i] = a.offs[min(base + 64 * i + lane, a.G - 1)];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const bool there = base + 64 * i + lane < a.G;
+      const int to = min(max(ends[i], 0), a.M), before = __shfl_up(to, 1), from = lane ? before : start;
+      start = __builtin_amdgcn_readlane(to, 63);
+      const uint64_t with = __ballot(there && to > from);
+      const int n = __popcll(with);
+      if (which < used + n) {
+        const uint64_t it = __ballot(there && to > from && __popcll(with & ((uint64_t(1) << lane) - 1)) == which - used);
+        const int at = __ffsll(static_cast<unsigned long long>(it)) - 1;
+        g = base + 64 * i + at;
+        row0 = __builtin_amdgcn_readlane(from, at);
+        rows = __builtin_amdgcn_readlane(to, at) - row0;
+        return true;
+      }
+      used += n;
+    }
+  }
+  return false;
+}
+
+__device__ __forceinline__ void put(void* out, int dtype, int64_t at, float v) {
+  if (dtype == GMM_DT_BF16) static_cast<Bf16*>(out)[at] = rounded<Bf16>(v);
+  else if (dtype == GMM_DT_F16) static_cast<F16*>(out)[at] = rounded<F16>(v);
+  else static_cast<float*>(out)[at] = v;
+}
+
+// A sum in fp32, by its column's scale, then by its row's: no product fused with the rounding to 16 bits that follows.
+__device__ __forceinline__ float scaled(int sum, float column, float row) {
+  float v = float(sum) * column * row;
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// GLU: a strip is 32 gate columns and their 32 partners, N / 2 further on; the result is silu(gate) * partner.
+template <int MF, bool GLU>
+__global__ void __launch_bounds__(kThreads, MF == 4 ? 1 : 2) int8_few_kernel(const FewArgs a) {
+  using S = Strip<I8x2, GMM_W_COLS, MF, 1>;
+  constexpr int FR = S::FR, OUT = GLU ? kColumns / 2 : kColumns;
+  static_assert(16 * FR == kColumns, "");
+  __shared__ SkinnyShared<S, kWaves> shared;
+  const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
+  int g = 0, row0 = 0, rows = a.M;
+  if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int width = GLU ? a.N / 2 : a.N, first = tile * OUT;
+  S s;
+  s.lane = lane;
+  s.lds = shared.wave[wave];
+  s.w_buf = buffer(static_cast<const uint16_t*>(a.b) + g * a.b_sg, a.b_bytes);
+  s.a_buf = buffer(a.a, a.a_bytes);
+  s.a_plane = 0;
+  if constexpr (GLU) s.set_columns(first, width - first, 1, uint32_t(a.b_ld), OUT, width + first);
+  else s.set_columns(first, width - first, 1, uint32_t(a.b_ld));
+  const float* const columns = a.b_scale + int64_t(g) * a.N;
+  const auto source = [&](int r) {      // row of a, or -1
+    const int at = a.row_index ? a.row_index[row0 + r] : row0 + r;
+    return uint32_t(at) < uint32_t(a.a_rows) ? at : -1;
+  };
+  s.set_rows([&](int r) {
+    const int at = r < rows ? source(r) : -1;
+    return at < 0 ? kNowhere : uint32_t(at) * uint32_t(a.a_ld) * 2;
+  });
+  f32x4 acc[MF][FR];
+  clear(acc);
+  s.template run<kWaves>(rows, part * a.k_part, min(a.K, (part + 1) * a.k_part), wave, acc);
+#pragma unroll
+  for (int m = 0; m < MF; ++m) {
+    if (16 * m >= rows) break;
+    __syncthreads();
+    shared.sums.put(wave, lane, acc[m]);
+    __syncthreads();
+    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+      const int oc = u % OUT, og = u / OUT, col = first + oc;
+      if (col >= width) continue;
+      const auto sums = [&](int c) { return shared.sums.whole(S::product_of(c), S::lane_of(c), og); };
+      const i32x4 h = sums(oc), partner = GLU ? sums(OUT + oc) : i32x4{0, 0, 0, 0};
+      const float cs = columns[col], ps = GLU ? columns[width + col] : 0.0f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int r = 16 * m + 4 * og + v;
+        if (r >= rows) break;
+        const int64_t row = row0 + r;
+        if (a.result == kSums) {
+          static_cast<int32_t*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = h[v];
+          continue;
+        }
+        const int from = source(r);
+        const float rs = from < 0 ? 0.0f : a.a_scale[from];
+        const float f = scaled(h[v], cs, rs);
+        if constexpr (GLU) {
+          static_cast<float*>(a.out)[row * width + col] = f / (1.0f + __expf(-f)) * scaled(partner[v], ps, rs);
+        } else if (a.result == kScaled) {
+          static_cast<float*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = f;
+        } else {
+          put(a.out, a.out_dtype, row * a.out_ld + col, f);
+        }
+      }
+    }
+  }
+}
+
+// Planes of integer sums added up and scaled.
+__global__ void __launch_bounds__(kThreads) int8_finish_kernel(const FewArgs a, const int32_t* __restrict__ planes) {
+  const int col = blockIdx.x * kThreads + threadIdx.x, row = blockIdx.y;
+  if (col >= a.N) return;
+  const int32_t* at = planes + int64_t(row) * a.N + col;
+  int sum = 0;
+  in_fours(a.parts, [&](int p, bool in) {
+    const int v = at[int64_t(p) * a.M * a.N];
+    sum += in ? v : 0;
+  });
+  put(a.out, a.out_dtype, row * a.out_ld + col, scaled(sum, a.b_scale[col], a.a_scale[row]));
+}
+
+// out[t] = sum over j of weight * sum over the parts of y, in that order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) int8_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ token_rows,
+                                                                const float* __restrict__ slot_weight, T* __restrict__ out, int top_k, int parts,
+                                                                int slots, int H, int64_t out_ld) {
+  const int t = blockIdx.y, c = blockIdx.x * kThreads + threadIdx.x, lane = threadIdx.x & 63;
+  const int mine = t * top_k + min(lane, top_k - 1);
+  const int row = token_rows[mine], weight = __builtin_bit_cast(int, slot_weight[mine]);      // of choice j: in lane j
+  const float* const from = y + min(c, H - 1);
+  float sum = 0, v = 0;
+  int j = 0, part = 0;
+  in_fours(top_k * parts, [&](int, bool in) {
+    const float one = from[(int64_t(part) * slots + __builtin_amdgcn_readlane(row, j)) * H];
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(weight, j));
+    v = in ? (part ? v : 0.0f) + one : v;
+    const bool last = part == parts - 1;
+    if (in && last) sum += w * v;
+    part = last ? 0 : part + 1;
+    j = min(j + last, top_k - 1);
+  });
+  if (c < H) out[t * out_ld + c] = rounded<T>(sum);
+}
+
+// ---------------------------------------------------------------- host side
+// Parts of k (in pairs of integers), each a multiple of a step and at least as long as the waves' steps together, so that there are about three
+// workgroups to a compute unit.
+void cut(int64_t K, int64_t strips, int64_t cus, int32_t& parts, int32_t& each) {
+  constexpr int64_t step = 64, least = step * kWaves;
+  int64_t want = strips > 0 ? 3 * cus / strips : 1;
+  if (want > K / least) want = K / least;
+  if (want > 16) want = 16;
+  if (want < 1) want = 1;
+  each = int32_t(round_up((K + want - 1) / want, step));
+  parts = each ? int32_t((K + each - 1) / each) : 1;
+}
+
+FewArgs from_params(const GmmInt8Params& p) {
+  FewArgs a{};
+  a.a = p.a; a.b = p.b; a.a_scale = p.a_scale; a.b_scale = p.b_scale; a.offs = p.jag == GMM_JAG_M ? p.offs : nullptr; a.row_index = p.gather;
+  a.out = p.c; a.a_ld = p.a_sm; a.b_sg = p.b_sg; a.b_ld = p.b_sn; a.out_ld = p.c_sm;
+  a.G = p.G; a.M = p.M; a.N = p.N; a.K = p.K; a.a_rows = p.gather ? p.a_rows : p.M;
+  a.used = a.offs ? gmm_min(p.G, p.M) : 1;
+  a.most = p.M;
+  a.tiles = gmm_cdiv(p.N, kColumns);
+  a.parts = 1;
+  a.k_part = int32_t(round_up(p.K, 64));
+  return a;
+}
+
+bool sizes_fit(FewArgs& a) {
+  if (a.a_rows > 0 && int64_t(a.a_rows) * a.a_ld >= (int64_t(1) << 30)) return false;
+  a.a_bytes = uint32_t((int64_t(a.a_rows - 1) * a.a_ld + a.K) * 2);
+  a.b_bytes = matrix_bytes(a.K, a.N, 1, a.b_ld);
+  return a.K >= 8 && a.b_bytes != 0;
+}
+
+template <bool GLU>
+int launch(const FewArgs& a, hipStream_t stream) {
+  const dim3 grid(unsigned(int64_t(a.used) * a.tiles * a.parts)), block(kThreads);
+  if (a.most <= 16) hipLaunchKernelGGL((int8_few_kernel<1, GLU>), grid, block, 0, stream, a);
+  else if (a.most <= 32) hipLaunchKernelGGL((int8_few_kernel<2, GLU>), grid, block, 0, stream, a);
+  else if (a.most <= 48) hipLaunchKernelGGL((int8_few_kernel<3, GLU>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((int8_few_kernel<4, GLU>), grid, block, 0, stream, a);
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+bool gmm_int8_few_preferred(const GmmInt8Params& p, int) {
+  FewArgs a = from_params(p);
+  if (p.k_odd || !sizes_fit(a) || int64_t(a.used) * a.tiles >= (int64_t(1) << 27)) return false;
+  return p.M <= kMaxTokens;
+}
+
+int64_t gmm_int8_few_bytes(const GmmInt8Params& p, int num_cus) {
+  FewArgs a = from_params(p);
+  if (a.offs) return 0;
+  cut(a.K, a.tiles, num_cus, a.parts, a.k_part);
+  return a.parts > 1 ? int64_t(a.parts) * a.M * a.N * 4 : 0;
+}
+
+int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_bytes, int out_dtype, int num_cus, hipStream_t stream) {
+  FewArgs a = from_params(p);
+  if (!sizes_fit(a)) return GMM_ERR_UNSUPPORTED;
+  a.out_dtype = out_dtype;
+  a.result = kOut;
+  if (!a.offs && planes && planes_bytes >= gmm_int8_few_bytes(p, num_cus)) cut(a.K, a.tiles, num_cus, a.parts, a.k_part);
+  if (a.parts == 1) return launch<false>(a, stream);
+  FewArgs u = a;
+  u.out = planes;
+  u.result = kSums;
+  const int rc = launch<false>(u, stream);
+  if (rc != GMM_OK) return rc;
+  hipLaunchKernelGGL(int8_finish_kernel, dim3(unsigned(gmm_cdiv(a.N, kThreads)), unsigned(a.M)), dim3(kThreads), 0, stream, a,
+                     static_cast<const int32_t*>(planes));
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+namespace {
+
+// ---------------------------------------------------------------- linear layer
+struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; };
+
+bool plan_linear(int64_t T, int64_t K, int64_t N, LinearPlan& p) {
+  if (T < 0 || T > kMaxTokens || K < 0 || K >= 131072 || N < 0 || N >= (int64_t(1) << 31)) return false;
+  int32_t parts, each;
+  cut((K + 1) / 2, (N + kColumns - 1) / kColumns, gmm_num_cus() > 0 ? gmm_num_cus() : 256, parts, each);
+  p.pitch = round_up(K > 0 ? K : 1, 16);
+  p.scale_at = T * p.pitch;
+  p.planes_at = round_up(p.scale_at + 4 * T, 16);
+  p.bytes = p.planes_at + (parts > 1 ? parts * T * N * 4 : 0);
+  return true;
+}
+
+// ---------------------------------------------------------------- expert layer
+struct LayerPlan {
+  int64_t slots, used, x_pitch, act_pitch, table_bytes;
+  int64_t table_at, x_at, x_scale_at, h_at, act_at, act_scale_at, y_at, bytes;
+  int32_t up_parts, up_k, down_parts, down_k;
+  bool activated;      // by the first product
+};
+
+bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t kind, LayerPlan& p) {
+  if (T < 0 || T > kMaxTokens || E < 1 || H < 1 || I < 1 || H >= 131072 || I >= 131072 || k < 1) return false;
+  p.table_bytes = gmm_moe_route_workspace_bytes(T, E, k);
+  if (p.table_bytes < 0 || k > 32 || k > E) return false;
+  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256, N = kind == GMM_ACT_SWIGLU ? 2 * I : I;
+  p.slots = T * k;
+  p.used = p.slots < E ? p.slots : E;
+  cut(H / 2, p.used * ((N + kColumns - 1) / kColumns), cus, p.up_parts, p.up_k);
+  cut(I / 2, p.used * ((H + kColumns - 1) / kColumns), cus, p.down_parts, p.down_k);
+  p.activated = p.up_parts == 1 && kind == GMM_ACT_SWIGLU;
+  p.x_pitch = round_up(H, 16);
+  p.act_pitch = round_up(I, 16);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) { const int64_t from = at; at = round_up(at + bytes, 256); return from; };
+  take((E + 4 * p.slots) * 4);
+  p.table_at = take(p.table_bytes);
+  p.x_at = take(T * p.x_pitch);
+  p.x_scale_at = take(4 * T);
+  p.h_at = take((p.activated ? I : p.up_parts * N) * p.slots * 4);
+  p.act_at = take(p.slots * p.act_pitch);
+  p.act_scale_at = take(4 * p.slots);
+  p.y_at = take(p.down_parts * p.slots * H * 4);
+  p.bytes = at;
+  return true;
+}
+
+bool lies(const void* p, int64_t stride, int64_t width, int64_t count) {
+  return aligned16(p) && (stride & 15) == 0 && stride >= 0 && (stride >= width || count <= 1) && stride < (int64_t(1) << 23);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gmm_int8_linear_workspace_bytes(int64_t rows, int64_t K, int64_t N) {
+  LinearPlan p;
+  return plan_linear(rows, K, N, p) ? p.bytes : -1;
+}
+
+int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* out, int64_t rows, int64_t K, int64_t N, int64_t x_stride,
+                    int64_t b_stride_n, int64_t out_stride, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  LinearPlan plan;
+  if (rows < 0 || K < 0 || N < 0) return GMM_ERR_BAD_ARGUMENT;
+  if (dtype < GMM_DT_BF16 || dtype > GMM_DT_F32 || !plan_linear(rows, K, N, plan) || (K & 1) || K < 16) return GMM_ERR_UNSUPPORTED;
+  if (rows == 0 || N == 0) return GMM_OK;
+  if (!x || !b || !b_scale || !out || (rows > 1 && (x_stride < K || out_stride < N)) || !lies(b, b_stride_n, K, N)) return GMM_ERR_BAD_ARGUMENT;
+  if (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)) return GMM_ERR_WORKSPACE;
+  const int cus = gmm_num_cus();
+  if (cus <= 0) return GMM_ERR_LAUNCH;
+  char* const ws = static_cast<char*>(workspace);
+  GmmInt8Params p{};
+  p.a = ws; p.b = b; p.c = out; p.G = 1; p.jag = GMM_JAG_NONE; p.M = int32_t(rows); p.N = int32_t(N); p.K = int32_t(K / 2);
+  p.a_sm = plan.pitch / 2; p.a_sk = 1; p.b_sk = 1; p.b_sn = b_stride_n / 2; p.c_sm = out_stride; p.c_sn = 1; p.a_rows = int32_t(rows);
+  p.a_scale = reinterpret_cast<float*>(ws + plan.scale_at);
+  p.b_scale = b_scale;
+  if (!gmm_int8_few_preferred(p, cus)) return GMM_ERR_UNSUPPORTED;
+  const int rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws), reinterpret_cast<float*>(ws + plan.scale_at), rows, K, x_stride, plan.pitch,
+                                   dtype, stream);
+  return rc == GMM_OK ? gmm_launch_int8_few(p, ws + plan.planes_at, plan.bytes - plan.planes_at, dtype, cus, static_cast<hipStream_t>(stream)) : rc;
+}
+
+int64_t gmm_int8_moe_few_workspace_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner, int32_t kind) {
+  LayerPlan p;
+  return plan_layer(tokens, experts, top_k, hidden, inner, kind, p) ? p.bytes : -1;
+}
+
+int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, const float* up_scale, const int8_t* w_down, const float* down_scale,
+                     void* out, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner, int64_t x_stride, int64_t logits_stride,
+                     int64_t up_stride_g, int64_t up_stride_n, int64_t down_stride_g, int64_t down_stride_n, int64_t out_stride, int32_t kind,
+                     int32_t renormalize, int32_t dtype, int32_t logits_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  LayerPlan p;
+  if (kind < GMM_ACT_SILU || kind > GMM_ACT_SWIGLU || tokens < 0 || experts < 1 || top_k < 1 || top_k > experts) return GMM_ERR_BAD_ARGUMENT;
+  if ((dtype != GMM_DT_BF16 && dtype != GMM_DT_F16) || logits_dtype < GMM_DT_BF16 || logits_dtype > GMM_DT_F32) return GMM_ERR_UNSUPPORTED;
+  if (!plan_layer(tokens, experts, top_k, hidden, inner, kind, p) || (hidden & 1) || (inner & 1) || hidden < 16 || inner < 16) return GMM_ERR_UNSUPPORTED;
+  if (tokens == 0) return GMM_OK;
+  const int64_t N = kind == GMM_ACT_SWIGLU ? 2 * inner : inner;
+  if (!x || !logits || !w_up || !up_scale || !w_down || !down_scale || !out) return GMM_ERR_BAD_ARGUMENT;
+  if (tokens > 1 && (x_stride < hidden || out_stride < hidden || logits_stride < experts)) return GMM_ERR_BAD_ARGUMENT;
+  if (!lies(w_up, up_stride_n, hidden, N) || !lies(w_down, down_stride_n, inner, hidden) || up_stride_g < 0 || down_stride_g < 0 ||
+      (up_stride_g & 15) || (down_stride_g & 15)) return GMM_ERR_BAD_ARGUMENT;
+  if (!workspace || workspace_bytes < p.bytes || !aligned16(workspace)) return GMM_ERR_WORKSPACE;
+  char* const ws = static_cast<char*>(workspace);
+  int32_t* const offs = reinterpret_cast<int32_t*>(ws);
+  int32_t* const slot_expert = offs + experts;
+  float* const slot_weight = reinterpret_cast<float*>(slot_expert + p.slots);
+  int32_t* const row_token = slot_expert + 2 * p.slots;
+  int32_t* const token_rows = slot_expert + 3 * p.slots;
+  const auto at = [&](int64_t offset) { return reinterpret_cast<float*>(ws + offset); };
+  hipStream_t s = static_cast<hipStream_t>(stream);
+
+  FewArgs u{};
+  u.a = ws + p.x_at; u.a_scale = at(p.x_scale_at); u.a_ld = p.x_pitch / 2; u.a_rows = int32_t(tokens); u.row_index = row_token;
+  u.b = w_up; u.b_scale = up_scale; u.b_sg = up_stride_g / 2; u.b_ld = up_stride_n / 2; u.offs = offs; u.out = ws + p.h_at;
+  u.G = int32_t(experts); u.M = int32_t(p.slots); u.N = int32_t(N); u.K = int32_t(hidden / 2); u.used = int32_t(p.used);
+  u.most = int32_t(tokens);      // a token chooses an expert once
+  u.parts = p.up_parts; u.k_part = p.up_k;
+  u.result = p.activated ? kActivated : kScaled;
+  u.tiles = p.activated ? gmm_cdiv(int(inner), kColumns / 2) : gmm_cdiv(int(N), kColumns);
+  FewArgs d{};
+  d.a = ws + p.act_at; d.a_scale = at(p.act_scale_at); d.a_ld = p.act_pitch / 2; d.a_rows = int32_t(p.slots);
+  d.b = w_down; d.b_scale = down_scale; d.b_sg = down_stride_g / 2; d.b_ld = down_stride_n / 2; d.offs = offs; d.out = ws + p.y_at;
+  d.G = int32_t(experts); d.M = int32_t(p.slots); d.N = int32_t(hidden); d.K = int32_t(inner / 2); d.used = int32_t(p.used);
+  d.most = int32_t(tokens);
+  d.parts = p.down_parts; d.k_part = p.down_k; d.result = kScaled; d.tiles = gmm_cdiv(int(hidden), kColumns);
+  if (!sizes_fit(u) || !sizes_fit(d)) return GMM_ERR_UNSUPPORTED;
+  if (p.used * u.tiles * u.parts >= (int64_t(1) << 31) || p.used * d.tiles * d.parts >= (int64_t(1) << 31)) return GMM_ERR_UNSUPPORTED;
+
+  int rc = gmm_moe_route(logits, tokens > 1 ? logits_stride : experts, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert, slot_weight,
+                         row_token, token_rows, ws + p.table_at, p.table_bytes, stream);
+  if (rc == GMM_OK) rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws + p.x_at), at(p.x_scale_at), tokens, hidden, x_stride, p.x_pitch, dtype, stream);
+  if (rc == GMM_OK) rc = p.activated ? launch<true>(u, s) : launch<false>(u, s);
+  if (rc == GMM_OK)
+    rc = p.activated ? gmm_int8_quantize(ws + p.h_at, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots, inner, inner, p.act_pitch,
+                                         GMM_DT_F32, stream)
+                     : gmm_int8_gated_parts(at(p.h_at), p.up_parts, p.slots * N, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots,
+                                            inner, N, p.act_pitch, kind, s);
+  if (rc == GMM_OK) rc = launch<false>(d, s);
+  if (rc != GMM_OK) return rc;
+  const dim3 grid(unsigned((hidden + kThreads - 1) / kThreads), unsigned(tokens));
+  if (dtype == GMM_DT_BF16)
+    hipLaunchKernelGGL(int8_combine_kernel<Bf16>, grid, dim3(kThreads), 0, s, at(p.y_at), token_rows, slot_weight, static_cast<Bf16*>(out), int(top_k),
+                       p.down_parts, int(p.slots), int(hidden), out_stride);
+  else
+    hipLaunchKernelGGL(int8_combine_kernel<F16>, grid, dim3(kThreads), 0, s, at(p.y_at), token_rows, slot_weight, static_cast<F16*>(out), int(top_k),
+                       p.down_parts, int(p.slots), int(hidden), out_stride);
+  return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -35,6 +35,15 @@ __device__ __forceinline__ f32x4 mfma(F16, u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Two 8-bit integers: everything that counts elements counts pairs of them, and a product of 32 values of k is one of 64.  Its sums are 32-bit
+// integers, kept as the bits of the registers that hold fp32 sums otherwise.
+struct I8x2 { uint16_t bits; };
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma(I8x2, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                                          __builtin_bit_cast(i32x4, c), 0, 0, 0));
+}
+
 // Buffer of `bytes` bytes (below 2^31) at a base that all lanes share.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint32_t bytes) {
   const uint64_t at = reinterpret_cast<uint64_t>(base);
@@ -380,6 +389,13 @@ struct SkinnySums {
     f32x4 s = of(0, i, j, g);
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) s += of(w, i, j, g);
+    return s;
+  }
+  // The same of integers.
+  __device__ __forceinline__ i32x4 whole(int i, int j, int g) const {
+    i32x4 s = __builtin_bit_cast(i32x4, of(0, i, j, g));
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += __builtin_bit_cast(i32x4, of(w, i, j, g));
     return s;
   }
 };

@@ -4,11 +4,12 @@ layer, the grouped product, and the whole mixture-of-experts layer, whose activa
     y[t, n] = a.scale[t] * b.scale[n] * sum over k of a.values[t, k] * b.values[k, n]
 
 Weights are rounded once (:func:`quantize_columns`), activations in each call (:func:`quantize_rows`).  Sums are exact, scales are applied in
-float32, the result is rounded once.  No count reaches the host.  Registered as torch custom ops (``grouped_mm_bf16_amd::int8_quantize``,
-``int8_gated``, ``int8_mm``), which calls dispatch to while a model around them is being traced or compiled.  The reference has no counterpart.
+float32, the result is rounded once.  No count reaches the host.  Up to ``FEW_ROWS`` rows weights are streamed past the rows, more go through tiles.
+Registered as torch custom ops (``grouped_mm_bf16_amd::int8_quantize``, ``int8_mm``, ``int8_linear``, ``int8_layer``), which calls dispatch to while a model around them is being traced or compiled.  The reference has no counterpart.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -30,6 +31,19 @@ class Columns(NamedTuple):
     """A matrix, or one for each group, whose columns have a scale each: column n stands for ``scale[n] * values[:, n]``."""
     values: torch.Tensor     # int8 [K, N] or [G, K, N], contiguous along K
     scale: torch.Tensor      # float32 [N] or [G, N]
+
+
+FEW_ROWS = 64        # up to which weights are streamed past the rows, not tiled
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(device: int, T: int, K: int, N: int) -> int:
+    return _lib.load().gmm_int8_linear_workspace_bytes(T, K, N)
+
+
+@functools.lru_cache(maxsize=4096)
+def _layer_bytes(device: int, T: int, E: int, top_k: int, H: int, inner: int, kind: int) -> int:
+    return _lib.load().gmm_int8_moe_few_workspace_bytes(T, E, top_k, H, inner, kind)
 
 
 def _pitch(width: int) -> int:
@@ -212,6 +226,32 @@ def grouped_int8_mm(a: Rows, b: Columns, offs: torch.Tensor, out_dtype: torch.dt
     return _mm(a, row_index, b, offs, out_dtype)
 
 
+def _linear_now(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    x = moe_train._rows(x)
+    (T, K), N = x.shape, values.size(1)
+    if 0 < T <= FEW_ROWS and N:
+        b = _aligned(values.t())
+        out = torch.empty(T, N, device=x.device, dtype=x.dtype)
+        with _guard(x):
+            nbytes = _linear_bytes(x.device.index, T, K, N)
+            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            rc = _lib.load().gmm_int8_linear(x.data_ptr(), b.data_ptr(), scale.data_ptr(), out.data_ptr(), T, K, N, x.stride(0),
+                                             b.stride(0) if N > 1 else _pitch(K), N, _dtype_code(x.dtype), ws.data_ptr(), nbytes,
+                                             kernels.current_stream(x.device))
+        if rc != _lib.ERR_UNSUPPORTED:
+            _lib.check(rc, "linear_int8")
+            return out
+    return _mm(_quantize(x), None, Columns(values, scale), None, x.dtype)
+
+
+_linear_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_linear", mutates_args=())(_linear_now)
+
+
+@_linear_op.register_fake
+def _linear_fake(x, values, scale):
+    return x.new_empty(x.size(0), values.size(1))
+
+
 def linear_int8(x: torch.Tensor, weight: Columns) -> torch.Tensor:
     """``int8_mm(quantize_rows(x), weight)`` in x's type: x [T, K], bf16, fp16 or fp32; weight of :func:`quantize_columns`, [K, N].  Forward only."""
     _dtype_code(x.dtype)
@@ -222,7 +262,7 @@ def linear_int8(x: torch.Tensor, weight: Columns) -> torch.Tensor:
         raise RuntimeError(f"linear_int8: contraction dimensions have to match, got {x.size(1)} and {weight.values.size(0)}")
     _require_gpu(x)
     _forward_only("linear_int8", x)
-    return _mm(_quantize(x), None, weight, None, x.dtype)
+    return (_linear_op if torch.compiler.is_compiling() else _linear_now)(x, weight.values, weight.scale)
 
 
 # ------------------------------------------------------------------ the expert layer
@@ -237,12 +277,40 @@ def _gated_now(h: torch.Tensor, kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
     return values, scale
 
 
-_gated_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_gated", mutates_args=())(_gated_now)
+def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor,
+               top_k: int, kind: int, renormalize: bool) -> torch.Tensor:
+    (T, H), (E, inner, _) = x.shape, down.shape
+    if 0 < T <= FEW_ROWS:
+        rows, b, d = moe_train._rows(x), _aligned(up.transpose(1, 2)), _aligned(down.transpose(1, 2))
+        logits = router_logits if T == 1 and router_logits.stride(1) == 1 else moe_train._rows(router_logits)
+        nbytes = _layer_bytes(x.device.index, T, E, top_k, H, inner, kind)
+        if nbytes >= 0:
+            out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+            with _guard(x):
+                ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+                rc = _lib.load().gmm_int8_moe_few(rows.data_ptr(), logits.data_ptr(), b.data_ptr(), up_scale.data_ptr(), d.data_ptr(),
+                                                  down_scale.data_ptr(), out.data_ptr(), T, E, top_k, H, inner, rows.stride(0), logits.stride(0),
+                                                  b.stride(0) if E > 1 else 0, b.stride(1) if b.size(1) > 1 else _pitch(H),
+                                                  d.stride(0) if E > 1 else 0, d.stride(1) if H > 1 else _pitch(inner), H, kind, renormalize,
+                                                  _dtype_code(x.dtype), _dtype_code(router_logits.dtype), ws.data_ptr(), nbytes,
+                                                  kernels.current_stream(x.device))
+            if rc != _lib.ERR_UNSUPPORTED:
+                _lib.check(rc, "moe_forward_int8")
+                return out
+    routing = moe.moe_route(router_logits, top_k, renormalize)
+    h = _mm(_quantize(x), routing.row_token, Columns(up, up_scale), routing.offs, torch.float32)
+    values, scale = _gated_now(h, kind)
+    del h
+    y = _mm(Rows(values[:, :inner], scale), None, Columns(down, down_scale), routing.offs, x.dtype)
+    return moe_train._sum_now(y, routing.token_rows, routing.slot_weight, T, top_k)
 
 
-@_gated_op.register_fake
-def _gated_fake(h, kind):
-    return h.new_empty(h.size(0), _pitch(h.size(1) // (1 + kind)), dtype=torch.int8), h.new_empty(h.size(0))
+_layer_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_layer", mutates_args=())(_layer_now)
+
+
+@_layer_op.register_fake
+def _layer_fake(x, router_logits, up, up_scale, down, down_scale, top_k, kind, renormalize):
+    return x.new_empty(x.shape)
 
 
 def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_up: Columns, w_down: Columns, top_k: int, activation: str = "swiglu",
@@ -251,8 +319,8 @@ def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_up: Columns
     either product.
 
     x [T, H], bf16 or fp16; router_logits [T, E]; w_up of :func:`quantize_columns`, [E, H, I] ("silu") or [E, H, 2 I] ("swiglu": gate columns first);
-    w_down [E, I, H].  The activation takes the first product in float32; the experts' rows are rounded to x's type, their weighted sum again.
-    Forward only.
+    w_down [E, I, H].  The activation takes the first product in float32.  Of more than ``FEW_ROWS`` tokens the experts' rows are rounded to x's type and
+    their weighted sum again, of fewer the sum alone.  Forward only.
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
         raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")
@@ -272,10 +340,9 @@ def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_up: Columns
     if router_logits.device != x.device:
         raise RuntimeError(f"moe_forward_int8: all operands have to be on {x.device}")
     _forward_only("moe_forward_int8", x, router_logits)
-    compiling = torch.compiler.is_compiling()
-    routing = moe.moe_route(router_logits, top_k, renormalize)
-    h = _mm(_quantize(x), routing.row_token, w_up, routing.offs, torch.float32)
-    values, scale = (_gated_op if compiling else _gated_now)(h, kind)
-    del h
-    y = _mm(Rows(values[:, :w_down.values.size(1)], scale), None, w_down, routing.offs, x.dtype)
-    return (moe_train._sum_op if compiling else moe_train._sum_now)(y, routing.token_rows, routing.slot_weight, x.size(0), top_k)
+    if not 1 <= top_k <= min(E, 32):
+        raise RuntimeError(f"top_k must be in [1, min(experts, 32)], got {top_k} for {E} experts")
+    if E > 1023:
+        raise RuntimeError("Can't process more than 1024 groups")
+    _dtype_code(router_logits.dtype)
+    return (_layer_op if torch.compiler.is_compiling() else _layer_now)(x, router_logits, *w_up, *w_down, top_k, kind, bool(renormalize))

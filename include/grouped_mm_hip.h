@@ -337,6 +337,23 @@ int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index,
                 const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
                 int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* For a few rows, in one call each, with `workspace` of ..._workspace_bytes(..) bytes (-1: sizes out of range), 16-byte aligned, contents of no matter:
+ *   gmm_int8_linear   gmm_int8_quantize of x [rows, K] (dtype), then gmm_int8_mm with b [K, N], into out [rows, N] (dtype).  rows <= 64, K even and
+ *                     at least 16 (else GMM_ERR_UNSUPPORTED)
+ *   gmm_int8_moe_few  gmm_moe_route, then sum over j < top_k of slot_weight[t, j] * (act(x[t] @ w_up[e]) @ w_down[e]): w_up [experts, hidden, inner or
+ *                     2 * inner (kind GMM_ACT_SWIGLU: gate columns, then partners)], w_down [experts, inner, hidden], x and the activations rounded to 8
+ *                     bits, everything else in fp32, rounded once.  tokens <= 64, hidden and inner even and at least 16, dtype bf16 or fp16 (else
+ *                     GMM_ERR_UNSUPPORTED).  up_stride_.., down_stride_.. in bytes as for gmm_int8_mm, one matrix below 2 GiB. */
+int64_t gmm_int8_linear_workspace_bytes(int64_t rows, int64_t K, int64_t N);
+int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* out, int64_t rows, int64_t K, int64_t N, int64_t x_stride,
+                    int64_t b_stride_n, int64_t out_stride, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t gmm_int8_moe_few_workspace_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner, int32_t kind);
+int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, const float* up_scale, const int8_t* w_down, const float* down_scale,
+                     void* out, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner, int64_t x_stride,
+                     int64_t logits_stride, int64_t up_stride_g, int64_t up_stride_n, int64_t down_stride_g, int64_t down_stride_n,
+                     int64_t out_stride, int32_t kind, int32_t renormalize, int32_t dtype, int32_t logits_dtype, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 /* ---- What stands around the grouped products of an expert layer that is trained.  No counterpart in the reference.
  * Slot t * top_k + j is choice j of token t, token_rows (as gmm_moe_route writes it) its row among those sorted by expert; a slot whose row is
  * outside [0, rows) takes no part.  bf16, fp16 or fp32 (dtype), any width, any alignment, row strides in elements (at least the width where
