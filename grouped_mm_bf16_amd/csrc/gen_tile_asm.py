@@ -149,14 +149,16 @@ class Variant:
         """b_nt: B is copied with the non-temporal hint (a B panel that no other tile reads).
         act: SwiGLU epilogue -- of each 128 columns the first 64 are gates and the last 64 their partners;
         the tile stores silu(gate) * partner, 128 columns of a 16-bit output per 256 columns of the product.
-        act == 3: the product is rounded to the output's type before the activation, as by a kernel of its own."""
+        act == 3: the product is rounded to the output's type before the activation, as by a kernel of its own.
+        act == 4: 8-bit integers, an fp32 output: the activation of the scaled sums."""
         self.a_tr, self.b_tr, self.out_f32, self.tm, self.f16, self.b_nt = a_tr, b_tr, out_f32, tm, f16, b_nt
-        self.act = act in (1, 3)
+        self.act = act in (1, 3, 4)
+        self.scaled_act = act == 4
         self.rounded = act == 3
         self.partial = act == 2      # fp32 partial tile of a tile cut along K: stored through to memory (sc1)
-        assert not (self.act and (out_f32 or a_tr)) and not (self.partial and (not out_f32 or b_nt))
+        assert not (self.act and (out_f32 != self.scaled_act or a_tr)) and not (self.partial and (not out_f32 or b_nt))
         self.i8 = f16 >= 2               # 8-bit integers; a 16-bit output is bf16 (2) or fp16 (3)
-        assert not self.i8 or not (a_tr or b_tr or self.act)
+        assert not (self.i8 and (a_tr or b_tr)) and (not self.act or self.i8 == self.scaled_act)
         self.dt = "f16" if f16 & 1 else "bf16"   # element type of A, B and of a 16-bit output
         self.mfma = "v_mfma_i32_16x16x64_i8" if self.i8 else "v_mfma_f32_16x16x32_" + self.dt
         assert tm in (1, 2, 4) and (tm == 4 or not a_tr)
@@ -185,7 +187,7 @@ class Variant:
         self.b_stage = TR_STAGE if b_tr else KC_STAGE
         self.b_base = self.stages * self.a_stage   # LDS offset of B buffer 0
         self.name = "%s%s_%s_%s_m%d%s%s" % ("t" if a_tr else "k", "t" if b_tr else "k", "i8" if self.i8 else self.dt, "f32" if out_f32 else self.dt, 64 * tm,
-                                            "_bnt" if b_nt else "", ("", "_swiglu", "_partial", "_swiglu_rounded")[act])
+                                            "_bnt" if b_nt else "", ("", "_swiglu", "_partial", "_swiglu_rounded", "_swiglu_scaled")[act])
 
     def acc(self, i, j):
         """First accumulator register of the wave's 16 x 16 block (i, j), i < 2 tm, j < 8."""
@@ -614,11 +616,12 @@ def gen_epilogue(v, e, L):
     f32 = v.out_f32
     esz = 4 if f32 else 2
     nel = 16 // esz                       # elements of a 16-byte chunk
-    pitch = PITCH32 if f32 else (PITCH_ACT if v.act else PITCH)
+    # (64 activations in fp32 are as long as 128 16-bit columns)
+    pitch = PITCH if v.scaled_act else PITCH32 if f32 else PITCH_ACT if v.act else PITCH
     # groups of 32 rows (two MFMA block rows) per pass: one for fp32 (its rows are twice as long), two for a 16-bit
     # output -- staged in one pass of 128 rows, the first store of a tile left 0.3 us later (batched workload
     # 1 to 3 % slower, the others the same)
-    ipp = 1 if f32 else min(2, v.tm)
+    ipp = 1 if f32 and not v.scaled_act else min(2, v.tm)
     ncol = 64 if v.act else 16 * v.tn     # elements of a staged row
     rpi = 1024 // (ncol * esz)            # rows per read-back instruction (64 lanes x 16 bytes)
     depth = 4
@@ -653,6 +656,37 @@ def gen_epilogue(v, e, L):
         for il2 in range(2 * min(ipp, v.tm - p0)):
             i = 2 * p0 + il2                   # MFMA block row of the wave
             rowoff = 16 * il2 * pitch          # its first row in the staging area
+            if v.scaled_act:
+                # silu(g) * u = (g / (1 + 2^(-g log2 e))) * u, in that order: a gate far below zero makes the result zero, however large
+                # its partner.  Gate block j pairs with block j + 4, four elements advance together as below.
+                for j in range(4):
+                    b = t + 12 * (k % 2)
+                    k += 1
+                    for part, jj in ((b, j), (b + 4, j + 4)):
+                        for r in range(4):
+                            e("v_accvgpr_read_b32 %s, a%d" % (vr(part + r), v.acc(i, jj) + r))
+                        for r in range(4):
+                            e("v_cvt_f32_i32 %s, %s" % (vr(part + r), vr(part + r)))
+                        for r in range(4):
+                            e("v_mul_f32 %s, %s, %s" % (vr(part + r), vr(vcols + 4 * jj + r), vr(part + r)))
+                        for r in range(4):
+                            e("v_mul_f32 %s, %s, %s" % (vr(part + r), vr(vrows + i), vr(part + r)))
+                    for r in range(4):
+                        e("v_mul_f32 %s, 0xbfb8aa3b, %s" % (vr(b + 8 + r), vr(b + r)))
+                    for r in range(4):
+                        e("v_exp_f32 %s, %s" % (vr(b + 8 + r), vr(b + 8 + r)))
+                    e("s_nop 0")
+                    for r in range(4):
+                        e("v_add_f32 %s, 1.0, %s" % (vr(b + 8 + r), vr(b + 8 + r)))
+                    for r in range(4):
+                        e("v_rcp_f32 %s, %s" % (vr(b + 8 + r), vr(b + 8 + r)))
+                    e("s_nop 0")
+                    for r in range(4):
+                        e("v_mul_f32 %s, %s, %s" % (vr(b + r), vr(b + r), vr(b + 8 + r)))
+                    for r in range(4):
+                        e("v_mul_f32 %s, %s, %s" % (vr(b + r), vr(b + r), vr(b + 4 + r)))
+                    e("ds_write_b128 %s, %s offset:%d" % (vr(V_EPI), vr(b, 4), rowoff + 16 * j * 4))
+                continue
             if v.act:
                 # silu(g) * u = g * u / (1 + 2^(-g log2 e)); gate block j pairs with block j + 4 (64 columns on).
                 # Four elements advance together, so no result of a transcendental is read by the next instruction.
@@ -790,7 +824,7 @@ def emit(out, v):
     e = gen_variant(v)
     out.append("")
     out.append("template <> __device__ __forceinline__ void gmm_tile_asm<%d, %d, %d, %d, %d, %d, %d>(GmmTileRegs& r) {"
-               % (v.a_tr, v.b_tr, v.out_f32, v.tm, v.f16, v.b_nt, 2 if v.partial else 3 if v.rounded else 1 if v.act else 0))
+               % (v.a_tr, v.b_tr, v.out_f32, v.tm, v.f16, v.b_nt, 2 if v.partial else 3 if v.rounded else 4 if v.scaled_act else 1 if v.act else 0))
     out.append("  asm volatile(")
     out.append(e.text())
     out.append("      :")
@@ -819,12 +853,12 @@ def defines(out):
 
 
 def main_int8():
-    """Of the 8-bit products: bf16 (2), fp16 (3) or fp32 out; partial tiles are sums as they are, 32-bit integers."""
+    """Of the 8-bit products: bf16 (2), fp16 (3) or fp32 out; partial tiles are sums as they are, 32-bit integers; activations are fp32."""
     out = ["// Generated by gen_tile_asm.py -- do not edit.", "// The tile on 8-bit integers."]
     defines(out)
     for f16, f32 in ((2, 0), (2, 1), (3, 0)):
         for tm in (4, 2, 1):
-            for b_nt, act in ((0, 0), (1, 0), (0, 2)):
+            for b_nt, act in ((0, 0), (1, 0), (0, 2), (0, 4), (1, 4)):
                 if not (b_nt and tm == 4) and not (act and not f32):
                     emit(out, Variant(0, 0, f32, tm, f16, b_nt, act))
     sys.stdout.write("\n".join(out) + "\n")

@@ -370,13 +370,15 @@ int gmm_3d2d(const void* a, const void* b, void* out, const int32_t* offs, int32
   return run(pr, static_cast<hipStream_t>(stream));
 }
 
-int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, void* out,
-                const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
-                int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+// Checks of an 8-bit product, and its parameters; `out_cols` columns of the result.
+static int int8_params(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, void* out,
+                       const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t out_cols, int64_t K, int64_t a_stride,
+                       int64_t b_stride_g, int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, Problem& pr, GmmInt8Params& p, bool& nothing) {
   if (!dims_ok(M, N, a_rows) || K < 0 || K >= 131072 || G < 0 || G >= GMM_MAX_GROUPS || (!offs && G != 1)) return GMM_ERR_BAD_ARGUMENT;
   if (out_dtype < GMM_DT_BF16 || out_dtype > GMM_DT_F32) return GMM_ERR_UNSUPPORTED;
-  if (G == 0 || M == 0 || N == 0) return GMM_OK;
-  if (!out || (!row_index && a_rows != M) || (out_stride < N && M > 1)) return GMM_ERR_BAD_ARGUMENT;
+  nothing = G == 0 || M == 0 || N == 0;
+  if (nothing) return GMM_OK;
+  if (!out || (!row_index && a_rows != M) || (out_stride < out_cols && M > 1)) return GMM_ERR_BAD_ARGUMENT;
   if (!a_scale || !b_scale || (K > 0 && (!a || !b)) || !aligned16(a) || !aligned16(b)) return GMM_ERR_BAD_ARGUMENT;
   // rows of either operand may lie on one another only where there is one
   if ((a_stride & 15) || (b_stride_g & 15) || (b_stride_n & 15) || a_stride < 0 || b_stride_g < 0 || b_stride_n < 0) return GMM_ERR_BAD_ARGUMENT;
@@ -385,32 +387,63 @@ int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index,
   constexpr int64_t most = int64_t(1) << 22;
   if (a_stride >= 2 * most || b_stride_n >= 2 * most || out_stride >= (out_dtype == GMM_DT_F32 ? most / 2 : most)) return GMM_ERR_UNSUPPORTED;
   if (row_index && a_rows > (int64_t(1) << 31) / (a_stride > 0 ? a_stride : 1) - 1) return GMM_ERR_UNSUPPORTED;
-  const int cus = device_cus();
-  if (cus <= 0) return GMM_ERR_LAUNCH;
-  Problem pr{};
   pr.p = GmmParams{a, b, out, offs, G, offs ? GMM_JAG_M : GMM_JAG_NONE, int32_t(M), int32_t(N), int32_t((K + 1) / 2), 1,
                    0, a_stride / 2, 1, b_stride_g / 2, 1, b_stride_n / 2, 0, out_stride, 1, 0, 0};
   pr.p.gather = row_index;
   pr.p.a_rows = int32_t(a_rows);
-  set_workspace(pr, workspace, workspace_bytes);
-  GmmInt8Params p{};
+  p = GmmInt8Params{};
   static_cast<GmmParams&>(p) = pr.p;
   p.a_scale = a_scale;
   p.b_scale = b_scale;
   p.k_odd = int32_t(K & 1);
+  return GMM_OK;
+}
+
+int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, void* out,
+                const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
+                int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  Problem pr{};
+  GmmInt8Params p;
+  bool nothing = false;
+  const int bad = int8_params(a, a_scale, row_index, b, b_scale, out, offs, G, a_rows, M, N, N, K, a_stride, b_stride_g, b_stride_n, out_stride,
+                              out_dtype, pr, p, nothing);
+  if (bad || nothing) return bad;
+  const int cus = device_cus();
+  if (cus <= 0) return GMM_ERR_LAUNCH;
+  set_workspace(pr, workspace, workspace_bytes);
+  p.ws = pr.p.ws;
+  p.ws_parts = pr.p.ws_parts;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool few = gmm_int8_few_preferred(p, cus);
+  const bool few = gmm_int8_few_preferred(p);
   if (pr.eager_only) {
     GmmInt8Params full = p;
     full.ws_parts = 2 * cus;
-    const bool uses = few ? gmm_int8_few_bytes(p, cus) > 0 : gmm_int8_tile_uses_workspace(full, cus);
+    const bool uses = few ? gmm_int8_few_bytes(p) > 0 : gmm_int8_tile_uses_workspace(full, cus);
     if (uses && capture_id(s)) return GMM_ERR_WORKSPACE;
   }
   if (few) {
     char* const planes = p.ws ? static_cast<char*>(p.ws) + GMM_WS_HEADER : nullptr;
-    return gmm_launch_int8_few(p, planes, int64_t(p.ws_parts) * GMM_WS_SLOT, out_dtype, cus, s);
+    return gmm_launch_int8_few(p, planes, int64_t(p.ws_parts) * GMM_WS_SLOT, out_dtype, s);
   }
   return gmm_launch_int8_tile(p, out_dtype, cus, s) == 0 ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+int gmm_int8_gate_up(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, float* out,
+                     const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
+                     int64_t b_stride_n, int64_t out_stride, void* stream) {
+  Problem pr{};
+  GmmInt8Params p;
+  bool nothing = false;
+  if (N >= 0 && (N & 127)) return GMM_ERR_UNSUPPORTED;
+  const int bad = int8_params(a, a_scale, row_index, b, b_scale, out, offs, G, a_rows, M, N, N / 2, K, a_stride, b_stride_g, b_stride_n, out_stride,
+                              GMM_DT_F32, pr, p, nothing);
+  if (bad || nothing) return bad;
+  // partner columns half the matrix away, both reached from one tile's origin
+  if ((N / 2 + 256) * b_stride_n >= (int64_t(1) << 31)) return GMM_ERR_UNSUPPORTED;
+  const int cus = device_cus();
+  if (cus <= 0) return GMM_ERR_LAUNCH;
+  p.act = 4;
+  return gmm_launch_int8_tile(p, GMM_DT_F32, cus, static_cast<hipStream_t>(stream)) == 0 ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
 int gmm_zero_unowned(void* out, const int32_t* offs, int32_t G, int32_t by_columns, int64_t M, int64_t N, int64_t o_sm, int64_t o_sn,

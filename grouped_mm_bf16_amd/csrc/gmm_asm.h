@@ -186,8 +186,9 @@ __device__ __forceinline__ GmmTileDesc gmm_describe_tile(const P& p, const GmmTi
   }
   // gate and partner columns apart: the tile's first gate column; the last tile of an odd number of 64-column turns also
   // fetches columns that are not its own, whose results are not stored
-  const int b_n0 = ACT == 3 ? t.n0 / 2 : t.n0;
-  if (ACT == 3) dsc.b.apart = p.N / 2;
+  constexpr bool APART = ACT == 3 || ACT == 4;
+  const int b_n0 = APART ? t.n0 / 2 : t.n0;
+  if (APART) dsc.b.apart = p.N / 2;
   if (!B_TR) {
     dsc.b.base = b + int64_t(b_n0) * ldb + k_begin;
     dsc.b.bytes = (int64_t(p.N - 1 - b_n0) * ldb + (p.K - k_begin)) * 2;
@@ -214,8 +215,8 @@ __device__ __forceinline__ GmmTileDesc gmm_describe_tile(const P& p, const GmmTi
     dsc.k_odd = p.k_odd && t.k_hi == p.K;
     dsc.row_scale = p.gather ? p.a_scale : p.a_scale + t.m0;
     dsc.row_scales = p.gather ? p.a_rows : (p.jag == GMM_JAG_M ? t.m_hi : p.M) - t.m0;
-    dsc.col_scale = p.b_scale + int64_t(t.g) * p.N + t.n0;
-    dsc.col_scales = p.N - t.n0;
+    dsc.col_scale = p.b_scale + int64_t(t.g) * p.N + b_n0;
+    dsc.col_scales = p.N - b_n0;
   }
   return dsc;
 }

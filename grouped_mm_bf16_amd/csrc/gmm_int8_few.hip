@@ -1,6 +1,6 @@
 // Products of 8-bit integers for a few rows, a linear layer for a few tokens and the expert layer for them (gmm_int8_linear, gmm_int8_moe_few in
-// include/grouped_mm_hip.h).  Reading the weights bounds them: they are streamed past the rows as the 16-bit ones are (gmm_skinny.h), 64 columns
-// to a workgroup, whose waves share k; where that leaves compute units idle, k is cut into parts as well.
+// include/grouped_mm_hip.h).  Reading the weights bounds them: they are streamed past the rows as the 16-bit ones are (gmm_skinny.h), 16 to 64 columns
+// to a workgroup, whose waves share k (few_shape); where that leaves compute units idle, k is cut into parts as well.
 //   one matrix        parts are planes of integer sums, which a second kernel adds up and scales: exact, as in one part
 //   expert layer      route, rows of x to 8 bits, first product, activation to 8 bits, second product, sum over choices and parts.  The planes
 //                     between its launches are scaled fp32 values; SwiGLU is computed by the first product where k is in one part
@@ -18,8 +18,7 @@ namespace {
 
 using namespace gmm;
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kColumns = 64;
+constexpr int kThreads = 256;      // of the kernels behind the products
 constexpr int kMaxTokens = 64;
 
 enum Result : int { kOut, kSums, kScaled, kActivated };
@@ -36,7 +35,7 @@ struct FewArgs {
   uint32_t a_bytes, b_bytes;
   int32_t G, M, N, K, a_rows; // K: pairs
   int32_t used, most;         // groups that can have rows; rows that a group can have, 64 at most
-  int32_t tiles, parts, k_part;
+  int32_t columns, tiles, parts, k_part;      // of a strip (with its partners); strips; parts along k and their length
   int32_t result, out_dtype;
 };
 
@@ -83,13 +82,12 @@ __device__ __forceinline__ float scaled(int sum, float column, float row) {
   return v;
 }
 
-// GLU: a strip is 32 gate columns and their 32 partners, N / 2 further on; the result is silu(gate) * partner.
-template <int MF, bool GLU>
-__global__ void __launch_bounds__(kThreads, MF == 4 ? 1 : 2) int8_few_kernel(const FewArgs a) {
-  using S = Strip<I8x2, GMM_W_COLS, MF, 1>;
-  constexpr int FR = S::FR, OUT = GLU ? kColumns / 2 : kColumns;
-  static_assert(16 * FR == kColumns, "");
-  __shared__ SkinnyShared<S, kWaves> shared;
+// FR: a strip is 16 FR columns.  GLU: half of them gate columns, the others their partners, N / 2 further on; the result is silu(gate) * partner.
+template <int MF, int FR, int WAVES, bool GLU>
+__global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int8_few_kernel(const FewArgs a) {
+  using S = Skinny<I8x2, GMM_W_COLS, FR, MF, 1, GMM_A_STAGED, 2>;
+  constexpr int OUT = GLU ? 8 * FR : 16 * FR, THREADS = 64 * WAVES;
+  __shared__ SkinnyShared<S, WAVES> shared;
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
   int g = 0, row0 = 0, rows = a.M;
   if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) return;
@@ -114,14 +112,14 @@ __global__ void __launch_bounds__(kThreads, MF == 4 ? 1 : 2) int8_few_kernel(con
   });
   f32x4 acc[MF][FR];
   clear(acc);
-  s.template run<kWaves>(rows, part * a.k_part, min(a.K, (part + 1) * a.k_part), wave, acc);
+  s.template run<WAVES>(rows, part * a.k_part, min(a.K, (part + 1) * a.k_part), wave, acc);
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     if (16 * m >= rows) break;
     __syncthreads();
     shared.sums.put(wave, lane, acc[m]);
     __syncthreads();
-    for (int u = threadIdx.x; u < OUT * 4; u += kThreads) {
+    for (int u = threadIdx.x; u < OUT * 4; u += THREADS) {
       const int oc = u % OUT, og = u / OUT, col = first + oc;
       if (col >= width) continue;
       const auto sums = [&](int c) { return shared.sums.whole(S::product_of(c), S::lane_of(c), og); };
@@ -188,16 +186,37 @@ __global__ void __launch_bounds__(kThreads) int8_combine_kernel(const float* __r
 }
 
 // ---------------------------------------------------------------- host side
-// Parts of k (in pairs of integers), each a multiple of a step and at least as long as the waves' steps together, so that there are about three
-// workgroups to a compute unit.
-void cut(int64_t K, int64_t strips, int64_t cus, int32_t& parts, int32_t& each) {
-  constexpr int64_t step = 64, least = step * kWaves;
-  int64_t want = strips > 0 ? 3 * cus / strips : 1;
-  if (want > K / least) want = K / least;
-  if (want > 16) want = 16;
-  if (want < 1) want = 1;
-  each = int32_t(round_up((K + want - 1) / want, step));
-  parts = each ? int32_t((K + each - 1) / each) : 1;
+// How a product of up to `rows` rows of a group is laid out.  Measured alone, us, for rows x N x K of one matrix, weights from memory:
+//   64 columns, 4 waves    where such strips fill half the compute units and more: 1 x 14336 x 4096 12.5 (32 columns 13.0, 16 columns 15.9), 1 x 9216
+//                          x 2048 6.2 (7.4, 10.3), 48 x 14336 x 4096 18.1 (25.1; 64 in two parts 22.6), 48 x 9216 x 2048 11.6 (17.9); but 1 x 8192 x
+//                          8192 15.3 (16 columns 13.4), 48 x 8192 x 8192 24.6 (32 columns 21.3)
+//   16 columns, 16 waves   fewer columns and long, up to 16 rows: 1 x 4096 x 4096 6.2 (32 columns 6.5, 64 in three parts 7.7), 1 x 4096 x 14336 12.5
+//                          (13.5 in two parts, 13.3 in three); but 1 x 1536 x 2048 4.9 (4.3), 1 x 6144 x 768 5.5 (4.2)
+//   32 columns, 8 waves    what is left: short columns, or more rows, which narrower strips would read too often, then in as many parts of k as
+//                          fill the compute units: 48 x 4096 x 4096 12.3 in two parts, 12.9 in one (64 columns in three 12.7), 24 x 1536 x 2048 7.5
+//                          in four (7.4 in one), 48 x 4096 x 14336 20.3 in two (64 columns in four 19.2)
+struct Shape { int32_t columns, parts, k_part; };
+
+Shape few_shape(int64_t used, int64_t rows, int64_t N, int64_t K) {
+  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256, step = 64;
+  const auto strips = [&](int64_t columns) { return used * ((N + columns - 1) / columns); };
+  Shape s{64, 1, int32_t(round_up(K, step))};
+  if (16 * strips(64) >= 9 * cus) return s;
+  s.columns = rows <= 16 && K >= 2048 ? 16 : 32;
+  if (rows <= 16) return s;
+  int64_t want = strips(32) > 0 ? cus / strips(32) : 1;
+  if (want > K / (8 * step)) want = K / (8 * step);      // a step for each wave
+  if (want <= 1) return s;
+  s.k_part = int32_t(round_up((K + want - 1) / want, step));
+  s.parts = int32_t((K + s.k_part - 1) / s.k_part);
+  return s;
+}
+
+void set_shape(FewArgs& a, const Shape& s, bool glu = false) {
+  a.columns = s.columns;
+  a.parts = s.parts;
+  a.k_part = s.k_part;
+  a.tiles = glu ? gmm_cdiv(a.N / 2, s.columns / 2) : gmm_cdiv(a.N, s.columns);
 }
 
 FewArgs from_params(const GmmInt8Params& p) {
@@ -207,9 +226,7 @@ FewArgs from_params(const GmmInt8Params& p) {
   a.G = p.G; a.M = p.M; a.N = p.N; a.K = p.K; a.a_rows = p.gather ? p.a_rows : p.M;
   a.used = a.offs ? gmm_min(p.G, p.M) : 1;
   a.most = p.M;
-  a.tiles = gmm_cdiv(p.N, kColumns);
-  a.parts = 1;
-  a.k_part = int32_t(round_up(p.K, 64));
+  set_shape(a, few_shape(a.used, a.most, a.N, a.K));
   return a;
 }
 
@@ -222,35 +239,45 @@ bool sizes_fit(FewArgs& a) {
 
 template <bool GLU>
 int launch(const FewArgs& a, hipStream_t stream) {
-  const dim3 grid(unsigned(int64_t(a.used) * a.tiles * a.parts)), block(kThreads);
-  if (a.most <= 16) hipLaunchKernelGGL((int8_few_kernel<1, GLU>), grid, block, 0, stream, a);
-  else if (a.most <= 32) hipLaunchKernelGGL((int8_few_kernel<2, GLU>), grid, block, 0, stream, a);
-  else if (a.most <= 48) hipLaunchKernelGGL((int8_few_kernel<3, GLU>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((int8_few_kernel<4, GLU>), grid, block, 0, stream, a);
+  const dim3 grid(unsigned(int64_t(a.used) * a.tiles * a.parts));
+  const auto go = [&](auto mf, auto fr, auto waves) {
+    constexpr int MF = decltype(mf)::value, FR = decltype(fr)::value, WAVES = decltype(waves)::value;
+    hipLaunchKernelGGL((int8_few_kernel<MF, FR, WAVES, GLU>), grid, dim3(64 * WAVES), 0, stream, a);
+  };
+  const auto by_rows = [&](auto fr, auto waves) {
+    if (a.most <= 16) go(std::integral_constant<int, 1>{}, fr, waves);
+    else if (a.most <= 32) go(std::integral_constant<int, 2>{}, fr, waves);
+    else if (a.most <= 48) go(std::integral_constant<int, 3>{}, fr, waves);
+    else go(std::integral_constant<int, 4>{}, fr, waves);
+  };
+  if (a.columns == 64) by_rows(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+  else if (a.columns == 32) by_rows(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
+  else go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 
 }  // namespace
 
-bool gmm_int8_few_preferred(const GmmInt8Params& p, int) {
+bool gmm_int8_few_preferred(const GmmInt8Params& p) {
   FewArgs a = from_params(p);
   if (p.k_odd || !sizes_fit(a) || int64_t(a.used) * a.tiles >= (int64_t(1) << 27)) return false;
   return p.M <= kMaxTokens;
 }
 
-int64_t gmm_int8_few_bytes(const GmmInt8Params& p, int num_cus) {
-  FewArgs a = from_params(p);
-  if (a.offs) return 0;
-  cut(a.K, a.tiles, num_cus, a.parts, a.k_part);
-  return a.parts > 1 ? int64_t(a.parts) * a.M * a.N * 4 : 0;
+int64_t gmm_int8_few_bytes(const GmmInt8Params& p) {
+  const FewArgs a = from_params(p);
+  return !a.offs && a.parts > 1 ? int64_t(a.parts) * a.M * a.N * 4 : 0;
 }
 
-int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_bytes, int out_dtype, int num_cus, hipStream_t stream) {
+int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_bytes, int out_dtype, hipStream_t stream) {
   FewArgs a = from_params(p);
   if (!sizes_fit(a)) return GMM_ERR_UNSUPPORTED;
   a.out_dtype = out_dtype;
   a.result = kOut;
-  if (!a.offs && planes && planes_bytes >= gmm_int8_few_bytes(p, num_cus)) cut(a.K, a.tiles, num_cus, a.parts, a.k_part);
+  if (a.offs || !planes || planes_bytes < gmm_int8_few_bytes(p)) {      // the planes do not say whose scales their rows take
+    a.parts = 1;
+    a.k_part = int32_t(round_up(a.K, 64));
+  }
   if (a.parts == 1) return launch<false>(a, stream);
   FewArgs u = a;
   u.out = planes;
@@ -269,8 +296,7 @@ struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; };
 
 bool plan_linear(int64_t T, int64_t K, int64_t N, LinearPlan& p) {
   if (T < 0 || T > kMaxTokens || K < 0 || K >= 131072 || N < 0 || N >= (int64_t(1) << 31)) return false;
-  int32_t parts, each;
-  cut((K + 1) / 2, (N + kColumns - 1) / kColumns, gmm_num_cus() > 0 ? gmm_num_cus() : 256, parts, each);
+  const int64_t parts = few_shape(1, T, N, K / 2).parts;
   p.pitch = round_up(K > 0 ? K : 1, 16);
   p.scale_at = T * p.pitch;
   p.planes_at = round_up(p.scale_at + 4 * T, 16);
@@ -282,7 +308,7 @@ bool plan_linear(int64_t T, int64_t K, int64_t N, LinearPlan& p) {
 struct LayerPlan {
   int64_t slots, used, x_pitch, act_pitch, table_bytes;
   int64_t table_at, x_at, x_scale_at, h_at, act_at, act_scale_at, y_at, bytes;
-  int32_t up_parts, up_k, down_parts, down_k;
+  Shape up, down;
   bool activated;      // by the first product
 };
 
@@ -290,12 +316,12 @@ bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t k
   if (T < 0 || T > kMaxTokens || E < 1 || H < 1 || I < 1 || H >= 131072 || I >= 131072 || k < 1) return false;
   p.table_bytes = gmm_moe_route_workspace_bytes(T, E, k);
   if (p.table_bytes < 0 || k > 32 || k > E) return false;
-  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256, N = kind == GMM_ACT_SWIGLU ? 2 * I : I;
+  const int64_t N = kind == GMM_ACT_SWIGLU ? 2 * I : I;
   p.slots = T * k;
   p.used = p.slots < E ? p.slots : E;
-  cut(H / 2, p.used * ((N + kColumns - 1) / kColumns), cus, p.up_parts, p.up_k);
-  cut(I / 2, p.used * ((H + kColumns - 1) / kColumns), cus, p.down_parts, p.down_k);
-  p.activated = p.up_parts == 1 && kind == GMM_ACT_SWIGLU;
+  p.up = few_shape(p.used, T, N, H / 2);
+  p.down = few_shape(p.used, T, H, I / 2);
+  p.activated = p.up.parts == 1 && kind == GMM_ACT_SWIGLU;
   p.x_pitch = round_up(H, 16);
   p.act_pitch = round_up(I, 16);
   int64_t at = 0;
@@ -304,10 +330,10 @@ bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t k
   p.table_at = take(p.table_bytes);
   p.x_at = take(T * p.x_pitch);
   p.x_scale_at = take(4 * T);
-  p.h_at = take((p.activated ? I : p.up_parts * N) * p.slots * 4);
+  p.h_at = take((p.activated ? I : p.up.parts * N) * p.slots * 4);
   p.act_at = take(p.slots * p.act_pitch);
   p.act_scale_at = take(4 * p.slots);
-  p.y_at = take(p.down_parts * p.slots * H * 4);
+  p.y_at = take(p.down.parts * p.slots * H * 4);
   p.bytes = at;
   return true;
 }
@@ -333,18 +359,16 @@ int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* 
   if (rows == 0 || N == 0) return GMM_OK;
   if (!x || !b || !b_scale || !out || (rows > 1 && (x_stride < K || out_stride < N)) || !lies(b, b_stride_n, K, N)) return GMM_ERR_BAD_ARGUMENT;
   if (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)) return GMM_ERR_WORKSPACE;
-  const int cus = gmm_num_cus();
-  if (cus <= 0) return GMM_ERR_LAUNCH;
   char* const ws = static_cast<char*>(workspace);
   GmmInt8Params p{};
   p.a = ws; p.b = b; p.c = out; p.G = 1; p.jag = GMM_JAG_NONE; p.M = int32_t(rows); p.N = int32_t(N); p.K = int32_t(K / 2);
   p.a_sm = plan.pitch / 2; p.a_sk = 1; p.b_sk = 1; p.b_sn = b_stride_n / 2; p.c_sm = out_stride; p.c_sn = 1; p.a_rows = int32_t(rows);
   p.a_scale = reinterpret_cast<float*>(ws + plan.scale_at);
   p.b_scale = b_scale;
-  if (!gmm_int8_few_preferred(p, cus)) return GMM_ERR_UNSUPPORTED;
+  if (!gmm_int8_few_preferred(p)) return GMM_ERR_UNSUPPORTED;
   const int rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws), reinterpret_cast<float*>(ws + plan.scale_at), rows, K, x_stride, plan.pitch,
                                    dtype, stream);
-  return rc == GMM_OK ? gmm_launch_int8_few(p, ws + plan.planes_at, plan.bytes - plan.planes_at, dtype, cus, static_cast<hipStream_t>(stream)) : rc;
+  return rc == GMM_OK ? gmm_launch_int8_few(p, ws + plan.planes_at, plan.bytes - plan.planes_at, dtype, static_cast<hipStream_t>(stream)) : rc;
 }
 
 int64_t gmm_int8_moe_few_workspace_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t inner, int32_t kind) {
@@ -381,15 +405,15 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   u.b = w_up; u.b_scale = up_scale; u.b_sg = up_stride_g / 2; u.b_ld = up_stride_n / 2; u.offs = offs; u.out = ws + p.h_at;
   u.G = int32_t(experts); u.M = int32_t(p.slots); u.N = int32_t(N); u.K = int32_t(hidden / 2); u.used = int32_t(p.used);
   u.most = int32_t(tokens);      // a token chooses an expert once
-  u.parts = p.up_parts; u.k_part = p.up_k;
+  set_shape(u, p.up, p.activated);
   u.result = p.activated ? kActivated : kScaled;
-  u.tiles = p.activated ? gmm_cdiv(int(inner), kColumns / 2) : gmm_cdiv(int(N), kColumns);
   FewArgs d{};
   d.a = ws + p.act_at; d.a_scale = at(p.act_scale_at); d.a_ld = p.act_pitch / 2; d.a_rows = int32_t(p.slots);
   d.b = w_down; d.b_scale = down_scale; d.b_sg = down_stride_g / 2; d.b_ld = down_stride_n / 2; d.offs = offs; d.out = ws + p.y_at;
   d.G = int32_t(experts); d.M = int32_t(p.slots); d.N = int32_t(hidden); d.K = int32_t(inner / 2); d.used = int32_t(p.used);
   d.most = int32_t(tokens);
-  d.parts = p.down_parts; d.k_part = p.down_k; d.result = kScaled; d.tiles = gmm_cdiv(int(hidden), kColumns);
+  set_shape(d, p.down);
+  d.result = kScaled;
   if (!sizes_fit(u) || !sizes_fit(d)) return GMM_ERR_UNSUPPORTED;
   if (p.used * u.tiles * u.parts >= (int64_t(1) << 31) || p.used * d.tiles * d.parts >= (int64_t(1) << 31)) return GMM_ERR_UNSUPPORTED;
 
@@ -400,17 +424,17 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   if (rc == GMM_OK)
     rc = p.activated ? gmm_int8_quantize(ws + p.h_at, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots, inner, inner, p.act_pitch,
                                          GMM_DT_F32, stream)
-                     : gmm_int8_gated_parts(at(p.h_at), p.up_parts, p.slots * N, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots,
+                     : gmm_int8_gated_parts(at(p.h_at), p.up.parts, p.slots * N, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots,
                                             inner, N, p.act_pitch, kind, s);
   if (rc == GMM_OK) rc = launch<false>(d, s);
   if (rc != GMM_OK) return rc;
   const dim3 grid(unsigned((hidden + kThreads - 1) / kThreads), unsigned(tokens));
   if (dtype == GMM_DT_BF16)
     hipLaunchKernelGGL(int8_combine_kernel<Bf16>, grid, dim3(kThreads), 0, s, at(p.y_at), token_rows, slot_weight, static_cast<Bf16*>(out), int(top_k),
-                       p.down_parts, int(p.slots), int(hidden), out_stride);
+                       p.down.parts, int(p.slots), int(hidden), out_stride);
   else
     hipLaunchKernelGGL(int8_combine_kernel<F16>, grid, dim3(kThreads), 0, s, at(p.y_at), token_rows, slot_weight, static_cast<F16*>(out), int(top_k),
-                       p.down_parts, int(p.slots), int(hidden), out_stride);
+                       p.down.parts, int(p.slots), int(hidden), out_stride);
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
 }
 

@@ -35,6 +35,10 @@ bool gmm_int8_tile_uses_workspace(GmmInt8Params p, int num_cus) {
 
 int gmm_launch_int8_tile(GmmInt8Params p, int out_dtype, int num_cus, hipStream_t stream) {
   set_tiles(p, num_cus);
+  if (p.act) {
+    hipLaunchKernelGGL((gmm_asm_kernel<0, 0, 1, 2, 4, ORDER_PLAIN, GmmInt8Params>), dim3(p.num_wg), dim3(256), 0, stream, p);
+    return hipGetLastError() == hipSuccess ? 0 : 1;
+  }
   if (out_dtype == GMM_DT_BF16) return launch<0, 2>(p, stream);
   if (out_dtype == GMM_DT_F16) return launch<0, 3>(p, stream);
   return launch<1, 2>(p, stream);

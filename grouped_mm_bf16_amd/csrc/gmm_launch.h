@@ -27,9 +27,9 @@ int gmm_launch_int8_tile(GmmInt8Params p, int out_dtype, int num_cus, hipStream_
 bool gmm_int8_tile_uses_workspace(GmmInt8Params p, int num_cus);
 
 // The same product where the rows are few (gmm_int8_few.hip): true if it is faster there.  planes: room for gmm_int8_few_bytes(..) bytes, or null.
-bool gmm_int8_few_preferred(const GmmInt8Params& p, int num_cus);
-int64_t gmm_int8_few_bytes(const GmmInt8Params& p, int num_cus);
-int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_bytes, int out_dtype, int num_cus, hipStream_t stream);
+bool gmm_int8_few_preferred(const GmmInt8Params& p);
+int64_t gmm_int8_few_bytes(const GmmInt8Params& p);
+int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_bytes, int out_dtype, hipStream_t stream);
 // gmm_int8_gated of an operand that is the sum of `parts`, `plane` elements apart.
 int gmm_int8_gated_parts(const float* h, int parts, int64_t plane, int8_t* values, float* scale, int64_t rows, int64_t inner, int64_t h_stride,
                          int64_t values_stride, int32_t kind, hipStream_t stream);

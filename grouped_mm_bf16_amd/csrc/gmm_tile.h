@@ -38,6 +38,7 @@ struct GmmTileRegs {
 // their partners u; the tile stores silu(g) * u: 128 columns of a 16-bit output per 256-column tile.
 // ACT = 3: the same with g and u rounded to the output's type first, for a B that has all gate columns before all partner
 // columns (GmmOperand::apart).
+// ACT = 4: 8-bit integers, the activation of the scaled sums in fp32, for a B as with ACT = 3.
 template <int A_TR, int B_TR, int OUT_F32, int TM, int F16, int B_NT, int ACT>
 __device__ __forceinline__ void gmm_tile_asm(GmmTileRegs& r);
 
@@ -187,16 +188,17 @@ __device__ __forceinline__ void gmm_copy_offsets(int lane, int wave, const GmmOp
 template <int A_TR, int B_TR, int OUT_F32, int TM = 4, int F16 = 0, int B_NT = 0, int ACT = 0>
 __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned lds_base, int lane, int wave) {
   static_assert(TM == 4 || !A_TR, "short tiles exist for a K-contiguous A only");
-  static_assert(!(ACT & 1) || (!A_TR && !OUT_F32), "the SwiGLU epilogue: K-contiguous A, 16-bit output");
+  constexpr bool GATED = ACT == 1 || ACT == 3 || ACT == 4, APART = ACT == 3 || ACT == 4;
+  static_assert(!GATED || (!A_TR && OUT_F32 == (ACT == 4)), "the SwiGLU epilogue: K-contiguous A, 16-bit output, or fp32 of 8-bit integers");
   static_assert(ACT != 2 || (OUT_F32 && !B_NT), "partial tiles are fp32");
-  static_assert(F16 < 2 || (!A_TR && !B_TR && !(ACT & 1)), "8-bit integers: both operands contiguous along K");
+  static_assert(F16 < 2 || (!A_TR && !B_TR && (!GATED || ACT == 4)), "8-bit integers: both operands contiguous along K");
   constexpr int WROWS = 32 * TM;  // rows of the tile per wave row
   constexpr int B_BASE = GmmTileLayout<A_TR, TM>::b_base;
   const int wm = wave & 1, wn = wave >> 1;
   const int nk = (t.klen + GMM_TILE_K - 1) / GMM_TILE_K;
   GmmTileRegs r;
   gmm_copy_offsets<A_TR, 2 * TM>(lane, wave, t.a, t.klen, t.khead, nk, r.voa_head, r.voa, r.voa_tail);
-  gmm_copy_offsets<B_TR, 8, ACT == 3>(lane, wave, t.b, t.klen, t.khead, nk, r.vob_head, r.vob, r.vob_tail);
+  gmm_copy_offsets<B_TR, 8, APART>(lane, wave, t.b, t.klen, t.khead, nk, r.vob_head, r.vob, r.vob_tail);
   // Fragment read addresses.  An MFMA fragment is 16 rows (or columns) x 32 k: lane l holds row l % 16,
   // k 8 (l / 16) .. + 7.  K-contiguous operand: one ds_read_b128 of chunk 4 sp + l / 16 of the lane's row
   // (sp = k half of the K tile; one address per half, 16-row blocks are immediate offsets).  Transposed
@@ -225,10 +227,10 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
   // Epilogue: the wave stages its block in LDS and reads it back row by row, 16 bytes per lane (see
   // gen_tile_asm.py).  ESZ bytes per element: a lane's chunk is NEL = 16 / ESZ columns, a row of the wave's
   // 128 columns takes LPR lanes, a read-back instruction covers 64 / LPR rows.
-  constexpr int WCOLS = (ACT & 1) ? 64 : 128;                   // output columns of a wave
+  constexpr int WCOLS = GATED ? 64 : 128;                   // output columns of a wave
   constexpr int ESZ = OUT_F32 ? 4 : 2, NEL = 16 / ESZ, LPR = WCOLS / NEL;
-  constexpr int EPITCH = OUT_F32 ? GMM_TILE_PITCH32 : ((ACT & 1) ? GMM_TILE_PITCH_ACT : GMM_TILE_PITCH);
-  constexpr int STAGE_ROWS = OUT_F32 ? 32 : WROWS;        // rows a wave stages per pass
+  constexpr int EPITCH = ACT == 4 ? GMM_TILE_PITCH : OUT_F32 ? GMM_TILE_PITCH32 : GATED ? GMM_TILE_PITCH_ACT : GMM_TILE_PITCH;
+  constexpr int STAGE_ROWS = OUT_F32 && ACT != 4 ? 32 : WROWS;        // rows a wave stages per pass
   int partial = 0;
   {
     const int row_t = wm * WROWS + lane / LPR, col_t = wn * WCOLS + (lane % LPR) * NEL;
@@ -259,7 +261,7 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
       const int idx = wave * per_wave + lane, line = t.share * per_tile + idx;
       if (lane < per_wave && idx < per_tile && line < 256) {
         int col = B_TR ? (line & 3) * 64 : line;
-        if (ACT == 3) col = gmm_apart_column(col, t.b.apart);
+        if (APART) col = gmm_apart_column(col, t.b.apart);
         off_b = B_TR ? (line >> 2) * t.b.ld * 2 + col * 2 : col * t.b.ld * 2;
       }
     }
@@ -304,7 +306,7 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
     int row = at;
     if (t.a.gather) row = at < t.a.gather_n ? t.a.gather[at] : -1;
     r.scale[0] = row >= 0 && row < t.row_scales ? row * 4 : (int)GMM_OOB;
-    r.scale[1] = at * 4;
+    r.scale[1] = (APART ? gmm_apart_column(at, t.b.apart) : at) * 4;
     r.rsrc_rows = gmm_make_rsrc(t.row_scale, (long long)t.row_scales * 4);
     r.rsrc_cols = gmm_make_rsrc(t.col_scale, (long long)t.col_scales * 4);
     r.ra_addr[2] = lds_base + GMM_TILE_SCALES + (wm * WROWS + (lane & 15)) * 4;

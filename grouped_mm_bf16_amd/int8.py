@@ -277,6 +277,25 @@ def _gated_now(h: torch.Tensor, kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
     return values, scale
 
 
+def _activated(a: Rows, routing: moe.Routing, up: torch.Tensor, up_scale: torch.Tensor, kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The first product's activations in 8 bits; SwiGLU in the product's own kernel where that takes its columns."""
+    b = _aligned(up.transpose(1, 2))
+    (G, N, K), M = b.shape, routing.row_token.numel()
+    if kind and M and K and N % 128 == 0:
+        rows = _aligned(a.values)
+        act = torch.empty(M, N // 2, device=rows.device, dtype=torch.float32)
+        with _guard(rows):
+            rc = _lib.load().gmm_int8_gate_up(rows.data_ptr(), a.scale.data_ptr(), routing.row_token.data_ptr(), b.data_ptr(), up_scale.data_ptr(),
+                                              act.data_ptr(), routing.offs.data_ptr(), G, rows.size(0), M, N, K,
+                                              rows.stride(0) if rows.size(0) > 1 else _pitch(K), b.stride(0) if G > 1 else 0, b.stride(1), N // 2,
+                                              kernels.current_stream(rows.device))
+        if rc != _lib.ERR_UNSUPPORTED:
+            _lib.check(rc, "moe_forward_int8: first product")
+            return _quantize_now(act)
+        del act
+    return _gated_now(_mm_now(a.values, a.scale, routing.row_token, b, up_scale, routing.offs, torch.float32), kind)
+
+
 def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor,
                top_k: int, kind: int, renormalize: bool) -> torch.Tensor:
     (T, H), (E, inner, _) = x.shape, down.shape
@@ -298,9 +317,7 @@ def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, u
                 _lib.check(rc, "moe_forward_int8")
                 return out
     routing = moe.moe_route(router_logits, top_k, renormalize)
-    h = _mm(_quantize(x), routing.row_token, Columns(up, up_scale), routing.offs, torch.float32)
-    values, scale = _gated_now(h, kind)
-    del h
+    values, scale = _activated(_quantize(x), routing, up, up_scale, kind)
     y = _mm(Rows(values[:, :inner], scale), None, Columns(down, down_scale), routing.offs, x.dtype)
     return moe_train._sum_now(y, routing.token_rows, routing.slot_weight, T, top_k)
 

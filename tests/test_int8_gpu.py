@@ -279,6 +279,26 @@ def test_layer(T, E, k, H, inner, dtype, kind):
     assert (plain.f64(out) - want).norm() <= (2.5 * plain.UNIT[dtype] + 2.0 ** -8) * want.norm()
 
 
+@pytest.mark.parametrize("T,E,k,H,inner", [(65, 4, 2, 64, 64), (129, 3, 3, 333, 192), (400, 8, 2, 320, 192), (900, 5, 2, 1031, 320), (2500, 128, 8, 192, 64),
+                                           (1500, 4, 2, 512, 1024)])
+def test_layer_whose_first_product_activates(T, E, k, H, inner):
+    """Inner sizes of whole blocks of 64: SwiGLU in the tile's epilogue, tiles of every height."""
+    x, z, up, down = layer(T, E, H, inner, "swiglu")
+    out = int8.moe_forward_int8(x, z, up, down, k)
+    want = oracle.layer(x, z, up.values, up.scale, down.values, down.scale, k, "swiglu")
+    assert (plain.f64(out) - want).norm() <= (2.5 * 2.0 ** -8 + 2.0 ** -8) * want.norm()
+    # the two products of the layer one after the other, the first without the epilogue: the same but for the activation's last bits
+    r = int8.moe.moe_route(z, k)
+    a = int8.quantize_rows(x)
+    h = int8.grouped_int8_mm(a, up, r.offs, SF, r.row_token)
+    fused = int8._activated(a, r, up.values, up.scale, 1)
+    apart = int8._gated_now(h, 1)
+    # e^-g to a few units of fp32 of its exponent, |g| below 30; the maximum of the row alone stands in the scale
+    assert ((fused[1] - apart[1]).abs() <= 2.0 ** -18 * apart[1]).all()
+    step = (fused[0][:, :inner].int() - apart[0][:, :inner].int()).abs()
+    assert step.max() <= 1 and step.float().mean() <= 1e-3
+
+
 def test_layer_over_all_experts_and_halves_of_logits():
     x, z, up, down = layer(40, 10, 64, 64, "swiglu")
     out = int8.moe_forward_int8(x, z.to(BF), up, down, 3, renormalize=False)

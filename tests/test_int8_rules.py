@@ -148,13 +148,18 @@ def test_c_entries_refuse_without_a_launch():
     assert mm(sa=30) == mm(sg=250) == mm(sn=30) == mm(sa=16) == mm(sn=16) == mm(sa=-32) == mm(sn=-32) == mm(sg=-16) == 1
     assert mm(dt=3) == mm(dt=-1) == 2 and mm(sa=1 << 23) == mm(sn=1 << 23) == mm(so=1 << 22) == mm(idx=p, R=1 << 27) == 2
     assert mm(dt=2, so=1 << 21) == 2
+    def gate_up(a=p, out=p, offs=p, G=2, R=4, M=4, N=128, K=30, sa=32, sg=4096, sn=32, so=64):
+        return lib.gmm_int8_gate_up(a, p, p, p, p, out, offs, G, R, M, N, K, sa, sg, sn, so, None)
+
+    assert gate_up(N=64) == gate_up(N=130) == gate_up(sn=1 << 22, N=1024, so=512) == 2
+    assert gate_up(a=None) == gate_up(out=None) == gate_up(offs=None) == gate_up(so=63) == gate_up(K=-1) == gate_up(N=-128) == 1 and gate_up(M=0) == 0
     assert mm(M=0, R=0, a=None) == mm(N=0, b=None) == mm(G=0, offs=p) == 0
 
 
 # ------------------------------------------------------------------ the tile
 def variants():
     return [waits.gen.Variant(0, 0, f32, tm, f16, b_nt, act) for f16, f32 in ((2, 0), (2, 1), (3, 0)) for tm in (4, 2, 1)
-            for b_nt, act in ((0, 0), (1, 0), (0, 2)) if not (b_nt and tm == 4) and not (act and not f32)]
+            for b_nt, act in ((0, 0), (1, 0), (0, 2), (0, 4), (1, 4)) if not (b_nt and tm == 4) and not (act and not f32)]
 
 
 @pytest.mark.parametrize("v", variants(), ids=lambda v: f"{v.name}_{v.out_f32}_{v.f16}")
@@ -186,7 +191,7 @@ def test_scales_lie_behind_all_buffers_and_registers(v):
     e = g.gen_variant(v)
     reads = [line for line in e.lines if line.startswith("ds_read") and (f"v{g.V_RA + 2}" in line.split() or f"v{g.V_RB + 2} " in line + " ")]
     epilogue = e.lines[e.lines.index("; ---- epilogue"):]
-    scaled = [line for line in epilogue if line.startswith("v_mul_f32")]
+    scaled = [line for line in epilogue if line.startswith("v_mul_f32") and 48 <= int(line.split()[2].strip("v,") if line.split()[2][0] == "v" else 0)]
     assert len(scaled) == (0 if v.partial else 2 * 4 * 8 * 2 * v.tm)
     used = {r for line in scaled for r in waits.regs(line.split()[2].rstrip(","))}
     assert not used or used == set(range(48, 80 + 2 * v.tm))
