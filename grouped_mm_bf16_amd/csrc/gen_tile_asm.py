@@ -59,8 +59,8 @@ Registers:
 
 8-bit integers (f16 = 2, 3): the same tile on v_mfma_i32_16x16x64_i8, whose fragments are 16 bytes of K to a lane as well.  Every
 offset, step and K tile is one of bytes, so nothing but the instruction differs in the loop; "64 k" above are 128 bytes, 128
-integers.  Both operands are contiguous along K.  The prologue also copies the scales of the tile's rows and columns into LDS, before
-everything else (its first wait covers them); the epilogue turns each sum into fp32 and multiplies it by its column's, then its row's: a
+integers.  Both operands are contiguous along K.  The wrapper has copies of the scales of the tile's rows and columns on their way into LDS
+before everything else (the first wait covers them, it counts the youngest); the epilogue turns each sum into fp32 and multiplies it by its column's, then its row's: a
 weight's scale is small, and what overflows in between would have overflowed anyway.
 """
 import sys
@@ -111,11 +111,8 @@ S_RA, S_RB, S_RC = 36, 40, 44   # buffer resources
 S_SC = 48                        # scalars s[48:55]
 S_NK, S_ASTEP, S_BSTEP, S_LDS, S_ROWCNT, S_CSTEP, S_NVALID, S_SPARE = range(48, 56)
 S_T = 56                         # temporaries s[56:79]
-# 8-bit integers: byte offsets of the scale that this lane copies, of a row and of a column (+0, +1), their buffer resources, and
-# where they lie in LDS: 256 of rows, 256 of columns, behind the buffers of all tile heights.  Their read addresses come in
-# the unused halves of the fragment addresses.
-V_SCALE = V_IN + 66
-S_RROWS, S_RCOLS = 92, 96
+# 8-bit integers: where the scales lie in LDS, 256 of rows, 256 of columns, behind the buffers of all tile heights.  Their read addresses
+# come in the unused halves of the fragment addresses.
 SCALES = 147456
 
 
@@ -416,13 +413,6 @@ def gen_main(v, e, L):
     e("s_add_u32 %s, %s, %s" % (sr(s_waveA), sr(s_waveA), sr(S_LDS)))
     e("s_mul_i32 %s, %s, %d" % (sr(s_waveB), sr(sT + 19), v.nb * (TR_BLOCK if v.b_tr else 1024)))
     e("s_add_u32 %s, %s, %s" % (sr(s_waveB), sr(s_waveB), sr(S_LDS)))
-    if v.i8 and not v.partial:
-        e("s_lshl_b32 %s, %s, 8" % (sr(s_t1), sr(sT + 19)))
-        e("s_add_u32 %s, %s, %s" % (sr(s_t1), sr(s_t1), sr(S_LDS)))
-        for k, res in enumerate((S_RROWS, S_RCOLS)):
-            e("s_add_u32 m0, %s, %d" % (sr(s_t1), SCALES + 1024 * k))
-            e("s_nop 0")
-            e("buffer_load_dword %s, %s, 0 offen lds" % (vr(V_SCALE + k), sr(res, 4)))
     # tile 0 -> buffer 0 (head offsets)
     for n in range(v.ncopy):
         for ins in m0_gaps(v.dma(n, 0, "head", 0, 0, s_zero, s_zero, V_TMP)):
@@ -831,11 +821,8 @@ def emit(out, v):
     pins = [(V_VOA_HEAD, 8, "voa_head"), (V_VOB_HEAD, 8, "vob_head"), (V_VOA, 8, "voa"), (V_VOB, 8, "vob"),
             (V_VOA_TAIL, 8, "voa_tail"), (V_VOB_TAIL, 8, "vob_tail"), (V_RA, 4, "ra_addr"), (V_RB, 4, "rb_addr"),
             (V_EPI, 4, "epi"), (V_EPI2, 2, "epi2"), (V_TOUCH, 2, "touch"), (V_FIX, 4, "fix")]
-    if v.i8:
-        pins.append((V_SCALE, 2, "scale"))
     out.append("      : " + ", ".join('"{v[%d:%d]}"(r.%s)' % (b0, b0 + n - 1, name) for b0, n, name in pins) + ",")
-    scales = ', "{s[%d:%d]}"(r.rsrc_rows), "{s[%d:%d]}"(r.rsrc_cols)' % (S_RROWS, S_RROWS + 3, S_RCOLS, S_RCOLS + 3) if v.i8 else ""
-    out.append('        "{s[28:35]}"(r.masks), "{s[36:39]}"(r.rsrc_a), "{s[40:43]}"(r.rsrc_b), "{s[44:47]}"(r.rsrc_c), "{s[48:55]}"(r.scal)' + scales)
+    out.append('        "{s[28:35]}"(r.masks), "{s[36:39]}"(r.rsrc_a), "{s[40:43]}"(r.rsrc_b), "{s[44:47]}"(r.rsrc_c), "{s[48:55]}"(r.scal)')
     out.append("      : %s);" % clobbers(v))
     out.append("}")
 

@@ -435,6 +435,7 @@ int gmm_int8_gate_up(const int8_t* a, const float* a_scale, const int32_t* row_i
   GmmInt8Params p;
   bool nothing = false;
   if (N >= 0 && (N & 127)) return GMM_ERR_UNSUPPORTED;
+  if (!offs && G > 0) return GMM_ERR_BAD_ARGUMENT;
   const int bad = int8_params(a, a_scale, row_index, b, b_scale, out, offs, G, a_rows, M, N, N / 2, K, a_stride, b_stride_g, b_stride_n, out_stride,
                               GMM_DT_F32, pr, p, nothing);
   if (bad || nothing) return bad;

@@ -214,9 +214,10 @@ __device__ __forceinline__ GmmTileDesc gmm_describe_tile(const P& p, const GmmTi
     dsc.b.bytes = (dsc.b.bytes + 15) & ~15LL;
     dsc.k_odd = p.k_odd && t.k_hi == p.K;
     dsc.row_scale = p.gather ? p.a_scale : p.a_scale + t.m0;
-    dsc.row_scales = p.gather ? p.a_rows : (p.jag == GMM_JAG_M ? t.m_hi : p.M) - t.m0;
+    // (of gathered rows all, fewer than 2^27, since their matrix is below 2 GiB)
+    dsc.row_scales = p.gather ? p.a_rows : gmm_min((p.jag == GMM_JAG_M ? t.m_hi : p.M) - t.m0, 256);
     dsc.col_scale = p.b_scale + int64_t(t.g) * p.N + b_n0;
-    dsc.col_scales = p.N - b_n0;
+    dsc.col_scales = APART ? p.N - b_n0 : gmm_min(p.N - b_n0, 256);
   }
   return dsc;
 }

@@ -51,7 +51,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   constexpr int N = kVector<T>;
 #pragma unroll
   for (int q = 0; q < 8 / N; ++q) {
-    const Pack<T, N> a = unaligned<Pack<T, N>>(p + q * N);
+    const Pack<T, N> a = stream_in<Pack<T, N>, true>(p + q * N);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[q * N + i] = a.get(i);
   }
@@ -65,8 +65,7 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     float part[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) part[i] = v[q * N + i];
-    const Pack<T, N> a = Pack<T, N>::of(part);
-    __builtin_memcpy(p + q * N, &a, sizeof(a));
+    stream_out<true>(p + q * N, Pack<T, N>::of(part));
   }
 }
 

@@ -62,6 +62,27 @@ __device__ __forceinline__ V unaligned(const void* p) {
   return v;
 }
 
+// What is read or written once, past the caches' way if STREAM (non-temporal): not for rows that end inside an access, whose last cache line two
+// lanes ask for, one after the other.
+template <typename V, bool STREAM>
+__device__ __forceinline__ V stream_in(const void* p) {
+  if constexpr (STREAM && sizeof(V) == 16) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+    return __builtin_bit_cast(V, u32x4(__builtin_nontemporal_load(static_cast<const Words*>(p))));
+  } else {
+    return unaligned<V>(p);
+  }
+}
+template <bool STREAM, typename V>
+__device__ __forceinline__ void stream_out(void* p, const V& v) {
+  if constexpr (STREAM && sizeof(V) == 16) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+    __builtin_nontemporal_store(Words(__builtin_bit_cast(u32x4, v)), static_cast<Words*>(p));
+  } else {
+    __builtin_memcpy(p, &v, sizeof(V));
+  }
+}
+
 template <typename T> constexpr int kVector = 16 / int(sizeof(T));
 
 // Eight (fp32: four) elements to an access, which may begin anywhere.  Where fewer are left in a row (TAIL) the last eight are loaded: `skip`

@@ -21,8 +21,6 @@ struct GmmTileRegs {
   gmm_v4i fix;                 // LDS addresses of this thread's row in the first / last k chunk (A, A, B, B)
   gmm_v8i masks;               // keep-masks of the first and of the last 16-byte k chunk
   gmm_v4i rsrc_a, rsrc_b, rsrc_c;
-  gmm_v2i scale;               // 8-bit integers: byte offset of the row's scale that this thread copies, of the column's
-  gmm_v4i rsrc_rows, rsrc_cols;
   gmm_v8i scal;                // nk, a_step, b_step, lds_base, row_cnt, c_step, (unused), wave | flags << 8
 };
 
@@ -85,6 +83,16 @@ __device__ __forceinline__ gmm_v4i gmm_make_rsrc(const void* p, long long bytes)
 }
 
 __device__ __forceinline__ int gmm_swz(int row) { return (row >> 1) & 7; }
+
+// 64 of `count` (below 2^29) words, one a lane, from memory to LDS at `to`; past the end zeros.  The tile's first barrier stands behind a wait for it: the counter that its
+// copies are waited for with runs out in the order of their issue.
+__device__ __forceinline__ void gmm_copy_scales(unsigned to, const float* from, int count, int offset) {
+  const unsigned long long at = (unsigned long long)from;
+  const gmm_v4i rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)at), __builtin_amdgcn_readfirstlane((int)(unsigned)(at >> 32)),
+                        __builtin_amdgcn_readfirstlane(count * 4), 0x00020000};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane((int)to)), "v"(offset), "s"(rsrc) : "memory");
+}
 
 // One operand of a tile.  `base` points at element (row 0 of the tile, k_begin) of the operand;
 // `ld` is the leading dimension in elements; `bytes` is the distance from `base` to the end of the
@@ -197,6 +205,16 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
   const int wm = wave & 1, wn = wave >> 1;
   const int nk = (t.klen + GMM_TILE_K - 1) / GMM_TILE_K;
   GmmTileRegs r;
+  unsigned scales = lds_base + GMM_TILE_SCALES;
+  asm volatile("" : "+s"(scales));
+  if constexpr (F16 >= 2 && ACT != 2) {
+    // one row's and one column's scale by each thread, straight into LDS
+    const int at = wave * 64 + lane;
+    int row = at;
+    if (t.a.gather) row = at < t.a.gather_n ? t.a.gather[at] : -1;
+    gmm_copy_scales(scales + wave * 256, t.row_scale, t.row_scales, row >= 0 && row < t.row_scales ? row * 4 : (int)GMM_OOB);
+    gmm_copy_scales(scales + 1024 + wave * 256, t.col_scale, t.col_scales, (APART ? gmm_apart_column(at, t.b.apart) : at) * 4);
+  }
   gmm_copy_offsets<A_TR, 2 * TM>(lane, wave, t.a, t.klen, t.khead, nk, r.voa_head, r.voa, r.voa_tail);
   gmm_copy_offsets<B_TR, 8, APART>(lane, wave, t.b, t.klen, t.khead, nk, r.vob_head, r.vob, r.vob_tail);
   // Fragment read addresses.  An MFMA fragment is 16 rows (or columns) x 32 k: lane l holds row l % 16,
@@ -223,6 +241,10 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
     } else if (sp == 0) {
       r.rb_addr[0] = lds_base + B_BASE + (4 * q + (ii >> 2)) * GMM_TILE_TR_BLOCK + (wn * 128 + 4 * (ii & 3)) * 2;
     }
+  }
+  if constexpr (F16 >= 2 && ACT != 2) {
+    r.ra_addr[2] = scales + wm * WROWS * 4 + ii * 4;
+    r.rb_addr[2] = scales + 1024 + wn * 512 + q * 16;
   }
   // Epilogue: the wave stages its block in LDS and reads it back row by row, 16 bytes per lane (see
   // gen_tile_asm.py).  ESZ bytes per element: a lane's chunk is NEL = 16 / ESZ columns, a row of the wave's
@@ -300,20 +322,6 @@ __device__ __forceinline__ void gmm_tile_compute(const GmmTileDesc& t, unsigned 
       r.masks[w] = __builtin_amdgcn_readfirstlane((int)(h0 | h1));
       r.masks[4 + w] = __builtin_amdgcn_readfirstlane((int)(t0 | t1));
     }
-  }
-  if constexpr (F16 >= 2 && ACT != 2) {
-    const int at = wave * 64 + lane;
-    int row = at;
-    if (t.a.gather) row = at < t.a.gather_n ? t.a.gather[at] : -1;
-    r.scale[0] = row >= 0 && row < t.row_scales ? row * 4 : (int)GMM_OOB;
-    r.scale[1] = (APART ? gmm_apart_column(at, t.b.apart) : at) * 4;
-    r.rsrc_rows = gmm_make_rsrc(t.row_scale, (long long)t.row_scales * 4);
-    r.rsrc_cols = gmm_make_rsrc(t.col_scale, (long long)t.col_scales * 4);
-    r.ra_addr[2] = lds_base + GMM_TILE_SCALES + (wm * WROWS + (lane & 15)) * 4;
-    r.rb_addr[2] = lds_base + GMM_TILE_SCALES + 1024 + (wn * 128 + 4 * (lane >> 4)) * 4;
-  } else if constexpr (F16 >= 2) {
-    r.scale = gmm_v2i{0, 0};
-    r.rsrc_rows = r.rsrc_cols = gmm_v4i{0, 0, 0, 0};
   }
   const int sc[8] = {nk, a_step, b_step, (int)lds_base, t.row_cnt, c_step, n_valid, wave | (flags << 8)};
 #pragma unroll

@@ -6,7 +6,11 @@
 //   route      w = softmax of the chosen logits, or of all:  dl[e] = p[e] ([e chosen] dw[e] - sum over the chosen of p dw)
 //   gated      out = g s(g) u,  s(g) = 1 / (1 + e^-g):  dg = dout u s(g) (1 + g (1 - s(g))),  du = dout g s(g)
 // Memory bounds all of them.  Everything goes token by token, not row by row: what a token has once (x, dout, the sums) is read or written
-// once, its choices' rows once each, and the sums over choices need no atomics.  16 bytes to an access, at any address.
+// once, its choices' rows once each, and the sums over choices need no atomics.  16 bytes to an access, at any address; what is read or written
+// once goes past the caches (below: without / with).
+//   16384 tokens, 8 of 128 experts, bf16 rows of 2048   sort 115 / 103 us (5.9 TB/s; its one read through them, past them 114), sums 120 / 98 (6.2),
+//                                                       combine's gradients 283 / 243 (4.7)
+//   16384 x 14336 bf16                                  activation 265 / 251 (5.6), its gradient 446 / 428 (5.5)
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -39,47 +43,60 @@ template <typename T> __device__ __forceinline__ const T* row_of(const void* bas
 }
 template <typename T> __device__ __forceinline__ T* row_of(void* base, int64_t row, int64_t stride) { return static_cast<T*>(base) + row * stride; }
 
-// N elements from chunk c on; the last chunk begins earlier where fewer are left, and two lanes then write the same values to the same place.
-template <typename T, int N>
+// N elements from chunk c on.  Where rows are no WHOLE number of accesses the last one begins earlier, and two lanes write the same values to the same
+// place.
+template <typename T, int N, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) sort_rows_kernel(const RowArgs a) {
   const int lane = threadIdx.x & (a.lanes - 1);
   const int64_t t = int64_t(blockIdx.x) * (kBlock / a.lanes) + threadIdx.x / a.lanes;
   if (t >= a.tokens) return;
   for (int c = lane * N; c < a.width; c += a.lanes * N) {
-    const int at = Chunk<N, true>(c, a.width).at;
+    const int at = Chunk<N, !WHOLE>(c, a.width).at;
     const Pack<T, N> v = unaligned<Pack<T, N>>(row_of<T>(a.x, t, a.x_stride) + at);
     for (int j = 0; j < a.top_k; ++j) {
       const int64_t r = a.token_rows[t * a.top_k + j];
-      if (r >= 0 && r < a.rows) __builtin_memcpy(row_of<T>(a.out, r, a.out_stride) + at, &v, sizeof(v));
+      if (r >= 0 && r < a.rows) stream_out<WHOLE>(row_of<T>(a.out, r, a.out_stride) + at, v);
     }
   }
 }
 
-template <typename T, int N>
+constexpr int kAtOnce = 8;      // choices whose rows are on their way together
+
+template <typename T, int N, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) sum_rows_kernel(const RowArgs a) {
   const int lane = threadIdx.x & (a.lanes - 1);
   const int64_t t = int64_t(blockIdx.x) * (kBlock / a.lanes) + threadIdx.x / a.lanes;
   if (t >= a.tokens) return;
   for (int c = lane * N; c < a.width; c += a.lanes * N) {
-    const int at = Chunk<N, true>(c, a.width).at;
+    const int at = Chunk<N, !WHOLE>(c, a.width).at;
     float s[N] = {};
-    for (int j = 0; j < a.top_k; ++j) {
-      const int64_t r = a.token_rows[t * a.top_k + j];
-      if (r < 0 || r >= a.rows) continue;
-      const float w = a.weight ? a.weight[t * a.top_k + j] : 1.0f;
-      const Pack<T, N> v = unaligned<Pack<T, N>>(row_of<T>(a.x, r, a.x_stride) + at);
+    for (int first = 0; first < a.top_k; first += kAtOnce) {
+      Pack<T, N> v[kAtOnce];
+      float w[kAtOnce];
+      bool in[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[i] += w * v.get(i);
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int64_t slot = t * a.top_k + min(first + j, a.top_k - 1), r = a.token_rows[slot];
+        in[j] = first + j < a.top_k && r >= 0 && r < a.rows;
+        w[j] = a.weight ? a.weight[slot] : 1.0f;
+        if (in[j]) v[j] = stream_in<Pack<T, N>, WHOLE>(row_of<T>(a.x, r, a.x_stride) + at);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (in[j])
+#pragma unroll
+          for (int i = 0; i < N; ++i) s[i] += w[j] * v[j].get(i);
     }
-    const Pack<T, N> v = Pack<T, N>::of(s);
-    __builtin_memcpy(row_of<T>(a.out, t, a.out_stride) + at, &v, sizeof(v));
+    stream_out<WHOLE>(row_of<T>(a.out, t, a.out_stride) + at, Pack<T, N>::of(s));
   }
 }
 
-// Up to 64 lanes to a token.  Eight choices at a time: their sums of products stay in registers over all of the row.
-template <typename T, int N>
+// The sums of products of kAtOnce choices stay in registers over all of the row, then go over its lanes; those of several waves meet in LDS.  A wave to
+// a token, its row in pieces, took 276 us where four waves take 243.
+template <typename T, int N, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) combine_backward_kernel(const RowArgs a) {
-  constexpr int J = 8;
+  constexpr int J = kAtOnce, WAVES = kBlock / 64;
+  __shared__ float dots[WAVES][J];
   const int lane = threadIdx.x & (a.lanes - 1);
   const int64_t t = int64_t(blockIdx.x) * (kBlock / a.lanes) + threadIdx.x / a.lanes;
   const bool live = t < a.tokens;
@@ -95,13 +112,13 @@ __global__ void __launch_bounds__(kBlock) combine_backward_kernel(const RowArgs 
       dot[j] = 0;
     }
     for (int c = lane * N; live && c < a.width; c += a.lanes * N) {
-      const Chunk<N, true> chunk(c, a.width);
-      const Pack<T, N> d = unaligned<Pack<T, N>>(row_of<T>(a.x, t, a.x_stride) + chunk.at);
+      const Chunk<N, !WHOLE> chunk(c, a.width);
+      const Pack<T, N> d = stream_in<Pack<T, N>, WHOLE>(row_of<T>(a.x, t, a.x_stride) + chunk.at);
       Pack<T, N> y[J];
       if (a.dweight)
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (row[j] >= 0) y[j] = unaligned<Pack<T, N>>(row_of<T>(a.y, row[j], a.y_stride) + chunk.at);
+          if (row[j] >= 0) y[j] = stream_in<Pack<T, N>, WHOLE>(row_of<T>(a.y, row[j], a.y_stride) + chunk.at);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         if (row[j] < 0) continue;
@@ -111,18 +128,29 @@ __global__ void __launch_bounds__(kBlock) combine_backward_kernel(const RowArgs 
           if (a.dweight) dot[j] += chunk.own(i) ? d.get(i) * y[j].get(i) : 0.0f;
           dy[i] = w[j] * d.get(i);
         }
-        if (a.out) {
-          const Pack<T, N> v = Pack<T, N>::of(dy);
-          __builtin_memcpy(row_of<T>(a.out, row[j], a.out_stride) + chunk.at, &v, sizeof(v));
-        }
+        if (a.out) stream_out<WHOLE>(row_of<T>(a.out, row[j], a.out_stride) + chunk.at, Pack<T, N>::of(dy));
       }
     }
     if (!a.dweight) continue;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      for (int o = a.lanes / 2; o > 0; o >>= 1) dot[j] += __shfl_xor(dot[j], o);
-      if (lane == 0 && live && first + j < a.top_k) a.dweight[t * a.top_k + first + j] = dot[j];
+    for (int j = 0; j < J; ++j)
+      for (int o = min(a.lanes, 64) / 2; o > 0; o >>= 1) dot[j] += __shfl_xor(dot[j], o);
+    if (a.lanes > 64) {      // the same for the whole workgroup
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int j = 0; j < J; ++j) dots[threadIdx.x >> 6][j] = dot[j];
+      __syncthreads();
+      const int waves = a.lanes / 64, wave0 = threadIdx.x / a.lanes * waves;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        dot[j] = 0;
+        for (int i = 0; i < waves; ++i) dot[j] += dots[wave0 + i][j];
+      }
     }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (lane == 0 && live && first + j < a.top_k) a.dweight[t * a.top_k + first + j] = dot[j];
   }
 }
 
@@ -160,8 +188,8 @@ __global__ void __launch_bounds__(kBlock) route_backward_kernel(const float* __r
     float p = 0, d = 0;
     bool chosen = false;
     for (int j = 0; j < k; ++j) {
-      const int ej = __shfl(mine, j);
-      const float wj = __shfl(w, j), gj = __shfl(g, j);
+      const int ej = __builtin_amdgcn_readlane(mine, j);
+      const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j)), gj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), j));
       if (ej == e) { p = wj; d = gj; chosen = true; }
     }
     if (e >= E) continue;
@@ -185,7 +213,7 @@ struct GatedArgs {
 // e^-g, accurate for fp32 values, the hardware's for 16-bit ones, whose rounding is 2^13 times as large.
 template <typename T> __device__ __forceinline__ float exp_minus(float g) { return sizeof(T) == 4 ? expf(-g) : __expf(-g); }
 
-template <typename T, int N, bool SWIGLU, bool BACK>
+template <typename T, int N, bool WHOLE, bool SWIGLU, bool BACK>
 __global__ void __launch_bounds__(kBlock) gated_kernel(const GatedArgs a) {
   const int lane = threadIdx.x & (a.lanes - 1);
   const int64_t r = int64_t(blockIdx.x) * (kBlock / a.lanes) + threadIdx.x / a.lanes;
@@ -193,11 +221,11 @@ __global__ void __launch_bounds__(kBlock) gated_kernel(const GatedArgs a) {
   const T* h = row_of<T>(a.h, r, a.h_stride);
   T* out = row_of<T>(a.out, r, a.out_stride);
   for (int c = lane * N; c < a.inner; c += a.lanes * N) {
-    const int at = Chunk<N, true>(c, a.inner).at;
-    const Pack<T, N> gate = unaligned<Pack<T, N>>(h + at);
+    const int at = Chunk<N, !WHOLE>(c, a.inner).at;
+    const Pack<T, N> gate = stream_in<Pack<T, N>, WHOLE>(h + at);
     Pack<T, N> up, d;
-    if constexpr (SWIGLU) up = unaligned<Pack<T, N>>(h + a.inner + at);
-    if constexpr (BACK) d = unaligned<Pack<T, N>>(row_of<T>(a.dout, r, a.dout_stride) + at);
+    if constexpr (SWIGLU) up = stream_in<Pack<T, N>, WHOLE>(h + a.inner + at);
+    if constexpr (BACK) d = stream_in<Pack<T, N>, WHOLE>(row_of<T>(a.dout, r, a.dout_stride) + at);
     float first[N], second[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -215,12 +243,8 @@ __global__ void __launch_bounds__(kBlock) gated_kernel(const GatedArgs a) {
         }
       }
     }
-    const Pack<T, N> v = Pack<T, N>::of(first);
-    __builtin_memcpy(out + at, &v, sizeof(v));
-    if constexpr (BACK && SWIGLU) {
-      const Pack<T, N> u = Pack<T, N>::of(second);
-      __builtin_memcpy(out + a.inner + at, &u, sizeof(u));
-    }
+    stream_out<WHOLE>(out + at, Pack<T, N>::of(first));
+    if constexpr (BACK && SWIGLU) stream_out<WHOLE>(out + a.inner + at, Pack<T, N>::of(second));
   }
 }
 
@@ -234,13 +258,14 @@ int lanes_for(int64_t chunks, int most) {
 
 bool stride_fits(int64_t stride, int64_t rows, int64_t width) { return stride >= width || rows <= 1; }
 
-// f(element type, elements to an access) for rows of `width` elements.
+// f(element type, elements to an access, whether rows are whole numbers of them) for rows of `width` elements.
 template <typename F>
 int by_type(int32_t dtype, int64_t width, F&& f) {
   const auto go = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (width >= kVector<T>) f(t, std::integral_constant<int, kVector<T>>{});
-    else f(t, std::integral_constant<int, 1>{});
+    if (width >= kVector<T> && width % kVector<T> == 0) f(t, std::integral_constant<int, kVector<T>>{}, std::true_type{});
+    else if (width >= kVector<T>) f(t, std::integral_constant<int, kVector<T>>{}, std::false_type{});
+    else f(t, std::integral_constant<int, 1>{}, std::false_type{});
   };
   if (dtype == GMM_DT_BF16) go(static_cast<Bf16*>(nullptr));
   else if (dtype == GMM_DT_F16) go(static_cast<F16*>(nullptr));
@@ -267,16 +292,17 @@ int gated(GatedArgs a, int64_t inner, int32_t kind, int32_t dtype, void* stream)
       (a.dout && !stride_fits(a.dout_stride, a.rows, inner))) return GMM_ERR_BAD_ARGUMENT;
   a.inner = int32_t(inner);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return by_type(dtype, inner, [&](auto* t, auto n) {
+  return by_type(dtype, inner, [&](auto* t, auto n, auto whole) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = decltype(n)::value;
+    constexpr bool WHOLE = decltype(whole)::value;
     GatedArgs b = a;
     b.lanes = lanes_for((inner + N - 1) / N, kBlock);
     const dim3 grid(groups_of(a.rows, b.lanes)), block(kBlock);
-    if (a.dout && parts == 2) hipLaunchKernelGGL((gated_kernel<T, N, true, true>), grid, block, 0, s, b);
-    else if (a.dout) hipLaunchKernelGGL((gated_kernel<T, N, false, true>), grid, block, 0, s, b);
-    else if (parts == 2) hipLaunchKernelGGL((gated_kernel<T, N, true, false>), grid, block, 0, s, b);
-    else hipLaunchKernelGGL((gated_kernel<T, N, false, false>), grid, block, 0, s, b);
+    if (a.dout && parts == 2) hipLaunchKernelGGL((gated_kernel<T, N, WHOLE, true, true>), grid, block, 0, s, b);
+    else if (a.dout) hipLaunchKernelGGL((gated_kernel<T, N, WHOLE, false, true>), grid, block, 0, s, b);
+    else if (parts == 2) hipLaunchKernelGGL((gated_kernel<T, N, WHOLE, true, false>), grid, block, 0, s, b);
+    else hipLaunchKernelGGL((gated_kernel<T, N, WHOLE, false, false>), grid, block, 0, s, b);
   });
 }
 
@@ -293,11 +319,12 @@ int gmm_moe_sort_rows(const void* x, const int32_t* token_rows, void* out, int64
   RowArgs a{};
   a.x = x; a.out = out; a.token_rows = token_rows; a.tokens = tokens; a.rows = out_rows; a.x_stride = x_stride; a.out_stride = out_stride;
   a.top_k = int32_t(top_k); a.width = int32_t(hidden);
-  return by_type(dtype, hidden, [&](auto* t, auto n) {
+  return by_type(dtype, hidden, [&](auto* t, auto n, auto whole) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = decltype(n)::value;
+    constexpr bool WHOLE = decltype(whole)::value;
     a.lanes = lanes_for((hidden + N - 1) / N, kBlock);
-    hipLaunchKernelGGL((sort_rows_kernel<T, N>), dim3(groups_of(tokens, a.lanes)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL((sort_rows_kernel<T, N, WHOLE>), dim3(groups_of(tokens, a.lanes)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
   });
 }
 
@@ -310,11 +337,12 @@ int gmm_moe_sum_rows(const void* y, const int32_t* token_rows, const float* slot
   RowArgs a{};
   a.x = y; a.out = out; a.token_rows = token_rows; a.weight = slot_weight; a.tokens = tokens; a.rows = y_rows; a.x_stride = y_stride;
   a.out_stride = out_stride; a.top_k = int32_t(top_k); a.width = int32_t(hidden);
-  return by_type(dtype, hidden, [&](auto* t, auto n) {
+  return by_type(dtype, hidden, [&](auto* t, auto n, auto whole) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = decltype(n)::value;
+    constexpr bool WHOLE = decltype(whole)::value;
     a.lanes = lanes_for((hidden + N - 1) / N, kBlock);
-    hipLaunchKernelGGL((sum_rows_kernel<T, N>), dim3(groups_of(tokens, a.lanes)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL((sum_rows_kernel<T, N, WHOLE>), dim3(groups_of(tokens, a.lanes)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
   });
 }
 
@@ -330,11 +358,12 @@ int gmm_moe_combine_backward(const void* dout, const void* y, const int32_t* tok
   RowArgs a{};
   a.x = dout; a.y = y; a.out = dy; a.token_rows = token_rows; a.weight = slot_weight; a.dweight = dweight; a.tokens = tokens; a.rows = y_rows;
   a.x_stride = dout_stride; a.y_stride = y_stride; a.out_stride = dy_stride; a.top_k = int32_t(top_k); a.width = int32_t(hidden);
-  return by_type(dtype, hidden, [&](auto* t, auto n) {
+  return by_type(dtype, hidden, [&](auto* t, auto n, auto whole) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = decltype(n)::value;
-    a.lanes = lanes_for((hidden + N - 1) / N, 64);
-    hipLaunchKernelGGL((combine_backward_kernel<T, N>), dim3(groups_of(tokens, a.lanes)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
+    constexpr bool WHOLE = decltype(whole)::value;
+    a.lanes = lanes_for((hidden + N - 1) / N, kBlock);
+    hipLaunchKernelGGL((combine_backward_kernel<T, N, WHOLE>), dim3(groups_of(tokens, a.lanes)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
   });
 }
 

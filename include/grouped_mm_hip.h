@@ -338,7 +338,7 @@ int gmm_int8_mm(const int8_t* a, const float* a_scale, const int32_t* row_index,
                 int64_t b_stride_n, int64_t out_stride, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*   gmm_int8_gate_up   silu(first half of the columns) * second half of gmm_int8_mm's result in fp32, never stored as a whole: out float [M, N / 2].
- *                      N a multiple of 128 (else GMM_ERR_UNSUPPORTED, also where half a matrix reaches 2 GiB). */
+ *                      N a multiple of 128 (else GMM_ERR_UNSUPPORTED, also where half a matrix reaches 2 GiB), offs not NULL. */
 int gmm_int8_gate_up(const int8_t* a, const float* a_scale, const int32_t* row_index, const int8_t* b, const float* b_scale, float* out,
                      const int32_t* offs, int32_t G, int64_t a_rows, int64_t M, int64_t N, int64_t K, int64_t a_stride, int64_t b_stride_g,
                      int64_t b_stride_n, int64_t out_stride, void* stream);
