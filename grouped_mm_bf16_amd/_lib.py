@@ -58,7 +58,7 @@ SIGNATURES = {
     "gmm_int8_gated": (ctypes.c_int, [_vp] * 3 + [_i64] * 4 + [_i32, _vp]),
     "gmm_int8_mm": (ctypes.c_int, [_vp] * 7 + [_i32] + [_i64] * 8 + [_i32, _vp, _i64, _vp]),
     "gmm_int8_gate_up": (ctypes.c_int, [_vp] * 7 + [_i32] + [_i64] * 8 + [_vp]),
-    "gmm_int8_linear_workspace_bytes": (_i64, [_i64] * 3),
+    "gmm_int8_linear_workspace_bytes": (_i64, [_i64] * 3 + [_i32]),
     "gmm_int8_linear": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp, _i64, _vp]),
     "gmm_int8_moe_few_workspace_bytes": (_i64, [_i64] * 5 + [_i32]),
     "gmm_int8_moe_few": (ctypes.c_int, [_vp] * 7 + [_i64] * 12 + [_i32] * 4 + [_vp, _i64, _vp]),

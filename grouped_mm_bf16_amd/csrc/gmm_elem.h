@@ -100,6 +100,24 @@ struct Chunk {
   __device__ __forceinline__ bool own(int i) const { return in && (!TAIL || i >= skip); }
 };
 
+// Scale of a row that becomes 8-bit integers, from its largest magnitude as bits (NaN and infinities are above all others).
+struct RowScale {
+  bool finite;
+  float scale, inverse;
+  __device__ __forceinline__ explicit RowScale(uint32_t most) {
+    const float largest = __uint_as_float(most);
+    finite = most < 0x7f800000u;
+    scale = (largest < 0x1p-100f ? 0x1p-100f : largest) / 127.0f;
+    inverse = finite ? 1.0f / scale : 0.0f;
+  }
+  // x / scale to the nearest fp32 value: the reciprocal's product, corrected by its residual.  Adding 1.5 * 2^23 rounds to a whole number, whose two's
+  // complement the low bits then are.
+  __device__ __forceinline__ uint32_t rounded_bits(float x) const {
+    const float q = x * inverse;
+    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, scale, x), inverse, q) + 12582912.0f) & 0xffu;
+  }
+};
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace gmm

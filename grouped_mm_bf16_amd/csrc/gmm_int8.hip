@@ -18,7 +18,6 @@ using namespace gmm;
 
 constexpr int kSpan = 16;      // elements that a lane turns into one store of 16 bytes
 constexpr int kGroup = 256;
-constexpr float kSmallest = 0x1p-100f;
 
 struct QuantArgs {
   const void* x;
@@ -121,16 +120,8 @@ __global__ void __launch_bounds__(kGroup) quantize_kernel(const QuantArgs a) {
     for (int w = 0; w < WAVES; ++w) most = max(most, slots[w]);
   }
   if (!live) return;
-  const bool finite = most < 0x7f800000u;
-  const float largest = __uint_as_float(most), scale = (largest < kSmallest ? kSmallest : largest) / 127.0f;
-  const float inverse = finite ? 1.0f / scale : 0.0f;
-  if (lane == 0) a.scale[r] = scale;
-  // x / scale to the nearest fp32 value: the reciprocal's product, corrected by its residual.  Adding 1.5 * 2^23 rounds to a whole number, whose two's
-  // complement the low bits then are.
-  const auto rounded_bits = [&](float x) {
-    const float q = x * inverse;
-    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, scale, x), inverse, q) + 12582912.0f) & 0xffu;
-  };
+  const RowScale s(most);
+  if (lane == 0) a.scale[r] = s.scale;
   int8_t* const to = a.values + r * a.values_stride;
   const auto store = [&](int c, const float (&f)[kSpan]) {
     u32x4 w;
@@ -138,8 +129,8 @@ __global__ void __launch_bounds__(kGroup) quantize_kernel(const QuantArgs a) {
     for (int q = 0; q < 4; ++q) {
       w[q] = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[q] |= rounded_bits(f[4 * q + i]) << 8 * i;
-      if (!finite) w[q] = 0;
+      for (int i = 0; i < 4; ++i) w[q] |= s.rounded_bits(f[4 * q + i]) << 8 * i;
+      if (!s.finite) w[q] = 0;
     }
     *reinterpret_cast<u32x4*>(to + c) = w;
   };

@@ -4,6 +4,7 @@
 //   one matrix        parts are planes of integer sums, which a second kernel adds up and scales: exact, as in one part
 //   expert layer      route, rows of x to 8 bits, first product, activation to 8 bits, second product, sum over choices and parts.  The planes
 //                     between its launches are scaled fp32 values; SwiGLU is computed by the first product where k is in one part
+// Of a few short rows every workgroup makes the 8-bit ones itself, while its first weights are on their way (rounds_here): a launch less.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -37,7 +38,10 @@ struct FewArgs {
   int32_t used, most;         // groups that can have rows; rows that a group can have, 64 at most
   int32_t columns, tiles, parts, k_part;      // of a strip (with its partners); strips; parts along k and their length
   int32_t result, out_dtype;
+  int32_t x_dtype;            // of rows that are rounded here: a is x, a_ld its elements from one row to the next
 };
+
+constexpr int kNotRounded = -1;
 
 // The `which`-th group that has rows, found by every wave for itself.
 __device__ __forceinline__ bool find_group(const FewArgs& a, int which, int& g, int& row0, int& rows) {
@@ -82,12 +86,92 @@ __device__ __forceinline__ float scaled(int sum, float column, float row) {
   return v;
 }
 
+// Eight values of x to an access, so many accesses to a thread, as many elements of all rows as leave LDS for other workgroups.
+template <typename X> constexpr int kAccesses = sizeof(X) == 2 ? 8 : 4;
+constexpr int64_t kMostRounded = 16384;
+
+// Rows of x that a workgroup rounds for itself, as gmm_int8_quantize does.
+template <typename X, int WAVES>
+struct RowsHere {
+  static constexpr int THREADS = 64 * WAVES, N = kAccesses<X>;
+  Pack<X, kVector<X>> v[N][8 / kVector<X>];
+
+  // f(access, row, column of the first of eight elements, how many of them are the one before's) for the thread's accesses.
+  template <typename F>
+  static __device__ __forceinline__ void each(int rows, int K, F&& f) {
+    const int per_row = (K + 7) / 8;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = int(threadIdx.x) + i * THREADS, r = at / per_row;
+      if (r >= rows) break;
+      const Chunk<8, true> c((at - r * per_row) * 8, K);
+      f(i, r, c.at, c.skip);
+    }
+  }
+
+  // row(r): where row r of x is, null: zeros.
+  template <typename R>
+  __device__ __forceinline__ void load(int rows, int K, R&& row) {
+    each(rows, K, [&](int i, int r, int c, int) {
+      const X* from = row(r);
+#pragma unroll
+      for (int q = 0; q < 8 / kVector<X>; ++q)
+        if (from) v[i][q] = unaligned<Pack<X, kVector<X>>>(from + c + q * kVector<X>);
+    });
+  }
+
+  // Into LDS, row r from to + r * pitch on, and the scales.  All threads; ends with a barrier.  most[]: zeros, behind a barrier.
+  template <typename R>
+  __device__ __forceinline__ void round(int rows, int K, R&& row, char* to, int pitch, uint32_t* most, float* scale) {
+    const int lane = threadIdx.x & 63;
+    each(rows, K, [&](int i, int r, int, int) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) m = max(m, __float_as_uint(v[i][q / kVector<X>].get(q % kVector<X>)) & 0x7fffffffu);
+      if (!row(r)) m = 0;
+      // one row in all of the wave's lanes: they have one maximum
+      if (__all(r == __builtin_amdgcn_readfirstlane(r)) && __popcll(__ballot(1)) == 64) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = max(m, uint32_t(__shfl_xor(int(m), o)));
+        if (lane == 0) atomicMax(&most[r], m);
+      } else {
+        atomicMax(&most[r], m);
+      }
+    });
+    __syncthreads();
+    each(rows, K, [&](int i, int r, int c, int skip) {
+      const uint32_t bits = most[r];
+      const RowScale s(bits);
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) w[q / 4] |= s.rounded_bits(v[i][q / kVector<X>].get(q % kVector<X>)) << q % 4 * 8;
+      if (!s.finite || !row(r)) w[0] = w[1] = 0;
+      if (skip == 0) *reinterpret_cast<uint2*>(to + r * pitch + c) = make_uint2(w[0], w[1]);
+      else
+#pragma unroll
+        for (int q = 1; q < 8; ++q) if (q >= skip) to[r * pitch + c + q] = char(w[q / 4] >> q % 4 * 8);
+    });
+    if (int(threadIdx.x) < rows) scale[threadIdx.x] = row(threadIdx.x) ? RowScale(most[threadIdx.x]).scale : 0.0f;
+    __syncthreads();
+  }
+};
+
 // FR: a strip is 16 FR columns.  GLU: half of them gate columns, the others their partners, N / 2 further on; the result is silu(gate) * partner.
-template <int MF, int FR, int WAVES, bool GLU>
+// X: the rows are values of this type, rounded here (up to 16 of them, k in one part); void: 8-bit integers.
+template <typename X, int MF, int FR, int WAVES, bool GLU>
 __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int8_few_kernel(const FewArgs a) {
-  using S = Skinny<I8x2, GMM_W_COLS, FR, MF, 1, GMM_A_STAGED, 2>;
+  constexpr bool HERE = !std::is_void_v<X>;
+  static_assert(!HERE || MF == 1, "");
+  using S = Skinny<I8x2, GMM_W_COLS, FR, MF, 1, HERE ? GMM_A_RESIDENT : GMM_A_STAGED, 2>;
   constexpr int OUT = GLU ? 8 * FR : 16 * FR, THREADS = 64 * WAVES;
   __shared__ SkinnyShared<S, WAVES> shared;
+  extern __shared__ __align__(16) char rows_here[];      // HERE: 8-bit rows
+  __shared__ uint32_t most_here[16];
+  __shared__ float scale_here[16];
+  if constexpr (HERE) {
+    if (threadIdx.x < 16) most_here[threadIdx.x] = 0;
+    __syncthreads();
+  }
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
   int g = 0, row0 = 0, rows = a.M;
   if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) return;
@@ -97,7 +181,6 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   s.lane = lane;
   s.lds = shared.wave[wave];
   s.w_buf = buffer(static_cast<const uint16_t*>(a.b) + g * a.b_sg, a.b_bytes);
-  s.a_buf = buffer(a.a, a.a_bytes);
   s.a_plane = 0;
   if constexpr (GLU) s.set_columns(first, width - first, 1, uint32_t(a.b_ld), OUT, width + first);
   else s.set_columns(first, width - first, 1, uint32_t(a.b_ld));
@@ -106,13 +189,31 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
     const int at = a.row_index ? a.row_index[row0 + r] : row0 + r;
     return uint32_t(at) < uint32_t(a.a_rows) ? at : -1;
   };
-  s.set_rows([&](int r) {
-    const int at = r < rows ? source(r) : -1;
-    return at < 0 ? kNowhere : uint32_t(at) * uint32_t(a.a_ld) * 2;
-  });
   f32x4 acc[MF][FR];
   clear(acc);
-  s.template run<WAVES>(rows, part * a.k_part, min(a.K, (part + 1) * a.k_part), wave, acc);
+  if constexpr (HERE) {
+    const auto row = [&](int r) {
+      const int at = source(r);
+      return at < 0 ? static_cast<const X*>(nullptr) : static_cast<const X*>(a.a) + at * a.a_ld;
+    };
+    RowsHere<X, WAVES> x;
+    typename S::Step step[S::STEPS];
+    s.pitch = (a.K * 2 + 31) & ~15;      // rows in other banks
+    s.resident = rows_here;
+    s.resident_k = 0;
+    s.resident_rows = rows;
+    x.load(rows, 2 * a.K, row);
+    s.template prime<1, WAVES>(step, wave * S::KS, a.K);
+    x.round(rows, 2 * a.K, row, rows_here, s.pitch, most_here, scale_here);
+    s.template primed<1, WAVES>(step, wave * S::KS, a.K, acc);
+  } else {
+    s.a_buf = buffer(a.a, a.a_bytes);
+    s.set_rows([&](int r) {
+      const int at = r < rows ? source(r) : -1;
+      return at < 0 ? kNowhere : uint32_t(at) * uint32_t(a.a_ld) * 2;
+    });
+    s.template run<WAVES>(rows, part * a.k_part, min(a.K, (part + 1) * a.k_part), wave, acc);
+  }
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     if (16 * m >= rows) break;
@@ -134,8 +235,13 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
           static_cast<int32_t*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = h[v];
           continue;
         }
-        const int from = source(r);
-        const float rs = from < 0 ? 0.0f : a.a_scale[from];
+        float rs;
+        if constexpr (HERE) {
+          rs = scale_here[r];
+        } else {
+          const int from = source(r);
+          rs = from < 0 ? 0.0f : a.a_scale[from];
+        }
         const float f = scaled(h[v], cs, rs);
         if constexpr (GLU) {
           static_cast<float*>(a.out)[row * width + col] = f / (1.0f + __expf(-f)) * scaled(partner[v], ps, rs);
@@ -224,6 +330,7 @@ FewArgs from_params(const GmmInt8Params& p) {
   a.a = p.a; a.b = p.b; a.a_scale = p.a_scale; a.b_scale = p.b_scale; a.offs = p.jag == GMM_JAG_M ? p.offs : nullptr; a.row_index = p.gather;
   a.out = p.c; a.a_ld = p.a_sm; a.b_sg = p.b_sg; a.b_ld = p.b_sn; a.out_ld = p.c_sm;
   a.G = p.G; a.M = p.M; a.N = p.N; a.K = p.K; a.a_rows = p.gather ? p.a_rows : p.M;
+  a.x_dtype = kNotRounded;
   a.used = a.offs ? gmm_min(p.G, p.M) : 1;
   a.most = p.M;
   set_shape(a, few_shape(a.used, a.most, a.N, a.K));
@@ -237,23 +344,43 @@ bool sizes_fit(FewArgs& a) {
   return a.K >= 8 && a.b_bytes != 0;
 }
 
-template <bool GLU>
-int launch(const FewArgs& a, hipStream_t stream) {
+// Are the rows rounded by every workgroup for itself?  1 x 4096 x 4096 with its rounding XX us, in a launch of its own XX.
+bool rounds_here(int64_t rows, int64_t K, const Shape& s, int32_t x_dtype) {
+  const int64_t threads = s.columns == 64 ? 256 : s.columns == 32 ? 512 : 1024, each = x_dtype == GMM_DT_F32 ? kAccesses<float> : kAccesses<Bf16>;
+  return rows <= 16 && s.parts == 1 && rows * K <= kMostRounded && rows * ((K + 7) / 8) <= threads * each;
+}
+
+template <typename X, bool GLU>
+int launch_rows(const FewArgs& a, hipStream_t stream) {
+  constexpr bool HERE = !std::is_void_v<X>;
   const dim3 grid(unsigned(int64_t(a.used) * a.tiles * a.parts));
+  const int lds = HERE ? a.most * ((a.K * 2 + 31) & ~15) : 0;
   const auto go = [&](auto mf, auto fr, auto waves) {
     constexpr int MF = decltype(mf)::value, FR = decltype(fr)::value, WAVES = decltype(waves)::value;
-    hipLaunchKernelGGL((int8_few_kernel<MF, FR, WAVES, GLU>), grid, dim3(64 * WAVES), 0, stream, a);
+    hipLaunchKernelGGL((int8_few_kernel<X, MF, FR, WAVES, GLU>), grid, dim3(64 * WAVES), lds, stream, a);
   };
   const auto by_rows = [&](auto fr, auto waves) {
-    if (a.most <= 16) go(std::integral_constant<int, 1>{}, fr, waves);
-    else if (a.most <= 32) go(std::integral_constant<int, 2>{}, fr, waves);
-    else if (a.most <= 48) go(std::integral_constant<int, 3>{}, fr, waves);
-    else go(std::integral_constant<int, 4>{}, fr, waves);
+    if constexpr (!HERE) {
+      if (a.most > 48) return go(std::integral_constant<int, 4>{}, fr, waves);
+      if (a.most > 32) return go(std::integral_constant<int, 3>{}, fr, waves);
+      if (a.most > 16) return go(std::integral_constant<int, 2>{}, fr, waves);
+    }
+    go(std::integral_constant<int, 1>{}, fr, waves);
   };
   if (a.columns == 64) by_rows(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
   else if (a.columns == 32) by_rows(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
   else go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
   return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+}
+
+template <bool GLU>
+int launch(const FewArgs& a, hipStream_t stream) {
+  if (a.x_dtype == GMM_DT_BF16) return launch_rows<Bf16, GLU>(a, stream);
+  if (a.x_dtype == GMM_DT_F16) return launch_rows<F16, GLU>(a, stream);
+  if constexpr (!GLU) {
+    if (a.x_dtype == GMM_DT_F32) return launch_rows<float, GLU>(a, stream);
+  }
+  return launch_rows<void, GLU>(a, stream);
 }
 
 }  // namespace
@@ -292,15 +419,17 @@ int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_byt
 namespace {
 
 // ---------------------------------------------------------------- linear layer
-struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; };
+struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; bool here; };
 
-bool plan_linear(int64_t T, int64_t K, int64_t N, LinearPlan& p) {
+bool plan_linear(int64_t T, int64_t K, int64_t N, int32_t dtype, LinearPlan& p) {
   if (T < 0 || T > kMaxTokens || K < 0 || K >= 131072 || N < 0 || N >= (int64_t(1) << 31)) return false;
-  const int64_t parts = few_shape(1, T, N, K / 2).parts;
+  const Shape shape = few_shape(1, T, N, K / 2);
+  const int64_t parts = shape.parts;
+  p.here = rounds_here(T, K, shape, dtype);
   p.pitch = round_up(K > 0 ? K : 1, 16);
   p.scale_at = T * p.pitch;
   p.planes_at = round_up(p.scale_at + 4 * T, 16);
-  p.bytes = p.planes_at + (parts > 1 ? parts * T * N * 4 : 0);
+  p.bytes = p.here ? 0 : p.planes_at + (parts > 1 ? parts * T * N * 4 : 0);
   return true;
 }
 
@@ -310,6 +439,7 @@ struct LayerPlan {
   int64_t table_at, x_at, x_scale_at, h_at, act_at, act_scale_at, y_at, bytes;
   Shape up, down;
   bool activated;      // by the first product
+  bool x_here, act_here;      // rows that the products round themselves
 };
 
 bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t kind, LayerPlan& p) {
@@ -322,6 +452,8 @@ bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t k
   p.up = few_shape(p.used, T, N, H / 2);
   p.down = few_shape(p.used, T, H, I / 2);
   p.activated = p.up.parts == 1 && kind == GMM_ACT_SWIGLU;
+  p.x_here = rounds_here(T, H, p.up, GMM_DT_BF16);
+  p.act_here = p.activated && rounds_here(T, I, p.down, GMM_DT_F32);
   p.x_pitch = round_up(H, 16);
   p.act_pitch = round_up(I, 16);
   int64_t at = 0;
@@ -346,19 +478,19 @@ bool lies(const void* p, int64_t stride, int64_t width, int64_t count) {
 
 extern "C" {
 
-int64_t gmm_int8_linear_workspace_bytes(int64_t rows, int64_t K, int64_t N) {
+int64_t gmm_int8_linear_workspace_bytes(int64_t rows, int64_t K, int64_t N, int32_t dtype) {
   LinearPlan p;
-  return plan_linear(rows, K, N, p) ? p.bytes : -1;
+  return plan_linear(rows, K, N, dtype, p) ? p.bytes : -1;
 }
 
 int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* out, int64_t rows, int64_t K, int64_t N, int64_t x_stride,
                     int64_t b_stride_n, int64_t out_stride, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   LinearPlan plan;
   if (rows < 0 || K < 0 || N < 0) return GMM_ERR_BAD_ARGUMENT;
-  if (dtype < GMM_DT_BF16 || dtype > GMM_DT_F32 || !plan_linear(rows, K, N, plan) || (K & 1) || K < 16) return GMM_ERR_UNSUPPORTED;
+  if (dtype < GMM_DT_BF16 || dtype > GMM_DT_F32 || !plan_linear(rows, K, N, dtype, plan) || (K & 1) || K < 16) return GMM_ERR_UNSUPPORTED;
   if (rows == 0 || N == 0) return GMM_OK;
   if (!x || !b || !b_scale || !out || (rows > 1 && (x_stride < K || out_stride < N)) || !lies(b, b_stride_n, K, N)) return GMM_ERR_BAD_ARGUMENT;
-  if (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)) return GMM_ERR_WORKSPACE;
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace))) return GMM_ERR_WORKSPACE;
   char* const ws = static_cast<char*>(workspace);
   GmmInt8Params p{};
   p.a = ws; p.b = b; p.c = out; p.G = 1; p.jag = GMM_JAG_NONE; p.M = int32_t(rows); p.N = int32_t(N); p.K = int32_t(K / 2);
@@ -366,6 +498,11 @@ int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* 
   p.a_scale = reinterpret_cast<float*>(ws + plan.scale_at);
   p.b_scale = b_scale;
   if (!gmm_int8_few_preferred(p)) return GMM_ERR_UNSUPPORTED;
+  if (plan.here) {
+    FewArgs f = from_params(p);
+    f.a = x; f.a_ld = rows > 1 ? x_stride : K; f.x_dtype = dtype; f.out_dtype = dtype; f.result = kOut;
+    return sizes_fit(f) ? launch<false>(f, static_cast<hipStream_t>(stream)) : GMM_ERR_UNSUPPORTED;
+  }
   const int rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws), reinterpret_cast<float*>(ws + plan.scale_at), rows, K, x_stride, plan.pitch,
                                    dtype, stream);
   return rc == GMM_OK ? gmm_launch_int8_few(p, ws + plan.planes_at, plan.bytes - plan.planes_at, dtype, static_cast<hipStream_t>(stream)) : rc;
@@ -405,6 +542,8 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   u.b = w_up; u.b_scale = up_scale; u.b_sg = up_stride_g / 2; u.b_ld = up_stride_n / 2; u.offs = offs; u.out = ws + p.h_at;
   u.G = int32_t(experts); u.M = int32_t(p.slots); u.N = int32_t(N); u.K = int32_t(hidden / 2); u.used = int32_t(p.used);
   u.most = int32_t(tokens);      // a token chooses an expert once
+  u.x_dtype = kNotRounded;
+  if (p.x_here) { u.a = x; u.a_ld = tokens > 1 ? x_stride : hidden; u.x_dtype = dtype; }
   set_shape(u, p.up, p.activated);
   u.result = p.activated ? kActivated : kScaled;
   FewArgs d{};
@@ -412,6 +551,8 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   d.b = w_down; d.b_scale = down_scale; d.b_sg = down_stride_g / 2; d.b_ld = down_stride_n / 2; d.offs = offs; d.out = ws + p.y_at;
   d.G = int32_t(experts); d.M = int32_t(p.slots); d.N = int32_t(hidden); d.K = int32_t(inner / 2); d.used = int32_t(p.used);
   d.most = int32_t(tokens);
+  d.x_dtype = kNotRounded;
+  if (p.act_here) { d.a = ws + p.h_at; d.a_ld = inner; d.x_dtype = GMM_DT_F32; }
   set_shape(d, p.down);
   d.result = kScaled;
   if (!sizes_fit(u) || !sizes_fit(d)) return GMM_ERR_UNSUPPORTED;
@@ -419,9 +560,9 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
 
   int rc = gmm_moe_route(logits, tokens > 1 ? logits_stride : experts, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert, slot_weight,
                          row_token, token_rows, ws + p.table_at, p.table_bytes, stream);
-  if (rc == GMM_OK) rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws + p.x_at), at(p.x_scale_at), tokens, hidden, x_stride, p.x_pitch, dtype, stream);
+  if (rc == GMM_OK && !p.x_here) rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws + p.x_at), at(p.x_scale_at), tokens, hidden, x_stride, p.x_pitch, dtype, stream);
   if (rc == GMM_OK) rc = p.activated ? launch<true>(u, s) : launch<false>(u, s);
-  if (rc == GMM_OK)
+  if (rc == GMM_OK && !p.act_here)
     rc = p.activated ? gmm_int8_quantize(ws + p.h_at, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots, inner, inner, p.act_pitch,
                                          GMM_DT_F32, stream)
                      : gmm_int8_gated_parts(at(p.h_at), p.up.parts, p.slots * N, reinterpret_cast<int8_t*>(ws + p.act_at), at(p.act_scale_at), p.slots,

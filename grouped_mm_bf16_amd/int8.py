@@ -37,8 +37,8 @@ FEW_ROWS = 64        # up to which weights are streamed past the rows, not tiled
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_bytes(device: int, T: int, K: int, N: int) -> int:
-    return _lib.load().gmm_int8_linear_workspace_bytes(T, K, N)
+def _linear_bytes(device: int, T: int, K: int, N: int, code: int) -> int:
+    return _lib.load().gmm_int8_linear_workspace_bytes(T, K, N, code)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -233,10 +233,11 @@ def _linear_now(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor) -> t
         b = _aligned(values.t())
         out = torch.empty(T, N, device=x.device, dtype=x.dtype)
         with _guard(x):
-            nbytes = _linear_bytes(x.device.index, T, K, N)
-            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            code = _dtype_code(x.dtype)
+            nbytes = _linear_bytes(x.device.index, T, K, N, code)
+            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes > 0 else None
             rc = _lib.load().gmm_int8_linear(x.data_ptr(), b.data_ptr(), scale.data_ptr(), out.data_ptr(), T, K, N, x.stride(0),
-                                             b.stride(0) if N > 1 else _pitch(K), N, _dtype_code(x.dtype), ws.data_ptr(), nbytes,
+                                             b.stride(0) if N > 1 else _pitch(K), N, code, None if ws is None else ws.data_ptr(), nbytes,
                                              kernels.current_stream(x.device))
         if rc != _lib.ERR_UNSUPPORTED:
             _lib.check(rc, "linear_int8")
