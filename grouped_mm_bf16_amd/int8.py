@@ -51,8 +51,9 @@ def _pitch(width: int) -> int:
     return max(16, (width + 15) // 16 * 16)
 
 
-def _forward_only(what: str, *tensors: torch.Tensor) -> None:
-    if any(t.requires_grad for t in tensors) and torch.is_grad_enabled() or derivatives.forward_mode() and derivatives.tangent(*tensors):
+def _forward_only(what: str, x: torch.Tensor, other: Optional[torch.Tensor] = None) -> None:
+    if (x.requires_grad or other is not None and other.requires_grad) and torch.is_grad_enabled() or (
+            derivatives.forward_mode() and derivatives.tangent(*(t for t in (x, other) if t is not None))):
         raise RuntimeError(f"{what} is forward only: call it under torch.no_grad(), or with detached operands")
 
 
@@ -122,23 +123,35 @@ def _aligned(values: torch.Tensor) -> torch.Tensor:
     return own.copy_(values)
 
 
+def _columns(values: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """Columns [K, N] or [G, K, N], contiguous along K, copied only where they do not lie at multiples of 16 bytes; and the bytes from one group, one
+    column to the next."""
+    *lead, K, N = values.shape
+    stride = values.stride()
+    sg, sn = stride[0] if lead and lead[0] > 1 else 0, stride[-1] if N > 1 else _pitch(K)
+    if (values.data_ptr() | sg | sn) & 15 or sn < K:
+        values = _aligned(values.transpose(-2, -1)).transpose(-2, -1)
+        stride = values.stride()
+        sg, sn = stride[0] if lead and lead[0] > 1 else 0, stride[-1] if N > 1 else _pitch(K)
+    return values, sg, sn
+
+
 def _mm_now(a: torch.Tensor, a_scale: torch.Tensor, row_index: Optional[torch.Tensor], b: torch.Tensor, b_scale: torch.Tensor,
             offs: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
-    """b [G, N, K]; G = 1 without offs."""
-    G, N, K = b.shape
+    """b [G, K, N], or without offs [K, N]."""
+    G, (K, N) = 1 if offs is None else b.size(0), b.shape[-2:]
     M = a.size(0) if row_index is None else row_index.numel()
     out = torch.empty(M, N, device=a.device, dtype=out_dtype)
     if out.numel() == 0:
         return out
     if K == 0:
         return out.zero_()
-    a, b = _aligned(a), _aligned(b)
+    a, (b, sg, sn) = _aligned(a), _columns(b)
     lib = _lib.load()
-    pitch = lambda stride, count, width: stride if count > 1 else _pitch(width)
     with _guard(a):
         args = (a.data_ptr(), a_scale.data_ptr(), None if row_index is None else row_index.data_ptr(), b.data_ptr(), b_scale.data_ptr(), out.data_ptr(),
-                None if offs is None else offs.data_ptr(), G, a.size(0), M, N, K, pitch(a.stride(0), a.size(0), K),
-                b.stride(0) if G > 1 else 0, pitch(b.stride(1), N, K), N, _dtype_code(out_dtype))
+                None if offs is None else offs.data_ptr(), G, a.size(0), M, N, K, a.stride(0) if a.size(0) > 1 else _pitch(K), sg, sn, N,
+                _dtype_code(out_dtype))
         rc = kernels.call_with_workspace(lib.gmm_int8_mm, args, a.device, kernels.current_stream(a.device))
     _lib.check(rc, "int8 product")
     return out
@@ -149,26 +162,25 @@ _mm_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_mm", mutates_args=()
 
 @_mm_op.register_fake
 def _mm_fake(a, a_scale, row_index, b, b_scale, offs, out_dtype):
-    return a.new_empty(a.size(0) if row_index is None else row_index.numel(), b.size(1), dtype=out_dtype)
+    return a.new_empty(a.size(0) if row_index is None else row_index.numel(), b.size(-1), dtype=out_dtype)
 
 
 def _mm(a: Rows, row_index: Optional[torch.Tensor], b: Columns, offs: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
-    values = b.values.transpose(-2, -1)
-    return (_mm_op if torch.compiler.is_compiling() else _mm_now)(a.values, a.scale, row_index, values if values.dim() == 3 else values.unsqueeze(0),
-                                                                  b.scale, offs, out_dtype)
+    return (_mm_op if torch.compiler.is_compiling() else _mm_now)(a.values, a.scale, row_index, b.values, b.scale, offs, out_dtype)
 
 
 def _check_columns(what: str, b: Columns, device: torch.device, dims: int) -> None:
-    if b.values.dtype != torch.int8 or b.values.dim() != dims:
-        raise RuntimeError(f"{what}: the columns' values have to be {dims}D int8, got {b.values.dim()}D {b.values.dtype}")
-    shape = b.values.shape[:-2] + b.values.shape[-1:]
-    if b.scale.dtype != torch.float32 or b.scale.shape != shape or not b.scale.is_contiguous():
-        raise RuntimeError(f"{what}: the columns' scale has to be a contiguous float32 tensor {tuple(shape)}, got {tuple(b.scale.shape)} {b.scale.dtype}")
-    if b.values.numel() and b.values.stride(-2) != 1 and b.values.size(-2) > 1:
-        raise RuntimeError(f"{what}: the columns' values have to be contiguous along K, as quantize_columns lays them out; got strides {tuple(b.values.stride())}")
-    if b.values.size(-2) > MAX_K:
-        raise RuntimeError(f"{what}: K is at most {MAX_K}, got {b.values.size(-2)}")
-    if b.values.device != device or b.scale.device != device:
+    values, scale = b
+    if values.dtype != torch.int8 or values.dim() != dims:
+        raise RuntimeError(f"{what}: the columns' values have to be {dims}D int8, got {values.dim()}D {values.dtype}")
+    *lead, K, N = values.shape
+    if scale.dtype != torch.float32 or scale.shape != (*lead, N) or not scale.is_contiguous():
+        raise RuntimeError(f"{what}: the columns' scale has to be a contiguous float32 tensor {(*lead, N)}, got {tuple(scale.shape)} {scale.dtype}")
+    if K > 1 and values.stride()[-2] != 1 and values.numel():
+        raise RuntimeError(f"{what}: the columns' values have to be contiguous along K, as quantize_columns lays them out; got strides {tuple(values.stride())}")
+    if K > MAX_K:
+        raise RuntimeError(f"{what}: K is at most {MAX_K}, got {K}")
+    if values.device != device or scale.device != device:
         raise RuntimeError(f"{what}: all operands have to be on {device}")
 
 
@@ -227,18 +239,17 @@ def grouped_int8_mm(a: Rows, b: Columns, offs: torch.Tensor, out_dtype: torch.dt
 
 
 def _linear_now(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
-    x = moe_train._rows(x)
+    x = x if x.is_contiguous() else moe_train._rows(x)
     (T, K), N = x.shape, values.size(1)
     if 0 < T <= FEW_ROWS and N:
-        b = _aligned(values.t())
+        b, _, sn = _columns(values)
         out = torch.empty(T, N, device=x.device, dtype=x.dtype)
         with _guard(x):
             code = _dtype_code(x.dtype)
             nbytes = _linear_bytes(x.device.index, T, K, N, code)
             ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes > 0 else None
-            rc = _lib.load().gmm_int8_linear(x.data_ptr(), b.data_ptr(), scale.data_ptr(), out.data_ptr(), T, K, N, x.stride(0),
-                                             b.stride(0) if N > 1 else _pitch(K), N, code, None if ws is None else ws.data_ptr(), nbytes,
-                                             kernels.current_stream(x.device))
+            rc = _lib.load().gmm_int8_linear(x.data_ptr(), b.data_ptr(), scale.data_ptr(), out.data_ptr(), T, K, N, x.stride(0), sn,
+                                             N, code, None if ws is None else ws.data_ptr(), nbytes, kernels.current_stream(x.device))
         if rc != _lib.ERR_UNSUPPORTED:
             _lib.check(rc, "linear_int8")
             return out
@@ -280,16 +291,15 @@ def _gated_now(h: torch.Tensor, kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def _activated(a: Rows, routing: moe.Routing, up: torch.Tensor, up_scale: torch.Tensor, kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The first product's activations in 8 bits; SwiGLU in the product's own kernel where that takes its columns."""
-    b = _aligned(up.transpose(1, 2))
-    (G, N, K), M = b.shape, routing.row_token.numel()
+    b, sg, sn = _columns(up)
+    (G, K, N), M = b.shape, routing.row_token.numel()
     if kind and M and K and N % 128 == 0:
         rows = _aligned(a.values)
         act = torch.empty(M, N // 2, device=rows.device, dtype=torch.float32)
         with _guard(rows):
             rc = _lib.load().gmm_int8_gate_up(rows.data_ptr(), a.scale.data_ptr(), routing.row_token.data_ptr(), b.data_ptr(), up_scale.data_ptr(),
                                               act.data_ptr(), routing.offs.data_ptr(), G, rows.size(0), M, N, K,
-                                              rows.stride(0) if rows.size(0) > 1 else _pitch(K), b.stride(0) if G > 1 else 0, b.stride(1), N // 2,
-                                              kernels.current_stream(rows.device))
+                                              rows.stride(0) if rows.size(0) > 1 else _pitch(K), sg, sn, N // 2, kernels.current_stream(rows.device))
         if rc != _lib.ERR_UNSUPPORTED:
             _lib.check(rc, "moe_forward_int8: first product")
             return _quantize_now(act)
@@ -301,7 +311,8 @@ def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, u
                top_k: int, kind: int, renormalize: bool) -> torch.Tensor:
     (T, H), (E, inner, _) = x.shape, down.shape
     if 0 < T <= FEW_ROWS:
-        rows, b, d = moe_train._rows(x), _aligned(up.transpose(1, 2)), _aligned(down.transpose(1, 2))
+        rows = x if x.is_contiguous() else moe_train._rows(x)
+        (b, up_g, up_n), (d, down_g, down_n) = _columns(up), _columns(down)
         logits = router_logits if T == 1 and router_logits.stride(1) == 1 else moe_train._rows(router_logits)
         nbytes = _layer_bytes(x.device.index, T, E, top_k, H, inner, kind)
         if nbytes >= 0:
@@ -310,9 +321,7 @@ def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, u
                 ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
                 rc = _lib.load().gmm_int8_moe_few(rows.data_ptr(), logits.data_ptr(), b.data_ptr(), up_scale.data_ptr(), d.data_ptr(),
                                                   down_scale.data_ptr(), out.data_ptr(), T, E, top_k, H, inner, rows.stride(0), logits.stride(0),
-                                                  b.stride(0) if E > 1 else 0, b.stride(1) if b.size(1) > 1 else _pitch(H),
-                                                  d.stride(0) if E > 1 else 0, d.stride(1) if H > 1 else _pitch(inner), H, kind, renormalize,
-                                                  _dtype_code(x.dtype), _dtype_code(router_logits.dtype), ws.data_ptr(), nbytes,
+                                                  up_g, up_n, down_g, down_n, H, kind, renormalize, _dtype_code(x.dtype), _dtype_code(router_logits.dtype), ws.data_ptr(), nbytes,
                                                   kernels.current_stream(x.device))
             if rc != _lib.ERR_UNSUPPORTED:
                 _lib.check(rc, "moe_forward_int8")
