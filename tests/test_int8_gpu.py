@@ -299,6 +299,20 @@ def test_layer_whose_first_product_activates(T, E, k, H, inner):
     assert step.max() <= 1 and step.float().mean() <= 1e-3
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,E,k,H,inner", [(1, 128, 8, 2048, 768), (2, 40, 8, 130, 64), (16, 4, 1, 72, 128), (5, 3, 3, 2056, 200), (8, 2, 2, 1034, 66), (1, 16, 16, 16, 16),
+                                           (1, 1, 1, 4096, 32), (17, 6, 1, 136, 64)])
+def test_layer_of_a_few_slots(T, E, k, H, inner, dtype):
+    """The second product's last workgroups add up the result: strips that end inside, experts without rows, on one workspace again and again."""
+    for seed in range(3):
+        x, z, up, down = layer(T, E, H, inner, "swiglu", dtype, seed)
+        out = int8.moe_forward_int8(x, z, up, down, k)
+        want = oracle.layer(x, z, up.values, up.scale, down.values, down.scale, k, "swiglu")
+        assert (plain.f64(out) - want).norm() <= (2.5 * plain.UNIT[dtype] + 2.0 ** -8) * want.norm()
+        for _ in range(5):
+            assert torch.equal(int8.moe_forward_int8(x, z, up, down, k), out)
+
+
 def test_layer_over_all_experts_and_halves_of_logits():
     x, z, up, down = layer(40, 10, 64, 64, "swiglu")
     out = int8.moe_forward_int8(x, z.to(BF), up, down, 3, renormalize=False)
