@@ -102,14 +102,20 @@ __device__ __forceinline__ float scaled(int sum, float column, float row) {
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t joined(const FewArgs& a) { return buffer(a.out, uint32_t(a.M) * uint32_t(a.N) * 4); }
 
-// The last workgroup of a strip adds up what all of them left, in the order of the choices whichever it is.  Nobody waits for anybody.
+// The last workgroup of a strip adds up what all of them left, in the order of the choices whichever it is.  Nobody waits for anybody.  Choices
+// that are not there take part as zeros: asked for each, the compiler makes every load wait for the one before it.
 template <int OUT, int THREADS>
 __device__ __forceinline__ void join(const FewArgs& a, int tile) {
-  __shared__ int last;
+  __shared__ int last, rows[kJoinSlots];
+  __shared__ float weights[kJoinSlots];
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)
     last = __hip_atomic_fetch_add(&a.arrived[tile * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(a.used) - 1;
+  if (int(threadIdx.x) < a.M) {
+    rows[threadIdx.x] = a.token_rows[threadIdx.x];
+    weights[threadIdx.x] = a.slot_weight[threadIdx.x];
+  }
   __syncthreads();
   if (!last) return;
   const __amdgpu_buffer_rsrc_t y = joined(a);
@@ -117,11 +123,20 @@ __device__ __forceinline__ void join(const FewArgs& a, int tile) {
     const int t = u / OUT, col = tile * OUT + u % OUT;
     if (col >= a.N) continue;
     float sum = 0;
-    in_fours(a.top_k, [&](int j, bool in) {
-      const int slot = t * a.top_k + j;
-      const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(y, int((uint32_t(a.token_rows[slot]) * a.N + col) * 4), 0, kDeviceScope));
-      sum += in ? a.slot_weight[slot] * v : 0.0f;
-    });
+    for (int j = 0; j < a.top_k; j += 8) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = rows[t * a.top_k + min(j + i, a.top_k - 1)];
+        v[i] = __builtin_amdgcn_raw_buffer_load_b32(y, int((uint32_t(row) * a.N + col) * 4), 0, kDeviceScope);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t there = j + i < a.top_k ? ~0u : 0u;
+        const float w = __uint_as_float(__float_as_uint(weights[t * a.top_k + min(j + i, a.top_k - 1)]) & there);
+        sum += w * __uint_as_float(v[i] & there);
+      }
+    }
     put(a.sum, a.out_dtype, t * a.sum_ld + col, sum);
   }
 }
@@ -217,7 +232,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
   int g = 0, row0 = 0, rows = a.M;
   if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) {
-    if constexpr (!GLU) if (a.result == kJoined) join<OUT, THREADS>(a, tile);      // it is counted as well
+    if constexpr (!GLU && MF == 1) if (a.result == kJoined) join<OUT, THREADS>(a, tile);      // it is counted as well
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -227,6 +242,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   s.lds = shared.wave[wave];
   s.w_buf = buffer(static_cast<const uint16_t*>(a.b) + g * a.b_sg, a.b_bytes);
   s.a_plane = 0;
+  s.turn = blockIdx.x / 8;
   if constexpr (GLU) s.set_columns(first, width - first, 1, uint32_t(a.b_ld), OUT, width + first);
   else s.set_columns(first, width - first, 1, uint32_t(a.b_ld));
   const float* const columns = a.b_scale + int64_t(g) * a.N;
@@ -248,9 +264,10 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
     s.resident_k = 0;
     s.resident_rows = rows;
     x.load(rows, 2 * a.K, row);
-    s.template prime<1, WAVES>(step, wave * S::KS, a.K);
+    typename S::template Cycle<1, WAVES> cycle(wave * S::KS, a.K, s.turn);
+    cycle.prime(s, step);
     x.round(rows, 2 * a.K, row, rows_here, s.pitch, most_here, scale_here);
-    s.template primed<1, WAVES>(step, wave * S::KS, a.K, acc);
+    cycle.primed(s, step, acc);
   } else {
     s.a_buf = buffer(a.a, a.a_bytes);
     s.set_rows([&](int r) {
@@ -300,7 +317,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
       }
     }
   }
-  if constexpr (!GLU) if (a.result == kJoined) join<OUT, THREADS>(a, tile);
+  if constexpr (!GLU && MF == 1) if (a.result == kJoined) join<OUT, THREADS>(a, tile);
 }
 
 // Planes of integer sums added up and scaled.

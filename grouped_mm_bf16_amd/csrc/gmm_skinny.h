@@ -17,6 +17,8 @@
 // A goes through LDS as well, for the same reason.  Its rows that do not exist read as zeros and cost no access.  LDS is a wave's own
 // here: its instructions run in order, nobody waits for anybody.  The waves of a workgroup share the range of k and add up in LDS.
 #pragma once
+#include <type_traits>
+
 #include "gmm_elem.h"
 
 namespace gmm {
@@ -75,6 +77,7 @@ constexpr int GMM_A_RESIDENT = 2;    // lies in LDS
 template <typename T, int LAY, int FR_, int MF, int NA, int AM, int ST>
 struct Skinny {
   static constexpr int FR = FR_, STEPS = ST;
+  static constexpr bool CYCLIC = std::is_same_v<T, I8x2>;     // sums of integers, which no order changes
   static constexpr int KS = LAY == GMM_W_COLS ? 64 : 32;      // k of a step
   static constexpr int KH = KS / 32;                          // products' halves of it
   static constexpr int COLUMNS = 16 * FR;
@@ -100,6 +103,7 @@ struct Skinny {
   uint32_t a_plane;       // bytes from the high to the low plane
   const char* resident;   // GMM_A_RESIDENT: row 0 of the high plane, from k = resident_k on,
   int pitch, resident_k, resident_rows;   // bytes from one row to the next, number of rows
+  uint32_t turn;          // CYCLIC: the step that is the first
 
   struct Step { u32x4 w[WL]; u32x4 a[AM == GMM_A_RESIDENT ? 1 : NA][AL]; };
 
@@ -177,12 +181,15 @@ struct Skinny {
     } else if constexpr (LAY == GMM_W_COLS) {
       const uint32_t at = w_at + uint32_t(k) * 2 - back(k + 8 * (lane & 7), end);
       const bool in = k + 8 * (lane & 7) < end;
+      uint32_t outside = in ? 0 : kNowhere;
+      if constexpr (CYCLIC) asm volatile("" : "+v"(outside));      // or the compiler branches around the loads, and they wait for one another
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
         const int c = 8 * i + (lane >> 3);
         const bool second = 8 * i >= w_half;
-        w[i] = __builtin_amdgcn_raw_buffer_load_b128(
-            w_buf, int(in && c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere), 0, kStream);
+        const uint32_t there = at + 8 * i * w_step_n + (second ? w_jump : 0);
+        const bool has = c - (second ? w_half : 0) < columns;
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(CYCLIC ? (has ? there : kNowhere) | outside : in && has ? there : kNowhere), 0, kStream);
       }
     } else if constexpr (LAY == GMM_W_THIN) {
 #pragma unroll
@@ -339,11 +346,55 @@ struct Skinny {
       }
   }
 
+  // The same from the `turn`-th step on and round to the one before it (CYCLIC).
+  template <int M, int WAVES>
+  struct Cycle {
+    int next, begin, last, end, left, at[ST];
+    __device__ __forceinline__ Cycle(int begin_, int end_, uint32_t turn) : begin(begin_), end(end_) {
+      constexpr int NEXT = WAVES * KS;
+      left = begin < end ? (end - begin + NEXT - 1) / NEXT : 0;
+      last = begin + left * NEXT;
+      next = begin + (left ? int(turn % uint32_t(left)) * NEXT : 0);
+    }
+    __device__ __forceinline__ int advance() {      // past the last step: to the end
+      const int k = left > 0 ? next : end;
+      --left;
+      next += WAVES * KS;
+      next = next >= last ? begin : next;
+      return k;
+    }
+    __device__ __forceinline__ void prime(const Skinny& s, Step (&step)[ST]) {
+#pragma unroll
+      for (int u = 0; u < ST; ++u) {
+        at[u] = advance();
+        s.load<M>(step[u], at[u], end);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __device__ __forceinline__ void primed(const Skinny& s, Step (&step)[ST], f32x4 (&acc)[MF][FR]) {
+      for (int todo = (last - begin) / (WAVES * KS); todo > 0; todo -= ST)
+#pragma unroll
+        for (int u = 0; u < ST; ++u) {
+          s.multiply<M>(step[u], at[u], end, acc);
+          __builtin_amdgcn_sched_barrier(0);
+          at[u] = advance();
+          s.load<M>(step[u], at[u], end);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  };
+
   template <int M, int WAVES>
   __device__ __forceinline__ void steps(int begin, int end, f32x4 (&acc)[MF][FR]) const {
     Step step[ST];
-    prime<M, WAVES>(step, begin, end);
-    primed<M, WAVES>(step, begin, end, acc);
+    if constexpr (CYCLIC) {
+      Cycle<M, WAVES> c(begin, end, turn);
+      c.prime(*this, step);
+      c.primed(*this, step, acc);
+    } else {
+      prime<M, WAVES>(step, begin, end);
+      primed<M, WAVES>(step, begin, end, acc);
+    }
   }
 
   // The part of wave `wave` of WAVES of the product over begin .. end: the waves' steps lie side by side in memory.  rows: how many there
