@@ -23,10 +23,6 @@ using namespace gmm;
 constexpr int kMaxTokens = 64;
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
-// Slots (choices of all tokens; at most a wave's lanes) and experts up to which a workgroup routes for itself, one wave to a token.  1 token, 1 of
-// 8 experts of 3674 -> 2 x 151 18 us, with a launch for the routing 20; 64 slots, 4 of 8 experts of 432 -> 2 x 10752 87 and 81.
-constexpr int kRouteSlots = 32, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
-
 // Slots up to which the second product's last workgroup of some columns adds them up: a launch less, but one workgroup reads what otherwise
 // all of them would.  2 tokens, 6 of 34 experts of 280 -> 600 16 us, with a launch for the sums 17 (1 token of small experts 15 and 16); 6
 // tokens, 4 of 8 experts of 432 -> 2 x 10752 60 and 56.
@@ -106,75 +102,6 @@ struct Choice {
   }
 };
 
-// Routing by every workgroup for itself: up to kRouteSlots slots, kRouteExperts experts, a wave to a token.  The first workgroup leaves the
-// results for the kernels behind.  Rows are sorted by expert, stably, as gmm_moe_route has them.
-struct FewRouting {
-  int32_t expert[kRouteSlots];
-  float weight[kRouteSlots];
-  int32_t token[kRouteSlots];     // of a row of the expert that this workgroup looks for
-  int32_t found, row0, rows;
-};
-
-__device__ __forceinline__ bool route_here(const FewArgs& a, FewRouting& r, int which, int& expert, int& row0, int& rows) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int t = wave; t < a.tokens; t += kWaves) {
-    int e;
-    float w;
-    const auto choose = [&](auto zero) {
-      using L = decltype(zero);
-      MoeTopk<L, kRouteKeys> token;
-      token.load(static_cast<const L*>(a.logits) + t * a.logits_ld, a.experts, lane);
-      token.choose(a.experts, a.top_k, a.renormalize, lane, e, w);
-    };
-    if (a.logits_dtype == GMM_DT_BF16) choose(Bf16{});
-    else if (a.logits_dtype == GMM_DT_F16) choose(F16{});
-    else choose(0.0f);
-    if (lane < a.top_k) {
-      r.expert[t * a.top_k + lane] = e;
-      r.weight[t * a.top_k + lane] = w;
-    }
-  }
-  __syncthreads();
-  if (wave == 0) {
-    const int e = lane < a.slots ? r.expert[lane] : a.experts;
-    int row = 0, before = 0;     // slots ahead of the lane's; experts ahead of its own
-    bool head = lane < a.slots;  // the first slot of its expert
-    for (int s = 0; s < a.slots; ++s) {
-      const int other = __builtin_amdgcn_readlane(e, s);
-      row += other < e || (other == e && s < lane);
-      head = head && !(other == e && s < lane);
-    }
-    const uint64_t heads = __ballot(head);
-    for (uint64_t todo = heads; todo; todo &= todo - 1)
-      before += __builtin_amdgcn_readlane(e, __ffsll(static_cast<unsigned long long>(todo)) - 1) < e;
-    const uint64_t it = __ballot(head && before == which);
-    if (it) {
-      const int at = __ffsll(static_cast<unsigned long long>(it)) - 1;
-      const int mine = __builtin_amdgcn_readlane(e, at), first = __builtin_amdgcn_readlane(row, at);
-      const uint64_t same = __ballot(e == mine);
-      if (e == mine) r.token[row - first] = lane / a.top_k;
-      if (lane == 0) { r.expert[0] = mine; r.row0 = first; r.rows = __popcll(same); }
-    }
-    if (lane == 0) r.found = it != 0;
-    if (blockIdx.x == 0 && lane < a.slots) {
-      a.token_rows[lane] = row;
-      a.slot_weight[lane] = r.weight[lane];
-    }
-    if (blockIdx.x == 0)
-      for (int i = lane; i < a.experts; i += 64) {
-        int to = 0;
-        for (int s = 0; s < a.slots; ++s) to += __builtin_amdgcn_readlane(e, s) <= i;
-        a.offs[i] = to;
-      }
-  }
-  __syncthreads();
-  if (!r.found) return false;
-  expert = __builtin_amdgcn_readfirstlane(r.expert[0]);
-  row0 = __builtin_amdgcn_readfirstlane(r.row0);
-  rows = __builtin_amdgcn_readfirstlane(r.rows);
-  return true;
-}
-
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
 
 // act[r] = act(x[token of row r] @ w_up[e]), or parts of the product.  GLU: a strip is 8 * FR gate columns and their partners.
@@ -191,7 +118,8 @@ __global__ void __launch_bounds__(kThreads, few_groups(LAY, MF)) few_up_kernel(c
     for (int i = threadIdx.x; i < a.strips; i += kThreads) a.arrived[i * kLine] = 0;
   if constexpr (ROUTE) {
     __shared__ FewRouting routing;
-    if (!route_here(a, routing, item / a.tiles, expert, row0, rows)) return;
+    const RouteHere here{a.logits, a.logits_ld, a.offs, a.token_rows, a.slot_weight, a.tokens, a.experts, a.top_k, a.slots, a.renormalize, a.logits_dtype};
+    if (!route_here<kWaves>(here, routing, item / a.tiles, expert, row0, rows)) return;
     row_token = routing.token;
   } else {
     int used;

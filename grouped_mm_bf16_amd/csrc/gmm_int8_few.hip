@@ -4,7 +4,11 @@
 //   one matrix        parts are planes of integer sums, which a second kernel adds up and scales: exact, as in one part
 //   expert layer      route, rows of x to 8 bits, first product, activation to 8 bits, second product, sum over choices and parts.  The planes
 //                     between its launches are scaled fp32 values; SwiGLU is computed by the first product where k is in one part
-// Of a few short rows every workgroup makes the 8-bit ones itself, while its first weights are on their way (rounds_here): a launch less.
+// Of a few short rows every workgroup makes the 8-bit ones itself, while its first weights are on their way (rounds_here), and the layer's routing
+// (routes_here) and sums (kJoinSlots) as well: of one token two launches are left.
+// Columns of 4096 values lie in the same memory channels, so workgroups that run side by side begin at different places along k (Cycle): 1 x 14336 x
+// 4096 12.8 -> 11.4 us, 48 rows 18.1 -> 17.2, 1 x 28672 x 4096 21.3 -> 19.5.
+// One layer of 24 tokens, all 8 experts of 4096 -> 2 x 14336 (1.41 GB of weights): 214 to 232 us, 6.1 to 6.6 TB/s (a copy reaches 5.1, which writes as well).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -13,6 +17,7 @@
 #include "../../include/grouped_mm_hip.h"
 #include "gmm_device.h"
 #include "gmm_launch.h"
+#include "gmm_route.h"
 #include "gmm_skinny.h"
 
 namespace {
@@ -53,6 +58,7 @@ struct FewArgs {
   int64_t sum_ld;
   int32_t tokens, top_k;
   int32_t clear;              // counters that this launch clears
+  RouteHere route;            // where the workgroups route for themselves
 };
 
 constexpr int kNotRounded = -1;
@@ -213,7 +219,8 @@ struct RowsHere {
 
 // FR: a strip is 16 FR columns.  GLU: half of them gate columns, the others their partners, N / 2 further on; the result is silu(gate) * partner.
 // X: the rows are values of this type, rounded here (up to 16 of them, k in one part); void: 8-bit integers.
-template <typename X, int MF, int FR, int WAVES, bool GLU>
+// ROUTE: every workgroup routes for itself (GLU and X alone).
+template <typename X, int MF, int FR, int WAVES, bool GLU, bool ROUTE>
 __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int8_few_kernel(const FewArgs a) {
   constexpr bool HERE = !std::is_void_v<X>;
   static_assert(!HERE || MF == 1, "");
@@ -231,7 +238,12 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
     for (int i = threadIdx.x; i < a.clear; i += THREADS) a.arrived[i * kLine] = 0;
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
   int g = 0, row0 = 0, rows = a.M;
-  if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) {
+  const int32_t* row_index = a.row_index;      // of the group's rows
+  if constexpr (ROUTE) {
+    __shared__ FewRouting routing;
+    if (!route_here<WAVES>(a.route, routing, item / a.tiles, g, row0, rows)) return;
+    row_index = routing.token;
+  } else if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) {
     if constexpr (!GLU && MF == 1) if (a.result == kJoined) join<OUT, THREADS>(a, tile);      // it is counted as well
     return;
   }
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   else s.set_columns(first, width - first, 1, uint32_t(a.b_ld));
   const float* const columns = a.b_scale + int64_t(g) * a.N;
   const auto source = [&](int r) {      // row of a, or -1
-    const int at = a.row_index ? a.row_index[row0 + r] : row0 + r;
+    const int at = ROUTE ? row_index[r] : row_index ? row_index[row0 + r] : row0 + r;
     return uint32_t(at) < uint32_t(a.a_rows) ? at : -1;
   };
   f32x4 acc[MF][FR];
@@ -415,14 +427,21 @@ bool rounds_here(int64_t rows, int64_t K, const Shape& s, int32_t x_dtype) {
   return rows <= 16 && s.parts == 1 && rows * K <= kMostRounded && rows * ((K + 7) / 8) <= threads * each;
 }
 
-template <typename X, bool GLU>
+// Do the workgroups of this product route for themselves?  In one round of them, in which that is as long in all as in one.  1 token, 8 of 128 experts
+// of 2048 -> 2 x 768 19.6 us, with a launch for the routing 22.5.
+bool routes_here(int64_t used, int64_t tiles, int64_t slots, int64_t experts) {
+  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256;
+  return used * tiles <= 4 * cus && slots <= kRouteSlots && experts <= kRouteExperts;
+}
+
+template <typename X, bool GLU, bool ROUTE = false>
 int launch_rows(const FewArgs& a, hipStream_t stream) {
   constexpr bool HERE = !std::is_void_v<X>;
   const dim3 grid(unsigned(int64_t(a.used) * a.tiles * a.parts));
   const int lds = HERE ? a.most * ((a.K * 2 + 31) & ~15) : 0;
   const auto go = [&](auto mf, auto fr, auto waves) {
     constexpr int MF = decltype(mf)::value, FR = decltype(fr)::value, WAVES = decltype(waves)::value;
-    hipLaunchKernelGGL((int8_few_kernel<X, MF, FR, WAVES, GLU>), grid, dim3(64 * WAVES), lds, stream, a);
+    hipLaunchKernelGGL((int8_few_kernel<X, MF, FR, WAVES, GLU, ROUTE>), grid, dim3(64 * WAVES), lds, stream, a);
   };
   const auto by_rows = [&](auto fr, auto waves) {
     if constexpr (!HERE) {
@@ -440,6 +459,9 @@ int launch_rows(const FewArgs& a, hipStream_t stream) {
 
 template <bool GLU>
 int launch(const FewArgs& a, hipStream_t stream) {
+  if constexpr (GLU) {
+    if (a.route.logits) return a.x_dtype == GMM_DT_BF16 ? launch_rows<Bf16, true, true>(a, stream) : launch_rows<F16, true, true>(a, stream);
+  }
   if (a.x_dtype == GMM_DT_BF16) return launch_rows<Bf16, GLU>(a, stream);
   if (a.x_dtype == GMM_DT_F16) return launch_rows<F16, GLU>(a, stream);
   if constexpr (!GLU) {
@@ -632,8 +654,13 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   if (!sizes_fit(u) || !sizes_fit(d)) return GMM_ERR_UNSUPPORTED;
   if (p.used * u.tiles * u.parts >= (int64_t(1) << 31) || p.used * d.tiles * d.parts >= (int64_t(1) << 31)) return GMM_ERR_UNSUPPORTED;
 
-  int rc = gmm_moe_route(logits, tokens > 1 ? logits_stride : experts, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert, slot_weight,
-                         row_token, token_rows, ws + p.table_at, p.table_bytes, stream);
+  int rc = GMM_OK;
+  const int64_t logits_ld = tokens > 1 ? logits_stride : experts;
+  if (p.x_here && p.activated && routes_here(p.used, u.tiles, p.slots, experts))
+    u.route = {logits, logits_ld, offs, token_rows, slot_weight, int32_t(tokens), int32_t(experts), int32_t(top_k), int32_t(p.slots), renormalize, logits_dtype};
+  else
+    rc = gmm_moe_route(logits, logits_ld, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert, slot_weight, row_token, token_rows,
+                       ws + p.table_at, p.table_bytes, stream);
   if (rc == GMM_OK && !p.x_here) rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws + p.x_at), at(p.x_scale_at), tokens, hidden, x_stride, p.x_pitch, dtype, stream);
   if (rc == GMM_OK) rc = p.activated ? launch<true>(u, s) : launch<false>(u, s);
   if (rc == GMM_OK && !p.act_here)

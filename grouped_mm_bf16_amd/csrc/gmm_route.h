@@ -1,4 +1,5 @@
-// Top-k choice of one token by one wave, for the routing (gmm_moe.hip) and the kernels that route for themselves (gmm_few.hip).
+// Top-k choice of one token by one wave, for the routing (gmm_moe.hip) and the kernels that route for themselves (gmm_few.hip,
+// gmm_int8_few.hip).
 #pragma once
 #include "gmm_elem.h"
 
@@ -104,5 +105,88 @@ struct MoeTopk {
     weight = p / den;
   }
 };
+
+// Slots (choices of all tokens; at most a wave's lanes) and experts up to which a workgroup routes for itself, one wave to a token.  1 token, 1 of
+// 8 experts of 3674 -> 2 x 151 18 us, with a launch for the routing 20; 64 slots, 4 of 8 experts of 432 -> 2 x 10752 87 and 81.
+constexpr int kRouteSlots = 32, kRouteKeys = 4, kRouteExperts = 64 * kRouteKeys;
+
+// Routing by every workgroup for itself: up to kRouteSlots slots, kRouteExperts experts, a wave to a token.  The first workgroup leaves the
+// results for the kernels behind.  Rows are sorted by expert, stably, as gmm_moe_route has them.
+struct RouteHere {
+  const void* logits;
+  int64_t logits_ld;
+  int32_t* offs;
+  int32_t* token_rows;
+  float* slot_weight;
+  int32_t tokens, experts, top_k, slots, renormalize, logits_dtype;
+};
+
+struct FewRouting {
+  int32_t expert[kRouteSlots];
+  float weight[kRouteSlots];
+  int32_t token[kRouteSlots];     // of a row of the expert that this workgroup looks for
+  int32_t found, row0, rows;
+};
+
+template <int WAVES>
+__device__ __forceinline__ bool route_here(const RouteHere& a, FewRouting& r, int which, int& expert, int& row0, int& rows) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int t = wave; t < a.tokens; t += WAVES) {
+    int e;
+    float w;
+    const auto choose = [&](auto zero) {
+      using L = decltype(zero);
+      MoeTopk<L, kRouteKeys> token;
+      token.load(static_cast<const L*>(a.logits) + t * a.logits_ld, a.experts, lane);
+      token.choose(a.experts, a.top_k, a.renormalize, lane, e, w);
+    };
+    if (a.logits_dtype == GMM_DT_BF16) choose(Bf16{});
+    else if (a.logits_dtype == GMM_DT_F16) choose(F16{});
+    else choose(0.0f);
+    if (lane < a.top_k) {
+      r.expert[t * a.top_k + lane] = e;
+      r.weight[t * a.top_k + lane] = w;
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int e = lane < a.slots ? r.expert[lane] : a.experts;
+    int row = 0, before = 0;     // slots ahead of the lane's; experts ahead of its own
+    bool head = lane < a.slots;  // the first slot of its expert
+    for (int s = 0; s < a.slots; ++s) {
+      const int other = __builtin_amdgcn_readlane(e, s);
+      row += other < e || (other == e && s < lane);
+      head = head && !(other == e && s < lane);
+    }
+    const uint64_t heads = __ballot(head);
+    for (uint64_t todo = heads; todo; todo &= todo - 1)
+      before += __builtin_amdgcn_readlane(e, __ffsll(static_cast<unsigned long long>(todo)) - 1) < e;
+    const uint64_t it = __ballot(head && before == which);
+    if (it) {
+      const int at = __ffsll(static_cast<unsigned long long>(it)) - 1;
+      const int mine = __builtin_amdgcn_readlane(e, at), first = __builtin_amdgcn_readlane(row, at);
+      const uint64_t same = __ballot(e == mine);
+      if (e == mine) r.token[row - first] = lane / a.top_k;
+      if (lane == 0) { r.expert[0] = mine; r.row0 = first; r.rows = __popcll(same); }
+    }
+    if (lane == 0) r.found = it != 0;
+    if (blockIdx.x == 0 && lane < a.slots) {
+      a.token_rows[lane] = row;
+      a.slot_weight[lane] = r.weight[lane];
+    }
+    if (blockIdx.x == 0)
+      for (int i = lane; i < a.experts; i += 64) {
+        int to = 0;
+        for (int s = 0; s < a.slots; ++s) to += __builtin_amdgcn_readlane(e, s) <= i;
+        a.offs[i] = to;
+      }
+  }
+  __syncthreads();
+  if (!r.found) return false;
+  expert = __builtin_amdgcn_readfirstlane(r.expert[0]);
+  row0 = __builtin_amdgcn_readfirstlane(r.row0);
+  rows = __builtin_amdgcn_readfirstlane(r.rows);
+  return true;
+}
 
 }  // namespace gmm
