@@ -91,10 +91,10 @@ def gated_backward(grad, h, kind):
     return out, UNIT[dtype] * out.abs() + TINY[dtype] + bound
 
 
-def dropout_bits(n, seed, offset, site=0):
-    """16 bits for each of n elements, from Philox 4x32-10 in Python's own whole numbers, a block at a time."""
+def dropout_bits(n, seed, offset, site=0, first=0):
+    """16 bits for each of n elements from element 8 * first on, from Philox 4x32-10 in Python's own whole numbers, a block at a time."""
     low, blocks = 0xffffffff, []
-    for b in range(-(-n // 8)):
+    for b in range(first, first - (-n // 8)):
         c = [b & low, (b >> 32 | site << 16) & low, offset & low, offset >> 32 & low]
         k = [seed & low, seed >> 32 & low]
         for _ in range(10):
