@@ -2,7 +2,8 @@
 // The mask is never stored: the backward pass makes the same bits again.  Element i of x, rows one after the other, has bits 16 (i % 8) ..
 // of block i / 8 of Philox 4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3, 2011): key rng[0], counter
 // (i / 8, rng[1]), the call's site in the counter's bits 48 .. 63.  16 bits to an element make a block's ten rounds, 20 products of 32 bits,
-// serve eight elements: with 32 bits each the rounds, not memory, would bound 16-bit rows.
+// serve eight elements: with 32 bits each the rounds, not memory, would bound 16-bit rows.  What is read or written once goes past the caches.
+//   16384 x 4096 bf16   with a residual 63 us (6.4 TB/s), its gradient 43 (6.2)
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -2,7 +2,8 @@
 //   scale[r] = max(max |x[r]|, 2^-100) / 127,   q[r, c] = x[r, c] / scale[r], rounded to a whole number, ties to even
 // of x as it is, or of the activation between an expert layer's products, which is computed here from their fp32 result: no rounding to 16 bits
 // stands between the two.  A row with an infinity or NaN in it has that as its scale and zeros for values: products with it are NaN.  Memory
-// bounds it: a row is read once and stays in registers between its maximum and its rounding.
+// bounds it: a row is read once and stays in registers between its maximum and its rounding, 16 to 256 lanes to a row by its length.
+//   8192 rows of 4096 bf16   16.6 us (6.0 TB/s)      32008 rows of 768 fp32   20.9 us (5.9 TB/s)
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
