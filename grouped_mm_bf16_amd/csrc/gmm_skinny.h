@@ -181,15 +181,19 @@ struct Skinny {
     } else if constexpr (LAY == GMM_W_COLS) {
       const uint32_t at = w_at + uint32_t(k) * 2 - back(k + 8 * (lane & 7), end);
       const bool in = k + 8 * (lane & 7) < end;
-      uint32_t outside = in ? 0 : kNowhere;
+      [[maybe_unused]] uint32_t outside = in ? 0 : kNowhere;
       if constexpr (CYCLIC) asm volatile("" : "+v"(outside));      // or the compiler branches around the loads, and they wait for one another
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
         const int c = 8 * i + (lane >> 3);
         const bool second = 8 * i >= w_half;
-        const uint32_t there = at + 8 * i * w_step_n + (second ? w_jump : 0);
-        const bool has = c - (second ? w_half : 0) < columns;
-        w[i] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(CYCLIC ? (has ? there : kNowhere) | outside : in && has ? there : kNowhere), 0, kStream);
+        if constexpr (CYCLIC) {
+          const uint32_t from = c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere;
+          w[i] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(from | outside), 0, kStream);
+        } else {
+          w[i] = __builtin_amdgcn_raw_buffer_load_b128(
+              w_buf, int(in && c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere), 0, kStream);
+        }
       }
     } else if constexpr (LAY == GMM_W_THIN) {
 #pragma unroll
