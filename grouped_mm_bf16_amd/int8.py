@@ -5,7 +5,8 @@ layer, the grouped product, and the whole mixture-of-experts layer, whose activa
 
 Weights are rounded once (:func:`quantize_columns`), activations in each call (:func:`quantize_rows`).  Sums are exact, scales are applied in
 float32, the result is rounded once.  No count reaches the host.  Up to ``FEW_ROWS`` rows weights are streamed past the rows, more go through tiles.
-Registered as torch custom ops (``grouped_mm_bf16_amd::int8_quantize``, ``int8_mm``, ``int8_linear``, ``int8_layer``), which calls dispatch to while a model around them is being traced or compiled.  The reference has no counterpart.
+Registered as torch custom ops (``grouped_mm_bf16_amd::int8_quantize``, ``int8_mm``, ``int8_linear``, ``int8_layer``), which calls dispatch to while a
+model around them is being traced or compiled.  Forward only.  The reference has no counterpart.
 """
 from __future__ import annotations
 
@@ -182,6 +183,7 @@ def _check_columns(what: str, b: Columns, device: torch.device, dims: int) -> No
         raise RuntimeError(f"{what}: K is at most {MAX_K}, got {K}")
     if values.device != device or scale.device != device:
         raise RuntimeError(f"{what}: all operands have to be on {device}")
+    _forward_only(what, scale)
 
 
 def _check_rows(what: str, a: Rows, K: int) -> None:
@@ -191,6 +193,7 @@ def _check_rows(what: str, a: Rows, K: int) -> None:
         raise RuntimeError(f"{what}: the rows' scale has to be a contiguous float32 tensor ({a.values.size(0)},), got {tuple(a.scale.shape)} {a.scale.dtype}")
     if a.scale.device != a.values.device:
         raise RuntimeError(f"{what}: all operands have to be on {a.values.device}")
+    _forward_only(what, a.scale)
     if a.values.size(1) != K:
         raise RuntimeError(f"{what}: contraction dimensions have to match, got {a.values.size(1)} and {K}")
 
@@ -314,19 +317,19 @@ def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, u
         rows = x if x.is_contiguous() else moe_train._rows(x)
         (b, up_g, up_n), (d, down_g, down_n) = _columns(up), _columns(down)
         logits = router_logits if T == 1 and router_logits.stride(1) == 1 else moe_train._rows(router_logits)
-        nbytes = _layer_bytes(x.device.index, T, E, top_k, H, inner, kind)
-        if nbytes >= 0:
-            out = torch.empty(T, H, device=x.device, dtype=x.dtype)
-            with _guard(x):
+        with _guard(x):
+            nbytes = _layer_bytes(x.device.index, T, E, top_k, H, inner, kind)
+            if nbytes >= 0:
+                out = torch.empty(T, H, device=x.device, dtype=x.dtype)
                 ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
                 rc = _lib.load().gmm_int8_moe_few(rows.data_ptr(), logits.data_ptr(), b.data_ptr(), up_scale.data_ptr(), d.data_ptr(),
                                                   down_scale.data_ptr(), out.data_ptr(), T, E, top_k, H, inner, rows.stride(0), logits.stride(0),
-                                                  up_g, up_n, down_g, down_n, H, kind, renormalize, _dtype_code(x.dtype), _dtype_code(router_logits.dtype), ws.data_ptr(), nbytes,
-                                                  kernels.current_stream(x.device))
-            if rc != _lib.ERR_UNSUPPORTED:
-                _lib.check(rc, "moe_forward_int8")
-                return out
-    routing = moe.moe_route(router_logits, top_k, renormalize)
+                                                  up_g, up_n, down_g, down_n, H, kind, renormalize, _dtype_code(x.dtype),
+                                                  _dtype_code(router_logits.dtype), ws.data_ptr(), nbytes, kernels.current_stream(x.device))
+        if nbytes >= 0 and rc != _lib.ERR_UNSUPPORTED:
+            _lib.check(rc, "moe_forward_int8")
+            return out
+    routing = moe.moe_route(moe_train._rows(router_logits), top_k, renormalize)
     values, scale = _activated(_quantize(x), routing, up, up_scale, kind)
     y = _mm(Rows(values[:, :inner], scale), None, Columns(down, down_scale), routing.offs, x.dtype)
     return moe_train._sum_now(y, routing.token_rows, routing.slot_weight, T, top_k)

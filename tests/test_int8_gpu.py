@@ -320,6 +320,22 @@ def test_layer_over_all_experts_and_halves_of_logits():
     assert (plain.f64(out) - want).norm() <= 2.0 ** -6 * want.norm()
 
 
+@pytest.mark.parametrize("T", [1, 6, 90])
+def test_layer_of_operands_that_lie_elsewhere(T):
+    """Rows apart, transposed ones, logits of which neither is contiguous, weights of experts far apart and at odd addresses."""
+    x, z, up, down = layer(T, 6, 136, 64, "swiglu")
+    want = int8.moe_forward_int8(x, z, up, down, 2)
+    apart = torch.zeros(T, 150, dtype=BF, device=DEV)[:, 3:139].copy_(x)
+    turned = x.t().contiguous().t()
+    far = lambda c: int8.Columns(torch.zeros(6, 3, *c.values.transpose(1, 2).shape[1:], dtype=torch.int8, device=DEV)[:, 1].copy_(c.values.transpose(1, 2)).transpose(1, 2), c.scale)
+    odd = lambda c: int8.Columns(torch.zeros(c.values.numel() + 1, dtype=torch.int8, device=DEV)[1:].reshape(c.values.transpose(1, 2).shape)
+                                 .copy_(c.values.transpose(1, 2)).transpose(1, 2), c.scale)
+    for rows in (apart, turned):
+        for logits in (z.t().contiguous().t(), torch.zeros(T, 9, device=DEV)[:, 2:8].copy_(z)):
+            for place in (far, odd):
+                assert torch.equal(int8.moe_forward_int8(rows, logits, place(up), place(down), 2), want)
+
+
 def test_layer_of_nothing():
     x, z, up, down = layer(3, 4, 64, 64, "swiglu")
     assert int8.moe_forward_int8(x[:0], z[:0], up, down, 2).shape == (0, 64)

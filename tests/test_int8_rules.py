@@ -45,6 +45,23 @@ def test_rounding_rules(no_launch, x, text):
             f(x)
 
 
+def test_scales_that_require_a_gradient(no_launch, monkeypatch):
+    """They would be constants without a word."""
+    learned = lambda t: t._replace(scale=t.scale.clone().requires_grad_())
+    offs, x, z = torch.zeros(2, dtype=torch.int32), torch.zeros(4, 32, dtype=BF), torch.zeros(4, 2)
+    calls = [lambda: int8.int8_mm(learned(rows()), columns()), lambda: int8.int8_mm(rows(), learned(columns())),
+             lambda: int8.grouped_int8_mm(learned(rows()), columns(2), offs), lambda: int8.grouped_int8_mm(rows(), learned(columns(2)), offs),
+             lambda: int8.linear_int8(x, learned(columns())),
+             lambda: int8.moe_forward_int8(x, z, learned(columns(2, N=16)), columns(2, K=8, N=32), 1),
+             lambda: int8.moe_forward_int8(x, z, columns(2, N=16), learned(columns(2, K=8, N=32)), 1)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="forward only"):
+            call()
+    monkeypatch.setattr(int8, "_mm_now", lambda a, *rest: torch.ones(1))
+    with torch.no_grad():
+        assert calls[0]() == calls[1]() == calls[2]() == calls[3]() == 1
+
+
 BAD_ROWS = [(rows(values=torch.zeros(4, 32)), "2D int8"), (rows(values=torch.zeros(32, dtype=torch.int8)), "2D int8"),
             (rows(scale=torch.zeros(3)), "rows' scale"), (rows(scale=torch.zeros(4, dtype=BF)), "rows' scale"), (rows(scale=torch.zeros(8)[::2]), "rows' scale"),
             (rows(K=31), "contraction dimensions")]
