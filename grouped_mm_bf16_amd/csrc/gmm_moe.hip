@@ -171,10 +171,14 @@ __global__ void __launch_bounds__(64) moe_scatter_kernel(const int32_t* __restri
 // Slots of one expert would count one after the other on one LDS word (131072 tokens that all choose expert 0 of 8 took 132 us):
 // each count is several words, for lanes next to each other.  us with the choice, three kernels / this one: 4096 tokens, 8 of
 // 128 experts 26 / 13; 16384, 2 of 8 21 / 12; 65536, 2 of 8 39 / 32; 131072, 1 of 8 47 / 38, of 64 52 / 41, all on one of them 52
-// / 40.  Counting grows with the slots, in every workgroup: past kPlaceSlots the three kernels.
+// / 40.  Counting grows with the slots, in every workgroup: past kPlaceSlots the three kernels, or two.
 constexpr int kPlaceWaves = 16;
 constexpr int kPlaceBlock = 64 * kPlaceWaves;
 constexpr int kPlaceSlots = 131072;
+// Where a call has a table of its own, counts from a kernel in front of the placing (moe_place_counted_kernel): another launch, but nobody counts what
+// others have.  us with the choice, one kernel / two: 2048 tokens, 8 of 128 experts 13.2 / 11.2, 4096 18.3 / 12.0, 8192 29.8 / 13.9, 16384 52.5 / 18.8;
+// 8192, 2 of 8 11.9 / 9.6, 65536 55 / 20; 131072, all on one expert 61 / 27; but 1024, 8 of 128 10.4 / 11.1.  The launch costs the host 2 us.
+constexpr int kCountedSlots = 16384;
 constexpr int kPlaceWords = (kPlaceWaves + 2 * 8) * (kMaxExperts + 1);   // LDS: kPlaceWaves * E cursors and the counts
 
 // Words of a count, as a power of two: 32 up to 32 experts, 8 from 128 on.  More of them cost more to clear and to add up than
@@ -275,6 +279,39 @@ __global__ void __launch_bounds__(kPlaceBlock) moe_place_kernel(const int32_t* _
     }
   }
   moe_place(words, blocks > 1 ? sums : nullptr, part, expert, own * kPlaceBlock, E, k, own == 0, offs, row_token, token_rows);
+}
+
+// The same from the table of moe_hist_kernel, a row of it for each workgroup (spb = kPlaceBlock): threads next to each other own experts, groups of
+// them every so many rows, eight of which are on their way together.
+__global__ void __launch_bounds__(kPlaceBlock) moe_place_counted_kernel(const int32_t* __restrict__ slot_expert, int slots, int E, int k,
+                                                                        const int32_t* __restrict__ table, int32_t* __restrict__ offs,
+                                                                        int32_t* __restrict__ row_token, int32_t* __restrict__ token_rows) {
+  __shared__ __align__(16) int32_t cursor[kPlaceWaves * (kMaxExperts + 1)];
+  __shared__ int32_t sums[2 * kMaxExperts];
+  __shared__ int32_t part[kPlaceWaves];
+  const int tid = threadIdx.x, own = blockIdx.x, blocks = gridDim.x;
+  const int expert = own * kPlaceBlock + tid < slots ? slot_bin(slot_expert[own * kPlaceBlock + tid], E) : -1;
+  for (int i = tid; i < kPlaceWaves * E / 4; i += kPlaceBlock) reinterpret_cast<int4*>(cursor)[i] = make_int4(0, 0, 0, 0);
+  for (int i = tid; i < 2 * E; i += kPlaceBlock) sums[i] = 0;
+  __syncthreads();
+  const int groups = kPlaceBlock / E, e = tid % E, g = tid / E;
+  if (g < groups) {
+    int before = 0, behind = 0;
+    for (int b0 = g; b0 < blocks; b0 += 8 * groups) {
+      int c[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = table[int64_t(min(b0 + i * groups, blocks - 1)) * E + e];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int b = b0 + i * groups;
+        before += c[i] & (b < own ? -1 : 0);
+        behind += c[i] & (b > own && b < blocks ? -1 : 0);
+      }
+    }
+    atomicAdd(&sums[e], before);
+    atomicAdd(&sums[E + e], behind);
+  }
+  moe_place(cursor, sums, part, expert, own * kPlaceBlock, E, k, own == 0, offs, row_token, token_rows);
 }
 
 // The whole routing of a decoding step, one launch: 16 tokens at a time, one to a wave, the next one's logits on their way while
@@ -395,10 +432,18 @@ bool plan_sort(int64_t tokens, int64_t top_k, SortPlan& pl) {
 }
 
 // Stable sort of the slots by expert: offs, row_token, token_rows.
+// table_shared: other calls may use it at the same time.
 int sort_planned(const int32_t* slot_expert, const SortPlan& pl, int64_t E, int64_t top_k, int32_t* offs, int32_t* row_token,
-                 int32_t* token_rows, int32_t* table, hipStream_t stream) {
+                 int32_t* token_rows, int32_t* table, bool table_shared, hipStream_t stream) {
+  const int blocks = (pl.slots + kPlaceBlock - 1) / kPlaceBlock;
+  if (pl.slots > kCountedSlots && blocks <= pl.nb && !(table_shared && pl.slots <= kPlaceSlots)) {
+    hipLaunchKernelGGL(moe_hist_kernel, dim3(blocks), dim3(256), 0, stream, slot_expert, pl.slots, kPlaceBlock, int(E), table);
+    hipLaunchKernelGGL(moe_place_counted_kernel, dim3(blocks), dim3(kPlaceBlock), 0, stream, slot_expert, pl.slots, int(E), int(top_k), table, offs,
+                       row_token, token_rows);
+    return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
+  }
   if (pl.slots > 0 && pl.slots <= kPlaceSlots) {
-    hipLaunchKernelGGL(moe_place_kernel, dim3((pl.slots + kPlaceBlock - 1) / kPlaceBlock), dim3(kPlaceBlock), 0, stream, slot_expert,
+    hipLaunchKernelGGL(moe_place_kernel, dim3(blocks), dim3(kPlaceBlock), 0, stream, slot_expert,
                        pl.slots, int(E), int(top_k), offs, row_token, token_rows);
     return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
   }
@@ -412,7 +457,7 @@ int sort_planned(const int32_t* slot_expert, const SortPlan& pl, int64_t E, int6
 
 int route_checked(const void* logits, int64_t ld, int dtype, int64_t tokens, int64_t E, int64_t top_k, int renorm,
                   int32_t* offs, int32_t* slot_expert, float* slot_weight, int32_t* row_token, int32_t* token_rows,
-                  int32_t* table, size_t table_bytes, hipStream_t stream) {
+                  int32_t* table, size_t table_bytes, bool table_shared, hipStream_t stream) {
   if (tokens < 0 || E < 1 || E > kMaxExperts || top_k < 1 || top_k > kMaxTopK || top_k > E) return GMM_ERR_BAD_ARGUMENT;
   if (dtype < GMM_DT_BF16 || dtype > GMM_DT_F32) return GMM_ERR_UNSUPPORTED;
   SortPlan pl;
@@ -448,7 +493,7 @@ int route_checked(const void* logits, int64_t ld, int dtype, int64_t tokens, int
     else topk(static_cast<const float*>(logits));
     if (one) return hipGetLastError() == hipSuccess ? GMM_OK : GMM_ERR_LAUNCH;
   }
-  return sort_planned(slot_expert, pl, E, top_k, offs, row_token, token_rows, table, stream);
+  return sort_planned(slot_expert, pl, E, top_k, offs, row_token, token_rows, table, table_shared, stream);
 }
 
 // Address of the current device's copy of `scratch`, looked up on the first call on that device.
@@ -471,7 +516,7 @@ int gmm_sort_slots(const int32_t* slot_expert, int64_t slots, int64_t E, int32_t
                    void* table, hipStream_t stream) {
   SortPlan pl;
   if (slots < 0 || E < 1 || E > kMaxExperts || !plan_sort(slots, 1, pl)) return GMM_ERR_BAD_ARGUMENT;
-  return sort_planned(slot_expert, pl, E, 1, offs, row_token, token_rows, static_cast<int32_t*>(table), stream);
+  return sort_planned(slot_expert, pl, E, 1, offs, row_token, token_rows, static_cast<int32_t*>(table), false, stream);
 }
 
 extern "C" {
@@ -487,7 +532,7 @@ int gmm_moe_route(const void* logits, int64_t logits_stride, int32_t logits_dtyp
                   int32_t* row_token, int32_t* token_rows, void* workspace, int64_t workspace_bytes, void* stream) {
   if (workspace_bytes < 0) return GMM_ERR_BAD_ARGUMENT;
   return route_checked(logits, logits_stride, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert,
-                       slot_weight, row_token, token_rows, static_cast<int32_t*>(workspace), size_t(workspace_bytes),
+                       slot_weight, row_token, token_rows, static_cast<int32_t*>(workspace), size_t(workspace_bytes), false,
                        static_cast<hipStream_t>(stream));
 }
 
@@ -497,7 +542,7 @@ int gmm_moe_route_noalloc(const void* logits, int64_t logits_stride, int32_t log
   int32_t* table = device_scratch();
   if (!table) return GMM_ERR_LAUNCH;
   return route_checked(logits, logits_stride, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert,
-                       slot_weight, row_token, token_rows, table, sizeof(int32_t) * size_t(kScratchInts),
+                       slot_weight, row_token, token_rows, table, sizeof(int32_t) * size_t(kScratchInts), true,
                        static_cast<hipStream_t>(stream));
 }
 
