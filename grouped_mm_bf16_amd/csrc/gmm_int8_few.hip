@@ -217,6 +217,14 @@ struct RowsHere {
   }
 };
 
+// LDS of a workgroup: the waves' own parts while they multiply, then the sums.
+template <typename S, int MF, int WAVES>
+union FewShared {
+  char wave[WAVES][S::LDS_BYTES > 0 ? S::LDS_BYTES : 16];
+  SkinnySums<WAVES, S::FR> sums[MF];
+  __device__ FewShared() {}
+};
+
 // FR: a strip is 16 FR columns.  GLU: half of them gate columns, the others their partners, N / 2 further on; the result is silu(gate) * partner.
 // X: the rows are values of this type, rounded here (up to 16 of them, k in one part); void: 8-bit integers.
 // ROUTE: every workgroup routes for itself (GLU and X alone).
@@ -226,10 +234,10 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   static_assert(!HERE || MF == 1, "");
   using S = Skinny<I8x2, GMM_W_COLS, FR, MF, 1, HERE ? GMM_A_RESIDENT : GMM_A_STAGED, 2>;
   constexpr int OUT = GLU ? 8 * FR : 16 * FR, THREADS = 64 * WAVES;
-  __shared__ SkinnyShared<S, WAVES> shared;
+  __shared__ FewShared<S, MF, WAVES> shared;
+  __shared__ float column_scales[16 * FR], row_scales[16 * MF];
   extern __shared__ __align__(16) char rows_here[];      // HERE: 8-bit rows
   __shared__ uint32_t most_here[16];
-  __shared__ float scale_here[16];
   if constexpr (HERE) {
     if (threadIdx.x < 16) most_here[threadIdx.x] = 0;
     __syncthreads();
@@ -262,6 +270,16 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
     const int at = ROUTE ? row_index[r] : row_index ? row_index[row0 + r] : row0 + r;
     return uint32_t(at) < uint32_t(a.a_rows) ? at : -1;
   };
+  // the scales are on their way during the product: asked for behind it they took a trip to memory each, one behind the other
+  const int mine = threadIdx.x;
+  float column_scale = 0, row_scale = 0;
+  if (mine < 16 * FR && first + mine % OUT < width) column_scale = columns[mine / OUT * width + first + mine % OUT];
+  if constexpr (!HERE) {
+    if (mine < rows) {
+      const int from = source(mine);
+      if (from >= 0) row_scale = a.a_scale[from];
+    }
+  }
   f32x4 acc[MF][FR];
   clear(acc);
   if constexpr (HERE) {
@@ -278,7 +296,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
     x.load(rows, 2 * a.K, row);
     typename S::template Cycle<1, WAVES> cycle(wave * S::KS, a.K, s.turn);
     cycle.prime(s, step);
-    x.round(rows, 2 * a.K, row, rows_here, s.pitch, most_here, scale_here);
+    x.round(rows, 2 * a.K, row, rows_here, s.pitch, most_here, row_scales);
     cycle.primed(s, step, acc);
   } else {
     s.a_buf = buffer(a.a, a.a_bytes);
@@ -288,44 +306,37 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
     });
     s.template run<WAVES>(rows, part * a.k_part, min(a.K, (part + 1) * a.k_part), wave, acc);
   }
+  __syncthreads();
 #pragma unroll
-  for (int m = 0; m < MF; ++m) {
-    if (16 * m >= rows) break;
-    __syncthreads();
-    shared.sums.put(wave, lane, acc[m]);
-    __syncthreads();
-    for (int u = threadIdx.x; u < OUT * 4; u += THREADS) {
-      const int oc = u % OUT, og = u / OUT, col = first + oc;
-      if (col >= width) continue;
-      const auto sums = [&](int c) { return shared.sums.whole(S::product_of(c), S::lane_of(c), og); };
-      const i32x4 h = sums(oc), partner = GLU ? sums(OUT + oc) : i32x4{0, 0, 0, 0};
-      const float cs = columns[col], ps = GLU ? columns[width + col] : 0.0f;
+  for (int m = 0; m < MF; ++m) shared.sums[m].put(wave, lane, acc[m]);
+  if (mine < 16 * FR) column_scales[mine] = column_scale;
+  if (!HERE && mine < 16 * MF) row_scales[mine] = row_scale;
+  __syncthreads();
+  const int blocks = (rows + 15) / 16;
+  for (int u = threadIdx.x; u < OUT * 4 * blocks; u += THREADS) {
+    const int oc = u % OUT, og = u / OUT % 4, m = u / OUT / 4, col = first + oc;
+    if (col >= width) continue;
+    const auto sums = [&](int c) { return shared.sums[m].whole(S::product_of(c), S::lane_of(c), og); };
+    const i32x4 h = sums(oc), partner = GLU ? sums(OUT + oc) : i32x4{0, 0, 0, 0};
+    const float cs = column_scales[oc], ps = GLU ? column_scales[OUT + oc] : 0.0f;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int r = 16 * m + 4 * og + v;
-        if (r >= rows) break;
-        const int64_t row = row0 + r;
-        if (a.result == kSums) {
-          static_cast<int32_t*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = h[v];
-          continue;
-        }
-        float rs;
-        if constexpr (HERE) {
-          rs = scale_here[r];
-        } else {
-          const int from = source(r);
-          rs = from < 0 ? 0.0f : a.a_scale[from];
-        }
-        const float f = scaled(h[v], cs, rs);
-        if constexpr (GLU) {
-          static_cast<float*>(a.out)[row * width + col] = f / (1.0f + __expf(-f)) * scaled(partner[v], ps, rs);
-        } else if (a.result == kJoined) {
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(f), joined(a), int((uint32_t(row) * a.N + col) * 4), 0, kDeviceScope);
-        } else if (a.result == kScaled) {
-          static_cast<float*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = f;
-        } else {
-          put(a.out, a.out_dtype, row * a.out_ld + col, f);
-        }
+    for (int v = 0; v < 4; ++v) {
+      const int r = 16 * m + 4 * og + v;
+      if (r >= rows) break;
+      const int64_t row = row0 + r;
+      if (a.result == kSums) {
+        static_cast<int32_t*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = h[v];
+        continue;
+      }
+      const float rs = row_scales[r], f = scaled(h[v], cs, rs);
+      if constexpr (GLU) {
+        static_cast<float*>(a.out)[row * width + col] = f / (1.0f + __expf(-f)) * scaled(partner[v], ps, rs);
+      } else if (a.result == kJoined) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(f), joined(a), int((uint32_t(row) * a.N + col) * 4), 0, kDeviceScope);
+      } else if (a.result == kScaled) {
+        static_cast<float*>(a.out)[(int64_t(part) * a.M + row) * a.N + col] = f;
+      } else {
+        put(a.out, a.out_dtype, row * a.out_ld + col, f);
       }
     }
   }
