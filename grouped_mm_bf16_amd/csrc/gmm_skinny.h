@@ -104,6 +104,7 @@ struct Skinny {
   const char* resident;   // GMM_A_RESIDENT: row 0 of the high plane, from k = resident_k on,
   int pitch, resident_k, resident_rows;   // bytes from one row to the next, number of rows
   uint32_t turn;          // CYCLIC: the step that is the first
+  uint32_t w_col[CYCLIC ? WL : 1];   // and byte offsets of the lane's columns, k = 0
 
   struct Step { u32x4 w[WL]; u32x4 a[AM == GMM_A_RESIDENT ? 1 : NA][AL]; };
 
@@ -143,6 +144,12 @@ struct Skinny {
       w_half = half ? half : COLUMNS;
       w_jump = half ? uint32_t(other - first - half) * w_step_n : 0;
       w_at = uint32_t(first + (lane >> 3)) * w_step_n + (lane & 7) * 16;
+      if constexpr (CYCLIC)
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+          const bool second = 8 * i >= w_half;
+          w_col[i] = 8 * i + (lane >> 3) - (second ? w_half : 0) < columns ? w_at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere;
+        }
     } else if constexpr (LAY == GMM_W_THIN) {
       const int c = lane % (2 * FR) * 8;
       columns = count - c;
@@ -164,6 +171,14 @@ struct Skinny {
     }
   }
 
+  // CYCLIC: what k adds to an offset; past the end, past every buffer (of columns and rows that do not exist it may lead back into it: their sums go
+  // nowhere).  Not asked for each load, or the compiler branches around them, and they wait for one another.
+  static __device__ __forceinline__ uint32_t from_k(bool in, int k, int at, int end) {
+    uint32_t along = in ? uint32_t(k) * 2 - back(at, end) : kNowhere;
+    asm volatile("" : "+v"(along));
+    return along;
+  }
+
   // Loads k .. k + KS - 1, of which those before `end` exist, and the first M of the sixteens of rows.
   template <int M>
   __device__ __forceinline__ void load(Step& s, int k, int end) const {
@@ -179,21 +194,20 @@ struct Skinny {
       for (int r = 0; r < 8; ++r)
         w[r] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(columns && kl + r < end ? at + r * w_step_k : kNowhere), 0, kStream);
     } else if constexpr (LAY == GMM_W_COLS) {
-      const uint32_t at = w_at + uint32_t(k) * 2 - back(k + 8 * (lane & 7), end);
       const bool in = k + 8 * (lane & 7) < end;
-      [[maybe_unused]] uint32_t outside = in ? 0 : kNowhere;
-      if constexpr (CYCLIC) asm volatile("" : "+v"(outside));      // or the compiler branches around the loads, and they wait for one another
+      if constexpr (CYCLIC) {
+        const uint32_t along = from_k(in, k, k + 8 * (lane & 7), end);
+#pragma unroll
+        for (int i = 0; i < WL; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(w_col[i] + along), 0, kStream);
+        return;
+      }
+      const uint32_t at = w_at + uint32_t(k) * 2 - back(k + 8 * (lane & 7), end);
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
         const int c = 8 * i + (lane >> 3);
         const bool second = 8 * i >= w_half;
-        if constexpr (CYCLIC) {
-          const uint32_t from = c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere;
-          w[i] = __builtin_amdgcn_raw_buffer_load_b128(w_buf, int(from | outside), 0, kStream);
-        } else {
-          w[i] = __builtin_amdgcn_raw_buffer_load_b128(
-              w_buf, int(in && c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere), 0, kStream);
-        }
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(
+            w_buf, int(in && c - (second ? w_half : 0) < columns ? at + 8 * i * w_step_n + (second ? w_jump : 0) : kNowhere), 0, kStream);
       }
     } else if constexpr (LAY == GMM_W_THIN) {
 #pragma unroll
@@ -240,6 +254,9 @@ struct Skinny {
             const uint32_t hi = element(a_buf, a_at[i] != kNowhere && kl + 2 * q + 1 < end ? at + 4 * q + 2 : kNowhere);
             s.a[p][i][q] = lo | hi << 16;
           }
+        } else if constexpr (CYCLIC) {
+          const uint32_t along = from_k(k + 8 * (lane % CH) < end, k, k + 8 * (lane % CH), end);
+          s.a[p][i] = __builtin_amdgcn_raw_buffer_load_b128(a_buf, int(a_at[i] + p * a_plane + along), 0, 0);
         } else {
           const bool in = a_at[i] != kNowhere && k + 8 * (lane % CH) < end;
           const uint32_t at = a_at[i] + p * a_plane + uint32_t(k) * 2 - back(k + 8 * (lane % CH), end);

@@ -183,7 +183,8 @@ def _check_columns(what: str, b: Columns, device: torch.device, dims: int) -> No
         raise RuntimeError(f"{what}: K is at most {MAX_K}, got {K}")
     if values.device != device or scale.device != device:
         raise RuntimeError(f"{what}: all operands have to be on {device}")
-    _forward_only(what, scale)
+    if scale.requires_grad or derivatives.forward_mode():
+        _forward_only(what, scale)
 
 
 def _check_rows(what: str, a: Rows, K: int) -> None:
