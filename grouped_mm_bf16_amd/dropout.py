@@ -20,19 +20,21 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as a matrix of rows whose elements are contiguous; copied only where its strides allow no such view."""
     if x.dim() != 2:
         x = x.reshape(-1, x.size(-1)) if x.numel() and x.dim() else x.reshape(1, x.numel())
-    if x.numel() and (x.stride(1) != 1 and x.size(1) > 1 or x.size(0) > 1 and x.stride(0) < x.size(1)):
-        x = x.contiguous()
-    return x
+    if x.is_contiguous():
+        return x
+    (rows, width), (step, between) = x.shape, x.stride()
+    return x.contiguous() if between != 1 and width > 1 or rows > 1 and step < width else x
 
 
 def _launch(x: torch.Tensor, limit: int, rng: torch.Tensor, site: int, residual: Optional[torch.Tensor], used: Optional[torch.Tensor]) -> torch.Tensor:
     rows, width = x.shape
-    out = torch.empty(rows, width, device=x.device, dtype=x.dtype)
+    device, dtype = x.device, x.dtype
+    out = torch.empty(rows, width, device=device, dtype=dtype)
     with _guard(x):
         rc = _lib.load().gmm_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(), rng.data_ptr(),
                                      None if used is None else used.data_ptr(), rows, width, x.stride(0),
-                                     0 if residual is None else residual.stride(0), width, limit, site, _dtype_code(x.dtype),
-                                     kernels.current_stream(x.device))
+                                     0 if residual is None else residual.stride(0), width, limit, site, _dtype_code(dtype),
+                                     kernels.current_stream(device))
     _lib.check(rc, "dropout")
     return out
 
@@ -99,7 +101,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: Optional[tor
         raise RuntimeError(f"dropout: site has to be in [0, 65536), got {site}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise RuntimeError(f"dropout: residual has to be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
-    if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
+    if rng.dtype != torch.int64 or rng.dim() != 1 or rng.numel() != 2 or not rng.is_contiguous():
         raise RuntimeError("dropout: rng has to be a contiguous int64 tensor of two elements, seed and offset")
     _require_gpu(x)
     if rng.device != x.device or residual is not None and residual.device != x.device:

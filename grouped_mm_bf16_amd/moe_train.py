@@ -23,7 +23,10 @@ MAX_TOP_K = 32
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x with contiguous rows that do not overlap; copied only where they do not lie so."""
-    if x.numel() and (x.stride(1) != 1 and x.size(1) > 1 or x.size(0) > 1 and x.stride(0) < x.size(1)):
+    if x.is_contiguous():
+        return x
+    (rows, width), (step, between) = x.shape, x.stride()
+    if between != 1 and width > 1 or rows > 1 and step < width:
         return x.contiguous()
     return x
 
@@ -83,12 +86,16 @@ def _check_rows(what: str, x: torch.Tensor, routing: Routing, slots: int, weight
     if x.dim() != 2:
         raise RuntimeError(f"{what} takes a 2D tensor, got {x.dim()}D")
     _require_gpu(x)
-    for name, dtype in (("token_rows", torch.int32),) + ((("slot_weight", torch.float32),) if weights else ()):
-        t = getattr(routing, name)
-        if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or t.device != x.device:
-            raise RuntimeError(f"{what}: routing.{name} has to be a contiguous 1D {dtype} tensor on {x.device}, got {t.dim()}D {t.dtype} on {t.device}")
-        if t.numel() != slots:
-            raise RuntimeError(f"{what}: routing.{name} has to have tokens * top_k = {slots} elements, got {t.numel()}")
+    _check_routing(what, "token_rows", routing.token_rows, torch.int32, x.device, slots)
+    if weights:
+        _check_routing(what, "slot_weight", routing.slot_weight, torch.float32, x.device, slots)
+
+
+def _check_routing(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, slots: int) -> None:
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or t.device != device:
+        raise RuntimeError(f"{what}: routing.{name} has to be a contiguous 1D {dtype} tensor on {device}, got {t.dim()}D {t.dtype} on {t.device}")
+    if t.numel() != slots:
+        raise RuntimeError(f"{what}: routing.{name} has to have tokens * top_k = {slots} elements, got {t.numel()}")
 
 
 def _sort_now(x: torch.Tensor, token_rows: torch.Tensor) -> torch.Tensor:
@@ -221,11 +228,12 @@ def combine_rows(y: torch.Tensor, routing: Routing, top_k: int) -> torch.Tensor:
 
 # ------------------------------------------------------------------ activation
 def _gated_now(h: torch.Tensor, kind: int) -> torch.Tensor:
-    rows, inner = h.size(0), h.size(1) // (1 + kind)
-    out = torch.empty(rows, inner, device=h.device, dtype=h.dtype)
+    rows, width = h.shape
+    inner, device, dtype = width // 2 if kind else width, h.device, h.dtype
+    out = torch.empty(rows, inner, device=device, dtype=dtype)
     with _guard(h):
-        rc = _lib.load().gmm_gated(h.data_ptr(), out.data_ptr(), rows, inner, h.stride(0), inner, kind, _dtype_code(h.dtype),
-                                   kernels.current_stream(h.device))
+        rc = _lib.load().gmm_gated(h.data_ptr(), out.data_ptr(), rows, inner, h.stride(0), inner, kind, _dtype_code(dtype),
+                                   kernels.current_stream(device))
     _lib.check(rc, "gated")
     return out
 
@@ -239,10 +247,12 @@ def _gated_fake(h, kind):
 
 
 def _gated_backward_now(grad: torch.Tensor, h: torch.Tensor, kind: int) -> torch.Tensor:
-    out = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    rows, width = h.shape
+    device, dtype = h.device, h.dtype
+    out = torch.empty(rows, width, device=device, dtype=dtype)
     with _guard(h):
-        rc = _lib.load().gmm_gated_backward(grad.data_ptr(), h.data_ptr(), out.data_ptr(), h.size(0), grad.size(1), grad.stride(0), h.stride(0),
-                                            h.size(1), kind, _dtype_code(h.dtype), kernels.current_stream(h.device))
+        rc = _lib.load().gmm_gated_backward(grad.data_ptr(), h.data_ptr(), out.data_ptr(), rows, width // 2 if kind else width, grad.stride(0),
+                                            h.stride(0), width, kind, _dtype_code(dtype), kernels.current_stream(device))
     _lib.check(rc, "gated backward")
     return out
 
