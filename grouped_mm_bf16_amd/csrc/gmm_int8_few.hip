@@ -380,30 +380,56 @@ __global__ void __launch_bounds__(kThreads) int8_combine_kernel(const float* __r
 }
 
 // ---------------------------------------------------------------- host side
-// How a product of up to `rows` rows of a group is laid out.  Measured alone, us, for rows x N x K of one matrix, weights from memory:
-//   64 columns, 4 waves    where such strips fill half the compute units and more: 1 x 14336 x 4096 12.5 (32 columns 13.0, 16 columns 15.9), 1 x 9216
-//                          x 2048 6.2 (7.4, 10.3), 48 x 14336 x 4096 18.1 (25.1; 64 in two parts 22.6), 48 x 9216 x 2048 11.6 (17.9); but 1 x 8192 x
-//                          8192 15.3 (16 columns 13.4), 48 x 8192 x 8192 24.6 (32 columns 21.3)
-//   16 columns, 16 waves   fewer columns and long, up to 16 rows: 1 x 4096 x 4096 6.2 (32 columns 6.5, 64 in three parts 7.7), 1 x 4096 x 14336 12.5
-//                          (13.5 in two parts, 13.3 in three); but 1 x 1536 x 2048 4.9 (4.3), 1 x 6144 x 768 5.5 (4.2)
-//   32 columns, 8 waves    what is left: short columns, or more rows, which narrower strips would read too often, then in as many parts of k as
-//                          fill the compute units: 48 x 4096 x 4096 12.3 in two parts, 12.9 in one (64 columns in three 12.7), 24 x 1536 x 2048 7.5
-//                          in four (7.4 in one), 48 x 4096 x 14336 20.3 in two (64 columns in four 19.2)
+// How a product of up to `rows` rows of a group is laid out.  Measured alone, us, for rows x N x K of one matrix, weights from memory (8-bit rows unless
+// said otherwise):
+//   64 columns, 4 waves    where such strips fill half the compute units and more: 1 x 14336 x 4096 11.6 (32 columns 12.2), 1 x 9216 x 2048 6.4 (7.8),
+//                          48 x 14336 x 4096 16.6 (21.3; 64 in two parts 23.2), 48 x 9216 x 2048 11.2 (14.9); but 1 x 8192 x 8192 14.4 (14.4), 1 x 7168 x
+//                          7168 13.5 (11.1), 48 x 8192 x 8192 23.1 (18.8)
+//   16 columns, 16 waves   up to 16 rows, one round of long strips: 1 x 4096 x 14336 12.7 (32 columns 14.7, in two parts 13.8), 1 x 1024 x 8192 7.0 (8.5),
+//                          1 x 4096 x 4096 6.4 (6.4); but 1 x 4608 x 4608, more than a round, 10.5 (7.0), 1 x 2048 x 2048 5.3 (4.6)
+//   32 columns, 8 waves    what is left; of more rows and long columns in as many parts of k as fill the compute units: 48 x 4096 x 8192 14.0 in two
+//                          parts, 16.5 in one, 48 x 2048 x 8192 11.3 in four; 64 x 1024 x 4096 10.3, 11.5 in one; but 48
+//                          x 4096 x 4096 11.4 and 10.7, 48 x 1536 x 2048 8.4 in four and 7.8
+//   64 columns in parts    the longest, where four or more parts fill the compute units: 48 x 4096 x 28672 27.7 (32 columns in two parts 30.3), x 14336
+//                          19.3 (20.1), x 11008 17.1 (17.2); but 32 x 6144 x 16384 25.3 (32 columns 23.5), 64 x 2048 x 14336 16.3 in eight (15.7 in four)
+// Rows that every workgroup rounds for itself are rounded by more threads where it has more waves: 1 x 14336 x 4096 11.9 with 32 columns (64 14.4), 4 rows
+// 16.3 (19.8), 1 x 6144 x 4096 8.6 (16 columns 10.5), 1 x 2048 x 2048 5.3 with 16 (32 5.7); but 1 x 28672 x 2048 15.5 with 32 (64 12.2).
 struct Shape { int32_t columns, parts, k_part; };
 
+constexpr int64_t kStep = 64;      // k of a wave's step
+
 Shape few_shape(int64_t used, int64_t rows, int64_t N, int64_t K) {
-  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256, step = 64;
+  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256;
   const auto strips = [&](int64_t columns) { return used * ((N + columns - 1) / columns); };
-  Shape s{64, 1, int32_t(round_up(K, step))};
+  Shape s{64, 1, int32_t(round_up(K, kStep))};
   if (16 * strips(64) >= 9 * cus) return s;
-  s.columns = rows <= 16 && K >= 2048 ? 16 : 32;
-  if (rows <= 16) return s;
-  int64_t want = strips(32) > 0 ? cus / strips(32) : 1;
-  if (want > K / (8 * step)) want = K / (8 * step);      // a step for each wave
+  s.columns = rows <= 16 && K >= 2048 && strips(16) <= cus ? 16 : 32;
+  if (rows <= 16 || K <= 1024 || (K <= 2048 && 4 * strips(32) > cus)) return s;
+  if (K >= 6144 && 8 * strips(64) > cus && 4 * strips(64) <= cus) s.columns = 64;
+  int64_t want = strips(s.columns) > 0 ? cus / strips(s.columns) : 1;
+  if (want > K / (8 * kStep)) want = K / (8 * kStep);      // a step for each wave
   if (want <= 1) return s;
-  s.k_part = int32_t(round_up((K + want - 1) / want, step));
+  s.k_part = int32_t(round_up((K + want - 1) / want, kStep));
   s.parts = int32_t((K + s.k_part - 1) / s.k_part);
   return s;
+}
+
+// Are the rows rounded by every workgroup for itself?  1 x 4096 x 4096 with its rounding 6.0 us, in a launch of its own 2.3 and 5.4.
+bool rounds_here(int64_t rows, int64_t K, const Shape& s, int32_t x_dtype) {
+  const int64_t threads = s.columns == 64 ? 256 : s.columns == 32 ? 512 : 1024, each = x_dtype == GMM_DT_F32 ? kAccesses<float> : kAccesses<Bf16>;
+  return rows <= 16 && s.parts == 1 && rows * K <= kMostRounded && rows * ((K + 7) / 8) <= threads * each;
+}
+
+// The same of rows of x_dtype that may be rounded here.
+Shape few_shape(int64_t used, int64_t rows, int64_t N, int64_t K, int32_t x_dtype) {
+  const int64_t cus = gmm_num_cus() > 0 ? gmm_num_cus() : 256;
+  const auto strips = [&](int64_t columns) { return used * ((N + columns - 1) / columns); };
+  const Shape s = few_shape(used, rows, N, K);
+  Shape h{64, 1, int32_t(round_up(K, kStep))};
+  if (K >= 1024 && strips(16) <= cus) h.columns = 16;
+  else if (K >= 2048 && strips(32) <= 2 * cus) h.columns = 32;      // all of them at once
+  else h.columns = s.columns;
+  return rounds_here(rows, 2 * K, h, x_dtype) ? h : s;
 }
 
 void set_shape(FewArgs& a, const Shape& s, bool glu = false) {
@@ -430,12 +456,6 @@ bool sizes_fit(FewArgs& a) {
   a.a_bytes = uint32_t((int64_t(a.a_rows - 1) * a.a_ld + a.K) * 2);
   a.b_bytes = matrix_bytes(a.K, a.N, 1, a.b_ld);
   return a.K >= 8 && a.b_bytes != 0;
-}
-
-// Are the rows rounded by every workgroup for itself?  1 x 4096 x 4096 with its rounding 6.0 us, in a launch of its own 2.3 and 5.4.
-bool rounds_here(int64_t rows, int64_t K, const Shape& s, int32_t x_dtype) {
-  const int64_t threads = s.columns == 64 ? 256 : s.columns == 32 ? 512 : 1024, each = x_dtype == GMM_DT_F32 ? kAccesses<float> : kAccesses<Bf16>;
-  return rows <= 16 && s.parts == 1 && rows * K <= kMostRounded && rows * ((K + 7) / 8) <= threads * each;
 }
 
 // Do the workgroups of this product route for themselves?  In one round of them, in which that is as long in all as in one.  1 token, 8 of 128 experts
@@ -500,8 +520,7 @@ int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_byt
   a.out_dtype = out_dtype;
   a.result = kOut;
   if (a.offs || !planes || planes_bytes < gmm_int8_few_bytes(p)) {      // the planes do not say whose scales their rows take
-    a.parts = 1;
-    a.k_part = int32_t(round_up(a.K, 64));
+    if (a.parts > 1) set_shape(a, Shape{32, 1, int32_t(round_up(a.K, kStep))});
   }
   if (a.parts == 1) return launch<false>(a, stream);
   FewArgs u = a;
@@ -517,13 +536,13 @@ int gmm_launch_int8_few(const GmmInt8Params& p, void* planes, int64_t planes_byt
 namespace {
 
 // ---------------------------------------------------------------- linear layer
-struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; bool here; };
+struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; Shape shape; bool here; };
 
 bool plan_linear(int64_t T, int64_t K, int64_t N, int32_t dtype, LinearPlan& p) {
   if (T < 0 || T > kMaxTokens || K < 0 || K >= 131072 || N < 0 || N >= (int64_t(1) << 31)) return false;
-  const Shape shape = few_shape(1, T, N, K / 2);
-  const int64_t parts = shape.parts;
-  p.here = rounds_here(T, K, shape, dtype);
+  p.shape = few_shape(1, T, N, K / 2, dtype);
+  const int64_t parts = p.shape.parts;
+  p.here = rounds_here(T, K, p.shape, dtype);
   p.pitch = round_up(K > 0 ? K : 1, 16);
   p.scale_at = T * p.pitch;
   p.planes_at = round_up(p.scale_at + 4 * T, 16);
@@ -548,9 +567,9 @@ bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t k
   const int64_t N = kind == GMM_ACT_SWIGLU ? 2 * I : I;
   p.slots = T * k;
   p.used = p.slots < E ? p.slots : E;
-  p.up = few_shape(p.used, T, N, H / 2);
-  p.down = few_shape(p.used, T, H, I / 2);
+  p.up = few_shape(p.used, T, N, H / 2, GMM_DT_BF16);
   p.activated = p.up.parts == 1 && kind == GMM_ACT_SWIGLU;
+  p.down = p.activated ? few_shape(p.used, T, H, I / 2, GMM_DT_F32) : few_shape(p.used, T, H, I / 2);
   p.x_here = rounds_here(T, H, p.up, GMM_DT_BF16);
   p.act_here = p.activated && rounds_here(T, I, p.down, GMM_DT_F32);
   p.join = p.activated && p.slots <= kJoinSlots && p.down.parts == 1;
@@ -602,6 +621,7 @@ int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* 
   if (plan.here) {
     FewArgs f = from_params(p);
     f.a = x; f.a_ld = rows > 1 ? x_stride : K; f.x_dtype = dtype; f.out_dtype = dtype; f.result = kOut;
+    set_shape(f, plan.shape);
     return sizes_fit(f) ? launch<false>(f, static_cast<hipStream_t>(stream)) : GMM_ERR_UNSUPPORTED;
   }
   const int rc = gmm_int8_quantize(x, reinterpret_cast<int8_t*>(ws), reinterpret_cast<float*>(ws + plan.scale_at), rows, K, x_stride, plan.pitch,
