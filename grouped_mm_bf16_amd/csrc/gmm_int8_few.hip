@@ -25,7 +25,8 @@ namespace {
 using namespace gmm;
 
 constexpr int kThreads = 256;      // of the kernels behind the products
-constexpr int kMaxTokens = 64;
+constexpr int kMaxRows = 64;       // of a block
+constexpr int kMostRows = 256;     // of one matrix; tokens of an expert layer
 
 enum Result : int { kOut, kSums, kScaled, kActivated, kJoined };
 
@@ -46,7 +47,7 @@ struct FewArgs {
   int64_t a_ld, b_sg, b_ld, out_ld;      // pairs of integers (out_ld: elements)
   uint32_t a_bytes, b_bytes;
   int32_t G, M, N, K, a_rows; // K: pairs
-  int32_t used, most;         // groups that can have rows; rows that a group can have, 64 at most
+  int32_t most, block, items; // rows that a group can have; rows of a block, a multiple of 16; blocks of one group's rows that there can be
   int32_t columns, tiles, parts, k_part;      // of a strip (with its partners); strips; parts along k and their length
   int32_t result, out_dtype;
   int32_t x_dtype;            // of rows that are rounded here: a is x, a_ld its elements from one row to the next
@@ -63,7 +64,8 @@ struct FewArgs {
 
 constexpr int kNotRounded = -1;
 
-// The `which`-th group that has rows, found by every wave for itself.
+// The `which`-th block of up to BLOCK rows of a group, found by every wave for itself.
+template <int BLOCK>
 __device__ __forceinline__ bool find_group(const FewArgs& a, int which, int& g, int& row0, int& rows) {
   constexpr int AT_ONCE = 4;
   const int lane = threadIdx.x & 63;
@@ -78,13 +80,25 @@ __device__ __forceinline__ bool find_group(const FewArgs& a, int which, int& g, 
       const int to = min(max(ends[i], 0), a.M), before = __shfl_up(to, 1), from = lane ? before : start;
       start = __builtin_amdgcn_readlane(to, 63);
       const uint64_t with = __ballot(there && to > from);
-      const int n = __popcll(with);
+      int ahead = __popcll(with & ((uint64_t(1) << lane) - 1)), n = __popcll(with), own = there && to > from;      // blocks of lanes before the own
+      if (a.most > BLOCK) {      // a group may have several
+        own = own ? (to - from + BLOCK - 1) / BLOCK : 0;
+        ahead = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int up = __shfl_up(ahead, o);
+          ahead += lane >= o ? up : 0;
+        }
+        n = __builtin_amdgcn_readlane(ahead, 63);
+        ahead -= own;
+      }
       if (which < used + n) {
-        const uint64_t it = __ballot(there && to > from && __popcll(with & ((uint64_t(1) << lane) - 1)) == which - used);
+        const uint64_t it = __ballot(ahead <= which - used && which - used < ahead + own);
         const int at = __ffsll(static_cast<unsigned long long>(it)) - 1;
         g = base + 64 * i + at;
-        row0 = __builtin_amdgcn_readlane(from, at);
-        rows = __builtin_amdgcn_readlane(to, at) - row0;
+        const int skip = (which - used - __builtin_amdgcn_readlane(ahead, at)) * BLOCK;
+        row0 = __builtin_amdgcn_readlane(from, at) + skip;
+        rows = min(__builtin_amdgcn_readlane(to, at) - row0, BLOCK);
         return true;
       }
       used += n;
@@ -117,7 +131,7 @@ __device__ __forceinline__ void join(const FewArgs& a, int tile) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)
-    last = __hip_atomic_fetch_add(&a.arrived[tile * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(a.used) - 1;
+    last = __hip_atomic_fetch_add(&a.arrived[tile * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(a.items) - 1;
   if (int(threadIdx.x) < a.M) {
     rows[threadIdx.x] = a.token_rows[threadIdx.x];
     weights[threadIdx.x] = a.slot_weight[threadIdx.x];
@@ -245,13 +259,13 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   if (GLU && blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.clear; i += THREADS) a.arrived[i * kLine] = 0;
   const int part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, tile = item % a.tiles;
-  int g = 0, row0 = 0, rows = a.M;
+  int g = 0, row0 = a.offs ? 0 : item / a.tiles * 16 * MF, rows = min(a.M - row0, 16 * MF);
   const int32_t* row_index = a.row_index;      // of the group's rows
   if constexpr (ROUTE) {
     __shared__ FewRouting routing;
     if (!route_here<WAVES>(a.route, routing, item / a.tiles, g, row0, rows)) return;
     row_index = routing.token;
-  } else if (a.offs && !find_group(a, item / a.tiles, g, row0, rows)) {
+  } else if (a.offs && !find_group<16 * MF>(a, item / a.tiles, g, row0, rows)) {
     if constexpr (!GLU && MF == 1) if (a.result == kJoined) join<OUT, THREADS>(a, tile);      // it is counted as well
     return;
   }
@@ -262,7 +276,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 || MF == 4 ? 1 : 2) int
   s.lds = shared.wave[wave];
   s.w_buf = buffer(static_cast<const uint16_t*>(a.b) + g * a.b_sg, a.b_bytes);
   s.a_plane = 0;
-  s.turn = blockIdx.x / 8;
+  s.turn = (g * a.tiles + tile) * a.parts / 8;      // the same for all blocks of rows
   if constexpr (GLU) s.set_columns(first, width - first, 1, uint32_t(a.b_ld), OUT, width + first);
   else s.set_columns(first, width - first, 1, uint32_t(a.b_ld));
   const float* const columns = a.b_scale + int64_t(g) * a.N;
@@ -445,9 +459,10 @@ FewArgs from_params(const GmmInt8Params& p) {
   a.out = p.c; a.a_ld = p.a_sm; a.b_sg = p.b_sg; a.b_ld = p.b_sn; a.out_ld = p.c_sm;
   a.G = p.G; a.M = p.M; a.N = p.N; a.K = p.K; a.a_rows = p.gather ? p.a_rows : p.M;
   a.x_dtype = kNotRounded;
-  a.used = a.offs ? gmm_min(p.G, p.M) : 1;
   a.most = p.M;
-  set_shape(a, few_shape(a.used, a.most, a.N, a.K));
+  a.items = a.offs ? gmm_min(p.G, p.M) : int32_t((p.M + kMaxRows - 1) / kMaxRows);      // one matrix: blocks of the same length
+  a.block = int32_t(round_up(a.offs || a.items == 0 ? p.M : (p.M + a.items - 1) / a.items, 16));
+  set_shape(a, few_shape(a.items, gmm_min(a.most, a.block), a.N, a.K));
   return a;
 }
 
@@ -468,7 +483,7 @@ bool routes_here(int64_t used, int64_t tiles, int64_t slots, int64_t experts) {
 template <typename X, bool GLU, bool ROUTE = false>
 int launch_rows(const FewArgs& a, hipStream_t stream) {
   constexpr bool HERE = !std::is_void_v<X>;
-  const dim3 grid(unsigned(int64_t(a.used) * a.tiles * a.parts));
+  const dim3 grid(unsigned(int64_t(a.items) * a.tiles * a.parts));
   const int lds = HERE ? a.most * ((a.K * 2 + 31) & ~15) : 0;
   const auto go = [&](auto mf, auto fr, auto waves) {
     constexpr int MF = decltype(mf)::value, FR = decltype(fr)::value, WAVES = decltype(waves)::value;
@@ -476,9 +491,9 @@ int launch_rows(const FewArgs& a, hipStream_t stream) {
   };
   const auto by_rows = [&](auto fr, auto waves) {
     if constexpr (!HERE) {
-      if (a.most > 48) return go(std::integral_constant<int, 4>{}, fr, waves);
-      if (a.most > 32) return go(std::integral_constant<int, 3>{}, fr, waves);
-      if (a.most > 16) return go(std::integral_constant<int, 2>{}, fr, waves);
+      if (a.block > 48) return go(std::integral_constant<int, 4>{}, fr, waves);
+      if (a.block > 32) return go(std::integral_constant<int, 3>{}, fr, waves);
+      if (a.block > 16) return go(std::integral_constant<int, 2>{}, fr, waves);
     }
     go(std::integral_constant<int, 1>{}, fr, waves);
   };
@@ -505,8 +520,13 @@ int launch(const FewArgs& a, hipStream_t stream) {
 
 bool gmm_int8_few_preferred(const GmmInt8Params& p) {
   FewArgs a = from_params(p);
-  if (p.k_odd || !sizes_fit(a) || int64_t(a.used) * a.tiles >= (int64_t(1) << 27)) return false;
-  return p.M <= kMaxTokens;
+  if (p.k_odd || !sizes_fit(a) || int64_t(a.items) * a.tiles >= (int64_t(1) << 27)) return false;
+  if (p.M <= kMaxRows || a.offs) return p.M <= kMaxRows;
+  // Blocks of rows read the weights again, from the caches at best, where the tile has fewer tiles than compute units.  us, tile / here: 65 x 4096 x 4096
+  // 31.6 / 10.6, 256 34.1 / 17.4; 96 x 14336 x 4096 34.5 / 27.3, 128 35.6 / 36.2; 256 x 4096 x 14336 74.3 / 40.2; 160 x 6144 x 1024 15.1 / 14.3, 192 15.3
+  // / 20.1; 96 x 9216 x 2048 21.3 / 15.9, 128 21.8 / 24.8; 65 x 28672 x 4096 41.6 / 45.8.
+  const int64_t work = int64_t((p.N + 63) / 64) * ((p.M + 15) / 16);
+  return p.M <= kMostRows && (work <= 1024 || (work <= 1536 && p.K >= 2048));
 }
 
 int64_t gmm_int8_few_bytes(const GmmInt8Params& p) {
@@ -539,7 +559,7 @@ namespace {
 struct LinearPlan { int64_t pitch, scale_at, planes_at, bytes; Shape shape; bool here; };
 
 bool plan_linear(int64_t T, int64_t K, int64_t N, int32_t dtype, LinearPlan& p) {
-  if (T < 0 || T > kMaxTokens || K < 0 || K >= 131072 || N < 0 || N >= (int64_t(1) << 31)) return false;
+  if (T < 0 || T > kMaxRows || K < 0 || K >= 131072 || N < 0 || N >= (int64_t(1) << 31)) return false;
   p.shape = few_shape(1, T, N, K / 2, dtype);
   const int64_t parts = p.shape.parts;
   p.here = rounds_here(T, K, p.shape, dtype);
@@ -552,7 +572,7 @@ bool plan_linear(int64_t T, int64_t K, int64_t N, int32_t dtype, LinearPlan& p) 
 
 // ---------------------------------------------------------------- expert layer
 struct LayerPlan {
-  int64_t slots, used, x_pitch, act_pitch, table_bytes;
+  int64_t slots, used, block, items, x_pitch, act_pitch, table_bytes;
   int64_t table_at, arrived_at, x_at, x_scale_at, h_at, act_at, act_scale_at, y_at, bytes;
   Shape up, down;
   bool activated;      // by the first product
@@ -561,12 +581,20 @@ struct LayerPlan {
 };
 
 bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t kind, LayerPlan& p) {
-  if (T < 0 || T > kMaxTokens || E < 1 || H < 1 || I < 1 || H >= 131072 || I >= 131072 || k < 1) return false;
+  if (T < 0 || T > kMostRows || E < 1 || H < 1 || I < 1 || H >= 131072 || I >= 131072 || k < 1) return false;
   p.table_bytes = gmm_moe_route_workspace_bytes(T, E, k);
   if (p.table_bytes < 0 || k > 32 || k > E) return false;
   const int64_t N = kind == GMM_ACT_SWIGLU ? 2 * I : I;
   p.slots = T * k;
   p.used = p.slots < E ? p.slots : E;
+  // Experts have about as many rows as each other: blocks of one and a half times that, and what an expert has more is another one.  More rows than that on
+  // average, or tokens than kMostRows: through tiles.  us by rows of a block (and tiles): 64 tokens, 8 of 128 experts of 2048 -> 2 x 768, 4 rows 16: 121, 32:
+  // 123, 64: 186 (144), 192 tokens, 12 rows 144, 138, 220 (150); 2 of 8 of 4096 -> 2 x 14336, 96 tokens, 24 rows 32: 257, 48: 264 (335), 128, 32 rows 347, 283
+  // (343), 192, 48 rows 490, 394 (352); 6 of 64 of 2048 -> 2 x 1408, 256 tokens, 24 rows 140, 151 (139)
+  if (T > kMaxRows && p.slots > 32 * p.used) return false;
+  p.block = p.slots <= 24 * p.used ? 32 : p.slots <= 32 * p.used ? 48 : kMaxRows;
+  if (p.block > round_up(T, 16)) p.block = round_up(T, 16);
+  p.items = T <= p.block ? p.used : p.used + p.slots / p.block;
   p.up = few_shape(p.used, T, N, H / 2, GMM_DT_BF16);
   p.activated = p.up.parts == 1 && kind == GMM_ACT_SWIGLU;
   p.down = p.activated ? few_shape(p.used, T, H, I / 2, GMM_DT_F32) : few_shape(p.used, T, H, I / 2);
@@ -661,8 +689,8 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   FewArgs u{};
   u.a = ws + p.x_at; u.a_scale = at(p.x_scale_at); u.a_ld = p.x_pitch / 2; u.a_rows = int32_t(tokens); u.row_index = row_token;
   u.b = w_up; u.b_scale = up_scale; u.b_sg = up_stride_g / 2; u.b_ld = up_stride_n / 2; u.offs = offs; u.out = ws + p.h_at;
-  u.G = int32_t(experts); u.M = int32_t(p.slots); u.N = int32_t(N); u.K = int32_t(hidden / 2); u.used = int32_t(p.used);
-  u.most = int32_t(tokens);      // a token chooses an expert once
+  u.G = int32_t(experts); u.M = int32_t(p.slots); u.N = int32_t(N); u.K = int32_t(hidden / 2);
+  u.most = int32_t(tokens); u.block = int32_t(p.block); u.items = int32_t(p.items);      // a token chooses an expert once
   u.x_dtype = kNotRounded;
   if (p.x_here) { u.a = x; u.a_ld = tokens > 1 ? x_stride : hidden; u.x_dtype = dtype; }
   set_shape(u, p.up, p.activated);
@@ -670,8 +698,8 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
   FewArgs d{};
   d.a = ws + p.act_at; d.a_scale = at(p.act_scale_at); d.a_ld = p.act_pitch / 2; d.a_rows = int32_t(p.slots);
   d.b = w_down; d.b_scale = down_scale; d.b_sg = down_stride_g / 2; d.b_ld = down_stride_n / 2; d.offs = offs; d.out = ws + p.y_at;
-  d.G = int32_t(experts); d.M = int32_t(p.slots); d.N = int32_t(hidden); d.K = int32_t(inner / 2); d.used = int32_t(p.used);
-  d.most = int32_t(tokens);
+  d.G = int32_t(experts); d.M = int32_t(p.slots); d.N = int32_t(hidden); d.K = int32_t(inner / 2);
+  d.most = int32_t(tokens); d.block = int32_t(p.block); d.items = int32_t(p.items);
   d.x_dtype = kNotRounded;
   if (p.act_here) { d.a = ws + p.h_at; d.a_ld = inner; d.x_dtype = GMM_DT_F32; }
   set_shape(d, p.down);
@@ -683,7 +711,7 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
     u.clear = d.tiles;
   }
   if (!sizes_fit(u) || !sizes_fit(d)) return GMM_ERR_UNSUPPORTED;
-  if (p.used * u.tiles * u.parts >= (int64_t(1) << 31) || p.used * d.tiles * d.parts >= (int64_t(1) << 31)) return GMM_ERR_UNSUPPORTED;
+  if (p.items * u.tiles * u.parts >= (int64_t(1) << 31) || p.items * d.tiles * d.parts >= (int64_t(1) << 31)) return GMM_ERR_UNSUPPORTED;
 
   int rc = GMM_OK;
   const int64_t logits_ld = tokens > 1 ? logits_stride : experts;

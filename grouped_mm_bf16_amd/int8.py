@@ -4,7 +4,7 @@ layer, the grouped product, and the whole mixture-of-experts layer, whose activa
     y[t, n] = a.scale[t] * b.scale[n] * sum over k of a.values[t, k] * b.values[k, n]
 
 Weights are rounded once (:func:`quantize_columns`), activations in each call (:func:`quantize_rows`).  Sums are exact, scales are applied in
-float32, the result is rounded once.  No count reaches the host.  Up to ``FEW_ROWS`` rows weights are streamed past the rows, more go through tiles.
+float32, the result is rounded once.  No count reaches the host.  Past a few rows weights are streamed, more go through tiles.
 Registered as torch custom ops (``grouped_mm_bf16_amd::int8_quantize``, ``int8_mm``, ``int8_linear``, ``int8_layer``), which calls dispatch to while a
 model around them is being traced or compiled.  Forward only.  The reference has no counterpart.
 """
@@ -34,7 +34,8 @@ class Columns(NamedTuple):
     scale: torch.Tensor      # float32 [N] or [G, N]
 
 
-FEW_ROWS = 64        # up to which weights are streamed past the rows, not tiled
+FEW_ROWS = 64        # up to which a linear layer rounds its rows and streams the weights past them in one call
+FEW_TOKENS = 256     # up to which an expert layer does, if its experts have 32 rows each or fewer (up to FEW_ROWS tokens: any number)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -314,7 +315,7 @@ def _activated(a: Rows, routing: moe.Routing, up: torch.Tensor, up_scale: torch.
 def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor,
                top_k: int, kind: int, renormalize: bool) -> torch.Tensor:
     (T, H), (E, inner, _) = x.shape, down.shape
-    if 0 < T <= FEW_ROWS:
+    if 0 < T <= FEW_TOKENS:
         rows = x if x.is_contiguous() else moe_train._rows(x)
         (b, up_g, up_n), (d, down_g, down_n) = _columns(up), _columns(down)
         logits = router_logits if T == 1 and router_logits.stride(1) == 1 else moe_train._rows(router_logits)
@@ -350,8 +351,8 @@ def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_up: Columns
     either product.
 
     x [T, H], bf16 or fp16; router_logits [T, E]; w_up of :func:`quantize_columns`, [E, H, I] ("silu") or [E, H, 2 I] ("swiglu": gate columns first);
-    w_down [E, I, H].  The activation takes the first product in float32.  Of more than ``FEW_ROWS`` tokens the experts' rows are rounded to x's type and
-    their weighted sum again, of fewer the sum alone.  Forward only.
+    w_down [E, I, H].  The activation takes the first product in float32.  Up to ``FEW_TOKENS`` tokens whose experts have few rows each the weighted sum alone
+    is rounded to x's type, of more the experts' rows as well.  Forward only.
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
         raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")

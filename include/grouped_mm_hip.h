@@ -348,7 +348,8 @@ int gmm_int8_gate_up(const int8_t* a, const float* a_scale, const int32_t* row_i
  *                     at least 16 (else GMM_ERR_UNSUPPORTED)
  *   gmm_int8_moe_few  gmm_moe_route, then sum over j < top_k of slot_weight[t, j] * (act(x[t] @ w_up[e]) @ w_down[e]): w_up [experts, hidden, inner or
  *                     2 * inner (kind GMM_ACT_SWIGLU: gate columns, then partners)], w_down [experts, inner, hidden], x and the activations rounded to 8
- *                     bits, everything else in fp32, rounded once.  tokens <= 64, hidden and inner even and at least 16, dtype bf16 or fp16 (else
+ *                     bits, everything else in fp32, rounded once.  tokens <= 64, or <= 256 with at most 32 choices for an expert on average
+ *                     (tokens * top_k <= 32 * min(tokens * top_k, experts)); hidden and inner even and at least 16, dtype bf16 or fp16 (else
  *                     GMM_ERR_UNSUPPORTED).  up_stride_.., down_stride_.. in bytes as for gmm_int8_mm, one matrix below 2 GiB. */
 int64_t gmm_int8_linear_workspace_bytes(int64_t rows, int64_t K, int64_t N, int32_t dtype);
 int gmm_int8_linear(const void* x, const int8_t* b, const float* b_scale, void* out, int64_t rows, int64_t K, int64_t N, int64_t x_stride,

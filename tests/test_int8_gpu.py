@@ -313,6 +313,34 @@ def test_layer_of_a_few_slots(T, E, k, H, inner, dtype):
             assert torch.equal(int8.moe_forward_int8(x, z, up, down, k), out)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, SF])
+@pytest.mark.parametrize("M", [65, 80, 96, 97, 128, 129, 192, 193, 250, 256, 257])
+@pytest.mark.parametrize("K,N", [(136, 200), (1024, 64), (2050, 72), (4096, 1000), (16384, 136)])
+def test_blocks_of_rows(M, K, N, dtype):
+    """One matrix streamed past several blocks of rows, the last one shorter; long columns in parts; sums are exact, whatever computes them."""
+    a, b = make(M, K, N)
+    out = check(a, b, dtype)
+    for rows in (slice(0, 64), slice(64, 65), slice(M - 3, M)):
+        assert torch.equal(out[rows], int8.int8_mm(int8.Rows(a.values[rows], a.scale[rows]), b, dtype))
+
+
+@pytest.mark.parametrize("kind", ["silu", "swiglu"])
+@pytest.mark.parametrize("T,E,k,H,inner", [(17, 3, 3, 136, 64), (33, 40, 8, 256, 128), (64, 8, 8, 130, 70), (64, 5, 2, 512, 256), (65, 8, 2, 256, 128), (96, 8, 2, 1040, 72),
+                                           (128, 8, 2, 256, 192), (130, 8, 2, 64, 64), (200, 128, 8, 128, 64), (255, 64, 8, 72, 128), (256, 64, 8, 136, 64), (256, 300, 32, 64, 32),
+                                           (257, 64, 8, 64, 64)])
+def test_layer_of_blocks_of_rows(T, E, k, H, inner, kind):
+    """Experts of more rows than a block, of a few and of none; either side of every limit.  A skewed choice gives one expert all tokens."""
+    x, z, up, down = layer(T, E, H, inner, kind)
+    for skew in (False, True):
+        if skew:
+            z = z.clone()
+            z[:, E // 2] += 20
+        out = int8.moe_forward_int8(x, z, up, down, k, kind)
+        want = oracle.layer(x, z, up.values, up.scale, down.values, down.scale, k, kind)
+        assert (plain.f64(out) - want).norm() <= (2.5 * 2.0 ** -8 + 2.0 ** -8) * want.norm()
+        assert torch.equal(int8.moe_forward_int8(x, z, up, down, k, kind), out)
+
+
 def test_layer_over_all_experts_and_halves_of_logits():
     x, z, up, down = layer(40, 10, 64, 64, "swiglu")
     out = int8.moe_forward_int8(x, z.to(BF), up, down, 3, renormalize=False)
