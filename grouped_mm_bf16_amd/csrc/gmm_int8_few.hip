@@ -8,7 +8,7 @@
 // (routes_here) and sums (kJoinSlots) as well: of one token two launches are left.
 // Columns of 4096 values lie in the same memory channels, so workgroups that run side by side begin at different places along k (Cycle): 1 x 14336 x
 // 4096 12.8 -> 11.4 us, 48 rows 18.1 -> 17.2, 1 x 28672 x 4096 21.3 -> 19.5.
-// One layer of 24 tokens, all 8 experts of 4096 -> 2 x 14336 (1.41 GB of weights): 214 to 232 us, 6.1 to 6.6 TB/s (a copy reaches 5.1, which writes as well).
+// One layer of 24 tokens, all 8 experts of 4096 -> 2 x 14336 (1.41 GB of weights): 199 to 232 us, 6.1 to 7.1 TB/s (a copy reaches 5.1, which writes as well).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -27,6 +27,7 @@ using namespace gmm;
 constexpr int kThreads = 256;      // of the kernels behind the products
 constexpr int kMaxRows = 64;       // of a block
 constexpr int kMostRows = 256;     // of one matrix; tokens of an expert layer
+constexpr int kMostSlots = 1024;   // rows of many matrices
 
 enum Result : int { kOut, kSums, kScaled, kActivated, kJoined };
 
@@ -453,6 +454,17 @@ void set_shape(FewArgs& a, const Shape& s, bool glu = false) {
   a.tiles = glu ? gmm_cdiv(a.N / 2, s.columns / 2) : gmm_cdiv(a.N, s.columns);
 }
 
+// Rows of a block for `slots` rows over `used` groups, which have about as many as each other: one and a half times that, and what a group has more is
+// another block.  us by rows of a block (and through tiles), expert layers: 64 tokens, 8 of 128 experts of 2048 -> 2 x 768, 4 rows 16: 121, 32: 123, 64: 186
+// (144), 192 tokens, 12 rows 144, 138, 220 (150); 2 of 8 of 4096 -> 2 x 14336, 96 tokens, 24 rows 32: 257, 48: 264 (335), 128, 32 rows 347, 283 (343),
+// 192, 48 rows 490, 394 (352); 6 of 64 of 2048 -> 2 x 1408, 256 tokens, 24 rows 140, 151 (139).
+bool few_each(int64_t slots, int64_t used) { return slots <= 32 * used; }
+int64_t block_of(int64_t slots, int64_t used, int64_t most) {
+  const int64_t block = slots <= 24 * used ? 32 : few_each(slots, used) ? 48 : kMaxRows, all = round_up(most, 16);
+  return block < all ? block : all;
+}
+int64_t items_of(int64_t slots, int64_t used, int64_t most, int64_t block) { return most <= block ? used : used + slots / block; }
+
 FewArgs from_params(const GmmInt8Params& p) {
   FewArgs a{};
   a.a = p.a; a.b = p.b; a.a_scale = p.a_scale; a.b_scale = p.b_scale; a.offs = p.jag == GMM_JAG_M ? p.offs : nullptr; a.row_index = p.gather;
@@ -460,9 +472,16 @@ FewArgs from_params(const GmmInt8Params& p) {
   a.G = p.G; a.M = p.M; a.N = p.N; a.K = p.K; a.a_rows = p.gather ? p.a_rows : p.M;
   a.x_dtype = kNotRounded;
   a.most = p.M;
-  a.items = a.offs ? gmm_min(p.G, p.M) : int32_t((p.M + kMaxRows - 1) / kMaxRows);      // one matrix: blocks of the same length
-  a.block = int32_t(round_up(a.offs || a.items == 0 ? p.M : (p.M + a.items - 1) / a.items, 16));
-  set_shape(a, few_shape(a.items, gmm_min(a.most, a.block), a.N, a.K));
+  if (a.offs) {
+    const int used = gmm_min(p.G, p.M);
+    a.block = int32_t(p.M <= kMaxRows ? round_up(p.M, 16) : block_of(p.M, used, p.M));
+    a.items = int32_t(items_of(p.M, used, p.M, a.block));
+    set_shape(a, few_shape(used, gmm_min(a.most, a.block), a.N, a.K));
+  } else {      // one matrix: blocks of the same length
+    a.items = (p.M + kMaxRows - 1) / kMaxRows;
+    a.block = int32_t(round_up(a.items ? (p.M + a.items - 1) / a.items : 0, 16));
+    set_shape(a, few_shape(a.items, gmm_min(a.most, a.block), a.N, a.K));
+  }
   return a;
 }
 
@@ -521,7 +540,10 @@ int launch(const FewArgs& a, hipStream_t stream) {
 bool gmm_int8_few_preferred(const GmmInt8Params& p) {
   FewArgs a = from_params(p);
   if (p.k_odd || !sizes_fit(a) || int64_t(a.items) * a.tiles >= (int64_t(1) << 27)) return false;
-  if (p.M <= kMaxRows || a.offs) return p.M <= kMaxRows;
+  if (p.M <= kMaxRows) return true;
+  // us, tile / here, by all groups' rows: 128 groups of 2048 -> 1536 65 40.8 / 27.2, 256 67.1 / 53.5, 1024 73.5 / 65.8, 2048 73.5 / 72.4; 64 of 2048 -> 2816
+  // 256 69.3 / 56.5, 2048 70.6 / 85.1; 8 of 14336 -> 4096 65 108 / 76, 256 (32 each) 108 / 82; 32 of 1024 -> 1024 1024 (32 each) 16.4 / 14.5
+  if (a.offs) return p.M <= kMostSlots && few_each(p.M, gmm_min(p.G, p.M));
   // Blocks of rows read the weights again, from the caches at best, where the tile has fewer tiles than compute units.  us, tile / here: 65 x 4096 x 4096
   // 31.6 / 10.6, 256 34.1 / 17.4; 96 x 14336 x 4096 34.5 / 27.3, 128 35.6 / 36.2; 256 x 4096 x 14336 74.3 / 40.2; 160 x 6144 x 1024 15.1 / 14.3, 192 15.3
   // / 20.1; 96 x 9216 x 2048 21.3 / 15.9, 128 21.8 / 24.8; 65 x 28672 x 4096 41.6 / 45.8.
@@ -587,14 +609,9 @@ bool plan_layer(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, int64_t k
   const int64_t N = kind == GMM_ACT_SWIGLU ? 2 * I : I;
   p.slots = T * k;
   p.used = p.slots < E ? p.slots : E;
-  // Experts have about as many rows as each other: blocks of one and a half times that, and what an expert has more is another one.  More rows than that on
-  // average, or tokens than kMostRows: through tiles.  us by rows of a block (and tiles): 64 tokens, 8 of 128 experts of 2048 -> 2 x 768, 4 rows 16: 121, 32:
-  // 123, 64: 186 (144), 192 tokens, 12 rows 144, 138, 220 (150); 2 of 8 of 4096 -> 2 x 14336, 96 tokens, 24 rows 32: 257, 48: 264 (335), 128, 32 rows 347, 283
-  // (343), 192, 48 rows 490, 394 (352); 6 of 64 of 2048 -> 2 x 1408, 256 tokens, 24 rows 140, 151 (139)
-  if (T > kMaxRows && p.slots > 32 * p.used) return false;
-  p.block = p.slots <= 24 * p.used ? 32 : p.slots <= 32 * p.used ? 48 : kMaxRows;
-  if (p.block > round_up(T, 16)) p.block = round_up(T, 16);
-  p.items = T <= p.block ? p.used : p.used + p.slots / p.block;
+  if (T > kMaxRows && !few_each(p.slots, p.used)) return false;
+  p.block = block_of(p.slots, p.used, T);
+  p.items = items_of(p.slots, p.used, T, p.block);
   p.up = few_shape(p.used, T, N, H / 2, GMM_DT_BF16);
   p.activated = p.up.parts == 1 && kind == GMM_ACT_SWIGLU;
   p.down = p.activated ? few_shape(p.used, T, H, I / 2, GMM_DT_F32) : few_shape(p.used, T, H, I / 2);

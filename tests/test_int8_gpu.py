@@ -324,6 +324,17 @@ def test_blocks_of_rows(M, K, N, dtype):
         assert torch.equal(out[rows], int8.int8_mm(int8.Rows(a.values[rows], a.scale[rows]), b, dtype))
 
 
+@pytest.mark.parametrize("M,G,largest", [(65, 3, 60), (100, 40, 7), (128, 4, 128), (300, 10, 33), (512, 128, 100), (1000, 50, 49), (1024, 32, 48), (1024, 1023, 65), (1025, 64, 20),
+                                          (700, 21, 700)])
+def test_blocks_of_rows_of_groups(M, G, largest):
+    """Groups of none, one, exactly a block, a block and one, many blocks; either side of the limits."""
+    gen = torch.Generator().manual_seed(M + G)
+    sizes = torch.bincount(torch.randint(0, G, (M - largest,), generator=gen), minlength=G)
+    sizes[G // 2] += largest
+    check_groups(sizes.tolist(), 130, 72)
+    check_groups(sizes.tolist(), 1024, 264, gather=M)
+
+
 @pytest.mark.parametrize("kind", ["silu", "swiglu"])
 @pytest.mark.parametrize("T,E,k,H,inner", [(17, 3, 3, 136, 64), (33, 40, 8, 256, 128), (64, 8, 8, 130, 70), (64, 5, 2, 512, 256), (65, 8, 2, 256, 128), (96, 8, 2, 1040, 72),
                                            (128, 8, 2, 256, 192), (130, 8, 2, 64, 64), (200, 128, 8, 128, 64), (255, 64, 8, 72, 128), (256, 64, 8, 136, 64), (256, 300, 32, 64, 32),
