@@ -401,6 +401,31 @@ def test_captured_and_replayed(T):
         assert all(torch.equal(p, q) for p, q in zip(held, want))
 
 
+@pytest.mark.parametrize("M", [40, 100, 256])
+def test_captured_where_few_rows_are_cut(M):
+    """Parts of k lie in a workspace: the graphs' own, so they do not meet each other's or the eager calls'."""
+    a, b = make(M, 16384, 136)
+    other = int8.Rows(a.values.flip(0).contiguous(), a.scale)
+    want, want_other = int8.int8_mm(a, b), int8.int8_mm(other, b)
+    graphs = []
+    for rows in (a, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = int8.int8_mm(rows, b)
+        graphs.append((graph, held))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for _, held in graphs:
+            held.zero_()
+        torch.cuda.synchronize()
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = int8.int8_mm(a, b)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want) and torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want_other)
+
+
 def test_captured_where_tiles_are_cut():
     a, b = make(300, 8192, 512)
     int8.int8_mm(a, b)
