@@ -64,6 +64,7 @@ SIGNATURES = {
     "gmm_int8_moe_few": (ctypes.c_int, [_vp] * 7 + [_i64] * 12 + [_i32] * 4 + [_vp, _i64, _vp]),
     "gmm_moe_sort_rows": (ctypes.c_int, [_vp] * 3 + [_i64] * 6 + [_i32, _vp]),
     "gmm_moe_sum_rows": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp]),
+    "gmm_moe_sum_rows_f32": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp]),
     "gmm_moe_combine_backward": (ctypes.c_int, [_vp] * 6 + [_i64] * 7 + [_i32, _vp]),
     "gmm_moe_route_backward": (ctypes.c_int, [_vp] * 5 + [_i64] * 4 + [_i32, _vp]),
     "gmm_gated": (ctypes.c_int, [_vp] * 2 + [_i64] * 4 + [_i32, _i32, _vp]),

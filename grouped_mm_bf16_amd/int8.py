@@ -312,6 +312,17 @@ def _activated(a: Rows, routing: moe.Routing, up: torch.Tensor, up_scale: torch.
     return _gated_now(_mm_now(a.values, a.scale, routing.row_token, b, up_scale, routing.offs, torch.float32), kind)
 
 
+def _summed(y: torch.Tensor, routing: moe.Routing, tokens: int, top_k: int, dtype: torch.dtype) -> torch.Tensor:
+    """The weighted sums of the experts' rows, which stay in fp32 until then: rounded to 16 bits they were wrong by as much again as the result's own
+    rounding, and infinite in fp16 where the sum need not be."""
+    out = torch.empty(tokens, y.size(1), device=y.device, dtype=dtype)
+    with _guard(y):
+        rc = _lib.load().gmm_moe_sum_rows_f32(y.data_ptr(), routing.token_rows.data_ptr(), routing.slot_weight.data_ptr(), out.data_ptr(), tokens, top_k,
+                                              y.size(1), y.size(0), y.stride(0), y.size(1), _dtype_code(dtype), kernels.current_stream(y.device))
+    _lib.check(rc, "moe_forward_int8: sum of rows")
+    return out
+
+
 def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor,
                top_k: int, kind: int, renormalize: bool) -> torch.Tensor:
     (T, H), (E, inner, _) = x.shape, down.shape
@@ -333,8 +344,7 @@ def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, u
             return out
     routing = moe.moe_route(moe_train._rows(router_logits), top_k, renormalize)
     values, scale = _activated(_quantize(x), routing, up, up_scale, kind)
-    y = _mm(Rows(values[:, :inner], scale), None, Columns(down, down_scale), routing.offs, x.dtype)
-    return moe_train._sum_now(y, routing.token_rows, routing.slot_weight, T, top_k)
+    return _summed(_mm_now(values[:, :inner], scale, None, down, down_scale, routing.offs, torch.float32), routing, T, top_k, x.dtype)
 
 
 _layer_op = torch.library.custom_op("grouped_mm_bf16_amd::int8_layer", mutates_args=())(_layer_now)
@@ -351,8 +361,7 @@ def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_up: Columns
     either product.
 
     x [T, H], bf16 or fp16; router_logits [T, E]; w_up of :func:`quantize_columns`, [E, H, I] ("silu") or [E, H, 2 I] ("swiglu": gate columns first);
-    w_down [E, I, H].  The activation takes the first product in float32.  Up to ``FEW_TOKENS`` tokens whose experts have few rows each the weighted sum alone
-    is rounded to x's type, of more the experts' rows as well.  Forward only.
+    w_down [E, I, H].  The activation takes the first product in float32, the weighted sum the second, and is rounded once.  Forward only.
     """
     if x.dim() != 2 or router_logits.dim() != 2 or x.size(0) != router_logits.size(0):
         raise RuntimeError("x [T, H] and router_logits [T, E] must agree on T")

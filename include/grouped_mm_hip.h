@@ -368,6 +368,7 @@ int gmm_int8_moe_few(const void* x, const void* logits, const int8_t* w_up, cons
  *   gmm_moe_sort_rows         out[row of slot (t, j)] = x[t]: x [tokens, hidden], out [out_rows, hidden]
  *   gmm_moe_sum_rows          out[t] = sum of slot_weight[t, j] * y[row of slot (t, j)] (slot_weight NULL: ones): y [y_rows, hidden],
  *                             out [tokens, hidden]; without weights the gradient of gmm_moe_sort_rows
+ *   gmm_moe_sum_rows_f32      the same of rows in fp32, rounded to out_dtype
  *   gmm_moe_combine_backward  of gmm_moe_sum_rows, for dout [tokens, hidden]: dy[row of slot (t, j)] = slot_weight[t, j] * dout[t]  [y_rows,
  *                             hidden] (rows that no slot has are left as they are), dweight[t, j] = <dout[t], y[row of slot (t, j)]> float;
  *                             either may be NULL (without dweight y is not read) */
@@ -375,6 +376,8 @@ int gmm_moe_sort_rows(const void* x, const int32_t* token_rows, void* out, int64
                       int64_t out_rows, int64_t x_stride, int64_t out_stride, int32_t dtype, void* stream);
 int gmm_moe_sum_rows(const void* y, const int32_t* token_rows, const float* slot_weight, void* out, int64_t tokens, int64_t top_k,
                      int64_t hidden, int64_t y_rows, int64_t y_stride, int64_t out_stride, int32_t dtype, void* stream);
+int gmm_moe_sum_rows_f32(const float* y, const int32_t* token_rows, const float* slot_weight, void* out, int64_t tokens, int64_t top_k,
+                         int64_t hidden, int64_t y_rows, int64_t y_stride, int64_t out_stride, int32_t out_dtype, void* stream);
 int gmm_moe_combine_backward(const void* dout, const void* y, const int32_t* token_rows, const float* slot_weight, void* dy, float* dweight,
                              int64_t tokens, int64_t top_k, int64_t hidden, int64_t y_rows, int64_t dout_stride, int64_t y_stride,
                              int64_t dy_stride, int32_t dtype, void* stream);

@@ -57,3 +57,38 @@ def layer(x, logits, up, up_scale, down, down_scale, top_k, kind, renormalize=Tr
         y = (a8 @ down[e].cpu().double()) * f64(a_scale)[:, None] * f64(down_scale[e])
         out.index_add_(0, token, y * weight[token, j][:, None])
     return out
+
+
+def layer_within(x, logits, up, up_scale, down, down_scale, top_k, kind, renormalize=True):
+    """:func:`layer` and its bound element by element.
+
+    The activation in fp32: the sums are exact, three roundings make a gate (and its partner) of them, e^-g takes a few units and as many as its
+    argument's rounding leaves, then three roundings.  What that leaves decides a value's step of 8 bits only where the quotient lies that near a half:
+    those values may be a whole step off, the others are none, and a row's scale is off as its largest value is.  The experts' rows and their sum stay in
+    fp32, one rounding follows."""
+    dtype = x.dtype
+    x8, x_scale = quantize(x)
+    z = f64(logits)
+    chosen = torch.argsort(z, dim=1, descending=True, stable=True)[:, :top_k]
+    weight = torch.softmax(z.gather(1, chosen), 1) if renormalize else torch.softmax(z, 1).gather(1, chosen)
+    weight_err = (16 + 4 * (z.max(1).values - z.min(1).values))[:, None] * EPS32 * weight
+    out, bound = torch.zeros(x.shape, dtype=torch.float64), torch.zeros(x.shape, dtype=torch.float64)
+    inner = down.size(1)
+    for e in chosen.unique().tolist():
+        token, j = (chosen == e).nonzero(as_tuple=True)
+        h = (x8[token] @ up[e].cpu().double()) * f64(x_scale)[token, None] * f64(up_scale[e])
+        g = h[:, :inner]
+        a = torch.nn.functional.silu(g) if kind == "silu" else torch.nn.functional.silu(g) * h[:, inner:]
+        off = (3 * (1 + g.abs()) + 12 + 2 * g.abs() + 3 + 3) * EPS32
+        a8, a_scale = quantize(a)
+        # the row's largest value has the largest part in its scale, whichever of the largest it is
+        scale_off = off.amax(1, keepdim=True) + 2 * EPS32
+        q = a / f64(a_scale)[:, None]
+        near = ((q - q.floor()) - 0.5).abs() <= q.abs() * (off + scale_off + 2 * EPS32) + 1e-30
+        d = down[e].cpu().double() * f64(down_scale[e])
+        y = (a8 @ d) * f64(a_scale)[:, None]
+        y_err = (near.double() @ d.abs()) * f64(a_scale)[:, None] + (scale_off + 6 * EPS32) * y.abs()
+        w, w_err = weight[token, j][:, None], weight_err[token, j][:, None]
+        out.index_add_(0, token, y * w)
+        bound.index_add_(0, token, y_err * (w + w_err) + y.abs() * (w_err + (top_k + 2) * EPS32 * w))
+    return out, bound + UNIT[dtype] * (out.abs() + bound) + TINY[dtype]
