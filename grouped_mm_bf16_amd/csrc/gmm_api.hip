@@ -379,7 +379,8 @@ static int int8_params(const int8_t* a, const float* a_scale, const int32_t* row
   nothing = G == 0 || M == 0 || N == 0;
   if (nothing) return GMM_OK;
   if (!out || (!row_index && a_rows != M) || (out_stride < out_cols && M > 1)) return GMM_ERR_BAD_ARGUMENT;
-  if (!a_scale || !b_scale || (K > 0 && (!a || !b)) || !aligned16(a) || !aligned16(b)) return GMM_ERR_BAD_ARGUMENT;
+  const bool rows = !row_index || a_rows > 0;      // without any, `a` and its scales may be null
+  if ((rows && !a_scale) || !b_scale || (K > 0 && ((rows && !a) || !b)) || !aligned16(a) || !aligned16(b)) return GMM_ERR_BAD_ARGUMENT;
   // rows of either operand may lie on one another only where there is one
   if ((a_stride & 15) || (b_stride_g & 15) || (b_stride_n & 15) || a_stride < 0 || b_stride_g < 0 || b_stride_n < 0) return GMM_ERR_BAD_ARGUMENT;
   if ((a_stride < K && a_rows > 1) || (b_stride_n < K && N > 1)) return GMM_ERR_BAD_ARGUMENT;

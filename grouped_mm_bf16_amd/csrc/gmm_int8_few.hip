@@ -487,7 +487,7 @@ FewArgs from_params(const GmmInt8Params& p) {
 
 bool sizes_fit(FewArgs& a) {
   if (a.a_rows > 0 && int64_t(a.a_rows) * a.a_ld >= (int64_t(1) << 30)) return false;
-  a.a_bytes = uint32_t((int64_t(a.a_rows - 1) * a.a_ld + a.K) * 2);
+  a.a_bytes = uint32_t(gmm_rows_bytes(a.a_rows, a.a_ld, a.K));      // a row that does not exist is asked for behind it
   a.b_bytes = matrix_bytes(a.K, a.N, 1, a.b_ld);
   return a.K >= 8 && a.b_bytes != 0;
 }

@@ -78,6 +78,10 @@ struct GmmInt8Params : GmmParams {
   int32_t k_odd;          // the last pair along K has one element only
 };
 
+// Bytes of `rows` rows of K 16-bit elements, ld elements from one to the next, up to the last row's last element; of no rows none, however far apart
+// they would lie.
+GMM_HD int64_t gmm_rows_bytes(int64_t rows, int64_t ld, int64_t K) { return rows > 0 ? ((rows - 1) * ld + K) * 2 : 0; }
+
 constexpr int GMM_WS_HEADER = 4096;          // 1024 int32: arrival counters, one per tile of the split round, ...
 constexpr int GMM_WS_SLOT = 256 * 256 * 4;   // one fp32 partial tile
 constexpr int GMM_SPLIT_MAX = 8;             // most parts a tile is cut into

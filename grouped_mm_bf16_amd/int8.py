@@ -146,7 +146,7 @@ def _mm_now(a: torch.Tensor, a_scale: torch.Tensor, row_index: Optional[torch.Te
     out = torch.empty(M, N, device=a.device, dtype=out_dtype)
     if out.numel() == 0:
         return out
-    if K == 0:
+    if K == 0 or a.size(0) == 0:      # every row_index is outside a
         return out.zero_()
     a, (b, sg, sn) = _aligned(a), _columns(b)
     lib = _lib.load()

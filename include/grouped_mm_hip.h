@@ -324,7 +324,7 @@ int gmm_layer_norm_backward(const void* dy, const void* x, const void* weight, c
  *   gmm_int8_gated     the same of silu(h[r, c]) or silu(h[r, c]) * h[r, inner + c] (kind GMM_ACT_SILU, GMM_ACT_SWIGLU), h float [rows, ..]
  *   gmm_int8_mm        out[m, n] = a_scale[m'] * b_scale[g, n] * sum over k of a[m', k] * b[g, k, n]
  *                      for rows m of group g (offs as in gmm_2d3d; NULL: one group that has all M rows), m' = m or row_index[m] (row_index NULL: m;
- *                      outside [0, a_rows): a row of zeros).  a [a_rows, K] row-major, b [G, K, N] contiguous along K: a_stride, b_stride_g and
+ *                      outside [0, a_rows): a row of zeros; a_rows may be 0, a and a_scale then NULL).  a [a_rows, K] row-major, b [G, K, N] contiguous along K: a_stride, b_stride_g and
  *                      b_stride_n in bytes, multiples of 16, a and b 16-byte aligned; K < 131072 (sums are 32-bit integers, exact);
  *                      b_scale [G, N] contiguous; out [M, N] row-major, out_dtype any gmm_dtype, out_stride in elements; scaled in fp32, by the
  *                      column's scale and then by the row's, rounded once.  Bytes behind a row's or a column's end, up to the next multiple of 16, may be read and do not count.  With row_index,
