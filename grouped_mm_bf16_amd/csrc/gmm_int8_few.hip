@@ -65,7 +65,8 @@ struct FewArgs {
 
 constexpr int kNotRounded = -1;
 
-// The `which`-th block of up to BLOCK rows of a group, found by every wave for itself.
+// The `which`-th block of up to BLOCK rows of a group, found by every wave for itself.  A row is its that first has a higher offset: where offsets go down
+// as well as up the highest so far takes their place, so groups share no rows and have no more blocks than the launch.
 template <int BLOCK>
 __device__ __forceinline__ bool find_group(const FewArgs& a, int which, int& g, int& row0, int& rows) {
   constexpr int AT_ONCE = 4;
@@ -78,7 +79,16 @@ __device__ __forceinline__ bool find_group(const FewArgs& a, int which, int& g, 
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
       const bool there = base + 64 * i + lane < a.G;
-      const int to = min(max(ends[i], 0), a.M), before = __shfl_up(to, 1), from = lane ? before : start;
+      int to = min(max(ends[i], 0), a.M), before = __shfl_up(to, 1), from = lane ? before : start;
+      if (__ballot(to < from)) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int up = __shfl_up(to, o);
+          to = max(to, lane >= o ? up : start);
+        }
+        before = __shfl_up(to, 1);
+        from = lane ? before : start;
+      }
       start = __builtin_amdgcn_readlane(to, 63);
       const uint64_t with = __ballot(there && to > from);
       int ahead = __popcll(with & ((uint64_t(1) << lane) - 1)), n = __popcll(with), own = there && to > from;      // blocks of lanes before the own
