@@ -432,7 +432,7 @@ bool plan_sort(int64_t tokens, int64_t top_k, SortPlan& pl) {
 }
 
 // Stable sort of the slots by expert: offs, row_token, token_rows.
-// table_shared: other calls may use it at the same time.
+// table_shared: other calls may use it at the same time, so long as they have no more than kPlaceSlots.
 int sort_planned(const int32_t* slot_expert, const SortPlan& pl, int64_t E, int64_t top_k, int32_t* offs, int32_t* row_token,
                  int32_t* token_rows, int32_t* table, bool table_shared, hipStream_t stream) {
   const int blocks = (pl.slots + kPlaceBlock - 1) / kPlaceBlock;
@@ -530,6 +530,15 @@ int64_t gmm_moe_route_workspace_bytes(int64_t tokens, int64_t experts, int64_t t
 int gmm_moe_route(const void* logits, int64_t logits_stride, int32_t logits_dtype, int64_t tokens, int64_t experts,
                   int64_t top_k, int32_t renormalize, int32_t* offs, int32_t* slot_expert, float* slot_weight,
                   int32_t* row_token, int32_t* token_rows, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (workspace_bytes < 0) return GMM_ERR_BAD_ARGUMENT;
+  return route_checked(logits, logits_stride, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert,
+                       slot_weight, row_token, token_rows, static_cast<int32_t*>(workspace), size_t(workspace_bytes), true,
+                       static_cast<hipStream_t>(stream));
+}
+
+int gmm_moe_route_own(const void* logits, int64_t logits_stride, int32_t logits_dtype, int64_t tokens, int64_t experts,
+                      int64_t top_k, int32_t renormalize, int32_t* offs, int32_t* slot_expert, float* slot_weight,
+                      int32_t* row_token, int32_t* token_rows, void* workspace, int64_t workspace_bytes, void* stream) {
   if (workspace_bytes < 0) return GMM_ERR_BAD_ARGUMENT;
   return route_checked(logits, logits_stride, logits_dtype, tokens, experts, top_k, renormalize, offs, slot_expert,
                        slot_weight, row_token, token_rows, static_cast<int32_t*>(workspace), size_t(workspace_bytes), false,

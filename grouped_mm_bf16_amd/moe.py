@@ -56,10 +56,10 @@ def _route_now(router_logits: torch.Tensor, top_k: int, renormalize: bool) -> to
     buf = torch.empty(E + 4 * S + ws_bytes // 4, device=dev, dtype=torch.int32)
     base = buf.data_ptr()
     with _guard(router_logits):
-        rc = lib.gmm_moe_route(router_logits.data_ptr(), router_logits.stride(0) if T else E,
-                               _dtype_code(router_logits.dtype), T, E, top_k, int(bool(renormalize)),
-                               base, base + 4 * E, base + 4 * (E + S), base + 4 * (E + 2 * S), base + 4 * (E + 3 * S),
-                               base + 4 * (E + 4 * S), ws_bytes, kernels.current_stream(dev))
+        rc = lib.gmm_moe_route_own(router_logits.data_ptr(), router_logits.stride(0) if T else E,
+                                   _dtype_code(router_logits.dtype), T, E, top_k, int(bool(renormalize)),
+                                   base, base + 4 * E, base + 4 * (E + S), base + 4 * (E + 2 * S), base + 4 * (E + 3 * S),
+                                   base + 4 * (E + 4 * S), ws_bytes, kernels.current_stream(dev))
     _lib.check(rc, "moe_route")
     return buf
 
