@@ -463,7 +463,7 @@ int route_checked(const void* logits, int64_t ld, int dtype, int64_t tokens, int
   SortPlan pl;
   if (!plan_sort(tokens, top_k, pl)) return GMM_ERR_BAD_ARGUMENT;
   if (!offs) return GMM_ERR_BAD_ARGUMENT;
-  if (tokens > 0 && (!logits || !slot_expert || !slot_weight || !row_token || !token_rows || ld < E)) return GMM_ERR_BAD_ARGUMENT;
+  if (tokens > 0 && (!logits || !slot_expert || !slot_weight || !row_token || !token_rows || (ld < E && tokens > 1))) return GMM_ERR_BAD_ARGUMENT;
   if (size_t(pl.nb) * size_t(E) * sizeof(int32_t) > table_bytes) return GMM_ERR_WORKSPACE;
   if (pl.nb > 0 && !table) return GMM_ERR_BAD_ARGUMENT;
   if (tokens > 0) {

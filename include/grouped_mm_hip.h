@@ -185,8 +185,8 @@ int gmm_zero_unowned(void* out, const int32_t* offs, int32_t G, int32_t by_colum
  * its benchmark builds the sorted rows and `offs` with torch on the host side (bench/bench_2d3d.py:124-149:
  * randint / bincount / cumsum and an offs[-1].item() round trip).  Here everything stays on the device.
  *
- * Routing.  For each of `tokens` rows of `logits` [tokens, experts] (row stride logits_stride elements,
- * dtype a gmm_dtype) pick the top_k largest (ties: lower expert index first; logits must not be NaN; -inf
+ * Routing.  For each of `tokens` rows of `logits` [tokens, experts] (row stride logits_stride elements, of no
+ * matter for one token, dtype a gmm_dtype) pick the top_k largest (ties: lower expert index first; logits must not be NaN; -inf
  * masks an expert; a row whose maximum is +inf or -inf puts all weight, in equal shares, on the entries equal
  * to the maximum: the limit of the softmax), in
  * descending order.  Choice j of token t is SLOT t * top_k + j.  Outputs (device memory):
