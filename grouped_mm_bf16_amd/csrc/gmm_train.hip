@@ -233,17 +233,20 @@ __global__ void __launch_bounds__(kBlock) gated_kernel(const GatedArgs a) {
     float first[N], second[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float g = gate.get(i), e = exp_minus<T>(g), part = 1.0f / (1.0f + e);
+      // g s(g) as one quotient where the result is fp32: as a product with a reciprocal it is a rounding further off.  The slope s(g) (1 + g (1 - s(g))) is
+      // g s(g) (1 - s(g)) + s(g): a difference and a fused sum, three roundings fewer than with e^-g s(g) for 1 - s(g), after which the gradient of
+      // normal values in fp32 was 6.0e-8 off (the formula in elementary operations 5.6e-8, this 5.0e-8).  Neither takes longer: memory bounds it.
+      const float g = gate.get(i), t = 1.0f + exp_minus<T>(g), part = 1.0f / t, silu = sizeof(T) == 4 ? g / t : g * part;
       if constexpr (!BACK) {
-        first[i] = g * part;
+        first[i] = silu;
         if constexpr (SWIGLU) first[i] *= up.get(i);
       } else {
-        // 1 - s(g) = e s(g); where e is infinite that is 1
-        const float rest = __builtin_isinf(e) ? 1.0f : e * part;
-        first[i] = d.get(i) * part * (1.0f + g * rest);
+        const float slope = __builtin_fmaf(silu, 1.0f - part, part);
         if constexpr (SWIGLU) {
-          second[i] = d.get(i) * g * part;
-          first[i] *= up.get(i);
+          second[i] = d.get(i) * silu;
+          first[i] = d.get(i) * slope * up.get(i);      // a slope of zero makes it zero, however large the partner
+        } else {
+          first[i] = d.get(i) * slope;
         }
       }
     }
