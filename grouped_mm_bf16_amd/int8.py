@@ -20,6 +20,7 @@ from .kernels import _dtype_code, _guard, _require_gpu
 from .moe import ACTIVATIONS
 
 MAX_K = 131071       # sums of products of -128 .. 127 stay below 2^31
+MAX_GATHERED = 1 << 31     # bytes of rows that are gathered
 
 
 class Rows(NamedTuple):
@@ -228,8 +229,8 @@ def grouped_int8_mm(a: Rows, b: Columns, offs: torch.Tensor, out_dtype: torch.dt
                     row_index: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`int8_mm` of jagged rows: rows offs[g - 1] .. offs[g] - 1 of the result are those of a times b's matrix g.
 
-    a.values [M, K], b.values [G, K, N], offs int32 [G].  With row_index (int32 [M]) row m is row row_index[m] of a; a number outside a reads a row of
-    zeros.  Rows past the last offset are left uninitialised, as ``grouped_mm`` leaves them.
+    a.values [M, K], b.values [G, K, N], offs int32 [G].  With row_index (int32 [M]) row m is row row_index[m] of a, which then has less than 2 GiB; a number
+    outside a reads a row of zeros.  Rows past the last offset are left uninitialised, as ``grouped_mm`` leaves them.
     """
     _dtype_code(out_dtype)
     _check_columns("grouped_int8_mm", b, a.values.device, 3)
@@ -342,6 +343,11 @@ def _layer_now(x: torch.Tensor, router_logits: torch.Tensor, up: torch.Tensor, u
         if nbytes >= 0 and rc != _lib.ERR_UNSUPPORTED:
             _lib.check(rc, "moe_forward_int8")
             return out
+    most = MAX_GATHERED // _pitch(H) - 1
+    if T > most:      # tokens do not depend on one another
+        parts = -(-T // most)
+        return torch.cat([_layer_now(x_, z_, up, up_scale, down, down_scale, top_k, kind, renormalize)
+                          for x_, z_ in zip(x.tensor_split(parts), router_logits.tensor_split(parts))])
     routing = moe.moe_route(moe_train._rows(router_logits), top_k, renormalize)
     values, scale = _activated(_quantize(x), routing, up, up_scale, kind)
     return _summed(_mm_now(values[:, :inner], scale, None, down, down_scale, routing.offs, torch.float32), routing, T, top_k, x.dtype)
