@@ -110,8 +110,9 @@ struct RowScale {
     scale = (largest < 0x1p-100f ? 0x1p-100f : largest) / 127.0f;
     inverse = finite ? 1.0f / scale : 0.0f;
   }
-  // x / scale to the nearest fp32 value: the reciprocal's product, corrected by its residual.  Adding 1.5 * 2^23 rounds to a whole number, whose two's
-  // complement the low bits then are.
+  // x / scale rounded to a whole number as IEEE's quotient is: the reciprocal's product, corrected once by its residual.  That is another fp32 number than IEEE's
+  // only where the quotient lies within a few 2^-24 of their border, and makes another whole number only where one of the two is a half: none of the 2149 such pairs
+  // of 24-bit numbers does.  Adding 1.5 * 2^23 rounds to a whole number, whose two's complement the low bits then are.
   __device__ __forceinline__ uint32_t rounded_bits(float x) const {
     const float q = x * inverse;
     return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, scale, x), inverse, q) + 12582912.0f) & 0xffu;
