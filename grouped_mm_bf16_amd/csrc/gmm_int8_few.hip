@@ -7,7 +7,7 @@
 // Of a few short rows every workgroup makes the 8-bit ones itself, while its first weights are on their way (rounds_here), and the layer's routing
 // (routes_here) and sums (kJoinSlots) as well: of one token two launches are left.
 // Columns of 4096 values lie in the same memory channels, so workgroups that run side by side begin at different places along k (Cycle): 1 x 14336 x
-// 4096 12.8 -> 11.4 us, 48 rows 18.1 -> 17.2, 1 x 28672 x 4096 21.3 -> 19.5.
+// 4096 12.8 -> 11.4 us, 48 rows 18.1 -> 17.2 (16.6 since their scales are loaded ahead; 15.6 to 17.4 by the profiler), 1 x 28672 x 4096 21.3 -> 19.5.
 // One layer of 24 tokens, all 8 experts of 4096 -> 2 x 14336 (1.41 GB of weights): 199 to 232 us, 6.1 to 7.1 TB/s (a copy reaches 5.1, which writes as well).
 #include <hip/hip_runtime.h>
 

@@ -5,7 +5,7 @@
 // in the epilogue, one rounding follows.  Tile list, launch order and cut tiles are the 16-bit product's.
 //   8192 x 14336 x 4096 bf16 out                 354 us, 2.7 POP/s.  A K tile of 128 takes 1.37 us (3.1 POP/s); what is left is a tile's prologue and its
 //                                                stores, which all compute units make at once: 10 us a round
-//   8 of 128 experts, 4001 tokens, 2048 -> 2 x 768   164 us with SwiGLU in the epilogue, 768 -> 2048 148 to fp32 (bf16 124): 22 and 8 us of K tiles and the
+//   8 of 128 experts, 4001 tokens, 2048 -> 2 x 768   164 us with SwiGLU in the epilogue, 768 -> 2048 142 to 148 to fp32 (bf16 124): 22 and 8 us of K tiles and the
 //                                                same 10 of prologue and stores.  128-row tiles throughout, or groups in another order: no faster
 #define GMM_TILE_INT8
 #include "gmm_asm.h"

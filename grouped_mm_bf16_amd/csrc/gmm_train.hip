@@ -9,7 +9,7 @@
 // once, its choices' rows once each, and the sums over choices need no atomics.  16 bytes to an access, at any address; what is read or written
 // once goes past the caches (below: without / with).
 //   16384 tokens, 8 of 128 experts, bf16 rows of 2048   sort 115 / 103 us (5.9 TB/s; its one read through them, past them 114), sums 120 / 98 (6.2),
-//                                                       combine's gradients 283 / 243 (4.7)
+//                                                       combine's gradients 283 / 219 (5.2)
 //   16384 x 14336 bf16                                  activation 265 / 251 (5.6), its gradient 446 / 428 (5.5)
 #include <hip/hip_runtime.h>
 
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kBlock) sum_rows_kernel(const RowArgs a) {
 }
 
 // The sums of products of kAtOnce choices stay in registers over all of the row, then go over its lanes; those of several waves meet in LDS.  A wave to
-// a token, its row in pieces, took 276 us where four waves take 243.
+// a token, its row in pieces, takes an eighth longer.
 template <typename T, int N, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) combine_backward_kernel(const RowArgs a) {
   constexpr int J = kAtOnce, WAVES = kBlock / 64;
